@@ -134,12 +134,31 @@ _SIGNATURES: dict[str, list] = {
         c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
     ],
     "cdb_block_free": [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_void_p],
+    "cdb_kv8_append": [
+        c_void_p, c_int64, c_void_p, c_int64,  # qkv, stride, q_out, stride
+        c_void_p, c_void_p, c_int, c_int, c_int,  # codes, scales, num_cache_layers, cache_layer, num_blocks
+        c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p,  # block_table, stride, rows, width, item_slot, item_pos
+        c_int, c_void_p, c_void_p, c_int, c_void_p,  # rope_mode, cos, sin, rope_rows, qk_bias
+        c_int, c_int, c_int, c_int, c_void_p, c_void_p,  # num_items, num_heads, num_kv_heads, head_dim, status, stream
+    ],
+    "cdb_kv8_gather": [
+        c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+    ],
+    "cdb_kv8_decode_workspace_floats": [c_int, c_int],
+    "cdb_kv8_decode_attention": [
+        c_void_p, c_int64, c_void_p, c_int64,  # q, stride, out, stride
+        c_void_p, c_void_p, c_int, c_int, c_int,  # codes, scales, num_cache_layers, cache_layer, num_blocks
+        c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p,  # block_table, stride, rows, width, item_slot, item_pos
+        c_int, c_int, c_int, c_int, c_float, c_int,  # num_items, heads, kv_heads, head_dim, scale, num_ctas
+        c_void_p, c_int64, c_void_p, c_void_p, c_void_p,  # workspace, floats, counters, status, stream
+    ],
     "cdb_build_tables": [
         c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_void_p,
         c_void_p, c_void_p, c_void_p,
     ],
 }
-_RESTYPES = {"cdb_status_string": ctypes.c_char_p, "cdb_attn_scratch_bytes": c_int64, "cdb_gemm_workspace_elems": c_int64,
+_RESTYPES = {"cdb_status_string": ctypes.c_char_p, "cdb_kv8_decode_workspace_floats": c_int64,
+             "cdb_attn_scratch_bytes": c_int64, "cdb_gemm_workspace_elems": c_int64,
               "cdb_gemm_counter_elems": c_int}
 
 _LIB: ctypes.CDLL | None = None
@@ -192,7 +211,7 @@ def stream_ptr(stream: torch.cuda.Stream | None = None) -> int:
 
 _NO_LAUNCH = {
     "cdb_version", "cdb_status_string", "cdb_attn_scratch_bytes", "cdb_gemm_workspace_elems", "cdb_gemm_counter_elems",
-    "cdb_gemm_partial_splits",
+    "cdb_gemm_partial_splits", "cdb_kv8_decode_workspace_floats",
     "cdb_schedule_queues_init",
     "cdb_kv_blocks_host_copy",
 }

@@ -453,6 +453,68 @@ int cdb_build_tables(const int32_t* block_table, int64_t block_table_stride, con
                      int32_t* out_table, int64_t out_stride, int32_t* cu_seq_lens_q, int32_t* cu_seq_lens_k,
                      int32_t* status, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * 8-bit paged KV cache. Codes and scales of all cache layers:
+ *   codes  e4m3 [num_cache_layers][2 (K,V)][num_blocks][num_kv_heads][16][head_dim], 16-byte aligned
+ *   scales fp32 [num_cache_layers][2][num_blocks][num_kv_heads]
+ * value = code * scale of its (block, head). A scale is the smallest power of two 2^e (e >= -126)
+ * with amax <= 448 * 2^e over the block's finite values. Blocks are 16 tokens and addressed as in the
+ * bf16 pool: position p of slot s lies at place p % 16 of block block_table[s][p / 16], for every
+ * cache layer; a block of one layer, K or V, is 16 * num_kv_heads * head_dim contiguous bytes, so
+ * cdb_kv_blocks_host_copy moves codes as it moves bf16 blocks. head_dim 64, 96 or 128. The
+ * reference keeps its cache in the model's type only (continuous_batching/cache.py:131-145).
+ * block_table [table_rows][table_width] int32 with row stride block_table_stride. An index outside
+ * its range sets CDB_ERR_INDEX in *status and what it leads to is not read or written.
+ * ------------------------------------------------------------------------------------- */
+
+/* Add the rows' keys and values to the cache; the 8-bit sibling of cdb_rope_append_kv.
+ *   qkv        bf16 [num_items, qkv_stride]: q (num_heads), k, v (num_kv_heads each) side by side;
+ *              16-byte aligned, stride a multiple of 8.
+ *   q_out      bf16 rows of the rotated q (stride a multiple of 8, 16-byte aligned); may be qkv
+ *              itself; NULL leaves q alone.
+ *   rope_mode  0 none, 1 split halves (bf16 tables [rope_rows][head_dim]), 2 interleaved pairs
+ *              (fp32 tables [rope_rows][head_dim/2]). qk_bias: NULL or bf16 [num_heads +
+ *              num_kv_heads][head_dim], added to q and k first. Bias and rotation are computed in
+ *              fp32 and rounded once, to bf16 (q) and to e4m3 (k).
+ *   item_pos   position of each row, < 0: a padding row, skipped.
+ * Rows of one slot must be consecutive in the call, at ascending consecutive positions, each
+ * position once; a row that does not follow its predecessor within a block sets CDB_ERR_INDEX and is
+ * not written. The scale of a block whose place 0 is written now is set from the new rows alone; a
+ * block that already holds rows keeps its scale unless the new rows need a larger one, and then its
+ * earlier codes are rescaled (exact but for e4m3 subnormals). Infinities saturate, NaN stays NaN;
+ * neither enters the scale. Places behind the rows written keep their codes. */
+int cdb_kv8_append(const void* qkv, int64_t qkv_stride, void* q_out, int64_t q_out_stride, void* codes, float* scales,
+                   int num_cache_layers, int cache_layer, int num_blocks, const int32_t* block_table,
+                   int64_t block_table_stride, int table_rows, int table_width, const int32_t* item_slot,
+                   const int32_t* item_pos, int rope_mode, const void* rope_cos, const void* rope_sin, int rope_rows,
+                   const void* qk_bias, int num_items, int num_heads, int num_kv_heads, int head_dim, int32_t* status,
+                   void* stream);
+
+/* out[i] = block blocks[i] of one cache layer as bf16 [2][num_kv_heads][16][head_dim] (16-byte
+ * aligned; exact: a code times a power of two is a bf16 value). A block id out of range gives zeros. */
+int cdb_kv8_gather(const void* codes, const float* scales, int num_cache_layers, int cache_layer, int num_blocks,
+                   int num_kv_heads, int head_dim, const int32_t* blocks, int n, void* out, int32_t* status,
+                   void* stream);
+
+/* fp32 elements of cdb_kv8_decode_attention's workspace for num_ctas CTAs. */
+int64_t cdb_kv8_decode_workspace_floats(int num_ctas, int head_dim);
+
+/* Decode attention over the 8-bit cache: row i attends to positions 0 .. item_pos[i] of slot
+ * item_slot[i]; a row with item_pos < 0 is skipped and its out row left as it was. No work plan: the
+ * kernel cuts the pages of all rows into equal shares by the positions on the device.
+ *   q, out     bf16 rows of num_heads * head_dim, q rotated; 16-byte aligned, strides multiples
+ *              of 8. num_heads is a multiple of num_kv_heads; head h reads kv head
+ *              h / (num_heads / num_kv_heads).
+ *   num_ctas   CTAs to launch (two fit an SM); workspace: cdb_kv8_decode_workspace_floats of it;
+ *              counters [num_ctas] int32, zeroed before the first use, left zeroed. Calls that
+ *              share them must be ordered. */
+int cdb_kv8_decode_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* codes,
+                             const float* scales, int num_cache_layers, int cache_layer, int num_blocks,
+                             const int32_t* block_table, int64_t block_table_stride, int table_rows, int table_width,
+                             const int32_t* item_slot, const int32_t* item_pos, int num_items, int num_heads,
+                             int num_kv_heads, int head_dim, float scale, int num_ctas, float* workspace,
+                             int64_t workspace_floats, int32_t* counters, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
