@@ -152,6 +152,23 @@ _SIGNATURES: dict[str, list] = {
         c_int, c_int, c_int, c_int, c_float, c_int,  # num_items, heads, kv_heads, head_dim, scale, num_ctas
         c_void_p, c_int64, c_void_p, c_void_p, c_void_p,  # workspace, floats, counters, status, stream
     ],
+    "cdb_kv8_prefill_attention": [
+        c_void_p, c_int64, c_void_p, c_int64, c_int,  # q, stride, out, stride, num_rows
+        c_void_p, c_void_p, c_int, c_int, c_int,  # codes, scales, num_cache_layers, cache_layer, num_blocks
+        c_void_p, c_int64, c_int, c_int, c_void_p, c_int,  # block_table, stride, rows, width, tiles, num_tiles
+        c_int, c_int, c_int, c_float, c_void_p, c_void_p,  # heads, kv_heads, head_dim, scale, status, stream
+    ],
+    "cdb_step_tables": [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_int,  # slots, seq_len, new_len, row_len, num_requests
+        c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_void_p,  # block_table, stride, rows, width, ring, size, state
+        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,  # row_len_out, state_out, granted, cu_q, cu_k
+        c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,  # item_slot, item_pos, slot_map, capacity, tiles, capacity
+        c_void_p, c_void_p,  # status, stream
+    ],
+    "cdb_gemv_w4": [
+        c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64,  # x, ldx, w, ldw, scales, zeros, out, ldo
+        c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,  # M, N, K, group_size, num_sms, status, stream
+    ],
     "cdb_build_tables": [
         c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_void_p,
         c_void_p, c_void_p, c_void_p,

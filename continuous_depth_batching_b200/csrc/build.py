@@ -20,7 +20,7 @@ REPO = PKG.parent
 LIB_NAME = "libcdb_b200.so"
 SOURCES = [
     "attention.cu", "prefill_attention.cu", "elementwise.cu", "gemm.cu", "scheduler.cu", "fused_ops.cu", "kv_swap.cu",
-    "kv8_append.cu", "kv8_decode.cu",
+    "kv8_append.cu", "kv8_decode.cu", "kv8_prefill.cu", "gemv_w4.cu", "step_tables.cu",
 ]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -81,7 +81,7 @@ __device__ __forceinline__ void cluster_sync() {
 // NT: tiles of 8 tokens. GI: 32-k blocks that share a scale within a box (1, 2, or 4 for groups of 128
 // and multiples of it).
 template <int NT, int GI>
-__global__ void __launch_bounds__(kWarps * 32) gemv_kernel(const __grid_constant__ CUtensorMap wmap, const Params p) {
+__global__ void __launch_bounds__(kWarps * 32, 2) gemv_kernel(const __grid_constant__ CUtensorMap wmap, const Params p) {
   pdl_trigger();
   constexpr int MP = NT * 8;
   constexpr int GN = 8 / GI;  // scales of a row in one box
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kWarps * 32) gemv_kernel(const __grid_constant
       if (lane % (4 * GI) == 0) xsum[(sb * GN + lane / (4 * GI)) * MP + tok] = sum;
     }
     __syncthreads();
-    if (!live) continue;
+    if (!live || !ok) continue;  // (every warp passes the CTA's barriers)
     for (int i = c0; i < c0 + cn; ++i) {
       const int k0 = (sub0 + i) * kSub;
       float sa[GN], sb[GN], za[GN], zb[GN];
@@ -204,7 +204,6 @@ __global__ void __launch_bounds__(kWarps * 32) gemv_kernel(const __grid_constant
     }
     if (!ok) {  // a box that never came: the error is recorded; wait for the others in flight
       for (int i = c0; i < issued; ++i) mbar_wait(&s_bar[warp][i % kStages], (i / kStages) & 1, p.status);
-      break;
     }
   }
   __syncthreads();

@@ -1,0 +1,286 @@
+// A step's metadata from its requests' lengths, on the device: blocks taken from the FIFO ring for the
+// tokens to come, block tables, cumulative lengths, and for every new token its slot, position and
+// cache row, plus the prefill tiles.
+//
+// Integer work on a few bytes per request and token, bound by latency: one launch, one cluster of CTAs.
+// Every CTA reads the requests (two dependent loads) and scans them in shared memory, each for itself:
+// that costs less than handing the scans round. After one cluster barrier (every read of the allocator's
+// state lies before it, every write behind) each CTA writes its share of tokens, tiles and new blocks;
+// a token finds its request by bisection in shared memory and its block in the ring or in the request's
+// table row, so nobody waits for the table to be written.
+#include "cdb_common.cuh"
+
+namespace cdb {
+namespace step {
+
+constexpr int kThreads = 1024;
+constexpr int kBlock = 16;
+constexpr int kTile = 64;
+constexpr int kMaxRequests = 8192;
+
+struct Params {
+  const int32_t* slots;
+  const int32_t* seq_len;  // [table_rows] cached tokens per slot
+  const int32_t* new_len;  // [n]
+  const int32_t* row_len;  // [table_rows] blocks held per slot
+  int32_t* table;
+  int64_t table_stride;
+  int table_rows, table_width;
+  const int32_t* ring;
+  int ring_size;
+  const int32_t* state;  // {head, free, size, peak}
+  int32_t* row_len_out;
+  int32_t* state_out;
+  int32_t* granted;
+  int32_t* cu_q;
+  int32_t* cu_k;
+  int32_t* item_slot;
+  int32_t* item_pos;
+  int64_t* slot_map;
+  int cap;
+  int4* tiles;
+  int tile_cap;
+  int n;
+  int32_t* status;
+};
+
+// Block-wide exclusive scan of one value per thread; total receives the sum.
+__device__ __forceinline__ int64_t scan(int64_t v, int64_t* s_warp, int64_t& total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) s_warp[w] = x;
+  __syncthreads();
+  if (w == 0) {
+    int64_t y = s_warp[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t z = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) y += z;
+    }
+    s_warp[lane] = y;
+  }
+  __syncthreads();
+  const int64_t before = w ? s_warp[w - 1] : 0;
+  total = s_warp[31];
+  __syncthreads();
+  return before + x - v;
+}
+
+// Largest j with first[j] <= i, first ascending from 0 over n entries.
+__device__ __forceinline__ int find(const int32_t* first, int n, int i) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= i) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p, int ctas) {
+  pdl_trigger();
+  extern __shared__ int32_t smem[];
+  __shared__ int64_t s_warp[32];
+  const int n = p.n, rank = blockIdx.x;
+  int32_t* s_slot = smem;           // [n] -1: no such slot
+  int32_t* s_ctx = s_slot + n;      // cached tokens
+  int32_t* s_held = s_ctx + n;      // blocks held before
+  int32_t* s_need = s_held + n;     // blocks taken now; -1: refused
+  int32_t* s_block = s_need + n;    // [n] blocks taken before this request
+  int32_t* s_q = s_block + n;       // tokens before this request (its own tokens until they are scanned)
+  int32_t* s_t = s_q + n;           // tiles before this request
+  pdl_wait();
+
+  const int head = p.state[0], avail = p.state[1], peak = p.state[3];
+  const int nb = p.ring_size;
+  const bool sane = head >= 0 && head < nb && avail >= 0 && avail <= nb;
+  const int per = (n + kThreads - 1) / kThreads;
+  const int j0 = min(n, (int)threadIdx.x * per), j1 = min(n, j0 + per);
+  bool bad = !sane;
+  int64_t want = 0;
+  for (int j = j0; j < j1; ++j) {
+    const int slot = p.slots[j], fresh = p.new_len[j];
+    int ctx = 0, held = 0, need = -1;
+    const bool known = slot >= 0 && slot < p.table_rows;
+    if (known) {
+      ctx = p.seq_len[slot];
+      held = p.row_len[slot];
+      if (fresh >= 0 && ctx >= 0 && held >= 0) {
+        const int64_t total = ((int64_t)ctx + fresh + kBlock - 1) / kBlock;
+        if (total <= p.table_width && held <= p.table_width && sane) need = (int)(total > held ? total - held : 0);
+      }
+    }
+    bad = bad || !known || fresh < 0 || ctx < 0 || held < 0;
+    s_slot[j] = known ? slot : -1;
+    s_ctx[j] = ctx;
+    s_held[j] = held;
+    s_need[j] = need;
+    s_q[j] = fresh;
+    want += need > 0 ? need : 0;
+  }
+  int64_t all, all_q, all_k, all_t;
+  scan(want, s_warp, all);
+  if (all > avail) {  // not enough for everybody: in order, whoever still fits
+    if (threadIdx.x == 0) {
+      int left = avail;
+      for (int j = 0; j < n; ++j)
+        if (s_need[j] > left) s_need[j] = -1;
+        else if (s_need[j] > 0) left -= s_need[j];
+    }
+    __syncthreads();
+  }
+  int64_t blocks = 0, toks = 0, keys = 0, tls = 0;
+  for (int j = j0; j < j1; ++j) {
+    if (s_need[j] < 0) s_q[j] = 0;
+    blocks += s_need[j] > 0 ? s_need[j] : 0;
+    toks += s_q[j];
+    keys += s_need[j] < 0 ? 0 : (int64_t)s_ctx[j] + s_q[j];
+    tls += (s_q[j] + kTile - 1) / kTile;
+  }
+  int64_t b0 = scan(blocks, s_warp, all), q0 = scan(toks, s_warp, all_q), k0 = scan(keys, s_warp, all_k),
+          t0 = scan(tls, s_warp, all_t);
+  const bool fits = all_q <= p.cap && all_k <= 0x7fffffff && (p.tiles == nullptr || all_t <= p.tile_cap);
+  if (ctas > 1)
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  // Nothing was written so far: every CTA has read slots, lengths and state.
+  for (int j = j0; j < j1; ++j) {
+    const int fresh = s_q[j], need = s_need[j];
+    if (rank == 0) {
+      p.granted[j] = need >= 0 ? 1 : 0;
+      p.cu_q[j] = (int)q0;
+      p.cu_k[j] = (int)k0;
+      if (need >= 0) p.row_len_out[s_slot[j]] = s_held[j] + need;
+    }
+    s_block[j] = (int)b0;
+    s_q[j] = (int)q0;
+    s_t[j] = (int)t0;
+    b0 += need > 0 ? need : 0;
+    q0 += fresh;
+    k0 += need < 0 ? 0 : (int64_t)s_ctx[j] + fresh;
+    t0 += (fresh + kTile - 1) / kTile;
+  }
+  if (rank == 0) {
+    if (bad || !fits) set_error(p.status, CDB_ERR_INDEX);
+    if (threadIdx.x == 0) {
+      p.cu_q[n] = (int)all_q;
+      p.cu_k[n] = (int)all_k;
+      const int taken = (int)all;
+      p.state_out[0] = sane && nb > 0 ? (int)(((int64_t)head + taken) % nb) : head;
+      p.state_out[1] = avail - taken;
+      p.state_out[2] = nb;
+      p.state_out[3] = max(peak, nb - avail + taken);
+    }
+  }
+  __syncthreads();
+
+  const int first = rank * kThreads + threadIdx.x, step = ctas * kThreads;
+  // new blocks into the tables
+  for (int i = first; i < (int)all; i += step) {
+    const int j = find(s_block, n, i);  // the last request that starts at or before i: requests without blocks sort before
+    p.table[(int64_t)s_slot[j] * p.table_stride + s_held[j] + i - s_block[j]] = p.ring[(int)(((int64_t)head + i) % nb)];
+  }
+  // tokens
+  const int live = (int)(all_q < p.cap ? all_q : p.cap);
+  for (int i = first; i < p.cap; i += step) {
+    int slot = -1, pos = -1;
+    int64_t row = -1;
+    if (i < live) {
+      const int j = find(s_q, n, i);
+      slot = s_slot[j];
+      pos = s_ctx[j] + i - s_q[j];
+      const int page = pos / kBlock;
+      const int blk = page < s_held[j] ? p.table[(int64_t)slot * p.table_stride + page]
+                                       : p.ring[(int)(((int64_t)head + s_block[j] + page - s_held[j]) % nb)];
+      row = blk < 0 ? -1 : (int64_t)blk * kBlock + pos % kBlock;
+      if (blk < 0) set_error(p.status, CDB_ERR_INDEX);
+    }
+    p.item_slot[i] = slot;
+    p.item_pos[i] = pos;
+    p.slot_map[i] = row;
+  }
+  // tiles of up to 64 rows, in request order
+  if (p.tiles != nullptr) {
+    const int live_t = (int)(all_t < p.tile_cap ? all_t : p.tile_cap);
+    for (int i = first; i < p.tile_cap; i += step) {
+      int4 tile = make_int4(0, 0, 0, 0);
+      if (i < live_t && fits) {
+        const int j = find(s_t, n, i);
+        const int at = (i - s_t[j]) * kTile;
+        const int rows = (j + 1 < n ? s_q[j + 1] : (int)all_q) - s_q[j];
+        tile = make_int4(s_q[j] + at, min(kTile, rows - at), s_slot[j], s_ctx[j] + at);
+      }
+      p.tiles[i] = tile;
+    }
+  }
+}
+
+}  // namespace step
+}  // namespace cdb
+
+extern "C" int cdb_step_tables(const int32_t* slots, const int32_t* seq_len, const int32_t* new_len,
+                               const int32_t* row_len, int num_requests, int32_t* block_table,
+                               int64_t block_table_stride, int table_rows, int table_width, const int32_t* ring,
+                               int ring_size, const int32_t* state, int32_t* row_len_out, int32_t* state_out,
+                               int32_t* granted, int32_t* cu_seq_lens_q, int32_t* cu_seq_lens_k, int32_t* item_slot,
+                               int32_t* item_pos, int64_t* slot_map, int capacity, void* tiles, int tile_capacity,
+                               int32_t* status, void* stream) {
+  using namespace cdb;
+  using namespace cdb::step;
+  if (num_requests < 0 || capacity > (1 << 30) || tile_capacity > (1 << 30) || table_rows < 0 || table_width < 0 || ring_size < 0 || capacity < 0 || tile_capacity < 0 ||
+      row_len == nullptr || block_table == nullptr || ring == nullptr || state == nullptr || row_len_out == nullptr ||
+      state_out == nullptr || cu_seq_lens_q == nullptr || cu_seq_lens_k == nullptr ||
+      (num_requests > 0 && (slots == nullptr || seq_len == nullptr || new_len == nullptr || granted == nullptr)) ||
+      (capacity > 0 && (item_slot == nullptr || item_pos == nullptr || slot_map == nullptr)) ||
+      (reinterpret_cast<uintptr_t>(tiles) & 15) || (reinterpret_cast<uintptr_t>(slot_map) & 7))
+    return CDB_ERR_INVALID_ARGUMENT;
+  if (num_requests > kMaxRequests) return CDB_ERR_UNSUPPORTED;
+  Params p;
+  p.slots = slots;
+  p.seq_len = seq_len;
+  p.new_len = new_len;
+  p.row_len = row_len;
+  p.table = block_table;
+  p.table_stride = block_table_stride;
+  p.table_rows = table_rows;
+  p.table_width = table_width;
+  p.ring = ring;
+  p.ring_size = ring_size;
+  p.state = state;
+  p.row_len_out = row_len_out;
+  p.state_out = state_out;
+  p.granted = granted;
+  p.cu_q = cu_seq_lens_q;
+  p.cu_k = cu_seq_lens_k;
+  p.item_slot = item_slot;
+  p.item_pos = item_pos;
+  p.slot_map = slot_map;
+  p.cap = capacity;
+  p.tiles = static_cast<int4*>(tiles);
+  p.tile_cap = tile_capacity;
+  p.n = num_requests;
+  p.status = status;
+  // One CTA covers a decode step; more tokens are worth a cluster's launch and barrier.
+  const int ctas = capacity <= 2 * kThreads ? 1 : 8;
+  const size_t smem = (size_t)7 * num_requests * 4;
+  if (cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return CDB_ERR_CUDA;
+  prefer_max_shared(reinterpret_cast<const void*>(step_tables_kernel));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctas > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, step_tables_kernel, p, ctas) == cudaSuccess ? CDB_OK : CDB_ERR_CUDA;
+}

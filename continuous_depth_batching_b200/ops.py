@@ -489,3 +489,113 @@ def kv8_decode_attention(q, out, codes, scales, cache_layer, block_table, item_s
         block_table.shape[0], block_table.shape[1], item_slot.data_ptr(), item_pos.data_ptr(), n, num_heads, kv_heads,
         dim, scale, ctas, ws.data_ptr(), ws.numel(), counters.data_ptr(), _status(q).data_ptr(),
     )
+
+
+@_define(
+    "kv8_prefill_attention(Tensor q, Tensor(a!) out, Tensor codes, Tensor scales, int cache_layer, Tensor block_table, "
+    "Tensor tiles, int num_heads, float scale) -> ()"
+)
+def kv8_prefill_attention(q, out, codes, scales, cache_layer, block_table, tiles, num_heads, scale):
+    """Causal attention of prompt chunks over the 8-bit cache (``cdb_kv8_prefill_attention``).
+    ``tiles [n, 4]`` int32 as ``OuroRunner.prefill_tiles`` or ``step_tables`` make them: first row, rows
+    (at most 64; 0 for an unused entry), slot, position of the first row. The chunk's own keys and
+    values are in the cache already, ``q`` is rotated."""
+
+    dev = _one_device(q, out, codes, scales, block_table, tiles)
+    layers, blocks, kv_heads, dim = _kv8_cache(codes, scales, cache_layer)
+    _kv8_heads(num_heads, kv_heads)
+    if tiles.dtype != torch.int32 or tiles.dim() != 2 or tiles.shape[1] != 4 or not tiles.is_contiguous() or tiles.data_ptr() % 16:
+        raise ValueError(f"tiles must be a contiguous 16-byte aligned int32 tensor [n, 4], got {tiles.dtype} {tuple(tiles.shape)}")
+    if tiles.shape[0] > 65535:
+        raise ValueError(f"one call takes at most 65535 tiles, got {tiles.shape[0]}")
+    rows = q.shape[0]
+    _rows_of("q", q, 0, num_heads * dim)
+    _rows_of("out", out, rows, num_heads * dim)
+    _table_of("block_table", block_table)
+    _launch(
+        dev, "cdb_kv8_prefill_attention", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), rows,
+        codes.data_ptr(), scales.data_ptr(), layers, cache_layer, blocks, block_table.data_ptr(), block_table.stride(0),
+        block_table.shape[0], block_table.shape[1], tiles.data_ptr(), tiles.shape[0], num_heads, kv_heads, dim, scale,
+        _status(q).data_ptr(),
+    )
+
+
+@_define(
+    "step_tables(Tensor slots, Tensor seq_len, Tensor new_len, Tensor row_len, Tensor(a!) block_table, Tensor ring, "
+    "Tensor state, Tensor(b!) row_len_out, Tensor(c!) state_out, Tensor(d!) granted, Tensor(e!) cu_seq_lens_q, "
+    "Tensor(f!) cu_seq_lens_k, Tensor(g!) item_slot, Tensor(h!) item_pos, Tensor(i!) slot_map, Tensor(j!)? tiles) -> ()"
+)
+def step_tables(slots, seq_len, new_len, row_len, block_table, ring, state, row_len_out, state_out, granted,
+                cu_seq_lens_q, cu_seq_lens_k, item_slot, item_pos, slot_map, tiles):
+    """One step's metadata from its requests' lengths (``cdb_step_tables``): blocks for the new tokens
+    taken from the FIFO ring into ``block_table``, cumulative lengths, every token's slot, position and
+    cache row (-1 behind the last), and the prefill tiles. ``row_len_out`` / ``state_out`` may be
+    ``row_len`` / ``state`` themselves."""
+
+    dev = _one_device(slots, seq_len, new_len, row_len, block_table, ring, state, row_len_out, state_out, granted,
+                      cu_seq_lens_q, cu_seq_lens_k, item_slot, item_pos, slot_map, tiles)
+    n, rows = slots.numel(), row_len.numel()
+    _int_row("slots", slots, n)
+    _int_row("new_len", new_len, n)
+    _int_row("granted", granted, n)
+    _int_row("cu_seq_lens_q", cu_seq_lens_q, n + 1)
+    _int_row("cu_seq_lens_k", cu_seq_lens_k, n + 1)
+    _int_row("row_len", row_len, rows)
+    _int_row("row_len_out", row_len_out, rows)
+    _int_row("seq_len", seq_len, rows)
+    _int_row("ring", ring, 0)
+    _int_row("state", state, 4)
+    _int_row("state_out", state_out, 4)
+    _table_of("block_table", block_table)
+    if block_table.shape[0] < rows:
+        raise ValueError(f"block_table needs a row for each of the {rows} slots, got {block_table.shape[0]}")
+    cap = item_pos.numel()
+    _int_row("item_pos", item_pos, cap)
+    _int_row("item_slot", item_slot, cap)
+    _int_row("slot_map", slot_map, cap, torch.int64)
+    if n > 8192:
+        raise ValueError(f"one call takes at most 8192 requests, got {n}")
+    if tiles is not None and (tiles.dtype != torch.int32 or tiles.dim() != 2 or tiles.shape[1] != 4 or not tiles.is_contiguous() or tiles.data_ptr() % 16):
+        raise ValueError(f"tiles must be a contiguous 16-byte aligned int32 tensor [n, 4], got {tiles.dtype} {tuple(tiles.shape)}")
+    _launch(
+        dev, "cdb_step_tables", slots.data_ptr(), seq_len.data_ptr(), new_len.data_ptr(), row_len.data_ptr(), n,
+        block_table.data_ptr(), block_table.stride(0), rows, block_table.shape[1], ring.data_ptr(), ring.numel(),
+        state.data_ptr(), row_len_out.data_ptr(), state_out.data_ptr(), granted.data_ptr(), cu_seq_lens_q.data_ptr(),
+        cu_seq_lens_k.data_ptr(), item_slot.data_ptr(), item_pos.data_ptr(), slot_map.data_ptr(), cap,
+        _lib.ptr(tiles), 0 if tiles is None else tiles.shape[0], _status(slots).data_ptr(),
+    )
+
+
+@_define("gemv_w4(Tensor x, Tensor w, Tensor scales, Tensor? zeros, Tensor(a!) out) -> ()")
+def gemv_w4(x, w, scales, zeros, out):
+    """``out [M, N] = x [M, K] @ W.T`` for a few token rows, ``W = scales * (q - zeros)`` from 4-bit
+    ``w [N, K / 2]`` uint8 (low nibble first), bf16 ``scales [N, K / group]`` and uint8 ``zeros`` of the
+    same shape (None: 8) (``cdb_gemv_w4``). Groups of 32, 64 or a multiple of 128. The weights are
+    read once per 32 rows: above some hundred rows ``gemm_bf16`` is the better call."""
+
+    dev = _one_device(x, w, scales, zeros, out)
+    if w.dtype != torch.uint8 or w.dim() != 2 or w.shape[0] == 0 or w.shape[1] == 0 or w.stride(1) != 1:
+        raise ValueError(f"w must be a 2-D uint8 tensor [N, K / 2] with unit column stride, got {w.dtype} {tuple(w.shape)}")
+    n, k = w.shape[0], 2 * w.shape[1]
+    ldw = w.stride(0) if n > 1 else -(-w.shape[1] // 16) * 16
+    if k % 32 or ldw % 16 or ldw < w.shape[1] or w.data_ptr() % 16:
+        raise ValueError(f"w needs K a multiple of 32, a row stride that is a multiple of 16 bytes and 16-byte alignment, got K {k}")
+    _dtype("scales", scales, torch.bfloat16, 2)
+    groups = scales.shape[1]
+    if scales.shape[0] != n or groups == 0 or k % groups or not scales.is_contiguous():
+        raise ValueError(f"scales must be contiguous [{n}, K / group], got {tuple(scales.shape)} for K {k}")
+    group = k // groups
+    if group not in (32, 64) and group % 128:
+        raise ValueError(f"groups of 32, 64 or a multiple of 128 are taken, got {group}")
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape or not zeros.is_contiguous()):
+        raise ValueError(f"zeros must be a contiguous uint8 tensor {tuple(scales.shape)}, got {zeros.dtype} {tuple(zeros.shape)}")
+    m = x.shape[0]
+    _rows_of("x", x, m, k)
+    if x.shape[1] != k:
+        raise ValueError(f"x has {x.shape[1]} columns, the weights {k}")
+    if out.dtype != torch.bfloat16 or out.shape != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
+        raise ValueError(f"out must be a bf16 tensor [{m}, {n}] with unit column stride, got {out.dtype} {tuple(out.shape)}")
+    _launch(
+        dev, "cdb_gemv_w4", x.data_ptr(), max(x.stride(0), k), w.data_ptr(), ldw, scales.data_ptr(), _lib.ptr(zeros),
+        out.data_ptr(), max(out.stride(0), n), m, n, k, group, _sm_count(dev), _status(x).data_ptr(),
+    )

@@ -515,6 +515,60 @@ int cdb_kv8_decode_attention(const void* q, int64_t q_stride, void* out, int64_t
                              int num_kv_heads, int head_dim, float scale, int num_ctas, float* workspace,
                              int64_t workspace_floats, int32_t* counters, int32_t* status, void* stream);
 
+/* Causal prefill attention over the 8-bit cache; the 8-bit sibling of cdb_prefill_attention.
+ *   tiles      int4 [num_tiles] {first row, rows <= 64, slot, position of the first row}, 16-byte
+ *              aligned, num_tiles <= 65535: consecutive rows of one request; row r of a tile attends
+ *              to positions 0 .. position + r. An entry of 0 rows is skipped, and rows that no tile
+ *              names are left as they were. The rows' keys and values are in the cache
+ *              (cdb_kv8_append), q is rotated.
+ *   q, out, num_heads as cdb_kv8_decode_attention; num_rows: rows that q and out have. */
+int cdb_kv8_prefill_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, int num_rows,
+                              const void* codes, const float* scales, int num_cache_layers, int cache_layer,
+                              int num_blocks, const int32_t* block_table, int64_t block_table_stride, int table_rows,
+                              int table_width, const void* tiles, int num_tiles, int num_heads, int num_kv_heads,
+                              int head_dim, float scale, int32_t* status, void* stream);
+
+/* A step's metadata from its requests' lengths, in one launch: what _allocate_blocks_if_needed
+ * (scheduler_base.py:416-433) and _prepare_recurrent_stage_buffers (model_runner.py:704-754) do per
+ * request on the host. Request j (num_requests <= 8192; each slot at most once) in slot slots[j] has
+ * seq_len[slot] cached tokens, row_len[slot] blocks, and new_len[j] (>= 0) tokens to come.
+ *   blocks     a request needs ceil((seq_len + new_len) / 16) - row_len more blocks, taken from the
+ *              ring's head in request order and written behind those of its block-table row (ring and
+ *              state as cdb_block_alloc; ring_size entries). When the ring holds too few for all, or
+ *              a row would pass table_width, requests that do not fit are refused in order
+ *              (granted[j] = 0, no blocks, no tokens), later ones that do are served.
+ *   row_len_out [table_rows], state_out [4]: the allocator after the step; only rows of granted
+ *              requests are written. They may be row_len and state.
+ *   cu_seq_lens_q / _k  [num_requests + 1]: sums of new tokens and of seq_len + new_len (0 for a
+ *              refused request).
+ *   item_slot, item_pos, slot_map [capacity]: per new token, requests in order, its slot, position
+ *              and cache row (block * 16 + place); -1 behind the last token.
+ *   tiles      NULL, or int4 [tile_capacity] for the prefill attention entry points: runs of at most
+ *              64 rows in order, entries behind the last all zero.
+ * An unknown slot, a negative length, an invalid ring state, or more tokens or tiles than the
+ * capacities hold set CDB_ERR_INDEX (with too many tiles no tile is written). */
+int cdb_step_tables(const int32_t* slots, const int32_t* seq_len, const int32_t* new_len, const int32_t* row_len,
+                    int num_requests, int32_t* block_table, int64_t block_table_stride, int table_rows,
+                    int table_width, const int32_t* ring, int ring_size, const int32_t* state, int32_t* row_len_out,
+                    int32_t* state_out, int32_t* granted, int32_t* cu_seq_lens_q, int32_t* cu_seq_lens_k,
+                    int32_t* item_slot, int32_t* item_pos, int64_t* slot_map, int capacity, void* tiles,
+                    int tile_capacity, int32_t* status, void* stream);
+
+/* A few token rows times 4-bit weights with group scales (weight-only quantised nn.Linear):
+ *   out[m][n] = bf16( sum_j s[n][j] * sum over k in group j of (q[n][k] - z[n][j]) * x[m][k] ), fp32 sums.
+ *   x          bf16 [M][ldx], 16-byte aligned, ldx a multiple of 8.
+ *   w          uint8 [N][ldw], 16-byte aligned, ldw (bytes) a multiple of 16: byte k / 2 of row n
+ *              holds q[n][k] in its low nibble for even k, in its high nibble for odd k. K a
+ *              multiple of 32.
+ *   scales     bf16 [N][K / group_size]; group_size 32, 64 or a multiple of 128 that divides K.
+ *   zeros      uint8 [N][K / group_size], or NULL: 8 everywhere.
+ *   out        bf16 [M][ldo].
+ * The weights are read once for every 32 rows of x. Results do not depend on anything but the shapes
+ * and num_sms. */
+int cdb_gemv_w4(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* scales, const void* zeros,
+                void* out, int64_t ldo, int M, int N, int K, int group_size, int num_sms, int32_t* status,
+                void* stream);
+
 #ifdef __cplusplus
 }
 #endif
