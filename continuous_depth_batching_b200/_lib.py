@@ -14,6 +14,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libcdb_b200.so"
+TORCH_OPS_PATH = LIB_PATH.with_name("libcdb_torch.so")  # torch.ops.cdb.* defined in C++ over the C ABI
 
 # int32 entries of an attention work-plan header (CDB_ATTN_PLAN_HEADER_INTS in the C header)
 ATTN_PLAN_MAX_CHUNKS = 1024
@@ -203,6 +204,22 @@ def load() -> ctypes.CDLL:
         fn.restype = _RESTYPES.get(name, c_int)
     _LIB = lib
     return lib
+
+
+_TORCH_OPS_LOADED = False
+
+
+def load_torch_ops() -> None:
+    """Load the C++ operator library once (it registers its operators when it is loaded)."""
+
+    global _TORCH_OPS_LOADED
+    if _TORCH_OPS_LOADED:
+        return
+    load()
+    if not TORCH_OPS_PATH.exists():
+        raise CDBError(f"{TORCH_OPS_PATH} is missing: build it with `python -m continuous_depth_batching_b200.csrc.build`")
+    torch.ops.load_library(str(TORCH_OPS_PATH))
+    _TORCH_OPS_LOADED = True
 
 
 def exported_symbols() -> list[str]:

@@ -1,9 +1,10 @@
-"""Build libcdb_b200.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a.
+"""Build libcdb_b200.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a, and libcdb_torch.so
+(PyTorch operators in C++ over it) with g++.
 
     python -m continuous_depth_batching_b200.csrc.build
 
-The library lands next to the package (``continuous_depth_batching_b200/libcdb_b200.so``) so
-it ships with the source tree; it is loaded with ctypes by ``continuous_depth_batching_b200._lib``.
+The libraries land next to the package (``continuous_depth_batching_b200/libcdb_b200.so``) so
+they ship with the source tree; ``continuous_depth_batching_b200._lib`` loads them, the first with ctypes.
 """
 
 from __future__ import annotations
@@ -18,6 +19,7 @@ CSRC = Path(__file__).resolve().parent
 PKG = CSRC.parent
 REPO = PKG.parent
 LIB_NAME = "libcdb_b200.so"
+TORCH_LIB_NAME = "libcdb_torch.so"
 SOURCES = [
     "attention.cu", "prefill_attention.cu", "elementwise.cu", "gemm.cu", "scheduler.cu", "fused_ops.cu", "kv_swap.cu",
     "kv8_append.cu", "kv8_decode.cu", "kv8_prefill.cu", "gemv_w4.cu", "step_tables.cu",
@@ -85,9 +87,30 @@ def build_library(force: bool = False, verbose: bool = False, jobs: int | None =
         raise RuntimeError(f"nvcc failed for {failed}")
     lib = library_path()
     if force or _stale(lib, objs):
-        cmd = [nvcc, *ARCH_FLAGS, "-shared", "-o", str(lib), *map(str, objs)]
+        cmd = [nvcc, *ARCH_FLAGS, "-shared", "-Xlinker", f"-soname={LIB_NAME}", "-o", str(lib), *map(str, objs)]
         subprocess.run(cmd, check=True)
+    build_torch_ops(lib, force)
     return lib
+
+
+def build_torch_ops(lib: Path, force: bool = False) -> Path:
+    """Compile ``torch_ops.cpp`` against the installed torch and link it to the CUDA library."""
+
+    import torch
+
+    src, out = CSRC / "torch_ops.cpp", PKG / TORCH_LIB_NAME
+    if not force and not _stale(out, [src, lib, REPO / "include" / "cdb_b200.h"]):
+        return out
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc_path()).resolve().parent.parent
+    cmd = [
+        "g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}", f"-I{cuda / 'include'}", str(src),
+        "-o", str(out), str(lib), f"-L{root / 'lib'}", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+        f"-L{cuda / 'lib64'}", "-lcudart", "-Wl,-rpath,$ORIGIN",
+    ]
+    subprocess.run(cmd, check=True)
+    return out
 
 
 if __name__ == "__main__":

@@ -320,3 +320,106 @@ def test_decode_on_two_streams_and_in_two_graphs():
                     call(i)
         torch.cuda.synchronize()
         assert all(torch.equal(o, w) for o, w in zip(outs, want)), rep
+
+
+def _prefill(c: Cache, q, spans, heads, layer=1, extra_tiles=0, table=None, codes=None):
+    codes_g, scales, table_g = c.gpu()
+    tiles, row = [], 0
+    for s, (first, n) in enumerate(spans):
+        tiles += [(row + i, min(64, n - i), s, first + i) for i in range(0, n, 64)]
+        row += n
+    tiles = tiles[::-1] + [(0, 0, 0, 0)] * extra_tiles
+    out = torch.full((row, heads * c.codes.shape[-1]), 7.0, dtype=torch.bfloat16, device=DEV)
+    torch.ops.cdb.kv8_prefill_attention(q.to(DEV), out, codes_g, scales, layer, table_g,
+                                        torch.tensor(tiles, dtype=torch.int32, device=DEV), heads, c.codes.shape[-1] ** -0.5)
+    torch.cuda.synchronize()
+    assert ops.status_code() == 0
+    return out.cpu()
+
+
+def _check_prefill(out, c: Cache, q, spans, heads, layer=1):
+    d, row = c.codes.shape[-1], 0
+    for s, (first, n) in enumerate(spans):
+        o, a = ref.attend(q[row : row + n].view(n, heads, d), c.codes[layer], c.scales[layer], c.table[s], first, d**-0.5)
+        got = out[row : row + n].double().view(n, heads, d)
+        assert ((got - o).abs() <= 2.0**-8 * o.abs() + 2.0**-10 * a).all(), (s, first, n)
+        row += n
+
+
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("kv_heads,group", [(1, 1), (2, 3), (1, 8)])
+def test_prefill_matches_definition(d, kv_heads, group):
+    spans = [(0, 1), (0, 64), (5, 65), (100, 130), (63, 2), (300, 17), (0, 200), (1000, 64)]
+    heads = kv_heads * group
+    c = Cache([a + n for a, n in spans], kv_heads, d, seed=d + heads)
+    q = torch.randn(sum(n for _, n in spans), heads * d, generator=c.gen).bfloat16()
+    _check_prefill(_prefill(c, q, spans, heads, extra_tiles=3), c, q, spans, heads)
+
+
+def test_prefill_of_one_row_is_decode():
+    spans = [(p, 1) for p in (0, 3, 16, 200, 511)]
+    c = Cache([p + 1 for p, _ in spans], 2, 128, seed=30)
+    q = torch.randn(5, 4 * 128, generator=c.gen).bfloat16()
+    _check_prefill(_prefill(c, q, spans, 4), c, q, spans, 4)
+    _check_prefill(_decode(c, q, [p for p, _ in spans], 4), c, q, spans, 4)
+
+
+def test_prefill_scales_far_apart():
+    spans = [(40, 60)]
+    c = Cache([100], 1, 128, seed=31)
+    c.scales[1, 1, c.table[0, 1].long()] = 2.0**40
+    c.scales[1, 1, c.table[0, 3].long()] = 2.0**-40
+    c.scales[1, 1, c.table[0, 6].long()] = 2.0**-126
+    q = torch.randn(60, 128, generator=c.gen).bfloat16() * 30
+    _check_prefill(_prefill(c, q, spans, 1), c, q, spans, 1)
+
+
+def test_prefill_masked_places_hold_nan():
+    """NaN in keys and values that a row may not see does not reach it; rows that see it get it, in the
+    dims that hold it."""
+
+    spans = [(10, 80), (0, 50)]
+    c = Cache([90, 50], 1, 64, seed=32)
+    q = torch.randn(130, 2 * 64, generator=c.gen).bfloat16()
+    want = _prefill(c, q, spans, 2)
+    raw = c.codes.view(torch.uint8)
+    for s, (first, n) in enumerate(spans):  # behind the last token
+        end = first + n
+        raw[1, :, int(c.table[s, (end - 1) // BS]), :, (end - 1) % BS + 1 :] = 0xFF
+    assert torch.equal(_prefill(c, q, spans, 2), want)
+    raw[1, 1, int(c.table[0, 70 // BS]), 0, 70 % BS, 5] = 0x7F  # one value of position 70
+    got = _prefill(c, q, spans, 2)
+    sees = torch.zeros(130, dtype=torch.bool)
+    sees[60:80] = True  # positions 70 .. 89
+    bad = got.isnan().view(130, 2, 64)
+    assert bad[sees][:, :, 5].all() and bad.sum() == 20 * 2
+    assert torch.equal(got.nan_to_num(0)[~sees], want[~sees])
+    raw[1, 0, int(c.table[0, 64 // BS]), 0, 0, 0] = 0x7F  # a key of position 64: rows that see it are NaN throughout
+    got = _prefill(c, q, spans, 2)
+    assert torch.equal(got[:54], want[:54]) and got[54:80].isnan().all() and torch.equal(got[80:], want[80:])
+
+
+def test_prefill_refuses_tiles_that_do_not_fit():
+    c = Cache([64] * 2, 1, 64, seed=33, layers=1)
+    c.table[1, 2] = -5
+    codes, scales, table = c.gpu()
+    q = torch.randn(64, 64, device=DEV).bfloat16()
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    sp = torch.cuda.current_stream().cuda_stream
+
+    def call(*tile):
+        out = torch.full((64, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+        status.zero_()
+        t = torch.tensor([tile], dtype=torch.int32, device=DEV)
+        _lib.call("cdb_kv8_prefill_attention", _lib.ptr(q), 64, _lib.ptr(out), 64, 64, _lib.ptr(codes), _lib.ptr(scales), 1, 0,
+                  c.blocks, _lib.ptr(table), table.stride(0), 2, table.shape[1], _lib.ptr(t), 1, 1, 1, 64, 0.125,
+                  _lib.ptr(status), sp)
+        return out, int(status.item())
+
+    for tile in [(0, 65, 0, 0), (1, 64, 0, 0), (-1, 4, 0, 0), (0, 4, 2, 0), (0, 4, -1, 0), (0, 4, 0, -1), (0, 64, 0, 5000)]:
+        out, code = call(*tile)
+        assert code == 6 and (out == 7).all(), tile
+    out, code = call(0, 0, 99, -4)
+    assert code == 0 and (out == 7).all()
+    out, code = call(0, 64, 1, 0)  # a missing block: its keys do not count
+    assert code == 6 and out.isfinite().all() and (out[:, :] != 7).any()
