@@ -36,7 +36,8 @@ struct Params {
   const uint8_t* zeros;         // [N][groups] or null (8)
   __nv_bfloat16* out;
   int64_t ldo;
-  int m, n, k, groups, group;
+  int m, n, k, groups;
+  int group_boxes;  // 128-k spans of one group, for groups of 128 and more
   int subs;        // boxes along k
   int subs_cta;    // boxes of one CTA of the cluster
   int chunk_subs;  // boxes whose token rows are staged at a time
@@ -123,7 +124,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gemv_kernel(const __grid_const
   float acc[NT][4];
 #pragma unroll
   for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-  const int ra = min(row0 + g, p.n - 1), rb = min(row0 + g + 8, p.n - 1);
+  const int64_t ra = (int64_t)min(row0 + g, p.n - 1) * p.groups, rb = (int64_t)min(row0 + g + 8, p.n - 1) * p.groups;
+  const __nv_bfloat16 *scale_a = p.scales + ra, *scale_b = p.scales + rb;
+  const uint8_t *zero_a = p.zeros + ra, *zero_b = p.zeros + rb;
   bool ok = true;
 
   for (int c0 = 0; c0 < subs; c0 += p.chunk_subs) {
@@ -150,16 +153,20 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gemv_kernel(const __grid_const
     __syncthreads();
     if (!live || !ok) continue;  // (every warp passes the CTA's barriers)
     for (int i = c0; i < c0 + cn; ++i) {
-      const int k0 = (sub0 + i) * kSub;
+      // this box's scales and offsets 128 + z, two weight rows a lane
       float sa[GN], sb[GN], za[GN], zb[GN];
 #pragma unroll
       for (int j = 0; j < GN; ++j) {
-        const int grp = min((k0 + j * 32 * GI) / p.group, p.groups - 1);
-        const int64_t ia = (int64_t)ra * p.groups + grp, ib = (int64_t)rb * p.groups + grp;
-        sa[j] = bf16_to_f(p.scales[ia]);
-        sb[j] = bf16_to_f(p.scales[ib]);
-        za[j] = p.zeros != nullptr ? (float)(128 + p.zeros[ia]) : 136.f;
-        zb[j] = p.zeros != nullptr ? (float)(128 + p.zeros[ib]) : 136.f;
+        int grp = (sub0 + i) * GN + j;
+        if (GI == 4 && p.group_boxes > 1) grp /= p.group_boxes;
+        grp = min(grp, p.groups - 1);  // a box may reach past k: its x are zeros there
+        sa[j] = bf16_to_f(scale_a[grp]);
+        sb[j] = bf16_to_f(scale_b[grp]);
+        za[j] = zb[j] = 136.f;
+        if (p.zeros != nullptr) {
+          za[j] = (float)(128 + zero_a[grp]);
+          zb[j] = (float)(128 + zero_b[grp]);
+        }
       }
       ok = ok && __all_sync(kFull, mbar_wait(&s_bar[warp][i % kStages], (i / kStages) & 1, p.status));
       if (!ok) break;
@@ -325,15 +332,19 @@ extern "C" int cdb_gemv_w4(const void* x, int64_t ldx, const void* w, int64_t ld
   p.m = M;
   p.n = N;
   p.k = K;
-  p.group = group_size;
+  p.group_boxes = group_size > 128 ? group_size / 128 : 1;
   p.groups = K / group_size;
   p.subs = (K + kSub - 1) / kSub;
   p.status = status;
   const int nt = M > 24 ? 4 : (M + 7) / 8;
   const int row_ctas = (N + kWarps * kRows - 1) / (kWarps * kRows);
-  // Split k until there are two CTAs for every SM or a CTA would get less than one box.
+  // Split k over the cluster size that leaves the fewest boxes to the busiest of the 2 num_sms resident
+  // CTAs (rounds of CTAs times boxes of one); the smaller cluster where two are alike.
   int cluster = 1;
-  while (cluster < kMaxCluster && row_ctas * cluster < 2 * num_sms && cluster * 2 <= p.subs) cluster *= 2;
+  for (int c = 1, best = 0; c <= kMaxCluster && c <= p.subs; c *= 2) {
+    const int rounds = (row_ctas * c + 2 * num_sms - 1) / (2 * num_sms), cost = rounds * ((p.subs + c - 1) / c);
+    if (best == 0 || cost < best) best = cost, cluster = c;
+  }
   p.cluster = cluster;
   p.subs_cta = (p.subs + cluster - 1) / cluster;
   p.chunk_subs = p.subs_cta < 64 / (nt * 8) ? p.subs_cta : (64 / (nt * 8) > 0 ? 64 / (nt * 8) : 1);

@@ -5,7 +5,7 @@
 // bias and rotates in fp32, takes the tile's largest magnitude, settles the block's scale, rescales
 // the codes that were there when the scale grew, and writes codes and scale. Nobody else touches the
 // tile, so no atomics and no second pass over the new values. The query heads are rotated by other
-// warps of the same launch. Bound by bytes for prompts (q, k, v in, q and codes out) and by the chain
+// warps of the same launch, a few heads of a row or two at a time. Bound by bytes for prompts (q, k, v in, q and codes out) and by the chain
 // of dependent loads (position, block id, values) for a decode step.
 #include "kv8.cuh"
 
@@ -42,28 +42,45 @@ __device__ __forceinline__ void unpack8(uint4 w, float (&a)[8]) {
   a[4] = bf16lo(w.z), a[5] = bf16hi(w.z), a[6] = bf16lo(w.w), a[7] = bf16hi(w.w);
 }
 
-// Dims [x0, x0 + 8) of one head vector, biased and rotated in fp32 with no rounding in between (the
-// caller rounds once: to bf16 for q, to e4m3 for k). Every lane of the warp calls it, `on` or not:
-// the split-half partner chunk comes from the lane that holds it. Angles are the tables' values.
+// The cos and sin entries of dims [x0, x0 + 8) at one position: 8 + 8 bf16 (mode 1) or 4 + 4 fp32 (mode 2).
+struct Angles {
+  uint4 c, s;
+};
+
 template <int D>
-__device__ __forceinline__ void rotated8(const AppendParams& p, const __nv_bfloat16* x, const __nv_bfloat16* bias,
-                                         int mode, int pos, int x0, bool on, float (&y)[8]) {
-  constexpr int LPR = D / 8;  // lanes per row
-  const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-  unpack8(on ? ld16(x + x0) : z, y);
-  if (bias != nullptr) {
-    float b[8];
-    unpack8(on ? ld16(bias + x0) : z, b);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] += b[e];
+__device__ __forceinline__ Angles load_angles(const AppendParams& p, int mode, int pos, int x0, bool on) {
+  Angles a;
+  a.c = a.s = make_uint4(0u, 0u, 0u, 0u);
+  if (on && mode == 1) {
+    const int64_t at = (int64_t)pos * D + x0;
+    a.c = ld16(static_cast<const __nv_bfloat16*>(p.rope_cos) + at);
+    a.s = ld16(static_cast<const __nv_bfloat16*>(p.rope_sin) + at);
+  } else if (on && mode == 2) {
+    const int64_t at = (int64_t)pos * (D / 2) + x0 / 2;
+    a.c = ld16(static_cast<const float*>(p.rope_cos) + at);
+    a.s = ld16(static_cast<const float*>(p.rope_sin) + at);
   }
+  return a;
+}
+
+// One head vector's dims [x0, x0 + 8), biased and rotated in fp32 with no rounding in between (the caller
+// rounds once: to bf16 for q, to e4m3 for k). Every lane of the warp calls it: the split-half partner
+// chunk comes from the lane that holds it.
+template <int D>
+__device__ __forceinline__ void rotated8(uint4 raw, uint4 bias, int mode, const Angles& a, int x0, float (&y)[8]) {
+  constexpr int LPR = D / 8;  // lanes per row
+  unpack8(raw, y);
+  float b[8];
+  unpack8(bias, b);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] += b[e];
   if (mode == 1) {
     const int lane = threadIdx.x & 31;
     const bool low = x0 < D / 2;
     const int src = (low ? lane + LPR / 2 : lane - LPR / 2) & 31;
     float c[8], s[8];
-    unpack8(on ? ld16(static_cast<const __nv_bfloat16*>(p.rope_cos) + (int64_t)pos * D + x0) : z, c);
-    unpack8(on ? ld16(static_cast<const __nv_bfloat16*>(p.rope_sin) + (int64_t)pos * D + x0) : z, s);
+    unpack8(a.c, c);
+    unpack8(a.s, s);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float o = __shfl_sync(0xffffffffu, y[e], src);
@@ -72,16 +89,12 @@ __device__ __forceinline__ void rotated8(const AppendParams& p, const __nv_bfloa
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = fmaf(y[e], c[e], s[e]);
   } else if (mode == 2) {
-    const float4 zf = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int64_t at = (int64_t)pos * (D / 2) + x0 / 2;
-    const float4 c = on ? *reinterpret_cast<const float4*>(static_cast<const float*>(p.rope_cos) + at) : zf;
-    const float4 s = on ? *reinterpret_cast<const float4*>(static_cast<const float*>(p.rope_sin) + at) : zf;
-    const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+    const uint32_t cc[4] = {a.c.x, a.c.y, a.c.z, a.c.w}, ss[4] = {a.s.x, a.s.y, a.s.z, a.s.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float a = y[2 * i], b = y[2 * i + 1];
-      y[2 * i] = fmaf(a, cc[i], -b * ss[i]);
-      y[2 * i + 1] = fmaf(b, cc[i], a * ss[i]);
+      const float u = y[2 * i], v = y[2 * i + 1], c = __uint_as_float(cc[i]), s = __uint_as_float(ss[i]);
+      y[2 * i] = fmaf(u, c, -v * s);
+      y[2 * i + 1] = fmaf(v, c, u * s);
     }
   }
 }
@@ -91,129 +104,173 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a <= 3.402823466e38f ? a : 0.f;  // infinities saturate and NaN stays NaN, under the others' scale
 }
 
+// q: a warp rotates HB heads of RPI rows, with the rows' angles in registers and the heads' loads in
+// flight together.
+constexpr int HB = 4;
+
 template <int D>
-__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+__device__ __forceinline__ void rotate_q(const AppendParams& p, int row0, int head0) {
+  constexpr int LPR = D / 8, RPI = 32 / LPR;
+  const int lane = threadIdx.x & 31;
+  const int sub = lane / LPR, x0 = (lane % LPR) * 8;
+  const int r = row0 + sub;
+  const int pos = sub < RPI && r < p.num_items ? p.item_pos[r] : -1;
+  const bool on = pos >= 0 && (p.rope_mode == 0 || pos < p.rope_rows);
+  const Angles a = load_angles<D>(p, p.rope_mode, pos, x0, on);
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  uint4 raw[HB], bias[HB];
+#pragma unroll
+  for (int h = 0; h < HB; ++h) {
+    const bool has = on && head0 + h < p.num_heads;
+    raw[h] = has ? ld16(p.qkv + (int64_t)r * p.qkv_stride + (int64_t)(head0 + h) * D + x0) : zero;
+    bias[h] = has && p.qk_bias != nullptr ? ld16(p.qk_bias + (int64_t)(head0 + h) * D + x0) : zero;
+  }
+#pragma unroll
+  for (int h = 0; h < HB; ++h) {
+    float y[8];
+    rotated8<D>(raw[h], bias[h], p.rope_mode, a, x0, y);
+    if (on && head0 + h < p.num_heads)
+      *reinterpret_cast<uint4*>(p.q_out + (int64_t)r * p.q_out_stride + (int64_t)(head0 + h) * D + x0) =
+          make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
+                     pack_bf16x2(y[6], y[7]));
+  }
+}
+
+// The run of rows that starts at row r, if one does: its rows all lie in one block.
+struct Run {
+  int slot, pos, n;
+  int64_t blk;
+};
+
+// False where no run starts at r. Uniform over the warp.
+__device__ __forceinline__ bool find_run(const AppendParams& p, int r, Run& run) {
+  const int lane = threadIdx.x & 31;
+  // lane 16 looks at the row before, lanes 0..15 at rows r .. r + 15: two loads deep in all
+  const int at = lane == kBlock ? r - 1 : r + lane;
+  const bool in = at >= 0 && at < p.num_items && lane <= kBlock;
+  const int pos = in ? p.item_pos[at] : -1, slot = in ? p.item_slot[at] : -1;
+  run.pos = __shfl_sync(0xffffffffu, pos, 0);
+  run.slot = __shfl_sync(0xffffffffu, slot, 0);
+  const int before = __shfl_sync(0xffffffffu, pos, kBlock), before_slot = __shfl_sync(0xffffffffu, slot, kBlock);
+  if (run.pos < 0) return false;
+  if (before >= 0 && before_slot == run.slot && before / kBlock == run.pos / kBlock) {
+    // a later row of a run; one that does not follow its predecessor has no place in the block
+    if (before + 1 != run.pos && lane == 0) set_error(p.status, CDB_ERR_INDEX);
+    return false;
+  }
+  const bool next = lane < kBlock && slot == run.slot && pos == run.pos + lane && run.pos % kBlock + lane < kBlock;
+  run.n = __ffs(~__ballot_sync(0xffffffffu, next)) - 1;
+  run.blk = -1;
+  if (run.slot >= 0 && run.slot < p.bt_rows && run.pos / kBlock < p.bt_width &&
+      (p.rope_mode == 0 || run.pos + run.n <= p.rope_rows))
+    run.blk = p.block_table[(int64_t)run.slot * p.bt_stride + run.pos / kBlock];
+  if (run.blk < 0 || run.blk >= p.num_blocks) {
+    if (lane == 0) set_error(p.status, CDB_ERR_INDEX);
+    return false;
+  }
+  return true;
+}
+
+// k or v of one head of a run. ROWS: the most rows a run may have here (16, or what one pass holds).
+template <int D, int ROWS>
+__device__ __forceinline__ void write_tile(const AppendParams& p, int r, const Run& run, int head, bool is_v) {
+  constexpr int LPR = D / 8, RPI = 32 / LPR, IT = (ROWS + RPI - 1) / RPI;
+  const int lane = threadIdx.x & 31;
+  const int sub = lane / LPR, x0 = (lane % LPR) * 8;
+  const int mode = is_v ? 0 : p.rope_mode;
+  const int off = run.pos % kBlock;
+  const int64_t tile = ((int64_t)(is_v ? p.num_blocks : 0) + run.blk) * p.num_kv_heads + head;
+  uint8_t* codes = p.codes + tile * (kBlock * D);
+  const float was = off > 0 ? p.scales[tile] : 0.f;
+  const int64_t col = (int64_t)(p.num_heads + (is_v ? p.num_kv_heads : 0) + head) * D + x0;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  const uint4 bias =
+      !is_v && p.qk_bias != nullptr && sub < RPI ? ld16(p.qk_bias + (int64_t)(p.num_heads + head) * D + x0) : zero;
+  uint4 raw[IT];
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int j = it * RPI + sub;
+    raw[it] = sub < RPI && j < run.n ? ld16(p.qkv + (int64_t)(r + j) * p.qkv_stride + col) : zero;
+  }
+  float y[IT][8];
+  float amax = 0.f;
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int j = it * RPI + sub;
+    const bool on = sub < RPI && j < run.n;
+    const Angles a = load_angles<D>(p, mode, run.pos + j, x0, on);
+    rotated8<D>(raw[it], on ? bias : zero, mode, a, x0, y[it]);  // zeros where no row is
+#pragma unroll
+    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(y[it][e]));
+  }
+  amax = warp_max(amax);
+  float scale = block_scale(amax);
+  if (off > 0) {
+    if (was >= scale) {
+      scale = was;
+    } else {  // the block grows: its old codes move down by a power of two
+      const float ratio = was / scale;
+      for (int c = lane; c < off * LPR; c += 32) {
+        uint2* at = reinterpret_cast<uint2*>(codes + c * 8);
+        const uint2 old = *at;
+        const uint32_t w[2] = {old.x, old.y};
+        uint32_t o[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float a, b, c2, d;
+          unpack_f16x2(cvt_e4m3x2_f16x2(w[k] & 0xffffu), a, b);
+          unpack_f16x2(cvt_e4m3x2_f16x2(w[k] >> 16), c2, d);
+          o[k] = cvt_f32x2_e4m3x2(a * ratio, b * ratio) | (cvt_f32x2_e4m3x2(c2 * ratio, d * ratio) << 16);
+        }
+        *at = make_uint2(o[0], o[1]);
+      }
+    }
+  }
+  const float inv = 1.f / scale;
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int j = it * RPI + sub;
+    if (sub < RPI && j < run.n) {
+      const uint32_t lo = cvt_f32x2_e4m3x2(y[it][0] * inv, y[it][1] * inv) |
+                          (cvt_f32x2_e4m3x2(y[it][2] * inv, y[it][3] * inv) << 16);
+      const uint32_t hi = cvt_f32x2_e4m3x2(y[it][4] * inv, y[it][5] * inv) |
+                          (cvt_f32x2_e4m3x2(y[it][6] * inv, y[it][7] * inv) << 16);
+      *reinterpret_cast<uint2*>(codes + (off + j) * D + x0) = make_uint2(lo, hi);
+    }
+  }
+  if (lane == 0) p.scales[tile] = scale;
+}
+
+// A CTA takes `group` rows: blockIdx.y first counts the q warps' tasks (RPI rows x HB heads), then those
+// of the k and v warps (one head of one of them, every run that starts in the group).
+template <int D>
+__global__ void __launch_bounds__(256, D == 64 ? 3 : 2) append_kernel(const AppendParams p) {
   pdl_trigger();
   pdl_wait();
-  constexpr int LPR = D / 8;       // lanes of one row, 8 dims each
-  constexpr int RPI = 32 / LPR;    // rows per iteration (96: lanes 24..31 idle)
-  constexpr int IT = kBlock / RPI;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int RPI = 32 / (D / 8);
+  const int warp = threadIdx.x >> 5;
   const int row0 = blockIdx.x * p.group;
   const int rows = min(p.group, p.num_items - row0);
-  const bool in_row = lane < LPR * RPI;
-  const int sub = in_row ? lane / LPR : 0, x0 = in_row ? (lane % LPR) * 8 : 0;
-  const int q_tasks = p.q_out != nullptr ? p.num_heads : 0;
+  const int q_rows = (p.group + RPI - 1) / RPI, q_heads = (p.num_heads + HB - 1) / HB;
+  const int q_tasks = p.q_out != nullptr ? q_rows * q_heads : 0;
   const int tasks = q_tasks + 2 * p.num_kv_heads;
-  const int64_t k_col = (int64_t)p.num_heads * D, v_col = k_col + (int64_t)p.num_kv_heads * D;
-
   for (int task = blockIdx.y * 8 + warp; task < tasks; task += gridDim.y * 8) {
     if (task < q_tasks) {
-      const __nv_bfloat16* bias = p.qk_bias != nullptr ? p.qk_bias + (int64_t)task * D : nullptr;
-      for (int i = 0; i < rows; i += RPI) {
-        const int r = row0 + i + sub;
-        const int pos = in_row && i + sub < rows ? p.item_pos[r] : -1;
-        const bool on = pos >= 0 && (p.rope_mode == 0 || pos < p.rope_rows);
-        if (!__any_sync(0xffffffffu, on)) continue;
-        float y[8];
-        rotated8<D>(p, p.qkv + (int64_t)r * p.qkv_stride + (int64_t)task * D, bias, p.rope_mode, pos, x0, on, y);
-        if (on)
-          *reinterpret_cast<uint4*>(p.q_out + (int64_t)r * p.q_out_stride + (int64_t)task * D + x0) =
-              make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
-                         pack_bf16x2(y[6], y[7]));
-      }
+      const int i = task / q_heads, h = task - i * q_heads;
+      rotate_q<D>(p, row0 + i * RPI, h * HB);
       continue;
     }
     const int kt = task - q_tasks;
     const bool is_v = kt >= p.num_kv_heads;
     const int head = is_v ? kt - p.num_kv_heads : kt;
-    const int mode = is_v ? 0 : p.rope_mode;
-    const __nv_bfloat16* bias =
-        !is_v && p.qk_bias != nullptr ? p.qk_bias + (int64_t)(p.num_heads + head) * D : nullptr;
-    const int64_t col = (is_v ? v_col : k_col) + (int64_t)head * D;
-
     for (int i = 0; i < rows; ++i) {
-      // Rows i .. i + 15 of the call: where the run that starts at row i ends.
-      const int r = row0 + i;
-      const int pos = p.item_pos[r];
-      if (pos < 0) continue;
-      const int slot = p.item_slot[r];
-      if (r > 0) {
-        const int before = p.item_pos[r - 1];
-        if (before >= 0 && p.item_slot[r - 1] == slot && before / kBlock == pos / kBlock) {
-          // a later row of a run; one that does not follow its predecessor has no place in the block
-          if (before + 1 != pos && lane == 0) set_error(p.status, CDB_ERR_INDEX);
-          continue;
-        }
-      }
-      bool next = false;
-      if (lane < kBlock && r + lane < p.num_items)
-        next = p.item_slot[r + lane] == slot && p.item_pos[r + lane] == pos + lane &&
-               pos % kBlock + lane < kBlock;
-      const int n = __ffs(~__ballot_sync(0xffffffffu, next)) - 1;
-      int blk = -1;
-      if (slot >= 0 && slot < p.bt_rows && pos / kBlock < p.bt_width &&
-          (p.rope_mode == 0 || pos + n <= p.rope_rows))
-        blk = p.block_table[(int64_t)slot * p.bt_stride + pos / kBlock];
-      if (blk < 0 || blk >= p.num_blocks) {
-        if (lane == 0) set_error(p.status, CDB_ERR_INDEX);
-        continue;
-      }
-      const int off = pos % kBlock;
-      const int64_t tile = ((int64_t)(is_v ? p.num_blocks : 0) + blk) * p.num_kv_heads + head;
-      uint8_t* codes = p.codes + tile * (kBlock * D);
-      const float was = off > 0 ? p.scales[tile] : 0.f;
-
-      float y[IT][8];
-      float amax = 0.f;
-#pragma unroll
-      for (int it = 0; it < IT; ++it) {
-        if (it * RPI >= n) break;
-        const int j = it * RPI + sub;
-        const bool on = in_row && j < n;
-        rotated8<D>(p, p.qkv + (int64_t)(r + j) * p.qkv_stride + col, bias, mode, pos + j, x0, on, y[it]);
-        if (on) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(y[it][e]));
-        }
-      }
-      amax = warp_max(amax);
-      float scale = block_scale(amax);
-      if (off > 0) {
-        if (was >= scale) {
-          scale = was;
-        } else {  // the block grows: its old codes move down by a power of two
-          const float ratio = was / scale;
-          for (int c = lane; c < off * LPR; c += 32) {
-            uint2* at = reinterpret_cast<uint2*>(codes + c * 8);
-            const uint2 old = *at;
-            const uint32_t w[2] = {old.x, old.y};
-            uint32_t o[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              float a, b, c2, d;
-              unpack_f16x2(cvt_e4m3x2_f16x2(w[k] & 0xffffu), a, b);
-              unpack_f16x2(cvt_e4m3x2_f16x2(w[k] >> 16), c2, d);
-              o[k] = cvt_f32x2_e4m3x2(a * ratio, b * ratio) | (cvt_f32x2_e4m3x2(c2 * ratio, d * ratio) << 16);
-            }
-            *at = make_uint2(o[0], o[1]);
-          }
-        }
-      }
-      const float inv = 1.f / scale;
-#pragma unroll
-      for (int it = 0; it < IT; ++it) {
-        if (it * RPI >= n) break;
-        const int j = it * RPI + sub;
-        if (in_row && j < n) {
-          const uint32_t lo = cvt_f32x2_e4m3x2(y[it][0] * inv, y[it][1] * inv) |
-                              (cvt_f32x2_e4m3x2(y[it][2] * inv, y[it][3] * inv) << 16);
-          const uint32_t hi = cvt_f32x2_e4m3x2(y[it][4] * inv, y[it][5] * inv) |
-                              (cvt_f32x2_e4m3x2(y[it][6] * inv, y[it][7] * inv) << 16);
-          *reinterpret_cast<uint2*>(codes + (off + j) * D + x0) = make_uint2(lo, hi);
-        }
-      }
-      if (lane == 0) p.scales[tile] = scale;
+      Run run;
+      if (!find_run(p, row0 + i, run)) continue;
+      if (run.n <= RPI)
+        write_tile<D, RPI>(p, row0 + i, run, head, is_v);
+      else
+        write_tile<D, kBlock>(p, row0 + i, run, head, is_v);
+      i += run.n - 1;
     }
   }
 }
@@ -317,7 +374,9 @@ extern "C" int cdb_kv8_append(const void* qkv, int64_t qkv_stride, void* q_out, 
   // Decode steps have a run per row: one row per CTA spreads them. Prompts have a run per 16 rows, and
   // a CTA per row would start 15 of 16 kv warps for nothing.
   p.group = num_items <= 1024 ? 1 : kBlock;
-  const int tasks = (q_out != nullptr ? num_heads : 0) + 2 * num_kv_heads;
+  const int rpi = 32 / (head_dim / 8);
+  const int tasks =
+      (q_out != nullptr ? (p.group + rpi - 1) / rpi * ((num_heads + HB - 1) / HB) : 0) + 2 * num_kv_heads;
   const dim3 grid((num_items + p.group - 1) / p.group, min(65535, (tasks + 7) / 8));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (head_dim == 128)

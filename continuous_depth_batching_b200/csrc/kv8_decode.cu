@@ -19,12 +19,15 @@
 // Pieces of a segment (m, l, o) meet in two steps: the warps of a CTA through shared memory, CTAs
 // through the workspace, where the last one to arrive adds them up in CTA order. The result does not
 // depend on which one that is.
+#include <cuda.h>
+
 #include "kv8.cuh"
 
 namespace cdb {
 namespace kv8 {
 
 constexpr int kWarps = 8;
+constexpr int kMaxStages = 4;
 constexpr int kGroup = 8;  // query heads of one segment (the n of an m16n8k16 product)
 constexpr uint32_t kFull = 0xffffffffu;
 
@@ -62,9 +65,9 @@ __device__ __forceinline__ int row_pages(const DecodeParams& p, int b, bool& bad
   return pos / kBlock + 1;
 }
 
-// A place in the page stream: page `page` of row `row`, virtual head `vh` (kv head * groups + group).
+// A place in the page stream: page `page` of row `row`, query-head group `grp` of kv head `kvh`.
 struct Cursor {
-  int row, vh, page, pages, pos, slot;
+  int row, kvh, grp, page, pages, pos, slot;
 };
 
 __device__ __forceinline__ void load_row(const DecodeParams& p, Cursor& c) {
@@ -74,11 +77,14 @@ __device__ __forceinline__ void load_row(const DecodeParams& p, Cursor& c) {
   c.slot = p.item_slot[c.row];
 }
 
-__device__ __forceinline__ void advance(const DecodeParams& p, Cursor& c, int vheads) {
+// To the next page.
+__device__ __forceinline__ void advance(const DecodeParams& p, Cursor& c) {
   if (++c.page < c.pages) return;
   c.page = 0;
-  if (++c.vh < vheads) return;
-  c.vh = 0;
+  if (++c.grp < p.groups) return;
+  c.grp = 0;
+  if (++c.kvh < p.kv_heads) return;
+  c.kvh = 0;
   do {
     if (++c.row >= p.num_items) return;  // the stream's end
     load_row(p, c);
@@ -91,6 +97,22 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
+__device__ __forceinline__ void tensor_load(uint32_t dst, const CUtensorMap* map, int row, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(bar)
+      : "memory");
+}
+
+// 4 bytes to shared memory, asynchronously; async_arrive lets `bar` count their completion.
+__device__ __forceinline__ void async_copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -99,45 +121,60 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
 
 // Where a piece lies in its segment, for the joins.
 struct PieceTag {
-  int row, vh;
+  int row, kvh, grp;
   int first, last, pages;  // pages [first, last) of `pages`
 };
 
 template <int D>
 struct Shape {
-  static constexpr int KD = D / 4;        // dims of K that a lane multiplies: [t * KD, t * KD + KD) of rows g, g + 8
-  static constexpr int VD = D / 8;        // dims of V that a lane multiplies: [g * VD, g * VD + VD) of 4 tokens
-  static constexpr int KS = D / 16;       // k-steps of K q
-  static constexpr int MT = D / 16;       // m-tiles of V^T P
-  static constexpr int TILE = kBlock * D; // bytes of a K or V tile
+  static constexpr int KD = D / 4;         // dims of K that a lane multiplies: [t * KD, t * KD + KD) of rows g, g + 8
+  static constexpr int VD = D / 8;         // dims of V that a lane multiplies: [g * VD, g * VD + VD) of 4 tokens
+  static constexpr int KS = D / 16;        // k-steps of K q
+  static constexpr int MT = D / 16;        // m-tiles of V^T P
+  static constexpr int TILE = kBlock * D;  // bytes of a K or V tile
+  // Rows of 128 and 64 bytes come through a tensor map with the swizzle of that width, which spreads
+  // the fragment loads below over the banks (unswizzled, a V load hits each bank four times); rows of 96
+  // bytes spread by themselves and come as one untiled copy.
+  static constexpr bool SWIZZLED = D != 96;
 };
 
-// The running softmax of one segment piece and what a lane holds of V^T P: dims g * VD + 4 i + {0, 1, 2,
-// 3} of heads 2t, 2t + 1 in acc[2i][0, 2], acc[2i + 1][0, 2] (head 2t) and [1, 3] (head 2t + 1).
+// Byte offset of byte c (16-byte aligned) of row r in a tile.
 template <int D>
+__device__ __forceinline__ int tile_at(int r, int c) {
+  if (D == 128) return r * 128 + (c ^ ((r & 7) << 4));
+  if (D == 64) return r * 64 + (c ^ (((r >> 1) & 3) << 4));
+  return r * D + c;
+}
+
+// The running softmax of one segment piece and what a lane holds of V^T P: dims g * VD + 4 i + {0, 1, 2,
+// 3} of head 2t (h = 0) and 2t + 1 (h = 1) in acc[2i][h], acc[2i][2 + h], acc[2i + 1][h], acc[2i + 1][2 + h].
+// HN: heads a lane keeps (1 where a kv head has one query head: only h = 0 of t = 0 means anything then).
+template <int D, int HN>
 struct Running {
   float acc[Shape<D>::MT][4];
-  float m[2], mw[2], l[2];
+  float m[HN], mw[HN], l[HN];
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < Shape<D>::MT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-    m[0] = m[1] = mw[0] = mw[1] = -INFINITY;
-    l[0] = l[1] = 0.f;
+#pragma unroll
+    for (int h = 0; h < HN; ++h) {
+      m[h] = mw[h] = -INFINITY;
+      l[h] = 0.f;
+    }
   }
 };
 
 // q's rows of one segment as the B operand: head g of the group, dims [t * KD, (t + 1) * KD). e is the
 // power of two that was divided out (for heads 2t and 2t + 1).
-template <int D>
-__device__ __forceinline__ void load_q(const DecodeParams& p, int row, int vh, uint32_t (&qf)[Shape<D>::KS][2],
-                                       float (&factor)[2]) {
+template <int D, int HN>
+__device__ __forceinline__ void load_q(const DecodeParams& p, const Cursor& c, uint32_t (&qf)[Shape<D>::KS][2],
+                                       float (&factor)[HN]) {
   constexpr int KD = Shape<D>::KD;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int kvh = vh / p.groups, grp = vh - kvh * p.groups;
-  const int in_kv = grp * kGroup + g;
+  const int in_kv = c.grp * kGroup + g;
   const bool on = in_kv < p.heads_per_kv;
   const __nv_bfloat16* src =
-      p.q + (int64_t)row * p.q_stride + (int64_t)(kvh * p.heads_per_kv + (on ? in_kv : 0)) * D + t * KD;
+      p.q + (int64_t)c.row * p.q_stride + (int64_t)(c.kvh * p.heads_per_kv + (on ? in_kv : 0)) * D + t * KD;
   uint32_t w[KD / 2];
 #pragma unroll
   for (int i = 0; i < KD / 8; ++i) {
@@ -156,78 +193,113 @@ __device__ __forceinline__ void load_q(const DecodeParams& p, int row, int vh, u
 #pragma unroll
   for (int i = 0; i < KD / 2; ++i) qf[i >> 1][i & 1] = pack_f16x2(bf16lo(w[i]) * down, bf16hi(w[i]) * down);
   const float f = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
-  factor[0] = __shfl_sync(kFull, f, t * 8);  // lanes of head 2t, then 2t + 1
-  factor[1] = __shfl_sync(kFull, f, t * 8 + 4);
+#pragma unroll
+  for (int h = 0; h < HN; ++h) factor[h] = __shfl_sync(kFull, f, t * 8 + h * 4);  // the lanes of head 2t + h
 }
 
 // One page: `live` tokens of it count.
-template <int D>
+template <int D, int HN>
 __device__ __forceinline__ void page_step(const uint8_t* k, const uint8_t* v, float sk, float sv, int live,
-                                          const uint32_t (&qf)[Shape<D>::KS][2], const float (&factor)[2],
-                                          Running<D>& r) {
+                                          const uint32_t (&qf)[Shape<D>::KS][2], const float (&factor)[HN],
+                                          Running<D, HN>& r) {
   constexpr int KD = Shape<D>::KD, VD = Shape<D>::VD;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
-  {
-    uint32_t ka[KD / 4], kb[KD / 4];
-    const uint8_t* r0 = k + g * D + t * KD;
-    const uint8_t* r1 = r0 + 8 * D;
+  uint32_t ka[KD / 4], kb[KD / 4];
+  if constexpr (KD % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < KD / 16; ++i) {
+      const uint4 x = *reinterpret_cast<const uint4*>(k + tile_at<D>(g, t * KD + i * 16));
+      const uint4 y = *reinterpret_cast<const uint4*>(k + tile_at<D>(g + 8, t * KD + i * 16));
+      ka[4 * i] = x.x, ka[4 * i + 1] = x.y, ka[4 * i + 2] = x.z, ka[4 * i + 3] = x.w;
+      kb[4 * i] = y.x, kb[4 * i + 1] = y.y, kb[4 * i + 2] = y.z, kb[4 * i + 3] = y.w;
+    }
+  } else {
 #pragma unroll
     for (int i = 0; i < KD / 8; ++i) {
-      const uint2 x = *reinterpret_cast<const uint2*>(r0 + i * 8), y = *reinterpret_cast<const uint2*>(r1 + i * 8);
+      const uint2 x = *reinterpret_cast<const uint2*>(k + g * D + t * KD + i * 8);
+      const uint2 y = *reinterpret_cast<const uint2*>(k + (g + 8) * D + t * KD + i * 8);
       ka[2 * i] = x.x, ka[2 * i + 1] = x.y, kb[2 * i] = y.x, kb[2 * i + 1] = y.y;
     }
-#pragma unroll
-    for (int i = 0; i < KD / 4; ++i)
-      mma_f16(s, cvt_e4m3x2_f16x2(ka[i] & 0xffffu), cvt_e4m3x2_f16x2(kb[i] & 0xffffu), cvt_e4m3x2_f16x2(ka[i] >> 16),
-              cvt_e4m3x2_f16x2(kb[i] >> 16), qf[i][0], qf[i][1]);
   }
-  // s[0], s[1]: token g, heads 2t, 2t + 1; s[2], s[3]: token g + 8
-  const float ev = sv > 0.f ? __log2f(sv) : -126.f;
-  float pw[2][2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const float f = factor[h] * sk;
-    const float x0 = g < live ? s[h] * f : -INFINITY;
-    const float x1 = g + 8 < live ? s[2 + h] * f : -INFINITY;
-    float mx = fmaxf(x0, x1);
-    mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
-    mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
-    mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
-    // m and M move only when passed by 8: the weights stay within 2^8
-    if (mx > r.m[h] + 8.f) {
-      r.l[h] *= ex2(r.m[h] - mx);
-      r.m[h] = mx;
-    }
-    const bool up = mx + ev > r.mw[h] + 8.f;
-    if (__any_sync(kFull, up)) {
-      const float to = up ? mx + ev : r.mw[h];
-      const float down = up ? ex2(r.mw[h] - to) : 1.f;
-#pragma unroll
-      for (int i = 0; i < Shape<D>::MT; ++i) r.acc[i][h] *= down, r.acc[i][2 + h] *= down;
-      r.mw[h] = to;
-    }
-    const float p0 = x0 == -INFINITY ? 0.f : ex2(x0 - r.m[h]);
-    const float p1 = x1 == -INFINITY ? 0.f : ex2(x1 - r.m[h]);
-    r.l[h] += p0 + p1;
-    pw[0][h] = x0 == -INFINITY ? 0.f : ex2(x0 + ev - r.mw[h]);
-    pw[1][h] = x1 == -INFINITY ? 0.f : ex2(x1 + ev - r.mw[h]);
-  }
-  const uint32_t b0 = transpose8(pack_f16x2(pw[0][0], pw[0][1]));
-  const uint32_t b1 = transpose8(pack_f16x2(pw[1][0], pw[1][1]));
   // V: tokens 2t, 2t + 1, 2t + 8, 2t + 9, dims [g * VD, (g + 1) * VD)
   uint32_t vw[4][VD / 4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int tok = 2 * t + (j & 1) + 8 * (j >> 1);
-    const uint8_t* src = v + tok * D + g * VD;
+    if constexpr (VD == 16) {
+      const uint4 x = *reinterpret_cast<const uint4*>(v + tile_at<D>(tok, g * 16));
+      vw[j][0] = x.x, vw[j][1] = x.y, vw[j][2] = x.z, vw[j][3] = x.w;
+    } else if constexpr (VD == 8) {
+      const uint2 x = *reinterpret_cast<const uint2*>(v + tile_at<D>(tok, (g >> 1) * 16) + (g & 1) * 8);
+      vw[j][0] = x.x, vw[j][1] = x.y;
+    } else {
 #pragma unroll
-    for (int i = 0; i < VD / 4; ++i) vw[j][i] = *reinterpret_cast<const uint32_t*>(src + i * 4);
-    if (tok >= live) {  // codes behind the row's end may be anything, NaN too
-#pragma unroll
-      for (int i = 0; i < VD / 4; ++i) vw[j][i] = 0u;
+      for (int i = 0; i < VD / 4; ++i) vw[j][i] = *reinterpret_cast<const uint32_t*>(v + tok * D + g * VD + i * 4);
     }
   }
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < KD / 4; ++i)
+    mma_f16(s, cvt_e4m3x2_f16x2(ka[i] & 0xffffu), cvt_e4m3x2_f16x2(kb[i] & 0xffffu), cvt_e4m3x2_f16x2(ka[i] >> 16),
+            cvt_e4m3x2_f16x2(kb[i] >> 16), qf[i][0], qf[i][1]);
+  // s[h]: token g, head 2t + h; s[2 + h]: token g + 8
+  const float ev = sv > 0.f ? __log2f(sv) : -126.f;
+  float x[HN][2];
+  bool up = false;
+#pragma unroll
+  for (int h = 0; h < HN; ++h) {
+    const float f = factor[h] * sk;
+    x[h][0] = s[h] * f;
+    x[h][1] = s[2 + h] * f;
+  }
+  if (live < kBlock) {
+#pragma unroll
+    for (int h = 0; h < HN; ++h) {
+      if (g >= live) x[h][0] = -INFINITY;
+      if (g + 8 >= live) x[h][1] = -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // codes behind the row's end may be anything, NaN too
+      if (2 * t + (j & 1) + 8 * (j >> 1) >= live) {
+#pragma unroll
+        for (int i = 0; i < VD / 4; ++i) vw[j][i] = 0u;
+      }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < HN; ++h) {
+    const float mx = fmaxf(x[h][0], x[h][1]);
+    up = up || mx > r.m[h] + 8.f || mx + ev > r.mw[h] + 8.f;
+  }
+  // m and M only move when a logit passes them by 8 (the weights stay within 2^8): a vote a page
+  if (__any_sync(kFull, up)) {
+#pragma unroll
+    for (int h = 0; h < HN; ++h) {
+      float mx = fmaxf(x[h][0], x[h][1]);
+      mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
+      mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
+      mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
+      const float m = fmaxf(r.m[h], mx), mw = fmaxf(r.mw[h], mx + ev);
+      r.l[h] *= m == -INFINITY ? 1.f : ex2(r.m[h] - m);
+      const float down = mw == -INFINITY ? 1.f : ex2(r.mw[h] - mw);
+      r.m[h] = m;
+      r.mw[h] = mw;
+#pragma unroll
+      for (int i = 0; i < Shape<D>::MT; ++i) r.acc[i][h] *= down, r.acc[i][2 + h] *= down;
+    }
+  }
+  float pw[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+  for (int h = 0; h < HN; ++h) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const bool off = x[h][j] == -INFINITY;  // also where m is still -inf
+      r.l[h] += off ? 0.f : ex2(x[h][j] - r.m[h]);
+      pw[j][h] = off ? 0.f : ex2(x[h][j] + ev - r.mw[h]);
+    }
+  }
+  const uint32_t b0 = transpose8(pack_f16x2(pw[0][0], pw[0][1]));
+  const uint32_t b1 = transpose8(pack_f16x2(pw[1][0], pw[1][1]));
 #pragma unroll
   for (int i = 0; i < VD / 4; ++i) {
     const uint32_t lo0 = __byte_perm(vw[0][i], vw[1][i], 0x5140), hi0 = __byte_perm(vw[0][i], vw[1][i], 0x7362);
@@ -240,17 +312,17 @@ __device__ __forceinline__ void page_step(const uint8_t* k, const uint8_t* v, fl
 }
 
 // A finished segment's output, straight from a warp's registers (l already summed over the warp).
-template <int D>
-__device__ __forceinline__ void write_out(const DecodeParams& p, int row, int vh, const Running<D>& r) {
+template <int D, int HN>
+__device__ __forceinline__ void write_out(const DecodeParams& p, const Cursor& c, const Running<D, HN>& r) {
   constexpr int VD = Shape<D>::VD;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int kvh = vh / p.groups, grp = vh - kvh * p.groups;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int in_kv = grp * kGroup + 2 * t + h;
+  for (int h = 0; h < HN; ++h) {
+    const int in_kv = c.grp * kGroup + 2 * t + h;
     if (in_kv >= p.heads_per_kv) continue;
     const float f = r.l[h] > 0.f ? ex2(r.mw[h] - r.m[h]) / r.l[h] : (r.l[h] == 0.f ? 0.f : r.l[h]);
-    __nv_bfloat16* dst = p.out + (int64_t)row * p.out_stride + (int64_t)(kvh * p.heads_per_kv + in_kv) * D + g * VD;
+    __nv_bfloat16* dst =
+        p.out + (int64_t)c.row * p.out_stride + (int64_t)(c.kvh * p.heads_per_kv + in_kv) * D + g * VD;
 #pragma unroll
     for (int i = 0; i < VD / 4; ++i)
       *reinterpret_cast<uint2*>(dst + i * 4) =
@@ -260,12 +332,12 @@ __device__ __forceinline__ void write_out(const DecodeParams& p, int row, int vh
 }
 
 // A piece: per stored head D values of o = sum 2^(x-m) v, then m and l.
-template <int D>
-__device__ __forceinline__ void store_piece(float* dst, int heads, const Running<D>& r) {
+template <int D, int HN>
+__device__ __forceinline__ void store_piece(float* dst, int heads, const Running<D, HN>& r) {
   constexpr int VD = Shape<D>::VD;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < HN; ++h) {
     const int head = 2 * t + h;
     if (head >= heads) continue;
     float* o = dst + head * (D + 2);
@@ -283,22 +355,28 @@ __device__ __forceinline__ void store_piece(float* dst, int heads, const Running
   }
 }
 
-template <int D>
-__global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const DecodeParams p) {
+template <int D, int HN>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+    decode_kernel(const __grid_constant__ CUtensorMap map, const DecodeParams p) {
   pdl_trigger();
   constexpr int TILE = Shape<D>::TILE;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int64_t s_before[kWarps * 32 + 1];  // pages before each thread's rows
   __shared__ int64_t s_warp[kWarps];
   __shared__ PieceTag s_tag[kWarps][2];
-  __shared__ __align__(8) uint64_t s_bar[kWarps][4];
+  __shared__ __align__(8) uint64_t s_bar[kWarps][kMaxStages];
+  __shared__ __align__(8) float s_scale[kWarps][kMaxStages][2];  // K's and V's of a page; K's < 0: no such block
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int vheads = p.kv_heads * p.groups;
   const int piece_floats = p.stored_heads * (D + 2);
   uint8_t* ring = smem + (size_t)warp * p.stages * 2 * TILE;
-  float* s_piece = reinterpret_cast<float*>(smem + (size_t)kWarps * p.stages * 2 * TILE);
+  // A piece that ends inside its segment's first page run (slot 0) has a place of its own, one that ends
+  // the warp's share (slot 1) lies over the ring, which is empty by then.
+  float* piece[2] = {reinterpret_cast<float*>(smem + (size_t)kWarps * p.stages * 2 * TILE) + warp * piece_floats,
+                     reinterpret_cast<float*>(ring)};
   if (lane == 0) {
-    for (int i = 0; i < p.stages; ++i) mbar_init(&s_bar[warp][i], 1);
+    for (int i = 0; i < p.stages; ++i) mbar_init(&s_bar[warp][i], 2);
     fence_barrier_init();
     s_tag[warp][0].row = s_tag[warp][1].row = -1;
   }
@@ -353,14 +431,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const DecodePara
       ++c.row;
       load_row(p, c);
     }
-    c.vh = (int)(at / c.pages);
-    c.page = (int)(at - (int64_t)c.vh * c.pages);
+    const int vh = (int)(at / c.pages);
+    c.page = (int)(at - (int64_t)vh * c.pages);
+    c.kvh = vh / p.groups;
+    c.grp = vh - c.kvh * p.groups;
 
-    const int64_t v_tiles = (int64_t)p.num_blocks * p.kv_heads;
-    const uint32_t ring_u = smem_u32(ring);
+    const int v_tiles = p.num_blocks * p.kv_heads;
+    const uint32_t ring_u = smem_u32(ring), bar_u = smem_u32(&s_bar[warp][0]), scale_u = smem_u32(&s_scale[warp][0][0]);
     Cursor ahead = c;
-    int issued = 0;
-    // Lane i of the issuing window holds block ids of 32 pages of the cursor's row.
+    int issued = 0, put = 0;
+    // Lane i holds block ids of a window of 32 pages of the issuing cursor's row.
     int win_row = -1, win_first = 0, win_id = -1;
     auto issue = [&]() {
       const int first = ahead.page & ~31;
@@ -370,83 +450,84 @@ __global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const DecodePara
         win_id = first + lane < ahead.pages ? p.block_table[(int64_t)ahead.slot * p.bt_stride + first + lane] : -1;
       }
       const int blk = __shfl_sync(kFull, win_id, ahead.page & 31);
-      const int st = issued % p.stages;
       if (lane == 0) {
         if (blk >= 0 && blk < p.num_blocks) {
-          const int64_t tile = (int64_t)blk * p.kv_heads + ahead.vh / p.groups;
-          const uint32_t bar = smem_u32(&s_bar[warp][st]);
-          mbar_arrive_expect_tx(&s_bar[warp][st], 2 * TILE);
-          bulk_load(ring_u + st * 2 * TILE, p.codes + tile * TILE, TILE, bar);
-          bulk_load(ring_u + st * 2 * TILE + TILE, p.codes + (v_tiles + tile) * TILE, TILE, bar);
+          const int tile = blk * p.kv_heads + ahead.kvh;
+          const uint32_t bar = bar_u + put * 8, dst = ring_u + put * 2 * TILE;
+          mbar_arrive_expect_tx(&s_bar[warp][put], 2 * TILE);
+          if (Shape<D>::SWIZZLED) {
+            tensor_load(dst, &map, tile * kBlock, bar);
+            tensor_load(dst + TILE, &map, (v_tiles + tile) * kBlock, bar);
+          } else {
+            bulk_load(dst, p.codes + (int64_t)tile * TILE, TILE, bar);
+            bulk_load(dst + TILE, p.codes + (int64_t)(v_tiles + tile) * TILE, TILE, bar);
+          }
+          async_copy4(scale_u + put * 8, p.scales + tile);
+          async_copy4(scale_u + put * 8 + 4, p.scales + v_tiles + tile);
+          async_arrive(bar);
         } else {
           set_error(p.status, CDB_ERR_INDEX);
-          mbar_arrive(&s_bar[warp][st]);
+          s_scale[warp][put][0] = -1.f;
+          mbar_arrive(&s_bar[warp][put]);
+          mbar_arrive(&s_bar[warp][put]);
         }
       }
-      ++issued;
-      if (issued < count) advance(p, ahead, vheads);
+      put = put + 1 == p.stages ? 0 : put + 1;
+      if (++issued < count) advance(p, ahead);
     };
     for (int i = 0; i < p.stages && issued < count; ++i) issue();
 
-    Running<D> r;
+    Running<D, HN> r;
     uint32_t qf[Shape<D>::KS][2];
-    float factor[2];
-    int first = c.page, seg_row = -1, seg_vh = -1;
-    int own_row = -1, own_first = 0, own_id = -1;
+    float factor[HN];
+    int first = 0, get = 0;
+    uint32_t phase = 0;
+    bool fresh = true;
     for (int i = 0; i < count; ++i) {
-      if (c.row != seg_row || c.vh != seg_vh) {
-        seg_row = c.row;
-        seg_vh = c.vh;
+      if (fresh) {
         first = c.page;
-        load_q<D>(p, c.row, c.vh, qf, factor);
+        load_q<D, HN>(p, c, qf, factor);
         r.clear();
       }
-      const int wf = c.page & ~31;
-      if (c.row != own_row || wf != own_first) {
-        own_row = c.row;
-        own_first = wf;
-        own_id = wf + lane < c.pages ? p.block_table[(int64_t)c.slot * p.bt_stride + wf + lane] : -1;
+      if (!__all_sync(kFull, mbar_wait(&s_bar[warp][get], phase, p.status))) {
+        for (int j = i + 1; j < issued; ++j) {  // a copy that never came: the error is recorded; wait for the others
+          get = get + 1 == p.stages ? (phase ^= 1u, 0) : get + 1;
+          mbar_wait(&s_bar[warp][get], phase, p.status);
+        }
+        break;
       }
-      const int blk = __shfl_sync(kFull, own_id, c.page & 31);
-      const int st = i % p.stages;
-      const bool known = blk >= 0 && blk < p.num_blocks;
-      float sk = 0.f, sv = 1.f;
-      if (known) {
-        const int64_t tile = (int64_t)blk * p.kv_heads + c.vh / p.groups;
-        sk = p.scales[tile];
-        sv = p.scales[v_tiles + tile];
-      }
-      if (!__all_sync(kFull, mbar_wait(&s_bar[warp][st], (i / p.stages) & 1, p.status))) {
-        for (int j = i + 1; j < issued; ++j) mbar_wait(&s_bar[warp][j % p.stages], (j / p.stages) & 1, p.status);
-        break;  // a copy that never came: the error is recorded, the copies in flight have been waited for
-      }
-      if (known) {
+      const float2 sc = *reinterpret_cast<const float2*>(&s_scale[warp][get][0]);
+      if (sc.x >= 0.f) {
         const int live = c.page + 1 == c.pages ? (c.pos & (kBlock - 1)) + 1 : kBlock;
-        page_step<D>(ring + st * 2 * TILE, ring + st * 2 * TILE + TILE, sk, sv, live, qf, factor, r);
+        const uint8_t* at = ring + get * 2 * TILE;
+        page_step<D, HN>(at, at + TILE, sc.x, sc.y, live, qf, factor, r);
       }
+      get = get + 1 == p.stages ? (phase ^= 1u, 0) : get + 1;
       __syncwarp();
       if (issued < count) issue();
       const bool seg_end = c.page + 1 == c.pages;
+      fresh = seg_end;
       if (seg_end || i + 1 == count) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < HN; ++h) {
           r.l[h] += __shfl_xor_sync(kFull, r.l[h], 4);
           r.l[h] += __shfl_xor_sync(kFull, r.l[h], 8);
           r.l[h] += __shfl_xor_sync(kFull, r.l[h], 16);
         }
         if (seg_end && first == 0) {
-          write_out<D>(p, c.row, c.vh, r);
+          write_out<D, HN>(p, c, r);
         } else {
           const int slot = first == 0 ? 1 : 0;  // a piece that begins its segment is this warp's last
-          store_piece<D>(s_piece + (warp * 2 + slot) * piece_floats, p.stored_heads, r);
+          store_piece<D, HN>(piece[slot], p.stored_heads, r);
           if (lane == 0) {
             PieceTag tag;
-            tag.row = c.row, tag.vh = c.vh, tag.first = first, tag.last = c.page + 1, tag.pages = c.pages;
+            tag.row = c.row, tag.kvh = c.kvh, tag.grp = c.grp;
+            tag.first = first, tag.last = c.page + 1, tag.pages = c.pages;
             s_tag[warp][slot] = tag;
           }
         }
       }
-      if (i + 1 < count) advance(p, c, vheads);
+      if (i + 1 < count) advance(p, c);
     }
   }
   __syncthreads();
@@ -458,32 +539,37 @@ __global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const DecodePara
     bool leads = true;
     for (int j = 0; j < warp * 2 + slot; ++j) {
       const PieceTag& o = s_tag[j >> 1][j & 1];
-      leads = leads && !(o.row == lead.row && o.vh == lead.vh);
+      leads = leads && !(o.row == lead.row && o.kvh == lead.kvh && o.grp == lead.grp);
     }
     if (!leads) continue;
     int last = lead.last;
     unsigned members = 0;  // bit j: piece j belongs here
     for (int j = warp * 2 + slot; j < kWarps * 2; ++j) {
       const PieceTag& o = s_tag[j >> 1][j & 1];
-      if (o.row == lead.row && o.vh == lead.vh) {
+      if (o.row == lead.row && o.kvh == lead.kvh && o.grp == lead.grp) {
         members |= 1u << j;
         last = o.last;
       }
     }
     const bool whole = lead.first == 0 && last == lead.pages;
-    const int kvh = lead.vh / p.groups, grp = lead.vh - kvh * p.groups;
+    const int kvh = lead.kvh, grp = lead.grp;
     const int heads = min(kGroup, p.heads_per_kv - grp * kGroup);
+    // piece j of the CTA
+    auto at = [&](int j) {
+      return j & 1 ? reinterpret_cast<const float*>(smem + (size_t)(j >> 1) * p.stages * 2 * TILE)
+                   : reinterpret_cast<const float*>(smem + (size_t)kWarps * p.stages * 2 * TILE) + (j >> 1) * piece_floats;
+    };
     // stream places of the segment, to know the CTAs that share it
     const int pslot = lead.first > 0 ? 0 : 1;
     float* mine = p.parts + ((int64_t)blockIdx.x * 2 + pslot) * piece_floats;
     for (int h = 0; h < heads; ++h) {
       float m = -INFINITY;
-      for (unsigned b = members; b; b &= b - 1) m = fmaxf(m, s_piece[(__ffs(b) - 1) * piece_floats + h * (D + 2) + D]);
+      for (unsigned b = members; b; b &= b - 1) m = fmaxf(m, at(__ffs(b) - 1)[h * (D + 2) + D]);
       float l = 0.f, o[D / 32];
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
       for (unsigned b = members; b; b &= b - 1) {
-        const float* src = s_piece + (__ffs(b) - 1) * piece_floats + h * (D + 2);
+        const float* src = at(__ffs(b) - 1) + h * (D + 2);
         const float f = src[D] == -INFINITY ? 0.f : ex2(src[D] - m);
         l += src[D + 1] * f;
 #pragma unroll
@@ -512,7 +598,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const DecodePara
       bool bad = false;
       before += row_pages(p, b, bad);
     }
-    const int64_t seg0 = before * vheads + (int64_t)lead.vh * lead.pages;
+    const int64_t seg0 = before * vheads + (int64_t)(kvh * p.groups + grp) * lead.pages;
     const int c0 = (int)(seg0 / share), c1 = (int)((seg0 + lead.pages - 1) / share);
     __threadfence();
     __syncwarp();
@@ -546,18 +632,47 @@ __global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const DecodePara
   }
 }
 
-constexpr int kSmemLimit = 113 * 1024;  // two CTAs share an SM's 228 KB
+constexpr int kSmemLimit = 108 * 1024;  // dynamic: two CTAs, with their static 5 KB each, share an SM's 228 KB
 
-template <int D>
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult st;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &st) != cudaSuccess ||
+        st != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<EncodeFn>(ptr);
+  }();
+  return fn;
+}
+
+template <int D, int HN>
 static int launch_decode(DecodeParams p, int num_ctas, cudaStream_t st) {
-  const int pieces = kWarps * 2 * p.stored_heads * (D + 2) * 4;
-  p.stages = 4;
-  while (p.stages > 2 && kWarps * p.stages * 2 * Shape<D>::TILE + pieces > kSmemLimit - 4096) --p.stages;
-  const int smem = kWarps * p.stages * 2 * Shape<D>::TILE + pieces;
-  if (cudaFuncSetAttribute(decode_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+  CUtensorMap map = {};
+  if (Shape<D>::SWIZZLED) {  // this layer's tiles, K then V, as rows of D bytes
+    EncodeFn encode = encode_fn();
+    const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)2 * p.num_blocks * p.kv_heads * kBlock};
+    const cuuint64_t strides[1] = {(cuuint64_t)D};
+    const cuuint32_t box[2] = {(cuuint32_t)D, (cuuint32_t)kBlock}, ones[2] = {1, 1};
+    if (encode == nullptr ||
+        encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(p.codes), dims, strides, box, ones,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return CDB_ERR_TMA_ENCODE;
+  }
+  const int pieces = kWarps * p.stored_heads * (D + 2) * 4;
+  p.stages = kMaxStages;
+  while (p.stages > 2 && 1024 + kWarps * p.stages * 2 * Shape<D>::TILE + pieces > kSmemLimit) --p.stages;
+  const int smem = 1024 + kWarps * p.stages * 2 * Shape<D>::TILE + pieces;
+  auto kernel = decode_kernel<D, HN>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return CDB_ERR_CUDA;
-  launch_pdl(decode_kernel<D>, dim3(num_ctas), dim3(kWarps * 32), smem, st, p);
-  return cudaPeekAtLastError() == cudaSuccess ? CDB_OK : CDB_ERR_CUDA;
+  return launch_pdl(kernel, dim3(num_ctas), dim3(kWarps * 32), smem, st, map, p) == cudaSuccess ? CDB_OK
+                                                                                                : CDB_ERR_CUDA;
 }
 
 }  // namespace kv8
@@ -581,6 +696,7 @@ extern "C" int cdb_kv8_decode_attention(const void* q, int64_t q_stride, void* o
       cache_layer >= num_cache_layers || num_blocks <= 0 || num_items < 0 || num_kv_heads <= 0 || num_heads <= 0 ||
       num_heads % num_kv_heads != 0 || table_rows < 0 || table_width < 0 || num_ctas <= 0)
     return CDB_ERR_INVALID_ARGUMENT;
+  if ((int64_t)num_blocks * num_kv_heads * 2 * kBlock > 0x7fffffff) return CDB_ERR_UNSUPPORTED;  // tile rows are int32
   if (head_dim != 64 && head_dim != 96 && head_dim != 128) return CDB_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(q) & 15) || (q_stride & 7) || (reinterpret_cast<uintptr_t>(out) & 15) ||
       (out_stride & 7))
@@ -617,7 +733,12 @@ extern "C" int cdb_kv8_decode_attention(const void* q, int64_t q_stride, void* o
   p.counters = counters;
   p.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128) return launch_decode<128>(p, num_ctas, st);
-  if (head_dim == 96) return launch_decode<96>(p, num_ctas, st);
-  return launch_decode<64>(p, num_ctas, st);
+  if (p.heads_per_kv == 1) {
+    if (head_dim == 128) return launch_decode<128, 1>(p, num_ctas, st);
+    if (head_dim == 96) return launch_decode<96, 1>(p, num_ctas, st);
+    return launch_decode<64, 1>(p, num_ctas, st);
+  }
+  if (head_dim == 128) return launch_decode<128, 2>(p, num_ctas, st);
+  if (head_dim == 96) return launch_decode<96, 2>(p, num_ctas, st);
+  return launch_decode<64, 2>(p, num_ctas, st);
 }
