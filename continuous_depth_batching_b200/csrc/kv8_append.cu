@@ -104,17 +104,17 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a <= 3.402823466e38f ? a : 0.f;  // infinities saturate and NaN stays NaN, under the others' scale
 }
 
-// q: a warp rotates HB heads of RPI rows, with the rows' angles in registers and the heads' loads in
+// q: a warp rotates HB heads of RPI rows (those before `end`), with the rows' angles in registers and the heads' loads in
 // flight together.
 constexpr int HB = 4;
 
 template <int D>
-__device__ __forceinline__ void rotate_q(const AppendParams& p, int row0, int head0) {
+__device__ __forceinline__ void rotate_q(const AppendParams& p, int row0, int end, int head0) {
   constexpr int LPR = D / 8, RPI = 32 / LPR;
   const int lane = threadIdx.x & 31;
   const int sub = lane / LPR, x0 = (lane % LPR) * 8;
   const int r = row0 + sub;
-  const int pos = sub < RPI && r < p.num_items ? p.item_pos[r] : -1;
+  const int pos = sub < RPI && r < end ? p.item_pos[r] : -1;
   const bool on = pos >= 0 && (p.rope_mode == 0 || pos < p.rope_rows);
   const Angles a = load_angles<D>(p, p.rope_mode, pos, x0, on);
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) append_kernel(const Appe
   for (int task = blockIdx.y * 8 + warp; task < tasks; task += gridDim.y * 8) {
     if (task < q_tasks) {
       const int i = task / q_heads, h = task - i * q_heads;
-      rotate_q<D>(p, row0 + i * RPI, h * HB);
+      rotate_q<D>(p, row0 + i * RPI, row0 + rows, h * HB);
       continue;
     }
     const int kt = task - q_tasks;
