@@ -1,11 +1,13 @@
 // Decode attention over the 8-bit paged cache (layout in kv8.cuh): one query row per item, any
 // number of query heads per kv head.
 //
-// Work. The pages of all (row, kv head, group of up to 8 query heads) segments, in that order, form
-// one stream that is cut into equal shares, one per CTA, and each share into eight, one per warp: a
-// long row is spread over the whole GPU and short rows are packed, by the positions that lie on the
-// device. Each warp streams its pages through a ring of its own in shared memory (a page is two
-// contiguous tiles, K and V, one bulk copy each), so no warp waits for another until its share ends.
+// Work. The pages (blocks) of all (row, kv head, group of up to 8 query heads) segments, in that order
+// and in pairs, form one stream that is cut into equal shares, one per CTA, and each share into one per
+// warp: a long row is spread over the whole GPU and short rows are packed, by the positions that lie on
+// the device. Each warp streams its pairs of pages through a ring of its own in shared memory (a page is
+// two contiguous tiles, K and V, one copy each), so no warp waits for another until its share ends. Pairs,
+// because a page alone leaves the warp with one chain of dependent products and pays for the loop, the
+// copies' bookkeeping and the softmax's vote by itself.
 //
 // Mathematics. Per page, with K the 16 x D tile of codes: S = K q (tensor cores, f16 operands, fp32
 // accumulators). Codes convert to f16 exactly, and q is divided by a power of two that brings its
@@ -26,7 +28,8 @@
 namespace cdb {
 namespace kv8 {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 12;
+constexpr int kThreads = kWarps * 32;
 constexpr int kMaxStages = 4;
 constexpr int kGroup = 8;  // query heads of one segment (the n of an m16n8k16 product)
 constexpr uint32_t kFull = 0xffffffffu;
@@ -46,41 +49,42 @@ struct DecodeParams {
   const int32_t* item_pos;
   int num_items;
   float scale_log2;
-  int min_share;     // pages of one CTA's share, at least
-  int stages;        // pages of a warp's ring
+  int min_share;     // pairs of one CTA's share, at least
+  int stages;        // pairs in a warp's ring
   int stored_heads;  // heads of a stored piece: min(heads_per_kv, kGroup)
-  float* parts;      // [CTAs][2][stored_heads][D + 2]
+  float* parts;      // [CTAs][2][stored_heads][D + 2], then, unless they fit shared memory, each CTA's
+  float* first;      // [CTAs][kWarps][stored_heads][D + 2] first pieces of the warps; null: shared memory
   int32_t* counters;
   int32_t* status;
 };
 
-// Cached pages of row b; 0 for a padding row and for one whose indexes do not fit the table.
-__device__ __forceinline__ int row_pages(const DecodeParams& p, int b, bool& bad) {
+// Pairs of cached pages of row b; 0 for a padding row and for one whose indexes do not fit the table.
+__device__ __forceinline__ int row_pairs(const DecodeParams& p, int b, bool& bad) {
   const int pos = p.item_pos[b], slot = p.item_slot[b];
   if (pos < 0) return 0;
   if (slot < 0 || slot >= p.bt_rows || pos / kBlock >= p.bt_width) {
     bad = true;
     return 0;
   }
-  return pos / kBlock + 1;
+  return pos / (2 * kBlock) + 1;
 }
 
-// A place in the page stream: page `page` of row `row`, query-head group `grp` of kv head `kvh`.
+// A place in the stream: pair `pair` of row `row`, query-head group `grp` of kv head `kvh`.
 struct Cursor {
-  int row, kvh, grp, page, pages, pos, slot;
+  int row, kvh, grp, pair, pairs, pos, slot;
 };
 
 __device__ __forceinline__ void load_row(const DecodeParams& p, Cursor& c) {
   bool bad = false;
-  c.pages = row_pages(p, c.row, bad);
+  c.pairs = row_pairs(p, c.row, bad);
   c.pos = p.item_pos[c.row];
   c.slot = p.item_slot[c.row];
 }
 
-// To the next page.
+// To the next pair.
 __device__ __forceinline__ void advance(const DecodeParams& p, Cursor& c) {
-  if (++c.page < c.pages) return;
-  c.page = 0;
+  if (++c.pair < c.pairs) return;
+  c.pair = 0;
   if (++c.grp < p.groups) return;
   c.grp = 0;
   if (++c.kvh < p.kv_heads) return;
@@ -88,7 +92,7 @@ __device__ __forceinline__ void advance(const DecodeParams& p, Cursor& c) {
   do {
     if (++c.row >= p.num_items) return;  // the stream's end
     load_row(p, c);
-  } while (c.pages == 0);
+  } while (c.pairs == 0);
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -122,7 +126,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
 // Where a piece lies in its segment, for the joins.
 struct PieceTag {
   int row, kvh, grp;
-  int first, last, pages;  // pages [first, last) of `pages`
+  int first, last, pairs;  // pairs [first, last) of `pairs`
 };
 
 template <int D>
@@ -197,14 +201,11 @@ __device__ __forceinline__ void load_q(const DecodeParams& p, const Cursor& c, u
   for (int h = 0; h < HN; ++h) factor[h] = __shfl_sync(kFull, f, t * 8 + h * 4);  // the lanes of head 2t + h
 }
 
-// One page: `live` tokens of it count.
-template <int D, int HN>
-__device__ __forceinline__ void page_step(const uint8_t* k, const uint8_t* v, float sk, float sv, int live,
-                                          const uint32_t (&qf)[Shape<D>::KS][2], const float (&factor)[HN],
-                                          Running<D, HN>& r) {
-  constexpr int KD = Shape<D>::KD, VD = Shape<D>::VD;
+// The fragments of one page's K: rows g and g + 8, dims [t * KD, (t + 1) * KD).
+template <int D>
+__device__ __forceinline__ void load_k(const uint8_t* k, uint32_t (&ka)[D / 16], uint32_t (&kb)[D / 16]) {
+  constexpr int KD = Shape<D>::KD;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint32_t ka[KD / 4], kb[KD / 4];
   if constexpr (KD % 16 == 0) {
 #pragma unroll
     for (int i = 0; i < KD / 16; ++i) {
@@ -221,8 +222,13 @@ __device__ __forceinline__ void page_step(const uint8_t* k, const uint8_t* v, fl
       ka[2 * i] = x.x, ka[2 * i + 1] = x.y, kb[2 * i] = y.x, kb[2 * i + 1] = y.y;
     }
   }
-  // V: tokens 2t, 2t + 1, 2t + 8, 2t + 9, dims [g * VD, (g + 1) * VD)
-  uint32_t vw[4][VD / 4];
+}
+
+// The fragments of one page's V: tokens 2t, 2t + 1, 2t + 8, 2t + 9, dims [g * VD, (g + 1) * VD).
+template <int D>
+__device__ __forceinline__ void load_v(const uint8_t* v, uint32_t (&vw)[4][D / 32]) {
+  constexpr int VD = Shape<D>::VD;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int tok = 2 * t + (j & 1) + 8 * (j >> 1);
@@ -237,49 +243,79 @@ __device__ __forceinline__ void page_step(const uint8_t* k, const uint8_t* v, fl
       for (int i = 0; i < VD / 4; ++i) vw[j][i] = *reinterpret_cast<const uint32_t*>(v + tok * D + g * VD + i * 4);
     }
   }
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
+}
+
+// One pair of pages at `at` (K, V of the first, K, V of the second). scale: K's and V's of the first, then
+// of the second; K's < 0 where the page does not exist. `live` tokens of the pair count.
+template <int D, int HN>
+__device__ __forceinline__ void pair_step(const uint8_t* at, const float4 scale, int live,
+                                          const uint32_t (&qf)[Shape<D>::KS][2], const float (&factor)[HN],
+                                          Running<D, HN>& r) {
+  constexpr int KD = Shape<D>::KD, VD = Shape<D>::VD, TILE = Shape<D>::TILE;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float s[2][4];
 #pragma unroll
-  for (int i = 0; i < KD / 4; ++i)
-    mma_f16(s, cvt_e4m3x2_f16x2(ka[i] & 0xffffu), cvt_e4m3x2_f16x2(kb[i] & 0xffffu), cvt_e4m3x2_f16x2(ka[i] >> 16),
-            cvt_e4m3x2_f16x2(kb[i] >> 16), qf[i][0], qf[i][1]);
-  // s[h]: token g, head 2t + h; s[2 + h]: token g + 8
-  const float ev = sv > 0.f ? __log2f(sv) : -126.f;
-  float x[HN][2];
-  bool up = false;
+  for (int pg = 0; pg < 2; ++pg) {
+    uint32_t ka[KD / 4], kb[KD / 4];
+    load_k<D>(at + pg * 2 * TILE, ka, kb);
+    s[pg][0] = s[pg][1] = s[pg][2] = s[pg][3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < KD / 4; ++i)
+      mma_f16(s[pg], cvt_e4m3x2_f16x2(ka[i] & 0xffffu), cvt_e4m3x2_f16x2(kb[i] & 0xffffu),
+              cvt_e4m3x2_f16x2(ka[i] >> 16), cvt_e4m3x2_f16x2(kb[i] >> 16), qf[i][0], qf[i][1]);
+  }
+  uint32_t vw[2][4][VD / 4];
+  load_v<D>(at + TILE, vw[0]);
+  load_v<D>(at + 3 * TILE, vw[1]);
+  // s[pg][h]: token g, head 2t + h; s[pg][2 + h]: token g + 8
+  const float ks[2] = {scale.x, scale.z};
+  const float ev[2] = {scale.y > 0.f ? __log2f(scale.y) : -126.f, scale.w > 0.f ? __log2f(scale.w) : -126.f};
+  float x[HN][4];
 #pragma unroll
   for (int h = 0; h < HN; ++h) {
-    const float f = factor[h] * sk;
-    x[h][0] = s[h] * f;
-    x[h][1] = s[2 + h] * f;
-  }
-  if (live < kBlock) {
 #pragma unroll
-    for (int h = 0; h < HN; ++h) {
-      if (g >= live) x[h][0] = -INFINITY;
-      if (g + 8 >= live) x[h][1] = -INFINITY;
+    for (int pg = 0; pg < 2; ++pg) {
+      const float f = factor[h] * ks[pg];
+      x[h][2 * pg] = s[pg][h] * f;
+      x[h][2 * pg + 1] = s[pg][2 + h] * f;
     }
+  }
+  if (live < 2 * kBlock || ks[0] < 0.f || ks[1] < 0.f) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {  // codes behind the row's end may be anything, NaN too
-      if (2 * t + (j & 1) + 8 * (j >> 1) >= live) {
+    for (int pg = 0; pg < 2; ++pg) {
+      const int end = ks[pg] < 0.f ? 0 : live - pg * kBlock;
 #pragma unroll
-        for (int i = 0; i < VD / 4; ++i) vw[j][i] = 0u;
+      for (int h = 0; h < HN; ++h) {
+        if (g >= end) x[h][2 * pg] = -INFINITY;
+        if (g + 8 >= end) x[h][2 * pg + 1] = -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // codes behind the row's end may be anything, NaN too
+        if (2 * t + (j & 1) + 8 * (j >> 1) >= end) {
+#pragma unroll
+          for (int i = 0; i < VD / 4; ++i) vw[pg][j][i] = 0u;
+        }
       }
     }
   }
+  // m and M only move when a logit passes them by 8 (the weights stay within 2^8): a vote a pair
+  bool up = false;
 #pragma unroll
   for (int h = 0; h < HN; ++h) {
-    const float mx = fmaxf(x[h][0], x[h][1]);
-    up = up || mx > r.m[h] + 8.f || mx + ev > r.mw[h] + 8.f;
+    const float a = fmaxf(x[h][0], x[h][1]), b = fmaxf(x[h][2], x[h][3]);
+    up = up || fmaxf(a, b) > r.m[h] + 8.f || fmaxf(a + ev[0], b + ev[1]) > r.mw[h] + 8.f;
   }
-  // m and M only move when a logit passes them by 8 (the weights stay within 2^8): a vote a page
   if (__any_sync(kFull, up)) {
 #pragma unroll
     for (int h = 0; h < HN; ++h) {
-      float mx = fmaxf(x[h][0], x[h][1]);
-      mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
-      mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
-      mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
-      const float m = fmaxf(r.m[h], mx), mw = fmaxf(r.mw[h], mx + ev);
+      const float a = fmaxf(x[h][0], x[h][1]), b = fmaxf(x[h][2], x[h][3]);
+      float mx = fmaxf(a, b), mz = fmaxf(a + ev[0], b + ev[1]);
+#pragma unroll
+      for (int d = 4; d <= 16; d <<= 1) {
+        mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, d));
+        mz = fmaxf(mz, __shfl_xor_sync(kFull, mz, d));
+      }
+      const float m = fmaxf(r.m[h], mx), mw = fmaxf(r.mw[h], mz);
       r.l[h] *= m == -INFINITY ? 1.f : ex2(r.m[h] - m);
       const float down = mw == -INFINITY ? 1.f : ex2(r.mw[h] - mw);
       r.m[h] = m;
@@ -288,26 +324,32 @@ __device__ __forceinline__ void page_step(const uint8_t* k, const uint8_t* v, fl
       for (int i = 0; i < Shape<D>::MT; ++i) r.acc[i][h] *= down, r.acc[i][2 + h] *= down;
     }
   }
-  float pw[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+  float pw[4][2];
 #pragma unroll
-  for (int h = 0; h < HN; ++h) {
+  for (int j = 0; j < 4; ++j) {
+    pw[j][1] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int h = 0; h < HN; ++h) {
       const bool off = x[h][j] == -INFINITY;  // also where m is still -inf
       r.l[h] += off ? 0.f : ex2(x[h][j] - r.m[h]);
-      pw[j][h] = off ? 0.f : ex2(x[h][j] + ev - r.mw[h]);
+      pw[j][h] = off ? 0.f : ex2(x[h][j] + ev[j >> 1] - r.mw[h]);
     }
   }
-  const uint32_t b0 = transpose8(pack_f16x2(pw[0][0], pw[0][1]));
-  const uint32_t b1 = transpose8(pack_f16x2(pw[1][0], pw[1][1]));
 #pragma unroll
-  for (int i = 0; i < VD / 4; ++i) {
-    const uint32_t lo0 = __byte_perm(vw[0][i], vw[1][i], 0x5140), hi0 = __byte_perm(vw[0][i], vw[1][i], 0x7362);
-    const uint32_t lo1 = __byte_perm(vw[2][i], vw[3][i], 0x5140), hi1 = __byte_perm(vw[2][i], vw[3][i], 0x7362);
-    mma_f16(r.acc[2 * i], cvt_e4m3x2_f16x2(lo0 & 0xffffu), cvt_e4m3x2_f16x2(lo0 >> 16),
-            cvt_e4m3x2_f16x2(lo1 & 0xffffu), cvt_e4m3x2_f16x2(lo1 >> 16), b0, b1);
-    mma_f16(r.acc[2 * i + 1], cvt_e4m3x2_f16x2(hi0 & 0xffffu), cvt_e4m3x2_f16x2(hi0 >> 16),
-            cvt_e4m3x2_f16x2(hi1 & 0xffffu), cvt_e4m3x2_f16x2(hi1 >> 16), b0, b1);
+  for (int pg = 0; pg < 2; ++pg) {
+    const uint32_t b0 = transpose8(pack_f16x2(pw[2 * pg][0], pw[2 * pg][1]));
+    const uint32_t b1 = transpose8(pack_f16x2(pw[2 * pg + 1][0], pw[2 * pg + 1][1]));
+#pragma unroll
+    for (int i = 0; i < VD / 4; ++i) {
+      const uint32_t lo0 = __byte_perm(vw[pg][0][i], vw[pg][1][i], 0x5140);
+      const uint32_t hi0 = __byte_perm(vw[pg][0][i], vw[pg][1][i], 0x7362);
+      const uint32_t lo1 = __byte_perm(vw[pg][2][i], vw[pg][3][i], 0x5140);
+      const uint32_t hi1 = __byte_perm(vw[pg][2][i], vw[pg][3][i], 0x7362);
+      mma_f16(r.acc[2 * i], cvt_e4m3x2_f16x2(lo0 & 0xffffu), cvt_e4m3x2_f16x2(lo0 >> 16),
+              cvt_e4m3x2_f16x2(lo1 & 0xffffu), cvt_e4m3x2_f16x2(lo1 >> 16), b0, b1);
+      mma_f16(r.acc[2 * i + 1], cvt_e4m3x2_f16x2(hi0 & 0xffffu), cvt_e4m3x2_f16x2(hi0 >> 16),
+              cvt_e4m3x2_f16x2(hi1 & 0xffffu), cvt_e4m3x2_f16x2(hi1 >> 16), b0, b1);
+    }
   }
 }
 
@@ -356,25 +398,30 @@ __device__ __forceinline__ void store_piece(float* dst, int heads, const Running
 }
 
 template <int D, int HN>
-__global__ void __launch_bounds__(kWarps * 32, 2)
+__global__ void __launch_bounds__(kThreads, 1)
     decode_kernel(const __grid_constant__ CUtensorMap map, const DecodeParams p) {
   pdl_trigger();
-  constexpr int TILE = Shape<D>::TILE;
+  constexpr int TILE = Shape<D>::TILE, PAIR = 4 * TILE;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ int64_t s_before[kWarps * 32 + 1];  // pages before each thread's rows
+  __shared__ int64_t s_before[kThreads + 1];  // pairs before each thread's rows
   __shared__ int64_t s_warp[kWarps];
   __shared__ PieceTag s_tag[kWarps][2];
   __shared__ __align__(8) uint64_t s_bar[kWarps][kMaxStages];
-  __shared__ __align__(8) float s_scale[kWarps][kMaxStages][2];  // K's and V's of a page; K's < 0: no such block
+  __shared__ __align__(16) float s_scale[kWarps][kMaxStages][4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int vheads = p.kv_heads * p.groups;
   const int piece_floats = p.stored_heads * (D + 2);
-  uint8_t* ring = smem + (size_t)warp * p.stages * 2 * TILE;
-  // A piece that ends inside its segment's first page run (slot 0) has a place of its own, one that ends
-  // the warp's share (slot 1) lies over the ring, which is empty by then.
-  float* piece[2] = {reinterpret_cast<float*>(smem + (size_t)kWarps * p.stages * 2 * TILE) + warp * piece_floats,
-                     reinterpret_cast<float*>(ring)};
+  const int ring_bytes = p.stages * PAIR;
+  uint8_t* ring = smem + (size_t)warp * ring_bytes;
+  // Places of the CTA's pieces. A piece that ends inside its segment's share (slot 0) has one of its own, in
+  // shared memory or in the workspace; one that ends the warp's share (slot 1) lies over the warp's ring,
+  // which is empty by then.
+  float* first_pieces = p.first != nullptr ? p.first + (int64_t)blockIdx.x * kWarps * piece_floats
+                                           : reinterpret_cast<float*>(smem + (size_t)kWarps * ring_bytes);
+  auto place = [&](int w, int slot) {
+    return slot ? reinterpret_cast<float*>(smem + (size_t)w * ring_bytes) : first_pieces + w * piece_floats;
+  };
   if (lane == 0) {
     for (int i = 0; i < p.stages; ++i) mbar_init(&s_bar[warp][i], 2);
     fence_barrier_init();
@@ -382,12 +429,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   }
   pdl_wait();
 
-  // ---- the page stream: pages before every thread's rows
-  const int per = (p.num_items + kWarps * 32 - 1) / (kWarps * 32);
+  // ---- the stream: pairs before every thread's rows
+  const int per = (p.num_items + kThreads - 1) / kThreads;
   {
     int64_t mine = 0;
     bool bad = false;
-    for (int b = threadIdx.x * per; b < min(p.num_items, (int)(threadIdx.x + 1) * per); ++b) mine += row_pages(p, b, bad);
+    for (int b = threadIdx.x * per; b < min(p.num_items, (int)(threadIdx.x + 1) * per); ++b) mine += row_pairs(p, b, bad);
     if (bad && blockIdx.x == 0) set_error(p.status, CDB_ERR_INDEX);
     int64_t x = mine;
 #pragma unroll
@@ -398,27 +445,28 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     if (lane == 31) s_warp[warp] = x;
     __syncthreads();
     int64_t base = 0, all = 0;
+#pragma unroll
     for (int i = 0; i < kWarps; ++i) {
       if (i < warp) base += s_warp[i];
       all += s_warp[i];
     }
     s_before[threadIdx.x] = base + x - mine;
-    if (threadIdx.x == 0) s_before[kWarps * 32] = all;
+    if (threadIdx.x == 0) s_before[kThreads] = all;
     __syncthreads();
   }
-  const int64_t total = s_before[kWarps * 32] * vheads;
+  const int64_t total = s_before[kThreads] * vheads;
   const int64_t even = (total + gridDim.x - 1) / gridDim.x;
   const int64_t share = even > p.min_share ? even : p.min_share;
   const int64_t begin = share * blockIdx.x, end = begin + share < total ? begin + share : total;
+  if (begin >= end) return;  // uniform over the CTA
   const int64_t wshare = (end - begin + kWarps - 1) / kWarps;
   const int64_t wbegin = begin + wshare * warp;
-  const int count = (int)((wbegin + wshare < end ? wbegin + wshare : end) - wbegin);  // this warp's pages, if > 0
-  if (begin >= end) return;  // uniform over the CTA
+  const int count = (int)((wbegin + wshare < end ? wbegin + wshare : end) - wbegin);  // this warp's pairs, if > 0
 
   if (count > 0) {
-    // the row that holds page wbegin
+    // the row that holds pair wbegin
     Cursor c;
-    int lo = 0, hi = kWarps * 32;
+    int lo = 0, hi = kThreads;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (s_before[mid] * vheads <= wbegin) lo = mid; else hi = mid;
@@ -426,13 +474,13 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     int64_t at = wbegin - s_before[lo] * vheads;
     c.row = lo * per;
     load_row(p, c);
-    while (at >= (int64_t)c.pages * vheads) {
-      at -= (int64_t)c.pages * vheads;
+    while (at >= (int64_t)c.pairs * vheads) {
+      at -= (int64_t)c.pairs * vheads;
       ++c.row;
       load_row(p, c);
     }
-    const int vh = (int)(at / c.pages);
-    c.page = (int)(at - (int64_t)vh * c.pages);
+    const int vh = (int)(at / c.pairs);
+    c.pair = (int)(at - (int64_t)vh * c.pairs);
     c.kvh = vh / p.groups;
     c.grp = vh - c.kvh * p.groups;
 
@@ -440,38 +488,42 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     const uint32_t ring_u = smem_u32(ring), bar_u = smem_u32(&s_bar[warp][0]), scale_u = smem_u32(&s_scale[warp][0][0]);
     Cursor ahead = c;
     int issued = 0, put = 0;
-    // Lane i holds block ids of a window of 32 pages of the issuing cursor's row.
+    // Lane i holds the block id of page i of a window of 32 pages of the issuing cursor's row.
     int win_row = -1, win_first = 0, win_id = -1;
     auto issue = [&]() {
-      const int first = ahead.page & ~31;
+      const int page = 2 * ahead.pair, first = page & ~31;
       if (ahead.row != win_row || first != win_first) {
         win_row = ahead.row;
         win_first = first;
-        win_id = first + lane < ahead.pages ? p.block_table[(int64_t)ahead.slot * p.bt_stride + first + lane] : -1;
+        win_id = first + lane <= ahead.pos / kBlock ? p.block_table[(int64_t)ahead.slot * p.bt_stride + first + lane]
+                                                     : INT32_MIN;  // behind the row's last page
       }
-      const int blk = __shfl_sync(kFull, win_id, ahead.page & 31);
+      const int id[2] = {__shfl_sync(kFull, win_id, page & 31), __shfl_sync(kFull, win_id, (page & 31) + 1)};
       if (lane == 0) {
-        if (blk >= 0 && blk < p.num_blocks) {
-          const int tile = blk * p.kv_heads + ahead.kvh;
-          const uint32_t bar = bar_u + put * 8, dst = ring_u + put * 2 * TILE;
-          mbar_arrive_expect_tx(&s_bar[warp][put], 2 * TILE);
-          if (Shape<D>::SWIZZLED) {
-            tensor_load(dst, &map, tile * kBlock, bar);
-            tensor_load(dst + TILE, &map, (v_tiles + tile) * kBlock, bar);
+        const uint32_t bar = bar_u + put * 8, dst = ring_u + put * PAIR, to = scale_u + put * 16;
+        const bool ok[2] = {id[0] >= 0 && id[0] < p.num_blocks, id[1] >= 0 && id[1] < p.num_blocks};
+        mbar_arrive_expect_tx(&s_bar[warp][put], (ok[0] ? 2 * TILE : 0) + (ok[1] ? 2 * TILE : 0));
+#pragma unroll
+        for (int pg = 0; pg < 2; ++pg) {
+          if (ok[pg]) {
+            const int tile = id[pg] * p.kv_heads + ahead.kvh;
+            if (Shape<D>::SWIZZLED) {
+              tensor_load(dst + pg * 2 * TILE, &map, tile * kBlock, bar);
+              tensor_load(dst + pg * 2 * TILE + TILE, &map, (v_tiles + tile) * kBlock, bar);
+            } else {
+              bulk_load(dst + pg * 2 * TILE, p.codes + (int64_t)tile * TILE, TILE, bar);
+              bulk_load(dst + pg * 2 * TILE + TILE, p.codes + (int64_t)(v_tiles + tile) * TILE, TILE, bar);
+            }
+            async_copy4(to + pg * 8, p.scales + tile);
+            async_copy4(to + pg * 8 + 4, p.scales + v_tiles + tile);
           } else {
-            bulk_load(dst, p.codes + (int64_t)tile * TILE, TILE, bar);
-            bulk_load(dst + TILE, p.codes + (int64_t)(v_tiles + tile) * TILE, TILE, bar);
+            if (id[pg] != INT32_MIN) set_error(p.status, CDB_ERR_INDEX);
+            s_scale[warp][put][2 * pg] = -1.f;
           }
-          async_copy4(scale_u + put * 8, p.scales + tile);
-          async_copy4(scale_u + put * 8 + 4, p.scales + v_tiles + tile);
-          async_arrive(bar);
-        } else {
-          set_error(p.status, CDB_ERR_INDEX);
-          s_scale[warp][put][0] = -1.f;
-          mbar_arrive(&s_bar[warp][put]);
-          mbar_arrive(&s_bar[warp][put]);
         }
+        async_arrive(bar);
       }
+      __syncwarp();  // lane 0's own stores to s_scale
       put = put + 1 == p.stages ? 0 : put + 1;
       if (++issued < count) advance(p, ahead);
     };
@@ -485,7 +537,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     bool fresh = true;
     for (int i = 0; i < count; ++i) {
       if (fresh) {
-        first = c.page;
+        first = c.pair;
         load_q<D, HN>(p, c, qf, factor);
         r.clear();
       }
@@ -496,16 +548,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         }
         break;
       }
-      const float2 sc = *reinterpret_cast<const float2*>(&s_scale[warp][get][0]);
-      if (sc.x >= 0.f) {
-        const int live = c.page + 1 == c.pages ? (c.pos & (kBlock - 1)) + 1 : kBlock;
-        const uint8_t* at = ring + get * 2 * TILE;
-        page_step<D, HN>(at, at + TILE, sc.x, sc.y, live, qf, factor, r);
-      }
+      const float4 sc = *reinterpret_cast<const float4*>(&s_scale[warp][get][0]);
+      const bool seg_end = c.pair + 1 == c.pairs;
+      pair_step<D, HN>(ring + get * PAIR, sc, seg_end ? (c.pos & (2 * kBlock - 1)) + 1 : 2 * kBlock, qf, factor, r);
       get = get + 1 == p.stages ? (phase ^= 1u, 0) : get + 1;
       __syncwarp();
       if (issued < count) issue();
-      const bool seg_end = c.page + 1 == c.pages;
       fresh = seg_end;
       if (seg_end || i + 1 == count) {
 #pragma unroll
@@ -518,11 +566,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
           write_out<D, HN>(p, c, r);
         } else {
           const int slot = first == 0 ? 1 : 0;  // a piece that begins its segment is this warp's last
-          store_piece<D, HN>(piece[slot], p.stored_heads, r);
+          store_piece<D, HN>(place(warp, slot), p.stored_heads, r);
           if (lane == 0) {
             PieceTag tag;
             tag.row = c.row, tag.kvh = c.kvh, tag.grp = c.grp;
-            tag.first = first, tag.last = c.page + 1, tag.pages = c.pages;
+            tag.first = first, tag.last = c.pair + 1, tag.pairs = c.pairs;
             s_tag[warp][slot] = tag;
           }
         }
@@ -551,14 +599,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         last = o.last;
       }
     }
-    const bool whole = lead.first == 0 && last == lead.pages;
+    const bool whole = lead.first == 0 && last == lead.pairs;
     const int kvh = lead.kvh, grp = lead.grp;
     const int heads = min(kGroup, p.heads_per_kv - grp * kGroup);
-    // piece j of the CTA
-    auto at = [&](int j) {
-      return j & 1 ? reinterpret_cast<const float*>(smem + (size_t)(j >> 1) * p.stages * 2 * TILE)
-                   : reinterpret_cast<const float*>(smem + (size_t)kWarps * p.stages * 2 * TILE) + (j >> 1) * piece_floats;
-    };
+    auto at = [&](int j) { return place(j >> 1, j & 1); };  // piece j of the CTA
     // stream places of the segment, to know the CTAs that share it
     const int pslot = lead.first > 0 ? 0 : 1;
     float* mine = p.parts + ((int64_t)blockIdx.x * 2 + pslot) * piece_floats;
@@ -592,14 +636,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
       }
     }
     if (whole) continue;
-    // The segment's first page in the stream, from this CTA's own place in it.
+    // The segment's first pair in the stream tells which CTAs share it.
     int64_t before = s_before[lead.row / per];
     for (int b = lead.row / per * per; b < lead.row; ++b) {
       bool bad = false;
-      before += row_pages(p, b, bad);
+      before += row_pairs(p, b, bad);
     }
-    const int64_t seg0 = before * vheads + (int64_t)(kvh * p.groups + grp) * lead.pages;
-    const int c0 = (int)(seg0 / share), c1 = (int)((seg0 + lead.pages - 1) / share);
+    const int64_t seg0 = before * vheads + (int64_t)(kvh * p.groups + grp) * lead.pairs;
+    const int c0 = (int)(seg0 / share), c1 = (int)((seg0 + lead.pairs - 1) / share);
     __threadfence();
     __syncwarp();
     int arrived = 0;
@@ -632,7 +676,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   }
 }
 
-constexpr int kSmemLimit = 108 * 1024;  // dynamic: two CTAs, with their static 5 KB each, share an SM's 228 KB
+constexpr int kSmemLimit = 220 * 1024;  // dynamic, beside 5 KB of static shared memory
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -664,14 +708,18 @@ static int launch_decode(DecodeParams p, int num_ctas, cudaStream_t st) {
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return CDB_ERR_TMA_ENCODE;
   }
+  // Two pairs a warp in flight at least; first pieces that do not fit beside them go to the workspace.
+  constexpr int RING = kWarps * 4 * Shape<D>::TILE;
   const int pieces = kWarps * p.stored_heads * (D + 2) * 4;
-  p.stages = kMaxStages;
-  while (p.stages > 2 && 1024 + kWarps * p.stages * 2 * Shape<D>::TILE + pieces > kSmemLimit) --p.stages;
-  const int smem = 1024 + kWarps * p.stages * 2 * Shape<D>::TILE + pieces;
+  const bool inside = 1024 + 2 * RING + pieces <= kSmemLimit;
+  if (inside) p.first = nullptr;
+  p.stages = (kSmemLimit - 1024 - (inside ? pieces : 0)) / RING;
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  const int smem = 1024 + p.stages * RING + (inside ? pieces : 0);
   auto kernel = decode_kernel<D, HN>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return CDB_ERR_CUDA;
-  return launch_pdl(kernel, dim3(num_ctas), dim3(kWarps * 32), smem, st, map, p) == cudaSuccess ? CDB_OK
+  return launch_pdl(kernel, dim3(num_ctas), dim3(kThreads), smem, st, map, p) == cudaSuccess ? CDB_OK
                                                                                                 : CDB_ERR_CUDA;
 }
 
@@ -680,7 +728,7 @@ static int launch_decode(DecodeParams p, int num_ctas, cudaStream_t st) {
 
 extern "C" int64_t cdb_kv8_decode_workspace_floats(int num_ctas, int head_dim) {
   if (num_ctas <= 0 || head_dim <= 0) return 0;
-  return (int64_t)num_ctas * 2 * cdb::kv8::kGroup * (head_dim + 2);
+  return (int64_t)num_ctas * (2 + cdb::kv8::kWarps) * cdb::kv8::kGroup * (head_dim + 2);
 }
 
 extern "C" int cdb_kv8_decode_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride,
@@ -727,9 +775,10 @@ extern "C" int cdb_kv8_decode_attention(const void* q, int64_t q_stride, void* o
   p.item_pos = item_pos;
   p.num_items = num_items;
   p.scale_log2 = scale * kLog2e;
-  p.min_share = 8;
+  p.min_share = kWarps;
   p.stages = 0;
   p.parts = workspace;
+  p.first = workspace + (int64_t)num_ctas * 2 * p.stored_heads * (head_dim + 2);
   p.counters = counters;
   p.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

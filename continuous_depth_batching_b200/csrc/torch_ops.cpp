@@ -223,7 +223,7 @@ void kv8_decode_attention(const Tensor& q, const Tensor& out, const Tensor& code
   const auto dev = one_device(q, out, codes, scales, block_table, item_slot, item_pos);
   const c10::cuda::CUDAGuard guard(dev);
   const auto stream = c10::cuda::getCurrentCUDAStream(dev.index());
-  const int ctas = 2 * sm_count(dev);
+  const int ctas = sm_count(dev);
   const Tensor& status = status_word(dev);
   const auto [ws, counters] = decode_workspace(dev, stream, ctas, c.dim);
   check(cdb_kv8_decode_attention(ptr<void>(q), q.stride(0), ptr<void>(out), out.stride(0), ptr<void>(codes),

@@ -505,7 +505,7 @@ int64_t cdb_kv8_decode_workspace_floats(int num_ctas, int head_dim);
  *   q, out     bf16 rows of num_heads * head_dim, q rotated; 16-byte aligned, strides multiples
  *              of 8. num_heads is a multiple of num_kv_heads; head h reads kv head
  *              h / (num_heads / num_kv_heads).
- *   num_ctas   CTAs to launch (two fit an SM); workspace: cdb_kv8_decode_workspace_floats of it;
+ *   num_ctas   CTAs to launch (one fits an SM); workspace: cdb_kv8_decode_workspace_floats of it;
  *              counters [num_ctas] int32, zeroed before the first use, left zeroed. Calls that
  *              share them must be ordered. */
 int cdb_kv8_decode_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* codes,

@@ -195,4 +195,4 @@ def test_c_abi_refuses_on_the_host():
                                some, some, some, 1, None, 0, None, None) == unsupported
     assert lib.cdb_step_tables(some, some, some, some, 1, some, 5, 3, 5, None, 9, some, some, some, some, some, some,
                                some, some, some, 1, None, 0, None, None) == inval
-    assert lib.cdb_kv8_decode_workspace_floats(296, 128) == 296 * 2 * 8 * 130
+    assert lib.cdb_kv8_decode_workspace_floats(148, 128) >= 148 * 2 * 8 * 130
