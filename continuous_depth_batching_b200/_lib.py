@@ -146,6 +146,7 @@ _SIGNATURES: dict[str, list] = {
         c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
     ],
     "cdb_kv8_decode_workspace_floats": [c_int, c_int],
+    "cdb_kv8_decode_counters": [c_int],
     "cdb_kv8_decode_attention": [
         c_void_p, c_int64, c_void_p, c_int64,  # q, stride, out, stride
         c_void_p, c_void_p, c_int, c_int, c_int,  # codes, scales, num_cache_layers, cache_layer, num_blocks
@@ -245,7 +246,7 @@ def stream_ptr(stream: torch.cuda.Stream | None = None) -> int:
 
 _NO_LAUNCH = {
     "cdb_version", "cdb_status_string", "cdb_attn_scratch_bytes", "cdb_gemm_workspace_elems", "cdb_gemm_counter_elems",
-    "cdb_gemm_partial_splits", "cdb_kv8_decode_workspace_floats",
+    "cdb_gemm_partial_splits", "cdb_kv8_decode_workspace_floats", "cdb_kv8_decode_counters",
     "cdb_schedule_queues_init",
     "cdb_kv_blocks_host_copy",
 }

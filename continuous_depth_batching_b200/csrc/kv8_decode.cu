@@ -19,8 +19,8 @@
 // keys) whatever the blocks' scales are. O = V^T P (tensor cores again) in fp32.
 //
 // Pieces of a segment (m, l, o) meet in two steps: the warps of a CTA through shared memory, CTAs
-// through the workspace, where the last one to arrive adds them up in CTA order. The result does not
-// depend on which one that is.
+// through the workspace, where the last one to arrive adds them up in CTA order, head by head. The result
+// does not depend on which one that is.
 #include <cuda.h>
 
 #include "kv8.cuh"
@@ -580,96 +580,96 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
 
-  // ---- join the pieces: warp w leads those segments whose first piece of this CTA is its own
-  for (int slot = 0; slot < 2; ++slot) {
-    const PieceTag lead = s_tag[warp][slot];
-    if (lead.row < 0) continue;
-    bool leads = true;
-    for (int j = 0; j < warp * 2 + slot; ++j) {
-      const PieceTag& o = s_tag[j >> 1][j & 1];
-      leads = leads && !(o.row == lead.row && o.kvh == lead.kvh && o.grp == lead.grp);
-    }
-    if (!leads) continue;
-    int last = lead.last;
-    unsigned members = 0;  // bit j: piece j belongs here
-    for (int j = warp * 2 + slot; j < kWarps * 2; ++j) {
-      const PieceTag& o = s_tag[j >> 1][j & 1];
-      if (o.row == lead.row && o.kvh == lead.kvh && o.grp == lead.grp) {
-        members |= 1u << j;
-        last = o.last;
-      }
-    }
-    const bool whole = lead.first == 0 && last == lead.pairs;
-    const int kvh = lead.kvh, grp = lead.grp;
+  // ---- join the pieces. Every warp sees which pieces belong together (lane j holds the tag of piece j);
+  // the (segment, head) pairs are dealt over the warps.
+  static_assert(2 * kWarps <= 32, "a lane per piece");
+  const PieceTag tag = s_tag[lane < 2 * kWarps ? lane >> 1 : 0][lane & 1];
+  const bool used = lane < 2 * kWarps && tag.row >= 0;
+  const int64_t key = used ? ((int64_t)tag.row * p.kv_heads + tag.kvh) * p.groups + tag.grp : -1 - lane;
+  const unsigned group = __match_any_sync(kFull, key);
+  unsigned leaders = __ballot_sync(kFull, used && (group & ((1u << lane) - 1u)) == 0u);
+  int task = 0;
+  for (; leaders; leaders &= leaders - 1) {
+    const int lead = __ffs(leaders) - 1;
+    const unsigned members = __shfl_sync(kFull, group, lead);
+    const int row = __shfl_sync(kFull, tag.row, lead), kvh = __shfl_sync(kFull, tag.kvh, lead);
+    const int grp = __shfl_sync(kFull, tag.grp, lead), pairs = __shfl_sync(kFull, tag.pairs, lead);
+    const int first = __shfl_sync(kFull, tag.first, lead), last = __shfl_sync(kFull, tag.last, 31 - __clz(members));
+    const bool whole = first == 0 && last == pairs;
     const int heads = min(kGroup, p.heads_per_kv - grp * kGroup);
-    auto at = [&](int j) { return place(j >> 1, j & 1); };  // piece j of the CTA
-    // stream places of the segment, to know the CTAs that share it
-    const int pslot = lead.first > 0 ? 0 : 1;
-    float* mine = p.parts + ((int64_t)blockIdx.x * 2 + pslot) * piece_floats;
-    for (int h = 0; h < heads; ++h) {
-      float m = -INFINITY;
-      for (unsigned b = members; b; b &= b - 1) m = fmaxf(m, at(__ffs(b) - 1)[h * (D + 2) + D]);
-      float l = 0.f, o[D / 32];
+    for (int h = 0; h < heads; ++h, ++task) {
+      if (task % kWarps != warp) continue;
+      const bool mine = (members >> lane) & 1u;
+      const float* piece = mine ? place(lane >> 1, lane & 1) + h * (D + 2) : nullptr;
+      const float pm = mine ? piece[D] : -INFINITY;
+      float m = warp_max(pm);
+      const float pf = pm == -INFINITY ? 0.f : ex2(pm - m);
+      float l = warp_sum(mine ? piece[D + 1] * pf : 0.f);
+      float o[D / 32];
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
       for (unsigned b = members; b; b &= b - 1) {
-        const float* src = at(__ffs(b) - 1) + h * (D + 2);
-        const float f = src[D] == -INFINITY ? 0.f : ex2(src[D] - m);
-        l += src[D + 1] * f;
+        const int j = __ffs(b) - 1;
+        const float f = __shfl_sync(kFull, pf, j);
+        const float* src = place(j >> 1, j & 1) + h * (D + 2) + lane;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) o[i] += src[i * 32 + lane] * f;
+        for (int i = 0; i < D / 32; ++i) o[i] += src[i * 32] * f;
       }
-      if (whole) {
-        const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        __nv_bfloat16* dst =
-            p.out + (int64_t)lead.row * p.out_stride + (int64_t)(kvh * p.heads_per_kv + grp * kGroup + h) * D;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) dst[i * 32 + lane] = f_to_bf16(o[i] * f);
-      } else {
-        float* dst = mine + h * (D + 2);
+      if (!whole) {
+        // The CTAs that share the segment, from its first pair's place in the stream. This CTA's piece goes
+        // to the workspace; whoever is last adds all of them up, in CTA order.
+        int64_t before = s_before[row / per];
+        for (int b = row / per * per; b < row; ++b) {
+          bool bad = false;
+          before += row_pairs(p, b, bad);
+        }
+        const int64_t seg0 = before * vheads + (int64_t)(kvh * p.groups + grp) * pairs;
+        const int c0 = (int)(seg0 / share), c1 = (int)((seg0 + pairs - 1) / share);
+        const int64_t head_floats = D + 2;
+        float* dst = p.parts + ((int64_t)blockIdx.x * 2 + (first > 0 ? 0 : 1)) * piece_floats + h * head_floats;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) __stcg(dst + i * 32 + lane, o[i]);
         if (lane == 0) {
           __stcg(dst + D, m);
           __stcg(dst + D + 1, l);
         }
-      }
-    }
-    if (whole) continue;
-    // The segment's first pair in the stream tells which CTAs share it.
-    int64_t before = s_before[lead.row / per];
-    for (int b = lead.row / per * per; b < lead.row; ++b) {
-      bool bad = false;
-      before += row_pairs(p, b, bad);
-    }
-    const int64_t seg0 = before * vheads + (int64_t)(kvh * p.groups + grp) * lead.pairs;
-    const int c0 = (int)(seg0 / share), c1 = (int)((seg0 + lead.pairs - 1) / share);
-    __threadfence();
-    __syncwarp();
-    int arrived = 0;
-    if (lane == 0) arrived = atomicAdd(p.counters + c0, 1);
-    arrived = __shfl_sync(kFull, arrived, 0);
-    if (arrived != c1 - c0) continue;
-    __threadfence();
-    if (lane == 0) p.counters[c0] = 0;  // as the next launch expects it
-    for (int h = 0; h < heads; ++h) {
-      float m = -INFINITY;
-      for (int cta = c0; cta <= c1; ++cta)
-        m = fmaxf(m, __ldcg(p.parts + ((int64_t)cta * 2 + (cta == c0 ? 1 : 0)) * piece_floats + h * (D + 2) + D));
-      float l = 0.f, o[D / 32];
+        __threadfence();
+        __syncwarp();
+        int arrived = 0;
+        if (lane == 0) arrived = atomicAdd(p.counters + c0 * kGroup + h, 1);
+        arrived = __shfl_sync(kFull, arrived, 0);
+        if (arrived != c1 - c0) continue;
+        __threadfence();
+        if (lane == 0) p.counters[c0 * kGroup + h] = 0;  // as the next launch expects it
+        // the segment begins in c0's second place and goes on in the others' first
+        auto part = [&](int cta) {
+          return p.parts + ((int64_t)cta * 2 + (cta == c0 ? 1 : 0)) * piece_floats + h * head_floats;
+        };
+        m = -INFINITY;
+        l = 0.f;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
-      for (int cta = c0; cta <= c1; ++cta) {
-        const float* src = p.parts + ((int64_t)cta * 2 + (cta == c0 ? 1 : 0)) * piece_floats + h * (D + 2);
-        const float pm = __ldcg(src + D), pl = __ldcg(src + D + 1);
-        const float f = pm == -INFINITY ? 0.f : ex2(pm - m);
-        l += pl * f;
+        for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
+        for (int c = c0; c <= c1; c += 32) {  // 32 pieces at a time
+          const bool on = c + lane <= c1;
+          const float qm = on ? __ldcg(part(c + lane) + D) : -INFINITY, ql = on ? __ldcg(part(c + lane) + D + 1) : 0.f;
+          const float nm = fmaxf(m, warp_max(qm));
+          const float down = m == -INFINITY ? 0.f : ex2(m - nm), qf2 = qm == -INFINITY ? 0.f : ex2(qm - nm);
+          l = l * down + warp_sum(ql * qf2);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) o[i] += __ldcg(src + i * 32 + lane) * f;
+          for (int i = 0; i < D / 32; ++i) o[i] *= down;
+          m = nm;
+          const int n = min(32, c1 - c + 1);
+#pragma unroll 4
+          for (int j = 0; j < n; ++j) {
+            const float f = __shfl_sync(kFull, qf2, j);
+            const float* src = part(c + j) + lane;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) o[i] += __ldcg(src + i * 32) * f;
+          }
+        }
       }
       const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-      __nv_bfloat16* dst =
-          p.out + (int64_t)lead.row * p.out_stride + (int64_t)(kvh * p.heads_per_kv + grp * kGroup + h) * D;
+      __nv_bfloat16* dst = p.out + (int64_t)row * p.out_stride + (int64_t)(kvh * p.heads_per_kv + grp * kGroup + h) * D;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) dst[i * 32 + lane] = f_to_bf16(o[i] * f);
     }
@@ -725,6 +725,8 @@ static int launch_decode(DecodeParams p, int num_ctas, cudaStream_t st) {
 
 }  // namespace kv8
 }  // namespace cdb
+
+extern "C" int cdb_kv8_decode_counters(int num_ctas) { return num_ctas > 0 ? num_ctas * cdb::kv8::kGroup : 0; }
 
 extern "C" int64_t cdb_kv8_decode_workspace_floats(int num_ctas, int head_dim) {
   if (num_ctas <= 0 || head_dim <= 0) return 0;

@@ -133,16 +133,16 @@ void check(int rc, const char* what) { TORCH_CHECK(rc == CDB_OK, what, " failed:
 // calls on two streams never share one. A captured call takes its own from the graph's memory and
 // zeroes the counters inside the graph, so that two graphs may be replayed at once.
 std::pair<Tensor, Tensor> decode_workspace(c10::Device dev, c10::cuda::CUDAStream stream, int ctas, int dim) {
-  const int64_t floats = cdb_kv8_decode_workspace_floats(ctas, dim);
+  const int64_t floats = cdb_kv8_decode_workspace_floats(ctas, dim), counters = cdb_kv8_decode_counters(ctas);
   const auto f32 = at::TensorOptions().dtype(at::kFloat).device(dev);
   const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
-    return {at::empty({floats}, f32), at::zeros({ctas}, i32)};
+    return {at::empty({floats}, f32), at::zeros({counters}, i32)};
   static std::map<std::pair<int, cudaStream_t>, std::pair<Tensor, Tensor>> kept;
   std::lock_guard<std::mutex> lock(g_mutex);
   auto& ws = kept[{dev.index(), stream.stream()}];
-  if (!ws.first.defined() || ws.first.numel() < floats || ws.second.numel() < ctas)
-    ws = {at::empty({floats}, f32), at::zeros({ctas}, i32)};
+  if (!ws.first.defined() || ws.first.numel() < floats || ws.second.numel() < counters)
+    ws = {at::empty({floats}, f32), at::zeros({counters}, i32)};
   return ws;
 }
 

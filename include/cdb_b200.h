@@ -496,8 +496,9 @@ int cdb_kv8_gather(const void* codes, const float* scales, int num_cache_layers,
                    int num_kv_heads, int head_dim, const int32_t* blocks, int n, void* out, int32_t* status,
                    void* stream);
 
-/* fp32 elements of cdb_kv8_decode_attention's workspace for num_ctas CTAs. */
+/* fp32 elements of cdb_kv8_decode_attention's workspace, and its int32 counters, for num_ctas CTAs. */
 int64_t cdb_kv8_decode_workspace_floats(int num_ctas, int head_dim);
+int cdb_kv8_decode_counters(int num_ctas);
 
 /* Decode attention over the 8-bit cache: row i attends to positions 0 .. item_pos[i] of slot
  * item_slot[i]; a row with item_pos < 0 is skipped and its out row left as it was. No work plan: the
@@ -506,8 +507,8 @@ int64_t cdb_kv8_decode_workspace_floats(int num_ctas, int head_dim);
  *              of 8. num_heads is a multiple of num_kv_heads; head h reads kv head
  *              h / (num_heads / num_kv_heads).
  *   num_ctas   CTAs to launch (one fits an SM); workspace: cdb_kv8_decode_workspace_floats of it;
- *              counters [num_ctas] int32, zeroed before the first use, left zeroed. Calls that
- *              share them must be ordered. */
+ *              counters: cdb_kv8_decode_counters of it, zeroed before the first use, left zeroed.
+ *              Calls that share them must be ordered. */
 int cdb_kv8_decode_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* codes,
                              const float* scales, int num_cache_layers, int cache_layer, int num_blocks,
                              const int32_t* block_table, int64_t block_table_stride, int table_rows, int table_width,
