@@ -50,6 +50,7 @@ struct DecodeParams {
   int num_items;
   float scale_log2;
   int min_share;     // pairs of one CTA's share, at least
+  int whole_pairs;   // the longest segments that are kept in one CTA, where there are few
   int stages;        // pairs in a warp's ring
   int stored_heads;  // heads of a stored piece: min(heads_per_kv, kGroup)
   float* parts;      // [CTAs][2][stored_heads][D + 2], then, unless they fit shared memory, each CTA's
@@ -406,6 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int64_t s_before[kThreads + 1];  // pairs before each thread's rows
   __shared__ int64_t s_warp[kWarps];
+  __shared__ int s_most[kWarps];
   __shared__ PieceTag s_tag[kWarps][2];
   __shared__ __align__(8) uint64_t s_bar[kWarps][kMaxStages];
   __shared__ __align__(16) float s_scale[kWarps][kMaxStages][4];
@@ -431,10 +433,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // ---- the stream: pairs before every thread's rows
   const int per = (p.num_items + kThreads - 1) / kThreads;
+  int longest;
   {
     int64_t mine = 0;
+    int most = 0;
     bool bad = false;
-    for (int b = threadIdx.x * per; b < min(p.num_items, (int)(threadIdx.x + 1) * per); ++b) mine += row_pairs(p, b, bad);
+    for (int b = threadIdx.x * per; b < min(p.num_items, (int)(threadIdx.x + 1) * per); ++b) {
+      const int n = row_pairs(p, b, bad);
+      mine += n;
+      most = max(most, n);
+    }
     if (bad && blockIdx.x == 0) set_error(p.status, CDB_ERR_INDEX);
     int64_t x = mine;
 #pragma unroll
@@ -442,13 +450,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t y = __shfl_up_sync(kFull, x, o);
       if (lane >= o) x += y;
     }
-    if (lane == 31) s_warp[warp] = x;
+    most = __reduce_max_sync(kFull, most);
+    if (lane == 31) s_warp[warp] = x, s_most[warp] = most;
     __syncthreads();
     int64_t base = 0, all = 0;
+    longest = 0;
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
       if (i < warp) base += s_warp[i];
       all += s_warp[i];
+      longest = max(longest, s_most[i]);
     }
     s_before[threadIdx.x] = base + x - mine;
     if (threadIdx.x == 0) s_before[kThreads] = all;
@@ -457,7 +468,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t total = s_before[kThreads] * vheads;
   const int64_t even = (total + gridDim.x - 1) / gridDim.x;
   const int64_t share = even > p.min_share ? even : p.min_share;
-  const int64_t begin = share * blockIdx.x, end = begin + share < total ? begin + share : total;
+  int64_t begin = share * blockIdx.x, end = begin + share < total ? begin + share : total;
+  if ((int64_t)p.num_items * vheads <= gridDim.x && longest <= p.whole_pairs) {
+    // Few short segments: a CTA for each, so that none has to meet another's piece in the workspace.
+    const int row = blockIdx.x / vheads, vh = blockIdx.x - row * vheads;
+    if (row >= p.num_items) return;
+    bool bad = false;
+    const int n = row_pairs(p, row, bad);
+    begin = s_before[row] * vheads + (int64_t)vh * n;  // (per is 1: rows are fewer than CTAs)
+    end = begin + n;
+  }
   if (begin >= end) return;  // uniform over the CTA
   const int64_t wshare = (end - begin + kWarps - 1) / kWarps;
   const int64_t wbegin = begin + wshare * warp;
@@ -778,6 +798,7 @@ extern "C" int cdb_kv8_decode_attention(const void* q, int64_t q_stride, void* o
   p.num_items = num_items;
   p.scale_log2 = scale * kLog2e;
   p.min_share = kWarps;
+  p.whole_pairs = 4 * kWarps;
   p.stages = 0;
   p.parts = workspace;
   p.first = workspace + (int64_t)num_ctas * 2 * p.stored_heads * (head_dim + 2);
