@@ -764,7 +764,8 @@ extern "C" int cdb_kv8_decode_attention(const void* q, int64_t q_stride, void* o
   using namespace cdb::kv8;
   if (codes == nullptr || scales == nullptr || (reinterpret_cast<uintptr_t>(codes) & 15) || cache_layer < 0 ||
       cache_layer >= num_cache_layers || num_blocks <= 0 || num_items < 0 || num_kv_heads <= 0 || num_heads <= 0 ||
-      num_heads % num_kv_heads != 0 || table_rows < 0 || table_width < 0 || num_ctas <= 0)
+      num_heads % num_kv_heads != 0 || table_rows < 0 || table_width < 0 || num_ctas <= 0 || !(scale > 0.f) ||
+      scale > 1e30f)
     return CDB_ERR_INVALID_ARGUMENT;
   if ((int64_t)num_blocks * num_kv_heads * 2 * kBlock > 0x7fffffff) return CDB_ERR_UNSUPPORTED;  // tile rows are int32
   if (head_dim != 64 && head_dim != 96 && head_dim != 128) return CDB_ERR_UNSUPPORTED;

@@ -2,29 +2,42 @@
 // consecutive query rows of one request, as cdb_prefill_attention takes them, any number of query heads
 // per kv head.
 //
-// A CTA takes one tile and one query head: 4 warps of 16 query rows. The tile's keys come in steps of
-// 64 (4 blocks): bulk copies bring the codes (8 contiguous tiles of 16 x D bytes) two steps ahead, the
-// CTA turns them into f16 (exact) in shared memory once, and the warps multiply from there (f16
-// m16n8k16, fp32 accumulators). Arithmetic as in the decode kernel: q over a power of two, x = S *
-// (scale log2e 2^e s_k) in fp32, an online base-2 softmax with l relative to the maximum m of x, and the
-// weights of V, 2^(x-m) s_v, relative to their own maximum M of x + log2 s_v, rounded to f16 (2^-11).
-// Bound by the tensor cores' mma.sync rate and by the softmax between the two products.
+// A CTA takes 128 query rows of one head: a tile and, where the list has it, the request's next one (so a
+// long chunk fills the tensor core's 128 rows; a lone tile leaves half of them idle). Keys come in steps of
+// 64 (4 blocks). Roles:
+//   warps 0..3  softmax: thread r owns query row r, so its maximum, sum and weights need no exchange;
+//   warps 4..7  bring the codes (bulk copies of whole (block, head) tiles, two steps ahead) and turn them into
+//               f16, exactly, in the tensor core's layout: K as it lies, V transposed. One of their threads
+//               issues the products: S = Q K^T (128 x 64 x D) one step ahead of O += P V (128 x D x 64), both
+//               tcgen05 with f16 operands in shared memory and fp32 accumulators in tensor memory.
+// Two CTAs share an SM (256 of its 512 tensor-memory columns, 113 KB of shared memory each): one computes
+// exponentials while the other multiplies.
 //
-// A masked key never counts, whatever it holds: its x is replaced, and a NaN in its V, which a product
-// with weight zero would spread, is taken out of the tiles that the diagonal crosses and put back for
-// the rows that see it.
+// Arithmetic as in the decode kernel: q over a power of two per row, an online base-2 softmax with l relative
+// to a maximum m of the logits x, the weights of V, w = 2^x s_v, relative to their own maximum M and rounded
+// to f16 (2^-11). m and M move only when passed by 8, and then the row's O is rescaled in tensor memory.
+// One exponential a key: w 2^-M = 2^(S f + log2 s_v - M), and l takes the sum of a block's weights times the
+// block's 2^(M - m) / s_v, unless that factor is so far from 1 that the weights could have underflowed.
+//
+// Measured bounds: exponentials and their neighbours (issue slots), then the products.
+//
+// A masked key never counts, whatever it holds: its logit is replaced, and a NaN in its V, which a product
+// with weight zero would spread, is taken out in the steps that the diagonal crosses and put back at the end
+// for the rows that see it.
 #include "kv8.cuh"
-#include "smem_tile.cuh"
 
 namespace cdb {
 namespace kv8 {
 
-using prefill::ldsm_x4;
-using prefill::ldsm_x4_t;
-using prefill::RowPitch;
-using prefill::swz;
-
-constexpr int TQ = 64, TK = 64;
+constexpr int TR = 64;   // rows of a listed tile
+constexpr int TM = 128;  // rows of a CTA
+constexpr int TK = 64;   // keys of a step
+constexpr int kSoftmax = 128, kConvert = 128;
+constexpr int kPrefillThreads = kSoftmax + kConvert;
+constexpr int kMeta = 4;            // steps whose scales are kept
+constexpr int kDiagonal = 3;        // steps that the diagonal of 128 rows can cross
+constexpr int kPairLimit = 2048;    // longest tile list that every CTA searches for its neighbours
+constexpr uint32_t kTmemCols = 256;
 constexpr uint32_t kAll = 0xffffffffu;
 
 struct PrefillParams {
@@ -39,10 +52,43 @@ struct PrefillParams {
   int64_t bt_stride;
   int bt_rows, bt_width;
   const int4* tiles;  // {first row, rows, slot, position of the first row}
-  int num_rows;       // rows of q and out
+  int num_tiles;
+  int num_rows;  // rows of q and out
   float scale_log2;
   int32_t* status;
 };
+
+template <int D>
+struct Tile {
+  static constexpr int BLK = kBlock * D;          // bytes of one block's codes
+  static constexpr int ATOMS = (D + 63) / 64;     // 128-byte swizzle atoms of a row of D f16
+  static constexpr int VBLK = BLK + 32;           // a staged block of V: 32 bytes on spread the banks
+  static constexpr int OFF_Q = 0;                 // f16 [ATOMS][128][64]
+  static constexpr int OFF_K = OFF_Q + ATOMS * TM * 128;  // f16 [ATOMS][64][64]
+  static constexpr int OFF_V = OFF_K + ATOMS * TK * 128;  // f16 [D][64 keys]
+  static constexpr int OFF_P = OFF_V + D * 128;   // f16 [128][64 keys]
+  static constexpr int OFF_SK = OFF_P + TM * 128; // codes [2][4 blocks]
+  static constexpr int OFF_SV = OFF_SK + 2 * 4 * BLK;
+  static constexpr int OFF_BAR = (OFF_SV + 2 * 4 * VBLK + 15) / 16 * 16;
+  static constexpr int SMEM = OFF_BAR + 512;
+  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
+};
+
+// Barriers and small state behind the tiles.
+struct Shared {
+  uint64_t staged[2];        // a step's copies have landed (4 threads announce them)
+  uint64_t sfull[2];         // S product done: S in tensor memory, K's place free
+  uint64_t sfree[2];         // S read (first: q written)
+  uint64_t pfull, odone;     // weights written / O product done with them and with V
+  uint64_t meta[kMeta];      // a step's scales written
+  uint64_t drain;
+  alignas(16) float scale[kMeta][2][4];  // K's scale (< 0: no such block), log2 of V's
+  unsigned long long nan[kDiagonal];
+  uint32_t tmem;
+  int abort;
+  int found[4];              // counts of the tile search, rows of the partner
+};
+static_assert(sizeof(Shared) <= 512 && alignof(Shared) == 16, "room behind the tiles");
 
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
@@ -50,300 +96,546 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
+// Matrix descriptor of a K-major operand in 128-byte swizzled rows of 64 f16, 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t operand(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// D[tmem] (+)= A B^T, kind::f16 with f16 operands: fp32 accumulators, M = 128.
+__device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+  const uint32_t none = 0, acc = add;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+      "l"(operand(a)), "l"(operand(b)), "r"(idesc), "r"(acc), "r"(none)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 32 columns of this warp's 32 tensor-memory lanes.
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
+      : "memory");
+}
+// Waits for this thread's tensor-memory loads; the registers pass through it, so no use can move ahead.
+__device__ __forceinline__ void wait_loads(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+               "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+               "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+               "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Bounded wait that also gives up once another role has.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int32_t* status, volatile int* abort) {
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 255u && *abort) return false;
+  }
+  set_error(status, CDB_ERR_DEVICE_TIMEOUT);
+  *abort = 1;
+  return false;
+}
+
+// What a CTA does with the list entry that it was started for: its own rows and the partner's.
+struct Rows {
+  int row0, n, slot, pos;
+};
+
+__device__ __forceinline__ bool fits(const PrefillParams& p, int4 tile) {
+  return tile.y <= TR && tile.x >= 0 && tile.x <= p.num_rows - tile.y && tile.z >= 0 && tile.z < p.bt_rows &&
+         tile.w >= 0 && (tile.w + tile.y - 1) / kBlock < p.bt_width;
+}
+
+// Decides from the whole list whether this entry stands alone, takes the request's next 64 rows along, or is
+// itself taken along (then n = 0). A request's tiles are counted in order of position; one with an even count
+// before it leads. Both ends of a pair see the same counts, so each row is computed exactly once; entries that
+// overlap another of their slot are not paired.
+__device__ __forceinline__ Rows choose_rows(const PrefillParams& p, Shared& sh, int4 tile) {
+  Rows me = {tile.x, tile.y, tile.z, tile.w};
+  if (p.num_tiles > kPairLimit || p.num_tiles < 2) return me;
+  int before_lead = 0, before_me = 0, before_next = 0;
+  bool lead = false;
+  for (int i = threadIdx.x; i < p.num_tiles; i += kPrefillThreads) {
+    const int4 o = p.tiles[i];
+    if (o.y <= 0 || o.z != tile.z) continue;
+    before_lead += o.w < tile.w - TR;
+    before_me += o.w < tile.w;
+    before_next += o.w < tile.w + TR;
+    lead = lead || (o.w == tile.w - TR && o.x == tile.x - TR && o.y == TR && o.w >= 0 && o.x >= 0);
+    if (o.w == tile.w + TR && o.x == tile.x + TR && fits(p, o)) sh.found[3] = o.y;
+  }
+  before_lead = __reduce_add_sync(kAll, before_lead);
+  before_me = __reduce_add_sync(kAll, before_me);
+  before_next = __reduce_add_sync(kAll, before_next);
+  if ((threadIdx.x & 31) == 0) {
+    atomicAdd(&sh.found[0], before_lead);
+    atomicAdd(&sh.found[1], before_me);
+    atomicAdd(&sh.found[2], before_next);
+  }
+  const bool led = __syncthreads_or(lead);
+  const int c0 = sh.found[0], c1 = sh.found[1], c2 = sh.found[2];
+  if (led && c0 % 2 == 0 && c1 == c0 + 1) me.n = 0;
+  else if (tile.y == TR && sh.found[3] > 0 && c1 % 2 == 0 && c2 == c1 + 1) me.n += sh.found[3];
+  return me;
+}
+
 template <int D>
-__global__ void __launch_bounds__(128, 3) prefill_kernel(const PrefillParams p) {
+__global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const PrefillParams p) {
+  using T = Tile<D>;
   pdl_trigger();
-  constexpr int KS = D / 16, NT = D / 8, PITCH = RowPitch<D>::BYTES;
-  constexpr int BLK = kBlock * D;     // bytes of one block's codes
-  constexpr int STAGE = 8 * BLK;      // 4 blocks of K, 4 of V
-  extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t* sk = smem;                 // f16 [64][D]
-  uint8_t* sv = sk + TK * PITCH;      // f16 [64][D]
-  uint8_t* stage = sv + TK * PITCH;   // [2][STAGE]
-  __shared__ __align__(8) uint64_t s_bar[2];
-  __shared__ float s_scale[4][2][4];  // [step % 4][K, V][block]; a negative K scale: no such block
-  __shared__ unsigned long long s_nan;
-  const uint32_t sk_u = smem_u32(sk), sv_u = smem_u32(sv);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(TK >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
+  constexpr uint32_t kIdescO = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Shared& sh = *reinterpret_cast<Shared*>(smem + T::OFF_BAR);
+  const uint32_t base = smem_u32(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    mbar_init(&s_bar[0], 4);
-    mbar_init(&s_bar[1], 4);
-    s_nan = 0ull;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.staged[i], 4);
+      mbar_init(&sh.sfull[i], 1);
+      mbar_init(&sh.sfree[i], kSoftmax);
+    }
+    for (int i = 0; i < kMeta; ++i) mbar_init(&sh.meta[i], 4);
+    mbar_init(&sh.pfull, kSoftmax);
+    mbar_init(&sh.odone, 1);
+    mbar_init(&sh.drain, 1);
+    for (int i = 0; i < kDiagonal; ++i) sh.nan[i] = 0ull;
+    for (int i = 0; i < 4; ++i) sh.found[i] = 0;
+    sh.abort = (base & 1023u) != 0u;  // the swizzle counts on it
     fence_barrier_init();
   }
   __syncthreads();
   pdl_wait();
 
   const int4 tile = p.tiles[blockIdx.y];
-  const int head = blockIdx.x, kvh = head / p.heads_per_kv;
-  const int row0 = tile.x, nrows = tile.y, slot = tile.z, pos0 = tile.w;
-  if (nrows <= 0) return;  // an unused entry of the list
-  if (nrows > TQ || row0 < 0 || row0 > p.num_rows - nrows || slot < 0 || slot >= p.bt_rows || pos0 < 0 ||
-      (pos0 + nrows - 1) / kBlock >= p.bt_width) {
+  if (tile.y <= 0) return;  // an unused entry of the list
+  if (!fits(p, tile) || sh.abort) {
     if (tid == 0) set_error(p.status, CDB_ERR_INDEX);
     return;
   }
-  const int kv_len = pos0 + nrows;
-  const int steps = (kv_len + TK - 1) / TK;
-  const int blocks = (kv_len + kBlock - 1) / kBlock;
-  const int32_t* bt = p.block_table + (int64_t)slot * p.bt_stride;
-  const int64_t v_tiles = (int64_t)p.num_blocks * p.kv_heads;
-
-  // Threads 0..3 bring one block of every step each: the id a step ahead of its copies, the copies two
-  // steps ahead of their use, the scales with them.
-  int id = -1;
-  auto fetch_id = [&](int step) {
-    const int b = step * 4 + tid;
-    id = step < steps && b < blocks ? bt[b] : -1;
-  };
-  float hold_k = -1.f, hold_v = 1.f;
-  auto issue = [&](int step) {
-    if (step >= steps) return;
-    uint64_t* bar = &s_bar[step & 1];
-    const bool used = step * 4 + tid < blocks;
-    const bool known = used && id >= 0 && id < p.num_blocks;
-    hold_k = -1.f;
-    hold_v = 1.f;
-    if (known) {
-      const int64_t at = (int64_t)id * p.kv_heads + kvh;
-      mbar_arrive_expect_tx(bar, 2 * BLK);
-      const uint32_t dst = smem_u32(stage) + (step & 1) * STAGE + tid * BLK;
-      bulk_copy(dst, p.codes + at * BLK, BLK, smem_u32(bar));
-      bulk_copy(dst + 4 * BLK, p.codes + (v_tiles + at) * BLK, BLK, smem_u32(bar));
-      hold_k = p.scales[at];
-      hold_v = p.scales[v_tiles + at];
-    } else {
-      if (used) set_error(p.status, CDB_ERR_INDEX);
-      mbar_arrive(bar);
-    }
-  };
-  auto post = [&](int step) {
-    s_scale[step & 3][0][tid] = hold_k;
-    s_scale[step & 3][1][tid] = hold_v > 0.f ? __log2f(hold_v) : -126.f;
-  };
-  if (tid < 4) {
-    fetch_id(0);
-    issue(0);
-    post(0);
-    fetch_id(1);
-    issue(1);
-    fetch_id(2);
+  const Rows me = choose_rows(p, sh, tile);
+  if (me.n == 0) return;  // the entry before takes these rows along
+  const int head = blockIdx.x, kvh = head / p.heads_per_kv;
+  const int kv_len = me.pos + me.n;
+  const int steps = (kv_len + TK - 1) / TK, blocks = (kv_len + kBlock - 1) / kBlock;
+  const int diagonal = me.pos / TK;  // the first step that holds a key which some row may not see
+  if (warp == 4) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = sh.tmem;          // S: two buffers of 64 columns; O: 128 columns on
+  const uint32_t tmem_o = tmem + 2 * TK;
+  volatile int* abort = &sh.abort;
 
-  // q fragments, divided by a power of two per row
-  uint32_t qa[KS][4];
-  float factor[2];
-  const int qr[2] = {warp * 16 + g, warp * 16 + g + 8};
-  {
-    float amax[2] = {0.f, 0.f};
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const bool on = qr[r] < nrows;
-      const __nv_bfloat16* src = p.q + (int64_t)(row0 + (on ? qr[r] : 0)) * p.q_stride + (int64_t)head * D + 2 * t;
-#pragma unroll
-      for (int kk = 0; kk < KS; ++kk) {
-        qa[kk][r] = on ? *reinterpret_cast<const uint32_t*>(src + kk * 16) : 0u;
-        qa[kk][2 + r] = on ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8) : 0u;
-        amax[r] = fmaxf(amax[r], fmaxf(fmaxf(fabsf(bf16lo(qa[kk][r])), fabsf(bf16hi(qa[kk][r]))),
-                                       fmaxf(fabsf(bf16lo(qa[kk][2 + r])), fabsf(bf16hi(qa[kk][2 + r])))));
+  if (warp >= 4) {
+    // ------------------------------------------------------------ codes to f16, and the products
+    const int ct = tid - kSoftmax, cw = warp - 4;
+    const int32_t* bt = p.block_table + (int64_t)me.slot * p.bt_stride;
+    const int64_t v_tiles = (int64_t)p.num_blocks * p.kv_heads;
+    // Threads 0..3 bring one block of every step each, its id a step ahead of its copies.
+    int id = -1;
+    float hold_k = -1.f, hold_v = 1.f;
+    auto fetch_id = [&](int step) {
+      const int b = step * 4 + ct;
+      id = step < steps && b < blocks ? bt[b] : -1;
+    };
+    auto issue = [&](int step) {
+      if (step >= steps) return;
+      uint64_t* bar = &sh.staged[step & 1];
+      const bool used = step * 4 + ct < blocks;
+      hold_k = -1.f;
+      hold_v = 1.f;
+      if (used && id >= 0 && id < p.num_blocks) {
+        const int64_t at = (int64_t)id * p.kv_heads + kvh;
+        mbar_arrive_expect_tx(bar, 2 * T::BLK);
+        bulk_copy(base + T::OFF_SK + ((step & 1) * 4 + ct) * T::BLK, p.codes + at * T::BLK, T::BLK, smem_u32(bar));
+        bulk_copy(base + T::OFF_SV + ((step & 1) * 4 + ct) * T::VBLK, p.codes + (v_tiles + at) * T::BLK, T::BLK,
+                  smem_u32(bar));
+        hold_k = p.scales[at];
+        hold_v = p.scales[v_tiles + at];
+      } else {
+        if (used) set_error(p.status, CDB_ERR_INDEX);
+        mbar_arrive(bar);
       }
-    }
+    };
+    auto post = [&](int step) {  // the scales that issue(step) fetched
+      if (step >= steps) return;
+      sh.scale[step & (kMeta - 1)][0][ct] = hold_k;
+      sh.scale[step & (kMeta - 1)][1][ct] = hold_v > 0.f ? __log2f(hold_v) : -126.f;
+      mbar_arrive(&sh.meta[step & (kMeta - 1)]);
+    };
+    // K of step j into place: 16 codes of a key at a time; a quarter warp covers four chunks of two keys.
+    auto convert_k = [&](int j) {
+      constexpr int C = D / 16;  // chunks of a key
+      const uint8_t* src = smem + T::OFF_SK + (j & 1) * 4 * T::BLK;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      amax[r] = fmaxf(amax[r], __shfl_xor_sync(kAll, amax[r], 1));
-      amax[r] = fmaxf(amax[r], __shfl_xor_sync(kAll, amax[r], 2));
-      int e = (int)(__float_as_uint(amax[r]) >> 23) - 127;
-      e = amax[r] == 0.f ? 0 : max(-126, min(126, e));
-      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-      factor[r] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
-#pragma unroll
-      for (int kk = 0; kk < KS; ++kk) {
-        qa[kk][r] = pack_f16x2(bf16lo(qa[kk][r]) * down, bf16hi(qa[kk][r]) * down);
-        qa[kk][2 + r] = pack_f16x2(bf16lo(qa[kk][2 + r]) * down, bf16hi(qa[kk][2 + r]) * down);
-      }
-    }
-  }
-
-  float o[NT][4];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, mw[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  const int qpos[2] = {pos0 + qr[0], pos0 + qr[1]};
-
-  for (int st = 0; st < steps; ++st) {
-    // also: the f16 tiles of the last step have been read
-    if (!__syncthreads_and(mbar_wait(&s_bar[st & 1], (st >> 1) & 1, p.status))) {
-      // a copy that never came: the error is recorded; wait for the next step's, in flight
-      if (st + 1 < steps) mbar_wait(&s_bar[(st + 1) & 1], ((st + 1) >> 1) & 1, p.status);
-      break;
-    }
-    const int key0 = st * TK;
-    const bool diagonal = key0 + TK - 1 > pos0;
-    const uint8_t* src = stage + (st & 1) * STAGE;
-    // codes -> f16: a thread takes 16 bytes at a time
-    for (int i = tid; i < 2 * TK * D / 16; i += 128) {
-      const int r = i / (D / 16), c = i % (D / 16);  // rows 0..63 K, 64..127 V
-      uint4 w = *reinterpret_cast<const uint4*>(src + (int64_t)i * 16);
-      const int key = r & 63;
-      if (r >= TK) {
-        if (key0 + key >= kv_len || s_scale[st & 3][0][key >> 4] < 0.f) w = make_uint4(0u, 0u, 0u, 0u);
-        if (diagonal) {
-          uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-          uint32_t any = 0u;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t nan = ((ws[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // the bytes 0x7f and 0xff
-            any |= nan;
-            ws[e] &= ~(nan | (nan - (nan >> 7)));
-          }
-          if (any) atomicOr(&s_nan, 1ull << key);
-          w = make_uint4(ws[0], ws[1], ws[2], ws[3]);
+      for (int i0 = 0; i0 < TK * C; i0 += kConvert) {
+        const int i = i0 + ct;
+        int key, c;
+        if (C == 6) {
+          key = i / 6;
+          c = i - key * 6;
+        } else {
+          const int rest = i >> 2;
+          key = C == 8 ? (rest & 7) + ((rest >> 4) << 3) : rest;
+          c = (i & 3) + (C == 8 ? ((rest >> 3) & 1) * 4 : 0);
         }
+        const uint4 w = *reinterpret_cast<const uint4*>(src + key * D + c * 16);
+        uint8_t* dst = smem + T::OFF_K + (c >> 2) * (TK * 128) + key * 128;
+        const int ch = (c & 3) * 2;
+        *reinterpret_cast<uint4*>(dst + ((ch ^ (key & 7)) << 4)) =
+            make_uint4(cvt_e4m3x2_f16x2(w.x & 0xffffu), cvt_e4m3x2_f16x2(w.x >> 16), cvt_e4m3x2_f16x2(w.y & 0xffffu),
+                       cvt_e4m3x2_f16x2(w.y >> 16));
+        *reinterpret_cast<uint4*>(dst + (((ch + 1) ^ (key & 7)) << 4)) =
+            make_uint4(cvt_e4m3x2_f16x2(w.z & 0xffffu), cvt_e4m3x2_f16x2(w.z >> 16), cvt_e4m3x2_f16x2(w.w & 0xffffu),
+                       cvt_e4m3x2_f16x2(w.w >> 16));
       }
-      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-      uint32_t f[8];
+    };
+    // V of step j into place, transposed: 8 tokens of 4 dims at a time; lanes over the 4 blocks and 8 groups
+    // of dims.
+    auto convert_v = [&](int j) {
+      const int b = lane & 3;
+      const bool have = sh.scale[j & (kMeta - 1)][0][b] >= 0.f;
+#pragma unroll 1
+      for (int u = cw; u < 2 * (D / 32); u += 4) {
+        const int half = u & 1, d0 = (u >> 1) * 32 + (lane >> 2) * 4;
+        const uint8_t* src = smem + T::OFF_SV + ((j & 1) * 4 + b) * T::VBLK + half * 8 * D + d0;
+        const int key0 = b * kBlock + half * 8;
+        const int live = have ? kv_len - j * TK - key0 : 0;  // of these 8 tokens
+        uint32_t w[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        f[2 * e] = cvt_e4m3x2_f16x2(ws[e] & 0xffffu);
-        f[2 * e + 1] = cvt_e4m3x2_f16x2(ws[e] >> 16);
-      }
-      uint8_t* dst = r >= TK ? sv : sk;
-      *reinterpret_cast<uint4*>(dst + swz<D>(key, 2 * c)) = make_uint4(f[0], f[1], f[2], f[3]);
-      *reinterpret_cast<uint4*>(dst + swz<D>(key, 2 * c + 1)) = make_uint4(f[4], f[5], f[6], f[7]);
-    }
-    __syncthreads();
-    const unsigned long long nans = diagonal ? s_nan : 0ull;
-    if (nans) {  // rare: the rows that see a NaN of V get it here
-      for (unsigned long long b = nans; b; b &= b - 1) {
-        const int key = __ffsll((long long)b) - 1;
+        for (int r = 0; r < 8; ++r) {
+          w[r] = *reinterpret_cast<const uint32_t*>(src + r * D);
+          if (r >= live) w[r] = 0u;
+        }
+        if (j >= diagonal) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint8_t code = src[4 * BLK + key * D + j * 8 + 2 * t + e];
-            if ((code & 0x7fu) == 0x7fu) {
-              if (key0 + key <= qpos[0]) o[j][e] = NAN;
-              if (key0 + key <= qpos[1]) o[j][2 + e] = NAN;
+          for (int r = 0; r < 8; ++r) {
+            const uint32_t nan = ((w[r] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // the bytes 0x7f and 0xff
+            if (nan) {
+              w[r] &= ~(nan | (nan - (nan >> 7)));
+              atomicOr(&sh.nan[j - diagonal], 1ull << (key0 + r));
             }
           }
         }
-      }
-      __syncthreads();
-      if (tid == 0) s_nan = 0ull;
-    }
-    if (tid < 4) {  // this step's codes have been read
-      post(st + 1);
-      issue(st + 2);
-      fetch_id(st + 3);
-    }
-
-    float s[TK / 8][4];
+        const int ch = key0 >> 3;
 #pragma unroll
-    for (int j = 0; j < TK / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+        for (int e = 0; e < 4; e += 2) {
+          const uint32_t sel = e == 0 ? 0x5140u : 0x7362u;
+          uint32_t lo[4], hi[4];
 #pragma unroll
-    for (int kk = 0; kk < KS; ++kk) {
-#pragma unroll
-      for (int np = 0; np < TK / 16; ++np) {
-        uint32_t b0, b1, b2, b3;
-        ldsm_x4(sk_u + swz<D>(np * 16 + (lane & 7) + 8 * (lane >> 4), 2 * kk + ((lane >> 3) & 1)), b0, b1, b2, b3);
-        mma_f16(s[2 * np], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b0, b1);
-        mma_f16(s[2 * np + 1], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b2, b3);
-      }
-    }
-    // logits, their maxima, and the maxima of logit + log2 s_v
-    float mx[2] = {-INFINITY, -INFINITY}, mz[2] = {-INFINITY, -INFINITY};
-    float ev[4];
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const float ks = s_scale[st & 3][0][b];
-      ev[b] = s_scale[st & 3][1][b];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float f = factor[r] * ks;
-        float bm = -INFINITY;
-#pragma unroll
-        for (int j = 2 * b; j < 2 * b + 2; ++j) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& x = s[j][2 * r + e];
-            x *= f;
-            if (diagonal && key0 + j * 8 + 2 * t + e > qpos[r]) x = -INFINITY;
-            if (ks < 0.f) x = -INFINITY;
-            bm = fmaxf(bm, x);
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t pair = __byte_perm(w[2 * r], w[2 * r + 1], sel);
+            lo[r] = cvt_e4m3x2_f16x2(pair & 0xffffu);
+            hi[r] = cvt_e4m3x2_f16x2(pair >> 16);
           }
+          const int d = d0 + e;
+          *reinterpret_cast<uint4*>(smem + T::OFF_V + d * 128 + ((ch ^ (d & 7)) << 4)) =
+              make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          *reinterpret_cast<uint4*>(smem + T::OFF_V + (d + 1) * 128 + ((ch ^ ((d + 1) & 7)) << 4)) =
+              make_uint4(hi[0], hi[1], hi[2], hi[3]);
         }
-        mx[r] = fmaxf(mx[r], bm);
-        mz[r] = fmaxf(mz[r], bm + ev[b]);
       }
+    };
+    // What the converting threads wrote is the products' to read; true if all of them are well.
+    auto hand_over = [&](bool mine) {
+      fence_proxy_async_shared();
+      uint32_t all;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, %2, p;\n\t"
+          "selp.u32 %0, 1, 0, q;\n\t}"
+          : "=r"(all)
+          : "r"((uint32_t)mine), "n"(kConvert)
+          : "memory");
+      return all != 0u;
+    };
+
+    if (ct < 4) {
+      fetch_id(0);
+      issue(0);
+      post(0);
+      fetch_id(1);
+      issue(1);
+      fetch_id(2);
     }
+    int announced = min(2, steps);
+    bool ok = true;
+    // Step j: K of step j + 1 and its product S, then the product O of step j, then V of step j + 1.
+    for (int j = -1; j < steps && ok; ++j) {
+      const int n = j + 1;
+      if (n < steps) {
+        ok = wait_for(&sh.staged[n & 1], (n >> 1) & 1, p.status, abort);
+        if (ct < 4) post(n + 1);
+        ok = ok && wait_for(&sh.meta[n & (kMeta - 1)], (n / kMeta) & 1, p.status, abort);
+        if (j >= 0) ok = ok && wait_for(&sh.sfull[j & 1], (j >> 1) & 1, p.status, abort);  // K's place is free
+        if (ok) convert_k(n);
+        ok = hand_over(ok);
+        if (ct == 0 && ok) {
+          ok = wait_for(&sh.sfree[n & 1], (n >> 1) & 1, p.status, abort);
+          if (ok) {
+            fence_after();
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      mx[r] = fmaxf(mx[r], __shfl_xor_sync(kAll, mx[r], 1));
-      mx[r] = fmaxf(mx[r], __shfl_xor_sync(kAll, mx[r], 2));
-      mz[r] = fmaxf(mz[r], __shfl_xor_sync(kAll, mz[r], 1));
-      mz[r] = fmaxf(mz[r], __shfl_xor_sync(kAll, mz[r], 2));
-      const float nm = fmaxf(m[r], mx[r]), nw = fmaxf(mw[r], mz[r]);
-      l[r] *= nm == -INFINITY ? 1.f : ex2(m[r] - nm);
-      m[r] = nm;
-      const float down = nw == -INFINITY ? 1.f : ex2(mw[r] - nw);
-      mw[r] = nw;
-      if (__any_sync(kAll, down != 1.f)) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) o[j][2 * r] *= down, o[j][2 * r + 1] *= down;
-      }
-    }
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float f = m[r] == -INFINITY ? 0.f : ex2(ev[b] + m[r] - mw[r]);
-#pragma unroll
-        for (int j = 2 * b; j < 2 * b + 2; ++j) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& x = s[j][2 * r + e];
-            const float w = x == -INFINITY ? 0.f : ex2(x - m[r]);
-            l[r] += w;
-            x = w * f;
+            for (int kk = 0; kk < D / 16; ++kk)
+              product(tmem + (n & 1) * TK, base + T::OFF_Q + (kk >> 2) * (TM * 128) + (kk & 3) * 32,
+                      base + T::OFF_K + (kk >> 2) * (TK * 128) + (kk & 3) * 32, kIdescS, kk > 0);
+            commit(&sh.sfull[n & 1]);
           }
         }
       }
+      if (j >= 0) {
+        if (ct == 0 && ok) {
+          ok = wait_for(&sh.pfull, j & 1, p.status, abort);
+          if (ok) {
+            fence_after();
+#pragma unroll
+            for (int kk = 0; kk < TK / 16; ++kk)
+              product(tmem_o, base + T::OFF_P + kk * 32, base + T::OFF_V + kk * 32, kIdescO, j > 0 || kk > 0);
+            commit(&sh.odone);
+          }
+        }
+        ok = ok && wait_for(&sh.odone, j & 1, p.status, abort);  // V's place is free
+      }
+      if (n < steps) {
+        if (ok) convert_v(n);
+        ok = hand_over(ok);  // and this step's codes have been read
+        if (ct < 4) {
+          issue(n + 2);
+          fetch_id(n + 3);
+        }
+        announced = min(n + 3, steps);
+      }
     }
+    if (!ok)  // the copies in flight, after an abort; a step that has landed passes at once or runs into the limit
+      for (int j = max(0, announced - 2); j < announced; ++j) mbar_wait(&sh.staged[j & 1], (j >> 1) & 1, p.status);
+    if (ct == 0) {
+      commit(&sh.drain);  // on every path: no product may run when the tensor memory is freed
+      mbar_wait(&sh.drain, 0, p.status);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int r = tid;  // query row, and tensor-memory lane
+    const bool mine = r < me.n;
+    const bool rows_here = warp * 32 < me.n;  // a warp without rows only keeps the barriers going
+    const int qpos = me.pos + r;
+    float factor = 0.f;
+    {
+      const __nv_bfloat16* src = p.q + (int64_t)(me.row0 + (mine ? r : 0)) * p.q_stride + (int64_t)head * D;
+      float amax = 0.f;
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 w = *reinterpret_cast<const uint4*>(src + c * 8);
+        amax = fmaxf(amax, fmaxf(fmaxf(fmaxf(fabsf(bf16lo(w.x)), fabsf(bf16hi(w.x))), fmaxf(fabsf(bf16lo(w.y)), fabsf(bf16hi(w.y)))),
+                                 fmaxf(fmaxf(fabsf(bf16lo(w.z)), fabsf(bf16hi(w.z))), fmaxf(fabsf(bf16lo(w.w)), fabsf(bf16hi(w.w))))));
+      }
+      int e = (int)(__float_as_uint(amax) >> 23) - 127;
+      e = amax == 0.f ? 0 : max(-126, min(126, e));
+      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+      factor = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (mine) w = *reinterpret_cast<const uint4*>(src + c * 8);
+        uint8_t* dst = smem + T::OFF_Q + (c >> 3) * (TM * 128) + r * 128;
+        *reinterpret_cast<uint4*>(dst + (((c & 7) ^ (r & 7)) << 4)) =
+            make_uint4(pack_f16x2(bf16lo(w.x) * down, bf16hi(w.x) * down), pack_f16x2(bf16lo(w.y) * down, bf16hi(w.y) * down),
+                       pack_f16x2(bf16lo(w.z) * down, bf16hi(w.z) * down), pack_f16x2(bf16lo(w.w) * down, bf16hi(w.w) * down));
+      }
+    }
+    fence_proxy_async_shared();
+    mbar_arrive(&sh.sfree[0]);  // q is in place: the first product may go (its buffer is free anyway)
+    mbar_arrive(&sh.sfree[1]);
+
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    float m = -INFINITY, mw = -INFINITY, l = 0.f;
+    for (int j = 0; j < steps; ++j) {
+      if (!__all_sync(kAll, wait_for(&sh.sfull[j & 1], (j >> 1) & 1, p.status, abort) &&
+                                wait_for(&sh.meta[j & (kMeta - 1)], (j / kMeta) & 1, p.status, abort)))
+        break;
+      bool stop = false;
+      if (rows_here) {
+        fence_after();
+        uint32_t s[TK];
+        tmem_load(tmem + lanes + (j & 1) * TK, s);
+        tmem_load(tmem + lanes + (j & 1) * TK + 32, s + 32);
+        wait_loads(s);
+        wait_loads(s + 32);
+        fence_before();
+        mbar_arrive(&sh.sfree[j & 1]);
+        const float4 ks = *reinterpret_cast<const float4*>(sh.scale[j & (kMeta - 1)][0]);
+        const float4 vs = *reinterpret_cast<const float4*>(sh.scale[j & (kMeta - 1)][1]);
+        // logits are S * f; f stays above 0 (an all-zero block under a tiny q), below it no such block
+        const float f[4] = {ks.x < 0.f ? -1.f : fmaxf(factor * ks.x, 1.2e-38f), ks.y < 0.f ? -1.f : fmaxf(factor * ks.y, 1.2e-38f),
+                            ks.z < 0.f ? -1.f : fmaxf(factor * ks.z, 1.2e-38f), ks.w < 0.f ? -1.f : fmaxf(factor * ks.w, 1.2e-38f)};
+        const float ev[4] = {vs.x, vs.y, vs.z, vs.w};
+        if (j >= diagonal || f[0] < 0.f || f[1] < 0.f || f[2] < 0.f || f[3] < 0.f) {
+          const int seen = qpos - j * TK;  // the last key of the step that the row sees
 #pragma unroll
-    for (int k2 = 0; k2 < TK / 16; ++k2) {
-      const uint32_t a0 = pack_f16x2(s[2 * k2][0], s[2 * k2][1]), a1 = pack_f16x2(s[2 * k2][2], s[2 * k2][3]);
-      const uint32_t a2 = pack_f16x2(s[2 * k2 + 1][0], s[2 * k2 + 1][1]),
-                     a3 = pack_f16x2(s[2 * k2 + 1][2], s[2 * k2 + 1][3]);
+          for (int k = 0; k < TK; ++k)
+            if (k > seen || f[k >> 4] < 0.f) s[k] = f[k >> 4] < 0.f ? 0x7f800000u : 0xff800000u;
+        }
+        float mx = -INFINITY, mz = -INFINITY;
 #pragma unroll
-      for (int cp = 0; cp < NT / 2; ++cp) {
-        uint32_t b0, b1, b2, b3;
-        ldsm_x4_t(sv_u + swz<D>(k2 * 16 + (lane & 7) + 8 * ((lane >> 3) & 1), 2 * cp + (lane >> 4)), b0, b1, b2, b3);
-        mma_f16(o[2 * cp], a0, a1, a2, a3, b0, b1);
-        mma_f16(o[2 * cp + 1], a0, a1, a2, a3, b2, b3);
+        for (int b = 0; b < 4; ++b) {
+          // (a missing block's f is negative and its entries +inf: their products are -inf too)
+          float t0 = f[b] < 0.f ? INFINITY : -INFINITY, t1 = t0, t2 = t0, t3 = t0;
+          if (f[b] >= 0.f) {
+#pragma unroll
+            for (int k = 0; k < kBlock; k += 4) {
+              t0 = fmaxf(t0, __uint_as_float(s[b * 16 + k]));
+              t1 = fmaxf(t1, __uint_as_float(s[b * 16 + k + 1]));
+              t2 = fmaxf(t2, __uint_as_float(s[b * 16 + k + 2]));
+              t3 = fmaxf(t3, __uint_as_float(s[b * 16 + k + 3]));
+            }
+          }
+          const float x = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * f[b];
+          mx = fmaxf(mx, x);
+          mz = fmaxf(mz, x + ev[b]);
+        }
+        if (mx > m + 8.f) {
+          l *= ex2(m - mx);
+          m = mx;
+        }
+        const bool up = mz > mw + 8.f;
+        if (j > 0 && !wait_for(&sh.odone, (j - 1) & 1, p.status, abort)) stop = true;
+        stop = __any_sync(kAll, stop);
+        if (!stop && __any_sync(kAll, up)) {
+          const float to = up ? mz : mw;
+          if (j > 0) {
+            const float down = mw == -INFINITY ? (up ? 0.f : 1.f) : ex2(mw - to);
+            fence_after();
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_load(tmem_o + lanes + c, o);
+              wait_loads(o);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
+              tmem_store(tmem_o + lanes + c, o);
+            }
+            wait_stores();
+          }
+          mw = to;
+        }
+        if (!stop) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const float add = mw == -INFINITY ? 0.f : ev[b] - mw;  // (nothing seen yet: every entry is -inf)
+            const float ratio = m - mw + ev[b];  // log2 of weight over probability
+            float sum = 0.f;
+            if (__any_sync(kAll, ratio < -90.f)) {  // the weights may have underflowed: sum the probabilities themselves
+#pragma unroll
+              for (int k = 0; k < kBlock; ++k) {
+                const float x = __uint_as_float(s[b * 16 + k]) * f[b];
+                l += x == -INFINITY ? 0.f : ex2(x - m);
+              }
+            }
+            uint32_t w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float w0 = ex2(fmaf(__uint_as_float(s[b * 16 + 2 * k]), f[b], add));
+              const float w1 = ex2(fmaf(__uint_as_float(s[b * 16 + 2 * k + 1]), f[b], add));
+              sum += w0 + w1;
+              w[k] = pack_f16x2(w0, w1);
+            }
+            if (!__any_sync(kAll, ratio < -90.f) && mw != -INFINITY) l += sum * ex2(-ratio);
+            uint8_t* dst = smem + T::OFF_P + r * 128;
+            *reinterpret_cast<uint4*>(dst + (((2 * b) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(dst + (((2 * b + 1) ^ (r & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+        }
+      } else {
+        mbar_arrive(&sh.sfree[j & 1]);
+        stop = j > 0 && !__all_sync(kAll, wait_for(&sh.odone, (j - 1) & 1, p.status, abort));
+      }
+      if (stop) break;
+      fence_before();
+      fence_proxy_async_shared();
+      mbar_arrive(&sh.pfull);
+    }
+    if (rows_here && __all_sync(kAll, wait_for(&sh.odone, (steps - 1) & 1, p.status, abort))) {
+      fence_after();
+      const float g = l > 0.f ? ex2(mw - m) / l : (l == 0.f ? 0.f : l);
+      __nv_bfloat16* dst = p.out + (int64_t)(me.row0 + (mine ? r : 0)) * p.out_stride + (int64_t)head * D;
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        tmem_load(tmem_o + lanes + c, o);
+        wait_loads(o);
+        if (mine) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = pack_bf16x2(__uint_as_float(o[k + 2 * e]) * g, __uint_as_float(o[k + 2 * e + 1]) * g);
+            *reinterpret_cast<uint4*>(dst + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      // NaN that were taken out of V: back into the rows that see them, dim by dim (rare, so from global memory)
+      const int32_t* bt = p.block_table + (int64_t)me.slot * p.bt_stride;
+      for (int i = 0; i < kDiagonal; ++i) {
+        for (unsigned long long bits = sh.nan[i]; bits; bits &= bits - 1) {
+          const int key = (diagonal + i) * TK + __ffsll((long long)bits) - 1;
+          if (!mine || key > qpos) continue;
+          const int64_t at = (int64_t)p.num_blocks * p.kv_heads + (int64_t)bt[key / kBlock] * p.kv_heads + kvh;
+          const uint8_t* v = p.codes + at * T::BLK + (key % kBlock) * D;
+          for (int d = 0; d < D; ++d)
+            if ((v[d] & 0x7fu) == 0x7fu) dst[d] = f_to_bf16(NAN);
+        }
       }
     }
   }
-
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(kAll, l[r], 1);
-    l[r] += __shfl_xor_sync(kAll, l[r], 2);
-    if (qr[r] >= nrows) continue;
-    const float f = l[r] > 0.f ? ex2(mw[r] - m[r]) / l[r] : (l[r] == 0.f ? 0.f : l[r]);
-    __nv_bfloat16* dst = p.out + (int64_t)(row0 + qr[r]) * p.out_stride + (int64_t)head * D + 2 * t;
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-      *reinterpret_cast<uint32_t*>(dst + j * 8) = pack_bf16x2(o[j][2 * r] * f, o[j][2 * r + 1] * f);
-  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 4)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
 template <int D>
-static int launch_prefill(const PrefillParams& p, int num_heads, int num_tiles, cudaStream_t st) {
-  constexpr int SMEM = 2 * TK * RowPitch<D>::BYTES + 2 * 8 * kBlock * D;
-  if (cudaFuncSetAttribute(prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess)
+static int launch_prefill(const PrefillParams& p, int num_heads, cudaStream_t st) {
+  if (cudaFuncSetAttribute(prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<D>::SMEM) != cudaSuccess)
     return CDB_ERR_CUDA;
-  launch_pdl(prefill_kernel<D>, dim3(num_heads, num_tiles), dim3(128), SMEM, st, p);
-  return cudaPeekAtLastError() == cudaSuccess ? CDB_OK : CDB_ERR_CUDA;
+  return launch_pdl(prefill_kernel<D>, dim3(num_heads, p.num_tiles), dim3(kPrefillThreads), Tile<D>::SMEM, st, p) ==
+                 cudaSuccess
+             ? CDB_OK
+             : CDB_ERR_CUDA;
 }
 
 }  // namespace kv8
@@ -359,7 +651,7 @@ extern "C" int cdb_kv8_prefill_attention(const void* q, int64_t q_stride, void* 
   using namespace cdb::kv8;
   if (codes == nullptr || scales == nullptr || (reinterpret_cast<uintptr_t>(codes) & 15) || cache_layer < 0 ||
       cache_layer >= num_cache_layers || num_blocks <= 0 || num_rows < 0 || num_tiles < 0 || num_tiles > 65535 ||
-      num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads != 0 || table_rows < 0 || table_width < 0)
+      num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads != 0 || table_rows < 0 || table_width < 0 || !(scale > 0.f) || scale > 1e30f)
     return CDB_ERR_INVALID_ARGUMENT;
   if (head_dim != 64 && head_dim != 96 && head_dim != 128) return CDB_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(q) & 15) || (q_stride & 7) || (reinterpret_cast<uintptr_t>(out) & 15) ||
@@ -383,11 +675,12 @@ extern "C" int cdb_kv8_prefill_attention(const void* q, int64_t q_stride, void* 
   p.bt_rows = table_rows;
   p.bt_width = table_width;
   p.tiles = static_cast<const int4*>(tiles);
+  p.num_tiles = num_tiles;
   p.num_rows = num_rows;
   p.scale_log2 = scale * kLog2e;
   p.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128) return launch_prefill<128>(p, num_heads, num_tiles, st);
-  if (head_dim == 96) return launch_prefill<96>(p, num_heads, num_tiles, st);
-  return launch_prefill<64>(p, num_heads, num_tiles, st);
+  if (head_dim == 128) return launch_prefill<128>(p, num_heads, st);
+  if (head_dim == 96) return launch_prefill<96>(p, num_heads, st);
+  return launch_prefill<64>(p, num_heads, st);
 }

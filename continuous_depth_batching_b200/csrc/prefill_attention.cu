@@ -9,7 +9,6 @@
 // fp32 accumulation) with a base-2 online softmax in registers. Every K/V page is read once per
 // 64 queries instead of once per query.
 #include "cdb_common.cuh"
-#include "smem_tile.cuh"
 
 namespace cdb {
 namespace prefill {
@@ -35,6 +34,21 @@ struct Params {
   int32_t* status;
 };
 
+// Shared-memory row pitch of a [rows][D] bf16 tile. D = 64/128: rows of D*2 bytes with the
+// 16-byte chunk index XOR-swizzled by r % 8 (rows hold whole groups of 8 chunks). D = 96: 12
+// chunks per row do not form whole groups, so rows are padded to 13 chunks (208 bytes) instead;
+// the 8 rows one ldmatrix phase reads then start in distinct bank groups ((13 r + c) mod 8).
+template <int D>
+struct RowPitch {
+  static constexpr int BYTES = (D == 96) ? 208 : D * 2;
+  static constexpr bool XOR = (D != 96);
+};
+
+template <int D>
+__device__ __forceinline__ uint32_t swz(int r, int c) {
+  return (uint32_t)(r * RowPitch<D>::BYTES + ((RowPitch<D>::XOR ? (c ^ (r & 7)) : c) << 4));
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   const int n = valid ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
@@ -43,6 +57,17 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr));
 }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,

@@ -209,11 +209,16 @@ void kv8_gather(const Tensor& codes, const Tensor& scales, int64_t cache_layer, 
         "cdb_kv8_gather");
 }
 
+void check_scale(double scale) {
+  TORCH_CHECK_VALUE(scale > 0 && scale <= 1e30, "scale must be positive and finite, got ", scale);
+}
+
 void kv8_decode_attention(const Tensor& q, const Tensor& out, const Tensor& codes, const Tensor& scales,
                           int64_t cache_layer, const Tensor& block_table, const Tensor& item_slot,
                           const Tensor& item_pos, int64_t num_heads, double scale) {
   const Cache c = check_cache(codes, scales, cache_layer);
   check_heads(num_heads, c.heads);
+  check_scale(scale);
   const int64_t n = item_pos.numel();
   check_rows("q", q, n, num_heads * c.dim);
   check_rows("out", out, n, num_heads * c.dim);
@@ -240,6 +245,7 @@ void kv8_prefill_attention(const Tensor& q, const Tensor& out, const Tensor& cod
                            double scale) {
   const Cache c = check_cache(codes, scales, cache_layer);
   check_heads(num_heads, c.heads);
+  check_scale(scale);
   check_rows("q", q, 0, num_heads * c.dim);
   check_rows("out", out, q.size(0), num_heads * c.dim);
   check_table(block_table);

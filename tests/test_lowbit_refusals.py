@@ -108,6 +108,8 @@ def test_append_refuses(what, args):
     ("q must be", _decode_args(heads=6)),
     ("out must be", _decode_args(out=torch.zeros(2, 256, dtype=BF))),
     ("item_pos must be", _decode_args(pos=_ints(6)[::2])),
+    ("scale must be positive", _decode_args(scale=0.0)),
+    ("scale must be positive", _decode_args(scale=float("nan"))),
     ("scales must be", _decode_args(scales=torch.zeros(1, 2, 4, 2, dtype=torch.float64))),
 ])
 def test_decode_refuses(what, args):
@@ -118,6 +120,7 @@ def test_decode_refuses(what, args):
 @pytest.mark.parametrize("what,args", [
     ("tiles must be", _prefill_args(tiles=_ints(2, 3))),
     ("tiles must be", _prefill_args(tiles=_ints(2, 4, dtype=torch.int64))),
+    ("scale must be positive", _prefill_args(scale=-0.125)),
     ("65535 tiles", _prefill_args(tiles=_ints(65536, 4))),
     ("out must be", _prefill_args(out=torch.zeros(2, 256, dtype=BF))),
     ("multiple of the cache's 2 kv heads", _prefill_args(heads=5)),
