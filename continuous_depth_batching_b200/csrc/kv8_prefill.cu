@@ -82,7 +82,7 @@ struct Shared {
   uint64_t pfull, odone;     // weights written / O product done with them and with V
   uint64_t meta[kMeta];      // a step's scales written
   uint64_t drain;
-  alignas(16) float scale[kMeta][2][4];  // K's scale (< 0: no such block), log2 of V's
+  alignas(16) float scale[kMeta][2][4];  // K's (< 0: no such block) and V's
   unsigned long long nan[kDiagonal];
   uint32_t tmem;
   int abort;
@@ -94,6 +94,14 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar)
                : "memory");
+}
+
+// 4 bytes to shared memory, asynchronously; async_arrive lets `bar` count their completion.
+__device__ __forceinline__ void async_copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // Matrix descriptor of a K-major operand in 128-byte swizzled rows of 64 f16, 8-row groups 1024 bytes apart.
@@ -268,35 +276,31 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
     const int64_t v_tiles = (int64_t)p.num_blocks * p.kv_heads;
     // Threads 0..3 bring one block of every step each, its id a step ahead of its copies.
     int id = -1;
-    float hold_k = -1.f, hold_v = 1.f;
     auto fetch_id = [&](int step) {
       const int b = step * 4 + ct;
       id = step < steps && b < blocks ? bt[b] : -1;
     };
     auto issue = [&](int step) {
       if (step >= steps) return;
-      uint64_t* bar = &sh.staged[step & 1];
+      uint64_t *bar = &sh.staged[step & 1], *meta = &sh.meta[step & (kMeta - 1)];
+      float(&scale)[2][4] = sh.scale[step & (kMeta - 1)];
       const bool used = step * 4 + ct < blocks;
-      hold_k = -1.f;
-      hold_v = 1.f;
       if (used && id >= 0 && id < p.num_blocks) {
         const int64_t at = (int64_t)id * p.kv_heads + kvh;
         mbar_arrive_expect_tx(bar, 2 * T::BLK);
         bulk_copy(base + T::OFF_SK + ((step & 1) * 4 + ct) * T::BLK, p.codes + at * T::BLK, T::BLK, smem_u32(bar));
         bulk_copy(base + T::OFF_SV + ((step & 1) * 4 + ct) * T::VBLK, p.codes + (v_tiles + at) * T::BLK, T::BLK,
                   smem_u32(bar));
-        hold_k = p.scales[at];
-        hold_v = p.scales[v_tiles + at];
+        async_copy4(smem_u32(&scale[0][ct]), p.scales + at);
+        async_copy4(smem_u32(&scale[1][ct]), p.scales + v_tiles + at);
+        async_arrive(smem_u32(meta));
       } else {
         if (used) set_error(p.status, CDB_ERR_INDEX);
+        scale[0][ct] = -1.f;
+        scale[1][ct] = 1.f;
+        mbar_arrive(meta);
         mbar_arrive(bar);
       }
-    };
-    auto post = [&](int step) {  // the scales that issue(step) fetched
-      if (step >= steps) return;
-      sh.scale[step & (kMeta - 1)][0][ct] = hold_k;
-      sh.scale[step & (kMeta - 1)][1][ct] = hold_v > 0.f ? __log2f(hold_v) : -126.f;
-      mbar_arrive(&sh.meta[step & (kMeta - 1)]);
     };
     // K of step j into place: 16 codes of a key at a time; a quarter warp covers four chunks of two keys.
     auto convert_k = [&](int j) {
@@ -384,59 +388,67 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
       return all != 0u;
     };
 
+    // K of step n (its codes have landed and K's place is free) and its product S.
+    auto scores = [&](int n, bool ok) {
+      ok = ok && wait_for(&sh.staged[n & 1], (n >> 1) & 1, p.status, abort);
+      if (n > 0) ok = ok && wait_for(&sh.sfull[(n - 1) & 1], ((n - 1) >> 1) & 1, p.status, abort);
+      if (ok) convert_k(n);
+      ok = hand_over(ok);
+      if (ct == 0 && ok) {
+        ok = wait_for(&sh.sfree[n & 1], (n >> 1) & 1, p.status, abort);
+        if (ok) {
+          fence_after();
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            product(tmem + (n & 1) * TK, base + T::OFF_Q + (kk >> 2) * (TM * 128) + (kk & 3) * 32,
+                    base + T::OFF_K + (kk >> 2) * (TK * 128) + (kk & 3) * 32, kIdescS, kk > 0);
+          commit(&sh.sfull[n & 1]);
+        }
+      }
+      return ok;
+    };
+    // V of step n into place (free by now); then nobody needs the step's codes any more.
+    auto values = [&](int n, bool ok) {
+      ok = ok && wait_for(&sh.meta[n & (kMeta - 1)], (n / kMeta) & 1, p.status, abort);
+      if (ok) convert_v(n);
+      ok = hand_over(ok);
+      if (ct < 4) {
+        issue(n + 2);
+        fetch_id(n + 3);
+      }
+      return ok;
+    };
+
     if (ct < 4) {
       fetch_id(0);
       issue(0);
-      post(0);
       fetch_id(1);
       issue(1);
       fetch_id(2);
     }
     int announced = min(2, steps);
-    bool ok = true;
-    // Step j: K of step j + 1 and its product S, then the product O of step j, then V of step j + 1.
-    for (int j = -1; j < steps && ok; ++j) {
-      const int n = j + 1;
-      if (n < steps) {
-        ok = wait_for(&sh.staged[n & 1], (n >> 1) & 1, p.status, abort);
-        if (ct < 4) post(n + 1);
-        ok = ok && wait_for(&sh.meta[n & (kMeta - 1)], (n / kMeta) & 1, p.status, abort);
-        if (j >= 0) ok = ok && wait_for(&sh.sfull[j & 1], (j >> 1) & 1, p.status, abort);  // K's place is free
-        if (ok) convert_k(n);
-        ok = hand_over(ok);
-        if (ct == 0 && ok) {
-          ok = wait_for(&sh.sfree[n & 1], (n >> 1) & 1, p.status, abort);
-          if (ok) {
-            fence_after();
+    bool ok = scores(0, true);
+    if (steps > 1) ok = scores(1, ok);
+    ok = values(0, ok);
+    announced = min(3, steps);
+    // Step j: its product O as soon as its weights are there, meanwhile K of step j + 2 (whose S buffer the
+    // softmax of step j has read) and the product S, then V of step j + 1.
+    for (int j = 0; j < steps && ok; ++j) {
+      if (ct == 0) {
+        ok = wait_for(&sh.pfull, j & 1, p.status, abort);
+        if (ok) {
+          fence_after();
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              product(tmem + (n & 1) * TK, base + T::OFF_Q + (kk >> 2) * (TM * 128) + (kk & 3) * 32,
-                      base + T::OFF_K + (kk >> 2) * (TK * 128) + (kk & 3) * 32, kIdescS, kk > 0);
-            commit(&sh.sfull[n & 1]);
-          }
+          for (int kk = 0; kk < TK / 16; ++kk)
+            product(tmem_o, base + T::OFF_P + kk * 32, base + T::OFF_V + kk * 32, kIdescO, j > 0 || kk > 0);
+          commit(&sh.odone);
         }
       }
-      if (j >= 0) {
-        if (ct == 0 && ok) {
-          ok = wait_for(&sh.pfull, j & 1, p.status, abort);
-          if (ok) {
-            fence_after();
-#pragma unroll
-            for (int kk = 0; kk < TK / 16; ++kk)
-              product(tmem_o, base + T::OFF_P + kk * 32, base + T::OFF_V + kk * 32, kIdescO, j > 0 || kk > 0);
-            commit(&sh.odone);
-          }
-        }
-        ok = ok && wait_for(&sh.odone, j & 1, p.status, abort);  // V's place is free
-      }
-      if (n < steps) {
-        if (ok) convert_v(n);
-        ok = hand_over(ok);  // and this step's codes have been read
-        if (ct < 4) {
-          issue(n + 2);
-          fetch_id(n + 3);
-        }
-        announced = min(n + 3, steps);
+      if (j + 2 < steps) ok = scores(j + 2, ok);
+      ok = ok && wait_for(&sh.odone, j & 1, p.status, abort);  // V's place is free
+      if (j + 1 < steps) {
+        ok = values(j + 1, ok);
+        announced = min(j + 4, steps);
       }
     }
     if (!ok)  // the copies in flight, after an abort; a step that has landed passes at once or runs into the limit
@@ -501,7 +513,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
         // logits are S * f; f stays above 0 (an all-zero block under a tiny q), below it no such block
         const float f[4] = {ks.x < 0.f ? -1.f : fmaxf(factor * ks.x, 1.2e-38f), ks.y < 0.f ? -1.f : fmaxf(factor * ks.y, 1.2e-38f),
                             ks.z < 0.f ? -1.f : fmaxf(factor * ks.z, 1.2e-38f), ks.w < 0.f ? -1.f : fmaxf(factor * ks.w, 1.2e-38f)};
-        const float ev[4] = {vs.x, vs.y, vs.z, vs.w};
+        const float ev[4] = {vs.x > 0.f ? __log2f(vs.x) : -126.f, vs.y > 0.f ? __log2f(vs.y) : -126.f,
+                             vs.z > 0.f ? __log2f(vs.z) : -126.f, vs.w > 0.f ? __log2f(vs.w) : -126.f};
         if (j >= diagonal || f[0] < 0.f || f[1] < 0.f || f[2] < 0.f || f[3] < 0.f) {
           const int seen = qpos - j * TK;  // the last key of the step that the row sees
 #pragma unroll
@@ -552,30 +565,32 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
           mw = to;
         }
         if (!stop) {
+          const float off = m - mw;  // log2 of weight over probability, but for the block's log2 s_v
+          const bool far = __any_sync(kAll, off + fminf(fminf(ev[0], ev[1]), fminf(ev[2], ev[3])) < -90.f);
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
             const float add = mw == -INFINITY ? 0.f : ev[b] - mw;  // (nothing seen yet: every entry is -inf)
-            const float ratio = m - mw + ev[b];  // log2 of weight over probability
-            float sum = 0.f;
-            if (__any_sync(kAll, ratio < -90.f)) {  // the weights may have underflowed: sum the probabilities themselves
-#pragma unroll
-              for (int k = 0; k < kBlock; ++k) {
-                const float x = __uint_as_float(s[b * 16 + k]) * f[b];
-                l += x == -INFINITY ? 0.f : ex2(x - m);
-              }
-            }
+            float sum = 0.f, more = 0.f;
             uint32_t w[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const float w0 = ex2(fmaf(__uint_as_float(s[b * 16 + 2 * k]), f[b], add));
               const float w1 = ex2(fmaf(__uint_as_float(s[b * 16 + 2 * k + 1]), f[b], add));
-              sum += w0 + w1;
+              sum += w0;
+              more += w1;
               w[k] = pack_f16x2(w0, w1);
             }
-            if (!__any_sync(kAll, ratio < -90.f) && mw != -INFINITY) l += sum * ex2(-ratio);
             uint8_t* dst = smem + T::OFF_P + r * 128;
             *reinterpret_cast<uint4*>(dst + (((2 * b) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             *reinterpret_cast<uint4*>(dst + (((2 * b + 1) ^ (r & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+            if (!far) l += mw == -INFINITY ? 0.f : (sum + more) * ex2(-off - ev[b]);
+          }
+          if (far) {  // rare: the weights may have underflowed, so the probabilities are summed themselves
+#pragma unroll
+            for (int k = 0; k < TK; ++k) {
+              const float x = __uint_as_float(s[k]) * f[k >> 4];
+              l += x == -INFINITY ? 0.f : ex2(x - m);
+            }
           }
         }
       } else {
