@@ -6,10 +6,10 @@
 // long chunk fills the tensor core's 128 rows; a lone tile leaves half of them idle). Keys come in steps of
 // 64 (4 blocks). Roles:
 //   warps 0..3  softmax: thread r owns query row r, so its maximum, sum and weights need no exchange;
-//   warps 4..7  bring the codes (bulk copies of whole (block, head) tiles, two steps ahead) and turn them into
-//               f16, exactly, in the tensor core's layout: K as it lies, V transposed. One of their threads
-//               issues the products: S = Q K^T (128 x 64 x D) one step ahead of O += P V (128 x D x 64), both
-//               tcgen05 with f16 operands in shared memory and fp32 accumulators in tensor memory.
+//   warps 4, 5  keys: bring the codes (bulk copies of whole (block, head) tiles, two steps ahead), turn them
+//               into f16, exactly, and issue S = Q K^T (128 x 64 x D), two steps ahead of the softmax;
+//   warps 6, 7  values: the same with a transposition, and O += P V (128 x D x 64).
+// Both products are tcgen05 with f16 operands in shared memory and fp32 accumulators in tensor memory.
 // Two CTAs share an SM (256 of its 512 tensor-memory columns, 113 KB of shared memory each): one computes
 // exponentials while the other multiplies.
 //
@@ -32,9 +32,9 @@ namespace kv8 {
 constexpr int TR = 64;   // rows of a listed tile
 constexpr int TM = 128;  // rows of a CTA
 constexpr int TK = 64;   // keys of a step
-constexpr int kSoftmax = 128, kConvert = 128;
-constexpr int kPrefillThreads = kSoftmax + kConvert;
-constexpr int kMeta = 4;            // steps whose scales are kept
+constexpr int kSoftmax = 128, kConvert = 64;  // threads of the softmax, of the keys and of the values
+constexpr int kPrefillThreads = kSoftmax + 2 * kConvert;
+constexpr int kMeta = 8;            // steps whose scales are kept (keys run up to five steps ahead of the softmax)
 constexpr int kDiagonal = 3;        // steps that the diagonal of 128 rows can cross
 constexpr int kPairLimit = 2048;    // longest tile list that every CTA searches for its neighbours
 constexpr uint32_t kTmemCols = 256;
@@ -76,13 +76,13 @@ struct Tile {
 
 // Barriers and small state behind the tiles.
 struct Shared {
-  uint64_t staged[2];        // a step's copies have landed (4 threads announce them)
+  uint64_t staged_k[2], staged_v[2];  // a step's codes have landed (4 threads announce them)
   uint64_t sfull[2];         // S product done: S in tensor memory, K's place free
   uint64_t sfree[2];         // S read (first: q written)
   uint64_t pfull, odone;     // weights written / O product done with them and with V
   uint64_t meta[kMeta];      // a step's scales written
-  uint64_t drain;
-  alignas(16) float scale[kMeta][2][4];  // K's (< 0: no such block) and V's
+  uint64_t drain[2];         // all products done
+  alignas(16) float scale[kMeta][2][4];  // K's and V's; < 0: no such block
   unsigned long long nan[kDiagonal];
   uint32_t tmem;
   int abort;
@@ -228,14 +228,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.staged[i], 4);
+      mbar_init(&sh.staged_k[i], 4);
+      mbar_init(&sh.staged_v[i], 4);
+      mbar_init(&sh.drain[i], 1);
       mbar_init(&sh.sfull[i], 1);
       mbar_init(&sh.sfree[i], kSoftmax);
     }
-    for (int i = 0; i < kMeta; ++i) mbar_init(&sh.meta[i], 4);
+    for (int i = 0; i < kMeta; ++i) mbar_init(&sh.meta[i], 8);
     mbar_init(&sh.pfull, kSoftmax);
     mbar_init(&sh.odone, 1);
-    mbar_init(&sh.drain, 1);
     for (int i = 0; i < kDiagonal; ++i) sh.nan[i] = 0ull;
     for (int i = 0; i < 4; ++i) sh.found[i] = 0;
     sh.abort = (base & 1023u) != 0u;  // the swizzle counts on it
@@ -271,33 +272,35 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
 
   if (warp >= 4) {
     // ------------------------------------------------------------ codes to f16, and the products
-    const int ct = tid - kSoftmax, cw = warp - 4;
+    const bool values = warp >= 6;
+    const int ct = (tid - kSoftmax) & (kConvert - 1), cw = warp & 1;
     const int32_t* bt = p.block_table + (int64_t)me.slot * p.bt_stride;
-    const int64_t v_tiles = (int64_t)p.num_blocks * p.kv_heads;
-    // Threads 0..3 bring one block of every step each, its id a step ahead of its copies.
+    const int64_t first_tile = values ? (int64_t)p.num_blocks * p.kv_heads : 0;
+    uint64_t* staged = values ? sh.staged_v : sh.staged_k;
+    // Lanes 0..3 of the second warp (the first issues the products) bring one block of every step each, its
+    // id a step ahead of its copies.
+    const bool brings = cw == 1 && lane < 4;
     int id = -1;
     auto fetch_id = [&](int step) {
-      const int b = step * 4 + ct;
+      const int b = step * 4 + lane;
       id = step < steps && b < blocks ? bt[b] : -1;
     };
     auto issue = [&](int step) {
       if (step >= steps) return;
-      uint64_t *bar = &sh.staged[step & 1], *meta = &sh.meta[step & (kMeta - 1)];
-      float(&scale)[2][4] = sh.scale[step & (kMeta - 1)];
-      const bool used = step * 4 + ct < blocks;
+      uint64_t *bar = &staged[step & 1], *meta = &sh.meta[step & (kMeta - 1)];
+      float* scale = &sh.scale[step & (kMeta - 1)][values][lane];
+      const bool used = step * 4 + lane < blocks;
       if (used && id >= 0 && id < p.num_blocks) {
-        const int64_t at = (int64_t)id * p.kv_heads + kvh;
-        mbar_arrive_expect_tx(bar, 2 * T::BLK);
-        bulk_copy(base + T::OFF_SK + ((step & 1) * 4 + ct) * T::BLK, p.codes + at * T::BLK, T::BLK, smem_u32(bar));
-        bulk_copy(base + T::OFF_SV + ((step & 1) * 4 + ct) * T::VBLK, p.codes + (v_tiles + at) * T::BLK, T::BLK,
-                  smem_u32(bar));
-        async_copy4(smem_u32(&scale[0][ct]), p.scales + at);
-        async_copy4(smem_u32(&scale[1][ct]), p.scales + v_tiles + at);
+        const int64_t at = first_tile + (int64_t)id * p.kv_heads + kvh;
+        const uint32_t place = (step & 1) * 4 + lane;
+        mbar_arrive_expect_tx(bar, T::BLK);
+        bulk_copy(base + (values ? T::OFF_SV + place * T::VBLK : T::OFF_SK + place * T::BLK), p.codes + at * T::BLK,
+                  T::BLK, smem_u32(bar));
+        async_copy4(smem_u32(scale), p.scales + at);
         async_arrive(smem_u32(meta));
       } else {
         if (used) set_error(p.status, CDB_ERR_INDEX);
-        scale[0][ct] = -1.f;
-        scale[1][ct] = 1.f;
+        *scale = -1.f;
         mbar_arrive(meta);
         mbar_arrive(bar);
       }
@@ -306,7 +309,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
     auto convert_k = [&](int j) {
       constexpr int C = D / 16;  // chunks of a key
       const uint8_t* src = smem + T::OFF_SK + (j & 1) * 4 * T::BLK;
-#pragma unroll
+#pragma unroll 4
       for (int i0 = 0; i0 < TK * C; i0 += kConvert) {
         const int i = i0 + ct;
         int key, c;
@@ -333,9 +336,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
     // of dims.
     auto convert_v = [&](int j) {
       const int b = lane & 3;
-      const bool have = sh.scale[j & (kMeta - 1)][0][b] >= 0.f;
+      const bool have = sh.scale[j & (kMeta - 1)][1][b] >= 0.f;
 #pragma unroll 1
-      for (int u = cw; u < 2 * (D / 32); u += 4) {
+      for (int u = cw; u < 2 * (D / 32); u += 2) {
         const int half = u & 1, d0 = (u >> 1) * 32 + (lane >> 2) * 4;
         const uint8_t* src = smem + T::OFF_SV + ((j & 1) * 4 + b) * T::VBLK + half * 8 * D + d0;
         const int key0 = b * kBlock + half * 8;
@@ -375,51 +378,20 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
         }
       }
     };
-    // What the converting threads wrote is the products' to read; true if all of them are well.
+    // What the two warps wrote is the products' to read; true if all of their threads are well.
     auto hand_over = [&](bool mine) {
       fence_proxy_async_shared();
       uint32_t all;
       asm volatile(
-          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, %2, p;\n\t"
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, %3, %2, p;\n\t"
           "selp.u32 %0, 1, 0, q;\n\t}"
           : "=r"(all)
-          : "r"((uint32_t)mine), "n"(kConvert)
+          : "r"((uint32_t)mine), "n"(kConvert), "r"(values ? 2 : 1)
           : "memory");
       return all != 0u;
     };
 
-    // K of step n (its codes have landed and K's place is free) and its product S.
-    auto scores = [&](int n, bool ok) {
-      ok = ok && wait_for(&sh.staged[n & 1], (n >> 1) & 1, p.status, abort);
-      if (n > 0) ok = ok && wait_for(&sh.sfull[(n - 1) & 1], ((n - 1) >> 1) & 1, p.status, abort);
-      if (ok) convert_k(n);
-      ok = hand_over(ok);
-      if (ct == 0 && ok) {
-        ok = wait_for(&sh.sfree[n & 1], (n >> 1) & 1, p.status, abort);
-        if (ok) {
-          fence_after();
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            product(tmem + (n & 1) * TK, base + T::OFF_Q + (kk >> 2) * (TM * 128) + (kk & 3) * 32,
-                    base + T::OFF_K + (kk >> 2) * (TK * 128) + (kk & 3) * 32, kIdescS, kk > 0);
-          commit(&sh.sfull[n & 1]);
-        }
-      }
-      return ok;
-    };
-    // V of step n into place (free by now); then nobody needs the step's codes any more.
-    auto values = [&](int n, bool ok) {
-      ok = ok && wait_for(&sh.meta[n & (kMeta - 1)], (n / kMeta) & 1, p.status, abort);
-      if (ok) convert_v(n);
-      ok = hand_over(ok);
-      if (ct < 4) {
-        issue(n + 2);
-        fetch_id(n + 3);
-      }
-      return ok;
-    };
-
-    if (ct < 4) {
+    if (brings) {
       fetch_id(0);
       issue(0);
       fetch_id(1);
@@ -427,35 +399,63 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
       fetch_id(2);
     }
     int announced = min(2, steps);
-    bool ok = scores(0, true);
-    if (steps > 1) ok = scores(1, ok);
-    ok = values(0, ok);
-    announced = min(3, steps);
-    // Step j: its product O as soon as its weights are there, meanwhile K of step j + 2 (whose S buffer the
-    // softmax of step j has read) and the product S, then V of step j + 1.
-    for (int j = 0; j < steps && ok; ++j) {
-      if (ct == 0) {
-        ok = wait_for(&sh.pfull, j & 1, p.status, abort);
-        if (ok) {
-          fence_after();
+    // `go` is the same in all of the two warps' threads: they pass their barrier together or not at all.
+    bool go = true, ok = true;
+    if (!values) {
+      for (int n = 0; n < steps && go; ++n) {
+        ok = ok && wait_for(&staged[n & 1], (n >> 1) & 1, p.status, abort);
+        if (n > 0) ok = ok && wait_for(&sh.sfull[(n - 1) & 1], ((n - 1) >> 1) & 1, p.status, abort);  // K's place is free
+        if (ok) convert_k(n);
+        go = ok = hand_over(ok);
+        if (brings) {  // this step's codes have been read
+          issue(n + 2);
+          fetch_id(n + 3);
+        }
+        announced = min(n + 3, steps);
+        if (ct == 0 && ok) {
+          ok = wait_for(&sh.sfree[n & 1], (n >> 1) & 1, p.status, abort);
+          if (ok) {
+            fence_after();
 #pragma unroll
-          for (int kk = 0; kk < TK / 16; ++kk)
-            product(tmem_o, base + T::OFF_P + kk * 32, base + T::OFF_V + kk * 32, kIdescO, j > 0 || kk > 0);
-          commit(&sh.odone);
+            for (int kk = 0; kk < D / 16; ++kk)
+              product(tmem + (n & 1) * TK, base + T::OFF_Q + (kk >> 2) * (TM * 128) + (kk & 3) * 32,
+                      base + T::OFF_K + (kk >> 2) * (TK * 128) + (kk & 3) * 32, kIdescS, kk > 0);
+            commit(&sh.sfull[n & 1]);
+          }
         }
       }
-      if (j + 2 < steps) ok = scores(j + 2, ok);
-      ok = ok && wait_for(&sh.odone, j & 1, p.status, abort);  // V's place is free
-      if (j + 1 < steps) {
-        ok = values(j + 1, ok);
-        announced = min(j + 4, steps);
+    } else {
+      for (int j = -1; j < steps && go; ++j) {
+        if (j >= 0 && ct == 0) {
+          ok = wait_for(&sh.pfull, j & 1, p.status, abort);
+          if (ok) {
+            fence_after();
+#pragma unroll
+            for (int kk = 0; kk < TK / 16; ++kk)
+              product(tmem_o, base + T::OFF_P + kk * 32, base + T::OFF_V + kk * 32, kIdescO, j > 0 || kk > 0);
+            commit(&sh.odone);
+          }
+        }
+        const int n = j + 1;
+        if (n < steps) {
+          ok = ok && wait_for(&staged[n & 1], (n >> 1) & 1, p.status, abort) &&
+               wait_for(&sh.meta[n & (kMeta - 1)], (n / kMeta) & 1, p.status, abort);
+          if (j >= 0) ok = ok && wait_for(&sh.odone, j & 1, p.status, abort);  // V's place is free
+          if (ok) convert_v(n);
+          go = ok = hand_over(ok);
+          if (brings) {
+            issue(n + 2);
+            fetch_id(n + 3);
+          }
+          announced = min(n + 3, steps);
+        }
       }
     }
     if (!ok)  // the copies in flight, after an abort; a step that has landed passes at once or runs into the limit
-      for (int j = max(0, announced - 2); j < announced; ++j) mbar_wait(&sh.staged[j & 1], (j >> 1) & 1, p.status);
+      for (int j = max(0, announced - 2); j < announced; ++j) mbar_wait(&staged[j & 1], (j >> 1) & 1, p.status);
     if (ct == 0) {
-      commit(&sh.drain);  // on every path: no product may run when the tensor memory is freed
-      mbar_wait(&sh.drain, 0, p.status);
+      commit(&sh.drain[values]);  // on every path: no product may run when the tensor memory is freed
+      mbar_wait(&sh.drain[values], 0, p.status);
     }
     __syncwarp();
   } else {
