@@ -172,6 +172,8 @@ __device__ __forceinline__ void wait_stores() { asm volatile("tcgen05.wait::st.s
 
 // Bounded wait that also gives up once another role has.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int32_t* status, volatile int* abort) {
+  if (mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
   for (uint32_t i = 0; i < kSpinLimit; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((i & 255u) == 255u && *abort) return false;
@@ -317,7 +319,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
     auto convert_k = [&](int j) {
       constexpr int C = D / 16;  // chunks of a key
       const uint8_t* src = smem + T::OFF_SK + (j & 1) * 4 * T::BLK;
-#pragma unroll 4
+#pragma unroll
       for (int i0 = 0; i0 < TK * C; i0 += kConvert) {
         const int i = i0 + ct;
         int key, c;
@@ -345,7 +347,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
     auto convert_v = [&](int j) {
       const int b = lane & 3;
       const bool have = sh.scale[j & (kMeta - 1)][1][b] >= 0.f;
-#pragma unroll 1
+      const bool full = kv_len - j * TK >= TK && __all_sync(kAll, have);
+#pragma unroll 2
       for (int u = cw; u < 2 * (D / 32); u += 2) {
         const int half = u & 1, d0 = (u >> 1) * 32 + (lane >> 2) * 4;
         const uint8_t* src = smem + T::OFF_SV + ((j & 1) * 4 + b) * T::VBLK + half * 8 * D + d0;
@@ -355,7 +358,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
           w[r] = *reinterpret_cast<const uint32_t*>(src + r * D);
-          if (r >= live) w[r] = 0u;
+        }
+        if (!full) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (r >= live) w[r] = 0u;
         }
         if (j >= diagonal) {
 #pragma unroll
@@ -532,18 +539,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
         float mx = -INFINITY, mz = -INFINITY;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          // (a missing block's f is negative and its entries +inf: their products are -inf too)
-          float t0 = f[b] < 0.f ? INFINITY : -INFINITY, t1 = t0, t2 = t0, t3 = t0;
-          if (f[b] >= 0.f) {
+          // (a missing block's f is negative and its entries +inf: the largest product is -inf too)
+          float t0 = fmaxf(__uint_as_float(s[b * 16]), __uint_as_float(s[b * 16 + 1]));
+          float t1 = fmaxf(__uint_as_float(s[b * 16 + 2]), __uint_as_float(s[b * 16 + 3]));
 #pragma unroll
-            for (int k = 0; k < kBlock; k += 4) {
-              t0 = fmaxf(t0, __uint_as_float(s[b * 16 + k]));
-              t1 = fmaxf(t1, __uint_as_float(s[b * 16 + k + 1]));
-              t2 = fmaxf(t2, __uint_as_float(s[b * 16 + k + 2]));
-              t3 = fmaxf(t3, __uint_as_float(s[b * 16 + k + 3]));
-            }
+          for (int k = 4; k < kBlock; k += 4) {  // (three operands to a maximum)
+            t0 = fmaxf(fmaxf(t0, __uint_as_float(s[b * 16 + k])), __uint_as_float(s[b * 16 + k + 1]));
+            t1 = fmaxf(fmaxf(t1, __uint_as_float(s[b * 16 + k + 2])), __uint_as_float(s[b * 16 + k + 3]));
           }
-          const float x = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * f[b];
+          const float x = fmaxf(t0, t1) * f[b];
           mx = fmaxf(mx, x);
           mz = fmaxf(mz, x + ev[b]);
         }
