@@ -9,7 +9,9 @@
 //   warps 4, 5  keys: bring the codes (bulk copies of whole (block, head) tiles, two steps ahead), turn them
 //               into f16, exactly, and issue S = Q K^T (128 x 64 x D), two steps ahead of the softmax;
 //   warps 6, 7  values: the same with a transposition, and O += P V (128 x D x 64).
-// Both products are tcgen05 with f16 operands in shared memory and fp32 accumulators in tensor memory.
+// Both products are tcgen05 with f16 operands and fp32 accumulators in tensor memory. The softmax writes its
+// weights P there too, over the S that they come from, so that P is as double as S and the softmax of a step
+// need not wait for the product of the one before; V is double in shared memory for the same reason.
 // Two CTAs share an SM (256 of its 512 tensor-memory columns, 113 KB of shared memory each): one computes
 // exponentials while the other multiplies.
 //
@@ -65,9 +67,8 @@ struct Tile {
   static constexpr int VBLK = BLK + 32;           // a staged block of V: 32 bytes on spread the banks
   static constexpr int OFF_Q = 0;                 // f16 [ATOMS][128][64]
   static constexpr int OFF_K = OFF_Q + ATOMS * TM * 128;  // f16 [ATOMS][64][64]
-  static constexpr int OFF_V = OFF_K + ATOMS * TK * 128;  // f16 [D][64 keys]
-  static constexpr int OFF_P = OFF_V + D * 128;   // f16 [128][64 keys]
-  static constexpr int OFF_SK = OFF_P + TM * 128; // codes [2][4 blocks]
+  static constexpr int OFF_V = OFF_K + ATOMS * TK * 128;  // f16 [2][D][64 keys]
+  static constexpr int OFF_SK = OFF_V + 2 * D * 128;      // codes [2][4 blocks]
   static constexpr int OFF_SV = OFF_SK + 2 * 4 * BLK;
   static constexpr int OFF_BAR = (OFF_SV + 2 * 4 * VBLK + 15) / 16 * 16;
   static constexpr int SMEM = OFF_BAR + 512;
@@ -77,9 +78,9 @@ struct Tile {
 // Barriers and small state behind the tiles.
 struct Shared {
   uint64_t staged_k[2], staged_v[2];  // a step's codes have landed (4 threads announce them)
-  uint64_t sfull[2];         // S product done: S in tensor memory, K's place free
-  uint64_t sfree[2];         // S read (first: q written)
-  uint64_t pfull, odone;     // weights written / O product done with them and with V
+  uint64_t qfull;            // q in f16 written
+  uint64_t sfull[2];         // a step's S product done (and K's place free)
+  uint64_t pfull[2], odone[2];  // weights written / a step's O product done (and its V's and S's places free)
   uint64_t meta[kMeta];      // a step's scales written
   uint64_t drain[2];         // all products done
   alignas(16) float scale[kMeta][2][4];  // K's and V's; < 0: no such block
@@ -120,6 +121,16 @@ __device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b, uint
       "l"(operand(a)), "l"(operand(b)), "r"(idesc), "r"(acc), "r"(none)
       : "memory");
 }
+// The same with A in tensor memory: two f16 to a 32-bit column, rows on lanes.
+__device__ __forceinline__ void product_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+  const uint32_t none = 0, acc = add;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(operand(b)), "r"(idesc), "r"(acc), "r"(none)
+      : "memory");
+}
 __device__ __forceinline__ void commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
@@ -158,6 +169,12 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr)
+               : "memory");
+}
+
 // Waits for this thread's tensor-memory loads; the registers pass through it, so no use can move ahead.
 __device__ __forceinline__ void wait_loads(uint32_t* r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -242,11 +259,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
       mbar_init(&sh.staged_v[i], 4);
       mbar_init(&sh.drain[i], 1);
       mbar_init(&sh.sfull[i], 1);
-      mbar_init(&sh.sfree[i], kSoftmax);
+      mbar_init(&sh.pfull[i], kSoftmax);
+      mbar_init(&sh.odone[i], 1);
     }
     for (int i = 0; i < kMeta; ++i) mbar_init(&sh.meta[i], 8);
-    mbar_init(&sh.pfull, kSoftmax);
-    mbar_init(&sh.odone, 1);
+    mbar_init(&sh.qfull, kSoftmax);
     for (int i = 0; i < kDiagonal; ++i) sh.nan[i] = 0ull;
     for (int i = 0; i < 4; ++i) sh.found[i] = 0;
     sh.abort = (base & 1023u) != 0u;  // the swizzle counts on it
@@ -386,9 +403,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
             hi[r] = cvt_e4m3x2_f16x2(pair >> 16);
           }
           const int d = d0 + e;
-          *reinterpret_cast<uint4*>(smem + T::OFF_V + d * 128 + ((ch ^ (d & 7)) << 4)) =
+          *reinterpret_cast<uint4*>(smem + T::OFF_V + (j & 1) * (D * 128) + d * 128 + ((ch ^ (d & 7)) << 4)) =
               make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          *reinterpret_cast<uint4*>(smem + T::OFF_V + (d + 1) * 128 + ((ch ^ ((d + 1) & 7)) << 4)) =
+          *reinterpret_cast<uint4*>(smem + T::OFF_V + (j & 1) * (D * 128) + (d + 1) * 128 + ((ch ^ ((d + 1) & 7)) << 4)) =
               make_uint4(hi[0], hi[1], hi[2], hi[3]);
         }
       }
@@ -428,7 +445,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
         }
         announced = min(n + 3, steps);
         if (ct == 0 && ok) {
-          ok = wait_for(&sh.sfree[n & 1], (n >> 1) & 1, p.status, abort);
+          // q, and then the weights that lay over the place of this S, have been used
+          ok = n < 2 ? wait_for(&sh.qfull, 0, p.status, abort)
+                     : wait_for(&sh.odone[n & 1], ((n - 2) >> 1) & 1, p.status, abort);
           if (ok) {
             fence_after();
 #pragma unroll
@@ -440,22 +459,24 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
         }
       }
     } else {
-      for (int j = -1; j < steps && go; ++j) {
+      // V of steps 0 and 1, then step by step the product O and V two steps on, into the place that it left.
+      for (int j = -2; j < steps && go; ++j) {
         if (j >= 0 && ct == 0) {
-          ok = wait_for(&sh.pfull, j & 1, p.status, abort);
+          ok = wait_for(&sh.pfull[j & 1], (j >> 1) & 1, p.status, abort);
           if (ok) {
             fence_after();
 #pragma unroll
             for (int kk = 0; kk < TK / 16; ++kk)
-              product(tmem_o, base + T::OFF_P + kk * 32, base + T::OFF_V + kk * 32, kIdescO, j > 0 || kk > 0);
-            commit(&sh.odone);
+              product_tmem(tmem_o, tmem + (j & 1) * TK + kk * 8, base + T::OFF_V + (j & 1) * (D * 128) + kk * 32, kIdescO,
+                           j > 0 || kk > 0);
+            commit(&sh.odone[j & 1]);
           }
         }
-        const int n = j + 1;
+        const int n = j + 2;
         if (n < steps) {
           ok = ok && wait_for(&staged[n & 1], (n >> 1) & 1, p.status, abort) &&
                wait_for(&sh.meta[n & (kMeta - 1)], (n / kMeta) & 1, p.status, abort);
-          if (j >= 0) ok = ok && wait_for(&sh.odone, j & 1, p.status, abort);  // V's place is free
+          if (j >= 0) ok = ok && wait_for(&sh.odone[j & 1], (j >> 1) & 1, p.status, abort);
           if (ok) convert_v(n);
           go = ok = hand_over(ok);
           if (brings) {
@@ -504,8 +525,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
       }
     }
     fence_proxy_async_shared();
-    mbar_arrive(&sh.sfree[0]);  // q is in place: the first product may go (its buffer is free anyway)
-    mbar_arrive(&sh.sfree[1]);
+    mbar_arrive(&sh.qfull);
 
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     float m = -INFINITY, mw = -INFINITY, l = 0.f;
@@ -521,8 +541,6 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
         tmem_load(tmem + lanes + (j & 1) * TK + 32, s + 32);
         wait_loads(s);
         wait_loads(s + 32);
-        fence_before();
-        mbar_arrive(&sh.sfree[j & 1]);
         const float4 ks = *reinterpret_cast<const float4*>(sh.scale[j & (kMeta - 1)][0]);
         const float4 vs = *reinterpret_cast<const float4*>(sh.scale[j & (kMeta - 1)][1]);
         // logits are S * f; f stays above 0 (an all-zero block under a tiny q), below it no such block
@@ -556,11 +574,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
           m = mx;
         }
         const bool up = mz > mw + 8.f;
-        if (j > 0 && !wait_for(&sh.odone, (j - 1) & 1, p.status, abort)) stop = true;
-        stop = __any_sync(kAll, stop);
-        if (!stop && __any_sync(kAll, up)) {
+        if (__any_sync(kAll, up)) {
           const float to = up ? mz : mw;
-          if (j > 0) {
+          if (j > 0)  // the products so far have to be in O
+            stop = !__all_sync(kAll, wait_for(&sh.odone[(j - 1) & 1], ((j - 1) >> 1) & 1, p.status, abort));
+          if (j > 0 && !stop) {
             const float down = mw == -INFINITY ? (up ? 0.f : 1.f) : ex2(mw - to);
             fence_after();
 #pragma unroll 1
@@ -591,9 +609,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
               more += w1;
               w[k] = pack_f16x2(w0, w1);
             }
-            uint8_t* dst = smem + T::OFF_P + r * 128;
-            *reinterpret_cast<uint4*>(dst + (((2 * b) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<uint4*>(dst + (((2 * b + 1) ^ (r & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+            tmem_store8(tmem + lanes + (j & 1) * TK + b * 8, w);
             if (!far) l += mw == -INFINITY ? 0.f : (sum + more) * ex2(-off - ev[b]);
           }
           if (far) {  // rare: the weights may have underflowed, so the probabilities are summed themselves
@@ -603,17 +619,14 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
               l += x == -INFINITY ? 0.f : ex2(x - m);
             }
           }
+          wait_stores();
         }
-      } else {
-        mbar_arrive(&sh.sfree[j & 1]);
-        stop = j > 0 && !__all_sync(kAll, wait_for(&sh.odone, (j - 1) & 1, p.status, abort));
       }
       if (stop) break;
       fence_before();
-      fence_proxy_async_shared();
-      mbar_arrive(&sh.pfull);
+      mbar_arrive(&sh.pfull[j & 1]);
     }
-    if (rows_here && __all_sync(kAll, wait_for(&sh.odone, (steps - 1) & 1, p.status, abort))) {
+    if (rows_here && __all_sync(kAll, wait_for(&sh.odone[(steps - 1) & 1], ((steps - 1) >> 1) & 1, p.status, abort))) {
       fence_after();
       const float g = l > 0.f ? ex2(mw - m) / l : (l == 0.f ? 0.f : l);
       __nv_bfloat16* dst = p.out + (int64_t)(me.row0 + (mine ? r : 0)) * p.out_stride + (int64_t)head * D;
