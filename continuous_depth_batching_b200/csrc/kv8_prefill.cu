@@ -5,10 +5,11 @@
 // A CTA takes 128 query rows of one head: a tile and, where the list has it, the request's next one (so a
 // long chunk fills the tensor core's 128 rows; a lone tile leaves half of them idle). Keys come in steps of
 // 64 (4 blocks). Roles:
-//   warps 0..3  softmax: thread r owns query row r, so its maximum, sum and weights need no exchange;
-//   warps 4, 5  keys: bring the codes (bulk copies of whole (block, head) tiles, two steps ahead), turn them
-//               into f16, exactly, and issue S = Q K^T (128 x 64 x D), two steps ahead of the softmax;
-//   warps 6, 7  values: the same with a transposition, and O += P V (128 x D x 64).
+//   warps 0..3   softmax: thread r owns query row r, so its maximum, sum and weights need no exchange;
+//   warps 4..7   turn the codes into f16, exactly, in the tensor core's layout: K as it lies, V transposed;
+//   warps 8, 9   issue the products, S = Q K^T (128 x 64 x D) and O += P V (128 x D x 64);
+//   warps 10, 11 bring the codes of K and of V: bulk copies of whole (block, head) tiles, two steps ahead.
+// The softmax takes 136 of the registers, the conversion 72 and the rest 32 a thread (setmaxnreg; 80 at launch).
 // Both products are tcgen05 with f16 operands and fp32 accumulators in tensor memory. The softmax writes its
 // weights P there too, over the S that they come from, so that P is as double as S and the softmax of a step
 // need not wait for the product of the one before; V is double in shared memory for the same reason.
@@ -34,8 +35,8 @@ namespace kv8 {
 constexpr int TR = 64;   // rows of a listed tile
 constexpr int TM = 128;  // rows of a CTA
 constexpr int TK = 64;   // keys of a step
-constexpr int kSoftmax = 128, kConvert = 64;  // threads of the softmax, of the keys and of the values
-constexpr int kPrefillThreads = kSoftmax + 2 * kConvert;
+constexpr int kSoftmax = 128, kConvert = 128;  // threads of the softmax and of the conversion
+constexpr int kPrefillThreads = kSoftmax + kConvert + 128;
 constexpr int kMeta = 8;            // steps whose scales are kept (keys run up to five steps ahead of the softmax)
 constexpr int kDiagonal = 3;        // steps that the diagonal of 128 rows can cross
 constexpr int kPairLimit = 2048;    // longest tile list that every CTA searches for its neighbours
@@ -79,6 +80,7 @@ struct Tile {
 struct Shared {
   uint64_t staged_k[2], staged_v[2];  // a step's codes have landed (4 threads announce them)
   uint64_t qfull;            // q in f16 written
+  uint64_t kready[2], vready[2];  // a step's K, V in f16 written (and its codes read)
   uint64_t sfull[2];         // a step's S product done (and K's place free)
   uint64_t pfull[2], odone[2];  // weights written / a step's O product done (and its V's and S's places free)
   uint64_t meta[kMeta];      // a step's scales written
@@ -258,6 +260,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
       mbar_init(&sh.staged_k[i], 4);
       mbar_init(&sh.staged_v[i], 4);
       mbar_init(&sh.drain[i], 1);
+      mbar_init(&sh.kready[i], kConvert);
+      mbar_init(&sh.vready[i], kConvert);
       mbar_init(&sh.sfull[i], 1);
       mbar_init(&sh.pfull[i], kSoftmax);
       mbar_init(&sh.odone[i], 1);
@@ -284,7 +288,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
   const int kv_len = me.pos + me.n;
   const int steps = (kv_len + TK - 1) / TK, blocks = (kv_len + kBlock - 1) / kBlock;
   const int diagonal = me.pos / TK;  // the first step that holds a key which some row may not see
-  if (warp == 4) {
+  if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
                  "r"(kTmemCols)
                  : "memory");
@@ -297,41 +301,93 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
   const uint32_t tmem_o = tmem + 2 * TK;
   volatile int* abort = &sh.abort;
 
-  if (warp >= 4) {
-    // ------------------------------------------------------------ codes to f16, and the products
-    const bool values = warp >= 6;
-    const int ct = (tid - kSoftmax) & (kConvert - 1), cw = warp & 1;
-    const int32_t* bt = p.block_table + (int64_t)me.slot * p.bt_stride;
-    const int64_t first_tile = values ? (int64_t)p.num_blocks * p.kv_heads : 0;
-    uint64_t* staged = values ? sh.staged_v : sh.staged_k;
-    // Lanes 0..3 of the second warp (the first issues the products) bring one block of every step each, its
-    // id a step ahead of its copies.
-    const bool brings = cw == 1 && lane < 4;
-    int id = -1;
-    auto fetch_id = [&](int step) {
-      const int b = step * 4 + lane;
-      id = step < steps && b < blocks ? bt[b] : -1;
-    };
-    auto issue = [&](int step) {
-      if (step >= steps) return;
-      uint64_t *bar = &staged[step & 1], *meta = &sh.meta[step & (kMeta - 1)];
-      float* scale = &sh.scale[step & (kMeta - 1)][values][lane];
-      const bool used = step * 4 + lane < blocks;
-      if (used && id >= 0 && id < p.num_blocks) {
-        const int64_t at = first_tile + (int64_t)id * p.kv_heads + kvh;
-        const uint32_t place = (step & 1) * 4 + lane;
-        mbar_arrive_expect_tx(bar, T::BLK);
-        bulk_copy(base + (values ? T::OFF_SV + place * T::VBLK : T::OFF_SK + place * T::BLK), p.codes + at * T::BLK,
-                  T::BLK, smem_u32(bar));
-        async_copy4(smem_u32(scale), p.scales + at);
-        async_arrive(smem_u32(meta));
-      } else {
-        if (used) set_error(p.status, CDB_ERR_INDEX);
-        *scale = -1.f;
-        mbar_arrive(meta);
-        mbar_arrive(bar);
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+    if (warp >= 10) {
+      // ------------------------------------------------------------ codes into shared memory
+      const bool values = warp == 11;
+      const int32_t* bt = p.block_table + (int64_t)me.slot * p.bt_stride;
+      const int64_t first_tile = values ? (int64_t)p.num_blocks * p.kv_heads : 0;
+      uint64_t* staged = values ? sh.staged_v : sh.staged_k;
+      uint64_t* ready = values ? sh.vready : sh.kready;
+      // Lanes 0..3 bring one block of every step each, its id a step ahead of its copies.
+      int id = -1;
+      auto fetch_id = [&](int step) {
+        const int b = step * 4 + lane;
+        id = lane < 4 && step < steps && b < blocks ? bt[b] : -1;
+      };
+      auto issue = [&](int step) {
+        if (step >= steps || lane >= 4) return;
+        uint64_t *bar = &staged[step & 1], *meta = &sh.meta[step & (kMeta - 1)];
+        float* scale = &sh.scale[step & (kMeta - 1)][values][lane];
+        const bool used = step * 4 + lane < blocks;
+        if (used && id >= 0 && id < p.num_blocks) {
+          const int64_t at = first_tile + (int64_t)id * p.kv_heads + kvh;
+          const uint32_t place = (step & 1) * 4 + lane;
+          mbar_arrive_expect_tx(bar, T::BLK);
+          bulk_copy(base + (values ? T::OFF_SV + place * T::VBLK : T::OFF_SK + place * T::BLK), p.codes + at * T::BLK,
+                    T::BLK, smem_u32(bar));
+          async_copy4(smem_u32(scale), p.scales + at);
+          async_arrive(smem_u32(meta));
+        } else {
+          if (used) set_error(p.status, CDB_ERR_INDEX);
+          *scale = -1.f;
+          mbar_arrive(meta);
+          mbar_arrive(bar);
+        }
+      };
+      fetch_id(0);
+      issue(0);
+      fetch_id(1);
+      issue(1);
+      fetch_id(2);
+      int announced = min(2, steps);
+      for (int n = 0; n + 2 < steps; ++n) {  // step n's codes have been read: their place takes step n + 2's
+        if (!__all_sync(kAll, wait_for(&ready[n & 1], (n >> 1) & 1, p.status, abort))) break;
+        issue(n + 2);
+        fetch_id(n + 3);
+        announced = n + 3;
       }
-    };
+      for (int j = max(0, announced - 2); j < announced; ++j) mbar_wait(&staged[j & 1], (j >> 1) & 1, p.status);
+    } else {
+      // ------------------------------------------------------------ products
+      if (lane == 0 && warp == 8) {
+        for (int n = 0; n < steps; ++n) {
+          // K is there, and q; later the weights that lay over the place of this S have been used
+          if (!wait_for(&sh.kready[n & 1], (n >> 1) & 1, p.status, abort) ||
+              !(n < 2 ? wait_for(&sh.qfull, 0, p.status, abort)
+                      : wait_for(&sh.odone[n & 1], ((n - 2) >> 1) & 1, p.status, abort)))
+            break;
+          fence_after();
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            product(tmem + (n & 1) * TK, base + T::OFF_Q + (kk >> 2) * (TM * 128) + (kk & 3) * 32,
+                    base + T::OFF_K + (kk >> 2) * (TK * 128) + (kk & 3) * 32, kIdescS, kk > 0);
+          commit(&sh.sfull[n & 1]);
+        }
+      } else if (lane == 0) {
+        for (int j = 0; j < steps; ++j) {
+          if (!wait_for(&sh.vready[j & 1], (j >> 1) & 1, p.status, abort) ||
+              !wait_for(&sh.pfull[j & 1], (j >> 1) & 1, p.status, abort))
+            break;
+          fence_after();
+#pragma unroll
+          for (int kk = 0; kk < TK / 16; ++kk)
+            product_tmem(tmem_o, tmem + (j & 1) * TK + kk * 8, base + T::OFF_V + (j & 1) * (D * 128) + kk * 32, kIdescO,
+                         j > 0 || kk > 0);
+          commit(&sh.odone[j & 1]);
+        }
+      }
+      if (lane == 0) {  // on every path: no product may run when the tensor memory is freed
+        commit(&sh.drain[warp - 8]);
+        mbar_wait(&sh.drain[warp - 8], 0, p.status);
+      }
+      __syncwarp();
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ codes to f16
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    const int ct = tid - kSoftmax, cw = warp - 4;
     // K of step j into place: 16 codes of a key at a time; a quarter warp covers four chunks of two keys.
     auto convert_k = [&](int j) {
       constexpr int C = D / 16;  // chunks of a key
@@ -365,8 +421,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
       const int b = lane & 3;
       const bool have = sh.scale[j & (kMeta - 1)][1][b] >= 0.f;
       const bool full = kv_len - j * TK >= TK && __all_sync(kAll, have);
-#pragma unroll 2
-      for (int u = cw; u < 2 * (D / 32); u += 2) {
+#pragma unroll
+      for (int u0 = 0; u0 < 2 * (D / 32); u0 += 4) {
+        const int u = u0 + cw;
+        if (2 * (D / 32) % 4 != 0 && u >= 2 * (D / 32)) break;
         const int half = u & 1, d0 = (u >> 1) * 32 + (lane >> 2) * 4;
         const uint8_t* src = smem + T::OFF_SV + ((j & 1) * 4 + b) * T::VBLK + half * 8 * D + d0;
         const int key0 = b * kBlock + half * 8;
@@ -410,92 +468,24 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
         }
       }
     };
-    // What the two warps wrote is the products' to read; true if all of their threads are well.
-    auto hand_over = [&](bool mine) {
+    for (int n = 0; n < steps; ++n) {
+      bool ok = wait_for(&sh.staged_k[n & 1], (n >> 1) & 1, p.status, abort);
+      if (n > 0) ok = ok && wait_for(&sh.sfull[(n - 1) & 1], ((n - 1) >> 1) & 1, p.status, abort);  // K's place is free
+      if (!__all_sync(kAll, ok)) break;
+      convert_k(n);
       fence_proxy_async_shared();
-      uint32_t all;
-      asm volatile(
-          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, %3, %2, p;\n\t"
-          "selp.u32 %0, 1, 0, q;\n\t}"
-          : "=r"(all)
-          : "r"((uint32_t)mine), "n"(kConvert), "r"(values ? 2 : 1)
-          : "memory");
-      return all != 0u;
-    };
-
-    if (brings) {
-      fetch_id(0);
-      issue(0);
-      fetch_id(1);
-      issue(1);
-      fetch_id(2);
+      mbar_arrive(&sh.kready[n & 1]);
+      ok = wait_for(&sh.staged_v[n & 1], (n >> 1) & 1, p.status, abort) &&
+           wait_for(&sh.meta[n & (kMeta - 1)], (n / kMeta) & 1, p.status, abort);
+      if (n > 1) ok = ok && wait_for(&sh.odone[n & 1], ((n - 2) >> 1) & 1, p.status, abort);  // V's place is free
+      if (!__all_sync(kAll, ok)) break;
+      convert_v(n);
+      fence_proxy_async_shared();
+      mbar_arrive(&sh.vready[n & 1]);
     }
-    int announced = min(2, steps);
-    // `go` is the same in all of the two warps' threads: they pass their barrier together or not at all.
-    bool go = true, ok = true;
-    if (!values) {
-      for (int n = 0; n < steps && go; ++n) {
-        ok = ok && wait_for(&staged[n & 1], (n >> 1) & 1, p.status, abort);
-        if (n > 0) ok = ok && wait_for(&sh.sfull[(n - 1) & 1], ((n - 1) >> 1) & 1, p.status, abort);  // K's place is free
-        if (ok) convert_k(n);
-        go = ok = hand_over(ok);
-        if (brings) {  // this step's codes have been read
-          issue(n + 2);
-          fetch_id(n + 3);
-        }
-        announced = min(n + 3, steps);
-        if (ct == 0 && ok) {
-          // q, and then the weights that lay over the place of this S, have been used
-          ok = n < 2 ? wait_for(&sh.qfull, 0, p.status, abort)
-                     : wait_for(&sh.odone[n & 1], ((n - 2) >> 1) & 1, p.status, abort);
-          if (ok) {
-            fence_after();
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              product(tmem + (n & 1) * TK, base + T::OFF_Q + (kk >> 2) * (TM * 128) + (kk & 3) * 32,
-                      base + T::OFF_K + (kk >> 2) * (TK * 128) + (kk & 3) * 32, kIdescS, kk > 0);
-            commit(&sh.sfull[n & 1]);
-          }
-        }
-      }
-    } else {
-      // V of steps 0 and 1, then step by step the product O and V two steps on, into the place that it left.
-      for (int j = -2; j < steps && go; ++j) {
-        if (j >= 0 && ct == 0) {
-          ok = wait_for(&sh.pfull[j & 1], (j >> 1) & 1, p.status, abort);
-          if (ok) {
-            fence_after();
-#pragma unroll
-            for (int kk = 0; kk < TK / 16; ++kk)
-              product_tmem(tmem_o, tmem + (j & 1) * TK + kk * 8, base + T::OFF_V + (j & 1) * (D * 128) + kk * 32, kIdescO,
-                           j > 0 || kk > 0);
-            commit(&sh.odone[j & 1]);
-          }
-        }
-        const int n = j + 2;
-        if (n < steps) {
-          ok = ok && wait_for(&staged[n & 1], (n >> 1) & 1, p.status, abort) &&
-               wait_for(&sh.meta[n & (kMeta - 1)], (n / kMeta) & 1, p.status, abort);
-          if (j >= 0) ok = ok && wait_for(&sh.odone[j & 1], (j >> 1) & 1, p.status, abort);
-          if (ok) convert_v(n);
-          go = ok = hand_over(ok);
-          if (brings) {
-            issue(n + 2);
-            fetch_id(n + 3);
-          }
-          announced = min(n + 3, steps);
-        }
-      }
-    }
-    if (!ok)  // the copies in flight, after an abort; a step that has landed passes at once or runs into the limit
-      for (int j = max(0, announced - 2); j < announced; ++j) mbar_wait(&staged[j & 1], (j >> 1) & 1, p.status);
-    if (ct == 0) {
-      commit(&sh.drain[values]);  // on every path: no product may run when the tensor memory is freed
-      mbar_wait(&sh.drain[values], 0, p.status);
-    }
-    __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
     const int r = tid;  // query row, and tensor-memory lane
     const bool mine = r < me.n;
     const bool rows_here = warp * 32 < me.n;  // a warp without rows only keeps the barriers going
@@ -663,7 +653,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 4)
+  if (warp == 8)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
