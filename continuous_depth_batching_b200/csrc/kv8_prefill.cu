@@ -81,11 +81,11 @@ struct Shared {
   uint64_t staged_k[2], staged_v[2];  // a step's codes have landed (4 threads announce them)
   uint64_t qfull;            // q in f16 written
   uint64_t kready[2], vready[2];  // a step's K, V in f16 written (and its codes read)
-  uint64_t sfull[2];         // a step's S product done (and K's place free)
+  uint64_t sfull[2];         // a step's S product done (and K's place free) and its scales there
   uint64_t pfull[2], odone[2];  // weights written / a step's O product done (and its V's and S's places free)
   uint64_t meta[kMeta];      // a step's scales written
   uint64_t drain[2];         // all products done
-  alignas(16) float scale[kMeta][2][4];  // K's and V's; < 0: no such block
+  alignas(16) float scale[kMeta][2][4];  // K's (< 0: no such block) and V's, then V's log2
   unsigned long long nan[kDiagonal];
   uint32_t tmem;
   int abort;
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
       mbar_init(&sh.drain[i], 1);
       mbar_init(&sh.kready[i], kConvert);
       mbar_init(&sh.vready[i], kConvert);
-      mbar_init(&sh.sfull[i], 1);
+      mbar_init(&sh.sfull[i], 2);
       mbar_init(&sh.pfull[i], kSoftmax);
       mbar_init(&sh.odone[i], 1);
     }
@@ -351,19 +351,27 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
       for (int j = max(0, announced - 2); j < announced; ++j) mbar_wait(&staged[j & 1], (j >> 1) & 1, p.status);
     } else {
       // ------------------------------------------------------------ products
-      if (lane == 0 && warp == 8) {
+      if (warp == 8) {
         for (int n = 0; n < steps; ++n) {
-          // K is there, and q; later the weights that lay over the place of this S have been used
-          if (!wait_for(&sh.kready[n & 1], (n >> 1) & 1, p.status, abort) ||
-              !(n < 2 ? wait_for(&sh.qfull, 0, p.status, abort)
-                      : wait_for(&sh.odone[n & 1], ((n - 2) >> 1) & 1, p.status, abort)))
-            break;
-          fence_after();
+          // The step's scales (the softmax wants V's logarithms), K and q; later also that the weights which lay
+          // over the place of this S have been used.
+          const int sl = n & (kMeta - 1);
+          bool ok = wait_for(&sh.meta[sl], (n / kMeta) & 1, p.status, abort);
+          if (lane < 4) sh.scale[sl][1][lane] = sh.scale[sl][1][lane] > 0.f ? __log2f(sh.scale[sl][1][lane]) : -126.f;
+          ok = ok && wait_for(&sh.kready[n & 1], (n >> 1) & 1, p.status, abort) &&
+               (n < 2 ? wait_for(&sh.qfull, 0, p.status, abort)
+                      : wait_for(&sh.odone[n & 1], ((n - 2) >> 1) & 1, p.status, abort));
+          if (!__all_sync(kAll, ok)) break;
+          if (lane == 0) {
+            fence_after();
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            product(tmem + (n & 1) * TK, base + T::OFF_Q + (kk >> 2) * (TM * 128) + (kk & 3) * 32,
-                    base + T::OFF_K + (kk >> 2) * (TK * 128) + (kk & 3) * 32, kIdescS, kk > 0);
-          commit(&sh.sfull[n & 1]);
+            for (int kk = 0; kk < D / 16; ++kk)
+              product(tmem + (n & 1) * TK, base + T::OFF_Q + (kk >> 2) * (TM * 128) + (kk & 3) * 32,
+                      base + T::OFF_K + (kk >> 2) * (TK * 128) + (kk & 3) * 32, kIdescS, kk > 0);
+            commit(&sh.sfull[n & 1]);
+            mbar_arrive(&sh.sfull[n & 1]);  // releases the scales to whoever waits for S
+          }
+          __syncwarp();
         }
       } else if (lane == 0) {
         for (int j = 0; j < steps; ++j) {
@@ -419,7 +427,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
     // of dims.
     auto convert_v = [&](int j) {
       const int b = lane & 3;
-      const bool have = sh.scale[j & (kMeta - 1)][1][b] >= 0.f;
+      const bool have = sh.scale[j & (kMeta - 1)][0][b] >= 0.f;
       const bool full = kv_len - j * TK >= TK && __all_sync(kAll, have);
 #pragma unroll
       for (int u0 = 0; u0 < 2 * (D / 32); u0 += 4) {
@@ -493,25 +501,30 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
     float factor = 0.f;
     {
       const __nv_bfloat16* src = p.q + (int64_t)(me.row0 + (mine ? r : 0)) * p.q_stride + (int64_t)head * D;
+      uint4 w[D / 8];
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c)
+        w[c] = mine ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
       float amax = 0.f;
-#pragma unroll 4
+#pragma unroll
       for (int c = 0; c < D / 8; ++c) {
-        const uint4 w = *reinterpret_cast<const uint4*>(src + c * 8);
-        amax = fmaxf(amax, fmaxf(fmaxf(fmaxf(fabsf(bf16lo(w.x)), fabsf(bf16hi(w.x))), fmaxf(fabsf(bf16lo(w.y)), fabsf(bf16hi(w.y)))),
-                                 fmaxf(fmaxf(fabsf(bf16lo(w.z)), fabsf(bf16hi(w.z))), fmaxf(fabsf(bf16lo(w.w)), fabsf(bf16hi(w.w))))));
+        amax = fmaxf(fmaxf(amax, fabsf(bf16lo(w[c].x))), fabsf(bf16hi(w[c].x)));
+        amax = fmaxf(fmaxf(amax, fabsf(bf16lo(w[c].y))), fabsf(bf16hi(w[c].y)));
+        amax = fmaxf(fmaxf(amax, fabsf(bf16lo(w[c].z))), fabsf(bf16hi(w[c].z)));
+        amax = fmaxf(fmaxf(amax, fabsf(bf16lo(w[c].w))), fabsf(bf16hi(w[c].w)));
       }
       int e = (int)(__float_as_uint(amax) >> 23) - 127;
       e = amax == 0.f ? 0 : max(-126, min(126, e));
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
       factor = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
-#pragma unroll 4
+#pragma unroll
       for (int c = 0; c < D / 8; ++c) {
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (mine) w = *reinterpret_cast<const uint4*>(src + c * 8);
         uint8_t* dst = smem + T::OFF_Q + (c >> 3) * (TM * 128) + r * 128;
         *reinterpret_cast<uint4*>(dst + (((c & 7) ^ (r & 7)) << 4)) =
-            make_uint4(pack_f16x2(bf16lo(w.x) * down, bf16hi(w.x) * down), pack_f16x2(bf16lo(w.y) * down, bf16hi(w.y) * down),
-                       pack_f16x2(bf16lo(w.z) * down, bf16hi(w.z) * down), pack_f16x2(bf16lo(w.w) * down, bf16hi(w.w) * down));
+            make_uint4(pack_f16x2(bf16lo(w[c].x) * down, bf16hi(w[c].x) * down),
+                       pack_f16x2(bf16lo(w[c].y) * down, bf16hi(w[c].y) * down),
+                       pack_f16x2(bf16lo(w[c].z) * down, bf16hi(w[c].z) * down),
+                       pack_f16x2(bf16lo(w[c].w) * down, bf16hi(w[c].w) * down));
       }
     }
     fence_proxy_async_shared();
@@ -520,9 +533,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     float m = -INFINITY, mw = -INFINITY, l = 0.f;
     for (int j = 0; j < steps; ++j) {
-      if (!__all_sync(kAll, wait_for(&sh.sfull[j & 1], (j >> 1) & 1, p.status, abort) &&
-                                wait_for(&sh.meta[j & (kMeta - 1)], (j / kMeta) & 1, p.status, abort)))
-        break;
+      if (!__all_sync(kAll, wait_for(&sh.sfull[j & 1], (j >> 1) & 1, p.status, abort))) break;
       bool stop = false;
       if (rows_here) {
         fence_after();
@@ -536,8 +547,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
         // logits are S * f; f stays above 0 (an all-zero block under a tiny q), below it no such block
         const float f[4] = {ks.x < 0.f ? -1.f : fmaxf(factor * ks.x, 1.2e-38f), ks.y < 0.f ? -1.f : fmaxf(factor * ks.y, 1.2e-38f),
                             ks.z < 0.f ? -1.f : fmaxf(factor * ks.z, 1.2e-38f), ks.w < 0.f ? -1.f : fmaxf(factor * ks.w, 1.2e-38f)};
-        const float ev[4] = {vs.x > 0.f ? __log2f(vs.x) : -126.f, vs.y > 0.f ? __log2f(vs.y) : -126.f,
-                             vs.z > 0.f ? __log2f(vs.z) : -126.f, vs.w > 0.f ? __log2f(vs.w) : -126.f};
+        const float ev[4] = {vs.x, vs.y, vs.z, vs.w};
         if (j >= diagonal || f[0] < 0.f || f[1] < 0.f || f[2] < 0.f || f[3] < 0.f) {
           const int seen = qpos - j * TK;  // the last key of the step that the row sees
 #pragma unroll
