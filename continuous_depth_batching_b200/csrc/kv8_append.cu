@@ -136,74 +136,94 @@ __device__ __forceinline__ void rotate_q(const AppendParams& p, int row0, int en
   }
 }
 
-// The run of rows that starts at row r, if one does: its rows all lie in one block.
+// A run of rows of one block.
 struct Run {
   int slot, pos, n;
   int64_t blk;
 };
 
-// False where no run starts at r. Uniform over the warp.
-__device__ __forceinline__ bool find_run(const AppendParams& p, int r, Run& run) {
-  const int lane = threadIdx.x & 31;
-  // lane 16 looks at the row before, lanes 0..15 at rows r .. r + 15: two loads deep in all
-  const int at = lane == kBlock ? r - 1 : r + lane;
-  const bool in = at >= 0 && at < p.num_items && lane <= kBlock;
-  const int pos = in ? p.item_pos[at] : -1, slot = in ? p.item_slot[at] : -1;
-  run.pos = __shfl_sync(0xffffffffu, pos, 0);
-  run.slot = __shfl_sync(0xffffffffu, slot, 0);
-  const int before = __shfl_sync(0xffffffffu, pos, kBlock), before_slot = __shfl_sync(0xffffffffu, slot, kBlock);
-  if (run.pos < 0) return false;
-  if (before >= 0 && before_slot == run.slot && before / kBlock == run.pos / kBlock) {
-    // a later row of a run; one that does not follow its predecessor has no place in the block
-    if (before + 1 != run.pos && lane == 0) set_error(p.status, CDB_ERR_INDEX);
-    return false;
-  }
-  const bool next = lane < kBlock && slot == run.slot && pos == run.pos + lane && run.pos % kBlock + lane < kBlock;
-  run.n = __ffs(~__ballot_sync(0xffffffffu, next)) - 1;
+// The runs that start in rows [row0, row0 + 16): lane L looks at row row0 - 1 + L, so that the warp sees the
+// row before the group and every row that a run of the group can reach.
+struct Runs {
+  int slot, pos;             // this lane's row
+  unsigned starts, follows;  // lanes that start a run / follow their predecessor in one
+};
+
+__device__ __forceinline__ Runs find_runs(const AppendParams& p, int row0, int rows) {
+  const int lane = threadIdx.x & 31, at = row0 - 1 + lane;
+  const bool in = at >= 0 && at < p.num_items;
+  Runs r;
+  r.pos = in ? p.item_pos[at] : -1;
+  r.slot = in ? p.item_slot[at] : -1;
+  const int before = __shfl_up_sync(0xffffffffu, r.pos, 1), before_slot = __shfl_up_sync(0xffffffffu, r.slot, 1);
+  const bool same = lane > 0 && r.pos >= 0 && before >= 0 && before_slot == r.slot && before / kBlock == r.pos / kBlock;
+  const bool here = lane >= 1 && lane <= rows;
+  // a row that does not follow its predecessor in their block has no place there
+  if (here && same && before + 1 != r.pos) set_error(p.status, CDB_ERR_INDEX);
+  r.starts = __ballot_sync(0xffffffffu, here && r.pos >= 0 && !same);
+  r.follows = __ballot_sync(0xffffffffu, same && before + 1 == r.pos);
+  return r;
+}
+
+// The run that starts at lane s; false (and the error set) where its indexes do not fit.
+__device__ __forceinline__ bool take_run(const AppendParams& p, const Runs& r, int s, Run& run) {
+  run.slot = __shfl_sync(0xffffffffu, r.slot, s);
+  run.pos = __shfl_sync(0xffffffffu, r.pos, s);
+  run.n = s == 31 ? 1 : __ffs(~(r.follows >> (s + 1)));
   run.blk = -1;
   if (run.slot >= 0 && run.slot < p.bt_rows && run.pos / kBlock < p.bt_width &&
       (p.rope_mode == 0 || run.pos + run.n <= p.rope_rows))
     run.blk = p.block_table[(int64_t)run.slot * p.bt_stride + run.pos / kBlock];
-  if (run.blk < 0 || run.blk >= p.num_blocks) {
-    if (lane == 0) set_error(p.status, CDB_ERR_INDEX);
-    return false;
-  }
-  return true;
+  if (run.blk >= 0 && run.blk < p.num_blocks) return true;
+  if ((threadIdx.x & 31) == 0) set_error(p.status, CDB_ERR_INDEX);
+  return false;
 }
 
-// k or v of one head of a run. ROWS: the most rows a run may have here (16, or what one pass holds).
-template <int D, int ROWS>
-__device__ __forceinline__ void write_tile(const AppendParams& p, int r, const Run& run, int head, bool is_v) {
+// k or v of one head of a run. ROWS: the most rows a run may have here (16, or what one pass holds). The
+// rows stay in registers from the loads, all in flight together, to the codes; the largest magnitude is
+// taken over everything first, and again over the finite values in the rare tile that has others.
+template <int D, int ROWS, bool IS_V>
+__device__ __forceinline__ void write_tile(const AppendParams& p, int r, const Run& run, int head) {
   constexpr int LPR = D / 8, RPI = 32 / LPR, IT = (ROWS + RPI - 1) / RPI;
   const int lane = threadIdx.x & 31;
   const int sub = lane / LPR, x0 = (lane % LPR) * 8;
-  const int mode = is_v ? 0 : p.rope_mode;
   const int off = run.pos % kBlock;
-  const int64_t tile = ((int64_t)(is_v ? p.num_blocks : 0) + run.blk) * p.num_kv_heads + head;
+  const int64_t tile = ((int64_t)(IS_V ? p.num_blocks : 0) + run.blk) * p.num_kv_heads + head;
   uint8_t* codes = p.codes + tile * (kBlock * D);
   const float was = off > 0 ? p.scales[tile] : 0.f;
-  const int64_t col = (int64_t)(p.num_heads + (is_v ? p.num_kv_heads : 0) + head) * D + x0;
+  const __nv_bfloat16* src = p.qkv + (int64_t)(r + sub) * p.qkv_stride +
+                             (int64_t)(p.num_heads + (IS_V ? p.num_kv_heads : 0) + head) * D + x0;
+  const int64_t step = (int64_t)RPI * p.qkv_stride;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  const uint4 bias =
-      !is_v && p.qk_bias != nullptr && sub < RPI ? ld16(p.qk_bias + (int64_t)(p.num_heads + head) * D + x0) : zero;
+  const int rows = sub < RPI ? run.n - sub : 0;  // this lane's: it * RPI < rows
   uint4 raw[IT];
 #pragma unroll
-  for (int it = 0; it < IT; ++it) {
-    const int j = it * RPI + sub;
-    raw[it] = sub < RPI && j < run.n ? ld16(p.qkv + (int64_t)(r + j) * p.qkv_stride + col) : zero;
-  }
+  for (int it = 0; it < IT; ++it) raw[it] = it * RPI < rows ? ld16(src + it * step) : zero;
+  uint4 bias = zero;
+  if (!IS_V && p.qk_bias != nullptr && sub < RPI) bias = ld16(p.qk_bias + (int64_t)(p.num_heads + head) * D + x0);
   float y[IT][8];
   float amax = 0.f;
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
-    const int j = it * RPI + sub;
-    const bool on = sub < RPI && j < run.n;
-    const Angles a = load_angles<D>(p, mode, run.pos + j, x0, on);
-    rotated8<D>(raw[it], on ? bias : zero, mode, a, x0, y[it]);  // zeros where no row is
+    if constexpr (IS_V) {
+      unpack8(raw[it], y[it]);
+    } else {
+      const bool on = it * RPI < rows;
+      const Angles a = load_angles<D>(p, p.rope_mode, run.pos + it * RPI + sub, x0, on);
+      rotated8<D>(raw[it], on ? bias : zero, p.rope_mode, a, x0, y[it]);  // zeros where no row is
+    }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(y[it][e]));
+    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(y[it][e]));  // (a NaN is passed over)
   }
   amax = warp_max(amax);
+  if (amax > 3.402823466e38f) {  // infinities saturate, under the others' scale
+    amax = 0.f;
+#pragma unroll
+    for (int it = 0; it < IT; ++it)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(y[it][e]));
+    amax = warp_max(amax);
+  }
   float scale = block_scale(amax);
   if (off > 0) {
     if (was >= scale) {
@@ -227,15 +247,15 @@ __device__ __forceinline__ void write_tile(const AppendParams& p, int r, const R
     }
   }
   const float inv = 1.f / scale;
+  uint8_t* dst = codes + (off + sub) * D + x0;
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
-    const int j = it * RPI + sub;
-    if (sub < RPI && j < run.n) {
+    if (it * RPI < rows) {
       const uint32_t lo = cvt_f32x2_e4m3x2(y[it][0] * inv, y[it][1] * inv) |
                           (cvt_f32x2_e4m3x2(y[it][2] * inv, y[it][3] * inv) << 16);
       const uint32_t hi = cvt_f32x2_e4m3x2(y[it][4] * inv, y[it][5] * inv) |
                           (cvt_f32x2_e4m3x2(y[it][6] * inv, y[it][7] * inv) << 16);
-      *reinterpret_cast<uint2*>(codes + (off + j) * D + x0) = make_uint2(lo, hi);
+      *reinterpret_cast<uint2*>(dst + it * RPI * D) = make_uint2(lo, hi);
     }
   }
   if (lane == 0) p.scales[tile] = scale;
@@ -254,6 +274,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) append_kernel(const Appe
   const int q_rows = (p.group + RPI - 1) / RPI, q_heads = (p.num_heads + HB - 1) / HB;
   const int q_tasks = p.q_out != nullptr ? q_rows * q_heads : 0;
   const int tasks = q_tasks + 2 * p.num_kv_heads;
+  const Runs runs = find_runs(p, row0, rows);
   for (int task = blockIdx.y * 8 + warp; task < tasks; task += gridDim.y * 8) {
     if (task < q_tasks) {
       const int i = task / q_heads, h = task - i * q_heads;
@@ -263,14 +284,18 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) append_kernel(const Appe
     const int kt = task - q_tasks;
     const bool is_v = kt >= p.num_kv_heads;
     const int head = is_v ? kt - p.num_kv_heads : kt;
-    for (int i = 0; i < rows; ++i) {
+    for (unsigned left = runs.starts; left; left &= left - 1) {
+      const int at = __ffs(left) - 1;
       Run run;
-      if (!find_run(p, row0 + i, run)) continue;
-      if (run.n <= RPI)
-        write_tile<D, RPI>(p, row0 + i, run, head, is_v);
-      else
-        write_tile<D, kBlock>(p, row0 + i, run, head, is_v);
-      i += run.n - 1;
+      if (!take_run(p, runs, at, run)) continue;
+      const int r = row0 - 1 + at;
+      if (run.n <= RPI) {
+        if (is_v) write_tile<D, RPI, true>(p, r, run, head);
+        else write_tile<D, RPI, false>(p, r, run, head);
+      } else {
+        if (is_v) write_tile<D, kBlock, true>(p, r, run, head);
+        else write_tile<D, kBlock, false>(p, r, run, head);
+      }
     }
   }
 }
