@@ -139,7 +139,6 @@ __device__ __forceinline__ void rotate_q(const AppendParams& p, int row0, int en
 // A run of rows of one block.
 struct Run {
   int slot, pos, n;
-  int64_t blk;
 };
 
 // The runs that start in rows [row0, row0 + 16): lane L looks at row row0 - 1 + L, so that the warp sees the
@@ -165,32 +164,35 @@ __device__ __forceinline__ Runs find_runs(const AppendParams& p, int row0, int r
   return r;
 }
 
-// The run that starts at lane s; false (and the error set) where its indexes do not fit.
-__device__ __forceinline__ bool take_run(const AppendParams& p, const Runs& r, int s, Run& run) {
+// The run that starts at lane s.
+__device__ __forceinline__ Run take_run(const Runs& r, int s) {
+  Run run;
   run.slot = __shfl_sync(0xffffffffu, r.slot, s);
   run.pos = __shfl_sync(0xffffffffu, r.pos, s);
   run.n = s == 31 ? 1 : __ffs(~(r.follows >> (s + 1)));
-  run.blk = -1;
-  if (run.slot >= 0 && run.slot < p.bt_rows && run.pos / kBlock < p.bt_width &&
-      (p.rope_mode == 0 || run.pos + run.n <= p.rope_rows))
-    run.blk = p.block_table[(int64_t)run.slot * p.bt_stride + run.pos / kBlock];
-  if (run.blk >= 0 && run.blk < p.num_blocks) return true;
-  if ((threadIdx.x & 31) == 0) set_error(p.status, CDB_ERR_INDEX);
-  return false;
+  return run;
+}
+
+// The block that the run's rows lie in, -1 where its indexes do not fit.
+__device__ __forceinline__ int block_of(const AppendParams& p, const Run& run) {
+  if (run.slot < 0 || run.slot >= p.bt_rows || run.pos / kBlock >= p.bt_width ||
+      (p.rope_mode != 0 && run.pos + run.n > p.rope_rows))
+    return -1;
+  return p.block_table[(int64_t)run.slot * p.bt_stride + run.pos / kBlock];
 }
 
 // k or v of one head of a run. ROWS: the most rows a run may have here (16, or what one pass holds). The
-// rows stay in registers from the loads, all in flight together, to the codes; the largest magnitude is
-// taken over everything first, and again over the finite values in the rare tile that has others.
+// loads, the block id's among them, are in flight together; the rotated rows stay in registers from there to
+// the codes (rotating them twice, for a third CTA on the SM, measured 138 us against 114 on 55 x 96 prompts).
+// The magnitude is taken over everything first, and again over the finite values in the rare tile that has
+// others.
 template <int D, int ROWS, bool IS_V>
 __device__ __forceinline__ void write_tile(const AppendParams& p, int r, const Run& run, int head) {
   constexpr int LPR = D / 8, RPI = 32 / LPR, IT = (ROWS + RPI - 1) / RPI;
   const int lane = threadIdx.x & 31;
   const int sub = lane / LPR, x0 = (lane % LPR) * 8;
   const int off = run.pos % kBlock;
-  const int64_t tile = ((int64_t)(IS_V ? p.num_blocks : 0) + run.blk) * p.num_kv_heads + head;
-  uint8_t* codes = p.codes + tile * (kBlock * D);
-  const float was = off > 0 ? p.scales[tile] : 0.f;
+  const int blk = block_of(p, run);
   const __nv_bfloat16* src = p.qkv + (int64_t)(r + sub) * p.qkv_stride +
                              (int64_t)(p.num_heads + (IS_V ? p.num_kv_heads : 0) + head) * D + x0;
   const int64_t step = (int64_t)RPI * p.qkv_stride;
@@ -201,6 +203,13 @@ __device__ __forceinline__ void write_tile(const AppendParams& p, int r, const R
   for (int it = 0; it < IT; ++it) raw[it] = it * RPI < rows ? ld16(src + it * step) : zero;
   uint4 bias = zero;
   if (!IS_V && p.qk_bias != nullptr && sub < RPI) bias = ld16(p.qk_bias + (int64_t)(p.num_heads + head) * D + x0);
+  if (blk < 0 || blk >= p.num_blocks) {
+    if (lane == 0) set_error(p.status, CDB_ERR_INDEX);
+    return;
+  }
+  const int64_t tile = ((int64_t)(IS_V ? p.num_blocks : 0) + blk) * p.num_kv_heads + head;
+  uint8_t* codes = p.codes + tile * (kBlock * D);
+  const float was = off > 0 ? p.scales[tile] : 0.f;
   float y[IT][8];
   float amax = 0.f;
 #pragma unroll
@@ -286,8 +295,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) append_kernel(const Appe
     const int head = is_v ? kt - p.num_kv_heads : kt;
     for (unsigned left = runs.starts; left; left &= left - 1) {
       const int at = __ffs(left) - 1;
-      Run run;
-      if (!take_run(p, runs, at, run)) continue;
+      const Run run = take_run(runs, at);
       const int r = row0 - 1 + at;
       if (run.n <= RPI) {
         if (is_v) write_tile<D, RPI, true>(p, r, run, head);
