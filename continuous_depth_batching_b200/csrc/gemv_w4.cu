@@ -2,15 +2,15 @@
 //   out[m][n] = bf16( sum over groups j of s[n][j] * sum over k in group j of (q[n][k] - z[n][j]) x[m][k] )
 // Weights q are nibbles, two to a byte along k (low nibble first), as they are stored; no layout pass.
 //
-// Bound by the weights' bytes, N K / 2, for a few rows, and by the work of taking nibbles apart (an AND, an
-// OR and most of a shift for two weights) where the tokens fill the products. One CTA of 16 warps an SM
+// Bound by the weights' bytes, N K / 2, and by the instructions around a weight: seven for eight weights to
+// take nibbles apart, then the products and each group's scale. One CTA of 16 warps an SM
 // keeps its token rows in shared memory for good; `wk` warps share a tile of 16 weight rows, each with its
 // part of k, and add their parts through shared memory; the groups of wk warps walk over the row tiles.
 // A warp streams its boxes (16 rows x 128 bytes = 256 k, TMA with a 128-byte swizzle, so that the loads
 // below hit every bank once) through a ring of its own, across row tiles, so nobody waits but at the sum.
 //
 // The products run on the tensor cores (bf16 m16n8k16: 16 weight rows, 8 tokens). A nibble q becomes
-// the bf16 number 128 + q by one AND and one OR into the mantissa, exactly, and the offset is taken
+// the bf16 number 128 + q, exactly, when a byte 0x43 is set above it, and the offset is taken
 // off per group with the group's sum of x:
 //   sum (q - z) x = sum (128 + q) x - (128 + z) sum x,
 // both sums in fp32, then times the group's scale into the fp32 result: no weight is rounded. What the
@@ -64,8 +64,15 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Nibbles s and s + 4 of a word as the bf16 pair (128 + q_s, 128 + q_{s+4}).
-__device__ __forceinline__ uint32_t nibbles(uint32_t w, int s) { return ((w >> (4 * s)) & 0x000f000fu) | 0x43004300u; }
+// The 8 nibbles of a word as bf16 pairs 128 + q, of k (0, 2) (4, 6) (1, 3) (5, 7): the nibbles become bytes,
+// two at a time, and the byte 0x43 above one makes it 128 + q. Seven instructions for eight weights.
+__device__ __forceinline__ void nibbles(uint32_t w, uint32_t (&e)[4]) {
+  const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
+  e[0] = __byte_perm(even, 0x43434343u, 0x4140);
+  e[1] = __byte_perm(even, 0x43434343u, 0x4342);
+  e[2] = __byte_perm(odd, 0x43434343u, 0x4140);
+  e[3] = __byte_perm(odd, 0x43434343u, 0x4342);
+}
 
 // NT: tiles of 8 tokens. GI: 32-k blocks that share a scale within a box (1, 2, or 4 for groups of 128
 // and multiples of it).
@@ -81,7 +88,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) gemv_kernel(const __grid_const
   const int tokens = min(p.tokens, p.m - tok0);
   uint8_t* ring = smem + warp * p.stages * kTile;
   const uint32_t ring_u = smem_u32(ring), bar_u = smem_u32(&s_bar[warp][0]);
-  // token rows: 16-byte chunks of 8 k in the order (0,4) (1,5) (2,6) (3,7), rows 4 chunks (mod 8) apart
+  // token rows: 16-byte chunks of 8 k in the order of nibbles(), rows 4 chunks (mod 8) apart
   uint8_t* xs = smem + kWarps * p.stages * kTile;
   const int pitch = p.subs * 512 + 64;
   float* xsum = reinterpret_cast<float*>(xs + p.tokens * pitch);  // [subs * GN][NT * 8]
@@ -90,7 +97,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) gemv_kernel(const __grid_const
   // this warp's place: part `part` of row tiles group, group + groups, ...
   const int part = warp & (p.wk - 1);
   const int groups = gridDim.x * (kWarps / p.wk);
-  const int group = blockIdx.x * (kWarps / p.wk) + warp / p.wk;
+  const int group = blockIdx.x + gridDim.x * (warp / p.wk);  // few tiles spread over the SMs first
   const int each = (p.subs + p.wk - 1) / p.wk;
   const int sub0 = part * each, subs = max(0, min(each, p.subs - sub0));
   const int rounds = group < p.tiles ? (p.tiles - group + groups - 1) / groups : 0;
@@ -126,10 +133,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) gemv_kernel(const __grid_const
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (k < p.k) v = *reinterpret_cast<const uint4*>(p.x + (int64_t)(tok0 + tok) * p.ldx + k);
     uint4 o;
-    o.x = __byte_perm(v.x, v.z, 0x5410);
-    o.y = __byte_perm(v.x, v.z, 0x7632);
-    o.z = __byte_perm(v.y, v.w, 0x5410);
-    o.w = __byte_perm(v.y, v.w, 0x7632);
+    o.x = __byte_perm(v.x, v.y, 0x5410);
+    o.y = __byte_perm(v.z, v.w, 0x5410);
+    o.z = __byte_perm(v.x, v.y, 0x7632);
+    o.w = __byte_perm(v.z, v.w, 0x7632);
     *reinterpret_cast<uint4*>(xs + tok * pitch + sb * 512 + lane * 16) = o;
     float sum = ((bf16lo(v.x) + bf16hi(v.x)) + (bf16lo(v.y) + bf16hi(v.y))) +
                 ((bf16lo(v.z) + bf16hi(v.z)) + (bf16lo(v.w) + bf16hi(v.w)));
@@ -147,28 +154,31 @@ __global__ void __launch_bounds__(kWarps * 32, 1) gemv_kernel(const __grid_const
   int get = 0;
   uint32_t phase = 0;
   bool ok = true;
+  // The scales and zero points of a box: 2 GN (row half, group) entries, each loaded once in the four lanes of
+  // a row (entry e in lane e % 4) as scale bits and zero point in one word, a box ahead of their use.
+  uint32_t entry[(GN + 1) / 2];
+  auto load_entries = [&](int tile, int i) {
+#pragma unroll
+    for (int k = 0; k < (GN + 1) / 2; ++k) {
+      const int e = t + 4 * k, row = min(tile * kRows + g + 8 * (e / GN), p.n - 1);
+      int grp = (sub0 + i) * GN + e % GN;
+      if (GI == 4 && p.group_boxes > 1) grp /= p.group_boxes;
+      const int64_t at = (int64_t)row * p.groups + min(grp, p.groups - 1);  // a box may reach past k, onto zeros of x
+      entry[k] = ((uint32_t)__bfloat16_as_ushort(p.scales[at]) << 16) | (p.zeros != nullptr ? p.zeros[at] : 8u);
+    }
+  };
+  if (boxes > 0) load_entries(group, 0);
   for (int round = 0, tile = group; round < rounds; ++round, tile += groups) {
     const int row0 = tile * kRows;
-    const int64_t ra = (int64_t)min(row0 + g, p.n - 1) * p.groups, rb = (int64_t)min(row0 + g + 8, p.n - 1) * p.groups;
     float acc[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
     for (int i = 0; i < subs; ++i) {
-      // this box's scales and offsets 128 + z, two weight rows a lane
-      float sa[GN], sb[GN], za[GN], zb[GN];
+      uint32_t now[(GN + 1) / 2];
 #pragma unroll
-      for (int j = 0; j < GN; ++j) {
-        int grp = (sub0 + i) * GN + j;
-        if (GI == 4 && p.group_boxes > 1) grp /= p.group_boxes;
-        grp = min(grp, p.groups - 1);  // a box may reach past k: its x are zeros there
-        sa[j] = bf16_to_f(p.scales[ra + grp]);
-        sb[j] = bf16_to_f(p.scales[rb + grp]);
-        za[j] = zb[j] = 136.f;
-        if (p.zeros != nullptr) {
-          za[j] = (float)(128 + p.zeros[ra + grp]);
-          zb[j] = (float)(128 + p.zeros[rb + grp]);
-        }
-      }
+      for (int k = 0; k < (GN + 1) / 2; ++k) now[k] = entry[k];
+      if (i + 1 < subs) load_entries(tile, i + 1);
+      else if (round + 1 < rounds) load_entries(tile + groups, 0);
       ok = ok && __all_sync(kFull, mbar_wait(&s_bar[warp][get], phase, p.status));
       if (!ok) break;
       const uint8_t* w = ring + get * kTile + g * 128 + t * 4;
@@ -182,8 +192,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) gemv_kernel(const __grid_const
         const uint32_t wa = *reinterpret_cast<const uint32_t*>(w + ((b ^ g) << 4));
         const uint32_t wb = *reinterpret_cast<const uint32_t*>(w + 1024 + ((b ^ g) << 4));
         uint32_t ea[4], eb[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) ea[s] = nibbles(wa, s), eb[s] = nibbles(wb, s);
+        nibbles(wa, ea);
+        nibbles(wb, eb);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           const uint4 xv = *reinterpret_cast<const uint4*>(xrow[j] + i * 512 + b * 64);
@@ -192,13 +202,19 @@ __global__ void __launch_bounds__(kWarps * 32, 1) gemv_kernel(const __grid_const
         }
         if (b % GI == GI - 1) {
           const int grp = b / GI;
+          // scale, and 128 + zero point (2^15 + z by bits, less 2^15 - 128), of this lane's two rows
+          const uint32_t ua = __shfl_sync(kFull, now[grp / 4], grp % 4, 4);
+          const uint32_t ub = __shfl_sync(kFull, now[(GN + grp) / 4], (GN + grp) % 4, 4);
+          const float sa = __uint_as_float(ua & 0xffff0000u), sb = __uint_as_float(ub & 0xffff0000u);
+          const float za = __uint_as_float(__byte_perm(ua, 0x47000000u, 0x7404)) - 32640.f;
+          const float zb = __uint_as_float(__byte_perm(ub, 0x47000000u, 0x7404)) - 32640.f;
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             const float2 sx = *reinterpret_cast<const float2*>(sums + (i * GN + grp) * (NT * 8) + j * 8);
-            acc[j][0] = fmaf(sa[grp], fmaf(-za[grp], sx.x, prod[j][0]), acc[j][0]);
-            acc[j][1] = fmaf(sa[grp], fmaf(-za[grp], sx.y, prod[j][1]), acc[j][1]);
-            acc[j][2] = fmaf(sb[grp], fmaf(-zb[grp], sx.x, prod[j][2]), acc[j][2]);
-            acc[j][3] = fmaf(sb[grp], fmaf(-zb[grp], sx.y, prod[j][3]), acc[j][3]);
+            acc[j][0] = fmaf(sa, fmaf(-za, sx.x, prod[j][0]), acc[j][0]);
+            acc[j][1] = fmaf(sa, fmaf(-za, sx.y, prod[j][1]), acc[j][1]);
+            acc[j][2] = fmaf(sb, fmaf(-zb, sx.x, prod[j][2]), acc[j][2]);
+            acc[j][3] = fmaf(sb, fmaf(-zb, sx.y, prod[j][3]), acc[j][3]);
           }
         }
       }
@@ -339,17 +355,16 @@ extern "C" int cdb_gemv_w4(const void* x, int64_t ldx, const void* w, int64_t ld
   const int blocks = (M + most - 1) / most;
   p.tokens = (M + blocks - 1) / blocks;
   const int nt = (p.tokens + 7) / 8;
-  // Warps on a row tile: the fewest boxes for the busiest warp, a sum over warps counted as one box. Few
-  // row tiles spread over k that way, many stay with a warp each.
+  // Warps on a row tile: the fewest boxes one after another in a warp (a sum over warps counted as half of
+  // one), for the row tiles that an SM gets. Few row tiles spread over k that way.
+  const int ctas = p.tiles < num_sms ? p.tiles : num_sms, share = (p.tiles + ctas - 1) / ctas;
   p.wk = 1;
   for (int w = 1, best = 0; w <= kWarps && w <= p.subs; w *= 2) {
-    const int groups = num_sms * (kWarps / w), rounds = (p.tiles + groups - 1) / groups;
-    const int cost = rounds * ((p.subs + w - 1) / w + (w > 1 ? 1 : 0));
+    const int rounds = (share + kWarps / w - 1) / (kWarps / w);
+    const int cost = rounds * (2 * ((p.subs + w - 1) / w) + (w > 1 ? 1 : 0));
     if (best == 0 || cost < best) best = cost, p.wk = w;
   }
-  const int per_cta = kWarps / p.wk;
-  const int ctas = (p.tiles + per_cta - 1) / per_cta;
-  const dim3 grid(ctas < num_sms ? ctas : num_sms, blocks);
+  const dim3 grid(ctas, blocks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (gi == 1) return launch_tokens<1>(map, p, grid, nt, st);
   if (gi == 2) return launch_tokens<2>(map, p, grid, nt, st);
