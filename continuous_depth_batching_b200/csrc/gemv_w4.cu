@@ -55,6 +55,12 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+__device__ __forceinline__ uint32_t load_shared(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -62,6 +68,16 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// D = A B: the first product of a sum.
+__device__ __forceinline__ void mma_bf16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // The 8 nibbles of a word as bf16 pairs 128 + q, of k (0, 2) (4, 6) (1, 3) (5, 7): the nibbles become bytes,
@@ -156,48 +172,58 @@ __global__ void __launch_bounds__(kWarps * 32, 1) gemv_kernel(const __grid_const
   bool ok = true;
   // The scales and zero points of a box: 2 GN (row half, group) entries, each loaded once in the four lanes of
   // a row (entry e in lane e % 4) as scale bits and zero point in one word, a box ahead of their use.
-  uint32_t entry[(GN + 1) / 2];
-  auto load_entries = [&](int tile, int i) {
+  constexpr int EN = GN / 2;
+  uint32_t entry[EN];
+  int64_t entry_row[EN];  // place of each row's first group
+  auto entry_tile = [&](int tile) {
 #pragma unroll
-    for (int k = 0; k < (GN + 1) / 2; ++k) {
-      const int e = t + 4 * k, row = min(tile * kRows + g + 8 * (e / GN), p.n - 1);
-      int grp = (sub0 + i) * GN + e % GN;
+    for (int k = 0; k < EN; ++k)
+      entry_row[k] = (int64_t)min(tile * kRows + g + 8 * ((t + 4 * k) / GN), p.n - 1) * p.groups;
+  };
+  auto load_entries = [&](int i) {
+#pragma unroll
+    for (int k = 0; k < EN; ++k) {
+      int grp = (sub0 + i) * GN + (t + 4 * k) % GN;
       if (GI == 4 && p.group_boxes > 1) grp /= p.group_boxes;
-      const int64_t at = (int64_t)row * p.groups + min(grp, p.groups - 1);  // a box may reach past k, onto zeros of x
+      const int64_t at = entry_row[k] + min(grp, p.groups - 1);  // a box may reach past k, onto zeros of x
       entry[k] = ((uint32_t)__bfloat16_as_ushort(p.scales[at]) << 16) | (p.zeros != nullptr ? p.zeros[at] : 8u);
     }
   };
-  if (boxes > 0) load_entries(group, 0);
+  if (boxes > 0) {
+    entry_tile(group);
+    load_entries(0);
+  }
   for (int round = 0, tile = group; round < rounds; ++round, tile += groups) {
     const int row0 = tile * kRows;
     float acc[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
     for (int i = 0; i < subs; ++i) {
-      uint32_t now[(GN + 1) / 2];
+      uint32_t now[EN];
 #pragma unroll
-      for (int k = 0; k < (GN + 1) / 2; ++k) now[k] = entry[k];
-      if (i + 1 < subs) load_entries(tile, i + 1);
-      else if (round + 1 < rounds) load_entries(tile + groups, 0);
+      for (int k = 0; k < EN; ++k) now[k] = entry[k];
+      if (i + 1 < subs) {
+        load_entries(i + 1);
+      } else if (round + 1 < rounds) {
+        entry_tile(tile + groups);
+        load_entries(0);
+      }
       ok = ok && __all_sync(kFull, mbar_wait(&s_bar[warp][get], phase, p.status));
       if (!ok) break;
-      const uint8_t* w = ring + get * kTile + g * 128 + t * 4;
+      // word b of row g lies at (b ^ g) * 16: the place of word 0, with b's bits turned over
+      const uint32_t w = ring_u + get * kTile + g * 128 + (g << 4) + t * 4;
       float prod[NT][4];
 #pragma unroll
       for (int b = 0; b < 8; ++b) {
-        if (b % GI == 0) {
-#pragma unroll
-          for (int j = 0; j < NT; ++j) prod[j][0] = prod[j][1] = prod[j][2] = prod[j][3] = 0.f;
-        }
-        const uint32_t wa = *reinterpret_cast<const uint32_t*>(w + ((b ^ g) << 4));
-        const uint32_t wb = *reinterpret_cast<const uint32_t*>(w + 1024 + ((b ^ g) << 4));
+        const uint32_t wa = load_shared(w ^ (b << 4)), wb = load_shared((w ^ (b << 4)) + 1024);
         uint32_t ea[4], eb[4];
         nibbles(wa, ea);
         nibbles(wb, eb);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           const uint4 xv = *reinterpret_cast<const uint4*>(xrow[j] + i * 512 + b * 64);
-          mma_bf16(prod[j], ea[0], eb[0], ea[1], eb[1], xv.x, xv.y);
+          if (b % GI == 0) mma_bf16_first(prod[j], ea[0], eb[0], ea[1], eb[1], xv.x, xv.y);
+          else mma_bf16(prod[j], ea[0], eb[0], ea[1], eb[1], xv.x, xv.y);
           mma_bf16(prod[j], ea[2], eb[2], ea[3], eb[3], xv.z, xv.w);
         }
         if (b % GI == GI - 1) {
