@@ -3,7 +3,7 @@
 // Weights q are nibbles, two to a byte along k (low nibble first), as they are stored; no layout pass.
 //
 // Bound by the weights' bytes, N K / 2, and by the instructions around a weight: seven for eight weights to
-// take nibbles apart, then the products and each group's scale. One CTA of 16 warps an SM
+// take nibbles apart, then the products and each group's scale. One CTA of 16 or 24 warps an SM
 // keeps its token rows in shared memory for good; `wk` warps share a tile of 16 weight rows, each with its
 // part of k, and add their parts through shared memory; the groups of wk warps walk over the row tiles.
 // A warp streams its boxes (16 rows x 128 bytes = 256 k, TMA with a 128-byte swizzle, so that the loads
@@ -22,7 +22,8 @@
 namespace cdb {
 namespace w4 {
 
-constexpr int kWarps = 16;
+// Warps of a CTA (one CTA an SM) by its tiles of 8 tokens: one tile fits 80 registers a thread.
+__host__ __device__ constexpr int warps_of(int nt) { return nt == 1 ? 24 : 16; }
 constexpr int kRows = 16;  // weight rows of a tile
 constexpr int kSub = 256;  // k of one TMA box (128 bytes of a row)
 constexpr int kTile = kRows * kSub / 2;
@@ -93,9 +94,10 @@ __device__ __forceinline__ void nibbles(uint32_t w, uint32_t (&e)[4]) {
 // NT: tiles of 8 tokens. GI: 32-k blocks that share a scale within a box (1, 2, or 4 for groups of 128
 // and multiples of it).
 template <int NT, int GI>
-__global__ void __launch_bounds__(kWarps * 32, 1) gemv_kernel(const __grid_constant__ CUtensorMap wmap, const Params p) {
+__global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid_constant__ CUtensorMap wmap, const Params p) {
   pdl_trigger();
   constexpr int GN = 8 / GI;  // scales of a row in one box
+  constexpr int kWarps = warps_of(NT);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ __align__(8) uint64_t s_bar[kWarps][kMaxStages];
@@ -303,12 +305,14 @@ static EncodeFn encode_fn() {
 
 // Bytes of a CTA's shared memory but for the ring.
 static int64_t row_bytes(int subs, int nt, int gi, int tokens, int wk) {
+  const int kWarps = warps_of(nt);
   return 1024 + (int64_t)tokens * (subs * 512 + 64) + (int64_t)subs * (8 / gi) * nt * 8 * 4 +
          (wk > 1 ? (int64_t)kWarps * kRows * nt * 8 * 4 : 0);
 }
 
 template <int NT, int GI>
 static int launch(const CUtensorMap& map, Params p, dim3 grid, cudaStream_t st) {
+  constexpr int kWarps = warps_of(NT);
   const int64_t rest = row_bytes(p.subs, NT, GI, p.tokens, p.wk);
   p.stages = (int)((kSmem - rest) / (kWarps * kTile));
   if (p.stages > kMaxStages) p.stages = kMaxStages;
@@ -376,7 +380,7 @@ extern "C" int cdb_gemv_w4(const void* x, int64_t ldx, const void* w, int64_t ld
   int most = 0;
   for (int nt = 1; nt <= 4; ++nt)
     for (int tok = nt * 8 - 7; tok <= nt * 8; ++tok)
-      if (row_bytes(p.subs, nt, gi, tok, kWarps) + 2 * kWarps * kTile <= kSmem) most = tok;
+      if (row_bytes(p.subs, nt, gi, tok, 2) + 2 * warps_of(nt) * kTile <= kSmem) most = tok;
   if (most == 0) return CDB_ERR_UNSUPPORTED;  // K so long that one token row does not fit
   const int blocks = (M + most - 1) / most;
   p.tokens = (M + blocks - 1) / blocks;
@@ -385,8 +389,9 @@ extern "C" int cdb_gemv_w4(const void* x, int64_t ldx, const void* w, int64_t ld
   // one), for the row tiles that an SM gets. Few row tiles spread over k that way.
   const int ctas = p.tiles < num_sms ? p.tiles : num_sms, share = (p.tiles + ctas - 1) / ctas;
   p.wk = 1;
-  for (int w = 1, best = 0; w <= kWarps && w <= p.subs; w *= 2) {
-    const int rounds = (share + kWarps / w - 1) / (kWarps / w);
+  const int warps = warps_of(nt);
+  for (int w = 1, best = 0; warps % w == 0 && w <= p.subs; w *= 2) {
+    const int rounds = (share + warps / w - 1) / (warps / w);
     const int cost = rounds * (2 * ((p.subs + w - 1) / w) + (w > 1 ? 1 : 0));
     if (best == 0 || cost < best) best = cost, p.wk = w;
   }
