@@ -27,6 +27,7 @@ __host__ __device__ constexpr int warps_of(int nt) { return nt == 1 ? 24 : 16; }
 constexpr int kRows = 16;  // weight rows of a tile
 constexpr int kSub = 256;  // k of one TMA box (128 bytes of a row)
 constexpr int kTile = kRows * kSub / 2;
+constexpr int kPart = 20;  // pitch of 16 rows' sums: spreads the stores over the banks
 constexpr int kMaxStages = 4;
 constexpr int kSmem = 226 * 1024;  // dynamic shared memory that a CTA may take
 constexpr uint32_t kFull = 0xffffffffu;
@@ -42,7 +43,7 @@ struct Params {
   int group_boxes;  // 128-k spans of one group, for groups of 128 and more
   int subs;    // boxes along k
   int tiles;   // row tiles
-  int wk;      // warps that share a row tile (a power of two)
+  int wk;      // warps that share a row tile
   int tokens;  // token rows of a CTA (grid y counts blocks of them)
   int stages;
   int32_t* status;
@@ -56,10 +57,9 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-__device__ __forceinline__ uint32_t load_shared(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
+// The words of rows g and g + 8 of a box.
+__device__ __forceinline__ void load_rows(uint32_t addr, uint32_t& a, uint32_t& b) {
+  asm volatile("ld.shared.b32 %0, [%2];\n\tld.shared.b32 %1, [%2+1024];" : "=r"(a), "=r"(b) : "r"(addr) : "memory");
 }
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -110,10 +110,10 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid
   uint8_t* xs = smem + kWarps * p.stages * kTile;
   const int pitch = p.subs * 512 + 64;
   float* xsum = reinterpret_cast<float*>(xs + p.tokens * pitch);  // [subs * GN][NT * 8]
-  float* parts = xsum + p.subs * GN * NT * 8;                     // [warp][16 rows][NT * 8], where wk > 1
+  float* parts = xsum + p.subs * GN * NT * 8;                     // [warp][NT * 8][kPart], where wk > 1
 
   // this warp's place: part `part` of row tiles group, group + groups, ...
-  const int part = warp & (p.wk - 1);
+  const int part = warp % p.wk;
   const int groups = gridDim.x * (kWarps / p.wk);
   const int group = blockIdx.x + gridDim.x * (warp / p.wk);  // few tiles spread over the SMs first
   const int each = (p.subs + p.wk - 1) / p.wk;
@@ -140,27 +140,75 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid
       at_tile += groups;
     }
   };
-  // The weights come from no kernel of this library, so their loads need not wait for the predecessor.
+  // The weights and their scales come from no kernel of this library: they need not wait for the predecessor.
   while (issued < p.stages && issued < boxes) issue();
+  // The scales and zero points of a box: 2 GN (row half, group) entries, each loaded once in the four lanes of
+  // a row (entry e in lane e % 4) as scale bits and zero point in one word, a box ahead of their use.
+  constexpr int EN = GN / 2;
+  uint32_t entry[EN];
+  const __nv_bfloat16* entry_scale[EN];  // each row's first
+  const uint8_t* entry_zero[EN];
+  auto entry_tile = [&](int tile) {
+#pragma unroll
+    for (int k = 0; k < EN; ++k) {
+      const int64_t row = (int64_t)min(tile * kRows + g + 8 * ((t + 4 * k) / GN), p.n - 1) * p.groups;
+      entry_scale[k] = p.scales + row;
+      entry_zero[k] = p.zeros + row;
+    }
+  };
+  auto load_entries = [&](int i) {
+#pragma unroll
+    for (int k = 0; k < EN; ++k) {
+      int grp = (sub0 + i) * GN + (t + 4 * k) % GN;
+      if (GI == 4 && p.group_boxes > 1) grp /= p.group_boxes;
+      grp = min(grp, p.groups - 1);  // a box may reach past k, onto zeros of x
+      entry[k] = ((uint32_t)__bfloat16_as_ushort(entry_scale[k][grp]) << 16) | (p.zeros != nullptr ? entry_zero[k][grp] : 8u);
+    }
+  };
+  if (boxes > 0) {
+    entry_tile(group);
+    load_entries(0);
+  }
   pdl_wait();
 
-  // the token rows and the sums of x over each group: a warp takes one box of one token at a time
-  for (int j = warp; j < tokens * p.subs; j += kWarps) {
-    const int tok = j / p.subs, sb = j - tok * p.subs;
-    const int k = sb * kSub + lane * 8;
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (k < p.k) v = *reinterpret_cast<const uint4*>(p.x + (int64_t)(tok0 + tok) * p.ldx + k);
-    uint4 o;
-    o.x = __byte_perm(v.x, v.y, 0x5410);
-    o.y = __byte_perm(v.z, v.w, 0x5410);
-    o.z = __byte_perm(v.x, v.y, 0x7632);
-    o.w = __byte_perm(v.z, v.w, 0x7632);
-    *reinterpret_cast<uint4*>(xs + tok * pitch + sb * 512 + lane * 16) = o;
-    float sum = ((bf16lo(v.x) + bf16hi(v.x)) + (bf16lo(v.y) + bf16hi(v.y))) +
-                ((bf16lo(v.z) + bf16hi(v.z)) + (bf16lo(v.w) + bf16hi(v.w)));
+  // the token rows and the sums of x over each group: a warp takes boxes of tokens, several loads in flight
+  constexpr int AT_ONCE = 2 * NT;
+  {
+    const int step_tok = kWarps / p.subs, step_sub = kWarps - step_tok * p.subs;
+    int tok = warp / p.subs, sub = warp - tok * p.subs;  // this warp's next box of tokens
+    while (tok < tokens) {
+      uint4 v[AT_ONCE];
+      int toks[AT_ONCE], places[AT_ONCE];
 #pragma unroll
-    for (int d = 1; d < 4 * GI; d <<= 1) sum += __shfl_xor_sync(kFull, sum, d);
-    if (lane % (4 * GI) == 0) xsum[(sb * GN + lane / (4 * GI)) * (NT * 8) + tok] = sum;
+      for (int a = 0; a < AT_ONCE; ++a) {
+        const int k = sub * kSub + lane * 8;
+        v[a] = make_uint4(0u, 0u, 0u, 0u);
+        if (tok < tokens && k < p.k) v[a] = *reinterpret_cast<const uint4*>(p.x + (int64_t)(tok0 + tok) * p.ldx + k);
+        toks[a] = tok;
+        places[a] = sub;
+        tok += step_tok;
+        sub += step_sub;
+        if (sub >= p.subs) sub -= p.subs, ++tok;
+      }
+      float sum[AT_ONCE];
+#pragma unroll
+      for (int a = 0; a < AT_ONCE; ++a)
+        sum[a] = ((bf16lo(v[a].x) + bf16hi(v[a].x)) + (bf16lo(v[a].y) + bf16hi(v[a].y))) +
+                 ((bf16lo(v[a].z) + bf16hi(v[a].z)) + (bf16lo(v[a].w) + bf16hi(v[a].w)));
+#pragma unroll
+      for (int d = 1; d < 4 * GI; d <<= 1) {
+#pragma unroll
+        for (int a = 0; a < AT_ONCE; ++a) sum[a] += __shfl_xor_sync(kFull, sum[a], d);
+      }
+#pragma unroll
+      for (int a = 0; a < AT_ONCE; ++a) {
+        if (toks[a] >= tokens) break;
+        *reinterpret_cast<uint4*>(xs + toks[a] * pitch + places[a] * 512 + lane * 16) =
+            make_uint4(__byte_perm(v[a].x, v[a].y, 0x5410), __byte_perm(v[a].z, v[a].w, 0x5410),
+                       __byte_perm(v[a].x, v[a].y, 0x7632), __byte_perm(v[a].z, v[a].w, 0x7632));
+        if (lane % (4 * GI) == 0) xsum[(places[a] * GN + lane / (4 * GI)) * (NT * 8) + toks[a]] = sum[a];
+      }
+    }
   }
   __syncthreads();
 
@@ -172,29 +220,6 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid
   int get = 0;
   uint32_t phase = 0;
   bool ok = true;
-  // The scales and zero points of a box: 2 GN (row half, group) entries, each loaded once in the four lanes of
-  // a row (entry e in lane e % 4) as scale bits and zero point in one word, a box ahead of their use.
-  constexpr int EN = GN / 2;
-  uint32_t entry[EN];
-  int64_t entry_row[EN];  // place of each row's first group
-  auto entry_tile = [&](int tile) {
-#pragma unroll
-    for (int k = 0; k < EN; ++k)
-      entry_row[k] = (int64_t)min(tile * kRows + g + 8 * ((t + 4 * k) / GN), p.n - 1) * p.groups;
-  };
-  auto load_entries = [&](int i) {
-#pragma unroll
-    for (int k = 0; k < EN; ++k) {
-      int grp = (sub0 + i) * GN + (t + 4 * k) % GN;
-      if (GI == 4 && p.group_boxes > 1) grp /= p.group_boxes;
-      const int64_t at = entry_row[k] + min(grp, p.groups - 1);  // a box may reach past k, onto zeros of x
-      entry[k] = ((uint32_t)__bfloat16_as_ushort(p.scales[at]) << 16) | (p.zeros != nullptr ? p.zeros[at] : 8u);
-    }
-  };
-  if (boxes > 0) {
-    entry_tile(group);
-    load_entries(0);
-  }
   for (int round = 0, tile = group; round < rounds; ++round, tile += groups) {
     const int row0 = tile * kRows;
     float acc[NT][4];
@@ -210,14 +235,18 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid
         entry_tile(tile + groups);
         load_entries(0);
       }
-      ok = ok && __all_sync(kFull, mbar_wait(&s_bar[warp][get], phase, p.status));
-      if (!ok) break;
+      if (!__all_sync(kFull, mbar_try_wait(&s_bar[warp][get], phase)) &&
+          !__all_sync(kFull, mbar_wait(&s_bar[warp][get], phase, p.status))) {
+        ok = false;
+        break;
+      }
       // word b of row g lies at (b ^ g) * 16: the place of word 0, with b's bits turned over
       const uint32_t w = ring_u + get * kTile + g * 128 + (g << 4) + t * 4;
       float prod[NT][4];
 #pragma unroll
       for (int b = 0; b < 8; ++b) {
-        const uint32_t wa = load_shared(w ^ (b << 4)), wb = load_shared((w ^ (b << 4)) + 1024);
+        uint32_t wa, wb;
+        load_rows(w ^ (b << 4), wa, wb);
         uint32_t ea[4], eb[4];
         nibbles(wa, ea);
         nibbles(wb, eb);
@@ -262,20 +291,24 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid
       continue;
     }
     // the wk warps' parts, added in order
-    float* mine = parts + warp * (kRows * NT * 8);
+    constexpr int PART = NT * 8 * kPart;
+    float* mine = parts + warp * PART;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) mine[(j * 8 + 2 * t + (c & 1)) * kRows + g + 8 * (c >> 1)] = acc[j][c];
+      for (int c = 0; c < 4; ++c) mine[(j * 8 + 2 * t + (c & 1)) * kPart + g + 8 * (c >> 1)] = acc[j][c];
     }
-    const int first = warp & ~(p.wk - 1), id = 1 + warp / p.wk, threads = p.wk * 32;
+    const int id = 1 + warp / p.wk, threads = p.wk * 32;
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-    const float* from = parts + first * (kRows * NT * 8);
-    for (int e = part * 32 + lane; e < tokens * kRows; e += threads) {
-      float v = 0.f;
-      for (int w = 0; w < p.wk; ++w) v += from[w * (kRows * NT * 8) + e];
-      const int tok = e / kRows, row = row0 + e % kRows;
-      if (row < p.n) p.out[(int64_t)(tok0 + tok) * p.ldo + row] = f_to_bf16(v);
+    const float* from = parts + (warp - part) * PART;
+    const int row = lane % kRows;
+    __nv_bfloat16* dst = p.out + (int64_t)tok0 * p.ldo + row0 + row;
+#pragma unroll 4
+    for (int tok = part * 2 + lane / kRows; tok < tokens; tok += p.wk * 2) {
+      float v = from[tok * kPart + row];
+#pragma unroll 4
+      for (int w = 1; w < p.wk; ++w) v += from[w * PART + tok * kPart + row];
+      if (row0 + row < p.n) dst[(int64_t)tok * p.ldo] = f_to_bf16(v);
     }
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
   }
@@ -307,7 +340,7 @@ static EncodeFn encode_fn() {
 static int64_t row_bytes(int subs, int nt, int gi, int tokens, int wk) {
   const int kWarps = warps_of(nt);
   return 1024 + (int64_t)tokens * (subs * 512 + 64) + (int64_t)subs * (8 / gi) * nt * 8 * 4 +
-         (wk > 1 ? (int64_t)kWarps * kRows * nt * 8 * 4 : 0);
+         (wk > 1 ? (int64_t)kWarps * kPart * nt * 8 * 4 : 0);
 }
 
 template <int NT, int GI>
@@ -390,7 +423,8 @@ extern "C" int cdb_gemv_w4(const void* x, int64_t ldx, const void* w, int64_t ld
   const int ctas = p.tiles < num_sms ? p.tiles : num_sms, share = (p.tiles + ctas - 1) / ctas;
   p.wk = 1;
   const int warps = warps_of(nt);
-  for (int w = 1, best = 0; warps % w == 0 && w <= p.subs; w *= 2) {
+  for (int w = 1, best = 0; w <= warps && w <= p.subs; ++w) {
+    if (warps % w != 0) continue;
     const int rounds = (share + warps / w - 1) / (warps / w);
     const int cost = rounds * (2 * ((p.subs + w - 1) / w) + (w > 1 ? 1 : 0));
     if (best == 0 || cost < best) best = cost, p.wk = w;
