@@ -59,6 +59,11 @@ struct DecodeParams {
   int32_t* status;
 };
 
+// a / b for a, b >= 0: a 64-bit division takes some 400 cycles, and the numbers nearly always fit 32 bits.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
 // Pairs of cached pages of row b; 0 for a padding row and for one whose indexes do not fit the table.
 __device__ __forceinline__ int row_pairs(const DecodeParams& p, int b, bool& bad) {
   const int pos = p.item_pos[b], slot = p.item_slot[b];
@@ -75,15 +80,23 @@ struct Cursor {
   int row, kvh, grp, pair, pairs, pos, slot;
 };
 
-__device__ __forceinline__ void load_row(const DecodeParams& p, Cursor& c) {
-  bool bad = false;
-  c.pairs = row_pairs(p, c.row, bad);
-  c.pos = p.item_pos[c.row];
-  c.slot = p.item_slot[c.row];
+// Its row's position, slot and pairs. `rows`: {position, slot} of every row in shared memory (a row that does
+// not count has position -1), or null where there are more rows than threads.
+__device__ __forceinline__ void load_row(const DecodeParams& p, const int2* rows, Cursor& c) {
+  if (rows != nullptr) {
+    c.pos = rows[c.row].x;
+    c.slot = rows[c.row].y;
+    c.pairs = c.pos < 0 ? 0 : c.pos / (2 * kBlock) + 1;
+  } else {
+    bool bad = false;
+    c.pairs = row_pairs(p, c.row, bad);
+    c.pos = p.item_pos[c.row];
+    c.slot = p.item_slot[c.row];
+  }
 }
 
 // To the next pair.
-__device__ __forceinline__ void advance(const DecodeParams& p, Cursor& c) {
+__device__ __forceinline__ void advance(const DecodeParams& p, const int2* rows, Cursor& c) {
   if (++c.pair < c.pairs) return;
   c.pair = 0;
   if (++c.grp < p.groups) return;
@@ -92,7 +105,7 @@ __device__ __forceinline__ void advance(const DecodeParams& p, Cursor& c) {
   c.kvh = 0;
   do {
     if (++c.row >= p.num_items) return;  // the stream's end
-    load_row(p, c);
+    load_row(p, rows, c);
   } while (c.pairs == 0);
 }
 
@@ -171,22 +184,27 @@ struct Running {
 
 // q's rows of one segment as the B operand: head g of the group, dims [t * KD, (t + 1) * KD). e is the
 // power of two that was divided out (for heads 2t and 2t + 1).
-template <int D, int HN>
-__device__ __forceinline__ void load_q(const DecodeParams& p, const Cursor& c, uint32_t (&qf)[Shape<D>::KS][2],
-                                       float (&factor)[HN]) {
+template <int D>
+__device__ __forceinline__ void fetch_q(const DecodeParams& p, const Cursor& c, uint32_t (&w)[D / 8]) {
   constexpr int KD = Shape<D>::KD;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int in_kv = c.grp * kGroup + g;
   const bool on = in_kv < p.heads_per_kv;
   const __nv_bfloat16* src =
       p.q + (int64_t)c.row * p.q_stride + (int64_t)(c.kvh * p.heads_per_kv + (on ? in_kv : 0)) * D + t * KD;
-  uint32_t w[KD / 2];
 #pragma unroll
   for (int i = 0; i < KD / 8; ++i) {
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (on) v = *reinterpret_cast<const uint4*>(src + i * 8);
     w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
   }
+}
+
+template <int D, int HN>
+__device__ __forceinline__ void convert_q(const DecodeParams& p, const uint32_t (&w)[D / 8],
+                                          uint32_t (&qf)[Shape<D>::KS][2], float (&factor)[HN]) {
+  constexpr int KD = Shape<D>::KD;
+  const int t = threadIdx.x & 3;
   float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < KD / 2; ++i) amax = fmaxf(amax, fmaxf(fabsf(bf16lo(w[i])), fabsf(bf16hi(w[i]))));
@@ -408,6 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int64_t s_before[kThreads + 1];  // pairs before each thread's rows
   __shared__ int64_t s_warp[kWarps];
   __shared__ int s_most[kWarps];
+  __shared__ int2 s_row[kThreads];
   __shared__ PieceTag s_tag[kWarps][2];
   __shared__ __align__(8) uint64_t s_bar[kWarps][kMaxStages];
   __shared__ __align__(16) float s_scale[kWarps][kMaxStages][4];
@@ -425,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     return slot ? reinterpret_cast<float*>(smem + (size_t)w * ring_bytes) : first_pieces + w * piece_floats;
   };
   if (lane == 0) {
-    for (int i = 0; i < p.stages; ++i) mbar_init(&s_bar[warp][i], 2);
+    for (int i = 0; i < p.stages; ++i) mbar_init(&s_bar[warp][i], 5);  // expected bytes, and four lanes' scales
     fence_barrier_init();
     s_tag[warp][0].row = s_tag[warp][1].row = -1;
   }
@@ -433,6 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // ---- the stream: pairs before every thread's rows
   const int per = (p.num_items + kThreads - 1) / kThreads;
+  const int2* rows = per == 1 ? s_row : nullptr;
   int longest;
   {
     int64_t mine = 0;
@@ -442,6 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int n = row_pairs(p, b, bad);
       mine += n;
       most = max(most, n);
+      if (per == 1) s_row[b] = make_int2(n > 0 ? p.item_pos[b] : -1, p.item_slot[b]);
     }
     if (bad && blockIdx.x == 0) set_error(p.status, CDB_ERR_INDEX);
     int64_t x = mine;
@@ -466,44 +487,47 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
   }
   const int64_t total = s_before[kThreads] * vheads;
-  const int64_t even = (total + gridDim.x - 1) / gridDim.x;
+  const int64_t even = quotient(total + gridDim.x - 1, gridDim.x);
   const int64_t share = even > p.min_share ? even : p.min_share;
   int64_t begin = share * blockIdx.x, end = begin + share < total ? begin + share : total;
   if ((int64_t)p.num_items * vheads <= gridDim.x && longest <= p.whole_pairs) {
     // Few short segments: a CTA for each, so that none has to meet another's piece in the workspace.
     const int row = blockIdx.x / vheads, vh = blockIdx.x - row * vheads;
     if (row >= p.num_items) return;
-    bool bad = false;
-    const int n = row_pairs(p, row, bad);
+    const int n = s_row[row].x < 0 ? 0 : s_row[row].x / (2 * kBlock) + 1;
     begin = s_before[row] * vheads + (int64_t)vh * n;  // (per is 1: rows are fewer than CTAs)
     end = begin + n;
   }
   if (begin >= end) return;  // uniform over the CTA
-  const int64_t wshare = (end - begin + kWarps - 1) / kWarps;
+  const int64_t wshare = quotient(end - begin + kWarps - 1, kWarps);
   const int64_t wbegin = begin + wshare * warp;
   const int count = (int)((wbegin + wshare < end ? wbegin + wshare : end) - wbegin);  // this warp's pairs, if > 0
 
   if (count > 0) {
     // the row that holds pair wbegin
     Cursor c;
-    int lo = 0, hi = kThreads;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_before[mid] * vheads <= wbegin) lo = mid; else hi = mid;
-    }
+    // the last of the threads whose rows begin at or before it, found by two looks of the warp
+    static_assert(kThreads % 32 == 0 && kThreads / 32 <= 32, "32 samples, then the stretch between two");
+    constexpr int STRETCH = kThreads / 32;
+    const unsigned far = __ballot_sync(kFull, s_before[lane * STRETCH] * vheads <= wbegin);
+    const int near = (31 - __clz(far)) * STRETCH;
+    const unsigned in = __ballot_sync(kFull, lane < STRETCH && s_before[near + lane] * vheads <= wbegin);
+    const int lo = near + 31 - __clz(in);
     int64_t at = wbegin - s_before[lo] * vheads;
     c.row = lo * per;
-    load_row(p, c);
+    load_row(p, rows, c);
     while (at >= (int64_t)c.pairs * vheads) {
       at -= (int64_t)c.pairs * vheads;
       ++c.row;
-      load_row(p, c);
+      load_row(p, rows, c);
     }
-    const int vh = (int)(at / c.pairs);
+    const int vh = (int)quotient(at, c.pairs);
     c.pair = (int)(at - (int64_t)vh * c.pairs);
-    c.kvh = vh / p.groups;
+    c.kvh = p.groups == 1 ? vh : vh / p.groups;
     c.grp = vh - c.kvh * p.groups;
 
+    uint32_t qraw[D / 8];
+    fetch_q<D>(p, c, qraw);  // before the pages, which would keep it waiting
     const int v_tiles = p.num_blocks * p.kv_heads;
     const uint32_t ring_u = smem_u32(ring), bar_u = smem_u32(&s_bar[warp][0]), scale_u = smem_u32(&s_scale[warp][0][0]);
     Cursor ahead = c;
@@ -518,34 +542,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         win_id = first + lane <= ahead.pos / kBlock ? p.block_table[(int64_t)ahead.slot * p.bt_stride + first + lane]
                                                      : INT32_MIN;  // behind the row's last page
       }
-      const int id[2] = {__shfl_sync(kFull, win_id, page & 31), __shfl_sync(kFull, win_id, (page & 31) + 1)};
-      if (lane == 0) {
-        const uint32_t bar = bar_u + put * 8, dst = ring_u + put * PAIR, to = scale_u + put * 16;
-        const bool ok[2] = {id[0] >= 0 && id[0] < p.num_blocks, id[1] >= 0 && id[1] < p.num_blocks};
-        mbar_arrive_expect_tx(&s_bar[warp][put], (ok[0] ? 2 * TILE : 0) + (ok[1] ? 2 * TILE : 0));
-#pragma unroll
-        for (int pg = 0; pg < 2; ++pg) {
-          if (ok[pg]) {
-            const int tile = id[pg] * p.kv_heads + ahead.kvh;
-            if (Shape<D>::SWIZZLED) {
-              tensor_load(dst + pg * 2 * TILE, &map, tile * kBlock, bar);
-              tensor_load(dst + pg * 2 * TILE + TILE, &map, (v_tiles + tile) * kBlock, bar);
-            } else {
-              bulk_load(dst + pg * 2 * TILE, p.codes + (int64_t)tile * TILE, TILE, bar);
-              bulk_load(dst + pg * 2 * TILE + TILE, p.codes + (int64_t)(v_tiles + tile) * TILE, TILE, bar);
-            }
-            async_copy4(to + pg * 8, p.scales + tile);
-            async_copy4(to + pg * 8 + 4, p.scales + v_tiles + tile);
-          } else {
-            if (id[pg] != INT32_MIN) set_error(p.status, CDB_ERR_INDEX);
-            s_scale[warp][put][2 * pg] = -1.f;
-          }
+      // lane 0: K of the first page, 1: its V, 2 and 3: the second's
+      const int id = __shfl_sync(kFull, win_id, (page & 31) + ((lane >> 1) & 1));
+      const bool ok = id >= 0 && id < p.num_blocks;
+      const int known = __popc(__ballot_sync(kFull, ok && lane < 4));
+      const uint32_t bar = bar_u + put * 8;
+      if (lane == 0) mbar_arrive_expect_tx(&s_bar[warp][put], known * TILE);
+      __syncwarp();
+      if (lane < 4) {
+        const int tile = (lane & 1 ? v_tiles : 0) + id * p.kv_heads + ahead.kvh;
+        if (ok) {
+          const uint32_t dst = ring_u + put * PAIR + lane * TILE;
+          if (Shape<D>::SWIZZLED) tensor_load(dst, &map, tile * kBlock, bar);
+          else bulk_load(dst, p.codes + (int64_t)tile * TILE, TILE, bar);
+          async_copy4(scale_u + put * 16 + lane * 4, p.scales + tile);
+          async_arrive(bar);
+        } else {
+          if (id != INT32_MIN) set_error(p.status, CDB_ERR_INDEX);
+          s_scale[warp][put][lane] = -1.f;
+          mbar_arrive(&s_bar[warp][put]);
         }
-        async_arrive(bar);
       }
-      __syncwarp();  // lane 0's own stores to s_scale
       put = put + 1 == p.stages ? 0 : put + 1;
-      if (++issued < count) advance(p, ahead);
+      if (++issued < count) advance(p, rows, ahead);
     };
     for (int i = 0; i < p.stages && issued < count; ++i) issue();
 
@@ -558,7 +577,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < count; ++i) {
       if (fresh) {
         first = c.pair;
-        load_q<D, HN>(p, c, qf, factor);
+        if (i > 0) fetch_q<D>(p, c, qraw);
+        convert_q<D, HN>(p, qraw, qf, factor);
         r.clear();
       }
       if (!__all_sync(kFull, mbar_wait(&s_bar[warp][get], phase, p.status))) {
@@ -595,108 +615,111 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (i + 1 < count) advance(p, c);
+      if (i + 1 < count) advance(p, rows, c);
     }
   }
   __syncthreads();
 
-  // ---- join the pieces. Every warp sees which pieces belong together (lane j holds the tag of piece j);
-  // the (segment, head) pairs are dealt over the warps.
+  // ---- join the pieces. Every warp sees which pieces belong together (lane j holds the tag of piece j); head h
+  // of a segment falls to the warp h places after the one that its first piece comes from.
   static_assert(2 * kWarps <= 32, "a lane per piece");
   const PieceTag tag = s_tag[lane < 2 * kWarps ? lane >> 1 : 0][lane & 1];
   const bool used = lane < 2 * kWarps && tag.row >= 0;
   const int64_t key = used ? ((int64_t)tag.row * p.kv_heads + tag.kvh) * p.groups + tag.grp : -1 - lane;
   const unsigned group = __match_any_sync(kFull, key);
   unsigned leaders = __ballot_sync(kFull, used && (group & ((1u << lane) - 1u)) == 0u);
-  int task = 0;
+  if (p.stored_heads == 1) leaders &= 3u << (2 * warp);
   for (; leaders; leaders &= leaders - 1) {
     const int lead = __ffs(leaders) - 1;
+    int h = warp - (lead >> 1);
+    if (h < 0) h += kWarps;
+    if (h >= p.stored_heads) continue;
     const unsigned members = __shfl_sync(kFull, group, lead);
     const int row = __shfl_sync(kFull, tag.row, lead), kvh = __shfl_sync(kFull, tag.kvh, lead);
     const int grp = __shfl_sync(kFull, tag.grp, lead), pairs = __shfl_sync(kFull, tag.pairs, lead);
     const int first = __shfl_sync(kFull, tag.first, lead), last = __shfl_sync(kFull, tag.last, 31 - __clz(members));
-    const bool whole = first == 0 && last == pairs;
-    const int heads = min(kGroup, p.heads_per_kv - grp * kGroup);
-    for (int h = 0; h < heads; ++h, ++task) {
-      if (task % kWarps != warp) continue;
-      const bool mine = (members >> lane) & 1u;
-      const float* piece = mine ? place(lane >> 1, lane & 1) + h * (D + 2) : nullptr;
-      const float pm = mine ? piece[D] : -INFINITY;
-      float m = warp_max(pm);
-      const float pf = pm == -INFINITY ? 0.f : ex2(pm - m);
-      float l = warp_sum(mine ? piece[D + 1] * pf : 0.f);
-      float o[D / 32];
+    if (grp * kGroup + h >= p.heads_per_kv) continue;
+    const bool mine = (members >> lane) & 1u;
+    const float* piece = mine ? place(lane >> 1, lane & 1) + h * (D + 2) : nullptr;
+    const float pm = mine ? piece[D] : -INFINITY;
+    float m = warp_max(pm);
+    const float pf = pm == -INFINITY ? 0.f : ex2(pm - m);
+    float l = warp_sum(mine ? piece[D + 1] * pf : 0.f);
+    float o[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
+    const int end = 32 - __clz(members);
+#pragma unroll 2
+    for (int j = lead; j < end; ++j) {
+      const float f = __shfl_sync(kFull, pf, j);
+      if (!((members >> j) & 1u)) continue;
+      const float* src = place(j >> 1, j & 1) + h * (D + 2) + lane;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) o[i] += src[i * 32] * f;
+    }
+    if (first != 0 || last != pairs) {
+      // The segment goes on in other CTAs, which follow from its first pair's place in the stream. This CTA's
+      // piece goes to the workspace; whoever is last adds all of them up, in CTA order.
+      int64_t before = s_before[row / per];
+      for (int b = row / per * per; b < row; ++b) {
+        bool bad = false;
+        before += row_pairs(p, b, bad);
+      }
+      const int64_t seg0 = before * vheads + (int64_t)(kvh * p.groups + grp) * pairs;
+      const int c0 = (int)quotient(seg0, share), c1 = (int)quotient(seg0 + pairs - 1, share);
+      const int64_t head_floats = D + 2;
+      float* dst = p.parts + ((int64_t)blockIdx.x * 2 + (first > 0 ? 0 : 1)) * piece_floats + h * head_floats;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) __stcg(dst + i * 32 + lane, o[i]);
+      if (lane == 0) {
+        __stcg(dst + D, m);
+        __stcg(dst + D + 1, l);
+      }
+      __threadfence();
+      __syncwarp();
+      int arrived = 0;
+      if (lane == 0) arrived = atomicAdd(p.counters + c0 * kGroup + h, 1);
+      arrived = __shfl_sync(kFull, arrived, 0);
+      if (arrived != c1 - c0) continue;
+      __threadfence();
+      if (lane == 0) p.counters[c0 * kGroup + h] = 0;  // as the next launch expects it
+      // the segment begins in c0's second place and goes on in the others' first
+      auto part_of = [&](int cta) {
+        return p.parts + ((int64_t)cta * 2 + (cta == c0 ? 1 : 0)) * piece_floats + h * head_floats;
+      };
+      m = -INFINITY;
+      l = 0.f;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
-      for (unsigned b = members; b; b &= b - 1) {
-        const int j = __ffs(b) - 1;
-        const float f = __shfl_sync(kFull, pf, j);
-        const float* src = place(j >> 1, j & 1) + h * (D + 2) + lane;
+#pragma unroll 1
+      for (int c = c0; c <= c1; c += 32) {  // 32 pieces at a time
+        const bool on = c + lane <= c1;
+        const float qm = on ? __ldcg(part_of(c + lane) + D) : -INFINITY;
+        const float ql = on ? __ldcg(part_of(c + lane) + D + 1) : 0.f;
+        const float nm = fmaxf(m, warp_max(qm));
+        const float down = m == -INFINITY ? 0.f : ex2(m - nm), qf2 = qm == -INFINITY ? 0.f : ex2(qm - nm);
+        l = l * down + warp_sum(ql * qf2);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) o[i] += src[i * 32] * f;
-      }
-      if (!whole) {
-        // The CTAs that share the segment, from its first pair's place in the stream. This CTA's piece goes
-        // to the workspace; whoever is last adds all of them up, in CTA order.
-        int64_t before = s_before[row / per];
-        for (int b = row / per * per; b < row; ++b) {
-          bool bad = false;
-          before += row_pairs(p, b, bad);
-        }
-        const int64_t seg0 = before * vheads + (int64_t)(kvh * p.groups + grp) * pairs;
-        const int c0 = (int)(seg0 / share), c1 = (int)((seg0 + pairs - 1) / share);
-        const int64_t head_floats = D + 2;
-        float* dst = p.parts + ((int64_t)blockIdx.x * 2 + (first > 0 ? 0 : 1)) * piece_floats + h * head_floats;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) __stcg(dst + i * 32 + lane, o[i]);
-        if (lane == 0) {
-          __stcg(dst + D, m);
-          __stcg(dst + D + 1, l);
-        }
-        __threadfence();
-        __syncwarp();
-        int arrived = 0;
-        if (lane == 0) arrived = atomicAdd(p.counters + c0 * kGroup + h, 1);
-        arrived = __shfl_sync(kFull, arrived, 0);
-        if (arrived != c1 - c0) continue;
-        __threadfence();
-        if (lane == 0) p.counters[c0 * kGroup + h] = 0;  // as the next launch expects it
-        // the segment begins in c0's second place and goes on in the others' first
-        auto part = [&](int cta) {
-          return p.parts + ((int64_t)cta * 2 + (cta == c0 ? 1 : 0)) * piece_floats + h * head_floats;
-        };
-        m = -INFINITY;
-        l = 0.f;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
-        for (int c = c0; c <= c1; c += 32) {  // 32 pieces at a time
-          const bool on = c + lane <= c1;
-          const float qm = on ? __ldcg(part(c + lane) + D) : -INFINITY, ql = on ? __ldcg(part(c + lane) + D + 1) : 0.f;
-          const float nm = fmaxf(m, warp_max(qm));
-          const float down = m == -INFINITY ? 0.f : ex2(m - nm), qf2 = qm == -INFINITY ? 0.f : ex2(qm - nm);
-          l = l * down + warp_sum(ql * qf2);
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) o[i] *= down;
-          m = nm;
-          const int n = min(32, c1 - c + 1);
+        for (int i = 0; i < D / 32; ++i) o[i] *= down;
+        m = nm;
+        const int n = min(32, c1 - c + 1);
 #pragma unroll 4
-          for (int j = 0; j < n; ++j) {
-            const float f = __shfl_sync(kFull, qf2, j);
-            const float* src = part(c + j) + lane;
+        for (int j = 0; j < n; ++j) {
+          const float f = __shfl_sync(kFull, qf2, j);
+          const float* src = part_of(c + j) + lane;
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) o[i] += __ldcg(src + i * 32) * f;
-          }
+          for (int i = 0; i < D / 32; ++i) o[i] += __ldcg(src + i * 32) * f;
         }
       }
-      const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-      __nv_bfloat16* dst = p.out + (int64_t)row * p.out_stride + (int64_t)(kvh * p.heads_per_kv + grp * kGroup + h) * D;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) dst[i * 32 + lane] = f_to_bf16(o[i] * f);
     }
+    const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    __nv_bfloat16* dst = p.out + (int64_t)row * p.out_stride + (int64_t)(kvh * p.heads_per_kv + grp * kGroup + h) * D;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) dst[i * 32 + lane] = f_to_bf16(o[i] * f);
   }
 }
 
-constexpr int kSmemLimit = 220 * 1024;  // dynamic, beside 5 KB of static shared memory
+constexpr int kSmemLimit = 218 * 1024;  // dynamic, beside 8 KB of static shared memory
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
