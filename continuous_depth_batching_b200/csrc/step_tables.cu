@@ -44,31 +44,46 @@ struct Params {
   int32_t* status;
 };
 
-// Block-wide exclusive scan of one value per thread; total receives the sum.
-__device__ __forceinline__ int64_t scan(int64_t v, int64_t* s_warp, int64_t& total) {
+// What is summed over the requests: blocks taken, new tokens, keys, tiles.
+constexpr int kSums = 4;
+struct Sums {
+  int64_t v[kSums];
+  __device__ __forceinline__ void add(const Sums& o) {
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) v[i] += o.v[i];
+  }
+};
+
+// Block-wide exclusive scan of one Sums per thread; total receives the sum.
+__device__ __forceinline__ Sums scan(const Sums& mine, Sums* s_warp, Sums& total) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int64_t x = v;
+  Sums x = mine, y, before;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) {
+      const int64_t t = __shfl_up_sync(0xffffffffu, x.v[i], o);
+      if (lane >= o) x.v[i] += t;
+    }
   }
   if (lane == 31) s_warp[w] = x;
   __syncthreads();
-  if (w == 0) {
-    int64_t y = s_warp[lane];
+  y = s_warp[lane];  // every warp sums the warps before it
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t z = __shfl_up_sync(0xffffffffu, y, o);
-      if (lane >= o) y += z;
+  for (int o = 1; o < 32; o <<= 1) {
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) {
+      const int64_t t = __shfl_up_sync(0xffffffffu, y.v[i], o);
+      if (lane >= o) y.v[i] += t;
     }
-    s_warp[lane] = y;
   }
-  __syncthreads();
-  const int64_t before = w ? s_warp[w - 1] : 0;
-  total = s_warp[31];
-  __syncthreads();
-  return before + x - v;
+#pragma unroll
+  for (int i = 0; i < kSums; ++i) {
+    total.v[i] = __shfl_sync(0xffffffffu, y.v[i], 31);
+    const int64_t base = __shfl_sync(0xffffffffu, y.v[i], w > 0 ? w - 1 : 0);
+    before.v[i] = x.v[i] - mine.v[i] + (w > 0 ? base : 0);
+  }
+  return before;
 }
 
 // Largest j with first[j] <= i, first ascending from 0 over n entries.
@@ -84,7 +99,7 @@ __device__ __forceinline__ int find(const int32_t* first, int n, int i) {
 __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p, int ctas) {
   pdl_trigger();
   extern __shared__ int32_t smem[];
-  __shared__ int64_t s_warp[32];
+  __shared__ Sums s_warp[2][32];
   const int n = p.n, rank = blockIdx.x;
   int32_t* s_slot = smem;           // [n] -1: no such slot
   int32_t* s_ctx = s_slot + n;      // cached tokens
@@ -101,7 +116,6 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p, i
   const int per = (n + kThreads - 1) / kThreads;
   const int j0 = min(n, (int)threadIdx.x * per), j1 = min(n, j0 + per);
   bool bad = !sane;
-  int64_t want = 0;
   for (int j = j0; j < j1; ++j) {
     const int slot = p.slots[j], fresh = p.new_len[j];
     int ctx = 0, held = 0, need = -1;
@@ -120,11 +134,22 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p, i
     s_held[j] = held;
     s_need[j] = need;
     s_q[j] = fresh;
-    want += need > 0 ? need : 0;
   }
-  int64_t all, all_q, all_k, all_t;
-  scan(want, s_warp, all);
-  if (all > avail) {  // not enough for everybody: in order, whoever still fits
+  // What a request adds to the sums, and where they begin for this thread's requests.
+  auto adds = [&](int j) {
+    Sums a = {{0, 0, 0, 0}};
+    if (s_need[j] >= 0) a = {{s_need[j], s_q[j], (int64_t)s_ctx[j] + s_q[j], (s_q[j] + kTile - 1) / kTile}};
+    return a;
+  };
+  Sums all;
+  auto begin = [&](int which) {
+    Sums mine = {{0, 0, 0, 0}};
+    for (int j = j0; j < j1; ++j) mine.add(adds(j));
+    return scan(mine, s_warp[which], all);
+  };
+  Sums at = begin(0);
+  if (all.v[0] > avail) {  // not enough for everybody: in order, whoever still fits
+    __syncthreads();
     if (threadIdx.x == 0) {
       int left = avail;
       for (int j = 0; j < n; ++j)
@@ -132,43 +157,32 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p, i
         else if (s_need[j] > 0) left -= s_need[j];
     }
     __syncthreads();
+    at = begin(1);
   }
-  int64_t blocks = 0, toks = 0, keys = 0, tls = 0;
-  for (int j = j0; j < j1; ++j) {
-    if (s_need[j] < 0) s_q[j] = 0;
-    blocks += s_need[j] > 0 ? s_need[j] : 0;
-    toks += s_q[j];
-    keys += s_need[j] < 0 ? 0 : (int64_t)s_ctx[j] + s_q[j];
-    tls += (s_q[j] + kTile - 1) / kTile;
-  }
-  int64_t b0 = scan(blocks, s_warp, all), q0 = scan(toks, s_warp, all_q), k0 = scan(keys, s_warp, all_k),
-          t0 = scan(tls, s_warp, all_t);
+  const int64_t all_b = all.v[0], all_q = all.v[1], all_k = all.v[2], all_t = all.v[3];
   const bool fits = all_q <= p.cap && all_k <= 0x7fffffff && (p.tiles == nullptr || all_t <= p.tile_cap);
   if (ctas > 1)
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   // Nothing was written so far: every CTA has read slots, lengths and state.
   for (int j = j0; j < j1; ++j) {
-    const int fresh = s_q[j], need = s_need[j];
+    const Sums add = adds(j);
     if (rank == 0) {
-      p.granted[j] = need >= 0 ? 1 : 0;
-      p.cu_q[j] = (int)q0;
-      p.cu_k[j] = (int)k0;
-      if (need >= 0) p.row_len_out[s_slot[j]] = s_held[j] + need;
+      p.granted[j] = s_need[j] >= 0 ? 1 : 0;
+      p.cu_q[j] = (int)at.v[1];
+      p.cu_k[j] = (int)at.v[2];
+      if (s_need[j] >= 0) p.row_len_out[s_slot[j]] = s_held[j] + s_need[j];
     }
-    s_block[j] = (int)b0;
-    s_q[j] = (int)q0;
-    s_t[j] = (int)t0;
-    b0 += need > 0 ? need : 0;
-    q0 += fresh;
-    k0 += need < 0 ? 0 : (int64_t)s_ctx[j] + fresh;
-    t0 += (fresh + kTile - 1) / kTile;
+    s_block[j] = (int)at.v[0];
+    s_q[j] = (int)at.v[1];
+    s_t[j] = (int)at.v[3];
+    at.add(add);
   }
   if (rank == 0) {
     if (bad || !fits) set_error(p.status, CDB_ERR_INDEX);
     if (threadIdx.x == 0) {
       p.cu_q[n] = (int)all_q;
       p.cu_k[n] = (int)all_k;
-      const int taken = (int)all;
+      const int taken = (int)all_b;
       p.state_out[0] = sane && nb > 0 ? (int)(((int64_t)head + taken) % nb) : head;
       p.state_out[1] = avail - taken;
       p.state_out[2] = nb;
@@ -179,7 +193,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p, i
 
   const int first = rank * kThreads + threadIdx.x, step = ctas * kThreads;
   // new blocks into the tables
-  for (int i = first; i < (int)all; i += step) {
+  for (int i = first; i < (int)all_b; i += step) {
     const int j = find(s_block, n, i);  // the last request that starts at or before i: requests without blocks sort before
     p.table[(int64_t)s_slot[j] * p.table_stride + s_held[j] + i - s_block[j]] = p.ring[(int)(((int64_t)head + i) % nb)];
   }
