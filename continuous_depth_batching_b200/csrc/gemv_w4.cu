@@ -418,7 +418,8 @@ extern "C" int cdb_gemv_w4(const void* x, int64_t ldx, const void* w, int64_t ld
   if (most == 0) return CDB_ERR_UNSUPPORTED;  // K so long that one token row does not fit
   const int blocks = (M + most - 1) / most;
   p.tokens = (M + blocks - 1) / blocks;
-  const int nt = (p.tokens + 7) / 8;
+  int nt = (p.tokens + 7) / 8;  // one tile's 24 rings may not fit where two tiles' 16 do
+  while (row_bytes(p.subs, nt, gi, p.tokens, 2) + 2 * warps_of(nt) * kTile > kSmem) ++nt;
   // Warps on a row tile: the fewest boxes one after another in a warp (a sum over warps counted as half of
   // one), for the row tiles that an SM gets. Few row tiles spread over k that way.
   const int ctas = p.tiles < num_sms ? p.tiles : num_sms, share = (p.tiles + ctas - 1) / ctas;

@@ -17,7 +17,6 @@ namespace cdb {
 namespace kv8 {
 
 constexpr int kBlock = 16;
-constexpr float kMax = 448.f;  // largest finite e4m3
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Smallest power of two s (>= 2^-126) with amax <= 448 s; 448 = 1.75 * 2^8.

@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint8_t* codes, const
   }
 }
 
-static int done() { return cudaPeekAtLastError() == cudaSuccess ? CDB_OK : CDB_ERR_CUDA; }
+static int launched(cudaError_t e) { return e == cudaSuccess ? CDB_OK : CDB_ERR_CUDA; }
 
 }  // namespace kv8
 }  // namespace cdb
@@ -412,13 +412,9 @@ extern "C" int cdb_kv8_append(const void* qkv, int64_t qkv_stride, void* q_out, 
       (q_out != nullptr ? (p.group + rpi - 1) / rpi * ((num_heads + HB - 1) / HB) : 0) + 2 * num_kv_heads;
   const dim3 grid((num_items + p.group - 1) / p.group, min(65535, (tasks + 7) / 8));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128)
-    launch_pdl(append_kernel<128>, grid, dim3(256), 0, st, p);
-  else if (head_dim == 96)
-    launch_pdl(append_kernel<96>, grid, dim3(256), 0, st, p);
-  else
-    launch_pdl(append_kernel<64>, grid, dim3(256), 0, st, p);
-  return done();
+  return launched(head_dim == 128  ? launch_pdl(append_kernel<128>, grid, dim3(256), 0, st, p)
+                  : head_dim == 96 ? launch_pdl(append_kernel<96>, grid, dim3(256), 0, st, p)
+                                   : launch_pdl(append_kernel<64>, grid, dim3(256), 0, st, p));
 }
 
 extern "C" int cdb_kv8_gather(const void* codes, const float* scales, int num_cache_layers, int cache_layer,
@@ -435,8 +431,7 @@ extern "C" int cdb_kv8_gather(const void* codes, const float* scales, int num_ca
   const int64_t chunks = (int64_t)n * 2 * num_kv_heads * head_dim;  // 16 codes each
   const int64_t ctas = (chunks + 255) / 256;
   const int grid = (int)(ctas < 148 * 16 ? ctas : 148 * 16);
-  launch_pdl(gather_kernel, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream),
-             static_cast<const uint8_t*>(codes) + tiles * kBlock * head_dim, scales + tiles, num_blocks, num_kv_heads,
-             head_dim, blocks, chunks, static_cast<__nv_bfloat16*>(out), status);
-  return done();
+  return launched(launch_pdl(gather_kernel, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream),
+                             static_cast<const uint8_t*>(codes) + tiles * kBlock * head_dim, scales + tiles, num_blocks,
+                             num_kv_heads, head_dim, blocks, chunks, static_cast<__nv_bfloat16*>(out), status));
 }

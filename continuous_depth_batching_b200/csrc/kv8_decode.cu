@@ -490,12 +490,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t even = quotient(total + gridDim.x - 1, gridDim.x);
   const int64_t share = even > p.min_share ? even : p.min_share;
   int64_t begin = share * blockIdx.x, end = begin + share < total ? begin + share : total;
-  if ((int64_t)p.num_items * vheads <= gridDim.x && longest <= p.whole_pairs) {
+  if (rows != nullptr && (int64_t)p.num_items * vheads <= gridDim.x && longest <= p.whole_pairs) {
     // Few short segments: a CTA for each, so that none has to meet another's piece in the workspace.
     const int row = blockIdx.x / vheads, vh = blockIdx.x - row * vheads;
     if (row >= p.num_items) return;
     const int n = s_row[row].x < 0 ? 0 : s_row[row].x / (2 * kBlock) + 1;
-    begin = s_before[row] * vheads + (int64_t)vh * n;  // (per is 1: rows are fewer than CTAs)
+    begin = s_before[row] * vheads + (int64_t)vh * n;
     end = begin + n;
   }
   if (begin >= end) return;  // uniform over the CTA

@@ -14,7 +14,9 @@
 // weights P there too, over the S that they come from, so that P is as double as S and the softmax of a step
 // need not wait for the product of the one before; V is double in shared memory for the same reason.
 // Two CTAs share an SM (256 of its 512 tensor-memory columns, 113 KB of shared memory each): one computes
-// exponentials while the other multiplies.
+// exponentials while the other multiplies. A GEMM CTA that is launched early beside one of them holds its
+// columns while it waits for this kernel; it has no room in shared memory beside two, and at most 256 columns
+// where it fits beside one, so the allocation here never waits for a kernel that waits for this one.
 //
 // Arithmetic as in the decode kernel: q over a power of two per row, an online base-2 softmax with l relative
 // to a maximum m of the logits x, the weights of V, w = 2^x s_v, relative to their own maximum M and rounded
@@ -209,7 +211,7 @@ struct Rows {
 
 __device__ __forceinline__ bool fits(const PrefillParams& p, int4 tile) {
   return tile.y <= TR && tile.x >= 0 && tile.x <= p.num_rows - tile.y && tile.z >= 0 && tile.z < p.bt_rows &&
-         tile.w >= 0 && (tile.w + tile.y - 1) / kBlock < p.bt_width;
+         tile.w >= 0 && tile.w <= 0x7fffffff - 2 * TM && (tile.w + tile.y - 1) / kBlock < p.bt_width;
 }
 
 // Decides from the whole list whether this entry stands alone, takes the request's next 64 rows along, or is

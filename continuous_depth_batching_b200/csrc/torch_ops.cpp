@@ -107,7 +107,7 @@ std::mutex g_mutex;
 
 // The device-side status word that all ops of a device share; allocated by the first call.
 const Tensor& status_word(c10::Device dev) {
-  static std::map<int, Tensor> words;
+  static auto& words = *new std::map<int, Tensor>;  // never destroyed: the device may be gone by then
   std::lock_guard<std::mutex> lock(g_mutex);
   Tensor& word = words[dev.index()];
   if (!word.defined()) {
@@ -115,6 +115,7 @@ const Tensor& status_word(c10::Device dev) {
                 "torch.ops.cdb: the first call on a device allocates the shared status word; make one call before "
                 "capturing a CUDA graph");
     word = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(dev));
+    c10::cuda::getCurrentCUDAStream(dev.index()).synchronize();  // calls on other streams may write it next
   }
   return word;
 }
@@ -138,7 +139,7 @@ std::pair<Tensor, Tensor> decode_workspace(c10::Device dev, c10::cuda::CUDAStrea
   const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
     return {at::empty({floats}, f32), at::zeros({counters}, i32)};
-  static std::map<std::pair<int, cudaStream_t>, std::pair<Tensor, Tensor>> kept;
+  static auto& kept = *new std::map<std::pair<int, cudaStream_t>, std::pair<Tensor, Tensor>>;
   std::lock_guard<std::mutex> lock(g_mutex);
   auto& ws = kept[{dev.index(), stream.stream()}];
   if (!ws.first.defined() || ws.first.numel() < floats || ws.second.numel() < counters)

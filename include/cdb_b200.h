@@ -491,7 +491,8 @@ int cdb_kv8_append(const void* qkv, int64_t qkv_stride, void* q_out, int64_t q_o
                    void* stream);
 
 /* out[i] = block blocks[i] of one cache layer as bf16 [2][num_kv_heads][16][head_dim] (16-byte
- * aligned; exact: a code times a power of two is a bf16 value). A block id out of range gives zeros. */
+ * aligned; exact down to bf16's smallest: a code times a power of two is a bf16 value). A block id out
+ * of range gives zeros. */
 int cdb_kv8_gather(const void* codes, const float* scales, int num_cache_layers, int cache_layer, int num_blocks,
                    int num_kv_heads, int head_dim, const int32_t* blocks, int n, void* out, int32_t* status,
                    void* stream);
@@ -505,7 +506,7 @@ int cdb_kv8_decode_counters(int num_ctas);
  * kernel cuts the pages of all rows into equal shares by the positions on the device.
  *   q, out     bf16 rows of num_heads * head_dim, q rotated; 16-byte aligned, strides multiples
  *              of 8. num_heads is a multiple of num_kv_heads; head h reads kv head
- *              h / (num_heads / num_kv_heads).
+ *              h / (num_heads / num_kv_heads). scale > 0.
  *   num_ctas   CTAs to launch (one fits an SM); workspace: cdb_kv8_decode_workspace_floats of it;
  *              counters: cdb_kv8_decode_counters of it, zeroed before the first use, left zeroed.
  *              Calls that share them must be ordered. */
@@ -557,15 +558,17 @@ int cdb_step_tables(const int32_t* slots, const int32_t* seq_len, const int32_t*
 
 /* A few token rows times 4-bit weights with group scales (weight-only quantised nn.Linear):
  *   out[m][n] = bf16( sum_j s[n][j] * sum over k in group j of (q[n][k] - z[n][j]) * x[m][k] ), fp32 sums.
- *   x          bf16 [M][ldx], 16-byte aligned, ldx a multiple of 8.
+ *   x          bf16 [M][ldx], 16-byte aligned, ldx a multiple of 8, M <= 65535. Finite, sums of 143 |x|
+ *              over a group within fp32: a row that holds an infinity or NaN comes out as NaN.
  *   w          uint8 [N][ldw], 16-byte aligned, ldw (bytes) a multiple of 16: byte k / 2 of row n
  *              holds q[n][k] in its low nibble for even k, in its high nibble for odd k. K a
  *              multiple of 32.
  *   scales     bf16 [N][K / group_size]; group_size 32, 64 or a multiple of 128 that divides K.
  *   zeros      uint8 [N][K / group_size], or NULL: 8 everywhere.
  *   out        bf16 [M][ldo].
- * The weights are read once for every 32 rows of x. Results do not depend on anything but the shapes
- * and num_sms. */
+ * The weights are read once for every block of token rows: 32, or as many as fit shared memory beside
+ * the rings where K is long (11 at K = 5632). CDB_ERR_UNSUPPORTED where not one row fits (K above
+ * 38,656 at groups of 32, 46,592 at 64, 51,712 beyond). Results do not depend on anything but the shapes and num_sms. */
 int cdb_gemv_w4(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* scales, const void* zeros,
                 void* out, int64_t ldo, int M, int N, int K, int group_size, int num_sms, int32_t* status,
                 void* stream);

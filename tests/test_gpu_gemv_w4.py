@@ -66,6 +66,27 @@ def test_sizes(n, k, group, zeros, m):
     _check(out.cpu(), x, w, s, z, group)
 
 
+@pytest.mark.parametrize("m", [6, 8, 9, 11, 16])
+@pytest.mark.parametrize("n,k,group", [(50, 7424, 32), (50, 7936, 128), (20, 38656, 32)])
+def test_token_rows_that_nearly_fill_shared_memory(n, k, group, m):
+    """K where the rings that one tile of tokens would like do not fit beside its rows."""
+
+    w, s, z, g = _weights(n, k, group, True, k + m)
+    x = (torch.randn(m, k, generator=g) + 0.5).bfloat16()
+    out = torch.empty(m, n, dtype=torch.bfloat16, device=DEV)
+    torch.ops.cdb.gemv_w4(x.to(DEV), w.to(DEV), s.to(DEV), z.to(DEV), out)
+    torch.cuda.synchronize()
+    assert ops.status_code() == 0
+    _check(out.cpu(), x, w, s, z, group)
+
+
+def test_refuses_token_rows_that_do_not_fit():
+    w, s, z, g = _weights(4, 65536, 128, False, 9)
+    x = torch.zeros(1, 65536, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(RuntimeError, match="cdb_gemv_w4"):
+        torch.ops.cdb.gemv_w4(x, w.to(DEV), s.to(DEV), None, torch.empty(1, 4, dtype=torch.bfloat16, device=DEV))
+
+
 def test_strided_and_repeatable():
     """Rows of wider tensors; places between the rows stay; the same call gives the same bits."""
 

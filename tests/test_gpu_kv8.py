@@ -282,6 +282,29 @@ def test_indexes_out_of_range_are_reported_and_skipped():
     assert int(status.item()) == 6 and (back[0] == 0).all() and (back[1] != 7).any()
 
 
+@pytest.mark.parametrize("ctas", [1, 20, 148, 500])
+def test_decode_with_any_number_of_ctas(ctas):
+    """Through the C ABI: a few CTAs take everything; more CTAs than rows, with more rows than threads, too.
+    One launch in place of the other gives the same values within the tolerance."""
+
+    d, n = 64, 400
+    pos = [(7 * i) % 60 - 1 for i in range(n)]
+    slots = [i % 12 for i in range(n)]
+    c = Cache([60] * 12, 1, d, seed=12, layers=1)
+    codes, scales, table = c.gpu()
+    q = torch.randn(n, d, generator=c.gen).bfloat16()
+    qg, out = q.to(DEV), torch.full((n, d), 7.0, dtype=torch.bfloat16, device=DEV)
+    slot, posg = (torch.tensor(v, dtype=torch.int32, device=DEV) for v in (slots, pos))
+    ws = torch.empty(_lib.load().cdb_kv8_decode_workspace_floats(ctas, d), device=DEV)
+    ctr = torch.zeros(_lib.load().cdb_kv8_decode_counters(ctas), dtype=torch.int32, device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    _lib.call("cdb_kv8_decode_attention", _lib.ptr(qg), d, _lib.ptr(out), d, _lib.ptr(codes), _lib.ptr(scales), 1, 0, c.blocks,
+              _lib.ptr(table), table.stride(0), 12, table.shape[1], _lib.ptr(slot), _lib.ptr(posg), n, 1, 1, d, d**-0.5, ctas,
+              _lib.ptr(ws), ws.numel(), _lib.ptr(ctr), _lib.ptr(status), torch.cuda.current_stream().cuda_stream)
+    assert int(status.item()) == 0 and not ctr.any()
+    _check_rows(out.cpu(), c, q, pos, 1, layer=0, slots=slots)
+
+
 def test_decode_on_two_streams_and_in_two_graphs():
     """Calls that split rows, on two streams at once and in two graphs replayed at once, keep their
     workspaces apart."""
@@ -416,7 +439,8 @@ def test_prefill_refuses_tiles_that_do_not_fit():
                   _lib.ptr(status), sp)
         return out, int(status.item())
 
-    for tile in [(0, 65, 0, 0), (1, 64, 0, 0), (-1, 4, 0, 0), (0, 4, 2, 0), (0, 4, -1, 0), (0, 4, 0, -1), (0, 64, 0, 5000)]:
+    for tile in [(0, 65, 0, 0), (1, 64, 0, 0), (-1, 4, 0, 0), (0, 4, 2, 0), (0, 4, -1, 0), (0, 4, 0, -1), (0, 64, 0, 5000),
+                 (0, 64, 0, 2**31 - 8)]:
         out, code = call(*tile)
         assert code == 6 and (out == 7).all(), tile
     out, code = call(0, 0, 99, -4)
