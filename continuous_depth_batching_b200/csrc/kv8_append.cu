@@ -1,12 +1,18 @@
 // Writing and reading back the 8-bit paged KV cache (layout and scale rule in kv8.cuh).
 //
-// Append. The rows of a call that fall in one block form a run: the same slot, consecutive
-// positions. One warp owns a (run, kv head, K or V) tile: it loads the run's up to 16 rows, adds the
-// bias and rotates in fp32, takes the tile's largest magnitude, settles the block's scale, rescales
-// the codes that were there when the scale grew, and writes codes and scale. Nobody else touches the
-// tile, so no atomics and no second pass over the new values. The query heads are rotated by other
-// warps of the same launch, a few heads of a row or two at a time. Bound by bytes for prompts (q, k, v in, q and codes out) and by the chain
-// of dependent loads (position, block id, values) for a decode step.
+// Append. The rows of a call that fall in one block form a run: the same slot, consecutive positions. One warp
+// owns the (run, head) tiles of a few heads of K or V: it brings a head's up to 16 rows, adds the bias and
+// rotates in fp32, takes the tile's largest magnitude, settles the block's scale, rescales the codes that were
+// there when the scale grew, and writes codes and scale. Nobody else touches the tile, so no atomics and no
+// second pass over the new values. The query heads are rotated by other warps of the same launch.
+//
+// Bound: for prompts bytes (q, k, v in, q and codes out) and the instructions around a value, some 100 for 8 of
+// them in a lane; for a decode step the chain of dependent loads (position, block id, values). Measured: 4096
+// rows of prompts, 16 heads of 128: 22 us (84 MB, 3.8 TB/s); some 4000 rows of 55 heads of 96 with biases: 65 us
+// (3.4 TB/s; 85 us with the rows' angles read from global memory for each head and one head to a warp); 80
+// decode rows, 16 heads of 128: 3.9 us.
+//
+// Read-back (gather): bytes; 1 in, 2 out a code. 31 us for those 4000 rows (132 MB, 4.2 TB/s).
 #include "kv8.cuh"
 
 namespace cdb {
@@ -32,6 +38,7 @@ struct AppendParams {
   const __nv_bfloat16* qk_bias;  // [heads + kv heads][D] or null
   int num_items, num_heads, num_kv_heads;
   int group;  // rows whose runs one CTA starts
+  int heads;  // kv heads of a warp's task
   int32_t* status;
 };
 
@@ -104,8 +111,8 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a <= 3.402823466e38f ? a : 0.f;  // infinities saturate and NaN stays NaN, under the others' scale
 }
 
-// q: a warp rotates HB heads of RPI rows (those before `end`), with the rows' angles in registers and the heads' loads in
-// flight together.
+// q: a warp rotates HB heads of rows [row0, end), RPI rows at a time, with the rows' angles in registers, the
+// heads' loads in flight together and the next rows' behind them.
 constexpr int HB = 4;
 
 template <int D>
@@ -113,27 +120,48 @@ __device__ __forceinline__ void rotate_q(const AppendParams& p, int row0, int en
   constexpr int LPR = D / 8, RPI = 32 / LPR;
   const int lane = threadIdx.x & 31;
   const int sub = lane / LPR, x0 = (lane % LPR) * 8;
-  const int r = row0 + sub;
-  const int pos = sub < RPI && r < end ? p.item_pos[r] : -1;
-  const bool on = pos >= 0 && (p.rope_mode == 0 || pos < p.rope_rows);
-  const Angles a = load_angles<D>(p, p.rope_mode, pos, x0, on);
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  uint4 raw[HB], bias[HB];
+  uint4 raw[HB];
+  Angles a;
+  auto fetch = [&](int r) {
+    const int pos = sub < RPI && r < end ? p.item_pos[r] : -1;
+    const bool on = pos >= 0 && (p.rope_mode == 0 || pos < p.rope_rows);
 #pragma unroll
-  for (int h = 0; h < HB; ++h) {
-    const bool has = on && head0 + h < p.num_heads;
-    raw[h] = has ? ld16(p.qkv + (int64_t)r * p.qkv_stride + (int64_t)(head0 + h) * D + x0) : zero;
-    bias[h] = has && p.qk_bias != nullptr ? ld16(p.qk_bias + (int64_t)(head0 + h) * D + x0) : zero;
-  }
+    for (int h = 0; h < HB; ++h)
+      raw[h] = on && head0 + h < p.num_heads ? ld16(p.qkv + (int64_t)r * p.qkv_stride + (int64_t)(head0 + h) * D + x0)
+                                             : zero;
+    a = load_angles<D>(p, p.rope_mode, pos, x0, on);
+    return on;
+  };
+  bool on = fetch(row0 + sub);
+  for (int r = row0 + sub; r - sub < end; r += RPI) {
+    uint4 now[HB];
 #pragma unroll
-  for (int h = 0; h < HB; ++h) {
-    float y[8];
-    rotated8<D>(raw[h], bias[h], p.rope_mode, a, x0, y);
-    if (on && head0 + h < p.num_heads)
-      *reinterpret_cast<uint4*>(p.q_out + (int64_t)r * p.q_out_stride + (int64_t)(head0 + h) * D + x0) =
-          make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
-                     pack_bf16x2(y[6], y[7]));
+    for (int h = 0; h < HB; ++h) now[h] = raw[h];
+    const Angles angles = a;
+    const bool had = on;
+    on = fetch(r + RPI);
+#pragma unroll
+    for (int h = 0; h < HB; ++h) {
+      const uint4 bias = had && p.qk_bias != nullptr && head0 + h < p.num_heads
+                             ? ld16(p.qk_bias + (int64_t)(head0 + h) * D + x0)
+                             : zero;
+      float y[8];
+      rotated8<D>(now[h], bias, p.rope_mode, angles, x0, y);
+      if (had && head0 + h < p.num_heads)
+        *reinterpret_cast<uint4*>(p.q_out + (int64_t)r * p.q_out_stride + (int64_t)(head0 + h) * D + x0) =
+            make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
+                       pack_bf16x2(y[6], y[7]));
+    }
   }
+}
+
+// Shared memory of a warp: one head of a run of 16 rows, and their cos and sin, a whole warp's chunks at a time.
+__host__ __device__ constexpr int stage_bytes(int dim) { return 3 * kBlock / (32 / (dim / 8)) * 32 * 16; }
+
+__device__ __forceinline__ void async_copy16(uint4* dst, const void* src, bool on) {  // zeros where not on
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 16 : 0)
+               : "memory");
 }
 
 // A run of rows of one block.
@@ -181,13 +209,15 @@ __device__ __forceinline__ int block_of(const AppendParams& p, const Run& run) {
   return p.block_table[(int64_t)run.slot * p.bt_stride + run.pos / kBlock];
 }
 
-// k or v of one head of a run. ROWS: the most rows a run may have here (16, or what one pass holds). The
-// loads, the block id's among them, are in flight together; the rotated rows stay in registers from there to
-// the codes (rotating them twice, for a third CTA on the SM, measured 138 us against 114 on 55 x 96 prompts).
-// The magnitude is taken over everything first, and again over the finite values in the rare tile that has
-// others.
+// k or v of heads [head, end) of a run. ROWS: the most rows a run may have here (16, or what one pass holds).
+// A head's rows and the rows' angles come asynchronously into shared memory (`stage`: every lane's own chunks,
+// so no barrier), the first head's beside the block id, each next head's while the one before is turned into
+// codes: registers hold one head's rotated rows only. Those stay in registers from there to the codes (rotating them twice,
+// for a third CTA on the SM, measured 138 us against 114 on 55 x 96 prompts). The magnitude is taken over
+// everything first, and again over the finite values in the rare tile that has others.
 template <int D, int ROWS, bool IS_V>
-__device__ __forceinline__ void write_tile(const AppendParams& p, int r, const Run& run, int head) {
+__device__ __forceinline__ void write_tiles(const AppendParams& p, int r, const Run& run, int head, int end,
+                                            uint4* stage) {
   constexpr int LPR = D / 8, RPI = 32 / LPR, IT = (ROWS + RPI - 1) / RPI;
   const int lane = threadIdx.x & 31;
   const int sub = lane / LPR, x0 = (lane % LPR) * 8;
@@ -198,111 +228,137 @@ __device__ __forceinline__ void write_tile(const AppendParams& p, int r, const R
   const int64_t step = (int64_t)RPI * p.qkv_stride;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   const int rows = sub < RPI ? run.n - sub : 0;  // this lane's: it * RPI < rows
-  uint4 raw[IT];
-#pragma unroll
-  for (int it = 0; it < IT; ++it) raw[it] = it * RPI < rows ? ld16(src + it * step) : zero;
-  uint4 bias = zero;
-  if (!IS_V && p.qk_bias != nullptr && sub < RPI) bias = ld16(p.qk_bias + (int64_t)(p.num_heads + head) * D + x0);
-  if (blk < 0 || blk >= p.num_blocks) {
-    if (lane == 0) set_error(p.status, CDB_ERR_INDEX);
-    return;
-  }
-  const int64_t tile = ((int64_t)(IS_V ? p.num_blocks : 0) + blk) * p.num_kv_heads + head;
-  uint8_t* codes = p.codes + tile * (kBlock * D);
-  const float was = off > 0 ? p.scales[tile] : 0.f;
-  float y[IT][8];
-  float amax = 0.f;
-#pragma unroll
-  for (int it = 0; it < IT; ++it) {
-    if constexpr (IS_V) {
-      unpack8(raw[it], y[it]);
-    } else {
-      const bool on = it * RPI < rows;
-      const Angles a = load_angles<D>(p, p.rope_mode, run.pos + it * RPI + sub, x0, on);
-      rotated8<D>(raw[it], on ? bias : zero, p.rope_mode, a, x0, y[it]);  // zeros where no row is
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(y[it][e]));  // (a NaN is passed over)
-  }
-  amax = warp_max(amax);
-  if (amax > 3.402823466e38f) {  // infinities saturate, under the others' scale
-    amax = 0.f;
+  const bool biased = !IS_V && p.qk_bias != nullptr && sub < RPI;
+  const __nv_bfloat16* bias_at = p.qk_bias + (int64_t)(p.num_heads + head) * D + x0;
+  uint4* place = stage + lane;             // [IT][32 lanes] rows
+  uint4* turn = stage + kBlock / RPI * 32 + lane;  // [IT][cos, sin][32 lanes]
+  auto fetch = [&]() {
 #pragma unroll
     for (int it = 0; it < IT; ++it)
+      async_copy16(place + it * 32, it * RPI < rows ? src + it * step : p.qkv, it * RPI < rows);
+    src += D;
+  };
+  fetch();
+  if (!IS_V && p.rope_mode != 0) {
+    const char *c = static_cast<const char*>(p.rope_cos), *s = static_cast<const char*>(p.rope_sin);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(y[it][e]));
-    amax = warp_max(amax);
+    for (int it = 0; it < IT; ++it) {
+      const int pos = run.pos + it * RPI + sub;
+      const bool on = it * RPI < rows && pos < p.rope_rows;
+      // 2 D bytes a position in either mode, 16 of them for 8 dims
+      const int64_t at = on ? ((int64_t)pos * D + x0) * 2 : 0;
+      async_copy16(turn + it * 64, c + at, on);
+      async_copy16(turn + it * 64 + 32, s + at, on);
+    }
   }
-  float scale = block_scale(amax);
-  if (off > 0) {
-    if (was >= scale) {
-      scale = was;
-    } else {  // the block grows: its old codes move down by a power of two
-      const float ratio = was / scale;
-      for (int c = lane; c < off * LPR; c += 32) {
-        uint2* at = reinterpret_cast<uint2*>(codes + c * 8);
-        const uint2 old = *at;
-        const uint32_t w[2] = {old.x, old.y};
-        uint32_t o[2];
+  if (blk < 0 || blk >= p.num_blocks) {
+    if (lane == 0) set_error(p.status, CDB_ERR_INDEX);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    return;
+  }
+  int64_t tile = ((int64_t)(IS_V ? p.num_blocks : 0) + blk) * p.num_kv_heads + head;
+  for (; head < end; ++head, ++tile) {
+    uint8_t* codes = p.codes + tile * (kBlock * D);
+    const float was = off > 0 ? p.scales[tile] : 0.f;
+    const uint4 bias = biased ? ld16(bias_at) : zero;
+    bias_at += D;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    float y[IT][8];
+    float amax = 0.f;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float a, b, c2, d;
-          unpack_f16x2(cvt_e4m3x2_f16x2(w[k] & 0xffffu), a, b);
-          unpack_f16x2(cvt_e4m3x2_f16x2(w[k] >> 16), c2, d);
-          o[k] = cvt_f32x2_e4m3x2(a * ratio, b * ratio) | (cvt_f32x2_e4m3x2(c2 * ratio, d * ratio) << 16);
+    for (int it = 0; it < IT; ++it) {
+      const uint4 raw = place[it * 32];
+      if constexpr (IS_V) {
+        unpack8(raw, y[it]);
+      } else {
+        Angles a;
+        if (p.rope_mode != 0) a.c = turn[it * 64], a.s = turn[it * 64 + 32];
+        rotated8<D>(raw, it * RPI < rows ? bias : zero, p.rope_mode, a, x0, y[it]);  // zeros where no row is
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(y[it][e]));  // (a NaN is passed over)
+    }
+    if (head + 1 < end) fetch();  // over the rows just read: each lane's own
+    amax = warp_max(amax);
+    if (amax > 3.402823466e38f) {  // infinities saturate, under the others' scale
+      amax = 0.f;
+#pragma unroll
+      for (int it = 0; it < IT; ++it)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(y[it][e]));
+      amax = warp_max(amax);
+    }
+    float scale = block_scale(amax);
+    if (off > 0) {
+      if (was >= scale) {
+        scale = was;
+      } else {  // the block grows: its old codes move down by a power of two
+        const float ratio = was / scale;
+        for (int c = lane; c < off * LPR; c += 32) {
+          uint2* at = reinterpret_cast<uint2*>(codes + c * 8);
+          const uint2 old = *at;
+          const uint32_t w[2] = {old.x, old.y};
+          uint32_t o[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float a, b, c2, d;
+            unpack_f16x2(cvt_e4m3x2_f16x2(w[k] & 0xffffu), a, b);
+            unpack_f16x2(cvt_e4m3x2_f16x2(w[k] >> 16), c2, d);
+            o[k] = cvt_f32x2_e4m3x2(a * ratio, b * ratio) | (cvt_f32x2_e4m3x2(c2 * ratio, d * ratio) << 16);
+          }
+          *at = make_uint2(o[0], o[1]);
         }
-        *at = make_uint2(o[0], o[1]);
       }
     }
-  }
-  const float inv = 1.f / scale;
-  uint8_t* dst = codes + (off + sub) * D + x0;
+    const float inv = 1.f / scale;
+    uint8_t* dst = codes + (off + sub) * D + x0;
 #pragma unroll
-  for (int it = 0; it < IT; ++it) {
-    if (it * RPI < rows) {
-      const uint32_t lo = cvt_f32x2_e4m3x2(y[it][0] * inv, y[it][1] * inv) |
-                          (cvt_f32x2_e4m3x2(y[it][2] * inv, y[it][3] * inv) << 16);
-      const uint32_t hi = cvt_f32x2_e4m3x2(y[it][4] * inv, y[it][5] * inv) |
-                          (cvt_f32x2_e4m3x2(y[it][6] * inv, y[it][7] * inv) << 16);
-      *reinterpret_cast<uint2*>(dst + it * RPI * D) = make_uint2(lo, hi);
+    for (int it = 0; it < IT; ++it) {
+      if (it * RPI < rows) {
+        const uint32_t lo = cvt_f32x2_e4m3x2(y[it][0] * inv, y[it][1] * inv) |
+                            (cvt_f32x2_e4m3x2(y[it][2] * inv, y[it][3] * inv) << 16);
+        const uint32_t hi = cvt_f32x2_e4m3x2(y[it][4] * inv, y[it][5] * inv) |
+                            (cvt_f32x2_e4m3x2(y[it][6] * inv, y[it][7] * inv) << 16);
+        *reinterpret_cast<uint2*>(dst + it * RPI * D) = make_uint2(lo, hi);
+      }
     }
+    if (lane == 0) p.scales[tile] = scale;
   }
-  if (lane == 0) p.scales[tile] = scale;
 }
 
-// A CTA takes `group` rows: blockIdx.y first counts the q warps' tasks (RPI rows x HB heads), then those
-// of the k and v warps (one head of one of them, every run that starts in the group).
+// A CTA takes `group` rows: blockIdx.y first counts the q warps' tasks (HB heads), then those of the k and v
+// warps (`heads` heads of one of them, every run that starts in the group).
 template <int D>
-__global__ void __launch_bounds__(256, D == 64 ? 3 : 2) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(256, 2) append_kernel(const AppendParams p) {
   pdl_trigger();
   pdl_wait();
   constexpr int RPI = 32 / (D / 8);
   const int warp = threadIdx.x >> 5;
+  extern __shared__ uint4 smem[];
+  uint4* stage = smem + warp * (stage_bytes(D) / 16);
   const int row0 = blockIdx.x * p.group;
   const int rows = min(p.group, p.num_items - row0);
-  const int q_rows = (p.group + RPI - 1) / RPI, q_heads = (p.num_heads + HB - 1) / HB;
-  const int q_tasks = p.q_out != nullptr ? q_rows * q_heads : 0;
-  const int tasks = q_tasks + 2 * p.num_kv_heads;
+  const int q_tasks = p.q_out != nullptr ? (p.num_heads + HB - 1) / HB : 0;
+  const int kv_tasks = (p.num_kv_heads + p.heads - 1) / p.heads, tasks = q_tasks + 2 * kv_tasks;
   const Runs runs = find_runs(p, row0, rows);
   for (int task = blockIdx.y * 8 + warp; task < tasks; task += gridDim.y * 8) {
     if (task < q_tasks) {
-      const int i = task / q_heads, h = task - i * q_heads;
-      rotate_q<D>(p, row0 + i * RPI, row0 + rows, h * HB);
+      rotate_q<D>(p, row0, row0 + rows, task * HB);
       continue;
     }
     const int kt = task - q_tasks;
-    const bool is_v = kt >= p.num_kv_heads;
-    const int head = is_v ? kt - p.num_kv_heads : kt;
+    const bool is_v = kt >= kv_tasks;
+    const int head = (is_v ? kt - kv_tasks : kt) * p.heads, end = min(head + p.heads, p.num_kv_heads);
     for (unsigned left = runs.starts; left; left &= left - 1) {
       const int at = __ffs(left) - 1;
       const Run run = take_run(runs, at);
       const int r = row0 - 1 + at;
       if (run.n <= RPI) {
-        if (is_v) write_tile<D, RPI, true>(p, r, run, head);
-        else write_tile<D, RPI, false>(p, r, run, head);
+        if (is_v) write_tiles<D, RPI, true>(p, r, run, head, end, stage);
+        else write_tiles<D, RPI, false>(p, r, run, head, end, stage);
       } else {
-        if (is_v) write_tile<D, kBlock, true>(p, r, run, head);
-        else write_tile<D, kBlock, false>(p, r, run, head);
+        if (is_v) write_tiles<D, kBlock, true>(p, r, run, head, end, stage);
+        else write_tiles<D, kBlock, false>(p, r, run, head, end, stage);
       }
     }
   }
@@ -346,6 +402,13 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint8_t* codes, const
     dst[0] = lo;
     dst[1] = hi;
   }
+}
+
+template <int D>
+static cudaError_t launch_append(const AppendParams& p, dim3 grid, cudaStream_t st) {
+  constexpr int smem = 8 * stage_bytes(D);
+  const cudaError_t e = cudaFuncSetAttribute(append_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  return e != cudaSuccess ? e : launch_pdl(append_kernel<D>, grid, dim3(256), smem, st, p);
 }
 
 static int launched(cudaError_t e) { return e == cudaSuccess ? CDB_OK : CDB_ERR_CUDA; }
@@ -404,17 +467,19 @@ extern "C" int cdb_kv8_append(const void* qkv, int64_t qkv_stride, void* q_out, 
   p.num_heads = num_heads;
   p.num_kv_heads = num_kv_heads;
   p.status = status;
-  // Decode steps have a run per row: one row per CTA spreads them. Prompts have a run per 16 rows, and
-  // a CTA per row would start 15 of 16 kv warps for nothing.
+  // Decode steps have a run per row: a CTA per row and a head per warp spread them. Prompts have a run per 16
+  // rows, and a CTA per row would start 15 of 16 kv warps for nothing. Measured with 16 heads of 128, a row per
+  // CTA against 16: 80 decode rows 3.9 us (38), 512 16 (39), 1024 35 (54); prompts of 512 rows 10.5 (11.3), of
+  // 1024 19.7 (15.4), of 4096 72 (22). A warp's heads in prompts: 2, 3, 4, 6, 8 take 96, 95, 96, 99, 100 us on the
+  // 55 x 96 case (with its read-back), 11 take 113.
   p.group = num_items <= 1024 ? 1 : kBlock;
-  const int rpi = 32 / (head_dim / 8);
-  const int tasks =
-      (q_out != nullptr ? (p.group + rpi - 1) / rpi * ((num_heads + HB - 1) / HB) : 0) + 2 * num_kv_heads;
+  p.heads = p.group == 1 ? 1 : 4;
+  const int tasks = (q_out != nullptr ? (num_heads + HB - 1) / HB : 0) + 2 * ((num_kv_heads + p.heads - 1) / p.heads);
   const dim3 grid((num_items + p.group - 1) / p.group, min(65535, (tasks + 7) / 8));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return launched(head_dim == 128  ? launch_pdl(append_kernel<128>, grid, dim3(256), 0, st, p)
-                  : head_dim == 96 ? launch_pdl(append_kernel<96>, grid, dim3(256), 0, st, p)
-                                   : launch_pdl(append_kernel<64>, grid, dim3(256), 0, st, p));
+  if (head_dim == 128) return launched(launch_append<128>(p, grid, st));
+  if (head_dim == 96) return launched(launch_append<96>(p, grid, st));
+  return launched(launch_append<64>(p, grid, st));
 }
 
 extern "C" int cdb_kv8_gather(const void* codes, const float* scales, int num_cache_layers, int cache_layer,
