@@ -15,6 +15,12 @@
 //   sum (q - z) x = sum (128 + q) x - (128 + z) sum x,
 // both sums in fp32, then times the group's scale into the fp32 result: no weight is rounded. What the
 // offset cancels costs fp32's 2^-24 of 128 sum |x|, far below bf16's rounding of the result.
+//
+// Measured (weights of other layers between two calls, so from HBM; groups of 128): 2048 x 5632, 1 token 5.2 us;
+// 11264 x 2048, 24 tokens 12 us; 49152 x 2048, 8 tokens 20 us (2.6 TB/s; 21 us at groups of 64, 27 at 32). A call
+// costs some 4.5 us before and after its boxes: launch, token rows, the first box's latency, the sum. The rest goes
+// on instructions, about 400 a box of 16 x 256 weights with the ALU pipe, which takes a nibble apart, the fullest.
+// 24 warps against 16 for 8 tokens: 18.1 against 19.5 us (49152 x 2048, weights in L2).
 #include <cuda.h>
 
 #include "cdb_common.cuh"
@@ -91,9 +97,69 @@ __device__ __forceinline__ void nibbles(uint32_t w, uint32_t (&e)[4]) {
   e[3] = __byte_perm(odd, 0x43434343u, 0x4342);
 }
 
+// The scales and zero points of a box for this lane's rows, g and g + 8: scale bits, and 128 + zero point (2^15 + z
+// by bits, less 2^15 - 128).
+__device__ __forceinline__ float zero_of(uint32_t word, int byte) {
+  return __uint_as_float(__byte_perm(word, 0x47000000u, 0x7404 | byte << 4)) - 32640.f;
+}
+
+// WIDE: a row's scales of a box lie together and aligned, and every lane loads those of its two rows at once.
+template <int GN, bool WIDE>
+struct Entries;
+
+template <int GN>
+struct Entries<GN, true> {
+  uint32_t s[2][GN / 2], z[2];  // per row: GN bf16, GN bytes (8 at most: two words)
+  uint32_t z2[2];
+  __device__ __forceinline__ void load(const __nv_bfloat16* scale, const uint8_t* zero, int64_t to8, bool zeros) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const __nv_bfloat16* a = scale + r * to8;
+      if constexpr (GN == 8) {
+        const uint4 v = *reinterpret_cast<const uint4*>(a);
+        s[r][0] = v.x, s[r][1] = v.y, s[r][2] = v.z, s[r][3] = v.w;
+      } else if constexpr (GN == 4) {
+        const uint2 v = *reinterpret_cast<const uint2*>(a);
+        s[r][0] = v.x, s[r][1] = v.y;
+      } else {
+        s[r][0] = *reinterpret_cast<const uint32_t*>(a);
+      }
+      z[r] = z2[r] = 0x08080808u;
+      if (zeros) {
+        const uint8_t* b = zero + r * to8;
+        if constexpr (GN == 8) {
+          const uint2 v = *reinterpret_cast<const uint2*>(b);
+          z[r] = v.x, z2[r] = v.y;
+        } else if constexpr (GN == 4) {
+          z[r] = *reinterpret_cast<const uint32_t*>(b);
+        } else {
+          z[r] = *reinterpret_cast<const uint16_t*>(b);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void get(int r, int grp, float& scale, float& zero) const {
+    const uint32_t w = s[r][grp / 2];
+    scale = __uint_as_float(grp & 1 ? w & 0xffff0000u : w << 16);
+    zero = zero_of(grp < 4 ? z[r] : z2[r], grp & 3);
+  }
+};
+
+// Otherwise: 2 GN (row half, group) entries, each loaded once in the four lanes of a row (entry e in lane e % 4) as
+// scale bits and zero point in one word.
+template <int GN>
+struct Entries<GN, false> {
+  uint32_t e[GN / 2];
+  __device__ __forceinline__ void get(int r, int grp, float& scale, float& zero) const {
+    const uint32_t w = __shfl_sync(kFull, e[(r * GN + grp) / 4], (r * GN + grp) % 4, 4);
+    scale = __uint_as_float(w & 0xffff0000u);
+    zero = zero_of(w, 0);
+  }
+};
+
 // NT: tiles of 8 tokens. GI: 32-k blocks that share a scale within a box (1, 2, or 4 for groups of 128
 // and multiples of it).
-template <int NT, int GI>
+template <int NT, int GI, bool WIDE>
 __global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid_constant__ CUtensorMap wmap, const Params p) {
   pdl_trigger();
   constexpr int GN = 8 / GI;  // scales of a row in one box
@@ -144,27 +210,33 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid
   // 0.05 to 0.3 us a call.
   pdl_wait();
   while (issued < p.stages && issued < boxes) issue();
-  // The scales and zero points of a box: 2 GN (row half, group) entries, each loaded once in the four lanes of
-  // a row (entry e in lane e % 4) as scale bits and zero point in one word, a box ahead of their use.
-  constexpr int EN = GN / 2;
-  uint32_t entry[EN];
+  // The scales and zero points of a box, loaded a box ahead of their use.
+  constexpr int EN = WIDE ? 1 : GN / 2;
+  Entries<GN, WIDE> entry;
   const __nv_bfloat16* entry_scale[EN];  // each row's first
   const uint8_t* entry_zero[EN];
+  int64_t to8 = 0;  // WIDE: from the scales of row g to those of row g + 8
   auto entry_tile = [&](int tile) {
 #pragma unroll
     for (int k = 0; k < EN; ++k) {
-      const int64_t row = (int64_t)min(tile * kRows + g + 8 * ((t + 4 * k) / GN), p.n - 1) * p.groups;
-      entry_scale[k] = p.scales + row;
-      entry_zero[k] = p.zeros + row;
+      const int at = min(tile * kRows + g + (WIDE ? 0 : 8 * ((t + 4 * k) / GN)), p.n - 1);
+      if (WIDE) to8 = (int64_t)(min(tile * kRows + g + 8, p.n - 1) - at) * p.groups;
+      entry_scale[k] = p.scales + (int64_t)at * p.groups;
+      entry_zero[k] = p.zeros + (int64_t)at * p.groups;
     }
   };
   auto load_entries = [&](int i) {
+    if constexpr (WIDE) {
+      entry.load(entry_scale[0] + (sub0 + i) * GN, entry_zero[0] + (sub0 + i) * GN, to8, p.zeros != nullptr);
+    } else {
 #pragma unroll
-    for (int k = 0; k < EN; ++k) {
-      int grp = (sub0 + i) * GN + (t + 4 * k) % GN;
-      if (GI == 4 && p.group_boxes > 1) grp /= p.group_boxes;
-      grp = min(grp, p.groups - 1);  // a box may reach past k, onto zeros of x
-      entry[k] = ((uint32_t)__bfloat16_as_ushort(entry_scale[k][grp]) << 16) | (p.zeros != nullptr ? entry_zero[k][grp] : 8u);
+      for (int k = 0; k < EN; ++k) {
+        int grp = (sub0 + i) * GN + (t + 4 * k) % GN;
+        if (GI == 4 && p.group_boxes > 1) grp /= p.group_boxes;
+        grp = min(grp, p.groups - 1);  // a box may reach past k, onto zeros of x
+        entry.e[k] = ((uint32_t)__bfloat16_as_ushort(entry_scale[k][grp]) << 16) |
+                     (p.zeros != nullptr ? entry_zero[k][grp] : 8u);
+      }
     }
   };
   if (boxes > 0) {
@@ -227,9 +299,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
     for (int i = 0; i < subs; ++i) {
-      uint32_t now[EN];
-#pragma unroll
-      for (int k = 0; k < EN; ++k) now[k] = entry[k];
+      const Entries<GN, WIDE> now = entry;
       if (i + 1 < subs) {
         load_entries(i + 1);
       } else if (round + 1 < rounds) {
@@ -260,12 +330,9 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid
         }
         if (b % GI == GI - 1) {
           const int grp = b / GI;
-          // scale, and 128 + zero point (2^15 + z by bits, less 2^15 - 128), of this lane's two rows
-          const uint32_t ua = __shfl_sync(kFull, now[grp / 4], grp % 4, 4);
-          const uint32_t ub = __shfl_sync(kFull, now[(GN + grp) / 4], (GN + grp) % 4, 4);
-          const float sa = __uint_as_float(ua & 0xffff0000u), sb = __uint_as_float(ub & 0xffff0000u);
-          const float za = __uint_as_float(__byte_perm(ua, 0x47000000u, 0x7404)) - 32640.f;
-          const float zb = __uint_as_float(__byte_perm(ub, 0x47000000u, 0x7404)) - 32640.f;
+          float sa, sb, za, zb;
+          now.get(0, grp, sa, za);
+          now.get(1, grp, sb, zb);
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             const float2 sx = *reinterpret_cast<const float2*>(sums + (i * GN + grp) * (NT * 8) + j * 8);
@@ -344,25 +411,36 @@ static int64_t row_bytes(int subs, int nt, int gi, int tokens, int wk) {
          (wk > 1 ? (int64_t)kWarps * kPart * nt * 8 * 4 : 0);
 }
 
-template <int NT, int GI>
+template <int NT, int GI, bool WIDE>
 static int launch(const CUtensorMap& map, Params p, dim3 grid, cudaStream_t st) {
   constexpr int kWarps = warps_of(NT);
   const int64_t rest = row_bytes(p.subs, NT, GI, p.tokens, p.wk);
   p.stages = (int)((kSmem - rest) / (kWarps * kTile));
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   const size_t smem = rest + (size_t)kWarps * p.stages * kTile;
-  auto kernel = gemv_kernel<NT, GI>;
+  auto kernel = gemv_kernel<NT, GI, WIDE>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return CDB_ERR_CUDA;
   return launch_pdl(kernel, grid, dim3(kWarps * 32), smem, st, map, p) == cudaSuccess ? CDB_OK : CDB_ERR_CUDA;
 }
 
-template <int GI>
+template <int GI, bool WIDE>
 static int launch_tokens(const CUtensorMap& map, const Params& p, dim3 grid, int nt, cudaStream_t st) {
-  if (nt == 1) return launch<1, GI>(map, p, grid, st);
-  if (nt == 2) return launch<2, GI>(map, p, grid, st);
-  if (nt == 3) return launch<3, GI>(map, p, grid, st);
-  return launch<4, GI>(map, p, grid, st);
+  if (nt == 1) return launch<1, GI, WIDE>(map, p, grid, st);
+  if (nt == 2) return launch<2, GI, WIDE>(map, p, grid, st);
+  if (nt == 3) return launch<3, GI, WIDE>(map, p, grid, st);
+  return launch<4, GI, WIDE>(map, p, grid, st);
+}
+
+// A row's scales of a box are loaded together where every box has all its groups and their places are aligned.
+// Against one at a time: 5.2 us for 5.5 (2048 x 5632, 1 token), 21.3 for 22.7 (49152 x 2048, 8 tokens, groups of
+// 64), 12.8 for 14.7 (6144 x 2048, 32 tokens, groups of 64); the same at groups of 32.
+template <int GI>
+static int launch_groups(const CUtensorMap& map, const Params& p, dim3 grid, int nt, cudaStream_t st) {
+  constexpr int GN = 8 / GI;
+  const bool wide = p.group_boxes == 1 && p.groups % GN == 0 && reinterpret_cast<uintptr_t>(p.scales) % (2 * GN) == 0 &&
+                    reinterpret_cast<uintptr_t>(p.zeros) % GN == 0;
+  return wide ? launch_tokens<GI, true>(map, p, grid, nt, st) : launch_tokens<GI, false>(map, p, grid, nt, st);
 }
 
 }  // namespace w4
@@ -421,7 +499,7 @@ extern "C" int cdb_gemv_w4(const void* x, int64_t ldx, const void* w, int64_t ld
   int nt = (p.tokens + 7) / 8;  // one tile's 24 rings may not fit where two tiles' 16 do
   while (row_bytes(p.subs, nt, gi, p.tokens, 2) + 2 * warps_of(nt) * kTile > kSmem) ++nt;
   // Warps on a row tile: the fewest boxes one after another in a warp (a sum over warps counted as half of
-  // one), for the row tiles that an SM gets. Few row tiles spread over k that way.
+  // one), for the row tiles that an SM gets. Few row tiles spread over k that way
   const int ctas = p.tiles < num_sms ? p.tiles : num_sms, share = (p.tiles + ctas - 1) / ctas;
   p.wk = 1;
   const int warps = warps_of(nt);
@@ -433,7 +511,7 @@ extern "C" int cdb_gemv_w4(const void* x, int64_t ldx, const void* w, int64_t ld
   }
   const dim3 grid(ctas, blocks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (gi == 1) return launch_tokens<1>(map, p, grid, nt, st);
-  if (gi == 2) return launch_tokens<2>(map, p, grid, nt, st);
-  return launch_tokens<4>(map, p, grid, nt, st);
+  if (gi == 1) return launch_groups<1>(map, p, grid, nt, st);
+  if (gi == 2) return launch_groups<2>(map, p, grid, nt, st);
+  return launch_groups<4>(map, p, grid, nt, st);
 }
