@@ -24,7 +24,12 @@
 // One exponential a key: w 2^-M = 2^(S f + log2 s_v - M), and l takes the sum of a block's weights times the
 // block's 2^(M - m) / s_v, unless that factor is so far from 1 that the weights could have underflowed.
 //
-// Measured bounds: exponentials and their neighbours (issue slots), then the products.
+// Measured: 4096 rows at positions 4096 .. 8191, 16 heads of 128: 312 us, 660 TFLOP/s; chunks of up to 400
+// rows of 12 requests: 44 us, mostly the steps of the longest and a CTA's start. What bounds it is the softmax's way
+// through a step, some 2600 of 3200 cycles a step of each of the two CTAs: load S, maximum, exponentials, store P,
+// none of them long enough to hide the next one's latency. Tensor pipe 29% busy, shared memory 65%, issue slots
+// 55%, exponentials 35%. Tried: eight softmax warps with 16 rows each (four lanes a row) 349 us, for a third more
+// instructions; four more conversion warps 321 us.
 //
 // A masked key never counts, whatever it holds: its logit is replaced, and a NaN in its V, which a product
 // with weight zero would spread, is taken out in the steps that the diagonal crosses and put back at the end
@@ -398,7 +403,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
     // ------------------------------------------------------------ codes to f16
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     const int ct = tid - kSoftmax, cw = warp - 4;
-    // K of step j into place: 16 codes of a key at a time; a quarter warp covers four chunks of two keys.
+    // K of step j into place: 16 codes of a key at a time; a quarter warp covers four chunks of two keys, of 128
+    // bytes the lower half of one and the upper half of the other, so that it reads and writes every bank once.
     auto convert_k = [&](int j) {
       constexpr int C = D / 16;  // chunks of a key
       const uint8_t* src = smem + T::OFF_SK + (j & 1) * 4 * T::BLK;
@@ -412,7 +418,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
         } else {
           const int rest = i >> 2;
           key = C == 8 ? (rest & 7) + ((rest >> 4) << 3) : rest;
-          c = (i & 3) + (C == 8 ? ((rest >> 3) & 1) * 4 : 0);
+          c = (i & 3) + (C == 8 ? ((rest ^ (rest >> 3)) & 1) * 4 : 0);
         }
         const uint4 w = *reinterpret_cast<const uint4*>(src + key * D + c * 16);
         uint8_t* dst = smem + T::OFF_K + (c >> 2) * (TK * 128) + key * 128;
@@ -426,9 +432,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
       }
     };
     // V of step j into place, transposed: 8 tokens of 4 dims at a time; lanes over the 4 blocks and 8 groups
-    // of dims.
+    // of dims. Of two dims, every other group of lanes writes the second first: a quarter warp's rows then differ
+    // by an odd number, and its chunks lie in different banks.
     auto convert_v = [&](int j) {
-      const int b = lane & 3;
+      const int b = lane & 3, turn = (lane >> 2) & 1;
       const bool have = sh.scale[j & (kMeta - 1)][0][b] >= 0.f;
       const bool full = kv_len - j * TK >= TK && __all_sync(kAll, have);
 #pragma unroll
@@ -462,18 +469,18 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
         const int ch = key0 >> 3;
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
-          const uint32_t sel = e == 0 ? 0x5140u : 0x7362u;
-          uint32_t lo[4], hi[4];
+          const uint32_t sel = e == 0 ? (turn ? 0x4051u : 0x5140u) : (turn ? 0x6273u : 0x7362u);
+          uint32_t lo[4], hi[4];  // of dims first and second
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const uint32_t pair = __byte_perm(w[2 * r], w[2 * r + 1], sel);
             lo[r] = cvt_e4m3x2_f16x2(pair & 0xffffu);
             hi[r] = cvt_e4m3x2_f16x2(pair >> 16);
           }
-          const int d = d0 + e;
-          *reinterpret_cast<uint4*>(smem + T::OFF_V + (j & 1) * (D * 128) + d * 128 + ((ch ^ (d & 7)) << 4)) =
-              make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          *reinterpret_cast<uint4*>(smem + T::OFF_V + (j & 1) * (D * 128) + (d + 1) * 128 + ((ch ^ ((d + 1) & 7)) << 4)) =
+          const int first = d0 + e + turn, second = d0 + e + 1 - turn;
+          uint8_t* to = smem + T::OFF_V + (j & 1) * (D * 128);
+          *reinterpret_cast<uint4*>(to + first * 128 + ((ch ^ (first & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          *reinterpret_cast<uint4*>(to + second * 128 + ((ch ^ (second & 7)) << 4)) =
               make_uint4(hi[0], hi[1], hi[2], hi[3]);
         }
       }
