@@ -490,8 +490,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t even = quotient(total + gridDim.x - 1, gridDim.x);
   const int64_t share = even > p.min_share ? even : p.min_share;
   int64_t begin = share * blockIdx.x, end = begin + share < total ? begin + share : total;
-  if (rows != nullptr && (int64_t)p.num_items * vheads <= gridDim.x && longest <= p.whole_pairs) {
-    // Few short segments: a CTA for each, so that none has to meet another's piece in the workspace.
+  if (rows != nullptr && (int64_t)p.num_items * vheads <= gridDim.x && longest <= p.whole_pairs &&
+      (longest <= 2 * kWarps || 2 * even >= longest)) {
+    // Few short segments: a CTA for each, so that none has to meet another's piece in the workspace, unless
+    // cutting them would leave a CTA less than half of one. Measured (16 heads of 128), whole against cut: 1 row of
+    // 700 positions 11.2 us (12.7), 8 of 700 11.3 (13.9), 9 of 1400 14.6 (19.1); 1 of 1400 14.4 (12.3), 2 of 1400
+    // 14.4 (12.1), 1 of 3000 21.1 (13.7).
     const int row = blockIdx.x / vheads, vh = blockIdx.x - row * vheads;
     if (row >= p.num_items) return;
     const int n = s_row[row].x < 0 ? 0 : s_row[row].x / (2 * kBlock) + 1;
@@ -821,7 +825,7 @@ extern "C" int cdb_kv8_decode_attention(const void* q, int64_t q_stride, void* o
   p.item_pos = item_pos;
   p.num_items = num_items;
   p.scale_log2 = scale * kLog2e;
-  p.min_share = kWarps;
+  p.min_share = kWarps / 2;  // 1, 6, 12, 24 pairs: 12.4, 12.3, 12.9, 14.2 us for one row of 1400 positions
   p.whole_pairs = 4 * kWarps;
   p.stages = 0;
   p.parts = workspace;

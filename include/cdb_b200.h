@@ -522,7 +522,8 @@ int cdb_kv8_decode_attention(const void* q, int64_t q_stride, void* out, int64_t
  *              aligned, num_tiles <= 65535: consecutive rows of one request; row r of a tile attends
  *              to positions 0 .. position + r. An entry of 0 rows is skipped, and rows that no tile
  *              names are left as they were. The rows' keys and values are in the cache
- *              (cdb_kv8_append), q is rotated.
+ *              (cdb_kv8_append), q is rotated. The CTAs start in the list's
+ *              order. Beyond 384 tiles those of a request should follow one another.
  *   q, out, num_heads as cdb_kv8_decode_attention; num_rows: rows that q and out have. */
 int cdb_kv8_prefill_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, int num_rows,
                               const void* codes, const float* scales, int num_cache_layers, int cache_layer,

@@ -422,6 +422,39 @@ def test_prefill_masked_places_hold_nan():
     assert torch.equal(got[:54], want[:54]) and got[54:80].isnan().all() and torch.equal(got[80:], want[80:])
 
 
+@pytest.mark.parametrize("order", ["shuffled", "interleaved", "twice", "short_copy", "short_followers"])
+@pytest.mark.parametrize("pad", [0, 500])  # lists that are searched, and longer ones
+def test_prefill_takes_tiles_in_any_order(order, pad):
+    """Neighbours apart, requests in turn, every tile listed twice, a full tile also listed as a short one: each
+    row comes out once, as it does in order."""
+
+    spans = [(3, 300), (64, 200), (128, 128), (700, 65)]
+    c = Cache([a + n for a, n in spans], 1, 64, seed=34)
+    q = torch.randn(sum(n for _, n in spans), 2 * 64, generator=c.gen).bfloat16()
+    codes, scales, table = c.gpu()
+    tiles, row = [], 0
+    for s, (first, n) in enumerate(spans):
+        tiles += [(row + i, min(64, n - i), s, first + i) for i in range(0, n, 64)]
+        row += n
+    if order == "shuffled":
+        tiles = [tiles[i] for i in torch.randperm(len(tiles), generator=c.gen).tolist()]
+    elif order == "interleaved":
+        tiles = sorted(tiles, key=lambda t: (t[3] // 64 % 3, t[2]))
+    elif order == "twice":
+        tiles = [t for t in tiles for _ in range(2)]
+    elif order == "short_followers":
+        tiles = [e for t in tiles for e in ((t, (t[0], max(1, t[1] // 2), t[2], t[3])) if (t[3] - spans[t[2]][0]) // 64 % 2 else (t,))]
+    else:
+        tiles = [e for t in tiles for e in (t, (t[0], max(1, t[1] // 2), t[2], t[3]))]
+    tiles += [(0, 0, 0, 0)] * pad
+    out = torch.full((row, 2 * 64), 7.0, dtype=torch.bfloat16, device=DEV)
+    torch.ops.cdb.kv8_prefill_attention(q.to(DEV), out, codes, scales, 1, table,
+                                        torch.tensor(tiles, dtype=torch.int32, device=DEV), 2, 64**-0.5)
+    torch.cuda.synchronize()
+    assert ops.status_code() == 0
+    _check_prefill(out.cpu(), c, q, spans, 2)
+
+
 def test_prefill_refuses_tiles_that_do_not_fit():
     c = Cache([64] * 2, 1, 64, seed=33, layers=1)
     c.table[1, 2] = -5
