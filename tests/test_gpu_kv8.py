@@ -480,3 +480,51 @@ def test_prefill_refuses_tiles_that_do_not_fit():
     assert code == 0 and (out == 7).all()
     out, code = call(0, 64, 1, 0)  # a missing block: its keys do not count
     assert code == 6 and out.isfinite().all() and (out[:, :] != 7).any()
+
+
+def test_blocks_beyond_four_gigabytes():
+    """Codes that lie past 2^32 bytes from the cache's start, and past it from V's: the same values, bit for bit, as
+    from a small cache that holds the same blocks."""
+
+    d, heads, n = 128, 2, 70
+    far_blocks = 1 << 21  # 2 x 4 GiB of codes
+    c = Cache([n], 1, d, seed=40, layers=1)
+    ids = [int(b) for b in c.table[0] if b >= 0]
+    far = {b: far_blocks - 1 - 7 * i for i, b in enumerate(ids)}
+    far_table = c.table.clone()
+    far_table[0, : len(ids)] = torch.tensor([far[b] for b in ids], dtype=torch.int32)
+    qkv = torch.randn(n, (heads + 2) * d, generator=c.gen).bfloat16().to(DEV)
+    slot = torch.zeros(n, dtype=torch.int32, device=DEV)
+    pos = torch.arange(n, dtype=torch.int32, device=DEV)
+    tiles = torch.tensor([(0, 64, 0, 0), (64, 6, 0, 64)], dtype=torch.int32, device=DEV)
+    got = []
+    for blocks, table in ((c.blocks, c.table), (far_blocks, far_table)):
+        codes = torch.empty(1, 2, blocks, 1, BS, d, dtype=torch.float8_e4m3fn, device=DEV)
+        scales = torch.empty(1, 2, blocks, 1, device=DEV)
+        t = table.to(DEV)
+        q = torch.empty(n, heads * d, dtype=torch.bfloat16, device=DEV)
+        out, pre = torch.empty_like(q), torch.empty_like(q)
+        back = torch.empty(len(ids), 2, 1, BS, d, dtype=torch.bfloat16, device=DEV)
+        torch.ops.cdb.kv8_append(qkv, q, codes, scales, 0, t, slot, pos, None, None, None, 0, heads)
+        torch.ops.cdb.kv8_gather(codes, scales, 0, t[0, : len(ids)].contiguous(), back)
+        torch.ops.cdb.kv8_decode_attention(q, out, codes, scales, 0, t, slot, pos, heads, 0.1)
+        torch.ops.cdb.kv8_prefill_attention(q, pre, codes, scales, 0, t, tiles, heads, 0.1)
+        back[-1, :, :, n % BS :] = 0  # never written
+        got.append((q, out, pre, back))
+    torch.cuda.synchronize()
+    assert ops.status_code() == 0
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    assert got[0][1].isfinite().all() and (got[0][1].float() - got[0][2].float()).abs().max() < 0.1
+
+
+def test_no_rows():
+    c = Cache([16], 1, 64, seed=41, layers=1)
+    codes, scales, table = c.gpu()
+    none, ints = torch.empty(0, 3 * 64, dtype=torch.bfloat16, device=DEV), torch.empty(0, dtype=torch.int32, device=DEV)
+    q = torch.empty(0, 64, dtype=torch.bfloat16, device=DEV)
+    torch.ops.cdb.kv8_append(none, q, codes, scales, 0, table, ints, ints, None, None, None, 0, 1)
+    torch.ops.cdb.kv8_decode_attention(q, q.clone(), codes, scales, 0, table, ints, ints, 1, 0.1)
+    torch.ops.cdb.kv8_prefill_attention(q, q.clone(), codes, scales, 0, table, ints.view(0, 4), 1, 0.1)
+    torch.ops.cdb.kv8_gather(codes, scales, 0, ints, torch.empty(0, 2, 1, BS, 64, dtype=torch.bfloat16, device=DEV))
+    torch.cuda.synchronize()
+    assert ops.status_code() == 0 and torch.equal(codes.cpu().view(torch.uint8), c.codes.view(torch.uint8))
