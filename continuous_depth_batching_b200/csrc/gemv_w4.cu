@@ -17,7 +17,7 @@
 // offset cancels costs fp32's 2^-24 of 128 sum |x|, far below bf16's rounding of the result.
 //
 // Measured (weights of other layers between two calls, so from HBM; groups of 128): 2048 x 5632, 1 token 5.2 us;
-// 11264 x 2048, 24 tokens 12 us; 49152 x 2048, 8 tokens 20 us (2.6 TB/s; 21 us at groups of 64, 27 at 32). A call
+// 11264 x 2048, 24 tokens 11.4 us; 49152 x 2048, 8 tokens 19 us (2.8 TB/s; 21 us at groups of 64, 25 at 32). A call
 // costs some 4.5 us before and after its boxes: launch, token rows, the first box's latency, the sum. The rest goes
 // on instructions, about 400 a box of 16 x 256 weights with the ALU pipe, which takes a nibble apart, the fullest.
 // 24 warps against 16 for 8 tokens: 18.1 against 19.5 us (49152 x 2048, weights in L2).
@@ -52,6 +52,12 @@ struct Params {
   int wk;      // warps that share a row tile
   int tokens;  // token rows of a CTA (grid y counts blocks of them)
   int stages;
+  // quotients, which the device would take some 30 instructions each for
+  int by_wk, by_subs;      // 65536 / wk and / subs, rounded up: (warp * by_wk) >> 16 is warp / wk
+  int each;                // boxes along k of one of wk warps
+  int row_groups;          // groups of wk warps in the grid
+  int rounds, rest;        // row tiles of each, and of how many one more
+  int step_tok, step_sub;  // warps of a CTA / subs, and the remainder
   int32_t* status;
 };
 
@@ -111,7 +117,7 @@ template <int GN>
 struct Entries<GN, true> {
   uint32_t s[2][GN / 2], z[2];  // per row: GN bf16, GN bytes (8 at most: two words)
   uint32_t z2[2];
-  __device__ __forceinline__ void load(const __nv_bfloat16* scale, const uint8_t* zero, int64_t to8, bool zeros) {
+  __device__ __forceinline__ void load(const __nv_bfloat16* scale, const uint8_t* zero, int to8, bool zeros) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const __nv_bfloat16* a = scale + r * to8;
@@ -179,12 +185,11 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid
   float* parts = xsum + p.subs * GN * NT * 8;                     // [warp][NT * 8][kPart], where wk > 1
 
   // this warp's place: part `part` of row tiles group, group + groups, ...
-  const int part = warp % p.wk;
-  const int groups = gridDim.x * (kWarps / p.wk);
-  const int group = blockIdx.x + gridDim.x * (warp / p.wk);  // few tiles spread over the SMs first
-  const int each = (p.subs + p.wk - 1) / p.wk;
-  const int sub0 = part * each, subs = max(0, min(each, p.subs - sub0));
-  const int rounds = group < p.tiles ? (p.tiles - group + groups - 1) / groups : 0;
+  const int team = (warp * p.by_wk) >> 16, part = warp - team * p.wk;
+  const int groups = p.row_groups;
+  const int group = blockIdx.x + gridDim.x * team;  // few tiles spread over the SMs first
+  const int sub0 = part * p.each, subs = max(0, min(p.each, p.subs - sub0));
+  const int rounds = p.rounds + (group < p.rest ? 1 : 0);
   const int boxes = rounds * subs;
 
   if (lane == 0) {
@@ -213,29 +218,28 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid
   // The scales and zero points of a box, loaded a box ahead of their use.
   constexpr int EN = WIDE ? 1 : GN / 2;
   Entries<GN, WIDE> entry;
-  const __nv_bfloat16* entry_scale[EN];  // each row's first
-  const uint8_t* entry_zero[EN];
-  int64_t to8 = 0;  // WIDE: from the scales of row g to those of row g + 8
+  int64_t entry_at[EN];  // each row's first
+  int to8 = 0;           // WIDE: from the scales of row g to those of row g + 8
   auto entry_tile = [&](int tile) {
 #pragma unroll
     for (int k = 0; k < EN; ++k) {
       const int at = min(tile * kRows + g + (WIDE ? 0 : 8 * ((t + 4 * k) / GN)), p.n - 1);
-      if (WIDE) to8 = (int64_t)(min(tile * kRows + g + 8, p.n - 1) - at) * p.groups;
-      entry_scale[k] = p.scales + (int64_t)at * p.groups;
-      entry_zero[k] = p.zeros + (int64_t)at * p.groups;
+      if (WIDE) to8 = (min(tile * kRows + g + 8, p.n - 1) - at) * p.groups;
+      entry_at[k] = (int64_t)at * p.groups;
     }
   };
   auto load_entries = [&](int i) {
     if constexpr (WIDE) {
-      entry.load(entry_scale[0] + (sub0 + i) * GN, entry_zero[0] + (sub0 + i) * GN, to8, p.zeros != nullptr);
+      const int64_t at = entry_at[0] + (sub0 + i) * GN;
+      entry.load(p.scales + at, p.zeros + at, to8, p.zeros != nullptr);
     } else {
 #pragma unroll
       for (int k = 0; k < EN; ++k) {
         int grp = (sub0 + i) * GN + (t + 4 * k) % GN;
         if (GI == 4 && p.group_boxes > 1) grp /= p.group_boxes;
         grp = min(grp, p.groups - 1);  // a box may reach past k, onto zeros of x
-        entry.e[k] = ((uint32_t)__bfloat16_as_ushort(entry_scale[k][grp]) << 16) |
-                     (p.zeros != nullptr ? entry_zero[k][grp] : 8u);
+        const int64_t at = entry_at[k] + grp;
+        entry.e[k] = ((uint32_t)__bfloat16_as_ushort(p.scales[at]) << 16) | (p.zeros != nullptr ? p.zeros[at] : 8u);
       }
     }
   };
@@ -247,8 +251,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid
   // the token rows and the sums of x over each group: a warp takes boxes of tokens, several loads in flight
   constexpr int AT_ONCE = 2 * NT;
   {
-    const int step_tok = kWarps / p.subs, step_sub = kWarps - step_tok * p.subs;
-    int tok = warp / p.subs, sub = warp - tok * p.subs;  // this warp's next box of tokens
+    int tok = (warp * p.by_subs) >> 16, sub = warp - tok * p.subs;  // this warp's next box of tokens
     while (tok < tokens) {
       uint4 v[AT_ONCE];
       int toks[AT_ONCE], places[AT_ONCE];
@@ -259,8 +262,8 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid
         if (tok < tokens && k < p.k) v[a] = *reinterpret_cast<const uint4*>(p.x + (int64_t)(tok0 + tok) * p.ldx + k);
         toks[a] = tok;
         places[a] = sub;
-        tok += step_tok;
-        sub += step_sub;
+        tok += p.step_tok;
+        sub += p.step_sub;
         if (sub >= p.subs) sub -= p.subs, ++tok;
       }
       float sum[AT_ONCE];
@@ -366,7 +369,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid
 #pragma unroll
       for (int c = 0; c < 4; ++c) mine[(j * 8 + 2 * t + (c & 1)) * kPart + g + 8 * (c >> 1)] = acc[j][c];
     }
-    const int id = 1 + warp / p.wk, threads = p.wk * 32;
+    const int id = 1 + team, threads = p.wk * 32;
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
     const float* from = parts + (warp - part) * PART;
     const int row = lane % kRows;
@@ -509,6 +512,14 @@ extern "C" int cdb_gemv_w4(const void* x, int64_t ldx, const void* w, int64_t ld
     const int cost = rounds * (2 * ((p.subs + w - 1) / w) + (w > 1 ? 1 : 0));
     if (best == 0 || cost < best) best = cost, p.wk = w;
   }
+  p.by_wk = (65536 + p.wk - 1) / p.wk;
+  p.by_subs = (65536 + p.subs - 1) / p.subs;
+  p.each = (p.subs + p.wk - 1) / p.wk;
+  p.row_groups = ctas * (warps / p.wk);
+  p.rounds = p.tiles / p.row_groups;
+  p.rest = p.tiles % p.row_groups;
+  p.step_tok = warps / p.subs;
+  p.step_sub = warps % p.subs;
   const dim3 grid(ctas, blocks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (gi == 1) return launch_groups<1>(map, p, grid, nt, st);
