@@ -27,8 +27,8 @@
 // Measured: 4096 rows at positions 4096 .. 8191, 16 heads of 128: 312 us, 660 TFLOP/s; chunks of up to 400
 // rows of 12 requests: 44 us, mostly the steps of the longest and a CTA's start. What bounds it is the softmax's way
 // through a step, some 2600 of 3200 cycles a step of each of the two CTAs: load S, maximum, exponentials, store P,
-// none of them long enough to hide the next one's latency. Tensor pipe 29% busy, shared memory 65%, issue slots
-// 55%, exponentials 35%. Tried: eight softmax warps with 16 rows each (four lanes a row) 349 us, for a third more
+// none of them long enough to hide the next one's latency. Tensor pipe 33% busy, shared memory's load and store
+// path 45%, issue slots 55%, exponentials 36%. Tried: eight softmax warps with 16 rows each (four lanes a row) 349 us, for a third more
 // instructions; four more conversion warps 321 us.
 //
 // A masked key never counts, whatever it holds: its logit is replaced, and a NaN in its V, which a product

@@ -44,7 +44,7 @@ The low-bit decode step's ops (``csrc/torch_ops.cpp``; all write into tensors th
   ``OuroRunner.prefill_tiles`` make them (``cdb_kv8_prefill_attention``);
 * ``cdb::gemv_w4(x, w, scales, zeros, out)``: a few token rows times 4-bit weights ``w [N, K / 2]``
   uint8 with bf16 ``scales`` and uint8 ``zeros`` (or None: 8) ``[N, K / group]`` (``cdb_gemv_w4``). The
-  weights are read once per 32 rows: from some hundred rows on ``gemm_bf16`` is the better call.
+  weights are read once per up to 32 rows: from some hundred rows on ``gemm_bf16`` is the better call.
 """
 
 from __future__ import annotations
