@@ -21,6 +21,11 @@
 // Pieces of a segment (m, l, o) meet in two steps: the warps of a CTA through shared memory, CTAs
 // through the workspace, where the last one to arrive adds them up in CTA order, head by head. The result
 // does not depend on which one that is.
+//
+// Measured: 8 rows of 30,000 to 65,536 positions, 32 query heads on 8 of 128: 141 us, 5.6 TB/s, bound by HBM; 80 rows
+// at 64 to 1300, 16 heads: 47 us, 4.8 TB/s over all, of which 3.6 us go by before the first page and 4 in the joins;
+// one row of 700: 9.7 us, a chain of latencies. 12 warps, because 163 registers a thread (a head's q and output stay
+// in them) and rings of two pairs (8 KB each at 128) take the SM's registers and shared memory.
 #include <cuda.h>
 
 #include "kv8.cuh"

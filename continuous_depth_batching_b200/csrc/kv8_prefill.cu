@@ -28,8 +28,9 @@
 // rows of 12 requests: 44 us, mostly the steps of the longest and a CTA's start. What bounds it is the softmax's way
 // through a step, some 2600 of 3200 cycles a step of each of the two CTAs: load S, maximum, exponentials, store P,
 // none of them long enough to hide the next one's latency. Tensor pipe 33% busy, shared memory's load and store
-// path 45%, issue slots 55%, exponentials 36%. Tried: eight softmax warps with 16 rows each (four lanes a row) 349 us, for a third more
-// instructions; four more conversion warps 321 us.
+// path 45%, issue slots 55%, exponentials 36%. Tried: eight softmax warps with 16 rows each (four lanes a row) 349
+// us, for a third more instructions; four more conversion warps 321 us; masks and the rare sums in loops of their
+// own, for less code, 313 us.
 //
 // A masked key never counts, whatever it holds: its logit is replaced, and a NaN in its V, which a product
 // with weight zero would spread, is taken out in the steps that the diagonal crosses and put back at the end
@@ -567,8 +568,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
         const float4 ks = *reinterpret_cast<const float4*>(sh.scale[j & (kMeta - 1)][0]);
         const float4 vs = *reinterpret_cast<const float4*>(sh.scale[j & (kMeta - 1)][1]);
         // logits are S * f; f stays above 0 (an all-zero block under a tiny q), below it no such block
-        const float f[4] = {ks.x < 0.f ? -1.f : fmaxf(factor * ks.x, 1.2e-38f), ks.y < 0.f ? -1.f : fmaxf(factor * ks.y, 1.2e-38f),
-                            ks.z < 0.f ? -1.f : fmaxf(factor * ks.z, 1.2e-38f), ks.w < 0.f ? -1.f : fmaxf(factor * ks.w, 1.2e-38f)};
+        auto logit_factor = [&](float k) { return k < 0.f ? -1.f : fmaxf(factor * k, 1.2e-38f); };
+        const float f[4] = {logit_factor(ks.x), logit_factor(ks.y), logit_factor(ks.z), logit_factor(ks.w)};
         const float ev[4] = {vs.x, vs.y, vs.z, vs.w};
         if (j >= diagonal || f[0] < 0.f || f[1] < 0.f || f[2] < 0.f || f[3] < 0.f) {
           const int seen = qpos - j * TK;  // the last key of the step that the row sees
@@ -712,7 +713,8 @@ extern "C" int cdb_kv8_prefill_attention(const void* q, int64_t q_stride, void* 
   using namespace cdb::kv8;
   if (codes == nullptr || scales == nullptr || (reinterpret_cast<uintptr_t>(codes) & 15) || cache_layer < 0 ||
       cache_layer >= num_cache_layers || num_blocks <= 0 || num_rows < 0 || num_tiles < 0 || num_tiles > 65535 ||
-      num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads != 0 || table_rows < 0 || table_width < 0 || !(scale > 0.f) || scale > 1e30f)
+      num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads != 0 || table_rows < 0 || table_width < 0 ||
+      !(scale > 0.f) || scale > 1e30f)
     return CDB_ERR_INVALID_ARGUMENT;
   if (head_dim != 64 && head_dim != 96 && head_dim != 128) return CDB_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(q) & 15) || (q_stride & 7) || (reinterpret_cast<uintptr_t>(out) & 15) ||

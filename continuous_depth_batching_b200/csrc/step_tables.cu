@@ -245,7 +245,8 @@ extern "C" int cdb_step_tables(const int32_t* slots, const int32_t* seq_len, con
                                int32_t* status, void* stream) {
   using namespace cdb;
   using namespace cdb::step;
-  if (num_requests < 0 || capacity > (1 << 30) || tile_capacity > (1 << 30) || table_rows < 0 || table_width < 0 || ring_size < 0 || capacity < 0 || tile_capacity < 0 ||
+  if (num_requests < 0 || capacity < 0 || capacity > (1 << 30) || tile_capacity < 0 || tile_capacity > (1 << 30) ||
+      table_rows < 0 || table_width < 0 || ring_size < 0 ||
       row_len == nullptr || block_table == nullptr || ring == nullptr || state == nullptr || row_len_out == nullptr ||
       state_out == nullptr || cu_seq_lens_q == nullptr || cu_seq_lens_k == nullptr ||
       (num_requests > 0 && (slots == nullptr || seq_len == nullptr || new_len == nullptr || granted == nullptr)) ||
