@@ -19,6 +19,13 @@ namespace kv8 {
 constexpr int kBlock = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// The attention kernels hold the weights of V in f16, as 2^(x + log2 s_v - M + kLift): M is a maximum that lags its
+// logits by up to 8, so they reach 2^15, of f16's 65504. From 2^-21 of the largest weight on each is rounded by
+// 2^-11 of itself; below, f16's steps stay 2^-24, so by 2^-32 of the largest one. Without the lift a key that
+// takes the mass and whose value is near 0 pushes the others there: 2048 weights of 2^-20.7 of it were off by 1.5%.
+constexpr float kLift = 7.f;
+constexpr float kUnlift = 1.f / 128.f;  // 2^-kLift
+
 // Smallest power of two s (>= 2^-126) with amax <= 448 s; 448 = 1.75 * 2^8.
 __device__ __forceinline__ float block_scale(float amax) {
   const uint32_t bits = __float_as_uint(amax);

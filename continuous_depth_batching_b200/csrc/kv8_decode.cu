@@ -15,8 +15,8 @@
 // 2^-24 of the row's largest element. x = S * (scale log2e 2^e s_k) in fp32. The softmax runs online
 // in base 2: m is a maximum of x that only moves when x passes it by 8 (then l, the sum of 2^(x-m),
 // is rescaled), and the weights of V, 2^(x-m) s_v, are taken relative to their own maximum M of
-// x + log2 s_v, so that they fit f16 (at most 2^8; 2^-11 relative rounding each, averaged over the
-// keys) whatever the blocks' scales are. O = V^T P (tensor cores again) in fp32.
+// x + log2 s_v, so that they fit f16 whatever the blocks' scales are (kLift in kv8.cuh: 2^-11 relative rounding each,
+// averaged over the keys, or 2^-32 of the largest). O = V^T P (tensor cores again) in fp32.
 //
 // Pieces of a segment (m, l, o) meet in two steps: the warps of a CTA through shared memory, CTAs
 // through the workspace, where the last one to arrive adds them up in CTA order, head by head. The result
@@ -175,7 +175,7 @@ __device__ __forceinline__ int tile_at(int r, int c) {
 template <int D, int HN>
 struct Running {
   float acc[Shape<D>::MT][4];
-  float m[HN], mw[HN], l[HN];
+  float m[HN], mw[HN], l[HN];  // mw: M - kLift
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < Shape<D>::MT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
@@ -327,7 +327,7 @@ __device__ __forceinline__ void pair_step(const uint8_t* at, const float4 scale,
 #pragma unroll
   for (int h = 0; h < HN; ++h) {
     const float a = fmaxf(x[h][0], x[h][1]), b = fmaxf(x[h][2], x[h][3]);
-    up = up || fmaxf(a, b) > r.m[h] + 8.f || fmaxf(a + ev[0], b + ev[1]) > r.mw[h] + 8.f;
+    up = up || fmaxf(a, b) > r.m[h] + 8.f || fmaxf(a + ev[0], b + ev[1]) > r.mw[h] + (8.f + kLift);
   }
   if (__any_sync(kFull, up)) {
 #pragma unroll
@@ -339,7 +339,7 @@ __device__ __forceinline__ void pair_step(const uint8_t* at, const float4 scale,
         mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, d));
         mz = fmaxf(mz, __shfl_xor_sync(kFull, mz, d));
       }
-      const float m = fmaxf(r.m[h], mx), mw = fmaxf(r.mw[h], mz);
+      const float m = fmaxf(r.m[h], mx), mw = fmaxf(r.mw[h], mz - kLift);
       r.l[h] *= m == -INFINITY ? 1.f : ex2(r.m[h] - m);
       const float down = mw == -INFINITY ? 1.f : ex2(r.mw[h] - mw);
       r.m[h] = m;
@@ -386,7 +386,7 @@ __device__ __forceinline__ void write_out(const DecodeParams& p, const Cursor& c
   for (int h = 0; h < HN; ++h) {
     const int in_kv = c.grp * kGroup + 2 * t + h;
     if (in_kv >= p.heads_per_kv) continue;
-    const float f = r.l[h] > 0.f ? ex2(r.mw[h] - r.m[h]) / r.l[h] : (r.l[h] == 0.f ? 0.f : r.l[h]);
+    const float f = r.l[h] > 0.f ? ex2(r.mw[h] + kLift - r.m[h]) * kUnlift / r.l[h] : (r.l[h] == 0.f ? 0.f : r.l[h]);
     __nv_bfloat16* dst =
         p.out + (int64_t)c.row * p.out_stride + (int64_t)(c.kvh * p.heads_per_kv + in_kv) * D + g * VD;
 #pragma unroll
@@ -407,7 +407,7 @@ __device__ __forceinline__ void store_piece(float* dst, int heads, const Running
     const int head = 2 * t + h;
     if (head >= heads) continue;
     float* o = dst + head * (D + 2);
-    const float f = r.mw[h] == -INFINITY ? 0.f : ex2(r.mw[h] - r.m[h]);
+    const float f = r.mw[h] == -INFINITY ? 0.f : ex2(r.mw[h] + kLift - r.m[h]) * kUnlift;
 #pragma unroll
     for (int i = 0; i < VD / 4; ++i) {
       float2* at = reinterpret_cast<float2*>(o + g * VD + 4 * i);

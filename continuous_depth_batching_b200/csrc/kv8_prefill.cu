@@ -20,9 +20,10 @@
 //
 // Arithmetic as in the decode kernel: q over a power of two per row, an online base-2 softmax with l relative
 // to a maximum m of the logits x, the weights of V, w = 2^x s_v, relative to their own maximum M and rounded
-// to f16 (2^-11). m and M move only when passed by 8, and then the row's O is rescaled in tensor memory.
-// One exponential a key: w 2^-M = 2^(S f + log2 s_v - M), and l takes the sum of a block's weights times the
-// block's 2^(M - m) / s_v, unless that factor is so far from 1 that the weights could have underflowed.
+// to f16 (kLift in kv8.cuh: by 2^-11, or 2^-32 of the largest). m and M move only when passed by 8, and then the row's
+// O is rescaled in tensor memory.
+// One exponential a key: w 2^(kLift - M) = 2^(S f + log2 s_v - M + kLift), and l takes the sum of a block's weights times
+// the block's 2^(M - kLift - m) / s_v, unless that factor is so far from 1 that the weights could have underflowed.
 //
 // Measured: 4096 rows at positions 4096 .. 8191, 16 heads of 128: 312 us, 660 TFLOP/s; chunks of up to 400
 // rows of 12 requests: 44 us, mostly the steps of the longest and a CTA's start. What bounds it is the softmax's way
@@ -554,7 +555,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
     mbar_arrive(&sh.qfull);
 
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    float m = -INFINITY, mw = -INFINITY, l = 0.f;
+    float m = -INFINITY, mw = -INFINITY, l = 0.f;  // mw: M - kLift
     for (int j = 0; j < steps; ++j) {
       if (!__all_sync(kAll, wait_for(&sh.sfull[j & 1], (j >> 1) & 1, p.status, abort))) break;
       bool stop = false;
@@ -596,9 +597,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
           l *= ex2(m - mx);
           m = mx;
         }
-        const bool up = mz > mw + 8.f;
+        const bool up = mz > mw + (8.f + kLift);
         if (__any_sync(kAll, up)) {
-          const float to = up ? mz : mw;
+          const float to = up ? mz - kLift : mw;
           if (j > 0)  // the products so far have to be in O
             stop = !__all_sync(kAll, wait_for(&sh.odone[(j - 1) & 1], ((j - 1) >> 1) & 1, p.status, abort));
           if (j > 0 && !stop) {
@@ -651,7 +652,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
     }
     if (rows_here && __all_sync(kAll, wait_for(&sh.odone[(steps - 1) & 1], ((steps - 1) >> 1) & 1, p.status, abort))) {
       fence_after();
-      const float g = l > 0.f ? ex2(mw - m) / l : (l == 0.f ? 0.f : l);
+      const float g = l > 0.f ? ex2(mw + kLift - m) * kUnlift / l : (l == 0.f ? 0.f : l);
       __nv_bfloat16* dst = p.out + (int64_t)(me.row0 + (mine ? r : 0)) * p.out_stride + (int64_t)head * D;
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
