@@ -934,23 +934,6 @@ __global__ void __launch_bounds__(MAXT, (MAXT <= 256 ? 4 : 1))
 }
 
 // ------------------------------------------------------------------ tensor-map cache (host)
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeFn get_encode() {
-  static EncodeFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeFn>(ptr);
-  });
-  return fn;
-}
-
 struct MapKey {
   const void* base;
   int layers;
@@ -977,7 +960,7 @@ static int kv_tensor_map(CUtensorMap* out, const void* base, int layers, int64_t
     *out = it->second;
     return CDB_OK;
   }
-  EncodeFn enc = get_encode();
+  EncodeFn enc = tensor_map_encoder();
   if (enc == nullptr) return CDB_ERR_TMA_ENCODE;
   const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)rows, (cuuint64_t)(2 * layers)};
   const cuuint64_t strides[3] = {(cuuint64_t)d * 2, (cuuint64_t)heads * d * 2, (cuuint64_t)rows * heads * d * 2};
@@ -1209,7 +1192,7 @@ static int scratch_address(uint8_t** out) {
 
 // The KV pool tensor map, encoded on the stack (the cached path keeps a host-side table).
 static int encode_kv_map(CUtensorMap* map, const void* base, int layers, int64_t rows, int heads, int d, int hg) {
-  EncodeFn enc = get_encode();
+  EncodeFn enc = tensor_map_encoder();
   if (enc == nullptr) return CDB_ERR_TMA_ENCODE;
   const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)rows, (cuuint64_t)(2 * layers)};
   const cuuint64_t strides[3] = {(cuuint64_t)d * 2, (cuuint64_t)heads * d * 2, (cuuint64_t)rows * heads * d * 2};

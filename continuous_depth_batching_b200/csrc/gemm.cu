@@ -715,23 +715,6 @@ __global__ void __launch_bounds__(THREADS, (BN < 128 ? 2 : 1))
 }
 
 // ------------------------------------------------------------------ host side
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeFn encoder() {
-  static EncodeFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeFn>(ptr);
-  });
-  return fn;
-}
-
 struct Key {
   const void* ptr;
   int64_t rows, cols, ld;
@@ -758,7 +741,7 @@ static int matrix_map(CUtensorMap* out, const void* ptr, int64_t rows, int64_t c
     *out = it->second;
     return CDB_OK;
   }
-  EncodeFn enc = encoder();
+  EncodeFn enc = tensor_map_encoder();
   if (enc == nullptr) return CDB_ERR_TMA_ENCODE;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};

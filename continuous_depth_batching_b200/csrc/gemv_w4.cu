@@ -391,22 +391,6 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) gemv_kernel(const __grid
   }
 }
 
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeFn encode_fn() {
-  static EncodeFn fn = [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult st;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &st) != cudaSuccess ||
-        st != cudaDriverEntryPointSuccess)
-      ptr = nullptr;
-    return reinterpret_cast<EncodeFn>(ptr);
-  }();
-  return fn;
-}
-
 // Bytes of a CTA's shared memory but for the ring.
 static int64_t row_bytes(int subs, int nt, int gi, int tokens, int wk) {
   const int kWarps = warps_of(nt);
@@ -464,7 +448,7 @@ extern "C" int cdb_gemv_w4(const void* x, int64_t ldx, const void* w, int64_t ld
   if (M == 0) return CDB_OK;
   if (x == nullptr || w == nullptr || scales == nullptr || out == nullptr) return CDB_ERR_INVALID_ARGUMENT;
   if (M > 65535) return CDB_ERR_INVALID_ARGUMENT;
-  EncodeFn encode = encode_fn();
+  EncodeFn encode = tensor_map_encoder();
   if (encode == nullptr) return CDB_ERR_TMA_ENCODE;
   CUtensorMap map;
   const cuuint64_t dims[2] = {(cuuint64_t)(K / 2), (cuuint64_t)N};

@@ -730,27 +730,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 constexpr int kSmemLimit = 218 * 1024;  // dynamic, beside 8 KB of static shared memory
 
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeFn encode_fn() {
-  static EncodeFn fn = [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult st;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &st) != cudaSuccess ||
-        st != cudaDriverEntryPointSuccess)
-      ptr = nullptr;
-    return reinterpret_cast<EncodeFn>(ptr);
-  }();
-  return fn;
-}
-
 template <int D, int HN>
 static int launch_decode(DecodeParams p, int num_ctas, cudaStream_t st) {
   CUtensorMap map = {};
   if (Shape<D>::SWIZZLED) {  // this layer's tiles, K then V, as rows of D bytes
-    EncodeFn encode = encode_fn();
+    EncodeFn encode = tensor_map_encoder();
     const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)2 * p.num_blocks * p.kv_heads * kBlock};
     const cuuint64_t strides[1] = {(cuuint64_t)D};
     const cuuint32_t box[2] = {(cuuint32_t)D, (cuuint32_t)kBlock}, ones[2] = {1, 1};
