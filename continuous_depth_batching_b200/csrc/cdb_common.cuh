@@ -138,6 +138,23 @@ inline void prefer_max_shared(const void* kernel) {
     cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
 }
 
+// Lets a kernel take up to `most` bytes of dynamic shared memory on the current device (set once). The limit
+// belongs to the process, so it is the most that any call takes: one set to each call's own size could be lowered
+// by another thread's call between that and the launch, which then fails.
+inline cudaError_t allow_shared(const void* kernel, int most) {
+  static std::mutex mu;
+  static std::unordered_set<const void*> done[64];  // by device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  std::unordered_set<const void*>& here = done[dev & 63];
+  if (here.count(kernel)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e == cudaSuccess) here.insert(kernel);
+  return e;
+}
+
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

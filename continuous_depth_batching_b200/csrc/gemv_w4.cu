@@ -406,8 +406,7 @@ static int launch(const CUtensorMap& map, Params p, dim3 grid, cudaStream_t st) 
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   const size_t smem = rest + (size_t)kWarps * p.stages * kTile;
   auto kernel = gemv_kernel<NT, GI, WIDE>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return CDB_ERR_CUDA;
+  if (allow_shared(reinterpret_cast<const void*>(kernel), kSmem) != cudaSuccess) return CDB_ERR_CUDA;
   return launch_pdl(kernel, grid, dim3(kWarps * 32), smem, st, map, p) == cudaSuccess ? CDB_OK : CDB_ERR_CUDA;
 }
 

@@ -753,8 +753,7 @@ static int launch_decode(DecodeParams p, int num_ctas, cudaStream_t st) {
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   const int smem = 1024 + p.stages * RING + (inside ? pieces : 0);
   auto kernel = decode_kernel<D, HN>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return CDB_ERR_CUDA;
+  if (allow_shared(reinterpret_cast<const void*>(kernel), kSmemLimit) != cudaSuccess) return CDB_ERR_CUDA;
   return launch_pdl(kernel, dim3(num_ctas), dim3(kThreads), smem, st, map, p) == cudaSuccess ? CDB_OK
                                                                                                 : CDB_ERR_CUDA;
 }

@@ -283,7 +283,7 @@ extern "C" int cdb_step_tables(const int32_t* slots, const int32_t* seq_len, con
   // requests of one token 5.1 us (5.5), 1024 tokens 5.4 (5.8), 2048 6.8 (6.2), 16384 20 (7.4).
   const int ctas = capacity <= kThreads ? 1 : 8;
   const size_t smem = (size_t)7 * num_requests * 4;
-  if (cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  if (allow_shared(reinterpret_cast<const void*>(step_tables_kernel), 7 * kMaxRequests * 4) != cudaSuccess)
     return CDB_ERR_CUDA;
   prefer_max_shared(reinterpret_cast<const void*>(step_tables_kernel));
   cudaLaunchConfig_t cfg = {};
