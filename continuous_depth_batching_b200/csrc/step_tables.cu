@@ -116,6 +116,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p, i
   const bool sane = head >= 0 && head < nb && avail >= 0 && avail <= nb;
   const int per = (n + kThreads - 1) / kThreads;
   const int j0 = min(n, (int)threadIdx.x * per), j1 = min(n, j0 + per);
+  constexpr int64_t kMost = 0x7fffffff;  // positions and sums are given in 32 bits
   bool bad = !sane;
   for (int j = j0; j < j1; ++j) {
     const int slot = p.slots[j], fresh = p.new_len[j];
@@ -126,10 +127,11 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p, i
       held = p.row_len[slot];
       if (fresh >= 0 && ctx >= 0 && held >= 0) {
         const int64_t total = ((int64_t)ctx + fresh + kBlock - 1) / kBlock;
-        if (total <= p.table_width && held <= p.table_width && sane) need = (int)(total > held ? total - held : 0);
+        if (total <= p.table_width && held <= p.table_width && sane && (int64_t)ctx + fresh <= kMost)
+          need = (int)(total > held ? total - held : 0);
       }
     }
-    bad = bad || !known || fresh < 0 || ctx < 0 || held < 0;
+    bad = bad || !known || fresh < 0 || ctx < 0 || held < 0 || (int64_t)ctx + fresh > kMost;
     s_slot[j] = known ? slot : -1;
     s_ctx[j] = ctx;
     s_held[j] = held;
@@ -139,7 +141,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p, i
   // What a request adds to the sums, and where they begin for this thread's requests.
   auto adds = [&](int j) {
     Sums a = {{0, 0, 0, 0}};
-    if (s_need[j] >= 0) a = {{s_need[j], s_q[j], (int64_t)s_ctx[j] + s_q[j], (s_q[j] + kTile - 1) / kTile}};
+    if (s_need[j] >= 0) a = {{s_need[j], s_q[j], (int64_t)s_ctx[j] + s_q[j], ((int64_t)s_q[j] + kTile - 1) / kTile}};
     return a;
   };
   Sums all;
@@ -164,25 +166,27 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p, i
   const bool fits = all_q <= p.cap && all_k <= 0x7fffffff && (p.tiles == nullptr || all_t <= p.tile_cap);
   if (ctas > 1)
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  // Nothing was written so far: every CTA has read slots, lengths and state.
+  // Nothing was written so far: every CTA has read slots, lengths and state. Sums past 32 bits stay at the largest
+  // number, so that those in shared memory ascend, as the searches below need.
+  auto cut = [](int64_t v) { return (int)(v < kMost ? v : kMost); };
   for (int j = j0; j < j1; ++j) {
     const Sums add = adds(j);
     if (rank == 0) {
       p.granted[j] = s_need[j] >= 0 ? 1 : 0;
-      p.cu_q[j] = (int)at.v[1];
-      p.cu_k[j] = (int)at.v[2];
+      p.cu_q[j] = cut(at.v[1]);
+      p.cu_k[j] = cut(at.v[2]);
       if (s_need[j] >= 0) p.row_len_out[s_slot[j]] = s_held[j] + s_need[j];
     }
     s_block[j] = (int)at.v[0];
-    s_q[j] = (int)at.v[1];
-    s_t[j] = (int)at.v[3];
+    s_q[j] = cut(at.v[1]);
+    s_t[j] = cut(at.v[3]);
     at.add(add);
   }
   if (rank == 0) {
     if (bad || !fits) set_error(p.status, CDB_ERR_INDEX);
     if (threadIdx.x == 0) {
-      p.cu_q[n] = (int)all_q;
-      p.cu_k[n] = (int)all_k;
+      p.cu_q[n] = cut(all_q);
+      p.cu_k[n] = cut(all_k);
       const int taken = (int)all_b;
       p.state_out[0] = sane && nb > 0 ? (int)(((int64_t)head + taken) % nb) : head;
       p.state_out[1] = avail - taken;

@@ -543,13 +543,14 @@ int cdb_kv8_prefill_attention(const void* q, int64_t q_stride, void* out, int64_
  *   row_len_out [table_rows], state_out [4]: the allocator after the step; only rows of granted
  *              requests are written. They may be row_len and state.
  *   cu_seq_lens_q / _k  [num_requests + 1]: sums of new tokens and of seq_len + new_len (0 for a
- *              refused request).
+ *              refused request); a sum past 2^31 - 1 is given as that.
  *   item_slot, item_pos, slot_map [capacity]: per new token, requests in order, its slot, position
  *              and cache row (block * 16 + place); -1 behind the last token.
  *   tiles      NULL, or int4 [tile_capacity] for the prefill attention entry points: runs of at most
  *              64 rows in order, entries behind the last all zero.
- * An unknown slot, a negative length, an invalid ring state, or more tokens or tiles than the
- * capacities hold set CDB_ERR_INDEX (with too many tiles no tile is written). */
+ * An unknown slot, a negative length, seq_len + new_len past 2^31 - 1 (such requests are refused), an
+ * invalid ring state, a sum of keys past 2^31 - 1, or more tokens or tiles than the capacities hold set
+ * CDB_ERR_INDEX (with too many tokens those that fit are written; with any of the last three no tile is). */
 int cdb_step_tables(const int32_t* slots, const int32_t* seq_len, const int32_t* new_len, const int32_t* row_len,
                     int num_requests, int32_t* block_table, int64_t block_table_stride, int table_rows,
                     int table_width, const int32_t* ring, int ring_size, const int32_t* state, int32_t* row_len_out,
