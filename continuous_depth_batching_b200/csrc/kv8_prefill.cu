@@ -384,6 +384,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
                (n < 2 ? wait_for(&sh.qfull, 0, p.status, abort)
                       : wait_for(&sh.odone[n & 1], ((n - 2) >> 1) & 1, p.status, abort));
           if (!__all_sync(kAll, ok)) break;
+          __syncwarp();  // lane 0's arrival releases the scales that the other lanes stored
           if (lane == 0) {
             fence_after();
 #pragma unroll

@@ -1,0 +1,57 @@
+"""Prefill attention over the 8-bit cache: blocks that all differ in scale, long lists, calls without rows.
+Tolerance as in test_gpu_kv8: 2^-8 |o| + 2^-10 sum p |v| / sum p."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import continuous_depth_batching_b200.ops  # noqa: F401  (registers torch.ops.cdb.*)
+import kv8_reference as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BS = 16
+
+
+def _cache(pages, kv_heads, d, seed):
+    """``pages``: blocks of each slot."""
+
+    g = torch.Generator().manual_seed(seed)
+    blocks = sum(pages)
+    codes = (torch.randn(1, 2, blocks, kv_heads, BS, d, generator=g) * 90).clamp(-448, 448).to(torch.float8_e4m3fn)
+    scales = torch.exp2(torch.randint(-10, -4, (1, 2, blocks, kv_heads), generator=g).float())
+    table = torch.full((len(pages), max(pages)), -1, dtype=torch.int32)
+    ids = torch.randperm(blocks, generator=g).int()
+    for i, n in enumerate(pages):
+        table[i, :n], ids = ids[:n], ids[n:]
+    return codes, scales, table, g
+
+
+def _run(q, codes, scales, table, tiles, heads, rows=None):
+    d = codes.shape[-1]
+    out = torch.full((q.shape[0] if rows is None else rows, heads * d), 7.0, dtype=torch.bfloat16, device=DEV)
+    torch.ops.cdb.kv8_prefill_attention(q.to(DEV), out, codes.to(DEV), scales.to(DEV), 0, table.to(DEV),
+                                        torch.tensor(tiles, dtype=torch.int32, device=DEV).view(-1, 4), heads, d**-0.5)
+    return out.cpu()
+
+
+def _near(got, q, codes, scales, table_row, first, heads):
+    n, d = q.shape[0], codes.shape[-1]
+    o, a = ref.attend(q.view(n, heads, d), codes[0], scales[0], table_row, first, d**-0.5)
+    assert ((got.double().view(n, heads, d) - o).abs() <= 2.0**-8 * o.abs() + 2.0**-10 * a).all()
+
+
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_scales_of_each_block_by_themselves(d):
+    """V's scales differ by up to 2^20 from block to block, so one taken for its neighbour's shows; the same bits
+    from call to call."""
+
+    codes, scales, table, g = _cache([60], 2, d, d)
+    scales[0, 1] = torch.exp2(torch.randint(-20, 1, scales[0, 1].shape, generator=g).float())
+    q = torch.randn(200, 2 * d, generator=g).bfloat16()
+    tiles = [(i, min(64, 200 - i), 0, 700 + i) for i in range(0, 200, 64)]
+    got = _run(q, codes, scales, table, tiles, 2)
+    _near(got, q, codes, scales, table[0], 700, 2)
+    for _ in range(20):
+        assert torch.equal(_run(q, codes, scales, table, tiles, 2), got)
