@@ -10,6 +10,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <limits>
 #include <map>
 #include <mutex>
 #include <optional>
@@ -39,6 +40,12 @@ c10::Device one_device(const T&... ts) {
   return *dev;
 }
 
+// The C ABI counts in 32 bits; cut to them, a larger number would pass for another.
+int as_int(const char* name, int64_t v) {
+  TORCH_CHECK_VALUE(v <= std::numeric_limits<int>::max(), name, " must be below 2^31, got ", v);
+  return (int)v;
+}
+
 bool aligned16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0; }
 
 // A 2-D bf16 tensor of at least rows x cols whose rows may be accessed 16 bytes at a time.
@@ -61,6 +68,8 @@ void check_table(const Tensor& t) {
                         (t.size(0) <= 1 || t.stride(0) >= t.size(1)),
                     "block_table must be a 2-D int32 tensor with unit column stride, got ", t.scalar_type(), " ",
                     t.sizes());
+  as_int("block_table's rows", t.size(0));
+  as_int("block_table's columns", t.size(1));
 }
 
 void check_tiles(const Tensor& t) {
@@ -86,12 +95,13 @@ Cache check_cache(const Tensor& codes, const Tensor& scales, int64_t layer) {
   TORCH_CHECK_VALUE(dim == 64 || dim == 96 || dim == 128, "the 8-bit cache takes head dims 64, 96 and 128, got ", dim);
   TORCH_CHECK_VALUE(layer >= 0 && layer < codes.size(0), "cache_layer must be in [0, ", codes.size(0), "), got ", layer);
   TORCH_CHECK_VALUE(aligned16(codes), "codes must be 16-byte aligned");
-  return {(int)codes.size(0), (int)codes.size(2), (int)codes.size(3), (int)dim};
+  return {as_int("layers", codes.size(0)), as_int("blocks", codes.size(2)), as_int("kv heads", codes.size(3)), (int)dim};
 }
 
 void check_heads(int64_t heads, int64_t kv_heads) {
   TORCH_CHECK_VALUE(heads > 0 && heads % kv_heads == 0, "num_heads must be a positive multiple of the cache's ", kv_heads,
                     " kv heads, got ", heads);
+  as_int("num_heads", heads);
 }
 
 template <typename T>
@@ -152,8 +162,9 @@ void kv8_append(const Tensor& qkv, const OptTensor& q_out, const Tensor& codes, 
                 const OptTensor& rope_cos, const OptTensor& rope_sin, const OptTensor& qk_bias, int64_t rope_mode,
                 int64_t num_heads) {
   const Cache c = check_cache(codes, scales, cache_layer);
-  const int64_t n = item_pos.numel();
+  const int64_t n = as_int("item_pos's entries", item_pos.numel());
   TORCH_CHECK_VALUE(num_heads > 0, "num_heads must be positive, got ", num_heads);
+  as_int("num_heads", num_heads);
   check_rows("qkv", qkv, n, (num_heads + 2 * c.heads) * c.dim);
   if (q_out) check_rows("q_out", *q_out, n, num_heads * c.dim);
   check_ints("item_pos", item_pos, n);
@@ -172,7 +183,7 @@ void kv8_append(const Tensor& qkv, const OptTensor& q_out, const Tensor& codes, 
                             aligned16(*t),
                         "rope_cos and rope_sin must be contiguous 16-byte aligned ", type, " tensors [positions, ", cols,
                         "] in rope_mode ", rope_mode);
-    rope_rows = (int)rope_cos->size(0);
+    rope_rows = as_int("rope_cos's positions", rope_cos->size(0));
   }
   TORCH_CHECK_VALUE(!qk_bias || (qk_bias->scalar_type() == at::kBFloat16 &&
                                  qk_bias->numel() == (num_heads + c.heads) * c.dim && qk_bias->is_contiguous() &&
@@ -195,7 +206,7 @@ void kv8_append(const Tensor& qkv, const OptTensor& q_out, const Tensor& codes, 
 void kv8_gather(const Tensor& codes, const Tensor& scales, int64_t cache_layer, const Tensor& blocks,
                 const Tensor& out) {
   const Cache c = check_cache(codes, scales, cache_layer);
-  const int64_t n = blocks.numel();
+  const int64_t n = as_int("blocks' entries", blocks.numel());
   check_ints("blocks", blocks, n);
   TORCH_CHECK_VALUE(out.scalar_type() == at::kBFloat16 && out.dim() == 5 && out.size(0) == n && out.size(1) == 2 &&
                         out.size(2) == c.heads && out.size(3) == kBlock && out.size(4) == c.dim &&
@@ -220,7 +231,7 @@ void kv8_decode_attention(const Tensor& q, const Tensor& out, const Tensor& code
   const Cache c = check_cache(codes, scales, cache_layer);
   check_heads(num_heads, c.heads);
   check_scale(scale);
-  const int64_t n = item_pos.numel();
+  const int64_t n = as_int("item_pos's entries", item_pos.numel());
   check_rows("q", q, n, num_heads * c.dim);
   check_rows("out", out, n, num_heads * c.dim);
   check_ints("item_pos", item_pos, n);
@@ -248,6 +259,7 @@ void kv8_prefill_attention(const Tensor& q, const Tensor& out, const Tensor& cod
   check_heads(num_heads, c.heads);
   check_scale(scale);
   check_rows("q", q, 0, num_heads * c.dim);
+  as_int("q's rows", q.size(0));
   check_rows("out", out, q.size(0), num_heads * c.dim);
   check_table(block_table);
   check_tiles(tiles);
@@ -267,7 +279,9 @@ void step_tables(const Tensor& slots, const Tensor& seq_len, const Tensor& new_l
                  const Tensor& block_table, const Tensor& ring, const Tensor& state, const Tensor& row_len_out,
                  const Tensor& state_out, const Tensor& granted, const Tensor& cu_q, const Tensor& cu_k,
                  const Tensor& item_slot, const Tensor& item_pos, const Tensor& slot_map, const OptTensor& tiles) {
-  const int64_t n = slots.numel(), rows = row_len.numel(), cap = item_pos.numel();
+  const int64_t n = slots.numel(), rows = as_int("row_len's entries", row_len.numel()), cap = item_pos.numel();
+  TORCH_CHECK_VALUE(cap <= 1 << 30, "one call takes at most 2^30 tokens, got ", cap);
+  as_int("ring's entries", ring.numel());
   check_ints("slots", slots, n);
   check_ints("new_len", new_len, n);
   check_ints("granted", granted, n);
@@ -287,6 +301,7 @@ void step_tables(const Tensor& slots, const Tensor& seq_len, const Tensor& new_l
                     block_table.size(0));
   TORCH_CHECK_VALUE(n <= 8192, "one call takes at most 8192 requests, got ", n);
   if (tiles) check_tiles(*tiles);
+  TORCH_CHECK_VALUE(!tiles || tiles->size(0) <= 1 << 30, "one call takes at most 2^30 tiles, got ", tiles->size(0));
   const auto dev = one_device(slots, seq_len, new_len, row_len, block_table, ring, state, row_len_out, state_out,
                               granted, cu_q, cu_k, item_slot, item_pos, slot_map, tiles);
   const c10::cuda::CUDAGuard guard(dev);
@@ -305,6 +320,8 @@ void gemv_w4(const Tensor& x, const Tensor& w, const Tensor& scales, const OptTe
                     "w must be a 2-D uint8 tensor [N, K / 2] with unit column stride, got ", w.scalar_type(), " ",
                     w.sizes());
   const int64_t n = w.size(0), k = 2 * w.size(1), m = x.dim() == 2 ? x.size(0) : 0;
+  as_int("w's rows", n + 15);  // in whole tiles of 16
+  as_int("K", k);
   const int64_t ldw = n > 1 ? w.stride(0) : (w.size(1) + 15) / 16 * 16;
   TORCH_CHECK_VALUE(k % 32 == 0 && ldw % 16 == 0 && ldw >= w.size(1) && aligned16(w),
                     "w needs K a multiple of 32, a row stride that is a multiple of 16 bytes and 16-byte alignment, got K ",
@@ -320,6 +337,7 @@ void gemv_w4(const Tensor& x, const Tensor& w, const Tensor& scales, const OptTe
                                zeros->is_contiguous()),
                     "zeros must be a contiguous uint8 tensor ", scales.sizes());
   check_rows("x", x, 0, k);
+  TORCH_CHECK_VALUE(m <= 65535, "one call takes at most 65535 token rows, got ", m);
   TORCH_CHECK_VALUE(x.size(1) == k, "x has ", x.size(1), " columns, the weights ", k);
   TORCH_CHECK_VALUE(out.scalar_type() == at::kBFloat16 && out.dim() == 2 && out.size(0) == m && out.size(1) == n &&
                         (n == 1 || out.stride(1) == 1) && (m <= 1 || out.stride(0) >= n),
