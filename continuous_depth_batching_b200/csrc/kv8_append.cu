@@ -204,7 +204,7 @@ __device__ __forceinline__ Run take_run(const Runs& r, int s) {
 // The block that the run's rows lie in, -1 where its indexes do not fit.
 __device__ __forceinline__ int block_of(const AppendParams& p, const Run& run) {
   if (run.slot < 0 || run.slot >= p.bt_rows || run.pos / kBlock >= p.bt_width ||
-      (p.rope_mode != 0 && run.pos + run.n > p.rope_rows))
+      (p.rope_mode != 0 && run.pos > p.rope_rows - run.n))
     return -1;
   return p.block_table[(int64_t)run.slot * p.bt_stride + run.pos / kBlock];
 }
