@@ -723,7 +723,8 @@ extern "C" int cdb_kv8_prefill_attention(const void* q, int64_t q_stride, void* 
       (out_stride & 7) || (reinterpret_cast<uintptr_t>(tiles) & 15))
     return CDB_ERR_INVALID_ARGUMENT;
   if (num_tiles == 0) return CDB_OK;
-  if (q == nullptr || out == nullptr || block_table == nullptr || tiles == nullptr) return CDB_ERR_INVALID_ARGUMENT;
+  if ((num_rows > 0 && (q == nullptr || out == nullptr)) || block_table == nullptr || tiles == nullptr)
+    return CDB_ERR_INVALID_ARGUMENT;  // (with no rows no tile fits, and q and out are not touched)
   PrefillParams p;
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.q_stride = q_stride;

@@ -6,8 +6,9 @@ from __future__ import annotations
 import pytest
 import torch
 
-import continuous_depth_batching_b200.ops  # noqa: F401  (registers torch.ops.cdb.*)
+import continuous_depth_batching_b200.ops as ops
 import kv8_reference as ref
+from continuous_depth_batching_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -55,3 +56,18 @@ def test_scales_of_each_block_by_themselves(d):
     _near(got, q, codes, scales, table[0], 700, 2)
     for _ in range(20):
         assert torch.equal(_run(q, codes, scales, table, tiles, 2), got)
+
+
+def test_no_rows_and_a_padded_list():
+    """q and out without rows, as a step without prompts has them: unused entries are skipped, others reported."""
+
+    codes, scales, table, _ = _cache([2], 1, 64, 1)
+    none = torch.empty(0, 64, dtype=torch.bfloat16)
+    assert _run(none, codes, scales, table, [(0, 0, 0, 0)] * 3, 1).shape == (0, 64)
+    assert ops.status_code() == 0
+    codes, scales, table = codes.to(DEV), scales.to(DEV), table.to(DEV)
+    status, tile = torch.zeros(1, dtype=torch.int32, device=DEV), torch.tensor([[0, 3, 0, 0]], dtype=torch.int32, device=DEV)
+    p = _lib.ptr
+    _lib.call("cdb_kv8_prefill_attention", None, 64, None, 64, 0, p(codes), p(scales), 1, 0, 2, p(table), 2, 1, 2, p(tile), 1,
+              1, 1, 64, 0.125, p(status), torch.cuda.current_stream().cuda_stream)
+    assert int(status.item()) == 6
