@@ -211,7 +211,8 @@ _TORCH_OPS_LOADED = False
 
 
 def load_torch_ops() -> None:
-    """Load the C++ operator library once (it registers its operators when it is loaded)."""
+    """Load the C++ operator library once (it registers its operators when it is loaded). Raises
+    ``CDBError`` where it is missing or was built for another torch."""
 
     global _TORCH_OPS_LOADED
     if _TORCH_OPS_LOADED:
@@ -219,7 +220,13 @@ def load_torch_ops() -> None:
     load()
     if not TORCH_OPS_PATH.exists():
         raise CDBError(f"{TORCH_OPS_PATH} is missing: build it with `python -m continuous_depth_batching_b200.csrc.build`")
-    torch.ops.load_library(str(TORCH_OPS_PATH))
+    try:
+        torch.ops.load_library(str(TORCH_OPS_PATH))
+    except OSError as e:
+        raise CDBError(
+            f"{TORCH_OPS_PATH} does not load beside torch {torch.__version__}; build it for this one with "
+            f"`python -m continuous_depth_batching_b200.csrc.build`: {e}"
+        ) from e
     _TORCH_OPS_LOADED = True
 
 

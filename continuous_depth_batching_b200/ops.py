@@ -49,25 +49,37 @@ The low-bit decode step's ops (``csrc/torch_ops.cpp``; all write into tensors th
 
 from __future__ import annotations
 
+import warnings
+
 import torch
 
 from . import _lib
 
-_lib.load_torch_ops()
-
 __all__ = ["gemm_bf16", "mlp_gateup_silu", "lm_head_argmax", "add_rmsnorm", "paged_decode_attention", "exit_gate_route",
            "step_tables", "kv8_append", "kv8_gather", "kv8_decode_attention", "kv8_prefill_attention", "gemv_w4"]
 
-# Registered by libcdb_torch.so; they only write into tensors that they are given, so tracing has no
-# shapes to ask of them.
-step_tables = torch.ops.cdb.step_tables
-kv8_append = torch.ops.cdb.kv8_append
-kv8_gather = torch.ops.cdb.kv8_gather
-kv8_decode_attention = torch.ops.cdb.kv8_decode_attention
-kv8_prefill_attention = torch.ops.cdb.kv8_prefill_attention
-gemv_w4 = torch.ops.cdb.gemv_w4
-for _name in ("step_tables", "kv8_append", "kv8_gather", "kv8_decode_attention", "kv8_prefill_attention", "gemv_w4"):
-    torch.library.register_fake(f"cdb::{_name}", lambda *args, **kwargs: None)
+_LOWBIT = ("step_tables", "kv8_append", "kv8_gather", "kv8_decode_attention", "kv8_prefill_attention", "gemv_w4")
+_MISSING: str | None = None  # why the low-bit ops are not there; the others need the C library only
+try:
+    _lib.load_torch_ops()
+except _lib.CDBError as e:
+    _MISSING = str(e)
+    warnings.warn(f"torch.ops.cdb has no low-bit ops ({', '.join(_LOWBIT)}): {e}", RuntimeWarning, stacklevel=2)
+
+
+def _lowbit(name: str):
+    if _MISSING is None:
+        # They only write into tensors that they are given, so tracing has no shapes to ask of them.
+        torch.library.register_fake(f"cdb::{name}", lambda *args, **kwargs: None)
+        return getattr(torch.ops.cdb, name)
+
+    def absent(*args, **kwargs):
+        raise _lib.CDBError(f"torch.ops.cdb.{name}: {_MISSING}")
+
+    return absent
+
+
+step_tables, kv8_append, kv8_gather, kv8_decode_attention, kv8_prefill_attention, gemv_w4 = map(_lowbit, _LOWBIT)
 
 
 def _cuda(*tensors: torch.Tensor | None) -> None:
@@ -95,7 +107,15 @@ def _capturing(t: torch.Tensor) -> bool:
 def _status(t: torch.Tensor) -> torch.Tensor:
     idx = t.device.index
     if idx not in _STATUS:
-        _STATUS[idx] = torch.ops.cdb._status_word(t)  # raises while a graph is captured, if it has to allocate
+        if _MISSING is None:
+            _STATUS[idx] = torch.ops.cdb._status_word(t)  # raises while a graph is captured, if it has to allocate
+        elif _capturing(t):
+            raise RuntimeError(
+                "torch.ops.cdb: the first call on a device allocates the shared status word; make one call before "
+                "capturing a CUDA graph"
+            )
+        else:
+            _STATUS[idx] = torch.zeros(1, dtype=torch.int32, device=t.device)
     return _STATUS[idx]
 
 
@@ -165,7 +185,7 @@ def status_code(device: torch.device | str | int | None = None) -> int:
     """The device-side status word the ops share on ``device`` (0 = ok); reading it synchronises."""
 
     dev = torch.device("cuda") if device is None else torch.device(device)
-    return int(torch.ops.cdb._status_word(torch.empty(0, device=dev)).item())
+    return int(_status(torch.empty(0, device=dev)).item())
 
 
 @torch.library.custom_op("cdb::gemm_bf16", mutates_args=("out",))
