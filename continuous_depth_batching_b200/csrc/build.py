@@ -1,7 +1,8 @@
 """Build libcdb_b200.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a, and libcdb_torch.so
 (PyTorch operators in C++ over it) with g++.
 
-    python -m continuous_depth_batching_b200.csrc.build
+    python -m continuous_depth_batching_b200.csrc.build            # both
+    python -m continuous_depth_batching_b200.csrc.build --c-abi    # the first alone: no g++, no torch headers
 
 The libraries land next to the package (``continuous_depth_batching_b200/libcdb_b200.so``) so
 they ship with the source tree; ``continuous_depth_batching_b200._lib`` loads them, the first with ctypes.
@@ -89,7 +90,6 @@ def build_library(force: bool = False, verbose: bool = False, jobs: int | None =
     if force or _stale(lib, objs):
         cmd = [nvcc, *ARCH_FLAGS, "-shared", "-Xlinker", f"-soname={LIB_NAME}", "-o", str(lib), *map(str, objs)]
         subprocess.run(cmd, check=True)
-    build_torch_ops(lib, force)
     return lib
 
 
@@ -116,3 +116,5 @@ def build_torch_ops(lib: Path, force: bool = False) -> Path:
 if __name__ == "__main__":
     path = build_library(force="--force" in sys.argv, verbose="-v" in sys.argv)
     print(path)
+    if "--c-abi" not in sys.argv:
+        print(build_torch_ops(path, force="--force" in sys.argv))

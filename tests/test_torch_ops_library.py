@@ -1,5 +1,5 @@
 """libcdb_torch.so holds the low-bit operators only: without it, or with one of another torch, the rest of the
-package works as it does without them."""
+package works as it does without them, and the C library is built without torch's headers."""
 
 from __future__ import annotations
 
@@ -8,6 +8,8 @@ import sys
 from pathlib import Path
 
 import pytest
+
+from continuous_depth_batching_b200.csrc import build
 
 ROOT = Path(__file__).resolve().parent.parent
 IMPORT = """
@@ -67,3 +69,14 @@ def test_import_without_it(tmp_path, what):
 @pytest.mark.gpu
 def test_other_operators_run_without_it(tmp_path):
     _run(GPU, _another(tmp_path, "missing"))
+
+
+def test_the_c_library_alone_needs_no_torch(tmp_path, monkeypatch):
+    """build_library() runs nvcc only."""
+
+    ran = []
+    monkeypatch.setattr(build.subprocess, "run", lambda cmd, **kw: ran.append(cmd[0]))
+    monkeypatch.setattr(build, "PKG", tmp_path)
+    monkeypatch.setattr(build, "SOURCES", [])
+    build.build_library()
+    assert len(ran) == 1 and ran[0] == build.nvcc_path()
