@@ -94,12 +94,16 @@ def build_library(force: bool = False, verbose: bool = False, jobs: int | None =
 
 
 def build_torch_ops(lib: Path, force: bool = False) -> Path:
-    """Compile ``torch_ops.cpp`` against the installed torch and link it to the CUDA library."""
+    """Compile ``torch_ops.cpp`` against the installed torch and link it to the CUDA library. The
+    result fits that build of torch only, so it is built again for another one."""
 
     import torch
 
     src, out = CSRC / "torch_ops.cpp", PKG / TORCH_LIB_NAME
-    if not force and not _stale(out, [src, lib, REPO / "include" / "cdb_b200.h"]):
+    built_for = PKG / "_build" / "torch_ops.torch"
+    this = f"{torch.__version__} {torch.version.git_version} {torch.__file__}"
+    same = built_for.exists() and built_for.read_text() == this
+    if not force and same and not _stale(out, [src, lib, REPO / "include" / "cdb_b200.h"]):
         return out
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc_path()).resolve().parent.parent
@@ -110,6 +114,8 @@ def build_torch_ops(lib: Path, force: bool = False) -> Path:
         f"-L{cuda / 'lib64'}", "-lcudart", "-Wl,-rpath,$ORIGIN",
     ]
     subprocess.run(cmd, check=True)
+    built_for.parent.mkdir(exist_ok=True)
+    built_for.write_text(this)
     return out
 
 

@@ -8,7 +8,9 @@ import sys
 from pathlib import Path
 
 import pytest
+import torch
 
+from continuous_depth_batching_b200 import _lib
 from continuous_depth_batching_b200.csrc import build
 
 ROOT = Path(__file__).resolve().parent.parent
@@ -80,3 +82,17 @@ def test_the_c_library_alone_needs_no_torch(tmp_path, monkeypatch):
     monkeypatch.setattr(build, "SOURCES", [])
     build.build_library()
     assert len(ran) == 1 and ran[0] == build.nvcc_path()
+
+
+def test_built_again_for_another_torch(tmp_path, monkeypatch):
+    ran = []
+    monkeypatch.setattr(build, "PKG", tmp_path)
+    monkeypatch.setattr(build.subprocess, "run", lambda cmd, **kw: (ran.append(cmd[0]), (tmp_path / build.TORCH_LIB_NAME).touch()))
+    lib = _lib.LIB_PATH
+    build.build_torch_ops(lib)
+    build.build_torch_ops(lib)
+    assert len(ran) == 1
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    build.build_torch_ops(lib)
+    build.build_torch_ops(lib)
+    assert len(ran) == 2
