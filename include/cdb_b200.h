@@ -461,8 +461,9 @@ int cdb_build_tables(const int32_t* block_table, int64_t block_table_stride, con
  * with amax <= 448 * 2^e over the block's finite values. Blocks are 16 tokens and addressed as in the
  * bf16 pool: position p of slot s lies at place p % 16 of block block_table[s][p / 16], for every
  * cache layer; a block of one layer, K or V, is 16 * num_kv_heads * head_dim contiguous bytes, so
- * cdb_kv_blocks_host_copy moves codes as it moves bf16 blocks. head_dim 64, 96 or 128. The
- * reference keeps its cache in the model's type only (continuous_batching/cache.py:131-145).
+ * cdb_kv_blocks_host_copy moves codes as it moves bf16 blocks (row_bytes num_kv_heads * head_dim, block_size
+ * 16). Codes mean nothing without their scales, which a second call moves (row_bytes num_kv_heads * 4,
+ * block_size 1, kv_rows num_blocks). head_dim 64, 96 or 128. The reference keeps its cache in the model's type only (continuous_batching/cache.py:131-145).
  * block_table [table_rows][table_width] int32 with row stride block_table_stride. An index outside
  * its range sets CDB_ERR_INDEX in *status and what it leads to is not read or written.
  * ------------------------------------------------------------------------------------- */

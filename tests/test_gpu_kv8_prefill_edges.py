@@ -9,6 +9,7 @@ import torch
 import continuous_depth_batching_b200.ops as ops
 import kv8_reference as ref
 from continuous_depth_batching_b200 import _lib
+from continuous_depth_batching_b200.runner import OuroRunner
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -71,3 +72,30 @@ def test_no_rows_and_a_padded_list():
     _lib.call("cdb_kv8_prefill_attention", None, 64, None, 64, 0, p(codes), p(scales), 1, 0, 2, p(table), 2, 1, 2, p(tile), 1,
               1, 1, 64, 0.125, p(status), torch.cuda.current_stream().cuda_stream)
     assert int(status.item()) == 6
+
+
+@pytest.mark.parametrize("order", ["requests", "framework", "shuffled"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_list_of_more_tiles_than_are_searched(d, order):
+    """Some 450 tiles that all hold rows: neighbours pair, whatever stands between them is taken by itself."""
+
+    n = 150
+    g = torch.Generator().manual_seed(d)
+    ctx = (torch.randint(0, 6, (n,), generator=g) * torch.tensor([16, 64, 23]).repeat(n // 3)).tolist()
+    new = torch.randint(129, 190, (n,), generator=g).tolist()
+    codes, scales, table, g = _cache([-(-(a + b) // BS) for a, b in zip(ctx, new)], 1, d, d + 1)
+    slot = [s for s in range(n) for _ in range(new[s])]
+    pos = [ctx[s] + i for s in range(n) for i in range(new[s])]
+    tiles = OuroRunner.prefill_tiles(slot, pos)  # longest first
+    if order == "requests":
+        tiles = sorted(tiles)
+    elif order == "shuffled":
+        tiles = [tiles[i] for i in torch.randperm(len(tiles), generator=g).tolist()]
+    assert len(tiles) == 3 * n
+    q = torch.randn(len(slot), d, generator=g).bfloat16()
+    out = _run(q, codes, scales, table, tiles, 1)
+    assert ops.status_code() == 0
+    row = 0
+    for s in range(n):
+        _near(out[row : row + new[s]], q[row : row + new[s]], codes, scales, table[s], ctx[s], 1)
+        row += new[s]
