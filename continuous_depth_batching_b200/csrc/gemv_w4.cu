@@ -16,10 +16,16 @@
 // both sums in fp32, then times the group's scale into the fp32 result: no weight is rounded. What the
 // offset cancels costs fp32's 2^-24 of 128 sum |x|, far below bf16's rounding of the result.
 //
-// Measured (weights of other layers between two calls, so from HBM; groups of 128): 2048 x 5632, 1 token 5.2 us;
-// 11264 x 2048, 24 tokens 11.4 us; 49152 x 2048, 8 tokens 19 us (2.8 TB/s; 21 us at groups of 64, 25 at 32). A call
+// Token rows are kept whole, so only as many as fit beside the rings share one pass over the weights: 32 up to K =
+// 1792, 27 to 29 by group size at K = 2048, 16 at 4096, 11 or 12 at 5632, 6 at 8192, 3 at 14336. More of them take
+// another pass each time (grid y).
+//
+// Measured (weights of other layers between two calls, so from HBM; a graph of such calls; groups of 128): 2048 x 5632,
+// 1 token 5.3 us; 11264 x 2048, 24 tokens 11.5 us, 32 tokens, in two passes, 17.5; 49152 x 2048, 8 tokens 19 us
+// (2.8 TB/s; 20 us at groups of 64, 25 at 32). cdb_gemm_bf16 on the same shapes takes 9.2, 11.6, 11.6 and 37 us. A call
 // costs some 4.5 us before and after its boxes: launch, token rows, the first box's latency, the sum. The rest goes
-// on instructions, about 400 a box of 16 x 256 weights with the ALU pipe, which takes a nibble apart, the fullest.
+// on instructions, about 465 a box of 16 x 256 weights, all counted, with the ALU pipe, which takes a nibble apart,
+// the fullest.
 // 24 warps against 16 for 8 tokens: 18.1 against 19.5 us (49152 x 2048, weights in L2).
 #include <cuda.h>
 

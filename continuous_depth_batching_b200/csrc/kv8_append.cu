@@ -12,7 +12,8 @@
 // (3.4 TB/s; 85 us with the rows' angles read from global memory for each head and one head to a warp); 80
 // decode rows, 16 heads of 128: 3.9 us.
 //
-// Read-back (gather): bytes; 1 in, 2 out a code. 31 us for those 4000 rows (132 MB, 4.2 TB/s).
+// Read-back (gather): 1 byte in, 2 out a code. 29 us for those 4000 rows (132 MB, 4.5 TB/s; 20 us of bytes), half of
+// the issue slots busy with the index divisions of each 16 codes.
 #include "kv8.cuh"
 
 namespace cdb {

@@ -24,8 +24,10 @@
 //
 // Measured: 8 rows of 30,000 to 65,536 positions, 32 query heads on 8 of 128: 141 us, 5.6 TB/s, bound by HBM; 80 rows
 // at 64 to 1300, 16 heads: 47 us, 4.8 TB/s over all, of which 3.6 us go by before the first page and 4 in the joins;
-// one row of 700: 9.7 us, a chain of latencies. 12 warps, because 163 registers a thread (a head's q and output stay
-// in them) and rings of two pairs (8 KB each at 128) take the SM's registers and shared memory.
+// one row of 700: 9.7 us, a chain of latencies. (Eager calls; one from a captured graph takes 1 to 1.5 us more, 11.2
+// there, because a fill in front of it zeroes counters of its own: the graph may run beside others.) 12 warps, because
+// 163 registers a thread (a head's q and output stay in them) and rings of two pairs (8 KB each at 128) take the SM's
+// registers and shared memory.
 #include <cuda.h>
 
 #include "kv8.cuh"
@@ -322,7 +324,7 @@ __device__ __forceinline__ void pair_step(const uint8_t* at, const float4 scale,
       }
     }
   }
-  // m and M only move when a logit passes them by 8 (the weights stay within 2^8): a vote a pair
+  // m and M only move when a logit passes them by 8 (the weights stay within 2^8 of 2^kLift): a vote a pair
   bool up = false;
 #pragma unroll
   for (int h = 0; h < HN; ++h) {
@@ -498,9 +500,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (rows != nullptr && (int64_t)p.num_items * vheads <= gridDim.x && longest <= p.whole_pairs &&
       (longest <= 2 * kWarps || 2 * even >= longest)) {
     // Few short segments: a CTA for each, so that none has to meet another's piece in the workspace, unless
-    // cutting them would leave a CTA less than half of one. Measured (16 heads of 128), whole against cut: 1 row of
-    // 700 positions 11.2 us (12.7), 8 of 700 11.3 (13.9), 9 of 1400 14.6 (19.1); 1 of 1400 14.4 (12.3), 2 of 1400
-    // 14.4 (12.1), 1 of 3000 21.1 (13.7).
+    // cutting them would leave a CTA less than half of one. Measured (16 heads of 128, from a graph), whole against
+    // cut: 1 row of 700 positions 11.2 us (12.7), 8 of 700 11.3 (13.9), 9 of 1400 14.6 (19.1); 1 of 1400 14.4 (12.3),
+    // 2 of 1400 14.4 (12.1), 1 of 3000 21.1 (13.7).
     const int row = blockIdx.x / vheads, vh = blockIdx.x - row * vheads;
     if (row >= p.num_items) return;
     const int n = s_row[row].x < 0 ? 0 : s_row[row].x / (2 * kBlock) + 1;

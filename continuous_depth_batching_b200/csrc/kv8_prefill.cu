@@ -22,15 +22,15 @@
 // to a maximum m of the logits x, the weights of V, w = 2^x s_v, relative to their own maximum M and rounded
 // to f16 (kLift in kv8.cuh: by 2^-11, or 2^-32 of the largest). m and M move only when passed by 8, and then the row's
 // O is rescaled in tensor memory.
-// One exponential a key: w 2^(kLift - M) = 2^(S f + log2 s_v - M + kLift), and l takes the sum of a block's weights times
-// the block's 2^(M - kLift - m) / s_v, unless that factor is so far from 1 that the weights could have underflowed.
+// One exponential a key: w 2^(kLift - M) = 2^(S f + log2 s_v - M + kLift), and l takes the sum of a block's weights
+// times the block's 2^(M - kLift - m) / s_v, unless that factor is so far from 1 that the weights could have underflowed.
 //
 // Measured: 4096 rows at positions 4096 .. 8191, 16 heads of 128: 312 us, 660 TFLOP/s; chunks of up to 400
 // rows of 12 requests: 44 us, mostly the steps of the longest and a CTA's start. What bounds it is the softmax's way
 // through a step, some 2600 of 3200 cycles a step of each of the two CTAs: load S, maximum, exponentials, store P,
 // none of them long enough to hide the next one's latency. Tensor pipe 33% busy, shared memory's load and store
 // path 45%, issue slots 55%, exponentials 36%. Tried: eight softmax warps with 16 rows each (four lanes a row) 349
-// us, for a third more instructions; four more conversion warps 321 us; masks and the rare sums in loops of their
+// us, for a third more instructions; four more conversion warps 321 us; masks and the second sums in loops of their
 // own, for less code, 313 us.
 //
 // A masked key never counts, whatever it holds: its logit is replaced, and a NaN in its V, which a product
@@ -235,7 +235,9 @@ __device__ __forceinline__ bool follows(const PrefillParams& p, int4 a, int4 b) 
 // in order of position, one with an even count before it leads, entries that overlap another of their slot do not.
 // In a longer list a tile whose position lies in an even 64 leads where its partner is beside it in the list,
 // which costs no search: lone tiles, 1000 and 2000 of them, take 603 and 1200 us, searched 643 and 1352; pairs
-// 600 and 1194, searched 643 and 1333.
+// 600 and 1194, searched 643 and 1333. The order matters there: prompts of 384 rows, 16 heads of 128, longest tiles
+// first (so few pairs) against request order, 64 prompts (384 tiles, searched) 216 us for 278, 80 (480) 345 for 335; 250
+// prompts of 256 rows (1000 tiles) 637 for 599.
 __device__ __forceinline__ Rows choose_rows(const PrefillParams& p, Shared& sh, int4 tile, int4 before, int4 after,
                                             int4 mine) {
   Rows me = {tile.x, tile.y, tile.z, tile.w};
@@ -637,7 +639,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
             tmem_store8(tmem + lanes + (j & 1) * TK + b * 8, w);
             if (!far) l += mw == -INFINITY ? 0.f : (sum + more) * ex2(-off - ev[b]);
           }
-          if (far) {  // rare: the weights may have underflowed, so the probabilities are summed themselves
+          // The weights may have underflowed, so the probabilities are summed themselves. Also taken in the last step
+          // of a row whose end leaves a whole block of it unused, which counts as log2 s_v = -126.
+          if (far) {
 #pragma unroll
             for (int k = 0; k < TK; ++k) {
               const float x = __uint_as_float(s[k]) * f[k >> 4];

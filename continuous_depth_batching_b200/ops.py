@@ -41,10 +41,14 @@ The low-bit decode step's ops (``csrc/torch_ops.cpp``; all write into tensors th
   own, so calls on several streams and graphs need no order among them;
 * ``cdb::kv8_prefill_attention(q, out, codes, scales, cache_layer, block_table, tiles, num_heads,
   scale)``: causal attention of prompt chunks over it, by tiles as ``step_tables`` or
-  ``OuroRunner.prefill_tiles`` make them (``cdb_kv8_prefill_attention``);
+  ``OuroRunner.prefill_tiles`` make them (``cdb_kv8_prefill_attention``). Up to 384 tiles the order of
+  ``prefill_tiles``, longest first, is the faster one; in longer lists a request's tiles run in pairs only
+  beside one another, as ``step_tables`` lists them;
 * ``cdb::gemv_w4(x, w, scales, zeros, out)``: a few token rows times 4-bit weights ``w [N, K / 2]``
   uint8 with bf16 ``scales`` and uint8 ``zeros`` (or None: 8) ``[N, K / group]`` (``cdb_gemv_w4``). The
-  weights are read once per up to 32 rows: from some hundred rows on ``gemm_bf16`` is the better call.
+  weights are read once for as many rows as fit shared memory (32 up to K = 1792, 27 at 2048, 11 at 5632,
+  6 at 8192). It is faster than ``gemm_bf16`` with 16-bit weights up to some 16 to 24 rows at K = 2048 (by N
+  and group size) and 8 at K = 5632; 80 rows take it 39 us for 13 at 11264 x 2048 and 52 for 11 at 2048 x 5632.
 """
 
 from __future__ import annotations

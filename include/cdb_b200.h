@@ -463,7 +463,8 @@ int cdb_build_tables(const int32_t* block_table, int64_t block_table_stride, con
  * cache layer; a block of one layer, K or V, is 16 * num_kv_heads * head_dim contiguous bytes, so
  * cdb_kv_blocks_host_copy moves codes as it moves bf16 blocks (row_bytes num_kv_heads * head_dim, block_size
  * 16). Codes mean nothing without their scales, which a second call moves (row_bytes num_kv_heads * 4,
- * block_size 1, kv_rows num_blocks). head_dim 64, 96 or 128. The reference keeps its cache in the model's type only (continuous_batching/cache.py:131-145).
+ * block_size 1, kv_rows num_blocks). head_dim 64, 96 or 128. The reference keeps its cache in the
+ * model's type only (continuous_batching/cache.py:131-145).
  * block_table [table_rows][table_width] int32 with row stride block_table_stride. An index outside
  * its range sets CDB_ERR_INDEX in *status and what it leads to is not read or written.
  * ------------------------------------------------------------------------------------- */
@@ -524,7 +525,8 @@ int cdb_kv8_decode_attention(const void* q, int64_t q_stride, void* out, int64_t
  *              to positions 0 .. position + r. An entry of 0 rows is skipped, and rows that no tile
  *              names are left as they were. The rows' keys and values are in the cache
  *              (cdb_kv8_append), q is rotated. The CTAs start in the list's
- *              order. Beyond 384 tiles those of a request should follow one another.
+ *              order, the longest best first. Two tiles of a request share a CTA: of up to 384 entries
+ *              wherever they stand, of more where they stand beside each other in the list.
  *   q, out, num_heads as cdb_kv8_decode_attention; num_rows: rows that q and out have. */
 int cdb_kv8_prefill_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, int num_rows,
                               const void* codes, const float* scales, int num_cache_layers, int cache_layer,
@@ -569,8 +571,9 @@ int cdb_step_tables(const int32_t* slots, const int32_t* seq_len, const int32_t*
  *   scales     bf16 [N][K / group_size]; group_size 32, 64 or a multiple of 128 that divides K.
  *   zeros      uint8 [N][K / group_size], or NULL: 8 everywhere.
  *   out        bf16 [M][ldo].
- * The weights are read once for every block of token rows: 32, or as many as fit shared memory beside
- * the rings where K is long (11 at K = 5632). CDB_ERR_UNSUPPORTED where not one row fits (K above
+ * The weights are read once for every block of token rows: 32 up to K = 1792, then as many as fit shared
+ * memory (27 to 29 by group size at K = 2048, 16 at 4096, 11 or 12 at 5632, 6 at 8192, 3 at 14336), so beyond
+ * the first block cdb_gemm_bf16 is faster. CDB_ERR_UNSUPPORTED where not one row fits (K above
  * 38,656 at groups of 32, 46,592 at 64, 51,712 beyond). Results do not depend on anything but the shapes and num_sms. */
 int cdb_gemv_w4(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* scales, const void* zeros,
                 void* out, int64_t ldo, int M, int N, int K, int group_size, int num_sms, int32_t* status,
