@@ -27,7 +27,8 @@
 // one row of 700: 9.7 us, a chain of latencies. (Eager calls; one from a captured graph takes 1 to 1.5 us more, 11.2
 // there, because a fill in front of it zeroes counters of its own: the graph may run beside others.) 12 warps, because
 // 163 registers a thread (a head's q and output stay in them) and rings of two pairs (8 KB each at 128) take the SM's
-// registers and shared memory.
+// registers and shared memory. More than 8 query heads a kv head stream its pages once per 8 of them, the second time
+// from L2: 8 rows of 32,768 with 16 heads on 2 43 us (134 MB), 32 heads on 2 57 us.
 #include <cuda.h>
 
 #include "kv8.cuh"
