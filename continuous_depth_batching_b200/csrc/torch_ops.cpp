@@ -1,4 +1,4 @@
-// torch.ops.cdb.* of the low-bit decode step: argument checks (types and shapes first, then the device,
+// torch.ops.cdb.* of the low-bit decode step and of many continuations of one prompt: argument checks (types and shapes first, then the device,
 // so that a call with CPU tensors is told what else is wrong with it), workspaces and the launch on the current
 // stream, over the C ABI. In C++ because a decode step makes hundreds of these calls and each kernel
 // takes a few microseconds: the same checks cost 17 us of host time a call in Python.
@@ -14,6 +14,7 @@
 #include <map>
 #include <mutex>
 #include <optional>
+#include <tuple>
 #include <utility>
 
 #include "../../include/cdb_b200.h"
@@ -140,21 +141,39 @@ int sm_count(c10::Device dev) {
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == CDB_OK, what, " failed: ", cdb_status_string(rc), " (status ", rc, ")"); }
 
-// Piece buffer and arrival counters of the decode attention. Eager calls keep one per stream, so that
-// calls on two streams never share one. A captured call takes its own from the graph's memory and
+// Piece buffer and arrival counters of a decode attention (`op` tells them apart). Eager calls keep one per stream, so
+// that calls on two streams never share one. A captured call takes its own from the graph's memory and
 // zeroes the counters inside the graph, so that two graphs may be replayed at once.
-std::pair<Tensor, Tensor> decode_workspace(c10::Device dev, c10::cuda::CUDAStream stream, int ctas, int dim) {
-  const int64_t floats = cdb_kv8_decode_workspace_floats(ctas, dim), counters = cdb_kv8_decode_counters(ctas);
+enum Op { kKv8Decode, kPrefixDecode };
+std::pair<Tensor, Tensor> workspace(Op op, c10::Device dev, c10::cuda::CUDAStream stream, int64_t floats,
+                                    int64_t counters) {
   const auto f32 = at::TensorOptions().dtype(at::kFloat).device(dev);
   const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
     return {at::empty({floats}, f32), at::zeros({counters}, i32)};
-  static auto& kept = *new std::map<std::pair<int, cudaStream_t>, std::pair<Tensor, Tensor>>;
+  static auto& kept = *new std::map<std::tuple<Op, int, cudaStream_t>, std::pair<Tensor, Tensor>>;
   std::lock_guard<std::mutex> lock(g_mutex);
-  auto& ws = kept[{dev.index(), stream.stream()}];
+  auto& ws = kept[{op, dev.index(), stream.stream()}];
   if (!ws.first.defined() || ws.first.numel() < floats || ws.second.numel() < counters)
     ws = {at::empty({floats}, f32), at::zeros({counters}, i32)};
   return ws;
+}
+
+// The rotation's tables; returns their positions.
+int check_rope(const OptTensor& rope_cos, const OptTensor& rope_sin, int64_t rope_mode, int64_t dim) {
+  TORCH_CHECK_VALUE(rope_mode >= 0 && rope_mode <= 2,
+                    "rope_mode must be 0 (none), 1 (split halves) or 2 (interleaved pairs), got ", rope_mode);
+  if (rope_mode == 0) return 0;
+  TORCH_CHECK_VALUE(rope_cos && rope_sin && rope_cos->sizes() == rope_sin->sizes(),
+                    "rope_cos and rope_sin must be given, with one shape, when rope_mode is not 0");
+  const auto type = rope_mode == 1 ? at::kBFloat16 : at::kFloat;
+  const int64_t cols = rope_mode == 1 ? dim : dim / 2;
+  for (const Tensor* t : {&*rope_cos, &*rope_sin})
+    TORCH_CHECK_VALUE(t->scalar_type() == type && t->dim() == 2 && t->size(1) == cols && t->is_contiguous() &&
+                          aligned16(*t),
+                      "rope_cos and rope_sin must be contiguous 16-byte aligned ", type, " tensors [positions, ", cols,
+                      "] in rope_mode ", rope_mode);
+  return as_int("rope_cos's positions", rope_cos->size(0));
 }
 
 void kv8_append(const Tensor& qkv, const OptTensor& q_out, const Tensor& codes, const Tensor& scales,
@@ -170,21 +189,7 @@ void kv8_append(const Tensor& qkv, const OptTensor& q_out, const Tensor& codes, 
   check_ints("item_pos", item_pos, n);
   check_ints("item_slot", item_slot, n);
   check_table(block_table);
-  TORCH_CHECK_VALUE(rope_mode >= 0 && rope_mode <= 2,
-                    "rope_mode must be 0 (none), 1 (split halves) or 2 (interleaved pairs), got ", rope_mode);
-  int rope_rows = 0;
-  if (rope_mode != 0) {
-    TORCH_CHECK_VALUE(rope_cos && rope_sin && rope_cos->sizes() == rope_sin->sizes(),
-                      "rope_cos and rope_sin must be given, with one shape, when rope_mode is not 0");
-    const auto type = rope_mode == 1 ? at::kBFloat16 : at::kFloat;
-    const int64_t cols = rope_mode == 1 ? c.dim : c.dim / 2;
-    for (const Tensor* t : {&*rope_cos, &*rope_sin})
-      TORCH_CHECK_VALUE(t->scalar_type() == type && t->dim() == 2 && t->size(1) == cols && t->is_contiguous() &&
-                            aligned16(*t),
-                        "rope_cos and rope_sin must be contiguous 16-byte aligned ", type, " tensors [positions, ", cols,
-                        "] in rope_mode ", rope_mode);
-    rope_rows = as_int("rope_cos's positions", rope_cos->size(0));
-  }
+  const int rope_rows = check_rope(rope_cos, rope_sin, rope_mode, c.dim);
   TORCH_CHECK_VALUE(!qk_bias || (qk_bias->scalar_type() == at::kBFloat16 &&
                                  qk_bias->numel() == (num_heads + c.heads) * c.dim && qk_bias->is_contiguous() &&
                                  aligned16(*qk_bias)),
@@ -242,7 +247,8 @@ void kv8_decode_attention(const Tensor& q, const Tensor& out, const Tensor& code
   const auto stream = c10::cuda::getCurrentCUDAStream(dev.index());
   const int ctas = sm_count(dev);
   const Tensor& status = status_word(dev);
-  const auto [ws, counters] = decode_workspace(dev, stream, ctas, c.dim);
+  const auto [ws, counters] = workspace(kKv8Decode, dev, stream, cdb_kv8_decode_workspace_floats(ctas, c.dim),
+                                        cdb_kv8_decode_counters(ctas));
   check(cdb_kv8_decode_attention(ptr<void>(q), q.stride(0), ptr<void>(out), out.stride(0), ptr<void>(codes),
                                  ptr<float>(scales), c.layers, (int)cache_layer, c.blocks, ptr<int32_t>(block_table),
                                  block_table.stride(0), (int)block_table.size(0), (int)block_table.size(1),
@@ -351,6 +357,131 @@ void gemv_w4(const Tensor& x, const Tensor& w, const Tensor& scales, const OptTe
         "cdb_gemv_w4");
 }
 
+struct Pool {
+  int layers, heads, dim;
+  int64_t rows;
+};
+
+Pool check_pool(const Tensor& pool, int64_t layer) {
+  TORCH_CHECK_VALUE(pool.scalar_type() == at::kBFloat16 && pool.dim() == 5 && pool.is_contiguous() &&
+                        pool.size(1) == 2 && pool.size(2) >= kBlock && pool.size(3) > 0,
+                    "kv_pool must be a contiguous bf16 tensor [layers, 2, rows, kv heads, head dim] of at least ", kBlock,
+                    " rows, got ", pool.scalar_type(), " ", pool.sizes());
+  const int64_t dim = pool.size(4);
+  TORCH_CHECK_VALUE(dim == 64 || dim == 96 || dim == 128, "head dims 64, 96 and 128 are taken, got ", dim);
+  TORCH_CHECK_VALUE(layer >= 0 && layer < pool.size(0), "cache_layer must be in [0, ", pool.size(0), "), got ", layer);
+  TORCH_CHECK_VALUE(aligned16(pool), "kv_pool must be 16-byte aligned");
+  return {as_int("layers", pool.size(0)), as_int("kv heads", pool.size(3)), (int)dim, pool.size(2)};
+}
+
+// Bytes from a 2-D tensor's first element to behind its last.
+std::pair<uintptr_t, uintptr_t> extent(const Tensor& t, int64_t rows, int64_t cols) {
+  const auto at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+  return {at, at + (uintptr_t)(((rows - 1) * t.stride(0) + cols) * t.element_size())};
+}
+
+void qk_norm_rope_append(const Tensor& qkv, const OptTensor& q_out, const Tensor& kv_pool, int64_t cache_layer,
+                         const Tensor& block_table, const Tensor& item_slot, const Tensor& item_pos,
+                         const Tensor& q_weight, const Tensor& k_weight, const OptTensor& rope_cos,
+                         const OptTensor& rope_sin, int64_t rope_mode, int64_t num_heads, double eps) {
+  const Pool c = check_pool(kv_pool, cache_layer);
+  const int64_t n = as_int("item_pos's entries", item_pos.numel());
+  TORCH_CHECK_VALUE(num_heads > 0, "num_heads must be positive, got ", num_heads);
+  as_int("num_heads", num_heads);
+  const int64_t all = num_heads + 2 * (int64_t)c.heads;
+  TORCH_CHECK_VALUE(all <= 1 << 20, "one call takes at most 2^20 heads, got ", all);
+  check_rows("qkv", qkv, n, all * c.dim);
+  if (q_out) {
+    check_rows("q_out", *q_out, n, num_heads * c.dim);
+    if (n > 0 && !(q_out->const_data_ptr() == qkv.const_data_ptr() && (n == 1 || q_out->stride(0) == qkv.stride(0)))) {
+      const auto a = extent(qkv, n, all * c.dim), b = extent(*q_out, n, num_heads * c.dim);
+      TORCH_CHECK_VALUE(a.second <= b.first || b.second <= a.first,
+                        "q_out may be q's columns of qkv, but may not overlap qkv otherwise");
+    }
+  }
+  check_ints("item_pos", item_pos, n);
+  check_ints("item_slot", item_slot, n);
+  check_table(block_table);
+  for (const auto& [name, t] : {std::pair<const char*, const Tensor&>("q_weight", q_weight), {"k_weight", k_weight}})
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kBFloat16 && t.dim() == 1 && t.size(0) == c.dim && t.is_contiguous() &&
+                          aligned16(t),
+                      name, " must be a contiguous 16-byte aligned bf16 tensor of ", c.dim, ", got ", t.scalar_type(), " ",
+                      t.sizes());
+  TORCH_CHECK_VALUE(eps >= 0 && eps <= 1e30, "eps must be finite and not negative, got ", eps);
+  const int rope_rows = check_rope(rope_cos, rope_sin, rope_mode, c.dim);
+  const auto dev = one_device(qkv, q_out, kv_pool, block_table, item_slot, item_pos, q_weight, k_weight, rope_cos, rope_sin);
+  const c10::cuda::CUDAGuard guard(dev);
+  const bool rope = rope_mode != 0;
+  check(cdb_qk_norm_rope_append(
+            ptr<void>(qkv), qkv.stride(0), ptr<void>(q_out), q_out ? q_out->stride(0) : 0, ptr<void>(kv_pool), c.layers,
+            c.rows, (int)cache_layer, ptr<int32_t>(block_table), block_table.stride(0), (int)block_table.size(0),
+            (int)block_table.size(1), ptr<int32_t>(item_slot), ptr<int32_t>(item_pos), ptr<void>(q_weight),
+            ptr<void>(k_weight), (int)rope_mode, rope ? ptr<void>(rope_cos) : nullptr,
+            rope ? ptr<void>(rope_sin) : nullptr, rope_rows, (float)eps, (int)n, (int)num_heads, c.heads, c.dim,
+            ptr<int32_t>(status_word(dev)), c10::cuda::getCurrentCUDAStream(dev.index()).stream()),
+        "cdb_qk_norm_rope_append");
+}
+
+void prefix_decode_attention(const Tensor& q, const Tensor& out, const Tensor& kv_pool, int64_t cache_layer,
+                             const Tensor& block_table, const Tensor& item_slot, const Tensor& item_pos,
+                             const Tensor& group_start, const Tensor& prefix_len, int64_t num_heads, double scale) {
+  const Pool c = check_pool(kv_pool, cache_layer);
+  check_heads(num_heads, c.heads);
+  check_scale(scale);
+  const int64_t n = as_int("item_pos's entries", item_pos.numel());
+  const int64_t groups = as_int("prefix_len's entries", prefix_len.numel());
+  check_rows("q", q, n, num_heads * c.dim);
+  check_rows("out", out, n, num_heads * c.dim);
+  check_ints("item_pos", item_pos, n);
+  check_ints("item_slot", item_slot, n);
+  check_ints("prefix_len", prefix_len, groups);
+  check_ints("group_start", group_start, groups > 0 ? groups + 1 : 0);
+  check_table(block_table);
+  const auto dev = one_device(q, out, kv_pool, block_table, item_slot, item_pos, group_start, prefix_len);
+  const c10::cuda::CUDAGuard guard(dev);
+  const auto stream = c10::cuda::getCurrentCUDAStream(dev.index());
+  const int sms = sm_count(dev);
+  const Tensor& status = status_word(dev);
+  const auto [ws, counters] = workspace(
+      kPrefixDecode, dev, stream,
+      cdb_prefix_decode_workspace_floats((int)n, (int)groups, (int)num_heads, c.heads, c.dim, sms),
+      cdb_prefix_decode_counters((int)n, (int)num_heads, c.heads));
+  check(cdb_prefix_decode_attention(
+            ptr<void>(q), q.stride(0), ptr<void>(out), out.stride(0), ptr<void>(kv_pool), c.layers, c.rows,
+            (int)cache_layer, ptr<int32_t>(block_table), block_table.stride(0), (int)block_table.size(0),
+            (int)block_table.size(1), ptr<int32_t>(item_slot), ptr<int32_t>(item_pos), (int)n,
+            ptr<int32_t>(group_start), ptr<int32_t>(prefix_len), (int)groups, (int)num_heads, c.heads, c.dim,
+            (float)scale, sms, ptr<float>(ws), ws.numel(), ptr<int32_t>(counters), counters.numel(),
+            ptr<int32_t>(status), stream.stream()),
+        "cdb_prefix_decode_attention");
+}
+
+void sample_tokens(const Tensor& logits, const Tensor& uniform, const Tensor& temperature, const OptTensor& top_k,
+                   const OptTensor& top_p, const OptTensor& min_p, const Tensor& out_ids, const OptTensor& out_logprobs) {
+  const bool wide = logits.scalar_type() == at::kFloat;
+  TORCH_CHECK_VALUE((wide || logits.scalar_type() == at::kBFloat16) && logits.dim() == 2 && logits.size(1) > 0,
+                    "logits must be a 2-D bf16 or fp32 tensor [rows, vocabulary], got ", logits.scalar_type(), " ",
+                    logits.sizes());
+  const int64_t n = as_int("logits' rows", logits.size(0)), v = logits.size(1);
+  TORCH_CHECK_VALUE(v <= 1 << 24, "vocabularies of up to 2^24 are taken, got ", v);
+  TORCH_CHECK_VALUE((v == 1 || logits.stride(1) == 1) && (n <= 1 || logits.stride(0) >= v),
+                    "logits need unit column stride and rows that do not overlap, got strides ", logits.strides());
+  check_ints("uniform", uniform, n, at::kFloat);
+  check_ints("temperature", temperature, n, at::kFloat);
+  if (top_k) check_ints("top_k", *top_k, n);
+  if (top_p) check_ints("top_p", *top_p, n, at::kFloat);
+  if (min_p) check_ints("min_p", *min_p, n, at::kFloat);
+  check_ints("out_ids", out_ids, n, at::kLong);
+  if (out_logprobs) check_ints("out_logprobs", *out_logprobs, n, at::kFloat);
+  const auto dev = one_device(logits, uniform, temperature, top_k, top_p, min_p, out_ids, out_logprobs);
+  const c10::cuda::CUDAGuard guard(dev);
+  check(cdb_sample_tokens(ptr<void>(logits), wide, n > 1 ? logits.stride(0) : v, (int)n, (int)v, ptr<float>(uniform),
+                          ptr<float>(temperature), ptr<int32_t>(top_k), ptr<float>(top_p), ptr<float>(min_p),
+                          ptr<int64_t>(out_ids), ptr<float>(out_logprobs),
+                          c10::cuda::getCurrentCUDAStream(dev.index()).stream()),
+        "cdb_sample_tokens");
+}
+
 Tensor status(const Tensor& like) {
   const auto dev = one_device(like);
   const c10::cuda::CUDAGuard guard(dev);
@@ -376,6 +507,16 @@ TORCH_LIBRARY_FRAGMENT(cdb, m) {
       "Tensor state, Tensor(b!) row_len_out, Tensor(c!) state_out, Tensor(d!) granted, Tensor(e!) cu_seq_lens_q, "
       "Tensor(f!) cu_seq_lens_k, Tensor(g!) item_slot, Tensor(h!) item_pos, Tensor(i!) slot_map, Tensor(j!)? tiles) -> ()");
   m.def("gemv_w4(Tensor x, Tensor w, Tensor scales, Tensor? zeros, Tensor(a!) out) -> ()");
+  m.def(
+      "qk_norm_rope_append(Tensor qkv, Tensor(a!)? q_out, Tensor(b!) kv_pool, int cache_layer, Tensor block_table, Tensor "
+      "item_slot, Tensor item_pos, Tensor q_weight, Tensor k_weight, Tensor? rope_cos, Tensor? rope_sin, int rope_mode, "
+      "int num_heads, float eps) -> ()");
+  m.def(
+      "prefix_decode_attention(Tensor q, Tensor(a!) out, Tensor kv_pool, int cache_layer, Tensor block_table, Tensor "
+      "item_slot, Tensor item_pos, Tensor group_start, Tensor prefix_len, int num_heads, float scale) -> ()");
+  m.def(
+      "sample_tokens(Tensor logits, Tensor uniform, Tensor temperature, Tensor? top_k, Tensor? top_p, Tensor? min_p, "
+      "Tensor(a!) out_ids, Tensor(b!)? out_logprobs) -> ()");
   m.def("_status_word(Tensor like) -> Tensor");
 }
 
@@ -387,5 +528,8 @@ TORCH_LIBRARY_IMPL(cdb, CompositeExplicitAutograd, m) {
   m.impl("kv8_prefill_attention", &kv8_prefill_attention);
   m.impl("step_tables", &step_tables);
   m.impl("gemv_w4", &gemv_w4);
+  m.impl("qk_norm_rope_append", &qk_norm_rope_append);
+  m.impl("prefix_decode_attention", &prefix_decode_attention);
+  m.impl("sample_tokens", &sample_tokens);
   m.impl("_status_word", &status);
 }

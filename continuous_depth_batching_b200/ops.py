@@ -49,6 +49,21 @@ The low-bit decode step's ops (``csrc/torch_ops.cpp``; all write into tensors th
   weights are read once for as many rows as fit shared memory (32 up to K = 1792, 27 at 2048, 11 at 5632,
   6 at 8192). It is faster than ``gemm_bf16`` with 16-bit weights up to some 16 to 24 rows at K = 2048 (by N
   and group size) and 8 at K = 5632; 80 rows take it 39 us for 13 at 11264 x 2048 and 52 for 11 at 2048 x 5632.
+
+Many continuations of one prompt, over the bf16 paged cache ``kv_pool [layers, 2, rows, kv heads, head dim]`` of
+``paged_decode_attention`` (also in ``csrc/torch_ops.cpp``; head dims 64, 96 and 128, any multiple of the kv heads):
+
+* ``cdb::qk_norm_rope_append(qkv, q_out, kv_pool, cache_layer, block_table, item_slot, item_pos, q_weight,
+  k_weight, rope_cos, rope_sin, rope_mode, num_heads, eps)``: RMS norms of each head's query and key (weights
+  bf16 ``[head dim]``), rotation, append (``cdb_qk_norm_rope_append``). q goes to ``q_out``, which may be q's
+  columns of ``qkv``; None leaves q alone;
+* ``cdb::prefix_decode_attention(q, out, kv_pool, cache_layer, block_table, item_slot, item_pos, group_start,
+  prefix_len, num_heads, scale)``: decode attention in which rows ``group_start[g] .. group_start[g + 1] - 1``
+  share the blocks of their first ``prefix_len[g]`` tokens, read once for all of them
+  (``cdb_prefix_decode_attention``). Streams and graphs as ``kv8_decode_attention``;
+* ``cdb::sample_tokens(logits, uniform, temperature, top_k, top_p, min_p, out_ids, out_logprobs)``: the next
+  token of every row of bf16 or fp32 logits by temperature, top-k, top-p and min-p (None: off) from one given
+  random number a row (``cdb_sample_tokens``).
 """
 
 from __future__ import annotations
@@ -60,18 +75,21 @@ import torch
 from . import _lib
 
 __all__ = ["gemm_bf16", "mlp_gateup_silu", "lm_head_argmax", "add_rmsnorm", "paged_decode_attention", "exit_gate_route",
-           "step_tables", "kv8_append", "kv8_gather", "kv8_decode_attention", "kv8_prefill_attention", "gemv_w4"]
+           "step_tables", "kv8_append", "kv8_gather", "kv8_decode_attention", "kv8_prefill_attention", "gemv_w4",
+           "qk_norm_rope_append", "prefix_decode_attention", "sample_tokens"]
 
 _LOWBIT = ("step_tables", "kv8_append", "kv8_gather", "kv8_decode_attention", "kv8_prefill_attention", "gemv_w4")
-_MISSING: str | None = None  # why the low-bit ops are not there; the others need the C library only
+_CONTINUE = ("qk_norm_rope_append", "prefix_decode_attention", "sample_tokens")
+_MISSING: str | None = None  # why the ops above are not there; the others need the C library only
 try:
     _lib.load_torch_ops()
 except _lib.CDBError as e:
     _MISSING = str(e)
-    warnings.warn(f"torch.ops.cdb has no low-bit ops ({', '.join(_LOWBIT)}): {e}", RuntimeWarning, stacklevel=2)
+    warnings.warn(f"torch.ops.cdb has no low-bit ops ({', '.join(_LOWBIT)}) and none of {', '.join(_CONTINUE)}: {e}",
+                  RuntimeWarning, stacklevel=2)
 
 
-def _lowbit(name: str):
+def _compiled(name: str):
     if _MISSING is None:
         # They only write into tensors that they are given, so tracing has no shapes to ask of them.
         torch.library.register_fake(f"cdb::{name}", lambda *args, **kwargs: None)
@@ -83,7 +101,8 @@ def _lowbit(name: str):
     return absent
 
 
-step_tables, kv8_append, kv8_gather, kv8_decode_attention, kv8_prefill_attention, gemv_w4 = map(_lowbit, _LOWBIT)
+step_tables, kv8_append, kv8_gather, kv8_decode_attention, kv8_prefill_attention, gemv_w4 = map(_compiled, _LOWBIT)
+qk_norm_rope_append, prefix_decode_attention, sample_tokens = map(_compiled, _CONTINUE)
 
 
 def _cuda(*tensors: torch.Tensor | None) -> None:

@@ -579,6 +579,79 @@ int cdb_gemv_w4(const void* x, int64_t ldx, const void* w, int64_t ldw, const vo
                 void* out, int64_t ldo, int M, int N, int K, int group_size, int num_sms, int32_t* status,
                 void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Many continuations of one prompt, over the bf16 paged pool: kv[num_cache_layers][2][kv_rows]
+ * [num_kv_heads][head_dim], 16-byte aligned, blocks of 16 rows, block_table [table_rows][table_width]
+ * int32 with row stride block_table_stride; head_dim 64, 96 or 128; num_heads any multiple of
+ * num_kv_heads where a query head reads kv head h / (num_heads / num_kv_heads). An index outside its
+ * range sets CDB_ERR_INDEX in *status and what it leads to is not read or written. The reference keeps
+ * such a cache (continuous_batching/cache.py:131-145) for models without query and key norms, reads it
+ * once per request (transformers integrations/flash_paged.py:84-122) and takes the likeliest token.
+ * ------------------------------------------------------------------------------------- */
+
+/* Norms of each head's query and key, rotation, and append to the cache; cdb_rope_append_kv's sibling
+ * for models that normalise q and k (and for grouped heads).
+ *   qkv        bf16 [num_items, qkv_stride]: q (num_heads), k, v (num_kv_heads each) side by side;
+ *              16-byte aligned, stride a multiple of 8.
+ *   q_out      bf16 rows of the normed, rotated q (stride a multiple of 8, 16-byte aligned); may be
+ *              qkv itself; may not overlap it otherwise; NULL leaves q alone.
+ *   q_weight, k_weight  bf16 [head_dim], 16-byte aligned: y = x * rsqrt(mean(x^2) + eps) * weight.
+ *   rope_mode  0 none, 1 split halves (bf16 tables [rope_rows][head_dim]), 2 interleaved pairs (fp32
+ *              tables [rope_rows][head_dim/2]); tables 16-byte aligned.
+ *   item_pos   position of each row, < 0: a padding row, skipped. A (slot, position) stands once in a call.
+ * Norm and rotation are computed in fp32 and rounded once. */
+int cdb_qk_norm_rope_append(const void* qkv, int64_t qkv_stride, void* q_out, int64_t q_out_stride, void* kv_base,
+                            int num_cache_layers, int64_t kv_rows, int cache_layer, const int32_t* block_table,
+                            int64_t block_table_stride, int table_rows, int table_width, const int32_t* item_slot,
+                            const int32_t* item_pos, const void* q_weight, const void* k_weight, int rope_mode,
+                            const void* rope_cos, const void* rope_sin, int rope_rows, float eps, int num_items,
+                            int num_heads, int num_kv_heads, int head_dim, int32_t* status, void* stream);
+
+/* fp32 elements of cdb_prefix_decode_attention's workspace, and its int32 counters. */
+int64_t cdb_prefix_decode_workspace_floats(int num_items, int num_groups, int num_heads, int num_kv_heads,
+                                           int head_dim, int num_sms);
+int64_t cdb_prefix_decode_counters(int num_items, int num_heads, int num_kv_heads);
+
+/* Decode attention: row i attends to positions 0 .. item_pos[i] of slot item_slot[i]; a row with
+ * item_pos < 0 is skipped and its out row left as it was. Rows of a group share their first blocks, which
+ * are read once for all of them.
+ *   q, out       bf16 rows of num_heads * head_dim, q rotated; 16-byte aligned, strides multiples of 8.
+ *   group_start  [num_groups + 1] ascending: rows group_start[g] .. group_start[g + 1] - 1 are group g.
+ *                Rows before the first and behind the last group stand alone.
+ *   prefix_len   [num_groups]: the first prefix_len[g] / 16 (rounded down) entries of the rows' block-table
+ *                rows are the same blocks for every row of the group with item_pos >= 0. Blocks that some such row
+ *                does not see whole are not shared. num_groups 0: every row stands alone.
+ *                Group bounds that descend or leave [0, num_items] set CDB_ERR_INDEX, and no blocks are shared.
+ *   workspace    cdb_prefix_decode_workspace_floats elements, 16-byte aligned; counters:
+ *                cdb_prefix_decode_counters, zeroed before the first use, left zeroed. Calls that share
+ *                them must be ordered. scale > 0. */
+int cdb_prefix_decode_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* kv_base,
+                                int num_cache_layers, int64_t kv_rows, int cache_layer, const int32_t* block_table,
+                                int64_t block_table_stride, int table_rows, int table_width, const int32_t* item_slot,
+                                const int32_t* item_pos, int num_items, const int32_t* group_start,
+                                const int32_t* prefix_len, int num_groups, int num_heads, int num_kv_heads,
+                                int head_dim, float scale, int num_sms, float* workspace, int64_t workspace_floats,
+                                int32_t* counters, int64_t num_counters, int32_t* status, void* stream);
+
+/* The next token of every row of logits [num_rows][vocab] (bf16, or fp32 where logits_fp32; rows at
+ * logits_stride elements, aligned to their type) from one given random number a row.
+ *   A token weighs w = exp((logit - largest) / temperature[r]); tokens are ordered by falling logit, equal ones by
+ *   index. top_k keeps the first top_k[r]; top_p, of those, the ones before which less than top_p[r] of
+ *   their weight lies; min_p, of those, the ones with w >= min_p[r]; the first always stays. The token is the
+ *   least index at which the kept weights' running sum passes uniform[r] times their total.
+ *   top_k, top_p, min_p   [num_rows] each or NULL: off; off in a row where top_k <= 0 (or >= vocab), top_p >= 1,
+ *              min_p <= 0. NaN is off. top_p <= 0 keeps one token, min_p >= 1 the largest logits.
+ *   temperature [num_rows]: <= 0 or NaN takes the first of the largest logits.
+ *   uniform    [num_rows] in [0, 1); numbers outside count as the nearest inside, NaN as 0.
+ *   out_ids    int64 [num_rows]; out_logprobs fp32 [num_rows] or NULL: log of the token's share of the kept weights.
+ * Logits: NaN counts as -inf and is never drawn; where the largest is +inf, tokens at +inf weigh 1 and
+ * others 0. A row without a logit above -inf gives id -1 and log-probability NaN. Weights are whole
+ * multiples of 2^-S of the largest, S = min(48, 62 - ceil(log2 vocab)): below half of one a token is never drawn.
+ * vocab <= 2^24. The result depends on nothing but the row. */
+int cdb_sample_tokens(const void* logits, int logits_fp32, int64_t logits_stride, int num_rows, int vocab,
+                      const float* uniform, const float* temperature, const int32_t* top_k, const float* top_p,
+                      const float* min_p, int64_t* out_ids, float* out_logprobs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
