@@ -179,14 +179,13 @@ _SIGNATURES: dict[str, list] = {
         c_int, c_int, c_int, c_int, c_void_p, c_void_p,  # num_items, num_heads, num_kv_heads, head_dim, status, stream
     ],
     "cdb_prefix_decode_workspace_floats": [c_int, c_int, c_int, c_int, c_int, c_int],
-    "cdb_prefix_decode_counters": [c_int, c_int, c_int],
     "cdb_prefix_decode_attention": [
         c_void_p, c_int64, c_void_p, c_int64,  # q, stride, out, stride
         c_void_p, c_int, c_int64, c_int,  # kv_base, num_cache_layers, kv_rows, cache_layer
         c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p,  # block_table, stride, rows, width, item_slot, item_pos
         c_int, c_void_p, c_void_p, c_int,  # num_items, group_start, prefix_len, num_groups
         c_int, c_int, c_int, c_float, c_int,  # heads, kv_heads, head_dim, scale, num_sms
-        c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,  # workspace, floats, counters, number, status, stream
+        c_void_p, c_int64, c_void_p, c_void_p,  # workspace, floats, status, stream
     ],
     "cdb_sample_tokens": [
         c_void_p, c_int, c_int64, c_int, c_int,  # logits, logits_fp32, stride, num_rows, vocab
@@ -199,7 +198,7 @@ _SIGNATURES: dict[str, list] = {
     ],
 }
 _RESTYPES = {"cdb_status_string": ctypes.c_char_p, "cdb_kv8_decode_workspace_floats": c_int64,
-             "cdb_prefix_decode_workspace_floats": c_int64, "cdb_prefix_decode_counters": c_int64,
+             "cdb_prefix_decode_workspace_floats": c_int64,
              "cdb_attn_scratch_bytes": c_int64, "cdb_gemm_workspace_elems": c_int64,
               "cdb_gemm_counter_elems": c_int}
 
@@ -277,7 +276,7 @@ def stream_ptr(stream: torch.cuda.Stream | None = None) -> int:
 _NO_LAUNCH = {
     "cdb_version", "cdb_status_string", "cdb_attn_scratch_bytes", "cdb_gemm_workspace_elems", "cdb_gemm_counter_elems",
     "cdb_gemm_partial_splits", "cdb_kv8_decode_workspace_floats", "cdb_kv8_decode_counters",
-    "cdb_prefix_decode_workspace_floats", "cdb_prefix_decode_counters",
+    "cdb_prefix_decode_workspace_floats",
     "cdb_schedule_queues_init",
     "cdb_kv_blocks_host_copy",
 }

@@ -37,6 +37,7 @@
 // with weight zero would spread, is taken out in the steps that the diagonal crosses and put back at the end
 // for the rows that see it.
 #include "kv8.cuh"
+#include "tcgen05.cuh"
 
 namespace cdb {
 namespace kv8 {
@@ -116,88 +117,6 @@ __device__ __forceinline__ void async_copy4(uint32_t dst, const void* src) {
 __device__ __forceinline__ void async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
-
-// Matrix descriptor of a K-major operand in 128-byte swizzled rows of 64 f16, 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t operand(uint32_t addr) {
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-
-// D[tmem] (+)= A B^T, kind::f16 with f16 operands: fp32 accumulators, M = 128.
-__device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
-  const uint32_t none = 0, acc = add;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
-      "l"(operand(a)), "l"(operand(b)), "r"(idesc), "r"(acc), "r"(none)
-      : "memory");
-}
-// The same with A in tensor memory: two f16 to a 32-bit column, rows on lanes.
-__device__ __forceinline__ void product_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
-  const uint32_t none = 0, acc = add;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(operand(b)), "r"(idesc), "r"(acc), "r"(none)
-      : "memory");
-}
-__device__ __forceinline__ void commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// 32 columns of this warp's 32 tensor-memory lanes.
-__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(addr));
-}
-// 16 columns, there and back: the rescaling of O goes through few registers, beside the 64 of S.
-__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(addr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]),
-               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr)
-               : "memory");
-}
-
-// Waits for this thread's tensor-memory loads; the registers pass through it, so no use can move ahead.
-__device__ __forceinline__ void wait_loads(uint32_t* r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-               "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
-               "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-               "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-               :
-               : "memory");
-}
-__device__ __forceinline__ void wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Bounded wait that also gives up once another role has.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int32_t* status, volatile int* abort) {
@@ -391,8 +310,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
             fence_after();
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk)
-              product(tmem + (n & 1) * TK, base + T::OFF_Q + (kk >> 2) * (TM * 128) + (kk & 3) * 32,
-                      base + T::OFF_K + (kk >> 2) * (TK * 128) + (kk & 3) * 32, kIdescS, kk > 0);
+              product(tmem + (n & 1) * TK, operand(base + T::OFF_Q + (kk >> 2) * (TM * 128) + (kk & 3) * 32),
+                      operand(base + T::OFF_K + (kk >> 2) * (TK * 128) + (kk & 3) * 32), kIdescS, kk > 0);
             commit(&sh.sfull[n & 1]);
             mbar_arrive(&sh.sfull[n & 1]);  // releases the scales to whoever waits for S
           }
@@ -406,8 +325,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2) prefill_kernel(const Prefi
           fence_after();
 #pragma unroll
           for (int kk = 0; kk < TK / 16; ++kk)
-            product_tmem(tmem_o, tmem + (j & 1) * TK + kk * 8, base + T::OFF_V + (j & 1) * (D * 128) + kk * 32, kIdescO,
-                         j > 0 || kk > 0);
+            product_tmem(tmem_o, tmem + (j & 1) * TK + kk * 8, operand(base + T::OFF_V + (j & 1) * (D * 128) + kk * 32),
+                         kIdescO, j > 0 || kk > 0);
           commit(&sh.odone[j & 1]);
         }
       }

@@ -442,17 +442,16 @@ void prefix_decode_attention(const Tensor& q, const Tensor& out, const Tensor& k
   const auto stream = c10::cuda::getCurrentCUDAStream(dev.index());
   const int sms = sm_count(dev);
   const Tensor& status = status_word(dev);
-  const auto [ws, counters] = workspace(
-      kPrefixDecode, dev, stream,
-      cdb_prefix_decode_workspace_floats((int)n, (int)groups, (int)num_heads, c.heads, c.dim, sms),
-      cdb_prefix_decode_counters((int)n, (int)num_heads, c.heads));
+  const Tensor ws =
+      workspace(kPrefixDecode, dev, stream,
+                cdb_prefix_decode_workspace_floats((int)n, (int)groups, (int)num_heads, c.heads, c.dim, sms), 0)
+          .first;
   check(cdb_prefix_decode_attention(
             ptr<void>(q), q.stride(0), ptr<void>(out), out.stride(0), ptr<void>(kv_pool), c.layers, c.rows,
             (int)cache_layer, ptr<int32_t>(block_table), block_table.stride(0), (int)block_table.size(0),
             (int)block_table.size(1), ptr<int32_t>(item_slot), ptr<int32_t>(item_pos), (int)n,
             ptr<int32_t>(group_start), ptr<int32_t>(prefix_len), (int)groups, (int)num_heads, c.heads, c.dim,
-            (float)scale, sms, ptr<float>(ws), ws.numel(), ptr<int32_t>(counters), counters.numel(),
-            ptr<int32_t>(status), stream.stream()),
+            (float)scale, sms, ptr<float>(ws), ws.numel(), ptr<int32_t>(status), stream.stream()),
         "cdb_prefix_decode_attention");
 }
 

@@ -607,10 +607,9 @@ int cdb_qk_norm_rope_append(const void* qkv, int64_t qkv_stride, void* q_out, in
                             const void* rope_cos, const void* rope_sin, int rope_rows, float eps, int num_items,
                             int num_heads, int num_kv_heads, int head_dim, int32_t* status, void* stream);
 
-/* fp32 elements of cdb_prefix_decode_attention's workspace, and its int32 counters. */
+/* fp32 elements of cdb_prefix_decode_attention's workspace. */
 int64_t cdb_prefix_decode_workspace_floats(int num_items, int num_groups, int num_heads, int num_kv_heads,
                                            int head_dim, int num_sms);
-int64_t cdb_prefix_decode_counters(int num_items, int num_heads, int num_kv_heads);
 
 /* Decode attention: row i attends to positions 0 .. item_pos[i] of slot item_slot[i]; a row with
  * item_pos < 0 is skipped and its out row left as it was. Rows of a group share their first blocks, which
@@ -622,16 +621,16 @@ int64_t cdb_prefix_decode_counters(int num_items, int num_heads, int num_kv_head
  *                rows are the same blocks for every row of the group with item_pos >= 0. Blocks that some such row
  *                does not see whole are not shared. num_groups 0: every row stands alone.
  *                Group bounds that descend or leave [0, num_items] set CDB_ERR_INDEX, and no blocks are shared.
- *   workspace    cdb_prefix_decode_workspace_floats elements, 16-byte aligned; counters:
- *                cdb_prefix_decode_counters, zeroed before the first use, left zeroed. Calls that share
- *                them must be ordered. scale > 0. */
+ *   workspace    cdb_prefix_decode_workspace_floats elements, 16-byte aligned, in any state. Calls that share it
+ *                must be ordered. scale > 0.
+ * CDB_ERR_UNSUPPORTED above 2^30 - 17 cache rows or 2^30 - 1 (row, head)s. */
 int cdb_prefix_decode_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* kv_base,
                                 int num_cache_layers, int64_t kv_rows, int cache_layer, const int32_t* block_table,
                                 int64_t block_table_stride, int table_rows, int table_width, const int32_t* item_slot,
                                 const int32_t* item_pos, int num_items, const int32_t* group_start,
                                 const int32_t* prefix_len, int num_groups, int num_heads, int num_kv_heads,
                                 int head_dim, float scale, int num_sms, float* workspace, int64_t workspace_floats,
-                                int32_t* counters, int64_t num_counters, int32_t* status, void* stream);
+                                int32_t* status, void* stream);
 
 /* The next token of every row of logits [num_rows][vocab] (bf16, or fp32 where logits_fp32; rows at
  * logits_stride elements, aligned to their type) from one given random number a row.
