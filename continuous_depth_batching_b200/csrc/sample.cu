@@ -10,12 +10,14 @@
 // whole numbers: exact, the same in any order, and comparable with a border that lies next to them. 32-bit sums
 // would move the borders by 2^-24 of the total, which is the weight of whole tokens in a wide row.
 //
-// A CTA takes a row and reads it up to four times, the first from memory and the others from L2:
-//   1. its largest and least logit;
-//   2. (top-k, top-p; bf16 always) how many tokens each of 8192 bins has: the upper 16 bits of the logit's 32, so
-//      for bf16 a bin holds one value, over the 32 octaves below the row's largest magnitude, either sign;
-//   3. the kept weights of every warp's stretch of the row. bf16 looks a bin's weight up. fp32 computes it, and where
-//      the border falls into a bin, its neighbourhood's tokens are collected, sorted and summed exactly;
+// A CTA takes a row and reads it a few times, the first from memory and the others from L2:
+//   1. its largest and least logit, and every thread's largest;
+//   2. with top-k of up to half the threads: the tokens at or above the k-th largest of the threads' largest, a few more
+//      than k of them, which are sorted; the rest is done on them;
+//   2. with top-p, or more of top-k: how many tokens each of 8192 bins has: the upper 16 bits of the logit's 32, so for
+//      bf16 a bin holds one value, over the 32 octaves below the row's largest magnitude, either sign;
+//   3. the kept weights of every warp's stretch of the row. Behind bins bf16 looks a bin's weight up; fp32 computes it, and
+//      where the border falls into a bin, its neighbourhood's tokens are collected, sorted and summed exactly;
 //   4. the stretch in which the target lies, a few tokens to a thread.
 // Rows that this does not fit (an infinite largest logit, bf16 logits over more than 32 octaves, a border among more
 // fp32 tokens than the list holds) take `slow_row`, which finds its borders by bisection, a bit of the key a pass.
@@ -24,14 +26,13 @@
 namespace cdb {
 namespace sample {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
+constexpr int kMaxWarps = 32;
 constexpr int kHalf = 4096;              // bins of one sign: 32 octaves of 128
 constexpr int kBins = 2 * kHalf + 1;     // largest logits first; bin kHalf holds 0
-constexpr int kPerThread = (kBins + kThreads - 1) / kThreads;
-constexpr int kBinsPadded = kPerThread * kThreads;
+template <int kThreads>
+constexpr int kPadded = (kBins + kThreads) / kThreads * kThreads;  // and room for kNone
 constexpr int kList = 8192;              // fp32 tokens next to a border
-constexpr int kNone = kBinsPadded;       // no bin: weighs nothing
+constexpr int kNone = kBins;             // no bin: weighs nothing
 constexpr uint32_t kAll = 0xffffffffu;
 typedef unsigned long long u64;
 
@@ -59,8 +60,6 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float logit_of(uint32_t key) {
   return __uint_as_float(key ^ (key & 0x80000000u ? 0x80000000u : 0xffffffffu));
 }
-constexpr uint32_t kMinusInf = 0x007fffffu;  // key_of(-inf)
-constexpr uint32_t kPlusInf = 0xff800000u;
 
 template <typename T>
 __device__ __forceinline__ float load_one(const void* row, int i) {
@@ -84,6 +83,28 @@ struct Row {
     shift = (int)((reinterpret_cast<uintptr_t>(at) & 15) / sizeof(T));
     vectors = (vocab + shift + N - 1) / N;
   }
+  // Largest and least of a vector.
+  __device__ __forceinline__ void range(int j, float& top, float& least) const {
+    const int i = j * N - shift;
+    if (N == 8 && i >= 0 && i + N <= vocab) {  // two at a time
+      const uint4 w = *reinterpret_cast<const uint4*>(at + i);
+      const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(&w);
+      const __nv_bfloat162 a = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+      const __nv_bfloat162 b = __hmin2(__hmin2(v[0], v[1]), __hmin2(v[2], v[3]));
+      top = fmaxf(top, fmaxf(__low2float(a), __high2float(a)));
+      least = fminf(least, fminf(__low2float(b), __high2float(b)));
+      return;
+    }
+    float x[N];
+    load(j, x);
+#pragma unroll
+    for (int k = 0; k < N; ++k) top = fmaxf(top, x[k]), least = fminf(least, x[k]);
+  }
+  __device__ __forceinline__ bool reaches(int j, float from) const {
+    float top = -INFINITY, least = INFINITY;
+    range(j, top, least);
+    return top >= from;
+  }
   // Tokens outside the row come as NaN, which weighs nothing.
   __device__ __forceinline__ void load(int j, float (&x)[N]) const {
     const int i = j * N - shift;
@@ -105,13 +126,14 @@ struct Row {
 // ---------------------------------------------------------------------------------- sums over the CTA
 
 struct Scratch {
-  u64 sum[kWarps];
-  u64 sum2[kWarps];
-  int found;
+  u64 sum[kMaxWarps];
+  u64 sum2[kMaxWarps];
 };
 
 // Sum of the threads before this one, and of all.
+template <int kThreads>
 __device__ __forceinline__ u64 scan(u64 mine, u64& all, u64* red) {
+  constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   u64 x = mine;
 #pragma unroll
@@ -122,34 +144,70 @@ __device__ __forceinline__ u64 scan(u64 mine, u64& all, u64* red) {
   __syncthreads();
   if (lane == 31) red[warp] = x;
   __syncthreads();
-  u64 before = x - mine;
-  all = 0;
+  u64 w = lane < kWarps ? red[lane] : 0;
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    if (i < warp) before += red[i];
-    all += red[i];
+  for (int o = 1; o < kWarps; o <<= 1) {
+    const u64 y = __shfl_up_sync(kAll, w, o);
+    if (lane >= o) w += y;
   }
-  return before;
+  all = __shfl_sync(kAll, w, kWarps - 1);
+  const u64 before = __shfl_sync(kAll, w, (warp + 31) & 31);
+  return (warp ? before : 0) + x - mine;
 }
+template <int kThreads>
 __device__ __forceinline__ u64 block_sum(u64 v, u64* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  u64 t = 0;
+  const int lane = threadIdx.x & 31;
+  u64 t = lane < kThreads / 32 ? red[lane] : 0;
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) t += red[i];
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(kAll, t, o);
   return t;
 }
 
 // The product of a share in [0, 1] and a sum, rounded down (a running sum passes it where it passes the product) or up
-// (one is below it where it is below the product). NaN: 0.
+// (one is below it where it is below the product). NaN: 0. In whole numbers: 64-bit floating point takes longer here.
 __device__ __forceinline__ u64 share_of(float share, u64 sum, bool up = false) {
-  const double s = fmin(fmax((double)share, 0.), 1.);
-  const u64 m = (u64)(s * 9007199254740992.);  // 2^53 s, whole
-  const u64 low = m * sum;
-  return ((__umul64hi(m, sum) << 11) | (low >> 53)) + (up && (low & ((1ull << 53) - 1)) != 0);
+  if (!(share > 0.f)) return 0;
+  if (share >= 1.f) return sum;
+  const uint32_t b = __float_as_uint(share);
+  const u64 m = (b & 0x7fffffu) | (b >> 23 ? 0x800000u : 0u);
+  const int s = 150 - max((int)(b >> 23), 1);  // share = m 2^-s, s > 23
+  const u64 high = __umul64hi(m, sum), low = m * sum;
+  u64 whole, cut;
+  if (s < 64) whole = (high << (64 - s)) | (low >> s), cut = low << (64 - s);
+  else whole = s < 128 ? high >> (s - 64) : 0, cut = low | (s < 128 ? s > 64 ? high << (128 - s) : 0 : high);
+  return whole + (up && cut != 0);
+}
+
+// Sum of the lanes before this one.
+__device__ __forceinline__ u64 lane_scan(u64 mine) {
+  const int lane = threadIdx.x & 31;
+  u64 x = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 y = __shfl_up_sync(kAll, x, o);
+    if (lane >= o) x += y;
+  }
+  return x - mine;
+}
+// Of stretches, one to a lane, the one in which the target lies.
+struct Stretch {
+  int at;
+  u64 before, all, target;
+};
+__device__ __forceinline__ Stretch stretch_of(u64 mine, float share) {
+  const u64 before = lane_scan(mine);
+  Stretch s;
+  s.all = __shfl_sync(kAll, before + mine, 31);
+  s.target = share_of(share, s.all);
+  if (s.target >= s.all) s.target = s.all - 1;
+  s.at = __ffs(__ballot_sync(kAll, before <= s.target && s.target < before + mine)) - 1;
+  s.before = __shfl_sync(kAll, before, s.at);
+  return s;
 }
 
 // ---------------------------------------------------------------------------------- weights
@@ -165,33 +223,88 @@ struct Weigher {
 };
 
 // The same to 2^-30 of each weight from 32-bit operations, for every token of a row. With y = (top - l) log2(e) / t as a
-// sum of two floats: 2^-y = 2^-n 2^-(j / 256) 2^-r, the second from a table, the third from its series, |r| <= 2^-9.
+// sum of two floats: 2^-y = 2^-n 2^-(j / 1024) 2^-r, the second from a table, the third from its series, |r| <= 2^-11.
+constexpr int kTable = 1024;
+struct Powers {
+  uint2 at[kTable];
+};
+// 2^-(j / 1024) by products of 2^-(1 / 1024) in 64 bits: off by 2^-43 at most.
+constexpr uint32_t float_bits(uint32_t whole) {  // of a whole number in [2^30, 2^31], rounded down
+  return whole >= 0x80000000u ? 0x4f000000u : (0x4e800000u + ((whole - 0x40000000u) >> 7));
+}
+constexpr Powers powers() {
+  Powers p{};
+  double x = 2147483648.;
+  for (int j = 0; j < kTable; ++j, x *= 0.99932332750265075) {
+    p.at[j].x = (uint32_t)(x + 0.5);
+    p.at[j].y = float_bits(p.at[j].x);
+  }
+  return p;
+}
+__device__ const Powers g_powers = powers();
+template <typename T>
 struct FastWeigher {
   float top, c, c_low;  // log2(e) / t in two floats
-  int bits;             // S - 31
-  const uint2* table;   // {2^31 2^-(j / 256) whole, as a float}
+  int down;             // 63 - S
+  const uint2* table;   // {2^31 2^-(j / 1024) whole, as a float}
   __device__ __forceinline__ u64 operator()(float l) const {
     const float d = top - l;
-    // what the subtraction rounded away
-    const float back = d - top;
-    const float low = (top - (d - back)) - (l + back);
-    const float y = __fmul_rn(d, c);
-    if (!(y < 62.f)) return d == 0.f ? 1ull << (bits + 31) : 0ull;  // (also NaN: 0 / a tiny temperature, -inf)
-    const float e = fmaf(low, c, fmaf(d, c_low, fmaf(d, c, -y)));
-    const float round = y + 49152.f;  // to whole 1 / 256
-    const int step = __float_as_int(round) - __float_as_int(49152.f);
-    const float r = ((y - (round - 49152.f)) + e) * 0.693147180559945f;
-    const float q = r * fmaf(r, fmaf(r, 0.16666667f, -0.5f), 1.f);  // 1 - 2^-r
-    const uint2 t = table[step & 255];
+    const float y = fminf(__fmul_rn(d, c), 63.f);  // (NaN comes as 63 too, and 2^-63 as 0 below)
+    float e = fmaf(d, c_low, fmaf(d, c, -y));
+    if constexpr (sizeof(T) == 4) {  // what the subtraction rounded away
+      const float back = d - top;
+      e = fmaf((top - (d - back)) - (l + back), c, e);
+    }
+    const float round = y + 12288.f;  // to whole 1 / 1024
+    const int step = __float_as_int(round) - __float_as_int(12288.f);
+    const float r = (y - (round - 12288.f)) + e;
+    const float q = r * fmaf(r, -0.240226507f, 0.693147181f);  // 1 - 2^-r
+    const uint2 t = table[step & (kTable - 1)];
     const float less = fmaf(__uint_as_float(t.y), q, 12582912.f);  // + 1.5 * 2^23: its low bits are the whole number
     const uint32_t m = t.x - (uint32_t)(__float_as_int(less) - __float_as_int(12582912.f));
-    return ((u64)m << bits) >> (step >> 8);
+    u64 w;
+    asm("shr.u64 %0, %1, %2;" : "=l"(w) : "l"((u64)m << 32), "r"(down + (step >> 10)));
+    return w;
   }
 };
 
+// Sorts `size` (a power of two, at least 64) numbers, largest first; only zeros may stand more than once. Few of them
+// by counting for each the larger ones, 4 threads or more to each (64: 0.3 us, where the steps below take 3).
+template <int kThreads>
+__device__ __forceinline__ void sort(u64* list, int size) {
+  if (size * 4 <= kThreads) {
+    const int parts = min(32, kThreads / size), at = threadIdx.x / parts, part = threadIdx.x % parts;
+    const u64 mine = at < size ? list[at] : 0;
+    int larger = 0;
+    if (at < size)
+      for (int i = part; i < size; i += parts) larger += list[i] > mine;
+    for (int o = parts / 2; o > 0; o >>= 1) larger += __shfl_xor_sync(kAll, larger, o);
+    __syncthreads();
+    if (at < size && part == 0 && mine != 0) list[larger] = mine;
+    __syncthreads();
+    // zeros: behind the others, where some of those may have stood
+    if (at < size && part == 0 && mine == 0) larger = -1;
+    const int zeros = __syncthreads_count(at < size && part == 0 && larger == -1);
+    if ((int)threadIdx.x < zeros) list[size - 1 - threadIdx.x] = 0;
+    __syncthreads();
+    return;
+  }
+  for (int run = 2; run <= size; run <<= 1)
+    for (int step = run >> 1; step > 0; step >>= 1) {
+      for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+        const int a = 2 * i - (i & (step - 1)), b = a + step;
+        const u64 x = list[a], y = list[b];
+        if ((x < y) == ((a & run) == 0)) list[a] = y, list[b] = x;
+      }
+      // a warp's pairs stay within 64 places below that distance
+      if (step > 32 || (step == 1 && run >= 64)) __syncthreads();
+      else __syncwarp();
+    }
+}
+
 // ---------------------------------------------------------------------------------- any row, slowly
 
-template <typename T>
+template <typename T, int kThreads>
 __device__ __noinline__ void slow_row(const Params& p, int r, uint32_t top, float t, Scratch& sc) {
   const int tid = threadIdx.x, v = p.vocab;
   const void* row = static_cast<const T*>(p.logits) + (int64_t)r * p.stride;
@@ -210,7 +323,7 @@ __device__ __noinline__ void slow_row(const Params& p, int r, uint32_t top, floa
       const uint32_t probe = edge | (1u << bit);
       u64 n = 0;
       for (int i = tid; i < v; i += kThreads) n += load_key<T>(row, i) >= probe;
-      n = block_sum(n, sc.sum);
+      n = block_sum<kThreads>(n, sc.sum);
       if (n >= (u64)k) edge = probe;
       else above = n;
     }
@@ -224,7 +337,7 @@ __device__ __noinline__ void slow_row(const Params& p, int r, uint32_t top, floa
       const uint32_t key = load_key<T>(row, i);
       if (key > edge) total += weigh(logit_of(key));
     }
-    total = block_sum(total, sc.sum) + at_edge;
+    total = block_sum<kThreads>(total, sc.sum) + at_edge;
     const u64 want = share_of(tp, total, true);
     uint32_t e = 0;
     u64 above = 0;
@@ -235,7 +348,7 @@ __device__ __noinline__ void slow_row(const Params& p, int r, uint32_t top, floa
         const uint32_t key = load_key<T>(row, i);
         if (key >= probe && key > edge) n += weigh(logit_of(key));
       }
-      n = block_sum(n, sc.sum);
+      n = block_sum<kThreads>(n, sc.sum);
       if (probe <= edge) n += at_edge;
       if (n >= want && n > 0) e = probe;
       else above = n;
@@ -255,7 +368,7 @@ __device__ __noinline__ void slow_row(const Params& p, int r, uint32_t top, floa
   const int lo = min(v, tid * per), hi = min(v, lo + per);
   u64 n = 0, all;
   for (int i = lo; i < hi; ++i) n += load_key<T>(row, i) == edge;
-  const u64 ties_before = scan(n, all, sc.sum);
+  const u64 ties_before = scan<kThreads>(n, all, sc.sum);
   auto walk = [&](auto f) {
     u64 seen = ties_before;
     for (int i = lo; i < hi; ++i) {
@@ -267,7 +380,7 @@ __device__ __noinline__ void slow_row(const Params& p, int r, uint32_t top, floa
   };
   u64 mine = 0;
   walk([&](int, u64 w) { mine += w; });
-  u64 run = scan(mine, all, sc.sum);
+  u64 run = scan<kThreads>(mine, all, sc.sum);
   u64 want = share_of(p.uniform[r], all);
   if (want >= all) want = all - 1;
   if (run <= want && want < run + mine) {
@@ -284,14 +397,13 @@ __device__ __noinline__ void slow_row(const Params& p, int r, uint32_t top, floa
 
 // ---------------------------------------------------------------------------------- bins
 
-// `low`: (least biased exponent of the bins' 32 octaves) * 128, at least 0.
-// Logits of smaller magnitude share 0's bin (bf16 rows that have such go the slow way), larger ones have none.
+// `low`: (least biased exponent of the bins' 32 octaves) * 128, at least 128.
+// Logits of smaller magnitude share 0's bin (bf16 rows that have such go the slow way); larger ones, infinities and NaN have
+// none.
 __device__ __forceinline__ int bin_of(float x, int low) {
-  const uint32_t b = __float_as_uint(x);
-  const int mag = (int)((b >> 16) & 0x7fffu);
-  const int off = max(mag - low + 1, 0) * (mag != 0);
-  const int bin = (int32_t)b < 0 ? kHalf + off : kHalf - off;
-  return x == x && off <= kHalf ? bin : kNone;
+  const int b = __float_as_int(x);
+  const int off = max(((b >> 16) & 0x7fff) - (low - 1), 0);
+  return off <= kHalf ? (b < 0 ? kHalf + off : kHalf - off) : kNone;
 }
 // The least magnitude of a bin's logits, signed.
 __device__ __forceinline__ float logit_of_bin(int bin, int low) {
@@ -303,60 +415,55 @@ __device__ __forceinline__ float logit_of_bin(int bin, int low) {
 
 struct Shared {
   Scratch sc;
-  uint32_t red[2 * kWarps];
-  uint2 table[256];
+  uint32_t red[2 * kMaxWarps];
   int edge_bin, edge_count;  // the border: of that bin's tokens the first few are kept
-  int lo_bin, hi_bin;        // fp32: the bins whose tokens are collected
+  int lo_bin, hi_bin;        // the bins whose tokens are collected
   int list_n, list_over;
   int k_border;              // fp32: top-k ends among the binned tokens
   u64 edge;                  // fp32: the last token kept, as the list has it
-  u64 above;
+  u64 edge_w;                // bf16: the weight of the border's bin
+  double inv_t, unit;        // 1 / t and 2^-S
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const Params p) {
   constexpr bool WIDE = sizeof(T) == 4;
-  constexpr int N = Row<T>::N;
+  constexpr int N = Row<T>::N, kWarps = kThreads / 32, kBinsPadded = kPadded<kThreads>, kPerThread = kBinsPadded / kThreads;
   pdl_trigger();
   extern __shared__ __align__(16) uint8_t smem[];
-  uint32_t* counts = reinterpret_cast<uint32_t*>(smem);                        // [kBinsPadded + 1]
-  u64* weights = reinterpret_cast<u64*>(smem + (kBinsPadded + 4) * 4);         // bf16: [kBinsPadded + 1]
-  u64* list = weights;                                                         // fp32: [kList] {key, ~index}
+  uint32_t* counts = reinterpret_cast<uint32_t*>(smem);                 // [kBinsPadded + 4]
+  u64* weights = reinterpret_cast<u64*>(smem + (kBinsPadded + 4) * 4);  // [kBinsPadded + 1]
+  u64* list = weights;                                                  // or [kList] {key, ~index}
+  uint2* table = reinterpret_cast<uint2*>(smem + (kBinsPadded + 4) * 4 + (kBinsPadded + 2) * 8);  // [kTable]
   __shared__ Shared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.x;
   for (int i = tid; i < (kBinsPadded + 4) / 4; i += kThreads) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
-  if (WIDE && tid < 256) {
-    const double x = 2147483648. * exp2(-(double)tid / 256.);
-    sh.table[tid] = make_uint2((uint32_t)__double2ll_rn(x), __float_as_uint((float)x));
-  }
+  for (int i = tid; i < kTable; i += kThreads) table[i] = g_powers.at[i];
+  if (tid == 0) sh.unit = 1. / (double)(1ull << p.scale_bits);
+  if (tid == 0) sh.edge_bin = kNone, sh.edge_count = 0, sh.lo_bin = kBinsPadded, sh.hi_bin = -1, sh.list_n = 0, sh.list_over = 0, sh.k_border = 0;
   pdl_wait();
   const Row<T> row(p, r);
   const float t = p.temperature[r];
   const bool greedy = !(t > 0.f);
+  if (tid == 0) sh.inv_t = 1. / (double)t;
 
-  // ---- the largest logit, and the least above -inf
-  uint32_t top = 0, least = kAll;
-#pragma unroll 4
-  for (int j = tid; j < row.vectors; j += kThreads) {
-    float x[N];
-    row.load(j, x);
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const uint32_t key = key_of(x[k]);
-      top = max(top, key);
-      if (key > kMinusInf) least = min(least, key);
-    }
+  // ---- the largest logit, and the least
+  float top = -INFINITY, least = INFINITY;  // (maxima and minima leave NaN out)
+#pragma unroll 8
+  for (int j = tid; j < row.vectors; j += kThreads) row.range(j, top, least);
+  const float my_top = top;
+  {
+    uint32_t a = key_of(top), b = key_of(least);
+    a = __reduce_max_sync(kAll, a);
+    b = __reduce_min_sync(kAll, b);
+    if (lane == 0) sh.red[warp] = a, sh.red[kWarps + warp] = b;
+    __syncthreads();
+    a = __reduce_max_sync(kAll, sh.red[lane % kWarps]);
+    b = __reduce_min_sync(kAll, sh.red[kWarps + lane % kWarps]);
+    top = logit_of(a);
+    least = logit_of(b);
   }
-  top = __reduce_max_sync(kAll, top);
-  least = __reduce_min_sync(kAll, least);
-  if (lane == 0) sh.red[warp] = top, sh.red[kWarps + warp] = least;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    top = max(top, sh.red[i]);
-    least = min(least, sh.red[kWarps + i]);
-  }
-  if (top <= kMinusInf) {
+  if (top == -INFINITY) {
     if (tid == 0) {
       p.ids[r] = -1;
       if (p.logp) p.logp[r] = NAN;
@@ -365,12 +472,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   }
   if (greedy) {
     int first = INT32_MAX;
-    for (int j = tid; j < row.vectors; j += kThreads) {
+    for (int j = tid; j < row.vectors && my_top == top; j += kThreads) {
       float x[N];
       row.load(j, x);
 #pragma unroll
       for (int k = N - 1; k >= 0; --k)
-        if (key_of(x[k]) == top) first = min(first, j * N - row.shift + k);
+        if (x[k] == top) first = min(first, j * N - row.shift + k);
     }
     first = __reduce_min_sync(kAll, first);
     __syncthreads();
@@ -384,27 +491,117 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
     }
     return;
   }
-  if (top == kPlusInf) {
-    slow_row<T>(p, r, top, t, sh.sc);
-    return;
-  }
   const int k = p.top_k ? p.top_k[r] : 0;
   const float tp = p.top_p ? p.top_p[r] : 1.f, mp = p.min_p ? p.min_p[r] : 0.f;
   const bool by_k = k > 0 && k < p.vocab, by_p = tp < 1.f, by_m = mp > 0.f;
-  Weigher weigh;
-  weigh.top = (double)logit_of(top);
-  weigh.inv = 1. / (double)t;
-  weigh.one = (double)(1ull << p.scale_bits);
+  const u64 least_w = by_m ? share_of(mp, 1ull << p.scale_bits, true) : 0;
+  FastWeigher<T> weigh;
+  {
+    constexpr float kLog2e = 1.44269502f, kRest = 1.92596299e-8f;  // their sum is log2(e)
+    weigh.top = top;
+    weigh.c = kLog2e / t;
+    weigh.c_low = isinf(t) ? 0.f : (fmaf(-weigh.c, t, kLog2e) + kRest) / t;
+    weigh.down = 63 - p.scale_bits;
+    weigh.table = table;
+  }
+  if (isinf(top) || isinf(weigh.c)) {
+    slow_row<T, kThreads>(p, r, key_of(top), t, sh.sc);
+    return;
+  }
+  // the log-probability of a token among kept weights that add up to `all`
+  auto log_share = [&](float l, u64 all) {
+    return (float)(((double)l - (double)top) * sh.inv_t - log((double)all * sh.unit));
+  };
   // below this no weight is left
-  const double cutoff = weigh.top - (double)t * 0.6931471805599453 * (p.scale_bits + 2);
-  const float lowest = fmaxf(logit_of(least), (float)fmax(cutoff, -3.4e38));
-  const float widest = fmaxf(fabsf(logit_of(top)), fabsf(lowest));
-  const int low = max((int)(__float_as_uint(widest) >> 23) - 31, 0) * 128;
-  const bool bins = !WIDE || by_k || by_p;
+  const float cutoff = fmaxf(top - t * (0.694f * (float)(p.scale_bits + 2)) - 1e-6f * fabsf(top), -3.4e38f);
+  const float widest = fmaxf(fabsf(top), fabsf(fmaxf(least, cutoff)));
+  const int low = max((int)(__float_as_uint(widest) >> 23) - 31, 1) * 128;
+
+  // ---- top-k of a few
+  if (by_k && k <= kThreads / 2) {
+    // The bin of the k-th largest of the threads' largest: at least k tokens are in it or above. Where fewer threads
+    // have any, or theirs weigh nothing, there is none, and every token that weighs is taken.
+    const int my_bin = bin_of(my_top, low);
+    if (my_bin != kNone) atomicAdd(&counts[my_bin], 1u);
+    __syncthreads();
+    const int b0 = tid * kPerThread;
+    u64 mine = 0, all;
+#pragma unroll 3
+    for (int i = 0; i < kPerThread; ++i) mine += counts[b0 + i];
+    u64 before = scan<kThreads>(mine, all, sh.sc.sum);
+#pragma unroll 3
+    for (int i = 0; i < kPerThread; ++i) {
+      if (before < (u64)k && before + counts[b0 + i] >= (u64)k) sh.hi_bin = b0 + i;
+      before += counts[b0 + i];
+    }
+    __syncthreads();
+    // the least logit of that bin (of a negative or zero's, one that is less)
+    const int hi = sh.hi_bin;
+    const float from = hi < 0 ? fmaxf(least, cutoff) : logit_of_bin(hi < kHalf ? hi : hi + 1, low);
+#pragma unroll 4
+    for (int j = tid; j < row.vectors; j += kThreads) {
+      if (!row.reaches(j, from)) continue;
+      float x[N];
+      row.load(j, x);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (x[i] >= from) {
+          const int at = atomicAdd(&sh.list_n, 1);
+          if (at < kList) list[at] = (u64)key_of(x[i]) << 32 | (uint32_t)~(j * N - row.shift + i);
+        }
+    }
+    if (my_bin != kNone) counts[my_bin] = 0;  // (only that bin's threads, and for whoever comes next)
+    __syncthreads();
+    const int n = sh.list_n;
+    if (n <= kList) {
+      int size = 64;
+      while (size < n) size <<= 1;
+      for (int i = n + tid; i < size; i += kThreads) list[i] = 0;
+      __syncthreads();
+      sort<kThreads>(list, size);
+      // at most one of the first k to a thread: weights fall along the threads, so what is kept is a beginning of them
+      const int m = min(n, k);
+      const u64 w = tid < m ? weigh(logit_of((uint32_t)(list[tid] >> 32))) : 0;
+      u64 all_w;
+      const u64 before_w = scan<kThreads>(w, all_w, sh.sc.sum);
+      const u64 want = by_p ? share_of(tp, all_w, true) : ~0ull;
+      const bool keep = tid < m && (tid == 0 || (before_w < want && w >= least_w));
+      const int kept = __syncthreads_count(keep);
+      // in index order
+      u64* order = reinterpret_cast<u64*>(counts);  // {~index, place}
+      int size2 = 64;
+      while (size2 < kept) size2 <<= 1;
+      if (tid < size2) order[tid] = tid < kept ? (u64)(uint32_t)list[tid] << 32 | (uint32_t)tid : 0;
+      __syncthreads();
+      sort<kThreads>(order, size2);
+      const bool mine_kept = tid < kept;
+      const u64 at = mine_kept ? list[(uint32_t)order[tid]] : 0;
+      const float l = logit_of((uint32_t)(at >> 32));
+      const u64 w2 = mine_kept ? weigh(l) : 0;
+      u64 all2;
+      const u64 run = scan<kThreads>(w2, all2, sh.sc.sum);
+      u64 target = share_of(p.uniform[r], all2);
+      if (target >= all2) target = all2 - 1;
+      if (mine_kept && run <= target && target < run + w2) {
+        p.ids[r] = (int)~(uint32_t)at;
+        if (p.logp) p.logp[r] = log_share(l, all2);
+      }
+      return;
+    }
+    if (tid == 0) sh.hi_bin = -1, sh.list_n = 0;
+    __syncthreads();
+  }
 
   // ---- bins
+  const bool bins = by_k || by_p;
   if (bins) {
     bool strange = false;
+    // fp32: the mean logit of the bins whose tokens weigh e^-6 or more, of which few may make up the total
+    const int heavy = WIDE && by_p ? bin_of(top - 6.f * t, low) : -1;
+    if (WIDE && by_p) {
+      for (int i = tid; i < kBinsPadded; i += kThreads) weights[i] = 0;
+      __syncthreads();
+    }
 #pragma unroll 2
     for (int j = tid; j < row.vectors; j += kThreads) {
       float x[N];
@@ -414,85 +611,106 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
         const int bin = bin_of(x[i], low);
         if (!WIDE) strange |= bin == kHalf && x[i] != 0.f;
         if (bin != kNone) atomicAdd(&counts[bin], 1u);
+        if (WIDE && bin <= heavy && bin != kNone)
+          atomicAdd(reinterpret_cast<uint32_t*>(&weights[bin]), __float_as_uint(x[i]) & 0xffffu);
       }
     }
     if (__syncthreads_or(strange)) {
-      slow_row<T>(p, r, top, t, sh.sc);
+      slow_row<T, kThreads>(p, r, key_of(top), t, sh.sc);
       return;
     }
-    // Each thread a few neighbouring bins, largest logits first.
-    const int b0 = tid * kPerThread;
-    uint32_t n[kPerThread];
-    u64 w[kPerThread], mine_n = 0, mine_w = 0, all_n, all_w;
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-      n[i] = counts[b0 + i];
-      mine_n += n[i];
-      w[i] = 0;
+    // Their weights: neighbouring bins, which tend to be filled together, on different threads. Where fp32 has no mean
+    // it takes a bin's middle.
+    for (int b = tid; b < kBins; b += kThreads) {
+      const uint32_t n = counts[b];
+      if (n == 0) continue;
+      float l = logit_of_bin(b, low);
+      if (WIDE && b != kHalf) {
+        const uint32_t in = b <= heavy ? (uint32_t)__fdividef((float)(uint32_t)weights[b], (float)n) : 0x8000u;
+        l = fminf(__uint_as_float(__float_as_uint(l) + in), top);
+      }
+      weights[b] = weigh(l);
     }
-    u64 before = scan(mine_n, all_n, sh.sc.sum);
-    // tokens of each bin that top-k leaves; fp32 takes the middle of a bin for all of its tokens
-    if (tid == 0) sh.edge_bin = kNone, sh.edge_count = 0, sh.lo_bin = kBinsPadded, sh.hi_bin = -1, sh.list_n = 0, sh.list_over = 0, sh.k_border = 0;
     __syncthreads();
-#pragma unroll
+    // Each thread a few neighbouring bins, largest logits first: tokens of each that top-k leaves, and their mass.
+    const int b0 = tid * kPerThread;
+    u64 mine_n = 0, mine_w = 0, all_n, all_w;
+#pragma unroll 3
+    for (int i = 0; i < kPerThread; ++i) mine_n += counts[b0 + i];
+    u64 before = scan<kThreads>(mine_n, all_n, sh.sc.sum);
+#pragma unroll 3
     for (int i = 0; i < kPerThread; ++i) {
-      const uint32_t had = n[i];
+      const uint32_t had = counts[b0 + i];
+      uint32_t n = had;
       if (by_k) {
-        n[i] = before >= (u64)k ? 0u : (uint32_t)min((u64)n[i], (u64)k - before);
-        if ((n[i] < had && n[i] > 0) || (before + had == (u64)k && had > 0)) {
-          if (!WIDE) sh.edge_bin = b0 + i, sh.edge_count = (int)n[i];
+        n = before >= (u64)k ? 0u : (uint32_t)min((u64)had, (u64)k - before);
+        if ((n < had && n > 0) || (before + had == (u64)k && had > 0)) {
+          if (!WIDE) sh.edge_bin = b0 + i, sh.edge_count = (int)n;
           else atomicMin(&sh.lo_bin, b0 + i), atomicMax(&sh.hi_bin, b0 + i), sh.k_border = 1;
         }
+        counts[b0 + i] = n;
       }
       before += had;
-      if (n[i] > 0) {
-        float l = logit_of_bin(b0 + i, low);
-        if (WIDE) {
-          const float next = b0 + i < kHalf ? logit_of_bin(b0 + i - 1, low) : logit_of_bin(b0 + i + 1, low);
-          l = b0 + i == kHalf ? 0.f : fminf(0.5f * l + 0.5f * next, logit_of(top));
-        }
-        w[i] = weigh(l);
-        mine_w += w[i] * n[i];
-      }
+      if (n > 0) mine_w += weights[b0 + i] * n;
     }
-    if (by_p || !WIDE) {
-      u64 mass = scan(mine_w, all_w, sh.sc.sum);
-      const u64 want = by_p ? share_of(tp, all_w, true) : ~0ull;
-      // fp32: the border is somewhere within 2^-8 of the total (checked later); 2^-12 where bins are narrow would do
-      const u64 slack = WIDE ? (all_w >> 8) + 1 : 0;
-      const u64 want_lo = want > slack ? want - slack : 0, want_hi = want + slack;
-#pragma unroll
+    u64 mass = scan<kThreads>(mine_w, all_w, sh.sc.sum);
+    const u64 want = by_p ? share_of(tp, all_w, true) : ~0ull;
+    // fp32: the border is somewhere near (checked later): within 2^-11 of the total and five deviations of what
+    // the others' middles leave out, a token of half a bin's width h being off by up to w h / t, on average 0
+    u64 slack = 0;
+    if (WIDE && by_p) {
+      float off = 0.f;
+#pragma unroll 3
       for (int i = 0; i < kPerThread; ++i) {
-        if (n[i] == 0) continue;
-        const u64 here = w[i] * n[i];
-        if (by_p && !WIDE) {
-          const uint32_t had = n[i];
-          if (mass >= want) n[i] = 0;
-          else if (w[i] > 0 && mass + here >= want) n[i] = (uint32_t)min((u64)had, (want - mass + w[i] - 1) / w[i]);
-          if (mass == 0 && n[i] == 0) n[i] = 1;  // the first token always stays
-          if (n[i] > 0 && (n[i] < had || mass + here >= want)) sh.edge_bin = b0 + i, sh.edge_count = (int)n[i];
-        } else if (by_p) {
-          // bins that the border may fall into
-          if (mass <= want_hi && mass + here >= want_lo) atomicMin(&sh.lo_bin, b0 + i), atomicMax(&sh.hi_bin, b0 + i);
-        }
-        mass += here;
+        const int b = b0 + i;
+        if (counts[b] == 0 || b == kHalf || b <= heavy) continue;
+        const float width = fabsf(logit_of_bin(b, low)) * 0.0078125f / t;  // at most
+        const float one_off = (float)weights[b] * fminf(0.5f * width, 4.f);
+        off += (float)counts[b] * one_off * one_off * 0.333f;
       }
+      off = warp_sum(off);
+      if (lane == 0) sh.red[warp] = __float_as_uint(off);
+      __syncthreads();
+      off = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) off += __uint_as_float(sh.red[i]);
+      slack = (all_w >> 11) + 1 + (u64)fminf(5.f * sqrtf(off), (float)all_w);
+    }
+    const u64 want_lo = want > slack ? want - slack : 0, want_hi = want + slack;
+#pragma unroll 3
+    for (int i = 0; i < kPerThread; ++i) {
+      const int b = b0 + i;
+      uint32_t n = counts[b];
+      if (n == 0) {
+        if (!WIDE) weights[b] = 0;
+        continue;
+      }
+      const u64 w = weights[b], here = w * n;
+      if (WIDE) {  // bins that the border may fall into
+        if (by_p && mass <= want_hi && mass + here >= want_lo) atomicMin(&sh.lo_bin, b), atomicMax(&sh.hi_bin, b);
+      } else {
+        bool keep = true;
+        if (by_p) {
+          const uint32_t had = n;
+          if (mass >= want) n = mass == 0;  // the first token always stays
+          else if (w > 0 && mass + here >= want) n = (uint32_t)min((u64)had, (want - mass + w - 1) / w);
+          keep = n > 0;
+          if (keep && (n < had || mass + here >= want)) sh.edge_bin = b, sh.edge_count = (int)n;
+        }
+        if (!keep || w < least_w) weights[b] = 0;
+      }
+      mass += here;
     }
     __syncthreads();
     if (!WIDE) {
-      const float floor_w = by_m ? fminf(mp, 1.f) : 0.f;
-#pragma unroll
-      for (int i = 0; i < kPerThread; ++i) {
-        bool keep = n[i] > 0;
-        if (by_m && keep) {
-          const float l = logit_of_bin(b0 + i, low);
-          keep = l == logit_of(top) || weigh.share(l) >= (double)floor_w;
+      // the border's bin is counted token by token
+      if (tid == 0) {
+        weights[kNone] = 0;
+        if (sh.edge_bin != kNone) {
+          sh.edge_w = weights[sh.edge_bin];
+          weights[sh.edge_bin] = 0;
         }
-        // the border's bin is counted token by token
-        weights[b0 + i] = keep && b0 + i != sh.edge_bin ? w[i] : 0;
-        if (b0 + i == sh.edge_bin) sh.above = keep ? w[i] : 0;
       }
-      if (tid == 0) weights[kNone] = 0;
       __syncthreads();
     }
   }
@@ -500,9 +718,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   // ---- kept weights of every warp's stretch
   const int per_warp = (row.vectors + kWarps - 1) / kWarps;
   const int v0 = min(row.vectors, warp * per_warp), v1 = min(row.vectors, v0 + per_warp);
-  if constexpr (!WIDE) {
+  if (!WIDE && bins) {
     const int edge = sh.edge_bin;
-    const u64 edge_w = edge == kNone ? 0 : sh.above;
+    const u64 edge_w = edge == kNone ? 0 : sh.edge_w;
     const u64 edge_n = (u64)sh.edge_count;
     u64 sum = 0;
     uint32_t ties = 0;
@@ -523,30 +741,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
     if (lane == 0) sh.sc.sum[warp] = sum, sh.sc.sum2[warp] = ties;
     __syncthreads();
-    // stretch by stretch: ties before it, and the weight with those that stay
-    u64 run = 0, seen = 0, all = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      const u64 stay = seen >= edge_n ? 0 : min(sh.sc.sum2[i], edge_n - seen);
-      seen += sh.sc.sum2[i];
-      all += sh.sc.sum[i] + stay * edge_w;
-    }
-    u64 want = share_of(p.uniform[r], all);
-    if (want >= all) want = all - 1;
-    seen = 0;
-    int in = 0;
-    u64 run_in = 0, seen_in = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      const u64 stay = seen >= edge_n ? 0 : min(sh.sc.sum2[i], edge_n - seen);
-      const u64 here = sh.sc.sum[i] + stay * edge_w;
-      if (run <= want && want < run + here) in = i, run_in = run, seen_in = seen;
-      seen += sh.sc.sum2[i];
-      run += here;
-    }
+    // a stretch to a lane: ties before it, and the weight with those that stay
+    const u64 my_ties = lane < kWarps ? sh.sc.sum2[lane] : 0;
+    const u64 seen = lane_scan(my_ties);
+    const u64 stay = seen >= edge_n ? 0 : min(my_ties, edge_n - seen);
+    const Stretch in = stretch_of((lane < kWarps ? sh.sc.sum[lane] : 0) + stay * edge_w, p.uniform[r]);
+    const u64 seen_in = __shfl_sync(kAll, seen, in.at);
     __syncthreads();
     // ---- the stretch with the target, a vector or a few to a thread
-    const int s0 = min(row.vectors, in * per_warp), s1 = min(row.vectors, s0 + per_warp);
+    const int s0 = min(row.vectors, in.at * per_warp), s1 = min(row.vectors, s0 + per_warp);
     const int per = (s1 - s0 + kThreads - 1) / kThreads;
     const int j0 = min(s1, s0 + tid * per), j1 = min(s1, j0 + per);
     u64 mine = 0, mine_ties = 0, dummy;
@@ -560,11 +763,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
         mine_ties += bin == edge && edge != kNone;
       }
     }
-    u64 my_seen = seen_in + scan(mine_ties, dummy, sh.sc.sum);
+    u64 my_seen = seen_in + scan<kThreads>(mine_ties, dummy, sh.sc.sum);
     const u64 my_stay = my_seen >= edge_n ? 0 : min(mine_ties, edge_n - my_seen);
     mine += my_stay * edge_w;
-    u64 my_run = run_in + scan(mine, dummy, sh.sc.sum);
-    if (my_run <= want && want < my_run + mine) {
+    u64 my_run = in.before + scan<kThreads>(mine, dummy, sh.sc.sum);
+    if (my_run <= in.target && in.target < my_run + mine) {
       for (int j = j0; j < j1; ++j) {
         float x[N];
         row.load(j, x);
@@ -573,179 +776,161 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
           const int bin = bin_of(x[i], low);
           u64 w = weights[bin];
           if (bin == edge && edge != kNone && my_seen++ < edge_n) w = edge_w;
-          if (my_run <= want && want < my_run + w) {
+          if (my_run <= in.target && in.target < my_run + w) {
             p.ids[r] = j * N - row.shift + i;
-            if (p.logp) p.logp[r] = (float)(((double)x[i] - weigh.top) * weigh.inv - log((double)all / weigh.one));
+            if (p.logp) p.logp[r] = log_share(x[i], in.all);
           }
           my_run += w;
         }
       }
     }
-  } else {
-    FastWeigher fast;
-    {
-      const double c = 1.4426950408889634 / (double)t;
-      fast.top = logit_of(top);
-      fast.c = (float)c;
-      fast.c_low = isinf(fast.c) ? 0.f : (float)(c - (double)fast.c);
-      fast.bits = p.scale_bits - 31;
-      fast.table = sh.table;
-    }
-    const u64 least_w = by_m ? (u64)(fmin((double)mp, 1.) * weigh.one) : 0;
-    auto heavy = [&](u64 w, float l) { return !by_m || w >= least_w || l == fast.top; };
-    const bool edged = bins && sh.hi_bin >= 0;  // (top-k of more tokens than weigh anything leaves all)
-    const int lo = edged ? sh.lo_bin : kNone, hi = edged ? sh.hi_bin : kNone;
-    const bool all_rest = by_p && !sh.k_border;  // the total that top-p takes a share of goes on below the list
-    u64 sum = 0, rest = 0, all_above = 0;
-    uint32_t above_n = 0;
+    return;
+  }
+
+  const bool edged = WIDE && bins && sh.hi_bin >= 0;  // (top-k of more tokens than weigh anything leaves all)
+  const int lo = edged ? sh.lo_bin : kNone, hi = edged ? sh.hi_bin : kNone;
+  const bool all_rest = by_p && !sh.k_border;  // the total that top-p takes a share of goes on below the list
+  u64 sum = 0, rest = 0, all_above = 0;
+  uint32_t above_n = 0;
+  if (!edged) {
 #pragma unroll 2
     for (int j = v0 + lane; j < v1; j += 32) {
       float x[N];
       row.load(j, x);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if (!edged) {
-          const u64 w = fast(x[i]);
-          if (heavy(w, x[i])) sum += w;
-        } else {
-          const int bin = bin_of(x[i], low);
-          if (bin < lo) {
-            const u64 w = fast(x[i]);
-            ++above_n;
-            all_above += w;
-            if (heavy(w, x[i])) sum += w;
-          } else if (bin <= hi) {
-            const int at = atomicAdd(&sh.list_n, 1);
-            if (at < kList) list[at] = (u64)key_of(x[i]) << 32 | (uint32_t)~(j * N - row.shift + i);
-          } else if (all_rest) {
-            rest += fast(x[i]);
-          }
+        const u64 w = weigh(x[i]);
+        sum += by_m && w < least_w ? 0 : w;
+      }
+    }
+  } else {
+#pragma unroll 2
+    for (int j = v0 + lane; j < v1; j += 32) {
+      float x[N];
+      row.load(j, x);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int bin = bin_of(x[i], low);
+        const u64 w = weigh(x[i]);
+        const bool above = bin < lo;
+        above_n += above;
+        all_above += above ? w : 0;
+        sum += above && w >= least_w ? w : 0;
+        rest += bin > hi ? w : 0;
+        if (!above && bin <= hi) {
+          const int at = atomicAdd(&sh.list_n, 1);
+          if (at < kList) list[at] = (u64)key_of(x[i]) << 32 | (uint32_t)~(j * N - row.shift + i);
         }
       }
     }
-    u64 edge = 0;  // tokens at or above it (key, then lower indexes) are kept
-    if (edged) {
-      const u64 above_w = block_sum(all_above, sh.sc.sum), rest_w = block_sum(rest, sh.sc.sum);
-      const u64 n_above = block_sum(above_n, sh.sc.sum);
-      const int n = sh.list_n;
-      if (n > kList) {
-        slow_row<T>(p, r, top, t, sh.sc);
-        return;
-      }
-      // sort the list, largest first
-      int size = 32;
-      while (size < n) size <<= 1;
-      for (int i = n + tid; i < size; i += kThreads) list[i] = 0;
-      __syncthreads();
-      for (int run = 2; run <= size; run <<= 1)
-        for (int step = run >> 1; step > 0; step >>= 1) {
-          for (int i = tid; i < size / 2; i += kThreads) {
-            const int a = 2 * i - (i & (step - 1)), b = a + step;
-            const u64 x = list[a], y = list[b];
-            if ((x < y) == ((a & run) == 0)) list[a] = y, list[b] = x;
-          }
-          __syncthreads();
-        }
-      // their weights, and what top-k, then top-p leaves of them
-      const int per = (size + kThreads - 1) / kThreads, i0 = min(size, tid * per), i1 = min(size, i0 + per);
-      const u64 left_k = by_k ? ((u64)k > n_above ? (u64)k - n_above : 0) : ~0ull;
-      u64 mine = 0, all_w;
-      for (int i = i0; i < i1; ++i)
-        if (i < n && (u64)i < left_k) mine += fast(logit_of((uint32_t)(list[i] >> 32)));
-      u64 mass = above_w + scan(mine, all_w, sh.sc.sum);
-      const u64 total = above_w + all_w + rest_w;
-      const u64 want = by_p ? share_of(tp, total, true) : ~0ull;
-      if (tid == 0) sh.edge = 0, sh.list_over = 0;
-      __syncthreads();
-      // The last token kept; the first of all always is. A top-p border outside the list is a slow row.
-      for (int i = i0; i < i1; ++i) {
-        if (i >= n || (u64)i >= left_k) break;
-        const u64 w = fast(logit_of((uint32_t)(list[i] >> 32)));
-        const bool first = n_above == 0 && i == 0;
-        if (mass < want || first) {
-          const bool last = (u64)i + 1 >= left_k || (by_p && mass + w >= want);
-          if (last || i + 1 == n) sh.edge = list[i];
-          if (!last && i + 1 == n && by_p && rest_w > 0) sh.list_over = 1;  // the border lies below the list
-        }
-        mass += w;
-      }
-      if (by_p && tid == 0 && above_w >= want && n_above > 0) sh.list_over = 1;  // or above it
-      __syncthreads();
-      edge = sh.edge;
-      if (sh.list_over || edge == 0) {
-        slow_row<T>(p, r, top, t, sh.sc);
-        return;
-      }
+    if (!all_rest) rest = 0;
+  }
+  u64 edge = 0;  // tokens at or above it (key, then lower indexes) are kept
+  if (edged) {
+    const u64 above_w = block_sum<kThreads>(all_above, sh.sc.sum), rest_w = block_sum<kThreads>(rest, sh.sc.sum);
+    const u64 n_above = block_sum<kThreads>(above_n, sh.sc.sum);
+    const int n = sh.list_n;
+    if (n > kList) {
+      slow_row<T, kThreads>(p, r, key_of(top), t, sh.sc);
+      return;
     }
-    auto kept = [&](float l, int i, u64& w) {
-      w = 0;
-      if (!(l > -INFINITY)) return;
-      if (edged && ((u64)key_of(l) << 32 | (uint32_t)~i) < edge) return;
-      w = fast(l);
-      if (!heavy(w, l)) w = 0;
-    };
-    // the list's kept tokens belong to their stretches
-    if (lane == 0) sh.sc.sum2[warp] = 0;
+    // sort the list, largest first
+    int size = 64;
+    while (size < n) size <<= 1;
+    for (int i = n + tid; i < size; i += kThreads) list[i] = 0;
     __syncthreads();
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
-    if (edged) {
-      for (int i = tid; i < sh.list_n; i += kThreads) {
-        if (list[i] < edge) continue;
-        const int index = (int)~(uint32_t)list[i];
-        u64 w;
-        kept(logit_of((uint32_t)(list[i] >> 32)), index, w);
-        if (w) atomicAdd(&sh.sc.sum2[(index + row.shift) / N / per_warp], w);
+    sort<kThreads>(list, size);
+    // their weights, and what top-k, then top-p leaves of them
+    const int per = (size + kThreads - 1) / kThreads, i0 = min(size, tid * per), i1 = min(size, i0 + per);
+    const u64 left_k = by_k ? ((u64)k > n_above ? (u64)k - n_above : 0) : ~0ull;
+    u64 mine = 0, all_w;
+    for (int i = i0; i < i1; ++i)
+      if (i < n && (u64)i < left_k) mine += weigh(logit_of((uint32_t)(list[i] >> 32)));
+    u64 mass = above_w + scan<kThreads>(mine, all_w, sh.sc.sum);
+    const u64 total = above_w + all_w + rest_w;
+    const u64 want = by_p ? share_of(tp, total, true) : ~0ull;
+    if (tid == 0) sh.edge = 0, sh.list_over = 0;
+    __syncthreads();
+    // The last token kept; the first of all always is. A top-p border outside the list is a slow row.
+    for (int i = i0; i < i1; ++i) {
+      if (i >= n || (u64)i >= left_k) break;
+      const u64 w = weigh(logit_of((uint32_t)(list[i] >> 32)));
+      const bool first = n_above == 0 && i == 0;
+      if (mass < want || first) {
+        const bool last = (u64)i + 1 >= left_k || (by_p && mass + w >= want);
+        if (last || i + 1 == n) sh.edge = list[i];
+        if (!last && i + 1 == n && by_p && rest_w > 0) sh.list_over = 1;  // the border lies below the list
       }
+      mass += w;
     }
-    if (lane == 0) sh.sc.sum[warp] = sum;
+    if (by_p && tid == 0 && above_w >= want && n_above > 0) sh.list_over = 1;  // or above it
     __syncthreads();
-    u64 all = 0, run = 0, run_in = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) all += sh.sc.sum[i] + sh.sc.sum2[i];
-    u64 want = share_of(p.uniform[r], all);
-    if (want >= all) want = all - 1;
-    int in = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      const u64 here = sh.sc.sum[i] + sh.sc.sum2[i];
-      if (run <= want && want < run + here) in = i, run_in = run;
-      run += here;
+    edge = sh.edge;
+    if (sh.list_over || edge == 0) {
+      slow_row<T, kThreads>(p, r, key_of(top), t, sh.sc);
+      return;
     }
-    __syncthreads();
-    // ---- the stretch with the target, a vector or a few to a thread
-    const int s0 = min(row.vectors, in * per_warp), s1 = min(row.vectors, s0 + per_warp);
-    const int per = (s1 - s0 + kThreads - 1) / kThreads;
-    const int j0 = min(s1, s0 + tid * per), j1 = min(s1, j0 + per);
-    u64 mine = 0, dummy;
+  }
+  auto kept = [&](float l, int i) {
+    const u64 w = weigh(l);
+    const bool below = edged && ((u64)key_of(l) << 32 | (uint32_t)~i) < edge;
+    return below || w < least_w ? 0 : w;
+  };
+  // the list's kept tokens belong to their stretches
+  if (lane == 0) sh.sc.sum2[warp] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+  if (edged) {
+    for (int i = tid; i < sh.list_n; i += kThreads) {
+      if (list[i] < edge) continue;
+      const int index = (int)~(uint32_t)list[i];
+      const u64 w = kept(logit_of((uint32_t)(list[i] >> 32)), index);
+      if (w) atomicAdd(&sh.sc.sum2[(index + row.shift) / N / per_warp], w);
+    }
+  }
+  if (lane == 0) sh.sc.sum[warp] = sum;
+  __syncthreads();
+  const Stretch in = stretch_of(lane < kWarps ? sh.sc.sum[lane] + sh.sc.sum2[lane] : 0, p.uniform[r]);
+  __syncthreads();
+  // ---- the stretch with the target, a vector or a few to a thread
+  const int s0 = min(row.vectors, in.at * per_warp), s1 = min(row.vectors, s0 + per_warp);
+  const int per = (s1 - s0 + kThreads - 1) / kThreads;
+  const int j0 = min(s1, s0 + tid * per), j1 = min(s1, j0 + per);
+  u64 mine = 0, dummy;
+  for (int j = j0; j < j1; ++j) {
+    float x[N];
+    row.load(j, x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) mine += kept(x[i], j * N - row.shift + i);
+  }
+  u64 my_run = in.before + scan<kThreads>(mine, dummy, sh.sc.sum);
+  if (my_run <= in.target && in.target < my_run + mine) {
     for (int j = j0; j < j1; ++j) {
       float x[N];
       row.load(j, x);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        u64 w;
-        kept(x[i], j * N - row.shift + i, w);
-        mine += w;
-      }
-    }
-    u64 my_run = run_in + scan(mine, dummy, sh.sc.sum);
-    if (my_run <= want && want < my_run + mine) {
-      for (int j = j0; j < j1; ++j) {
-        float x[N];
-        row.load(j, x);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          u64 w;
-          kept(x[i], j * N - row.shift + i, w);
-          if (my_run <= want && want < my_run + w) {
-            p.ids[r] = j * N - row.shift + i;
-            if (p.logp) p.logp[r] = (float)(((double)x[i] - weigh.top) * weigh.inv - log((double)all / weigh.one));
-          }
-          my_run += w;
+        const u64 w = kept(x[i], j * N - row.shift + i);
+        if (my_run <= in.target && in.target < my_run + w) {
+          p.ids[r] = j * N - row.shift + i;
+          if (p.logp) p.logp[r] = log_share(x[i], in.all);
         }
+        my_run += w;
       }
     }
   }
+}
+
+template <typename T, int kThreads>
+static int launch(const Params& p, int rows, cudaStream_t st) {
+  constexpr int kBinsPadded = kPadded<kThreads>;
+  constexpr int SMEM = (kBinsPadded + 4) * 4 + (kBinsPadded + 2) * 8 + kTable * 8;
+  static_assert(kBinsPadded > kNone && kBinsPadded >= kList, "room for either use");
+  static_assert(1024 / kThreads * (SMEM + 2048) <= 228 * 1024, "CTAs an SM");
+  auto kernel = sample_kernel<T, kThreads>;
+  if (allow_shared(reinterpret_cast<const void*>(kernel), SMEM) != cudaSuccess) return CDB_ERR_CUDA;
+  return launch_pdl(kernel, dim3(rows), dim3(kThreads), SMEM, st, p) == cudaSuccess ? CDB_OK : CDB_ERR_CUDA;
 }
 
 }  // namespace sample
@@ -778,8 +963,7 @@ extern "C" int cdb_sample_tokens(const void* logits, int logits_fp32, int64_t lo
   while ((1 << bits) < vocab) ++bits;
   p.scale_bits = 62 - bits < 46 ? 62 - bits : 46;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int smem = (kBinsPadded + 4) * 4 + (logits_fp32 ? kList : kBinsPadded + 1) * 8;
-  auto* kernel = logits_fp32 ? sample_kernel<float> : sample_kernel<__nv_bfloat16>;
-  if (allow_shared(reinterpret_cast<const void*>(kernel), smem) != cudaSuccess) return CDB_ERR_CUDA;
-  return launch_pdl(kernel, dim3(num_rows), dim3(kThreads), smem, st, p) == cudaSuccess ? CDB_OK : CDB_ERR_CUDA;
+  // One CTA an SM has the whole SM while there are no more rows than SMs; two share it where there are more.
+  if (num_rows <= 148) return logits_fp32 ? launch<float, 1024>(p, num_rows, st) : launch<__nv_bfloat16, 1024>(p, num_rows, st);
+  return logits_fp32 ? launch<float, 512>(p, num_rows, st) : launch<__nv_bfloat16, 512>(p, num_rows, st);
 }
