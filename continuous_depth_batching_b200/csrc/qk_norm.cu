@@ -6,16 +6,18 @@
 // are copied.
 //
 // A head is a group of 8 or 16 lanes with 16 bytes each, so its sum of squares takes three or four shuffles
-// and a pair's other half (D / 2 further on, another lane's) four. A group takes up to four heads at once, so that
-// their loads are in flight together, over all of a row's heads before the next CTA's rows; a CTA takes several
-// rows where they have few heads. Everything is read and written once: bound by HBM over many rows, by a chain of
-// three latencies (position, block id and angles, stores) over few.
+// and a pair's other half (D / 2 further on, another lane's) four of packed values. A warp takes one row's heads, or a
+// slice of them where there are few rows: position, block id, angles and weights are the same for all of a row's
+// heads, so a lane loads its part of them once and multiplies the last two: a value costs a product with w c, one of
+// its partner with the partner's w s, and one with the norm. Heads of q come first, then k's, then the values, which
+// are only copied; four heads of a group are in flight at a time. Everything is read and written once: bound by HBM over
+// many rows, by a chain of three latencies (position, block id and angles, stores) over few.
 #include "cdb_common.cuh"
 
 namespace cdb {
 namespace qknorm {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kBlock = 16;  // tokens of one cache block
 constexpr int kDepth = 4;   // heads of a group in flight
 
@@ -37,7 +39,8 @@ struct Params {
   const void* rope_sin;
   int rope_rows;
   float eps;
-  int num_items, heads, kv_heads, rows_per_cta;
+  int num_items, heads, kv_heads;
+  int slices;  // warps of a row
   int32_t* status;
 };
 
@@ -47,112 +50,136 @@ __device__ __forceinline__ void unpack(const uint4& w, float (&v)[8]) {
 }
 
 template <int D, int MODE>
-__global__ void __launch_bounds__(kThreads) qk_norm_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 6) qk_norm_kernel(const Params p) {
   pdl_trigger();
   pdl_wait();
-  constexpr int LANES = D / 8;                 // lanes that hold a head
-  constexpr int GROUP = LANES <= 8 ? 8 : 16;   // lanes of a group (4 of 16 idle at 96)
-  constexpr int GROUPS = kThreads / GROUP;
-  const int c = threadIdx.x % GROUP, group = threadIdx.x / GROUP;
+  constexpr int LANES = D / 8;                // lanes that hold a head
+  constexpr int GROUP = LANES <= 8 ? 8 : 16;  // lanes of a group (4 of 16 idle at 96)
+  constexpr int GROUPS = 32 / GROUP;          // heads of a warp at a time
+  const int lane = threadIdx.x & 31, c = lane % GROUP, group = lane / GROUP;
   const bool lane_on = c < LANES;
   const int at = lane_on ? c * 8 : 0;
-  const int other = c < LANES / 2 ? c + LANES / 2 : c - LANES / 2;  // the lane with the pair's other half
-  const int row0 = blockIdx.x * p.rows_per_cta;
-  const int all = p.heads + 2 * p.kv_heads;
-  const int units = min(p.rows_per_cta, p.num_items - row0) * all;
-  const uint4 none = make_uint4(0u, 0u, 0u, 0u);
-  float wq[8], wk[8];
-  unpack(*reinterpret_cast<const uint4*>(p.q_weight + at), wq);
-  unpack(*reinterpret_cast<const uint4*>(p.k_weight + at), wk);
+  const bool lower = c < LANES / 2;
+  const int other = lower ? c + LANES / 2 : c - LANES / 2;  // the lane with the pair's other half
+  const int64_t task = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  const int row = (int)(task / p.slices), slice = (int)(task - (int64_t)row * p.slices);
+  if (row >= p.num_items) return;
+  const int pos = p.item_pos[row], slot = p.item_slot[row];
+  if (pos < 0) return;
+  if (slot < 0 || slot >= p.bt_rows || pos / kBlock >= p.bt_width || (MODE != 0 && pos >= p.rope_rows)) {
+    if (lane == 0) set_error(p.status, CDB_ERR_INDEX);
+    return;
+  }
+  const int64_t id = p.block_table[(int64_t)slot * p.bt_stride + pos / kBlock];
+  float cv[8], sv[8];  // cosines, and sines with the partner's sign
+  if (MODE == 1) {     // bf16 [positions][D]
+    unpack(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.rope_cos) + (int64_t)pos * D + at), cv);
+    unpack(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.rope_sin) + (int64_t)pos * D + at), sv);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sv[k] = lower ? -sv[k] : sv[k];
+  } else if (MODE == 2) {  // fp32 [positions][D / 2]
+    const float4 cw = *reinterpret_cast<const float4*>(static_cast<const float*>(p.rope_cos) + (int64_t)pos * (D / 2) + at / 2);
+    const float4 sw = *reinterpret_cast<const float4*>(static_cast<const float*>(p.rope_sin) + (int64_t)pos * (D / 2) + at / 2);
+    cv[0] = cv[1] = cw.x, cv[2] = cv[3] = cw.y, cv[4] = cv[5] = cw.z, cv[6] = cv[7] = cw.w;
+    sv[0] = -sw.x, sv[1] = sw.x, sv[2] = -sw.y, sv[3] = sw.y, sv[4] = -sw.z, sv[5] = sw.z, sv[6] = -sw.w, sv[7] = sw.w;
+  }
+  if (id < 0 || (id + 1) * kBlock > p.kv_rows) {
+    if (lane == 0) set_error(p.status, CDB_ERR_INDEX);
+    return;
+  }
+  const __nv_bfloat16* src = p.qkv + (int64_t)row * p.qkv_stride + at;
+  const int64_t kv_cols = (int64_t)p.kv_heads * D;
+  __nv_bfloat16* keys = p.keys + (id * kBlock + pos % kBlock) * kv_cols + at;
+  const int q_steps = (p.heads + GROUPS - 1) / GROUPS, k_steps = (p.kv_heads + GROUPS - 1) / GROUPS;
+  const int per = (q_steps + 2 * k_steps + p.slices - 1) / p.slices;
 
-  for (int u0 = 0; u0 < units; u0 += GROUPS * kDepth) {
-    uint4 x[kDepth], cs[kDepth][MODE == 0 ? 1 : 2];
-    __nv_bfloat16* dst[kDepth];
-    int kind[kDepth];  // 0 query, 1 key, 2 value
+  // `heads` heads from `from` on to `to`, of which this slice takes steps [a, b)
+  auto rotate = [&](const __nv_bfloat16* weight, const __nv_bfloat16* from, __nv_bfloat16* to, int heads, int a, int b) {
+    if (a >= b) return;
+    float wc[8], ws[8];
+    unpack(*reinterpret_cast<const uint4*>(weight + at), wc);
+    if (MODE == 1) unpack(*reinterpret_cast<const uint4*>(weight + (lane_on ? other * 8 : 0)), ws);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (MODE == 1) ws[k] *= sv[k];
+      if (MODE == 2) ws[k] = wc[k ^ 1] * sv[k];
+    }
+    if (MODE != 0) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) wc[k] *= cv[k];
+    }
+    for (int s = a; s < b; s += kDepth) {
+      uint4 x[kDepth];
+#pragma unroll
+      for (int i = 0; i < kDepth; ++i) {
+        const int h = (s + i) * GROUPS + group;
+        x[i] = s + i < b && h < heads && lane_on ? __ldcg(reinterpret_cast<const uint4*>(from + (int64_t)h * D))
+                                                 : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int i = 0; i < kDepth; ++i) {
+        if (s + i >= b) break;  // (the same for the whole warp)
+        const int h = (s + i) * GROUPS + group;
+        float y[8], z[8];
+        unpack(x[i], y);
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum = fmaf(y[k], y[k], sum);
+#pragma unroll
+        for (int o = GROUP / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float inv = rsqrtf(sum * (1.f / D) + p.eps);
+        if (MODE == 1)
+          unpack(make_uint4(__shfl_sync(0xffffffffu, x[i].x, other, GROUP), __shfl_sync(0xffffffffu, x[i].y, other, GROUP),
+                            __shfl_sync(0xffffffffu, x[i].z, other, GROUP), __shfl_sync(0xffffffffu, x[i].w, other, GROUP)),
+                 z);
+        // (scaled first: a product of large values and weights need not overflow before the norm)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          y[k] *= inv;
+          if (MODE == 1) z[k] *= inv;
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+          float lo = y[k] * wc[k], hi = y[k + 1] * wc[k + 1];
+          if (MODE != 0) {
+            lo = fmaf(MODE == 1 ? z[k] : y[k + 1], ws[k], lo);
+            hi = fmaf(MODE == 1 ? z[k + 1] : y[k], ws[k + 1], hi);
+          }
+          w[k / 2] = pack_bf16x2(lo, hi);
+        }
+        if (h < heads && lane_on)
+          *reinterpret_cast<uint4*>(to + (int64_t)h * D) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  };
+  const int s0 = slice * per, s1 = s0 + per, k_end = q_steps + k_steps, v_end = k_end + k_steps;
+  if (p.q_out != nullptr)
+    rotate(p.q_weight, src, p.q_out + (int64_t)row * p.q_out_stride + at, p.heads, min(s0, q_steps), min(s1, q_steps));
+  rotate(p.k_weight, src + (int64_t)p.heads * D, keys, p.kv_heads, min(max(s0, q_steps), k_end) - q_steps,
+         min(max(s1, q_steps), k_end) - q_steps);
+  const __nv_bfloat16* values = src + (int64_t)(p.heads + p.kv_heads) * D;
+  __nv_bfloat16* to = keys + p.kv_rows * kv_cols;
+  const int v1 = min(s1, v_end) - k_end;
+  for (int s = max(s0, k_end) - k_end; s < v1; s += kDepth) {
+    uint4 x[kDepth];
 #pragma unroll
     for (int i = 0; i < kDepth; ++i) {
-      const int u = u0 + i * GROUPS + group;
-      dst[i] = nullptr;
-      kind[i] = 2;
-      x[i] = none;
-      if (MODE != 0) cs[i][0] = cs[i][MODE == 0 ? 0 : 1] = none;
-      if (u >= units) continue;
-      const int r = u / all, h = u - r * all, row = row0 + r;
-      const int pos = p.item_pos[row];
-      if (pos < 0) continue;
-      kind[i] = h < p.heads ? 0 : (h < p.heads + p.kv_heads ? 1 : 2);
-      if (kind[i] == 0 && p.q_out == nullptr) continue;
-      const int slot = p.item_slot[row];
-      int64_t cache_row = -1;
-      if (slot >= 0 && slot < p.bt_rows && pos / kBlock < p.bt_width && (MODE == 0 || pos < p.rope_rows)) {
-        const int64_t id = p.block_table[(int64_t)slot * p.bt_stride + pos / kBlock];
-        if (id >= 0 && (id + 1) * kBlock <= p.kv_rows) cache_row = id * kBlock + pos % kBlock;
-      }
-      if (cache_row < 0) {
-        if (c == 0) set_error(p.status, CDB_ERR_INDEX);
-        continue;
-      }
-      if (kind[i] == 0)
-        dst[i] = p.q_out + (int64_t)row * p.q_out_stride + h * D + at;
-      else
-        dst[i] = p.keys + ((kind[i] == 2 ? p.kv_rows : 0) + cache_row) * ((int64_t)p.kv_heads * D) +
-                 (h - p.heads - (kind[i] == 2 ? p.kv_heads : 0)) * D + at;
-      if (!lane_on) continue;
-      x[i] = *reinterpret_cast<const uint4*>(p.qkv + (int64_t)row * p.qkv_stride + (int64_t)h * D + at);
-      if (MODE == 1 && kind[i] != 2) {  // bf16 [positions][D]
-        cs[i][0] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.rope_cos) + (int64_t)pos * D + at);
-        cs[i][MODE == 0 ? 0 : 1] =
-            *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.rope_sin) + (int64_t)pos * D + at);
-      } else if (MODE == 2 && kind[i] != 2) {  // fp32 [positions][D / 2]
-        cs[i][0] = *reinterpret_cast<const uint4*>(static_cast<const float*>(p.rope_cos) + (int64_t)pos * (D / 2) + at / 2);
-        cs[i][MODE == 0 ? 0 : 1] =
-            *reinterpret_cast<const uint4*>(static_cast<const float*>(p.rope_sin) + (int64_t)pos * (D / 2) + at / 2);
-      }
+      const int h = (s + i) * GROUPS + group;
+      if (s + i < v1 && h < p.kv_heads && lane_on) x[i] = __ldcg(reinterpret_cast<const uint4*>(values + (int64_t)h * D));
     }
 #pragma unroll
     for (int i = 0; i < kDepth; ++i) {
-      float y[8];
-      unpack(x[i], y);
-      float sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sum = fmaf(y[k], y[k], sum);
-#pragma unroll
-      for (int o = GROUP / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float inv = rsqrtf(sum * (1.f / D) + p.eps);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) y[k] = y[k] * inv * (kind[i] == 0 ? wq[k] : wk[k]);
-      if (MODE == 1) {
-        float cv[8], sv[8];
-        unpack(cs[i][0], cv);
-        unpack(cs[i][MODE == 0 ? 0 : 1], sv);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float z = __shfl_sync(0xffffffffu, y[k], other, GROUP);
-          y[k] = fmaf(y[k], cv[k], (c < LANES / 2 ? -z : z) * sv[k]);
-        }
-      } else if (MODE == 2) {
-        const uint4 cw = cs[i][0], sw = cs[i][MODE == 0 ? 0 : 1];
-        const float cv[4] = {__uint_as_float(cw.x), __uint_as_float(cw.y), __uint_as_float(cw.z), __uint_as_float(cw.w)};
-        const float sv[4] = {__uint_as_float(sw.x), __uint_as_float(sw.y), __uint_as_float(sw.z), __uint_as_float(sw.w)};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float a = y[2 * k], b = y[2 * k + 1];
-          y[2 * k] = fmaf(a, cv[k], -b * sv[k]);
-          y[2 * k + 1] = fmaf(b, cv[k], a * sv[k]);
-        }
-      }
-      if (dst[i] == nullptr || !lane_on) continue;
-      *reinterpret_cast<uint4*>(dst[i]) =
-          kind[i] == 2 ? x[i]
-                       : make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
-                                    pack_bf16x2(y[6], y[7]));
+      const int h = (s + i) * GROUPS + group;
+      if (s + i < v1 && h < p.kv_heads && lane_on) *reinterpret_cast<uint4*>(to + (int64_t)h * D) = x[i];
     }
   }
 }
 
 template <int D>
 static int launch(const Params& p, int mode, cudaStream_t st) {
-  const dim3 grid((unsigned)(((int64_t)p.num_items + p.rows_per_cta - 1) / p.rows_per_cta));
+  const int64_t warps = (int64_t)p.num_items * p.slices;
+  const dim3 grid((unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32)));
   auto* kernel = mode == 0 ? qk_norm_kernel<D, 0> : mode == 1 ? qk_norm_kernel<D, 1> : qk_norm_kernel<D, 2>;
   return launch_pdl(kernel, grid, dim3(kThreads), 0, st, p) == cudaSuccess ? CDB_OK : CDB_ERR_CUDA;
 }
@@ -206,9 +233,12 @@ extern "C" int cdb_qk_norm_rope_append(const void* qkv, int64_t qkv_stride, void
   p.num_items = num_items;
   p.heads = num_heads;
   p.kv_heads = num_kv_heads;
-  const int group = head_dim == 64 ? 8 : 16, places = kThreads / group * kDepth;
-  const int rows = places / (num_heads + 2 * num_kv_heads);
-  p.rows_per_cta = rows > 1 ? rows : 1;
+  // A warp's heads take a round of memory latency each kDepth steps, so few rows are cut into as many slices as leave each
+  // one round; many rows fill the GPU by themselves.
+  const int groups = head_dim == 64 ? 4 : 2;
+  const int steps = (num_heads + groups - 1) / groups + 2 * ((num_kv_heads + groups - 1) / groups);
+  const int most = (steps + kDepth - 1) / kDepth, want = 148 * 24 / num_items;
+  p.slices = want < 1 ? 1 : want < most ? want : most;
   p.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (head_dim == 128) return launch<128>(p, rope_mode, st);
