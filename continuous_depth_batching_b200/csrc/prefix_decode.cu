@@ -5,21 +5,22 @@
 // maximum of the logits, l the sum of 2^(x - m), o that of 2^(x - m) v) of any set of keys join by rescaling to
 // one m, so the two kinds of work need not wait for each other: one launch does both side by side, and a
 // last one joins. Three launches in all:
-//   plan    one CTA: how many blocks each group shares, how the work is cut into equal shares;
-//   attend  two CTAs an SM, each of one kind: `Shared` steps (below) or pages of single rows;
+//   plan    one CTA: how many blocks each group shares, where every CTA and warp begins;
+//   attend  a CTA an SM, of one kind: shared steps or pages of single rows;
 //   join    a warp (or a CTA) per row and head adds up its parts. Rows with one part are written by attend.
 // No counters and no atomics between CTAs: parts lie where the plan says, and are added in that order.
 //
-// Shared steps. A CTA takes 128 rows (request x query head of one kv head) over a share of the group's 64-key
-// steps. Warps 0..3 are the softmax, thread r owns row r; warp 4 brings pages (TMA, 128-byte swizzle, two steps
-// ahead); warp 5 issues the products: S = Q K^T (tcgen05, 128 x 64 x D) and O += P V (128 x D x 64), P written over
-// the S that it comes from in tensor memory, V as it lies in the cache (the product's inner index across
-// its rows). Two CTAs an SM, so that one's exponentials run beside the other's products.
+// Shared steps. Rows are request x query head of a kv head, 128 to a tile. The 64-key steps of all (group, kv head, two
+// tiles) form one stream that is cut evenly. In a CTA two teams of four softmax warps, thread r owning row r, have
+// accumulators of their own: S = Q K^T (tcgen05, 128 x 64 x D) and O += P V (128 x D x 64), P written over the S that it
+// comes from in tensor memory, V as it lies in the cache (the product's inner index across its rows). Each team takes a
+// tile through every step; a tile without a partner is taken by both teams, every other step to each. So one team's
+// exponentials run beside the other's products, and a step's keys are read once for 256 rows. One warp issues
+// each team's products and one brings the pages (TMA, 128-byte swizzle), five steps ahead.
 //
 // Pages of single rows. The pages of all (row, kv head, up to 8 query heads) form one stream that is cut into equal
-// shares for the warps of the other CTAs. A page's K and V go straight from memory into the registers
-// of m16n8k16 products: the inner index may be permuted at will, so lanes load 16 bytes side by side and q is
-// loaded by the same permutation. K of the next page is requested before this one's softmax, V after its product.
+// shares for the warps of the other CTAs. A warp brings its pages into a ring of its own (two pages of 8 KB at 128; with
+// 12 warps 192 KB of an SM are on their way) and multiplies them by m16n8k16 products: S^T = K Q^T, O^T = V^T P^T.
 //
 // The weights P are rounded to bf16 for their product with V (2^-8 of each), V's type; l is the sum of the
 // rounded weights, so what is common to them cancels. m only moves when passed by 8, which bf16's range allows.
@@ -34,22 +35,21 @@ constexpr int kBlock = 16;  // tokens of a page
 constexpr int TM = 128;     // rows of a shared step
 constexpr int TK = 64;      // keys of a shared step
 constexpr int kStepPages = TK / kBlock;
-constexpr int kStages = 2;
-constexpr int kThreads = 192;
-constexpr int kWarps = kThreads / 32;
+constexpr int kWarps = 12;
+constexpr int kThreads = kWarps * 32;
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanGroups = 2048;  // groups whose state fits the plan's shared memory
-constexpr int kHeads = 8;          // query heads of one single-row segment (n of an m16n8k16 product)
-constexpr uint32_t kTmemCols = 256;
+constexpr int kPlanItems = 1024;  // rows, and groups, whose state fits the plan's shared memory
+constexpr int kHeads = 8;         // query heads of one single-row segment (n of an m16n8k16 product)
+constexpr uint32_t kTmemCols = 256;  // of a team
 constexpr uint32_t kAll = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f;
+typedef unsigned long long u64;
 
 // What the plan leaves for the others.
 struct Header {
-  int shared_ctas;   // CTAs of attend that take shared steps
-  int pieces;        // of shared steps
-  int64_t pages;     // (row, kv head, head group) pages of single rows
-  int64_t share;     // of them a warp takes
+  int shared_ctas;  // CTAs of attend that take shared steps
+  int64_t steps;    // of all of them
+  int64_t share;    // pages of single rows that a warp takes
 };
 struct Item {
   int pos, slot;  // pos -1: skipped
@@ -57,12 +57,21 @@ struct Item {
   int shared;     // its first pages, which the group's steps cover
 };
 struct Group {
-  int splits;  // pieces of one (tile, kv head)
-  int pages;   // shared
-  int rows;    // requests x query heads of a kv head
-  int leader;  // the request whose block table is read
-  int base;    // row (of the parts) of its first part
-  int piece;   // its first piece
+  int pages;      // shared
+  int start;      // its first row
+  int rows;       // rows x query heads of a kv head
+  int slot;       // of its first live row, whose block table is read
+  int64_t steps;  // of the groups before it
+  int base;       // (row, head)s of the groups before it
+};
+// Where a CTA of shared steps begins: unit = (kv head, two tiles) of a group, step of the unit; and how many it takes.
+struct Start {
+  int group, unit, step, count;
+};
+// Where a warp of single rows begins, in a place for each warp of attend, and its row.
+struct WarpStart {
+  int row, vhead, page, count;
+  Item it;
 };
 
 struct Params {
@@ -90,12 +99,17 @@ struct Params {
   // the workspace
   Header* header;
   Item* items;
-  int64_t* before;   // [num_items + 1]: pages of the rows before each
-  Group* groups;     // [num_groups + 1]
-  int2* state;       // [num_groups]: the plan's, where it does not fit shared memory
-  float* shared_o;   // parts of shared steps: per (group, kv head, split) [D / 8][rows][8]
+  int64_t* before;    // [num_items + 1]: own pages of the rows before each
+  Group* groups;      // [num_groups + 1]
+  int2* state;        // [num_groups] and
+  u64* leader;        // [num_groups]: the plan's, where they do not fit shared memory
+  Start* starts;      // [num_ctas]
+  WarpStart* warps;   // [num_ctas * kWarps]
+  int64_t team_rows;  // of all parts of one of the two teams
+  float* shared_o;    // parts of shared steps: part (unit, team, CTA) at team * team_rows + unit's row + 128 * CTA,
+                      // [D / 8][rows][8]
   float2* shared_ml;  // [rows of parts] {m, l}
-  float* single;     // parts of single rows: [segment + warp][stored_heads][D + 4], m and l behind o
+  float* single;      // parts of single rows: [segment + warp][stored_heads][D + 4], m and l behind o
   int32_t* status;
 };
 
@@ -111,171 +125,200 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 
 // ---------------------------------------------------------------------------------------------- plan
 
-// Sums of the threads' values before this thread's, and of all.
-template <typename T>
-__device__ __forceinline__ T scan(T mine, T& all, T* red) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  T x = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const T y = __shfl_up_sync(kAll, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 31) red[warp] = x;
-  __syncthreads();
-  T w = red[lane];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const T y = __shfl_up_sync(kAll, w, o);
-    if (lane >= o) w += y;
-  }
-  all = __shfl_sync(kAll, w, 31);
-  const T base = __shfl_sync(kAll, w, (warp + 31) & 31);
-  return (warp ? base : T(0)) + x - mine;
+struct Sums {
+  int64_t pages, steps, rows;
+};
+__device__ __forceinline__ Sums operator+(const Sums& a, const Sums& b) {
+  return {a.pages + b.pages, a.steps + b.steps, a.rows + b.rows};
+}
+__device__ __forceinline__ Sums shifted(const Sums& x, int o) {
+  return {__shfl_up_sync(kAll, x.pages, o), __shfl_up_sync(kAll, x.steps, o), __shfl_up_sync(kAll, x.rows, o)};
 }
 
+__device__ __forceinline__ int steps_of(int pages) { return (pages + kStepPages - 1) / kStepPages; }
+__device__ __forceinline__ int tiles_of(int items, int tile_items) { return (items + tile_items - 1) / tile_items; }
+
+// One CTA. Threads take a stretch of the rows and one of the groups each, nearly always one of either, so that
+// one scan serves both. 3 us of a call, most of it latencies: bounds and positions, the scan, the starts.
 __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
+  __shared__ int s_start[kPlanItems + 1];
+  __shared__ int2 s_state[kPlanItems];  // {fewest whole pages that a row of the group sees, its rows}
+  __shared__ u64 s_leader[kPlanItems];  // {first live row, its slot}
+  __shared__ int64_t s_before[kPlanItems + 1];
+  __shared__ Sums s_sum[32];
   pdl_trigger();
   pdl_wait();
-  __shared__ int64_t red[32];
-  __shared__ int s_start[kPlanGroups + 1];
-  __shared__ int2 s_state[kPlanGroups];  // {least whole pages that a row sees, live rows}
-  __shared__ int s_leader[kPlanGroups];
-  __shared__ int64_t s_share[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int ng = p.tile_items > 0 ? p.num_groups : 0;
-  const bool fits = ng <= kPlanGroups;
+  const bool fits = ng <= kPlanItems, fits_items = p.num_items <= kPlanItems;
   int2* state = fits ? s_state : p.state;
-  // (a group's leader is kept in the group's own place where shared memory does not hold it)
+  u64* leader = fits ? s_leader : p.leader;
+  const int first_pos = tid < p.num_items ? p.item_pos[tid] : -1, first_slot = tid < p.num_items ? p.item_slot[tid] : -1;
   bool bad = false;
   for (int g = tid; g < p.num_groups; g += kPlanThreads) {
     const int a = p.group_start[g], b = p.group_start[g + 1];
     bad |= a < 0 || b < a || b > p.num_items;
     if (g < ng) {
-      if (fits) s_start[g] = a, s_leader[g] = INT32_MAX;
-      else p.groups[g].leader = INT32_MAX;
+      if (fits) s_start[g] = a;
       if (fits && g + 1 == ng) s_start[ng] = b;
       state[g] = make_int2(INT32_MAX, 0);
+      leader[g] = ~0ull;
     }
   }
   if (__syncthreads_or(bad)) {
     if (tid == 0) set_error(p.status, CDB_ERR_INDEX);
     ng = 0;
   }
+  const int* start = fits ? s_start : p.group_start;
   // rows: their groups, and what those have in common
-  for (int i = tid; i < p.num_items; i += kPlanThreads) {
+  auto row = [&](int i) {
     Item it;
-    it.pos = p.item_pos[i];
-    it.slot = p.item_slot[i];
+    it.pos = i == tid ? first_pos : p.item_pos[i];
+    it.slot = i == tid ? first_slot : p.item_slot[i];
     it.group = -1;
     it.shared = 0;
-    if (it.pos >= 0 && (it.slot < 0 || it.slot >= p.bt_rows || it.pos / kBlock >= p.bt_width)) {
-      set_error(p.status, CDB_ERR_INDEX);
+    if (it.pos < 0 || it.slot < 0 || it.slot >= p.bt_rows || it.pos / kBlock >= p.bt_width) {
+      if (it.pos >= 0) set_error(p.status, CDB_ERR_INDEX);
       it.pos = -1;
     }
-    if (it.pos < 0) it.pos = -1;
-    if (ng > 0) {
-      const int* start = fits ? s_start : p.group_start;
-      int lo = -1, hi = ng + 1;  // the last bound at or before i
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (start[mid] <= i) lo = mid;
-        else hi = mid;
-      }
-      if (lo >= 0 && lo < ng && it.pos >= 0) {
-        it.group = lo;
-        atomicMin(&state[lo].x, (it.pos + 1) / kBlock);
-        atomicAdd(&state[lo].y, 1);
-        atomicMin(fits ? &s_leader[lo] : &p.groups[lo].leader, i);
-      }
+    int lo = -1, hi = ng + 1;  // the last bound at or before i
+    while (ng > 0 && hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (start[mid] <= i) lo = mid;
+      else hi = mid;
     }
-    p.items[i] = it;
+    if (lo >= 0 && lo < ng && it.pos >= 0) it.group = lo;
+    return it;
+  };
+  const int per_i = (p.num_items + kPlanThreads - 1) / kPlanThreads;
+  const int i0 = min(p.num_items, tid * per_i), i1 = min(p.num_items, i0 + per_i);
+  Item mine = {-1, -1, -1, 0};
+  for (int i = i0; i < i1; ++i) {
+    const Item it = row(i);
+    if (it.group >= 0) {
+      atomicMin(&state[it.group].x, (it.pos + 1) / kBlock);
+      atomicAdd(&state[it.group].y, 1);
+      atomicMin(&leader[it.group], (u64)i << 32 | (uint32_t)it.slot);
+    }
+    if (per_i == 1) mine = it;
+    else p.items[i] = it;
   }
   __syncthreads();
-  // groups: a stretch of them to a thread
   auto pages_of = [&](int g) {
     const int2 st = fits ? s_state[g] : __ldcg(p.state + g);  // (atomics pass the first cache by)
     return st.y >= 2 ? min(max(p.prefix_len[g], 0) / kBlock, st.x) : 0;  // one row alone has nothing to share
   };
-  auto bound = [&](int g) { return fits ? s_start[g] : p.group_start[g]; };
-  auto tiles_of = [&](int g) { return (bound(g + 1) - bound(g) + p.tile_items - 1) / p.tile_items; };
+  auto units_of = [&](int g) {
+    return (int64_t)((tiles_of(start[g + 1] - start[g], p.tile_items) + 1) / 2) * p.kv_heads;
+  };
   const int per_g = (ng + kPlanThreads - 1) / kPlanThreads;
   const int g0 = min(ng, tid * per_g), g1 = min(ng, g0 + per_g);
-  int64_t steps = 0, all_steps;
-  for (int g = g0; g < g1; ++g)
-    steps += (int64_t)tiles_of(g) * p.kv_heads * ((pages_of(g) + kStepPages - 1) / kStepPages);
-  scan(steps, all_steps, red);
-  // rows: their own pages
-  const int per_i = (p.num_items + kPlanThreads - 1) / kPlanThreads;
-  const int i0 = min(p.num_items, tid * per_i), i1 = min(p.num_items, i0 + per_i);
-  int64_t own = 0, all_own;
-  auto own_of = [&](int i) {
-    const Item it = p.items[i];
-    return it.pos < 0 ? 0 : it.pos / kBlock + 1 - (it.group >= 0 ? pages_of(it.group) : 0);
-  };
-  for (int i = i0; i < i1; ++i) own += own_of(i);
-  int64_t run = scan(own, all_own, red);
+  Sums sum = {0, 0, 0};
   for (int i = i0; i < i1; ++i) {
-    p.before[i] = run;
-    run += own_of(i);
-    if (p.items[i].group >= 0) p.items[i].shared = pages_of(p.items[i].group);
+    if (per_i > 1) mine = p.items[i];
+    if (mine.group >= 0) mine.shared = pages_of(mine.group);
+    if (mine.pos >= 0) sum.pages += mine.pos / kBlock + 1 - mine.shared;
+    p.items[i] = mine;
   }
-  if (tid == 0) p.before[p.num_items] = all_own;
-  // CTAs by the bytes of either kind of work, and shares of them
-  const int64_t pages = all_own * p.kv_heads * p.head_groups;
-  const int64_t shared_pages = all_steps * kStepPages;
-  int ctas = 0;
-  if (all_steps > 0)
-    ctas = pages == 0 ? p.num_ctas
-                      : (int)min((int64_t)p.num_ctas - 1, max((int64_t)1, quotient((int64_t)p.num_ctas * shared_pages, shared_pages + pages)));
-  // Pieces end with their (tile, kv head). The shortest of 32 shares, from an even one to 2.9 of it, whose pieces
-  // do not outnumber the CTAs; where none is, an even one, and CTAs take several.
-  const int64_t even = ctas ? quotient(all_steps + ctas - 1, ctas) : 1;
-  const int64_t mine = max((int64_t)1, even + even * warp * 2 / 33);
-  int64_t pieces = 0;
-  for (int g = lane; g < ng; g += 32) {
-    const int n = (pages_of(g) + kStepPages - 1) / kStepPages;
-    if (n) pieces += (int64_t)tiles_of(g) * p.kv_heads * quotient(n + mine - 1, mine);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) pieces += __shfl_xor_sync(kAll, pieces, o);
-  if (lane == 0) s_share[warp] = pieces <= ctas ? mine : INT64_MAX;
-  __syncthreads();
-  int64_t share = s_share[lane];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) share = min(share, __shfl_xor_sync(kAll, share, o));
-  if (share == INT64_MAX) share = max((int64_t)1, even);
-  int64_t np = 0, rows = 0, all_np, all_rows;
   for (int g = g0; g < g1; ++g) {
-    const int n = (pages_of(g) + kStepPages - 1) / kStepPages;
-    const int64_t splits = quotient(n + share - 1, share);
-    np += (int64_t)tiles_of(g) * p.kv_heads * splits;
-    rows += (int64_t)(bound(g + 1) - bound(g)) * p.heads_per_kv * p.kv_heads * splits;
+    sum.steps += units_of(g) * steps_of(pages_of(g));
+    sum.rows += (int64_t)(start[g + 1] - start[g]) * p.heads_per_kv * p.kv_heads;
   }
-  np = scan(np, all_np, red);
-  rows = scan(rows, all_rows, red);
+  // before this thread, and all
+  Sums x = sum, all;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const Sums y = shifted(x, o);
+    if (lane >= o) x = x + y;
+  }
+  if (lane == 31) s_sum[warp] = x;
+  __syncthreads();
+  {
+    Sums w = s_sum[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const Sums y = shifted(w, o);
+      if (lane >= o) w = w + y;
+    }
+    all = {__shfl_sync(kAll, w.pages, 31), __shfl_sync(kAll, w.steps, 31), __shfl_sync(kAll, w.rows, 31)};
+    const int from = (warp + 31) & 31;
+    const Sums base = {__shfl_sync(kAll, w.pages, from), __shfl_sync(kAll, w.steps, from), __shfl_sync(kAll, w.rows, from)};
+    if (warp > 0) x = x + base;
+  }
+  int64_t pages = x.pages - sum.pages, steps = x.steps - sum.steps, rows = x.rows - sum.rows;
+  for (int i = i0; i < i1; ++i) {
+    if (per_i > 1) mine = p.items[i];
+    p.before[i] = pages;
+    if (fits_items) s_before[i] = pages;
+    if (mine.pos >= 0) pages += mine.pos / kBlock + 1 - mine.shared;
+  }
   for (int g = g0; g < g1; ++g) {
     Group gr;
     gr.pages = pages_of(g);
-    const int n = (gr.pages + kStepPages - 1) / kStepPages;
-    gr.splits = (int)quotient(n + share - 1, share);
-    gr.rows = (bound(g + 1) - bound(g)) * p.heads_per_kv;
-    gr.leader = fits ? s_leader[g] : __ldcg(&p.groups[g].leader);
+    gr.start = start[g];
+    gr.rows = (start[g + 1] - start[g]) * p.heads_per_kv;
+    gr.slot = (int)(uint32_t)(fits ? s_leader[g] : __ldcg(p.leader + g));
+    gr.steps = steps;
     gr.base = (int)rows;
-    gr.piece = (int)np;
-    np += (int64_t)tiles_of(g) * p.kv_heads * gr.splits;
-    rows += (int64_t)gr.rows * p.kv_heads * gr.splits;
     p.groups[g] = gr;
+    steps += units_of(g) * steps_of(gr.pages);
+    rows += (int64_t)gr.rows * p.kv_heads;
   }
+  // CTAs by the bytes of either kind of work
+  const int64_t vpages = all.pages * p.kv_heads * p.head_groups, shared_pages = all.steps * kStepPages;
+  int ctas = 0;
+  if (all.steps > 0)
+    ctas = vpages == 0 ? p.num_ctas
+                       : (int)min((int64_t)p.num_ctas - 1,
+                                  max((int64_t)1, quotient((int64_t)p.num_ctas * shared_pages, shared_pages + vpages)));
+  ctas = (int)min((int64_t)ctas, all.steps);  // each of them has one
+  const int64_t n_warps = (int64_t)(p.num_ctas - ctas) * kWarps;
+  const int64_t share = n_warps ? max((int64_t)1, quotient(vpages + n_warps - 1, n_warps)) : 1;
   if (tid == 0) {
+    p.before[p.num_items] = all.pages;
+    if (fits_items) s_before[p.num_items] = all.pages;
     Header h;
     h.shared_ctas = ctas;
-    h.pieces = (int)all_np;
-    h.pages = pages;
-    const int64_t warps = (int64_t)(p.num_ctas - ctas) * kWarps;
-    h.share = max((int64_t)1, warps ? quotient(pages + warps - 1, warps) : 1);
+    h.steps = all.steps;
+    h.share = share;
     *p.header = h;
+  }
+  __syncthreads();  // items, groups and sums are read across threads from here on
+  if (tid < ctas) {
+    const int64_t begin = quotient(all.steps * tid, ctas), end = quotient(all.steps * (tid + 1), ctas);
+    Start st = {0, 0, 0, (int)(end - begin)};
+    int lo = 0, hi = ng;  // the last group that begins at or before `begin`
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (p.groups[mid].steps <= begin) lo = mid;
+      else hi = mid;
+    }
+    st.group = lo;
+    const int n = steps_of(p.groups[lo].pages);
+    const int64_t at = begin - p.groups[lo].steps;
+    st.unit = n ? (int)quotient(at, n) : 0;
+    st.step = n ? (int)(at - (int64_t)st.unit * n) : 0;
+    p.starts[tid] = st;
+  }
+  const int vheads = p.kv_heads * p.head_groups;
+  for (int w = tid; w < n_warps; w += kPlanThreads) {
+    const int64_t begin = w * share, end = min(begin + share, vpages);
+    WarpStart ws = {0, 0, 0, (int)max((int64_t)0, min(end - begin, (int64_t)INT32_MAX)), {-1, -1, -1, 0}};
+    if (begin < end) {
+      int lo = 0, hi = p.num_items;  // the last row that begins at or before `begin`, so one that has pages
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if ((fits_items ? s_before[mid] : p.before[mid]) * vheads <= begin) lo = mid;
+        else hi = mid;
+      }
+      ws.row = lo;
+      ws.it = p.items[lo];
+      const int own = ws.it.pos / kBlock + 1 - ws.it.shared;
+      const int64_t at = begin - (fits_items ? s_before[lo] : p.before[lo]) * vheads;
+      ws.vhead = (int)quotient(at, own);
+      ws.page = ws.it.shared + (int)(at - (int64_t)ws.vhead * own);
+    }
+    p.warps[ctas * kWarps + w] = ws;
   }
 }
 
@@ -284,26 +327,40 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
 template <int D>
 struct Tile {
   static constexpr int ATOMS = (D + 63) / 64;  // 128-byte swizzle atoms of a row of D (96: the second one's end is zero)
-  static constexpr int OFF_K = ATOMS * TM * 128;                       // behind q [ATOMS][128][64]
-  static constexpr int STAGE = ATOMS * TK * 128;                       // K or V of a step, [ATOMS][64][64]
-  static constexpr int OFF_V = OFF_K + kStages * STAGE;
-  static constexpr int OFF_BAR = OFF_V + kStages * STAGE;
-  static constexpr int SMEM = OFF_BAR + 256;
-  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
+  static constexpr int STAGES = D == 64 ? 12 : 5;  // steps in the ring
+  static constexpr int STAGE = ATOMS * TK * 128;   // K or V of a step, [ATOMS][64][64]
+  static constexpr int Q = ATOMS * TM * 128;       // q of a tile, [ATOMS][128][64]
+  static constexpr int OFF_K = 2 * Q;
+  static constexpr int OFF_V = OFF_K + STAGES * STAGE;
+  static constexpr int OFF_BAR = OFF_V + STAGES * STAGE;
+  static constexpr int SMEM = OFF_BAR + 640;
+  static_assert(SMEM <= 227 * 1024, "shared memory of an SM");
+  // single rows
+  static constexpr int BOX = kBlock * 128;        // 64 columns of a page
+  static constexpr int PAGE = 2 * ATOMS * BOX;    // K and V of a page
+  static constexpr int SLOTS = D == 64 ? 4 : 2;   // pages in a warp's ring
+  static_assert(kWarps * SLOTS * PAGE <= OFF_BAR, "rings of all warps");
 };
 
+constexpr int kMaxStages = 12;
+constexpr int kMissing = 16;  // steps whose missing pages are kept: more than the ring and three steps of either team
+
 struct Shared {
-  uint64_t kfull[kStages], vfull[kStages];  // a step's K, V have landed
-  uint64_t qfull;                           // q of a piece written
-  uint64_t sfull[2];                        // S done (and K's place free), and the step's pages known
-  uint64_t pfull[2];                        // weights written
-  uint64_t odone[2];                        // O product done (V's and S's places free)
-  uint64_t drain;
-  int missing[4];                           // a step's pages that do not exist
+  uint64_t kfull[kMaxStages], vfull[kMaxStages];  // a step's K, V have landed
+  uint64_t kfree[kMaxStages], vfree[kMaxStages];  // and both teams have multiplied (or passed) it
+  uint64_t qfull, qfree;                          // q of a piece written, and not needed any more
+  struct Team {
+    uint64_t sfull[2];  // S done, and the step's pages known
+    uint64_t pfull[2];  // weights written
+    uint64_t odone[2];  // O product done (S's place free)
+    uint64_t drain;
+  } team[2];
+  int missing[kMissing];  // a step's pages that do not exist
   uint32_t tmem;
   int abort;
 };
-static_assert(sizeof(Shared) <= 256, "room behind the tiles");
+static_assert(sizeof(Shared) <= 640, "room behind the tiles");
+static_assert(kMissing > kMaxStages + 3, "see Shared");
 
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int32_t* status, volatile int* abort) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -325,245 +382,259 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
       : "memory");
 }
 
-// A piece of shared steps.
-struct Piece {
-  int group, tile, kvh, split;
-  int first, steps;  // its steps of the group's
-  int rows;          // of the tile
-  int pages;         // of the group
-  int leader;
-  int64_t part;  // row of the parts where its (group, kv head, split) begins
+// The CTA's way through its share of the steps, one unit at a time.
+struct Walk {
+  Start at;
+  Group g;
+  int kvh, tile;  // the first of the unit's tiles
+  bool both;      // it has two, one to a team
+  int steps;      // of this unit that the CTA takes, from step at.step on
+  __device__ __forceinline__ int rows(const Params& p, int team) const {
+    const int full = p.tile_items * p.heads_per_kv;
+    return min(full, g.rows - (both ? tile + team : tile) * full);
+  }
+  __device__ __forceinline__ void look(const Params& p) {
+    const int tiles = tiles_of(g.rows, p.tile_items * p.heads_per_kv), pairs = (tiles + 1) / 2;
+    kvh = at.unit / pairs;
+    tile = 2 * (at.unit - kvh * pairs);
+    both = tile + 1 < tiles;
+    steps = min(at.count, steps_of(g.pages) - at.step);
+  }
+  __device__ __forceinline__ void begin(const Params& p, const Start& s) {
+    at = s;
+    if (at.count <= 0) return;
+    g = p.groups[at.group];
+    look(p);
+  }
+  __device__ __forceinline__ bool on() const { return at.count > 0; }
+  __device__ __forceinline__ void next(const Params& p) {
+    at.count -= steps;
+    if (at.count <= 0) return;
+    at.step = 0;
+    ++at.unit;
+    if (at.unit == (tiles_of(g.rows, p.tile_items * p.heads_per_kv) + 1) / 2 * p.kv_heads) {
+      at.unit = 0;
+      do g = p.groups[++at.group];
+      while (g.pages == 0);
+    }
+    look(p);
+  }
 };
 
-__device__ __forceinline__ Piece find_piece(const Params& p, int index) {
-  // the last group that begins at or before it (those without pieces begin where their successor does)
-  const int lane = threadIdx.x & 31;
-  int lo = 0, n = p.num_groups;
-  while (n > 1) {
-    const int stride = (n + 31) / 32, at = lo + lane * stride;
-    const unsigned hit = __ballot_sync(kAll, at < lo + n && p.groups[at].piece <= index);
-    const int k = 31 - __clz(hit);
-    n = min(stride, n - k * stride);
-    lo += k * stride;
-  }
-  const Group g = p.groups[lo];
-  Piece me;
-  const int local = index - g.piece, per_head = g.splits;
-  const int unit = local / per_head;
-  me.split = local - unit * per_head;
-  me.tile = unit / p.kv_heads;
-  me.kvh = unit - me.tile * p.kv_heads;
-  me.group = lo;
-  const int n_steps = (g.pages + kStepPages - 1) / kStepPages;
-  me.first = (int)((int64_t)n_steps * me.split / per_head);
-  me.steps = (int)((int64_t)n_steps * (me.split + 1) / per_head) - me.first;
-  me.rows = min(p.tile_items * p.heads_per_kv, g.rows - me.tile * p.tile_items * p.heads_per_kv);
-  me.pages = g.pages;
-  me.leader = g.leader;
-  me.part = g.base + ((int64_t)me.kvh * per_head + me.split) * g.rows;
-  return me;
+// (row, head)s of the parts before a unit's: one team's parts of the units in their order, as long as their first tiles.
+__device__ __forceinline__ int64_t unit_base(const Params& p, const Group& g, int kvh, int tile) {
+  const int full = p.tile_items * p.heads_per_kv, tiles = tiles_of(g.rows, full), pairs = (tiles + 1) / 2;
+  const int of_head = (pairs - 1) * full + min(full, g.rows - 2 * (pairs - 1) * full);
+  return g.base + (int64_t)kvh * of_head + (int64_t)(tile / 2) * full;
 }
 
 template <int D>
-__device__ __forceinline__ void shared_steps(const CUtensorMap& map, const Params& p, const Header& h, uint8_t* smem) {
+__device__ __forceinline__ void shared_steps(const CUtensorMap& map, const Params& p, const Start& start, uint8_t* smem,
+                                             Shared& sh) {
   using T = Tile<D>;
+  constexpr int R = T::STAGES;
   constexpr uint32_t kBf16 = (1u << 4) | (1u << 7) | (1u << 10);  // fp32 accumulators, bf16 operands
   constexpr uint32_t kIdescS = kBf16 | ((uint32_t)(TK >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
   constexpr uint32_t kIdescO = kBf16 | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
-  Shared& sh = *reinterpret_cast<Shared*>(smem + T::OFF_BAR);
   const uint32_t base = smem_u32(smem);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&sh.kfull[i], 1);
-      mbar_init(&sh.vfull[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.sfull[i], 2);
-      mbar_init(&sh.pfull[i], TM);
-      mbar_init(&sh.odone[i], 1);
-    }
-    mbar_init(&sh.qfull, TM);
-    mbar_init(&sh.drain, 1);
-    sh.abort = (base & 1023u) != 0u;  // the swizzle counts on it
-    if (sh.abort) set_error(p.status, CDB_ERR_INVALID_ARGUMENT);
-    fence_barrier_init();
-  }
-  if (warp == 5) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
-                 "r"(kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  fence_before();
-  __syncthreads();
-  fence_after();
-  // Only now may the next kernel's CTAs come: one that holds tensor memory and waits for this kernel could otherwise
-  // be what the allocation above waits for.
-  pdl_trigger();
-  const uint32_t tmem = sh.tmem;  // S: two buffers of 64 columns; O: 128 columns on
-  const uint32_t tmem_o = tmem + 2 * TK;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort = &sh.abort;
+  Walk w;
 
-  // `t` counts the steps of all of the CTA's pieces, `c` the pieces: every barrier's phases follow from them.
-  if (warp == 4) {
+  // `t` counts the CTA's steps: step t lies in slot t % R of the ring. `j` counts a team's: its S lies in buffer j & 1. Every
+  // barrier's phase follows.
+  if (warp == 8) {
     // ------------------------------------------------------------ pages
     int t = 0;
     bool ok = true;
-    for (int index = blockIdx.x; index < h.pieces && ok; index += h.shared_ctas) {
-      const Piece me = find_piece(p, index);
-      const int32_t* bt = p.block_table + (int64_t)p.items[me.leader].slot * p.bt_stride;
-      // lane: page (lane & 3) of the step, columns 64 * ((lane >> 2) & 1); lanes 0..7 of K, 16..23 of V
-      const int page_of = lane & 3, atom = (lane >> 2) & 1;
-      const bool loads = (lane & 8) == 0 && atom < T::ATOMS;
+    // lane: page (lane & 3) of the step, columns 64 * ((lane >> 2) & 1); lanes 0..7 of K, 16..23 of V
+    const int page_of = lane & 3, atom = (lane >> 2) & 1;
+    const bool loads = (lane & 8) == 0 && atom < T::ATOMS;
+    for (w.begin(p, start); w.on() && ok; w.next(p)) {
+      const int32_t* bt = p.block_table + (int64_t)w.g.slot * p.bt_stride;
       auto fetch = [&](int n) {
-        const int page = (me.first + n) * kStepPages + page_of;
-        return n < me.steps && page < me.pages ? bt[page] : INT32_MIN;
+        const int page = (w.at.step + n) * kStepPages + page_of;
+        return n < w.steps && page < w.g.pages ? bt[page] : INT32_MIN;
       };
-      int id = fetch(0);
-      for (int n = 0; n < me.steps; ++n, ++t) {
-        const int next = fetch(n + 1);
-        const int stage = t % kStages;
+      int id = fetch(0), next = fetch(1);
+      for (int n = 0; n < w.steps; ++n, ++t) {
+        const int after = fetch(n + 2), slot = t % R;
         const bool have = id >= 0 && id < p.blocks;
         const unsigned gone = __ballot_sync(kAll, !have) & 15u;
         if (lane < kStepPages && !have && id != INT32_MIN) set_error(p.status, CDB_ERR_INDEX);
-        // behind the cache's rows a box comes as zeros
-        const int row = have ? id * kBlock : 2 * (int)p.kv_rows;
-        if (t >= kStages) ok = __all_sync(kAll, wait_for(&sh.sfull[t & 1], ((t - 2) >> 1) & 1, p.status, abort));
+        const int row = have ? id * kBlock : 2 * (int)p.kv_rows;  // behind the cache's rows a box comes as zeros
+        const uint32_t freed = (t / R + 1) & 1;                   // by step t - R
+        const uint32_t at = slot * T::STAGE + atom * (TK * 128) + page_of * (kBlock * 128);
+        if (t >= R) ok = __all_sync(kAll, wait_for(&sh.kfree[slot], freed, p.status, abort));
         if (!ok) break;
-        const uint32_t at = base + (lane < 16 ? T::OFF_K : T::OFF_V) + stage * T::STAGE + atom * (TK * 128) + page_of * (kBlock * 128);
         if (lane == 0) {
-          sh.missing[t & 3] = (int)gone;
-          mbar_arrive_expect_tx(&sh.kfull[stage], T::STAGE);
+          sh.missing[t % kMissing] = (int)gone;
+          mbar_arrive_expect_tx(&sh.kfull[slot], T::STAGE);
         }
         __syncwarp();
-        if (loads && lane < 16) load_box(at, &map, atom * 64, me.kvh, row, smem_u32(&sh.kfull[stage]));
-        if (t >= kStages) ok = __all_sync(kAll, wait_for(&sh.odone[t & 1], ((t - 2) >> 1) & 1, p.status, abort));
+        if (loads && lane < 16) load_box(base + T::OFF_K + at, &map, atom * 64, w.kvh, row, smem_u32(&sh.kfull[slot]));
+        if (t >= R) ok = __all_sync(kAll, wait_for(&sh.vfree[slot], freed, p.status, abort));
         if (!ok) {
-          if (lane == 0) mbar_wait(&sh.kfull[stage], (t / kStages) & 1, p.status);
+          if (lane == 0) mbar_wait(&sh.kfull[slot], (t / R) & 1, p.status);
           __syncwarp();
           break;
         }
-        if (lane == 16) mbar_arrive_expect_tx(&sh.vfull[stage], T::STAGE);
+        if (lane == 16) mbar_arrive_expect_tx(&sh.vfull[slot], T::STAGE);
         __syncwarp();
         if (loads && lane >= 16)
-          load_box(at, &map, atom * 64, me.kvh, have ? row + (int)p.kv_rows : row, smem_u32(&sh.vfull[stage]));
+          load_box(base + T::OFF_V + at, &map, atom * 64, w.kvh, have ? row + (int)p.kv_rows : row,
+                   smem_u32(&sh.vfull[slot]));
         id = next;
+        next = after;
       }
     }
     // nothing may be on its way when the CTA ends
-    for (int j = max(0, t - kStages); j < t; ++j) {
-      mbar_wait(&sh.kfull[j % kStages], (j / kStages) & 1, p.status);
-      mbar_wait(&sh.vfull[j % kStages], (j / kStages) & 1, p.status);
+    for (int j = max(0, t - R); j < t; ++j) {
+      mbar_wait(&sh.kfull[j % R], (j / R) & 1, p.status);
+      mbar_wait(&sh.vfull[j % R], (j / R) & 1, p.status);
     }
-  } else if (warp == 5) {
+  } else if (warp == 9 || warp == 10) {
     // ------------------------------------------------------------ products
-    int t = 0, c = 0;
+    const int team = warp - 9;
+    Shared::Team& tm = sh.team[team];
+    const uint32_t tmem = sh.tmem + team * kTmemCols, tmem_o = tmem + 2 * TK;
+    int t = 0, j = 0, c = 0;
     bool ok = true;
-    auto weigh = [&](int j, bool add) {  // O (+)= P V of step j
-      ok = ok && wait_for(&sh.vfull[j % kStages], (j / kStages) & 1, p.status, abort) &&
-           wait_for(&sh.pfull[j & 1], (j >> 1) & 1, p.status, abort);
+    auto weigh = [&](int step, int buffer, bool add) {  // O (+)= P V of a step, the team's last one
+      ok = ok && wait_for(&sh.vfull[step % R], (step / R) & 1, p.status, abort) &&
+           wait_for(&tm.pfull[buffer & 1], (buffer >> 1) & 1, p.status, abort);
       if (!ok) return;
       fence_after();
 #pragma unroll
       for (int kk = 0; kk < TK / 16; ++kk)
-        product_tmem(tmem_o, tmem + (j & 1) * TK + kk * 8,
-                     operand(base + T::OFF_V + (j % kStages) * T::STAGE + kk * 2048, TK * 128), kIdescO, add || kk > 0);
-      commit(&sh.odone[j & 1]);
+        product_tmem(tmem_o, tmem + (buffer & 1) * TK + kk * 8,
+                     operand(base + T::OFF_V + (step % R) * T::STAGE + kk * 2048, TK * 128), kIdescO, add || kk > 0);
+      commit(&tm.odone[buffer & 1]);
+      commit(&sh.vfree[step % R]);
     };
-    for (int index = blockIdx.x; index < h.pieces; index += h.shared_ctas, ++c) {
-      const Piece me = find_piece(p, index);
-      if (lane == 0) {
-        for (int n = 0; n < me.steps && ok; ++n, ++t) {
-          ok = wait_for(&sh.kfull[t % kStages], (t / kStages) & 1, p.status, abort);
-          if (n == 0) ok = ok && wait_for(&sh.qfull, c & 1, p.status, abort);
-          if (t >= 2) ok = ok && wait_for(&sh.odone[t & 1], ((t - 2) >> 1) & 1, p.status, abort);
+    for (w.begin(p, start); w.on(); w.next(p), ++c) {
+      if (lane == 0 && ok) {
+        ok = wait_for(&sh.qfull, c & 1, p.status, abort);
+        const uint32_t q = base + (w.both ? team * T::Q : 0);
+        int done = -1;  // the team's last step, whose weights are still to come
+        bool add = false;
+        for (const int end = t + w.steps; t < end && ok; ++t) {
+          const int slot = t % R;
+          ok = wait_for(&sh.kfull[slot], (t / R) & 1, p.status, abort);
+          if (!ok) break;
+          if (!w.both && (t & 1) != team) {  // the other team's
+            mbar_arrive(&sh.kfree[slot]);
+            ok = wait_for(&sh.vfull[slot], (t / R) & 1, p.status, abort);
+            if (ok) mbar_arrive(&sh.vfree[slot]);
+            continue;
+          }
+          if (j >= 2) ok = wait_for(&tm.odone[j & 1], ((j - 2) >> 1) & 1, p.status, abort);
           if (!ok) break;
           fence_after();
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            product(tmem + (t & 1) * TK, operand(base + (kk >> 2) * (TM * 128) + (kk & 3) * 32),
-                    operand(base + T::OFF_K + (t % kStages) * T::STAGE + (kk >> 2) * (TK * 128) + (kk & 3) * 32), kIdescS,
-                    kk > 0);
-          commit(&sh.sfull[t & 1]);
-          mbar_arrive(&sh.sfull[t & 1]);  // releases `missing` to whoever waits for S
-          if (n > 0) weigh(t - 1, n > 1);
+            product(tmem + (j & 1) * TK, operand(q + (kk >> 2) * (TM * 128) + (kk & 3) * 32),
+                    operand(base + T::OFF_K + slot * T::STAGE + (kk >> 2) * (TK * 128) + (kk & 3) * 32), kIdescS, kk > 0);
+          commit(&tm.sfull[j & 1]);
+          commit(&sh.kfree[slot]);
+          mbar_arrive(&tm.sfull[j & 1]);  // releases `missing` to whoever waits for S
+          if (done >= 0) {
+            weigh(done, j - 1, add);
+            add = true;
+          }
+          done = t;
+          ++j;
         }
-        if (ok) weigh(t - 1, me.steps > 1);
+        if (ok && done >= 0) weigh(done, j - 1, add);
       }
       __syncwarp();
     }
     if (lane == 0) {  // on every path: no product may run when the tensor memory is freed
-      commit(&sh.drain);
-      mbar_wait(&sh.drain, 0, p.status);
+      commit(&tm.drain);
+      mbar_wait(&tm.drain, 0, p.status);
     }
     __syncwarp();
-  } else {
+  } else if (warp < 8) {
     // ------------------------------------------------------------ softmax
-    const int r = tid;  // row of the tile, and tensor-memory lane
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    int t = 0;
+    const int team = warp >> 2, quarter = warp & 3;  // of the tensor memory's lanes
+    const int r = quarter * 32 + lane;               // row of the tile, and tensor-memory lane
+    Shared::Team& tm = sh.team[team];
+    const uint32_t tmem = sh.tmem + team * kTmemCols + ((uint32_t)(quarter * 32) << 16), tmem_o = tmem + 2 * TK;
+    int t = 0, j = 0, c = 0;
     bool ok = true;
-    for (int index = blockIdx.x; index < h.pieces && ok; index += h.shared_ctas) {
-      const Piece me = find_piece(p, index);
-      const bool mine = r < me.rows;
-      const bool rows_here = warp * 32 < me.rows;  // a warp without rows only keeps the barriers going
+    for (w.begin(p, start); w.on() && ok; w.next(p)) {
+      const int rows = w.rows(p, team);
+      const bool mine = r < rows;
+      const bool rows_here = quarter * 32 < rows;  // a warp without rows only keeps the barriers going
+      if (c > 0) {  // both teams are done with the last piece's q
+        mbar_arrive(&sh.qfree);
+        ok = __all_sync(kAll, wait_for(&sh.qfree, (c - 1) & 1, p.status, abort));
+        if (!ok) break;
+      }
+      ++c;
       {
-        const int local = r / p.heads_per_kv;
-        const int first = p.group_start[me.group] + me.tile * p.tile_items;
-        const __nv_bfloat16* src = p.q + (int64_t)(first + (mine ? local : 0)) * p.q_stride +
-                                   (int64_t)(me.kvh * p.heads_per_kv + (mine ? r - local * p.heads_per_kv : 0)) * D;
-        uint4 w[D / 8];
+        const int local = mine ? r / p.heads_per_kv : 0, tile = w.tile + (w.both ? team : 0);
+        const __nv_bfloat16* src = p.q + (int64_t)(w.g.start + tile * p.tile_items + local) * p.q_stride +
+                                   (int64_t)(w.kvh * p.heads_per_kv + (mine ? r - local * p.heads_per_kv : 0)) * D;
+        uint8_t* dst = smem + (w.both ? team * T::Q : 0) + r * 128;
+#pragma unroll 1
+        for (int half = w.both ? 0 : team; half < (w.both ? 2 : team + 1); ++half) {  // one tile: a half to each team
+          uint4 x[D / 16];
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-          w[i] = mine ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0u, 0u, 0u, 0u);
+          for (int i = 0; i < D / 16; ++i)
+            x[i] = mine ? *reinterpret_cast<const uint4*>(src + (half * (D / 16) + i) * 8) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-          *reinterpret_cast<uint4*>(smem + (i >> 3) * (TM * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = w[i];
+          for (int i = 0; i < D / 16; ++i) {
+            const int ch = half * (D / 16) + i;
+            *reinterpret_cast<uint4*>(dst + (ch >> 3) * (TM * 128) + (((ch & 7) ^ (r & 7)) << 4)) = x[i];
+          }
+        }
       }
       fence_proxy_async_shared();
       mbar_arrive(&sh.qfull);
       float m = -INFINITY, l = 0.f;
-      for (int n = 0; n < me.steps; ++n, ++t) {
-        ok = __all_sync(kAll, wait_for(&sh.sfull[t & 1], (t >> 1) & 1, p.status, abort));
+      bool some = false;
+      for (const int end = t + w.steps; t < end; ++t) {
+        if (!w.both && (t & 1) != team) continue;
+        ok = __all_sync(kAll, wait_for(&tm.sfull[j & 1], (j >> 1) & 1, p.status, abort));
         if (!ok) break;
         if (rows_here) {
           fence_after();
           uint32_t s[TK];
-          tmem_load(tmem + lanes + (t & 1) * TK, s);
-          tmem_load(tmem + lanes + (t & 1) * TK + 32, s + 32);
+          tmem_load(tmem + (j & 1) * TK, s);
+          tmem_load(tmem + (j & 1) * TK + 32, s + 32);
           wait_loads(s);
           wait_loads(s + 32);
-          const int gone = sh.missing[t & 3];
+          const int gone = sh.missing[t % kMissing];
           if (gone) {
 #pragma unroll
             for (int k = 0; k < TK; ++k)
               if ((gone >> (k / kBlock)) & 1) s[k] = 0xff800000u;
           }
-          float t0 = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
-          float t1 = fmaxf(__uint_as_float(s[2]), __uint_as_float(s[3]));
+          float x0 = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+          float x1 = fmaxf(__uint_as_float(s[2]), __uint_as_float(s[3]));
 #pragma unroll
           for (int k = 4; k < TK; k += 4) {  // (three operands to a maximum)
-            t0 = fmaxf(fmaxf(t0, __uint_as_float(s[k])), __uint_as_float(s[k + 1]));
-            t1 = fmaxf(fmaxf(t1, __uint_as_float(s[k + 2])), __uint_as_float(s[k + 3]));
+            x0 = fmaxf(fmaxf(x0, __uint_as_float(s[k])), __uint_as_float(s[k + 1]));
+            x1 = fmaxf(fmaxf(x1, __uint_as_float(s[k + 2])), __uint_as_float(s[k + 3]));
           }
-          const float mx = fmaxf(t0, t1) * p.scale_log2;
+          const float mx = fmaxf(x0, x1) * p.scale_log2;
           const bool up = mx > m + 8.f;
           if (__any_sync(kAll, up)) {
             const float to = up ? mx : m;
-            if (n > 0) {  // the products so far have to be in O
-              ok = __all_sync(kAll, wait_for(&sh.odone[(t - 1) & 1], ((t - 1) >> 1) & 1, p.status, abort));
+            if (some) {  // the products so far have to be in O
+              ok = __all_sync(kAll, wait_for(&tm.odone[(j - 1) & 1], ((j - 1) >> 1) & 1, p.status, abort));
               if (!ok) break;
               const float down = m == -INFINITY ? (up ? 0.f : 1.f) : ex2(m - to);
               l *= down;
               fence_after();
 #pragma unroll 1
-              for (int c = 0; c < D; c += 16) {
+              for (int d = 0; d < D; d += 16) {
                 uint32_t o[16];
-                tmem_load16(tmem_o + lanes + c, o);
+                tmem_load16(tmem_o + d, o);
 #pragma unroll
                 for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
-                tmem_store16(tmem_o + lanes + c, o);
+                tmem_store16(tmem_o + d, o);
               }
               wait_stores();
             }
@@ -573,69 +644,56 @@ __device__ __forceinline__ void shared_steps(const CUtensorMap& map, const Param
           float sum = 0.f, more = 0.f;
 #pragma unroll
           for (int b = 0; b < TK / 16; ++b) {
-            uint32_t w[8];
+            uint32_t x[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              w[k] = pack_bf16x2(ex2(fmaf(__uint_as_float(s[b * 16 + 2 * k]), p.scale_log2, off)),
+              x[k] = pack_bf16x2(ex2(fmaf(__uint_as_float(s[b * 16 + 2 * k]), p.scale_log2, off)),
                                  ex2(fmaf(__uint_as_float(s[b * 16 + 2 * k + 1]), p.scale_log2, off)));
-              sum += bf16lo(w[k]);
-              more += bf16hi(w[k]);
+              sum += bf16lo(x[k]);
+              more += bf16hi(x[k]);
             }
-            tmem_store8(tmem + lanes + (t & 1) * TK + b * 8, w);
+            tmem_store8(tmem + (j & 1) * TK + b * 8, x);
           }
           l += sum + more;
           wait_stores();
         }
         fence_before();
-        mbar_arrive(&sh.pfull[t & 1]);
+        mbar_arrive(&tm.pfull[j & 1]);
+        some = true;
+        ++j;
       }
       if (!ok) break;
-      ok = __all_sync(kAll, wait_for(&sh.odone[(t - 1) & 1], ((t - 1) >> 1) & 1, p.status, abort));
+      if (some) ok = __all_sync(kAll, wait_for(&tm.odone[(j - 1) & 1], ((j - 1) >> 1) & 1, p.status, abort));
       if (!ok) break;
       if (rows_here) {
-        fence_after();
-        const int64_t all = p.groups[me.group].rows;
-        const int64_t at = (int64_t)me.tile * p.tile_items * p.heads_per_kv + r;
-        float* dst = p.shared_o + me.part * D + at * 8;
+        const int64_t part =
+            team * p.team_rows + unit_base(p, w.g, w.kvh, w.tile) + (int64_t)blockIdx.x * TM;
+        if (some) {
+          fence_after();
+          float* dst = p.shared_o + part * D + r * 8;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_load(tmem_o + lanes + c, o);
-          wait_loads(o);
-          if (mine) {
+          for (int d = 0; d < D; d += 32) {
+            uint32_t o[32];
+            tmem_load(tmem_o + d, o);
+            wait_loads(o);
+            if (mine) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 4)
-              __stcg(reinterpret_cast<float4*>(dst + ((c + k) / 8) * all * 8 + (k & 4)),
-                     make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]),
-                                 __uint_as_float(o[k + 3])));
+              for (int k = 0; k < 32; k += 4)
+                __stcg(reinterpret_cast<float4*>(dst + (int64_t)((d + k) / 8) * rows * 8 + (k & 4)),
+                       make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]),
+                                   __uint_as_float(o[k + 3])));
+            }
           }
+          fence_before();
         }
-        if (mine) __stcg(p.shared_ml + me.part + at, make_float2(m, l));
-        fence_before();
+        if (mine) __stcg(p.shared_ml + part + r, make_float2(m, l));  // (-inf, 0) where the team had no step
       }
     }
   }
-  fence_before();
-  __syncthreads();
-  fence_after();
-  if (warp == 5)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
 // ---------------------------------------------------------------- pages of single rows
 
-__device__ __forceinline__ uint4 load16(const __nv_bfloat16* a) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(a));
-  return v;
-}
-__device__ __forceinline__ uint2 load8(const __nv_bfloat16* a) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(a));
-  return v;
-}
 // D += A B on bf16 operands, fp32 accumulators (m16n8k16).
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -649,6 +707,20 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
+}
+
+// Four 8 x 8 matrices of 16-bit values, a row to each lane's address (quarter warps in turn).
+__device__ __forceinline__ void load_matrices(uint32_t at, uint32_t (&m)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(m[0]), "=r"(m[1]), "=r"(m[2]), "=r"(m[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void load_transposed(uint32_t at, uint32_t (&m)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(m[0]), "=r"(m[1]), "=r"(m[2]), "=r"(m[3])
+               : "r"(at)
+               : "memory");
 }
 
 // A place in the stream: page `page` of row `row`, head group `grp` of kv head `kvh`.
@@ -674,143 +746,116 @@ __device__ __forceinline__ void advance(const Params& p, Cursor& c) {
 }
 
 template <int D>
-struct Page {
-  uint4 k[2][D / 32];  // tokens g, g + 8: dims i * 32 + t * 8
-  uint4 v[4][D / 64];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9: dims i * 64 + g * 8
-  uint2 w[4];          // of a head of 96: dims 64 + g * 4
-};
-
-template <int D>
-__device__ __forceinline__ void load_k(const Params& p, int64_t row, int kvh, Page<D>& x) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-      x.k[j][i] = load16(p.keys + ((row + g + 8 * j) * p.kv_heads + kvh) * D + i * 32 + t * 8);
-}
-template <int D>
-__device__ __forceinline__ void load_v(const Params& p, int64_t row, int kvh, Page<D>& x) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const __nv_bfloat16* src = p.keys + ((p.kv_rows + row + 2 * t + (j & 1) + 8 * (j >> 1)) * p.kv_heads + kvh) * D;
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) x.v[j][i] = load16(src + i * 64 + g * 8);
-    if (D == 96) x.w[j] = load8(src + 64 + g * 4);
-  }
-}
-
-template <int D>
-__device__ __forceinline__ void single_rows(const Params& p, const Header& h) {
-  pdl_trigger();
+__device__ __forceinline__ void single_rows(const CUtensorMap& map, const Params& p, const Header& h, uint8_t* smem,
+                                            uint64_t* bars) {
+  using T = Tile<D>;
   constexpr int MT = D / 16;
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int64_t warp = (int64_t)(blockIdx.x - h.shared_ctas) * kWarps + (threadIdx.x >> 5);
-  const int64_t begin = warp * h.share, end = min(begin + h.share, h.pages);
-  if (begin >= end) return;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, in_cta = threadIdx.x >> 5;
+  const int64_t warp = (int64_t)((int)blockIdx.x - h.shared_ctas) * kWarps + in_cta;
+  const WarpStart start = p.warps[(int64_t)blockIdx.x * kWarps + in_cta];
+  if (start.count <= 0) return;
+  uint64_t* full = bars + in_cta * T::SLOTS;  // a page has landed
+  if (lane == 0) {
+    for (int i = 0; i < T::SLOTS; ++i) mbar_init(&full[i], 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
   const int vheads = p.kv_heads * p.head_groups;
-  // the last row that begins at or before `begin` and has pages
   Cursor c;
-  {
-    int lo = 0, n = p.num_items;
-    while (n > 1) {
-      const int stride = (n + 31) / 32, at = lo + lane * stride;
-      const unsigned hit = __ballot_sync(kAll, at < lo + n && p.before[at] * vheads <= begin);
-      const int k = 31 - __clz(hit);
-      n = min(stride, n - k * stride);
-      lo += k * stride;
-    }
-    c.row = lo;
-    c.it = p.items[lo];
-    const int own = own_pages(c.it);
-    const int64_t at = begin - p.before[lo] * vheads;
-    const int vh = (int)quotient(at, own);
-    c.page = c.it.shared + (int)(at - (int64_t)vh * own);
-    c.kvh = vh / p.head_groups;
-    c.grp = vh - c.kvh * p.head_groups;
-  }
-  // lane i holds the block id of page i of a window of 32 pages of the row that is being loaded
+  c.row = start.row;
+  c.it = start.it;
+  c.kvh = start.vhead / p.head_groups;
+  c.grp = start.vhead - c.kvh * p.head_groups;
+  c.page = start.page;
+  const uint32_t ring = smem_u32(smem) + in_cta * (T::SLOTS * T::PAGE);
+  // lane i holds the block id of page i of a window of 32 pages of the row that is being brought
   int win_row = -1, win_first = 0, win_id = -1;
-  auto page_row = [&](const Cursor& a) -> int64_t {
-    const int first = a.page & ~31;
-    if (a.row != win_row || first != win_first) {
-      win_row = a.row;
-      win_first = first;
-      win_id = first + lane <= last_page(a) ? p.block_table[(int64_t)a.it.slot * p.bt_stride + first + lane] : -1;
-    }
-    const int id = __shfl_sync(kAll, win_id, a.page & 31);
-    if (id >= 0 && id < p.blocks) return (int64_t)id * kBlock;
-    if (lane == 0) set_error(p.status, CDB_ERR_INDEX);
-    return -1;
-  };
-  uint32_t qf[D / 16][2];
-  auto load_q = [&]() {
-    const int in_kv = c.grp * kHeads + g;
-    const bool on = in_kv < p.heads_per_kv;
-    const __nv_bfloat16* src =
-        p.q + (int64_t)c.row * p.q_stride + (int64_t)(c.kvh * p.heads_per_kv + (on ? in_kv : 0)) * D + t * 8;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      const uint4 w = on ? *reinterpret_cast<const uint4*>(src + i * 32) : make_uint4(0u, 0u, 0u, 0u);
-      qf[2 * i][0] = w.x, qf[2 * i][1] = w.y, qf[2 * i + 1][0] = w.z, qf[2 * i + 1][1] = w.w;
-    }
-  };
-  load_q();
-  Page<D> x;
-  int64_t row = page_row(c), next_row = -1;
-  if (row >= 0) {
-    load_k<D>(p, row, c.kvh, x);
-    load_v<D>(p, row, c.kvh, x);
-  }
   Cursor ahead = c;
+  int issued = 0, put = 0;
+  unsigned gone = 0;  // slots whose page does not exist
+  auto issue = [&]() {
+    const int first = ahead.page & ~31;
+    if (ahead.row != win_row || first != win_first) {
+      win_row = ahead.row;
+      win_first = first;
+      win_id = first + lane <= last_page(ahead) ? p.block_table[(int64_t)ahead.it.slot * p.bt_stride + first + lane] : -1;
+    }
+    const int id = __shfl_sync(kAll, win_id, ahead.page & 31);
+    const bool have = id >= 0 && id < p.blocks;
+    gone = have ? gone & ~(1u << put) : gone | 1u << put;
+    if (lane == 0) {
+      if (!have) set_error(p.status, CDB_ERR_INDEX);
+      mbar_arrive_expect_tx(&full[put], T::PAGE);
+    }
+    __syncwarp();
+    if (lane < 2 * T::ATOMS) {  // K's columns, then V's; behind the cache's rows a box comes as zeros
+      const bool value = lane >= T::ATOMS;
+      const int row = have ? id * kBlock + (value ? (int)p.kv_rows : 0) : 2 * (int)p.kv_rows;
+      load_box(ring + put * T::PAGE + lane * T::BOX, &map, (lane - (value ? T::ATOMS : 0)) * 64, ahead.kvh, row,
+               smem_u32(&full[put]));
+    }
+    put = put + 1 == T::SLOTS ? 0 : put + 1;
+    if (++issued < start.count) advance(p, ahead);
+  };
+  for (int i = 0; i < T::SLOTS && issued < start.count; ++i) issue();
+
+  uint32_t qf[MT][2];
   float acc[MT][4], m[2], l[2];
   bool fresh = true, whole = false;
-  for (int64_t i = begin; i < end; ++i) {
+  int get = 0;
+  uint32_t phase = 0;
+  // where this lane's row of the four matrices of a product's operand lies: K's 16 tokens x 16 dims, V's transposed
+  const int krow = (lane & 7) + (lane & 8), kch = lane >> 4, vrow = (lane & 7) + ((lane >> 4) << 3), vch = (lane >> 3) & 1;
+  for (int i = 0; i < start.count; ++i) {
     if (fresh) {
-      if (i > begin) load_q();
+      const int in_kv = c.grp * kHeads + g;
+      const bool on = in_kv < p.heads_per_kv;
+      const __nv_bfloat16* src =
+          p.q + (int64_t)c.row * p.q_stride + (int64_t)(c.kvh * p.heads_per_kv + (on ? in_kv : 0)) * D + 2 * t;
+#pragma unroll
+      for (int k = 0; k < MT; ++k) {
+        qf[k][0] = on ? *reinterpret_cast<const uint32_t*>(src + k * 16) : 0u;
+        qf[k][1] = on ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 8) : 0u;
+      }
       whole = c.page == c.it.shared;
 #pragma unroll
-      for (int j = 0; j < MT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+      for (int k = 0; k < MT; ++k) acc[k][0] = acc[k][1] = acc[k][2] = acc[k][3] = 0.f;
       m[0] = m[1] = -INFINITY;
       l[0] = l[1] = 0.f;
     }
-    const bool seg_end = c.page == last_page(c);
-    const bool more = i + 1 < end;
-    if (more) {
-      advance(p, ahead);
-      next_row = page_row(ahead);
+    const bool seg_end = c.page == last_page(c), more = i + 1 < start.count;
+    if (!__all_sync(kAll, mbar_wait(&full[get], phase, p.status))) {
+      for (int k = i + 1; k < issued; ++k) {  // a copy that never came: the error is recorded; wait for the others
+        get = get + 1 == T::SLOTS ? (phase ^= 1u, 0) : get + 1;
+        mbar_wait(&full[get], phase, p.status);
+      }
+      return;
     }
-    if (row >= 0) {
+    if (!((gone >> get) & 1u)) {
+      const uint32_t k_at = ring + get * T::PAGE, v_at = k_at + T::ATOMS * T::BOX;
       float s[2][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+      for (int k = 0; k < 2; ++k) s[k][0] = s[k][1] = s[k][2] = s[k][3] = 0.f;
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        mma_bf16(s[0], x.k[0][j].x, x.k[1][j].x, x.k[0][j].y, x.k[1][j].y, qf[2 * j][0], qf[2 * j][1]);
-        mma_bf16(s[1], x.k[0][j].z, x.k[1][j].z, x.k[0][j].w, x.k[1][j].w, qf[2 * j + 1][0], qf[2 * j + 1][1]);
+      for (int k = 0; k < MT; ++k) {
+        uint32_t a[4];
+        load_matrices(k_at + (k >> 2) * T::BOX + krow * 128 + ((((k & 3) * 2 + kch) ^ (krow & 7)) << 4), a);
+        mma_bf16(s[k & 1], a[0], a[1], a[2], a[3], qf[k][0], qf[k][1]);
       }
-      if (more && next_row >= 0) load_k<D>(p, next_row, ahead.kvh, x);
       // y[hd][j]: token g + 8 j, head 2t + hd
       float y[2][2];
 #pragma unroll
       for (int hd = 0; hd < 2; ++hd)
 #pragma unroll
         for (int j = 0; j < 2; ++j) y[hd][j] = (s[0][2 * j + hd] + s[1][2 * j + hd]) * p.scale_log2;
+      // what lies behind the row's end may be anything, NaN too
+      const int live = seg_end ? c.it.pos % kBlock + 1 : kBlock;
       if (seg_end) {
-        const int live = c.it.pos % kBlock + 1;
 #pragma unroll
         for (int hd = 0; hd < 2; ++hd)
 #pragma unroll
           for (int j = 0; j < 2; ++j)
             if (g + 8 * j >= live) y[hd][j] = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)  // what lies behind the row's end may be anything, NaN too
-          if (2 * t + (j & 1) + 8 * (j >> 1) >= live) {
-#pragma unroll
-            for (int k = 0; k < D / 64; ++k) x.v[j][k] = make_uint4(0u, 0u, 0u, 0u);
-            if (D == 96) x.w[j] = make_uint2(0u, 0u);
-          }
       }
       const bool up = fmaxf(y[0][0], y[0][1]) > m[0] + 8.f || fmaxf(y[1][0], y[1][1]) > m[1] + 8.f;
       if (__any_sync(kAll, up)) {
@@ -837,29 +882,19 @@ __device__ __forceinline__ void single_rows(const Params& p, const Header& h) {
         l[1] += bf16hi(w);
         pw[j] = transpose8(w);
       }
+      const uint32_t seen0 = (2 * t < live ? 0xffffu : 0u) | (2 * t + 1 < live ? 0xffff0000u : 0u);
+      const uint32_t seen1 = (2 * t + 8 < live ? 0xffffu : 0u) | (2 * t + 9 < live ? 0xffff0000u : 0u);
 #pragma unroll
-      for (int k = 0; k < D / 64; ++k) {
-        const uint32_t a[4][4] = {{x.v[0][k].x, x.v[0][k].y, x.v[0][k].z, x.v[0][k].w},
-                                  {x.v[1][k].x, x.v[1][k].y, x.v[1][k].z, x.v[1][k].w},
-                                  {x.v[2][k].x, x.v[2][k].y, x.v[2][k].z, x.v[2][k].w},
-                                  {x.v[3][k].x, x.v[3][k].y, x.v[3][k].z, x.v[3][k].w}};
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          mma_bf16(acc[4 * k + e], __byte_perm(a[0][e], a[1][e], 0x5410), __byte_perm(a[0][e], a[1][e], 0x7632),
-                   __byte_perm(a[2][e], a[3][e], 0x5410), __byte_perm(a[2][e], a[3][e], 0x7632), pw[0], pw[1]);
+      for (int k = 0; k < MT; ++k) {
+        uint32_t a[4];
+        load_transposed(v_at + (k >> 2) * T::BOX + vrow * 128 + ((((k & 3) * 2 + vch) ^ (vrow & 7)) << 4), a);
+        if (seg_end) a[0] &= seen0, a[1] &= seen0, a[2] &= seen1, a[3] &= seen1;
+        mma_bf16(acc[k], a[0], a[1], a[2], a[3], pw[0], pw[1]);
       }
-      if (D == 96) {
-        const uint32_t a[4][2] = {{x.w[0].x, x.w[0].y}, {x.w[1].x, x.w[1].y}, {x.w[2].x, x.w[2].y}, {x.w[3].x, x.w[3].y}};
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          mma_bf16(acc[D == 96 ? 4 + e : 0], __byte_perm(a[0][e], a[1][e], 0x5410), __byte_perm(a[0][e], a[1][e], 0x7632),
-                   __byte_perm(a[2][e], a[3][e], 0x5410), __byte_perm(a[2][e], a[3][e], 0x7632), pw[0], pw[1]);
-      }
-      if (more && next_row >= 0) load_v<D>(p, next_row, ahead.kvh, x);
-    } else if (more && next_row >= 0) {
-      load_k<D>(p, next_row, ahead.kvh, x);
-      load_v<D>(p, next_row, ahead.kvh, x);
     }
+    get = get + 1 == T::SLOTS ? (phase ^= 1u, 0) : get + 1;
+    __syncwarp();  // every lane has read the page
+    if (issued < start.count) issue();
     if (seg_end || !more) {
 #pragma unroll
       for (int hd = 0; hd < 2; ++hd) {
@@ -869,54 +904,88 @@ __device__ __forceinline__ void single_rows(const Params& p, const Header& h) {
       }
       const bool direct = seg_end && whole && c.it.shared == 0;
       const int64_t seg = (int64_t)c.row * vheads + c.kvh * p.head_groups + c.grp;
-      // o of head 2t + hd: dims 64 k + 8 g + 2 e + {0, 1} in acc[4 k + e][hd], [2 + hd]; of 96's end 64 + 4 g + 2 e
+      // o of head 2t + hd: dims 16 k + g in acc[k][hd], 16 k + 8 + g in acc[k][2 + hd]
 #pragma unroll
       for (int hd = 0; hd < 2; ++hd) {
         const int head = 2 * t + hd, in_kv = c.grp * kHeads + head;
         if (in_kv >= p.heads_per_kv) continue;
         if (direct) {
           const float f = l[hd] == 0.f ? 0.f : 1.f / l[hd];
-          __nv_bfloat16* dst = p.out + (int64_t)c.row * p.out_stride + (int64_t)(c.kvh * p.heads_per_kv + in_kv) * D;
+          __nv_bfloat16* dst =
+              p.out + (int64_t)c.row * p.out_stride + (int64_t)(c.kvh * p.heads_per_kv + in_kv) * D + g;
 #pragma unroll
-          for (int k = 0; k < D / 64; ++k) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(acc[4 * k + e][hd] * f, acc[4 * k + e][2 + hd] * f);
-            *reinterpret_cast<uint4*>(dst + 64 * k + 8 * g) = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int k = 0; k < MT; ++k) {
+            dst[k * 16] = f_to_bf16(acc[k][hd] * f);
+            dst[k * 16 + 8] = f_to_bf16(acc[k][2 + hd] * f);
           }
-          if (D == 96)
-            *reinterpret_cast<uint2*>(dst + 64 + 4 * g) =
-                make_uint2(pack_bf16x2(acc[MT - 2][hd] * f, acc[MT - 2][2 + hd] * f),
-                           pack_bf16x2(acc[MT - 1][hd] * f, acc[MT - 1][2 + hd] * f));
         } else {
-          float* dst = p.single + ((seg + warp) * p.stored_heads + head) * (D + 4);
+          float* dst = p.single + ((seg + warp) * p.stored_heads + head) * (D + 4) + g;
 #pragma unroll
-          for (int k = 0; k < D / 64; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; e += 2)
-              __stcg(reinterpret_cast<float4*>(dst + 64 * k + 8 * g + 2 * e),
-                     make_float4(acc[4 * k + e][hd], acc[4 * k + e][2 + hd], acc[4 * k + e + 1][hd], acc[4 * k + e + 1][2 + hd]));
-          if (D == 96)
-            __stcg(reinterpret_cast<float4*>(dst + 64 + 4 * g),
-                   make_float4(acc[MT - 2][hd], acc[MT - 2][2 + hd], acc[MT - 1][hd], acc[MT - 1][2 + hd]));
+          for (int k = 0; k < MT; ++k) {
+            __stcg(dst + k * 16, acc[k][hd]);
+            __stcg(dst + k * 16 + 8, acc[k][2 + hd]);
+          }
           if (g == 0) __stcg(reinterpret_cast<float2*>(dst + D), make_float2(m[hd], l[hd]));
         }
       }
     }
     fresh = seg_end;
-    row = next_row;
-    c = ahead;
+    if (more) advance(p, c);
   }
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 1)
     attend_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   pdl_wait();
   const Header h = *p.header;
-  if ((int)blockIdx.x < h.shared_ctas) shared_steps<D>(map, p, h, smem);
-  else single_rows<D>(p, h);
+  const int warp = threadIdx.x >> 5;
+  if ((int)blockIdx.x >= h.shared_ctas) {
+    pdl_trigger();
+    single_rows<D>(map, p, h, smem, reinterpret_cast<uint64_t*>(smem + Tile<D>::OFF_BAR));
+    return;
+  }
+  const Start start = p.starts[blockIdx.x];
+  Shared& sh = *reinterpret_cast<Shared*>(smem + Tile<D>::OFF_BAR);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < Tile<D>::STAGES; ++i) {
+      mbar_init(&sh.kfull[i], 1);
+      mbar_init(&sh.vfull[i], 1);
+      mbar_init(&sh.kfree[i], 2);
+      mbar_init(&sh.vfree[i], 2);
+    }
+    for (int i = 0; i < 4; ++i) {
+      Shared::Team& tm = sh.team[i >> 1];
+      mbar_init(&tm.sfull[i & 1], 2);
+      mbar_init(&tm.pfull[i & 1], TM);
+      mbar_init(&tm.odone[i & 1], 1);
+      if (i & 1) mbar_init(&tm.drain, 1);
+    }
+    mbar_init(&sh.qfull, 2 * TM);
+    mbar_init(&sh.qfree, 2 * TM);
+    sh.abort = (smem_u32(smem) & 1023u) != 0u;  // the swizzle counts on it
+    if (sh.abort) set_error(p.status, CDB_ERR_INVALID_ARGUMENT);
+    fence_barrier_init();
+  }
+  if (warp == 11) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                 "r"(2 * kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  // Only now may the next kernel's CTAs come: one that holds tensor memory and waits for this kernel could otherwise
+  // be what the allocation above waits for.
+  pdl_trigger();
+  shared_steps<D>(map, p, start, smem, sh);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 11)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sh.tmem), "r"(2 * kTmemCols) : "memory");
 }
 
 // ---------------------------------------------------------------------------------------------- join
@@ -942,13 +1011,26 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
   const int64_t seg = (int64_t)item * vheads + kvh * p.head_groups + grp;
   const int64_t seg0 = p.before[item] * vheads + (int64_t)(kvh * p.head_groups + grp) * own;
   const int64_t c0 = own ? quotient(seg0, h.share) : 0, c1 = own ? quotient(seg0 + own - 1, h.share) : -1;
-  Group gr = {};
-  int64_t first = 0;
+  int shared = 0, rows = 0;  // parts of shared steps; rows of each
+  bool both = false;         // a CTA has one of this tile's, not two
+  int64_t part = 0;          // its row in the first of them
+  const float* shared_o = nullptr;
   if (it.shared > 0) {
-    gr = p.groups[it.group];
-    first = (int64_t)(item - p.group_start[it.group]) * p.heads_per_kv + in_kv;
+    const Group gr = p.groups[it.group];
+    const int local = item - gr.start, tile = local / p.tile_items, in_tile = local - tile * p.tile_items;
+    const int n = steps_of(gr.pages), full = p.tile_items * p.heads_per_kv, tiles = tiles_of(gr.rows, full);
+    rows = min(full, gr.rows - tile * full);
+    both = (tile | 1) < tiles;
+    // the CTAs that hold the unit's steps: CTA c takes steps [steps c / ctas, steps (c + 1) / ctas)
+    const int64_t s0 = gr.steps + ((int64_t)kvh * ((tiles + 1) / 2) + tile / 2) * n, s1 = s0 + n - 1;
+    const int64_t b0 = quotient((s0 + 1) * h.shared_ctas - 1, h.steps), b1 = quotient((s1 + 1) * h.shared_ctas - 1, h.steps);
+    shared = (both ? 1 : 2) * (int)(b1 - b0 + 1);
+    const int64_t base = unit_base(p, gr, kvh, tile) + b0 * TM + (both ? (tile & 1) * p.team_rows : 0);
+    part = base + in_tile * p.heads_per_kv + in_kv;
+    shared_o = p.shared_o + base * D + (int64_t)(in_tile * p.heads_per_kv + in_kv) * 8;
   }
-  const int shared = it.shared > 0 ? gr.splits : 0;
+  // part j of the shared ones: a CTA's, or one of its two teams'
+  auto place = [&](int j) { return both ? (int64_t)j * TM : (j & 1) * p.team_rows + (int64_t)(j >> 1) * TM; };
   if (shared == 0 && c0 == c1) return;  // written already
   const int parts = shared + (int)(c1 - c0 + 1);
   float m = -INFINITY, l = 0.f;
@@ -957,7 +1039,7 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
     const int j = j0 + lane;
     float2 ml = make_float2(-INFINITY, 0.f);
     if (j < shared)
-      ml = __ldcg(p.shared_ml + gr.base + ((int64_t)kvh * shared + j) * gr.rows + first);
+      ml = __ldcg(p.shared_ml + part + place(j));
     else if (j < parts)
       ml = __ldcg(reinterpret_cast<const float2*>(
           p.single + ((seg + c0 + j - shared) * p.stored_heads + in_kv - grp * kHeads) * (D + 4) + D));
@@ -974,7 +1056,7 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
       if (lane < D / 4 && fk != 0.f) {
         const float* src;
         if (jj < shared)
-          src = p.shared_o + (gr.base + ((int64_t)kvh * shared + jj) * gr.rows) * D + ((int64_t)(lane >> 1) * gr.rows + first) * 8 + (lane & 1) * 4;
+          src = shared_o + place(jj) * D + (int64_t)(lane >> 1) * rows * 8 + (lane & 1) * 4;
         else
           src = p.single + ((seg + c0 + jj - shared) * p.stored_heads + in_kv - grp * kHeads) * (D + 4) + lane * 4;
         const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
@@ -1011,15 +1093,15 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
 // ---------------------------------------------------------------------------------------------- host
 
 struct Layout {
-  int64_t header, items, before, groups, state, shared_o, shared_ml, single, floats;
+  int64_t header, items, before, groups, state, leader, starts, warps, shared_o, shared_ml, single, floats;
 };
 
 static int64_t padded(int64_t floats) { return (floats + 3) / 4 * 4; }
 
 static Layout layout(int64_t items, int64_t groups, int64_t heads, int64_t kv_heads, int64_t dim, int64_t sms) {
   const int64_t ratio = heads / kv_heads, head_groups = (ratio + kHeads - 1) / kHeads;
-  const int64_t stored = ratio < kHeads ? ratio : kHeads, ctas = 2 * sms;
-  const int64_t rows = groups > 0 ? TM * ctas + items * heads : 0;  // pieces' shares are no shorter than an even one
+  const int64_t stored = ratio < kHeads ? ratio : kHeads;
+  const int64_t rows = groups > 0 ? 2 * (sms * TM + items * heads) : 0;  // of both teams' parts
   Layout l;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -1032,9 +1114,12 @@ static Layout layout(int64_t items, int64_t groups, int64_t heads, int64_t kv_he
   l.before = take((items + 1) * sizeof(int64_t));
   l.groups = take((groups + 1) * sizeof(Group));
   l.state = take(groups * sizeof(int2));
+  l.leader = take(groups * sizeof(u64));
+  l.starts = take(sms * sizeof(Start));
+  l.warps = take(sms * kWarps * sizeof(WarpStart));
   l.shared_o = take(rows * dim * 4);
   l.shared_ml = take(rows * 8);
-  l.single = take((items * kv_heads * head_groups + ctas * kWarps) * stored * (dim + 4) * 4);
+  l.single = take((items * kv_heads * head_groups + sms * kWarps) * stored * (dim + 4) * 4);
   l.floats = at;
   return l;
 }
@@ -1057,7 +1142,7 @@ static int launch(const Params& p, cudaStream_t st) {
   if (launch_pdl(attend, dim3(p.num_ctas), dim3(kThreads), Tile<D>::SMEM, st, map, p) != cudaSuccess)
     return CDB_ERR_CUDA;
   const int64_t units = (int64_t)p.num_items * p.kv_heads * p.heads_per_kv;
-  const cudaError_t e = units >= 8 * p.num_ctas
+  const cudaError_t e = units >= 16 * p.num_ctas
                             ? launch_pdl(join_kernel<D, 1>, dim3((unsigned)((units + 3) / 4)), dim3(128), 0, st, p)
                             : launch_pdl(join_kernel<D, 4>, dim3((unsigned)units), dim3(128), 0, st, p);
   return e == cudaSuccess ? CDB_OK : CDB_ERR_CUDA;
@@ -1124,13 +1209,17 @@ extern "C" int cdb_prefix_decode_attention(const void* q, int64_t q_stride, void
   p.group_start = group_start;
   p.prefix_len = prefix_len;
   p.num_groups = num_groups;
-  p.num_ctas = 2 * num_sms;
+  p.num_ctas = num_sms;
   p.scale_log2 = scale * kLog2e;
   p.header = reinterpret_cast<Header*>(workspace + at.header);
   p.items = reinterpret_cast<Item*>(workspace + at.items);
   p.before = reinterpret_cast<int64_t*>(workspace + at.before);
   p.groups = reinterpret_cast<Group*>(workspace + at.groups);
   p.state = reinterpret_cast<int2*>(workspace + at.state);
+  p.leader = reinterpret_cast<u64*>(workspace + at.leader);
+  p.starts = reinterpret_cast<Start*>(workspace + at.starts);
+  p.warps = reinterpret_cast<WarpStart*>(workspace + at.warps);
+  p.team_rows = (int64_t)num_sms * TM + (int64_t)num_items * num_heads;
   p.shared_o = workspace + at.shared_o;
   p.shared_ml = reinterpret_cast<float2*>(workspace + at.shared_ml);
   p.single = workspace + at.single;
