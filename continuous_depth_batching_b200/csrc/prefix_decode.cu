@@ -16,7 +16,8 @@
 // comes from in tensor memory, V as it lies in the cache (the product's inner index across its rows). Each team takes a
 // tile through every step; a tile without a partner is taken by both teams, every other step to each. So one team's
 // exponentials run beside the other's products, and a step's keys are read once for 256 rows. One warp issues
-// each team's products and one brings the pages (TMA, 128-byte swizzle), five steps ahead.
+// each team's products, one brings the pages of K and one those of V (TMA, 128-byte swizzle; a warp takes some 80 cycles to
+// issue a copy, so one for both was what bounded a step), five steps ahead.
 //
 // Pages of single rows. The pages of all (row, kv head, up to 8 query heads) form one stream that is cut into equal
 // shares for the warps of the other CTAs. A warp brings its pages into a ring of its own (two pages of 8 KB at 128; with
@@ -51,12 +52,14 @@ struct Header {
   int64_t steps;    // of all of them
   int64_t share;    // pages of single rows that a warp takes
 };
-struct Item {
-  int pos, slot;  // pos -1: skipped
-  int group;      // -1: alone
-  int shared;     // its first pages, which the group's steps cover
+struct alignas(16) Item {
+  int pos, slot;     // pos -1: skipped
+  int shared;        // its first pages, which its group's steps cover
+  int start;         // of the group: its first row,
+  int rows, base;    // rows x query heads of a kv head, (row, head)s of the groups before it,
+  int64_t steps;     // steps of the groups before it
 };
-struct Group {
+struct alignas(16) Group {
   int pages;      // shared
   int start;      // its first row
   int rows;       // rows x query heads of a kv head
@@ -65,13 +68,9 @@ struct Group {
   int base;       // (row, head)s of the groups before it
 };
 // Where a CTA of shared steps begins: unit = (kv head, two tiles) of a group, step of the unit; and how many it takes.
-struct Start {
+struct alignas(16) Start {
   int group, unit, step, count;
-};
-// Where a warp of single rows begins, in a place for each warp of attend, and its row.
-struct WarpStart {
-  int row, vhead, page, count;
-  Item it;
+  Group g;
 };
 
 struct Params {
@@ -104,10 +103,10 @@ struct Params {
   int2* state;        // [num_groups] and
   u64* leader;        // [num_groups]: the plan's, where they do not fit shared memory
   Start* starts;      // [num_ctas]
-  WarpStart* warps;   // [num_ctas * kWarps]
+  int4* warps;        // [2][num_ctas * kWarps]: where a warp of single rows begins {row, (kv head, head group), page, how
+                      // many pages}, and that row's {position, slot, shared pages}
   int64_t team_rows;  // of all parts of one of the two teams
-  float* shared_o;    // parts of shared steps: part (unit, team, CTA) at team * team_rows + unit's row + 128 * CTA,
-                      // [D / 8][rows][8]
+  float* shared_o;    // parts of shared steps: part (unit, team, CTA) at row team * team_rows + unit's + 128 * CTA, [rows][D]
   float2* shared_ml;  // [rows of parts] {m, l}
   float* single;      // parts of single rows: [segment + warp][stored_heads][D + 4], m and l behind o
   int32_t* status;
@@ -125,42 +124,64 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 
 // ---------------------------------------------------------------------------------------------- plan
 
-struct Sums {
-  int64_t pages, steps, rows;
-};
-__device__ __forceinline__ Sums operator+(const Sums& a, const Sums& b) {
-  return {a.pages + b.pages, a.steps + b.steps, a.rows + b.rows};
-}
-__device__ __forceinline__ Sums shifted(const Sums& x, int o) {
-  return {__shfl_up_sync(kAll, x.pages, o), __shfl_up_sync(kAll, x.steps, o), __shfl_up_sync(kAll, x.rows, o)};
-}
-
 __device__ __forceinline__ int steps_of(int pages) { return (pages + kStepPages - 1) / kStepPages; }
 __device__ __forceinline__ int tiles_of(int items, int tile_items) { return (items + tile_items - 1) / tile_items; }
 
-// One CTA. Threads take a stretch of the rows and one of the groups each, nearly always one of either, so that
-// one scan serves both. 3 us of a call, most of it latencies: bounds and positions, the scan, the starts.
+// The last of n places whose value, which never falls, is at most x; the first's is.
+template <typename F>
+__device__ __forceinline__ int last_at_most(int n, int64_t x, F value) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (value(mid) <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// How a call's work is cut, in units of 1/64 us, measured at 16 heads of 128: a CTA takes 0.8 us to a step (HBM) and 1.25
+// where both teams have a tile (exponentials), 0.2 us to a page of single rows, and 4 us longer to begin and end with
+// shared steps. So few rows on a short prompt are faster each by itself.
+constexpr int kStepCost = 51, kPairCost = 80, kPageCost = 13, kSharedCost = 256;
+
+struct PlanShared {
+  int start[kPlanItems + 1];
+  int prefix[kPlanItems];
+  int2 state[kPlanItems];  // {fewest whole pages that a row of the group sees, its rows}
+  u64 leader[kPlanItems];  // {first live row, its slot}
+  Group group[kPlanItems];
+  int64_t before[kPlanItems + 1];
+  int4 item[kPlanItems];  // {position, slot, shared pages, group}
+  int64_t sum[2][32];
+  int64_t steps, cost;  // of all groups
+  unsigned best;
+};
+
+// One CTA. A thread takes a stretch of the rows, nearly always one, the first warp the groups, and then some take the
+// starts of CTAs, some those of warps. Most of it is latencies: the bounds and positions, a row's group, the sums, the
+// starts.
 __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
-  __shared__ int s_start[kPlanItems + 1];
-  __shared__ int2 s_state[kPlanItems];  // {fewest whole pages that a row of the group sees, its rows}
-  __shared__ u64 s_leader[kPlanItems];  // {first live row, its slot}
-  __shared__ int64_t s_before[kPlanItems + 1];
-  __shared__ Sums s_sum[32];
+  extern __shared__ __align__(16) uint8_t plan_smem[];
+  PlanShared& sh = *reinterpret_cast<PlanShared*>(plan_smem);
   pdl_trigger();
-  pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) sh.best = ~0u;
+  pdl_wait();
   int ng = p.tile_items > 0 ? p.num_groups : 0;
   const bool fits = ng <= kPlanItems, fits_items = p.num_items <= kPlanItems;
-  int2* state = fits ? s_state : p.state;
-  u64* leader = fits ? s_leader : p.leader;
+  int2* state = fits ? sh.state : p.state;
+  u64* leader = fits ? sh.leader : p.leader;
   const int first_pos = tid < p.num_items ? p.item_pos[tid] : -1, first_slot = tid < p.num_items ? p.item_slot[tid] : -1;
   bool bad = false;
   for (int g = tid; g < p.num_groups; g += kPlanThreads) {
     const int a = p.group_start[g], b = p.group_start[g + 1];
     bad |= a < 0 || b < a || b > p.num_items;
     if (g < ng) {
-      if (fits) s_start[g] = a;
-      if (fits && g + 1 == ng) s_start[ng] = b;
+      if (fits) {
+        sh.start[g] = a;
+        if (g + 1 == ng) sh.start[ng] = b;
+        sh.prefix[g] = p.prefix_len[g];
+      }
       state[g] = make_int2(INT32_MAX, 0);
       leader[g] = ~0ull;
     }
@@ -169,156 +190,193 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
     if (tid == 0) set_error(p.status, CDB_ERR_INDEX);
     ng = 0;
   }
-  const int* start = fits ? s_start : p.group_start;
-  // rows: their groups, and what those have in common
-  auto row = [&](int i) {
-    Item it;
-    it.pos = i == tid ? first_pos : p.item_pos[i];
-    it.slot = i == tid ? first_slot : p.item_slot[i];
-    it.group = -1;
-    it.shared = 0;
-    if (it.pos < 0 || it.slot < 0 || it.slot >= p.bt_rows || it.pos / kBlock >= p.bt_width) {
-      if (it.pos >= 0) set_error(p.status, CDB_ERR_INDEX);
-      it.pos = -1;
-    }
-    int lo = -1, hi = ng + 1;  // the last bound at or before i
-    while (ng > 0 && hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (start[mid] <= i) lo = mid;
-      else hi = mid;
-    }
-    if (lo >= 0 && lo < ng && it.pos >= 0) it.group = lo;
-    return it;
-  };
+  const int* start = fits ? sh.start : p.group_start;
+  const int* prefix = fits ? sh.prefix : p.prefix_len;
   const int per_i = (p.num_items + kPlanThreads - 1) / kPlanThreads;
   const int i0 = min(p.num_items, tid * per_i), i1 = min(p.num_items, i0 + per_i);
-  Item mine = {-1, -1, -1, 0};
-  for (int i = i0; i < i1; ++i) {
-    const Item it = row(i);
-    if (it.group >= 0) {
-      atomicMin(&state[it.group].x, (it.pos + 1) / kBlock);
-      atomicAdd(&state[it.group].y, 1);
-      atomicMin(&leader[it.group], (u64)i << 32 | (uint32_t)it.slot);
+  // rows {position, slot, -, group}: kept by their thread, or where it has several of them found again
+  auto row = [&](int i, bool tell) {
+    int4 it = make_int4(i == tid ? first_pos : p.item_pos[i], i == tid ? first_slot : p.item_slot[i], 0, -1);
+    if (it.x < 0 || it.y < 0 || it.y >= p.bt_rows || it.x / kBlock >= p.bt_width) {
+      if (it.x >= 0 && tell) set_error(p.status, CDB_ERR_INDEX);
+      it.x = -1;
+    } else if (ng > 0 && start[0] <= i && i < start[ng]) {
+      it.w = last_at_most(ng, i, [&](int g) { return (int64_t)start[g]; });
     }
-    if (per_i == 1) mine = it;
-    else p.items[i] = it;
+    return it;
+  };
+  int4 mine = make_int4(-1, -1, 0, -1);
+  for (int i = i0; i < i1; ++i) {
+    mine = row(i, true);
+    if (mine.w >= 0) {
+      atomicMin(&state[mine.w].x, (mine.x + 1) / kBlock);
+      atomicAdd(&state[mine.w].y, 1);
+      atomicMin(&leader[mine.w], (u64)i << 32 | (uint32_t)mine.y);
+    }
   }
   __syncthreads();
   auto pages_of = [&](int g) {
-    const int2 st = fits ? s_state[g] : __ldcg(p.state + g);  // (atomics pass the first cache by)
-    return st.y >= 2 ? min(max(p.prefix_len[g], 0) / kBlock, st.x) : 0;  // one row alone has nothing to share
+    const int2 st = fits ? sh.state[g] : __ldcg(p.state + g);  // (atomics pass the first cache by)
+    return st.y >= 2 ? min(max(prefix[g], 0) / kBlock, st.x) : 0;  // one row alone has nothing to share
   };
-  auto units_of = [&](int g) {
-    return (int64_t)((tiles_of(start[g + 1] - start[g], p.tile_items) + 1) / 2) * p.kv_heads;
+  auto share_row = [&](int4& it) {
+    if (it.w >= 0) it.z = pages_of(it.w);
   };
-  const int per_g = (ng + kPlanThreads - 1) / kPlanThreads;
-  const int g0 = min(ng, tid * per_g), g1 = min(ng, g0 + per_g);
-  Sums sum = {0, 0, 0};
+  auto pages_in = [](const int4& it) { return it.x < 0 ? 0 : it.x / kBlock + 1; };
+  // pages of the rows before this thread's: their own ones, and all
+  int64_t own = 0, whole = 0;
   for (int i = i0; i < i1; ++i) {
-    if (per_i > 1) mine = p.items[i];
-    if (mine.group >= 0) mine.shared = pages_of(mine.group);
-    if (mine.pos >= 0) sum.pages += mine.pos / kBlock + 1 - mine.shared;
-    p.items[i] = mine;
+    if (per_i > 1) mine = row(i, false);
+    share_row(mine);
+    whole += pages_in(mine);
+    own += pages_in(mine) - mine.z;
   }
-  for (int g = g0; g < g1; ++g) {
-    sum.steps += units_of(g) * steps_of(pages_of(g));
-    sum.rows += (int64_t)(start[g + 1] - start[g]) * p.heads_per_kv * p.kv_heads;
-  }
-  // before this thread, and all
-  Sums x = sum, all;
+  int64_t x = own, y = whole;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const Sums y = shifted(x, o);
-    if (lane >= o) x = x + y;
+    const int64_t a = __shfl_up_sync(kAll, x, o), b = __shfl_up_sync(kAll, y, o);
+    if (lane >= o) x += a, y += b;
   }
-  if (lane == 31) s_sum[warp] = x;
+  if (lane == 31) sh.sum[0][warp] = x, sh.sum[1][warp] = y;
+  if (warp == 0) {  // the groups: 32 at a time
+    int64_t steps0 = 0, rows0 = 0, cost = 0;
+    for (int base = 0; base < ng; base += 32) {
+      const int g = base + lane;
+      Group gr = {};
+      int64_t steps = 0, rows = 0;
+      if (g < ng) {
+        gr.pages = pages_of(g);
+        gr.start = start[g];
+        const int n = start[g + 1] - start[g], tiles = tiles_of(n, p.tile_items);
+        gr.rows = n * p.heads_per_kv;
+        gr.slot = (int)(uint32_t)(fits ? sh.leader[g] : __ldcg(p.leader + g));
+        steps = (int64_t)((tiles + 1) / 2) * p.kv_heads * steps_of(gr.pages);
+        cost += ((int64_t)(tiles / 2) * kPairCost + (tiles & 1) * kStepCost) * p.kv_heads * steps_of(gr.pages);
+        rows = (int64_t)gr.rows * p.kv_heads;
+      }
+      int64_t s = steps, t = rows;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t a = __shfl_up_sync(kAll, s, o), b = __shfl_up_sync(kAll, t, o);
+        if (lane >= o) s += a, t += b;
+      }
+      gr.steps = steps0 + s - steps;
+      gr.base = (int)(rows0 + t - rows);
+      if (g < ng) {
+        if (fits) sh.group[g] = gr;
+        else p.groups[g] = gr;
+      }
+      steps0 += __shfl_sync(kAll, s, 31);
+      rows0 += __shfl_sync(kAll, t, 31);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) cost += __shfl_xor_sync(kAll, cost, o);
+    if (lane == 0) sh.steps = steps0, sh.cost = cost;
+  }
   __syncthreads();
+  int64_t all_own, all_whole;
   {
-    Sums w = s_sum[lane];
+    int64_t a = sh.sum[0][lane], b = sh.sum[1][lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const Sums y = shifted(w, o);
-      if (lane >= o) w = w + y;
+      const int64_t c = __shfl_up_sync(kAll, a, o), d = __shfl_up_sync(kAll, b, o);
+      if (lane >= o) a += c, b += d;
     }
-    all = {__shfl_sync(kAll, w.pages, 31), __shfl_sync(kAll, w.steps, 31), __shfl_sync(kAll, w.rows, 31)};
-    const int from = (warp + 31) & 31;
-    const Sums base = {__shfl_sync(kAll, w.pages, from), __shfl_sync(kAll, w.steps, from), __shfl_sync(kAll, w.rows, from)};
-    if (warp > 0) x = x + base;
+    all_own = __shfl_sync(kAll, a, 31), all_whole = __shfl_sync(kAll, b, 31);
+    const int64_t c = __shfl_sync(kAll, a, (warp + 31) & 31), d = __shfl_sync(kAll, b, (warp + 31) & 31);
+    if (warp > 0) x += c, y += d;
   }
-  int64_t pages = x.pages - sum.pages, steps = x.steps - sum.steps, rows = x.rows - sum.rows;
-  for (int i = i0; i < i1; ++i) {
-    if (per_i > 1) mine = p.items[i];
-    p.before[i] = pages;
-    if (fits_items) s_before[i] = pages;
-    if (mine.pos >= 0) pages += mine.pos / kBlock + 1 - mine.shared;
-  }
-  for (int g = g0; g < g1; ++g) {
-    Group gr;
-    gr.pages = pages_of(g);
-    gr.start = start[g];
-    gr.rows = (start[g + 1] - start[g]) * p.heads_per_kv;
-    gr.slot = (int)(uint32_t)(fits ? s_leader[g] : __ldcg(p.leader + g));
-    gr.steps = steps;
-    gr.base = (int)rows;
-    p.groups[g] = gr;
-    steps += units_of(g) * steps_of(gr.pages);
-    rows += (int64_t)gr.rows * p.kv_heads;
-  }
-  // CTAs by the bytes of either kind of work
-  const int64_t vpages = all.pages * p.kv_heads * p.head_groups, shared_pages = all.steps * kStepPages;
+  // the division of the CTAs that is done first, or none
+  const int vheads = p.kv_heads * p.head_groups;
+  int64_t all_steps = sh.steps;
   int ctas = 0;
-  if (all.steps > 0)
-    ctas = vpages == 0 ? p.num_ctas
-                       : (int)min((int64_t)p.num_ctas - 1,
-                                  max((int64_t)1, quotient((int64_t)p.num_ctas * shared_pages, shared_pages + vpages)));
-  ctas = (int)min((int64_t)ctas, all.steps);  // each of them has one
+  if (all_steps > 0) {
+    unsigned mine_t = ~0u;
+    const float cost = (float)sh.cost, rest = (float)(all_own * vheads) * kPageCost;
+    for (int c = tid; c <= p.num_ctas; c += kPlanThreads) {
+      const float with = cost / (float)min((int64_t)max(c, 1), all_steps) + kSharedCost;
+      const float time = c == 0             ? (float)(all_whole * vheads) * kPageCost / (float)p.num_ctas
+                         : c < p.num_ctas   ? fmaxf(with, rest / (float)(p.num_ctas - c))
+                         : rest == 0.f      ? with
+                                            : 4e6f;
+      mine_t = min(mine_t, (unsigned)fminf(time, 4e6f) << 10 | (unsigned)c);
+    }
+    mine_t = __reduce_min_sync(kAll, mine_t);
+    if (lane == 0) atomicMin(&sh.best, mine_t);
+    __syncthreads();
+    ctas = (int)min((int64_t)(sh.best & 1023u), all_steps);  // each of them has a step
+  }
+  const bool sharing = ctas > 0;
+  if (!sharing) all_steps = 0;
+  const int64_t all_pages = sharing ? all_own : all_whole, vpages = all_pages * vheads;
+  int64_t pages = sharing ? x - own : y - whole;
+  for (int i = i0; i < i1; ++i) {
+    if (per_i > 1) mine = row(i, false);
+    if (sharing) share_row(mine);
+    else mine.z = 0;
+    p.before[i] = pages;
+    if (fits_items) sh.before[i] = pages, sh.item[i] = mine;
+    pages += pages_in(mine) - mine.z;
+  }
   const int64_t n_warps = (int64_t)(p.num_ctas - ctas) * kWarps;
   const int64_t share = n_warps ? max((int64_t)1, quotient(vpages + n_warps - 1, n_warps)) : 1;
   if (tid == 0) {
-    p.before[p.num_items] = all.pages;
-    if (fits_items) s_before[p.num_items] = all.pages;
+    p.before[p.num_items] = all_pages;
+    if (fits_items) sh.before[p.num_items] = all_pages;
     Header h;
     h.shared_ctas = ctas;
-    h.steps = all.steps;
+    h.steps = all_steps;
     h.share = share;
     *p.header = h;
   }
-  __syncthreads();  // items, groups and sums are read across threads from here on
-  if (tid < ctas) {
-    const int64_t begin = quotient(all.steps * tid, ctas), end = quotient(all.steps * (tid + 1), ctas);
-    Start st = {0, 0, 0, (int)(end - begin)};
-    int lo = 0, hi = ng;  // the last group that begins at or before `begin`
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (p.groups[mid].steps <= begin) lo = mid;
-      else hi = mid;
-    }
-    st.group = lo;
-    const int n = steps_of(p.groups[lo].pages);
-    const int64_t at = begin - p.groups[lo].steps;
-    st.unit = n ? (int)quotient(at, n) : 0;
-    st.step = n ? (int)(at - (int64_t)st.unit * n) : 0;
-    p.starts[tid] = st;
-  }
-  const int vheads = p.kv_heads * p.head_groups;
-  for (int w = tid; w < n_warps; w += kPlanThreads) {
-    const int64_t begin = w * share, end = min(begin + share, vpages);
-    WarpStart ws = {0, 0, 0, (int)max((int64_t)0, min(end - begin, (int64_t)INT32_MAX)), {-1, -1, -1, 0}};
-    if (begin < end) {
-      int lo = 0, hi = p.num_items;  // the last row that begins at or before `begin`, so one that has pages
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if ((fits_items ? s_before[mid] : p.before[mid]) * vheads <= begin) lo = mid;
-        else hi = mid;
+  __syncthreads();  // rows and groups are read across threads from here on
+  if (warp < 8) {
+    for (int i = tid; i < p.num_items; i += 256) {
+      int4 it = fits_items ? sh.item[i] : row(i, false);
+      if (!fits_items && sharing) share_row(it);
+      Item to = {it.x, it.y, it.z, 0, 0, 0, 0};
+      if (it.z > 0) {
+        const Group gr = fits ? sh.group[it.w] : p.groups[it.w];
+        to.start = gr.start;
+        to.rows = gr.rows;
+        to.base = gr.base;
+        to.steps = gr.steps;
       }
-      ws.row = lo;
-      ws.it = p.items[lo];
-      const int own = ws.it.pos / kBlock + 1 - ws.it.shared;
-      const int64_t at = begin - (fits_items ? s_before[lo] : p.before[lo]) * vheads;
-      ws.vhead = (int)quotient(at, own);
-      ws.page = ws.it.shared + (int)(at - (int64_t)ws.vhead * own);
+      p.items[i] = to;
     }
-    p.warps[ctas * kWarps + w] = ws;
+    for (int c = tid; c < ctas; c += 256) {
+      const int64_t begin = quotient(all_steps * c, ctas), end = quotient(all_steps * (c + 1), ctas);
+      Start st;
+      st.group = last_at_most(ng, begin, [&](int g) { return fits ? sh.group[g].steps : p.groups[g].steps; });
+      st.g = fits ? sh.group[st.group] : p.groups[st.group];
+      const int n = steps_of(st.g.pages);
+      st.unit = (int)quotient(begin - st.g.steps, n);
+      st.step = (int)(begin - st.g.steps - (int64_t)st.unit * n);
+      st.count = (int)(end - begin);
+      p.starts[c] = st;
+    }
+    if (fits && sharing)
+      for (int g = tid; g < ng; g += 256) p.groups[g] = sh.group[g];
+  } else {
+    for (int w = tid - 256; w < n_warps; w += kPlanThreads - 256) {
+      const int64_t begin = w * share, end = min(begin + share, vpages);
+      int4 from = make_int4(0, 0, 0, 0), of = make_int4(-1, -1, 0, 0);
+      if (begin < end) {  // its row is the last that begins at or before it, so one that has pages
+        auto before = [&](int i) { return fits_items ? sh.before[i] : p.before[i]; };
+        const int i = last_at_most(p.num_items, begin, [&](int j) { return before(j) * vheads; });
+        of = fits_items ? sh.item[i] : row(i, false);
+        if (!fits_items && sharing) share_row(of);
+        const int64_t at = begin - before(i) * vheads;
+        const int n = pages_in(of) - of.z;
+        from.x = i;
+        from.y = (int)quotient(at, n);
+        from.z = of.z + (int)(at - (int64_t)from.y * n);
+        from.w = (int)min(end - begin, (int64_t)INT32_MAX);
+      }
+      const int64_t to = (int64_t)ctas * kWarps + w;
+      p.warps[to] = from;
+      p.warps[(int64_t)p.num_ctas * kWarps + to] = of;
+    }
   }
 }
 
@@ -402,9 +460,8 @@ struct Walk {
   }
   __device__ __forceinline__ void begin(const Params& p, const Start& s) {
     at = s;
-    if (at.count <= 0) return;
-    g = p.groups[at.group];
-    look(p);
+    g = s.g;
+    if (at.count > 0) look(p);
   }
   __device__ __forceinline__ bool on() const { return at.count > 0; }
   __device__ __forceinline__ void next(const Params& p) {
@@ -443,13 +500,15 @@ __device__ __forceinline__ void shared_steps(const CUtensorMap& map, const Param
 
   // `t` counts the CTA's steps: step t lies in slot t % R of the ring. `j` counts a team's: its S lies in buffer j & 1. Every
   // barrier's phase follows.
-  if (warp == 8) {
-    // ------------------------------------------------------------ pages
+  if (warp == 8 || warp == 11) {
+    // ------------------------------------------------------------ pages, of K or of V
+    const bool values = warp == 11;
+    uint64_t *full = values ? sh.vfull : sh.kfull, *free = values ? sh.vfree : sh.kfree;
+    const uint32_t tiles = base + (values ? T::OFF_V : T::OFF_K);
     int t = 0;
     bool ok = true;
-    // lane: page (lane & 3) of the step, columns 64 * ((lane >> 2) & 1); lanes 0..7 of K, 16..23 of V
-    const int page_of = lane & 3, atom = (lane >> 2) & 1;
-    const bool loads = (lane & 8) == 0 && atom < T::ATOMS;
+    // lane: page (lane & 3) of the step, 64 columns from 64 * (lane >> 2) on
+    const int page_of = lane & 3, atom = lane >> 2;
     for (w.begin(p, start); w.on() && ok; w.next(p)) {
       const int32_t* bt = p.block_table + (int64_t)w.g.slot * p.bt_stride;
       auto fetch = [&](int n) {
@@ -461,38 +520,25 @@ __device__ __forceinline__ void shared_steps(const CUtensorMap& map, const Param
         const int after = fetch(n + 2), slot = t % R;
         const bool have = id >= 0 && id < p.blocks;
         const unsigned gone = __ballot_sync(kAll, !have) & 15u;
-        if (lane < kStepPages && !have && id != INT32_MIN) set_error(p.status, CDB_ERR_INDEX);
-        const int row = have ? id * kBlock : 2 * (int)p.kv_rows;  // behind the cache's rows a box comes as zeros
-        const uint32_t freed = (t / R + 1) & 1;                   // by step t - R
-        const uint32_t at = slot * T::STAGE + atom * (TK * 128) + page_of * (kBlock * 128);
-        if (t >= R) ok = __all_sync(kAll, wait_for(&sh.kfree[slot], freed, p.status, abort));
+        // behind the cache's rows a box comes as zeros
+        const int row = have ? id * kBlock + (values ? (int)p.kv_rows : 0) : 2 * (int)p.kv_rows;
+        if (t >= R) ok = __all_sync(kAll, wait_for(&free[slot], (t / R + 1) & 1, p.status, abort));  // by step t - R
         if (!ok) break;
         if (lane == 0) {
-          sh.missing[t % kMissing] = (int)gone;
-          mbar_arrive_expect_tx(&sh.kfull[slot], T::STAGE);
+          if (!values) sh.missing[t % kMissing] = (int)gone;
+          mbar_arrive_expect_tx(&full[slot], T::STAGE);
         }
         __syncwarp();
-        if (loads && lane < 16) load_box(base + T::OFF_K + at, &map, atom * 64, w.kvh, row, smem_u32(&sh.kfull[slot]));
-        if (t >= R) ok = __all_sync(kAll, wait_for(&sh.vfree[slot], freed, p.status, abort));
-        if (!ok) {
-          if (lane == 0) mbar_wait(&sh.kfull[slot], (t / R) & 1, p.status);
-          __syncwarp();
-          break;
-        }
-        if (lane == 16) mbar_arrive_expect_tx(&sh.vfull[slot], T::STAGE);
-        __syncwarp();
-        if (loads && lane >= 16)
-          load_box(base + T::OFF_V + at, &map, atom * 64, w.kvh, have ? row + (int)p.kv_rows : row,
-                   smem_u32(&sh.vfull[slot]));
+        if (atom < T::ATOMS)
+          load_box(tiles + slot * T::STAGE + atom * (TK * 128) + page_of * T::BOX, &map, atom * 64, w.kvh, row,
+                   smem_u32(&full[slot]));
+        if (!values && lane < kStepPages && !have && id != INT32_MIN) set_error(p.status, CDB_ERR_INDEX);
         id = next;
         next = after;
       }
     }
     // nothing may be on its way when the CTA ends
-    for (int j = max(0, t - R); j < t; ++j) {
-      mbar_wait(&sh.kfull[j % R], (j / R) & 1, p.status);
-      mbar_wait(&sh.vfull[j % R], (j / R) & 1, p.status);
-    }
+    for (int j = max(0, t - R); j < t; ++j) mbar_wait(&full[j % R], (j / R) & 1, p.status);
   } else if (warp == 9 || warp == 10) {
     // ------------------------------------------------------------ products
     const int team = warp - 9;
@@ -670,19 +716,37 @@ __device__ __forceinline__ void shared_steps(const CUtensorMap& map, const Param
             team * p.team_rows + unit_base(p, w.g, w.kvh, w.tile) + (int64_t)blockIdx.x * TM;
         if (some) {
           fence_after();
-          float* dst = p.shared_o + part * D + r * 8;
+          // O by CH columns through shared memory (q's of this tile, or of the tile that there is not), so that rows
+          // leave in whole lines
+          constexpr int CH = D == 64 ? 16 : 32, V = CH / 4;
+          const uint32_t stage = base + (w.both ? team * T::Q : T::Q + team * (T::Q / 2)) + quarter * (32 * CH * 4);
+          float* dst = p.shared_o + (part + quarter * 32) * D;
 #pragma unroll 1
-          for (int d = 0; d < D; d += 32) {
+          for (int d = 0; d < D; d += CH) {
             uint32_t o[32];
-            tmem_load(tmem_o + d, o);
-            wait_loads(o);
-            if (mine) {
-#pragma unroll
-              for (int k = 0; k < 32; k += 4)
-                __stcg(reinterpret_cast<float4*>(dst + (int64_t)((d + k) / 8) * rows * 8 + (k & 4)),
-                       make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]),
-                                   __uint_as_float(o[k + 3])));
+            if constexpr (CH == 32) {
+              tmem_load(tmem_o + d, o);
+              wait_loads(o);
+            } else {
+              tmem_load16(tmem_o + d, *reinterpret_cast<uint32_t(*)[16]>(o));
             }
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * (CH * 4) + ((k ^ (lane & (V - 1))) << 4)),
+                           "r"(o[4 * k]), "r"(o[4 * k + 1]), "r"(o[4 * k + 2]), "r"(o[4 * k + 3])
+                           : "memory");
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+              const int at = k * (32 / V) + lane / V, ch = lane % V;
+              float4 v;
+              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                           : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                           : "r"(stage + at * (CH * 4) + ((ch ^ (at & (V - 1))) << 4))
+                           : "memory");
+              if (quarter * 32 + at < rows) __stcg(reinterpret_cast<float4*>(dst + at * D + d + ch * 4), v);
+            }
+            __syncwarp();
           }
           fence_before();
         }
@@ -752,8 +816,10 @@ __device__ __forceinline__ void single_rows(const CUtensorMap& map, const Params
   constexpr int MT = D / 16;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, in_cta = threadIdx.x >> 5;
   const int64_t warp = (int64_t)((int)blockIdx.x - h.shared_ctas) * kWarps + in_cta;
-  const WarpStart start = p.warps[(int64_t)blockIdx.x * kWarps + in_cta];
-  if (start.count <= 0) return;
+  const int4 start = p.warps[(int64_t)blockIdx.x * kWarps + in_cta];
+  const int4 first = p.warps[(int64_t)(gridDim.x + blockIdx.x) * kWarps + in_cta];
+  const int count = start.w;
+  if (count <= 0) return;
   uint64_t* full = bars + in_cta * T::SLOTS;  // a page has landed
   if (lane == 0) {
     for (int i = 0; i < T::SLOTS; ++i) mbar_init(&full[i], 1);
@@ -762,11 +828,13 @@ __device__ __forceinline__ void single_rows(const CUtensorMap& map, const Params
   __syncwarp();
   const int vheads = p.kv_heads * p.head_groups;
   Cursor c;
-  c.row = start.row;
-  c.it = start.it;
-  c.kvh = start.vhead / p.head_groups;
-  c.grp = start.vhead - c.kvh * p.head_groups;
-  c.page = start.page;
+  c.row = start.x;
+  c.it.pos = first.x;
+  c.it.slot = first.y;
+  c.it.shared = first.z;
+  c.kvh = start.y / p.head_groups;
+  c.grp = start.y - c.kvh * p.head_groups;
+  c.page = start.z;
   const uint32_t ring = smem_u32(smem) + in_cta * (T::SLOTS * T::PAGE);
   // lane i holds the block id of page i of a window of 32 pages of the row that is being brought
   int win_row = -1, win_first = 0, win_id = -1;
@@ -795,9 +863,9 @@ __device__ __forceinline__ void single_rows(const CUtensorMap& map, const Params
                smem_u32(&full[put]));
     }
     put = put + 1 == T::SLOTS ? 0 : put + 1;
-    if (++issued < start.count) advance(p, ahead);
+    if (++issued < count) advance(p, ahead);
   };
-  for (int i = 0; i < T::SLOTS && issued < start.count; ++i) issue();
+  for (int i = 0; i < T::SLOTS && issued < count; ++i) issue();
 
   uint32_t qf[MT][2];
   float acc[MT][4], m[2], l[2];
@@ -806,7 +874,7 @@ __device__ __forceinline__ void single_rows(const CUtensorMap& map, const Params
   uint32_t phase = 0;
   // where this lane's row of the four matrices of a product's operand lies: K's 16 tokens x 16 dims, V's transposed
   const int krow = (lane & 7) + (lane & 8), kch = lane >> 4, vrow = (lane & 7) + ((lane >> 4) << 3), vch = (lane >> 3) & 1;
-  for (int i = 0; i < start.count; ++i) {
+  for (int i = 0; i < count; ++i) {
     if (fresh) {
       const int in_kv = c.grp * kHeads + g;
       const bool on = in_kv < p.heads_per_kv;
@@ -823,7 +891,7 @@ __device__ __forceinline__ void single_rows(const CUtensorMap& map, const Params
       m[0] = m[1] = -INFINITY;
       l[0] = l[1] = 0.f;
     }
-    const bool seg_end = c.page == last_page(c), more = i + 1 < start.count;
+    const bool seg_end = c.page == last_page(c), more = i + 1 < count;
     if (!__all_sync(kAll, mbar_wait(&full[get], phase, p.status))) {
       for (int k = i + 1; k < issued; ++k) {  // a copy that never came: the error is recorded; wait for the others
         get = get + 1 == T::SLOTS ? (phase ^= 1u, 0) : get + 1;
@@ -894,7 +962,7 @@ __device__ __forceinline__ void single_rows(const CUtensorMap& map, const Params
     }
     get = get + 1 == T::SLOTS ? (phase ^= 1u, 0) : get + 1;
     __syncwarp();  // every lane has read the page
-    if (issued < start.count) issue();
+    if (issued < count) issue();
     if (seg_end || !more) {
 #pragma unroll
       for (int hd = 0; hd < 2; ++hd) {
@@ -1011,23 +1079,24 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
   const int64_t seg = (int64_t)item * vheads + kvh * p.head_groups + grp;
   const int64_t seg0 = p.before[item] * vheads + (int64_t)(kvh * p.head_groups + grp) * own;
   const int64_t c0 = own ? quotient(seg0, h.share) : 0, c1 = own ? quotient(seg0 + own - 1, h.share) : -1;
-  int shared = 0, rows = 0;  // parts of shared steps; rows of each
+  int shared = 0;            // parts of shared steps
   bool both = false;         // a CTA has one of this tile's, not two
   int64_t part = 0;          // its row in the first of them
   const float* shared_o = nullptr;
   if (it.shared > 0) {
-    const Group gr = p.groups[it.group];
-    const int local = item - gr.start, tile = local / p.tile_items, in_tile = local - tile * p.tile_items;
-    const int n = steps_of(gr.pages), full = p.tile_items * p.heads_per_kv, tiles = tiles_of(gr.rows, full);
-    rows = min(full, gr.rows - tile * full);
+    Group gr;
+    gr.rows = it.rows;
+    gr.base = it.base;
+    const int local = item - it.start, tile = local / p.tile_items, in_tile = local - tile * p.tile_items;
+    const int n = steps_of(it.shared), full = p.tile_items * p.heads_per_kv, tiles = tiles_of(gr.rows, full);
     both = (tile | 1) < tiles;
     // the CTAs that hold the unit's steps: CTA c takes steps [steps c / ctas, steps (c + 1) / ctas)
-    const int64_t s0 = gr.steps + ((int64_t)kvh * ((tiles + 1) / 2) + tile / 2) * n, s1 = s0 + n - 1;
+    const int64_t s0 = it.steps + ((int64_t)kvh * ((tiles + 1) / 2) + tile / 2) * n, s1 = s0 + n - 1;
     const int64_t b0 = quotient((s0 + 1) * h.shared_ctas - 1, h.steps), b1 = quotient((s1 + 1) * h.shared_ctas - 1, h.steps);
     shared = (both ? 1 : 2) * (int)(b1 - b0 + 1);
     const int64_t base = unit_base(p, gr, kvh, tile) + b0 * TM + (both ? (tile & 1) * p.team_rows : 0);
     part = base + in_tile * p.heads_per_kv + in_kv;
-    shared_o = p.shared_o + base * D + (int64_t)(in_tile * p.heads_per_kv + in_kv) * 8;
+    shared_o = p.shared_o + part * D;
   }
   // part j of the shared ones: a CTA's, or one of its two teams'
   auto place = [&](int j) { return both ? (int64_t)j * TM : (j & 1) * p.team_rows + (int64_t)(j >> 1) * TM; };
@@ -1035,33 +1104,35 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
   const int parts = shared + (int)(c1 - c0 + 1);
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int j0 = (WARPS == 1 ? 0 : warp) * 32; j0 < parts; j0 += WARPS * 32) {
-    const int j = j0 + lane;
+  const int in_warp = WARPS == 1 ? 0 : warp;
+  // Eight parts of a warp at a time, {m, l} and o of all of them requested at once.
+  for (int j0 = in_warp; j0 < parts; j0 += 8 * WARPS) {
+    auto single_part = [&](int j) {
+      return p.single + ((seg + c0 + j - shared) * p.stored_heads + in_kv - grp * kHeads) * (D + 4);
+    };
     float2 ml = make_float2(-INFINITY, 0.f);
-    if (j < shared)
-      ml = __ldcg(p.shared_ml + part + place(j));
-    else if (j < parts)
-      ml = __ldcg(reinterpret_cast<const float2*>(
-          p.single + ((seg + c0 + j - shared) * p.stored_heads + in_kv - grp * kHeads) * (D + 4) + D));
+    const int j = j0 + lane * WARPS;
+    if (lane < 8 && j < parts)
+      ml = __ldcg(j < shared ? p.shared_ml + part + place(j) : reinterpret_cast<const float2*>(single_part(j) + D));
+    float4 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int jj = j0 + k * WARPS;
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (lane < D / 4 && jj < parts)
+        v[k] = __ldcg(reinterpret_cast<const float4*>(
+            (jj < shared ? shared_o + place(jj) * D : single_part(jj)) + lane * 4));
+    }
     const float to = fmaxf(m, warp_max(ml.x));
     const float down = m == -INFINITY ? 0.f : ex2(m - to), f = ml.x == -INFINITY ? 0.f : ex2(ml.x - to);
     m = to;
     l = l * down + warp_sum(ml.y * f);
     o.x *= down, o.y *= down, o.z *= down, o.w *= down;
-    const int n = min(32, parts - j0);
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
       const float fk = __shfl_sync(kAll, f, k);
-      const int jj = j0 + k;
-      if (lane < D / 4 && fk != 0.f) {
-        const float* src;
-        if (jj < shared)
-          src = shared_o + place(jj) * D + (int64_t)(lane >> 1) * rows * 8 + (lane & 1) * 4;
-        else
-          src = p.single + ((seg + c0 + jj - shared) * p.stored_heads + in_kv - grp * kHeads) * (D + 4) + lane * 4;
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-        o.x = fmaf(v.x, fk, o.x), o.y = fmaf(v.y, fk, o.y), o.z = fmaf(v.z, fk, o.z), o.w = fmaf(v.w, fk, o.w);
-      }
+      if (fk == 0.f) continue;  // (a part without keys has no o)
+      o.x = fmaf(v[k].x, fk, o.x), o.y = fmaf(v[k].y, fk, o.y), o.z = fmaf(v[k].z, fk, o.z), o.w = fmaf(v[k].w, fk, o.w);
     }
   }
   if (WARPS > 1) {
@@ -1116,7 +1187,7 @@ static Layout layout(int64_t items, int64_t groups, int64_t heads, int64_t kv_he
   l.state = take(groups * sizeof(int2));
   l.leader = take(groups * sizeof(u64));
   l.starts = take(sms * sizeof(Start));
-  l.warps = take(sms * kWarps * sizeof(WarpStart));
+  l.warps = take(2 * sms * kWarps * sizeof(int4));
   l.shared_o = take(rows * dim * 4);
   l.shared_ml = take(rows * 8);
   l.single = take((items * kv_heads * head_groups + sms * kWarps) * stored * (dim + 4) * 4);
@@ -1138,7 +1209,9 @@ static int launch(const Params& p, cudaStream_t st) {
     return CDB_ERR_TMA_ENCODE;
   auto attend = attend_kernel<D>;
   if (allow_shared(reinterpret_cast<const void*>(attend), Tile<D>::SMEM) != cudaSuccess) return CDB_ERR_CUDA;
-  if (launch_pdl(plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p) != cudaSuccess) return CDB_ERR_CUDA;
+  if (allow_shared(reinterpret_cast<const void*>(plan_kernel), sizeof(PlanShared)) != cudaSuccess ||
+      launch_pdl(plan_kernel, dim3(1), dim3(kPlanThreads), sizeof(PlanShared), st, p) != cudaSuccess)
+    return CDB_ERR_CUDA;
   if (launch_pdl(attend, dim3(p.num_ctas), dim3(kThreads), Tile<D>::SMEM, st, map, p) != cudaSuccess)
     return CDB_ERR_CUDA;
   const int64_t units = (int64_t)p.num_items * p.kv_heads * p.heads_per_kv;
@@ -1171,7 +1244,7 @@ extern "C" int cdb_prefix_decode_attention(const void* q, int64_t q_stride, void
   using namespace cdb::prefix;
   if (cache_layer < 0 || cache_layer >= num_cache_layers || kv_rows < kBlock || num_items < 0 || num_groups < 0 ||
       num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads != 0 || table_rows < 0 || table_width < 0 ||
-      num_sms <= 0 || !(scale > 0.f) || scale > 1e30f)
+      num_sms < 2 || num_sms > 1023 || !(scale > 0.f) || scale > 1e30f)
     return CDB_ERR_INVALID_ARGUMENT;
   if (head_dim != 64 && head_dim != 96 && head_dim != 128) return CDB_ERR_UNSUPPORTED;
   // cache rows, and the (row, head)s of a call, are counted in 32 bits
@@ -1218,7 +1291,7 @@ extern "C" int cdb_prefix_decode_attention(const void* q, int64_t q_stride, void
   p.state = reinterpret_cast<int2*>(workspace + at.state);
   p.leader = reinterpret_cast<u64*>(workspace + at.leader);
   p.starts = reinterpret_cast<Start*>(workspace + at.starts);
-  p.warps = reinterpret_cast<WarpStart*>(workspace + at.warps);
+  p.warps = reinterpret_cast<int4*>(workspace + at.warps);
   p.team_rows = (int64_t)num_sms * TM + (int64_t)num_items * num_heads;
   p.shared_o = workspace + at.shared_o;
   p.shared_ml = reinterpret_cast<float2*>(workspace + at.shared_ml);
