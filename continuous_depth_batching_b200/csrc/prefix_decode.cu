@@ -49,7 +49,7 @@ typedef unsigned long long u64;
 // What the plan leaves for the others.
 struct Header {
   int shared_ctas;  // CTAs of attend that take shared steps
-  int64_t steps;    // of all of them
+  int64_t cost;     // of all of their steps
   int64_t share;    // pages of single rows that a warp takes
 };
 struct alignas(16) Item {
@@ -57,14 +57,14 @@ struct alignas(16) Item {
   int shared;        // its first pages, which its group's steps cover
   int start;         // of the group: its first row,
   int rows, base;    // rows x query heads of a kv head, (row, head)s of the groups before it,
-  int64_t steps;     // steps of the groups before it
+  int64_t cost;      // cost of the groups before it
 };
 struct alignas(16) Group {
   int pages;      // shared
   int start;      // its first row
   int rows;       // rows x query heads of a kv head
   int slot;       // of its first live row, whose block table is read
-  int64_t steps;  // of the groups before it
+  int64_t steps, cost;  // of the groups before it
   int base;       // (row, head)s of the groups before it
 };
 // Where a CTA of shared steps begins: unit = (kv head, two tiles) of a group, step of the unit; and how many it takes.
@@ -139,10 +139,15 @@ __device__ __forceinline__ int last_at_most(int n, int64_t x, F value) {
   return lo;
 }
 
-// How a call's work is cut, in units of 1/64 us, measured at 16 heads of 128: a CTA takes 0.8 us to a step (HBM) and 1.25
-// where both teams have a tile (exponentials), 0.2 us to a page of single rows, and 4 us longer to begin and end with
-// shared steps. So few rows on a short prompt are faster each by itself.
-constexpr int kStepCost = 51, kPairCost = 80, kPageCost = 13, kSharedCost = 256;
+// How a call's work is cut, in units of 1/64 us, measured at 16 and 32 heads of 128: a CTA takes 1 us to a step (HBM) and
+// 1.3 where both teams have 128 rows (exponentials), 0.16 us to a page of single rows. Sharing costs another
+// 4 us (more parts, q, tensor memory), so few rows on a short prompt are faster each by itself: 4 rows on 700 tokens, 16
+// heads, take 17 us so and 24 shared.
+constexpr int kStepCost = 62, kPairCost = 83, kPageCost = 10, kSharedCost = 256;
+// Of a step of a group of `rows` (row, head)s, `full` to a tile.
+__device__ __forceinline__ int step_cost(int rows, int full) {
+  return kStepCost + (kPairCost - kStepCost) * min(max(rows - full, 0), full) / full;
+}
 
 struct PlanShared {
   int start[kPlanItems + 1];
@@ -239,11 +244,11 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
   }
   if (lane == 31) sh.sum[0][warp] = x, sh.sum[1][warp] = y;
   if (warp == 0) {  // the groups: 32 at a time
-    int64_t steps0 = 0, rows0 = 0, cost = 0;
+    int64_t steps0 = 0, rows0 = 0, cost0 = 0;
     for (int base = 0; base < ng; base += 32) {
       const int g = base + lane;
       Group gr = {};
-      int64_t steps = 0, rows = 0;
+      int64_t steps = 0, rows = 0, cost = 0;
       if (g < ng) {
         gr.pages = pages_of(g);
         gr.start = start[g];
@@ -251,16 +256,17 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
         gr.rows = n * p.heads_per_kv;
         gr.slot = (int)(uint32_t)(fits ? sh.leader[g] : __ldcg(p.leader + g));
         steps = (int64_t)((tiles + 1) / 2) * p.kv_heads * steps_of(gr.pages);
-        cost += ((int64_t)(tiles / 2) * kPairCost + (tiles & 1) * kStepCost) * p.kv_heads * steps_of(gr.pages);
+        cost = steps * step_cost(gr.rows, p.tile_items * p.heads_per_kv);
         rows = (int64_t)gr.rows * p.kv_heads;
       }
-      int64_t s = steps, t = rows;
+      int64_t s = steps, t = rows, u = cost;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t a = __shfl_up_sync(kAll, s, o), b = __shfl_up_sync(kAll, t, o);
-        if (lane >= o) s += a, t += b;
+        const int64_t a = __shfl_up_sync(kAll, s, o), b = __shfl_up_sync(kAll, t, o), c = __shfl_up_sync(kAll, u, o);
+        if (lane >= o) s += a, t += b, u += c;
       }
       gr.steps = steps0 + s - steps;
+      gr.cost = cost0 + u - cost;
       gr.base = (int)(rows0 + t - rows);
       if (g < ng) {
         if (fits) sh.group[g] = gr;
@@ -268,10 +274,9 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
       }
       steps0 += __shfl_sync(kAll, s, 31);
       rows0 += __shfl_sync(kAll, t, 31);
+      cost0 += __shfl_sync(kAll, u, 31);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) cost += __shfl_xor_sync(kAll, cost, o);
-    if (lane == 0) sh.steps = steps0, sh.cost = cost;
+    if (lane == 0) sh.steps = steps0, sh.cost = cost0;
   }
   __syncthreads();
   int64_t all_own, all_whole;
@@ -288,13 +293,14 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
   }
   // the division of the CTAs that is done first, or none
   const int vheads = p.kv_heads * p.head_groups;
-  int64_t all_steps = sh.steps;
+  const int64_t all_steps = sh.steps, all_cost = sh.cost;
+  const int most_ctas = (int)min(all_cost / kPairCost, (int64_t)p.num_ctas);  // each of them has a step of every unit it is in
   int ctas = 0;
-  if (all_steps > 0) {
+  if (most_ctas > 0) {
     unsigned mine_t = ~0u;
-    const float cost = (float)sh.cost, rest = (float)(all_own * vheads) * kPageCost;
+    const float cost = (float)all_cost, rest = (float)(all_own * vheads) * kPageCost;
     for (int c = tid; c <= p.num_ctas; c += kPlanThreads) {
-      const float with = cost / (float)min((int64_t)max(c, 1), all_steps) + kSharedCost;
+      const float with = cost / (float)min(max(c, 1), most_ctas) + kSharedCost;
       const float time = c == 0             ? (float)(all_whole * vheads) * kPageCost / (float)p.num_ctas
                          : c < p.num_ctas   ? fmaxf(with, rest / (float)(p.num_ctas - c))
                          : rest == 0.f      ? with
@@ -304,10 +310,9 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
     mine_t = __reduce_min_sync(kAll, mine_t);
     if (lane == 0) atomicMin(&sh.best, mine_t);
     __syncthreads();
-    ctas = (int)min((int64_t)(sh.best & 1023u), all_steps);  // each of them has a step
+    ctas = min((int)(sh.best & 1023u), most_ctas);
   }
   const bool sharing = ctas > 0;
-  if (!sharing) all_steps = 0;
   const int64_t all_pages = sharing ? all_own : all_whole, vpages = all_pages * vheads;
   int64_t pages = sharing ? x - own : y - whole;
   for (int i = i0; i < i1; ++i) {
@@ -325,7 +330,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
     if (fits_items) sh.before[p.num_items] = all_pages;
     Header h;
     h.shared_ctas = ctas;
-    h.steps = all_steps;
+    h.cost = all_cost;
     h.share = share;
     *p.header = h;
   }
@@ -340,18 +345,34 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
         to.start = gr.start;
         to.rows = gr.rows;
         to.base = gr.base;
-        to.steps = gr.steps;
+        to.cost = gr.cost;
       }
       p.items[i] = to;
     }
     for (int c = tid; c < ctas; c += 256) {
-      const int64_t begin = quotient(all_steps * c, ctas), end = quotient(all_steps * (c + 1), ctas);
+      // the first step whose cost begins at or behind the CTA's share of the cost
+      auto step_at = [&](int64_t cost, int& group, int64_t& local) {
+        group = last_at_most(ng, cost, [&](int g) { return fits ? sh.group[g].cost : p.groups[g].cost; });
+        const Group gr = fits ? sh.group[group] : p.groups[group];
+        const int w = step_cost(gr.rows, p.tile_items * p.heads_per_kv);
+        local = quotient(cost - gr.cost + w - 1, w);
+        return gr.steps + local;
+      };
       Start st;
-      st.group = last_at_most(ng, begin, [&](int g) { return fits ? sh.group[g].steps : p.groups[g].steps; });
+      int next_group;
+      int64_t local, next_local;
+      const int64_t begin = step_at(quotient(all_cost * c, ctas), st.group, local);
+      const int64_t end = c + 1 == ctas ? all_steps : step_at(quotient(all_cost * (c + 1), ctas), next_group, next_local);
       st.g = fits ? sh.group[st.group] : p.groups[st.group];
+      const int tiles = tiles_of(st.g.rows, p.tile_items * p.heads_per_kv);
+      if (local == (int64_t)((tiles + 1) / 2) * p.kv_heads * steps_of(st.g.pages)) {  // behind the group's last
+        local = 0;
+        do st.g = fits ? sh.group[++st.group] : p.groups[++st.group];
+        while (st.g.pages == 0);
+      }
       const int n = steps_of(st.g.pages);
-      st.unit = (int)quotient(begin - st.g.steps, n);
-      st.step = (int)(begin - st.g.steps - (int64_t)st.unit * n);
+      st.unit = (int)quotient(local, n);
+      st.step = (int)(local - (int64_t)st.unit * n);
       st.count = (int)(end - begin);
       p.starts[c] = st;
     }
@@ -1090,9 +1111,10 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p) {
     const int local = item - it.start, tile = local / p.tile_items, in_tile = local - tile * p.tile_items;
     const int n = steps_of(it.shared), full = p.tile_items * p.heads_per_kv, tiles = tiles_of(gr.rows, full);
     both = (tile | 1) < tiles;
-    // the CTAs that hold the unit's steps: CTA c takes steps [steps c / ctas, steps (c + 1) / ctas)
-    const int64_t s0 = it.steps + ((int64_t)kvh * ((tiles + 1) / 2) + tile / 2) * n, s1 = s0 + n - 1;
-    const int64_t b0 = quotient((s0 + 1) * h.shared_ctas - 1, h.steps), b1 = quotient((s1 + 1) * h.shared_ctas - 1, h.steps);
+    // the CTAs that hold the unit's steps: CTA c takes those that begin at costs [cost c / ctas, cost (c + 1) / ctas)
+    const int w = step_cost(it.rows, full);
+    const int64_t s0 = it.cost + ((int64_t)kvh * ((tiles + 1) / 2) + tile / 2) * n * w, s1 = s0 + (int64_t)(n - 1) * w;
+    const int64_t b0 = quotient((s0 + 1) * h.shared_ctas - 1, h.cost), b1 = quotient((s1 + 1) * h.shared_ctas - 1, h.cost);
     shared = (both ? 1 : 2) * (int)(b1 - b0 + 1);
     const int64_t base = unit_base(p, gr, kvh, tile) + b0 * TM + (both ? (tile & 1) * p.team_rows : 0);
     part = base + in_tile * p.heads_per_kv + in_kv;
