@@ -12,11 +12,15 @@ import torch
 
 import continuous_depth_batching_b200.ops as ops
 import continue_reference as ref
+from continuous_depth_batching_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 BS = 16
 I32 = dict(dtype=torch.int32, device=DEV)
+# How many SMs the C entry point is told to use; None: the operator, which names the device's. Sharing pays sooner
+# on few, and a CTA then takes several units, so small cases go every way: shared, each row alone, both at once.
+SMS = [None, 2, 3, 11]
 
 
 class Case:
@@ -57,18 +61,34 @@ class Case:
         self.pos = [l - 1 for l in self.lens]
         self.scale = d**-0.5
 
-    def run(self, start=None, prefix=None, out=None):
+    def run(self, start=None, prefix=None, sms=None):
         start, prefix = self.start if start is None else start, self.prefix if prefix is None else prefix
         wide = torch.full((self.n, self.heads * self.d + 8), 3.0, dtype=torch.bfloat16, device=DEV)
         qw = torch.zeros(self.n, self.heads * self.d + 16, dtype=torch.bfloat16, device=DEV)
         qw[:, : self.heads * self.d] = self.q.to(DEV)
         self.dev = dict(pool=self.pool.to(DEV), table=self.table.to(DEV)[:, : self.table.shape[1] - 3])
-        torch.ops.cdb.prefix_decode_attention(
-            qw[:, : self.heads * self.d], wide[:, : self.heads * self.d], self.dev["pool"], self.layer, self.dev["table"], torch.tensor(self.slot, **I32),
-            torch.tensor(self.pos, **I32), torch.tensor(start, **I32), torch.tensor(prefix, **I32), self.heads, self.scale)
+        q, out = qw[:, : self.heads * self.d], wide[:, : self.heads * self.d]
+        slot, pos = torch.tensor(self.slot, **I32), torch.tensor(self.pos, **I32)
+        start, prefix = torch.tensor(start, **I32), torch.tensor(prefix, **I32)
+        pool, table = self.dev["pool"], self.dev["table"]
+        if sms is None:
+            torch.ops.cdb.prefix_decode_attention(q, out, pool, self.layer, table, slot, pos, start, prefix, self.heads, self.scale)
+        else:
+            n, groups = self.n, prefix.numel()
+            floats = _lib.load().cdb_prefix_decode_workspace_floats(n, groups, self.heads, self.kv, self.d, sms)
+            ws = torch.full((floats + 64,), float("nan"), device=DEV)  # in any state; nothing behind it is written
+            _lib.call("cdb_prefix_decode_attention", *map(_lib.ptr, (q,)), q.stride(0), _lib.ptr(out), out.stride(0), _lib.ptr(pool), pool.shape[0], pool.shape[2],
+                      self.layer, _lib.ptr(table), table.stride(0), table.shape[0], table.shape[1], _lib.ptr(slot), _lib.ptr(pos), n, _lib.ptr(start),
+                      _lib.ptr(prefix), groups, self.heads, self.kv, self.d, self.scale, sms, _lib.ptr(ws), floats,
+                      _lib.ptr(torch.ops.cdb._status_word(q)), torch.cuda.current_stream().cuda_stream)
+            assert ws[floats:].isnan().all()
         torch.cuda.synchronize()
         assert (wide[:, self.heads * self.d :] == 3).all()
         return wide[:, : self.heads * self.d].cpu()
+
+    def check_all(self, rows=None, **how):
+        for sms in SMS:
+            self.check(self.run(sms=sms, **how), rows)
 
     def check(self, out, rows=None):
         for i in range(self.n) if rows is None else rows:
@@ -91,7 +111,7 @@ def test_head_layouts_and_groups(heads, kv, d, groups):
     n = sum(r for r, _ in groups)
     extra = [1 + int(x) for x in torch.randint(0, 60, (n,), generator=g)]
     c = Case(groups, extra, heads, kv, d, seed=heads + n)
-    c.check(c.run())
+    c.check_all()
     assert ops.status_code() == 0
 
 
@@ -101,16 +121,16 @@ def test_head_layouts_and_groups(heads, kv, d, groups):
 def test_prefix_lengths(heads, kv, d, prefix, rows):
     extra = [1 + (i * 7) % 40 for i in range(rows)]
     c = Case([(rows, prefix)], extra, heads, kv, d, seed=prefix)
-    c.check(c.run())
+    c.check_all()
     assert ops.status_code() == 0
 
 
 @pytest.mark.parametrize("rows", [1, 2, 127, 128, 129, 256, 300])
 def test_rows_around_a_tile(rows):
     c = Case([(rows, 200)], [1 + i % 30 for i in range(rows)], 2, 2, 64, seed=rows)
-    c.check(c.run())
+    c.check_all()
     c = Case([(rows, 96)], [1 + i % 3 for i in range(rows)], 6, 2, 64, seed=rows)
-    c.check(c.run())
+    c.check_all()
     assert ops.status_code() == 0
 
 
@@ -120,51 +140,66 @@ def test_many_groups_and_more_rows_than_threads():
     n = sum(r for r, _ in groups)
     assert n > 512
     c = Case(groups, [1 + int(x) for x in torch.randint(0, 90, (n,), generator=g)], 4, 2, 64)
-    c.check(c.run(), range(0, n, 3))
+    c.check_all(range(0, n, 5))
     assert ops.status_code() == 0
 
 
 @pytest.mark.parametrize("own", [1, 16, 17, 3000, 20000])
 def test_long_rows_of_their_own(own):
     c = Case([(3, 400), (1, 0)], [own, 5, own // 2 + 1, own], 8, 2, 128, seed=own)
-    c.check(c.run())
+    c.check_all()
     assert ops.status_code() == 0
 
 
 def test_a_long_prefix():
     c = Case([(7, 40000)], [1, 2, 30, 40, 500, 3, 9], 8, 2, 128)
-    c.check(c.run())
+    c.check_all()
     assert ops.status_code() == 0
 
 
 def test_groups_that_leave_rows_out_and_empty_ones():
     c = Case([(4, 160), (3, 320), (5, 80)], [3 * i + 1 for i in range(12)], 4, 4, 128)
-    want = c.run()
-    c.check(want)
-    c.check(c.run([4, 7], [320]))  # the second group alone
-    c.check(c.run([], []))  # every row alone
-    c.check(c.run([0], []))
-    c.check(c.run([0, 0, 4, 4, 7, 7, 12, 12], [50, 160, 9999, 320, 16, 80, 3]))  # empty groups between
-    c.check(c.run([1, 3, 5, 6], [100, 0, 320]))  # parts of them
-    c.check(c.run(prefix=[-5, 0, -(2**31)]))
-    c.check(c.run(prefix=[2**31 - 1] * 3, start=[0, 1, 1, 2]))  # more than the row: cut to what it sees
+    c.check_all()
+    for start, prefix in [
+        ([4, 7], [320]),  # the second group alone
+        ([], []),  # every row alone
+        ([0], []),
+        ([0, 0, 4, 4, 7, 7, 12, 12], [50, 160, 9999, 320, 16, 80, 3]),  # empty groups between
+        ([1, 3, 5, 6], [100, 0, 320]),  # parts of them
+        ([0, 4, 7, 12], [-5, 0, -(2**31)]),
+        ([0, 1, 1, 2], [2**31 - 1] * 3),  # more than the row: cut to what it sees
+    ]:
+        c.check_all(start=start, prefix=prefix)
     assert ops.status_code() == 0
 
 
 def test_rows_that_see_less_than_the_prefix_and_padding_rows():
     c = Case([(6, 320), (4, 64)], [5, 9, 40, 1, 2, 3, 4, 5, 6, 7], 8, 4, 64)
     c.pos[2] = 100  # ends inside the shared blocks
-    c.check(c.run())
+    c.check_all()
     c.pos[0], c.pos[4], c.slot[0] = -1, -1, -9
-    c.check(c.run())
+    c.check_all()
     c.pos[2] = 0
-    c.check(c.run())
+    c.check_all()
     for i in range(6):
         c.pos[i] = -1
-    c.check(c.run())
+    c.check_all()
     for i in range(10):
         c.pos[i] = -1
-    assert (c.run() == 3).all()
+    for sms in SMS:
+        assert (c.run(sms=sms) == 3).all()
+    assert ops.status_code() == 0
+
+
+def test_rows_that_see_shared_blocks_only():
+    """Positions that end a page, so that a row's own pages are none."""
+
+    c = Case([(5, 256), (3, 64)], [16, 1, 32, 16, 20, 16, 16, 16], 4, 2, 128)
+    for i in (0, 3):
+        c.pos[i] = 255
+    for i in (5, 6, 7):
+        c.pos[i] = 63
+    c.check_all()
     assert ops.status_code() == 0
 
 
@@ -175,32 +210,34 @@ def test_large_logits_and_a_dominant_key():
         c.pool[0, 0, rows[2] * BS + 3] *= scale_up
         own = c.table[c.slot[1]].long()[41] * BS
         c.pool[0, 0, own] *= scale_up
-        out = c.run()
-        for i in range(5):
+        for sms, i in ((sms, i) for sms in SMS for i in range(5)):
+            out = c.run(sms=sms)
             want, size = ref.attend(c.q[i].view(4, 128), c.pool[0], c.table[c.slot[i]], c.pos[i], c.scale, c.blocks)
             # logits of up to 30 x 10: their fp32 sums are off by up to 128 x 2^-24 x 300 = 2^-9
             tol = 2.0**-8 * want.abs() + 2.0**-8 * (size + want.abs()) + 2.0**-8 * size
             assert ((out[i].double().view(4, 128) - want).abs() <= tol).all()
 
 
-def test_nan_and_infinity_stay_in_the_rows_that_see_them():
+@pytest.mark.parametrize("sms", SMS)
+def test_nan_and_infinity_stay_in_the_rows_that_see_them(sms):
     c = Case([(4, 128), (3, 96)], [5, 40, 3, 20, 1, 2, 3], 4, 2, 64, seed=2)
-    clean = c.run()
+    clean = c.run(sms=sms)
     own = c.table[c.slot[1]].long()[9] * BS + 2  # position 146 of row 1
     c.pool[0, 0, own] = float("nan")
     c.pool[0, 1, c.table[c.slot[3]].long()[8] * BS] = float("inf")
-    out = c.run()
+    out = c.run(sms=sms)
     assert out[1].isnan().all() and (out[3] == float("inf")).all()
     keep = [0, 2, 4, 5, 6]
     assert torch.equal(out[keep], clean[keep])
     c.pool[0, 1, c.table[c.slot[4]].long()[0] * BS + 1] = float("nan")  # shared by the second group
-    out = c.run()
+    out = c.run(sms=sms)
     assert out[4:].isnan().all() and torch.equal(out[[0, 2]], clean[[0, 2]])
     assert ops.status_code() == 0
 
 
+@pytest.mark.parametrize("sms", SMS)
 @pytest.mark.parametrize("what", ["slot", "position", "own block", "own block past the cache", "shared block"])
-def test_indexes_out_of_range(what):
+def test_indexes_out_of_range(what, sms):
     c = Case([(3, 96), (2, 64)], [20, 3, 40, 5, 6], 4, 2, 64, seed=3)
     if what == "slot":
         c.slot[1] = 7
@@ -213,7 +250,7 @@ def test_indexes_out_of_range(what):
     else:
         for i in range(3):
             c.table[c.slot[i], 2] = 2**31 - 1
-    out = c.run()
+    out = c.run(sms=sms)
     assert ops.status_code() == 6
     torch.ops.cdb._status_word(c.dev["pool"]).zero_()
     if what in ("slot", "position"):
@@ -223,10 +260,11 @@ def test_indexes_out_of_range(what):
         c.check(out)  # without the keys of such blocks
 
 
+@pytest.mark.parametrize("sms", SMS)
 @pytest.mark.parametrize("start", [[0, 3, 2], [-1, 3, 5], [0, 3, 6], [4, 3, 5], [0, 2**31 - 1, 5]])
-def test_group_bounds_out_of_range(start):
+def test_group_bounds_out_of_range(start, sms):
     c = Case([(3, 96), (2, 64)], [20, 3, 40, 5, 6], 4, 2, 64, seed=3)
-    out = c.run(start=start)
+    out = c.run(start=start, sms=sms)
     assert ops.status_code() == 6
     torch.ops.cdb._status_word(c.dev["pool"]).zero_()
     c.check(out)
@@ -237,16 +275,27 @@ def test_no_rows_and_layers():
     torch.ops.cdb.prefix_decode_attention(z(0, 64), z(0, 64), z(1, 2, 16, 1, 64), 0, torch.zeros(1, 1, **I32), torch.zeros(0, **I32), torch.zeros(0, **I32),
                                           torch.zeros(2, **I32), torch.zeros(1, **I32), 1, 0.125)
     c = Case([(3, 100)], [5, 6, 70], 4, 2, 96, layers=3, layer=2)
-    c.check(c.run())
+    c.check_all()
     assert ops.status_code() == 0
 
 
 def test_the_same_bits_again():
     c = Case([(40, 3000), (9, 100)], [1 + (i * 37) % 300 for i in range(49)], 16, 4, 128)
-    first = c.run()
-    c.check(first, range(0, 49, 5))
-    for _ in range(4):
-        assert torch.equal(c.run(), first)
+    for sms in SMS:
+        first = c.run(sms=sms)
+        c.check(first, range(0, 49, 5))
+        for _ in range(3):
+            assert torch.equal(c.run(sms=sms), first)
+
+
+def test_more_rows_than_the_plan_keeps():
+    """More rows, and groups, than the plan's threads and shared memory hold."""
+
+    n = 2300
+    c = Case([(2, 48)] * 1100 + [(100, 600)], [1 + i % 20 for i in range(n)], 2, 1, 64, seed=8)
+    assert c.n == n and len(c.prefix) == 1101
+    c.check_all(list(range(0, 2200, 97)) + list(range(2200, n, 9)))
+    assert ops.status_code() == 0
 
 
 def test_a_cache_past_32_bits():
