@@ -5,7 +5,7 @@
 // maximum of the logits, l the sum of 2^(x - m), o that of 2^(x - m) v) of any set of keys join by rescaling to
 // one m, so the two kinds of work need not wait for each other: one launch does both side by side, and a
 // last one joins. Three launches in all:
-//   plan    one CTA: how many blocks each group shares, where every CTA and warp begins;
+//   plan    a few CTAs: how many blocks each group shares, where every CTA and warp begins;
 //   attend  a CTA an SM, of one kind: shared steps or pages of single rows;
 //   join    a warp (or a CTA) per row and head adds up its parts. Rows with one part are written by attend.
 // No counters and no atomics between CTAs: parts lie where the plan says, and are added in that order.
@@ -38,7 +38,8 @@ constexpr int TK = 64;      // keys of a shared step
 constexpr int kStepPages = TK / kBlock;
 constexpr int kWarps = 12;
 constexpr int kThreads = kWarps * 32;
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 256;
+constexpr int kPlanCtas = 8;
 constexpr int kPlanItems = 1024;  // rows, and groups, whose state fits the plan's shared memory
 constexpr int kHeads = 8;         // query heads of one single-row segment (n of an m16n8k16 product)
 constexpr uint32_t kTmemCols = 256;  // of a team
@@ -162,9 +163,10 @@ struct PlanShared {
   unsigned best;
 };
 
-// One CTA. A thread takes a stretch of the rows, nearly always one, the first warp the groups, and then some take the
-// starts of CTAs, some those of warps. Most of it is latencies: the bounds and positions, a row's group, the sums, the
-// starts.
+// A thread takes a stretch of the rows, the first warp the groups. Most of it is latencies: the bounds and positions, a
+// row's group, the sums. Every CTA does that much for itself, and then takes a part of the rows' and groups' records and of
+// the starts (one CTA of 1024 threads: 7.5 us for 64 rows, 2 of them the starts). What does not fit shared memory is left
+// to the first CTA alone.
 __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
   extern __shared__ __align__(16) uint8_t plan_smem[];
   PlanShared& sh = *reinterpret_cast<PlanShared*>(plan_smem);
@@ -174,6 +176,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
   pdl_wait();
   int ng = p.tile_items > 0 ? p.num_groups : 0;
   const bool fits = ng <= kPlanItems, fits_items = p.num_items <= kPlanItems;
+  if (!(fits && fits_items) && blockIdx.x > 0) return;
+  const int ctas_here = fits && fits_items ? kPlanCtas : 1;
   int2* state = fits ? sh.state : p.state;
   u64* leader = fits ? sh.leader : p.leader;
   const int first_pos = tid < p.num_items ? p.item_pos[tid] : -1, first_slot = tid < p.num_items ? p.item_slot[tid] : -1;
@@ -281,13 +285,13 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
   __syncthreads();
   int64_t all_own, all_whole;
   {
-    int64_t a = sh.sum[0][lane], b = sh.sum[1][lane];
+    int64_t a = lane < kPlanThreads / 32 ? sh.sum[0][lane] : 0, b = lane < kPlanThreads / 32 ? sh.sum[1][lane] : 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
+    for (int o = 1; o < kPlanThreads / 32; o <<= 1) {
       const int64_t c = __shfl_up_sync(kAll, a, o), d = __shfl_up_sync(kAll, b, o);
       if (lane >= o) a += c, b += d;
     }
-    all_own = __shfl_sync(kAll, a, 31), all_whole = __shfl_sync(kAll, b, 31);
+    all_own = __shfl_sync(kAll, a, kPlanThreads / 32 - 1), all_whole = __shfl_sync(kAll, b, kPlanThreads / 32 - 1);
     const int64_t c = __shfl_sync(kAll, a, (warp + 31) & 31), d = __shfl_sync(kAll, b, (warp + 31) & 31);
     if (warp > 0) x += c, y += d;
   }
@@ -319,24 +323,27 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
     if (per_i > 1) mine = row(i, false);
     if (sharing) share_row(mine);
     else mine.z = 0;
-    p.before[i] = pages;
+    if (blockIdx.x == 0) p.before[i] = pages;
     if (fits_items) sh.before[i] = pages, sh.item[i] = mine;
     pages += pages_in(mine) - mine.z;
   }
   const int64_t n_warps = (int64_t)(p.num_ctas - ctas) * kWarps;
   const int64_t share = n_warps ? max((int64_t)1, quotient(vpages + n_warps - 1, n_warps)) : 1;
   if (tid == 0) {
-    p.before[p.num_items] = all_pages;
+    if (blockIdx.x == 0) p.before[p.num_items] = all_pages;
     if (fits_items) sh.before[p.num_items] = all_pages;
     Header h;
     h.shared_ctas = ctas;
     h.cost = all_cost;
     h.share = share;
-    *p.header = h;
+    if (blockIdx.x == 0) *p.header = h;
   }
   __syncthreads();  // rows and groups are read across threads from here on
-  if (warp < 8) {
-    for (int i = tid; i < p.num_items; i += 256) {
+  // records and starts, one to a thread
+  const int64_t groups_end = (int64_t)p.num_items + (fits && sharing ? ng : 0), ctas_end = groups_end + ctas;
+  for (int64_t n = (int64_t)blockIdx.x * kPlanThreads + tid; n < ctas_end + n_warps; n += ctas_here * kPlanThreads) {
+    if (n < p.num_items) {
+      const int i = (int)n;
       int4 it = fits_items ? sh.item[i] : row(i, false);
       if (!fits_items && sharing) share_row(it);
       Item to = {it.x, it.y, it.z, 0, 0, 0, 0};
@@ -348,8 +355,11 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
         to.cost = gr.cost;
       }
       p.items[i] = to;
-    }
-    for (int c = tid; c < ctas; c += 256) {
+    } else if (n < groups_end) {
+      const int g = (int)(n - p.num_items);
+      p.groups[g] = sh.group[g];
+    } else if (n < ctas_end) {
+      const int c = (int)(n - groups_end);
       // the first step whose cost begins at or behind the CTA's share of the cost
       auto step_at = [&](int64_t cost, int& group, int64_t& local) {
         group = last_at_most(ng, cost, [&](int g) { return fits ? sh.group[g].cost : p.groups[g].cost; });
@@ -370,16 +380,13 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
         do st.g = fits ? sh.group[++st.group] : p.groups[++st.group];
         while (st.g.pages == 0);
       }
-      const int n = steps_of(st.g.pages);
-      st.unit = (int)quotient(local, n);
-      st.step = (int)(local - (int64_t)st.unit * n);
+      const int per = steps_of(st.g.pages);
+      st.unit = (int)quotient(local, per);
+      st.step = (int)(local - (int64_t)st.unit * per);
       st.count = (int)(end - begin);
       p.starts[c] = st;
-    }
-    if (fits && sharing)
-      for (int g = tid; g < ng; g += 256) p.groups[g] = sh.group[g];
-  } else {
-    for (int w = tid - 256; w < n_warps; w += kPlanThreads - 256) {
+    } else {
+      const int64_t w = n - ctas_end;
       const int64_t begin = w * share, end = min(begin + share, vpages);
       int4 from = make_int4(0, 0, 0, 0), of = make_int4(-1, -1, 0, 0);
       if (begin < end) {  // its row is the last that begins at or before it, so one that has pages
@@ -388,10 +395,10 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const Params p) {
         of = fits_items ? sh.item[i] : row(i, false);
         if (!fits_items && sharing) share_row(of);
         const int64_t at = begin - before(i) * vheads;
-        const int n = pages_in(of) - of.z;
+        const int own_pages = pages_in(of) - of.z;
         from.x = i;
-        from.y = (int)quotient(at, n);
-        from.z = of.z + (int)(at - (int64_t)from.y * n);
+        from.y = (int)quotient(at, own_pages);
+        from.z = of.z + (int)(at - (int64_t)from.y * own_pages);
         from.w = (int)min(end - begin, (int64_t)INT32_MAX);
       }
       const int64_t to = (int64_t)ctas * kWarps + w;
@@ -1232,7 +1239,7 @@ static int launch(const Params& p, cudaStream_t st) {
   auto attend = attend_kernel<D>;
   if (allow_shared(reinterpret_cast<const void*>(attend), Tile<D>::SMEM) != cudaSuccess) return CDB_ERR_CUDA;
   if (allow_shared(reinterpret_cast<const void*>(plan_kernel), sizeof(PlanShared)) != cudaSuccess ||
-      launch_pdl(plan_kernel, dim3(1), dim3(kPlanThreads), sizeof(PlanShared), st, p) != cudaSuccess)
+      launch_pdl(plan_kernel, dim3(kPlanCtas), dim3(kPlanThreads), sizeof(PlanShared), st, p) != cudaSuccess)
     return CDB_ERR_CUDA;
   if (launch_pdl(attend, dim3(p.num_ctas), dim3(kThreads), Tile<D>::SMEM, st, map, p) != cudaSuccess)
     return CDB_ERR_CUDA;
