@@ -27,12 +27,16 @@ namespace cdb {
 namespace sample {
 
 constexpr int kMaxWarps = 32;
-constexpr int kHalf = 4096;              // bins of one sign: 32 octaves of 128
-constexpr int kBins = 2 * kHalf + 1;     // largest logits first; bin kHalf holds 0
-template <int kThreads>
-constexpr int kPadded = (kBins + kThreads) / kThreads * kThreads;  // and room for kNone
-constexpr int kList = 8192;              // fp32 tokens next to a border
-constexpr int kNone = kBins;             // no bin: weighs nothing
+// Bins, 128 to an octave, largest logits first. fp32 does with 16 octaves: what is smaller is next to 0 and all but equal.
+template <typename T>
+struct Bins {
+  static constexpr int kHalf = sizeof(T) == 4 ? 2048 : 4096;  // of one sign; bin kHalf holds 0
+  static constexpr int kBins = 2 * kHalf + 1;
+  static constexpr int kNone = kBins;  // no bin: weighs nothing
+  template <int kThreads>
+  static constexpr int kPadded = (kBins + kThreads) / kThreads * kThreads;  // and room for kNone
+};
+constexpr int kList = 8192;  // fp32 tokens next to a border
 constexpr uint32_t kAll = 0xffffffffu;
 typedef unsigned long long u64;
 
@@ -128,6 +132,7 @@ struct Row {
 struct Scratch {
   u64 sum[kMaxWarps];
   u64 sum2[kMaxWarps];
+  u64 sum3[kMaxWarps];
 };
 
 // Sum of the threads before this one, and of all.
@@ -153,6 +158,26 @@ __device__ __forceinline__ u64 scan(u64 mine, u64& all, u64* red) {
   all = __shfl_sync(kAll, w, kWarps - 1);
   const u64 before = __shfl_sync(kAll, w, (warp + 31) & 31);
   return (warp ? before : 0) + x - mine;
+}
+// Sums of three numbers over the CTA, to all threads.
+template <int kThreads>
+__device__ __forceinline__ void block_sums(u64& a, u64& b, u64& c, Scratch& sc) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto over_warp = [&] {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      a += __shfl_xor_sync(kAll, a, o);
+      b += __shfl_xor_sync(kAll, b, o);
+      c += __shfl_xor_sync(kAll, c, o);
+    }
+  };
+  over_warp();
+  __syncthreads();
+  if (lane == 0) sc.sum[warp] = a, sc.sum2[warp] = b, sc.sum3[warp] = c;
+  __syncthreads();
+  const bool in = lane < kThreads / 32;
+  a = in ? sc.sum[lane] : 0, b = in ? sc.sum2[lane] : 0, c = in ? sc.sum3[lane] : 0;
+  over_warp();
 }
 template <int kThreads>
 __device__ __forceinline__ u64 block_sum(u64 v, u64* red) {
@@ -272,12 +297,14 @@ struct FastWeigher {
 // by counting for each the larger ones, 4 threads or more to each (64: 0.3 us, where the steps below take 3).
 template <int kThreads>
 __device__ __forceinline__ void sort(u64* list, int size) {
-  if (size * 4 <= kThreads) {
+  if (size * 2 <= kThreads) {
     const int parts = min(32, kThreads / size), at = threadIdx.x / parts, part = threadIdx.x % parts;
     const u64 mine = at < size ? list[at] : 0;
     int larger = 0;
-    if (at < size)
+    if (at < size) {
+#pragma unroll 8
       for (int i = part; i < size; i += parts) larger += list[i] > mine;
+    }
     for (int o = parts / 2; o > 0; o >>= 1) larger += __shfl_xor_sync(kAll, larger, o);
     __syncthreads();
     if (at < size && part == 0 && mine != 0) list[larger] = mine;
@@ -397,20 +424,31 @@ __device__ __noinline__ void slow_row(const Params& p, int r, uint32_t top, floa
 
 // ---------------------------------------------------------------------------------- bins
 
-// `low`: (least biased exponent of the bins' 32 octaves) * 128, at least 128.
+// `low`: (least biased exponent of the bins' octaves) * 128, at least 128.
 // Logits of smaller magnitude share 0's bin (bf16 rows that have such go the slow way); larger ones, infinities and NaN have
 // none.
+template <typename T>
 __device__ __forceinline__ int bin_of(float x, int low) {
+  constexpr int kHalf = Bins<T>::kHalf;
   const int b = __float_as_int(x);
   const int off = max(((b >> 16) & 0x7fff) - (low - 1), 0);
-  return off <= kHalf ? (b < 0 ? kHalf + off : kHalf - off) : kNone;
+  return off <= kHalf ? (b < 0 ? kHalf + off : kHalf - off) : Bins<T>::kNone;
 }
 // The least magnitude of a bin's logits, signed.
+template <typename T>
 __device__ __forceinline__ float logit_of_bin(int bin, int low) {
+  constexpr int kHalf = Bins<T>::kHalf;
   if (bin == kHalf) return 0.f;
   const int off = bin < kHalf ? kHalf - bin : bin - kHalf;
   const uint32_t mag = (uint32_t)(off - 1 + low) << 16;
   return __uint_as_float(bin < kHalf ? mag : mag | 0x80000000u);
+}
+// The least of the logits in a bin or above it. (Above all bins, -1: none that a row has.)
+template <typename T>
+__device__ __forceinline__ float least_of_bin(int bin, int low) {
+  constexpr int kHalf = Bins<T>::kHalf;
+  if (bin < kHalf) return logit_of_bin<T>(bin, low);
+  return __uint_as_float(0x80000000u | (((uint32_t)(bin - kHalf + low) << 16) - 1));
 }
 
 struct Shared {
@@ -428,13 +466,16 @@ struct Shared {
 template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const Params p) {
   constexpr bool WIDE = sizeof(T) == 4;
-  constexpr int N = Row<T>::N, kWarps = kThreads / 32, kBinsPadded = kPadded<kThreads>, kPerThread = kBinsPadded / kThreads;
+  constexpr int N = Row<T>::N, kWarps = kThreads / 32;
+  constexpr int kHalf = Bins<T>::kHalf, kBins = Bins<T>::kBins, kNone = Bins<T>::kNone;
+  constexpr int kBinsPadded = Bins<T>::template kPadded<kThreads>, kPerThread = kBinsPadded / kThreads;
+  constexpr int kWide = kBinsPadded > kList ? kBinsPadded : kList;
   pdl_trigger();
   extern __shared__ __align__(16) uint8_t smem[];
   uint32_t* counts = reinterpret_cast<uint32_t*>(smem);                 // [kBinsPadded + 4]
-  u64* weights = reinterpret_cast<u64*>(smem + (kBinsPadded + 4) * 4);  // [kBinsPadded + 1]
+  u64* weights = reinterpret_cast<u64*>(smem + (kBinsPadded + 4) * 4);  // [kWide + 2]
   u64* list = weights;                                                  // or [kList] {key, ~index}
-  uint2* table = reinterpret_cast<uint2*>(smem + (kBinsPadded + 4) * 4 + (kBinsPadded + 2) * 8);  // [kTable]
+  uint2* table = reinterpret_cast<uint2*>(smem + (kBinsPadded + 4) * 4 + (kWide + 2) * 8);  // [kTable]
   __shared__ Shared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.x;
   for (int i = tid; i < (kBinsPadded + 4) / 4; i += kThreads) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
@@ -515,13 +556,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   // below this no weight is left
   const float cutoff = fmaxf(top - t * (0.694f * (float)(p.scale_bits + 2)) - 1e-6f * fabsf(top), -3.4e38f);
   const float widest = fmaxf(fabsf(top), fabsf(fmaxf(least, cutoff)));
-  const int low = max((int)(__float_as_uint(widest) >> 23) - 31, 1) * 128;
+  const int low = max((int)(__float_as_uint(widest) >> 23) - (kHalf / 128 - 1), 1) * 128;
 
   // ---- top-k of a few
   if (by_k && k <= kThreads / 2) {
     // The bin of the k-th largest of the threads' largest: at least k tokens are in it or above. Where fewer threads
     // have any, or theirs weigh nothing, there is none, and every token that weighs is taken.
-    const int my_bin = bin_of(my_top, low);
+    const int my_bin = bin_of<T>(my_top, low);
     if (my_bin != kNone) atomicAdd(&counts[my_bin], 1u);
     __syncthreads();
     const int b0 = tid * kPerThread;
@@ -535,9 +576,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       before += counts[b0 + i];
     }
     __syncthreads();
-    // the least logit of that bin (of a negative or zero's, one that is less)
     const int hi = sh.hi_bin;
-    const float from = hi < 0 ? fmaxf(least, cutoff) : logit_of_bin(hi < kHalf ? hi : hi + 1, low);
+    const float from = hi < 0 ? fmaxf(least, cutoff) : least_of_bin<T>(hi, low);
 #pragma unroll 4
     for (int j = tid; j < row.vectors; j += kThreads) {
       if (!row.reaches(j, from)) continue;
@@ -597,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   if (bins) {
     bool strange = false;
     // fp32: the mean logit of the bins whose tokens weigh e^-6 or more, of which few may make up the total
-    const int heavy = WIDE && by_p ? bin_of(top - 6.f * t, low) : -1;
+    const int heavy = WIDE && by_p ? bin_of<T>(top - 6.f * t, low) : -1;
     if (WIDE && by_p) {
       for (int i = tid; i < kBinsPadded; i += kThreads) weights[i] = 0;
       __syncthreads();
@@ -608,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       row.load(j, x);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int bin = bin_of(x[i], low);
+        const int bin = bin_of<T>(x[i], low);
         if (!WIDE) strange |= bin == kHalf && x[i] != 0.f;
         if (bin != kNone) atomicAdd(&counts[bin], 1u);
         if (WIDE && bin <= heavy && bin != kNone)
@@ -624,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     for (int b = tid; b < kBins; b += kThreads) {
       const uint32_t n = counts[b];
       if (n == 0) continue;
-      float l = logit_of_bin(b, low);
+      float l = logit_of_bin<T>(b, low);
       if (WIDE && b != kHalf) {
         const uint32_t in = b <= heavy ? (uint32_t)__fdividef((float)(uint32_t)weights[b], (float)n) : 0x8000u;
         l = fminf(__uint_as_float(__float_as_uint(l) + in), top);
@@ -660,11 +700,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     u64 slack = 0;
     if (WIDE && by_p) {
       float off = 0.f;
+      const float per_width = 0.0078125f / t;
 #pragma unroll 3
       for (int i = 0; i < kPerThread; ++i) {
         const int b = b0 + i;
         if (counts[b] == 0 || b == kHalf || b <= heavy) continue;
-        const float width = fabsf(logit_of_bin(b, low)) * 0.0078125f / t;  // at most
+        const float width = fabsf(logit_of_bin<T>(b, low)) * per_width;  // at most
         const float one_off = (float)weights[b] * fminf(0.5f * width, 4.f);
         off += (float)counts[b] * one_off * one_off * 0.333f;
       }
@@ -730,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       row.load(j, x);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int bin = bin_of(x[i], low);
+        const int bin = bin_of<T>(x[i], low);
         sum += weights[bin];
         ties += bin == edge;
       }
@@ -758,7 +799,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       row.load(j, x);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int bin = bin_of(x[i], low);
+        const int bin = bin_of<T>(x[i], low);
         mine += weights[bin];
         mine_ties += bin == edge && edge != kNone;
       }
@@ -773,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
         row.load(j, x);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const int bin = bin_of(x[i], low);
+          const int bin = bin_of<T>(x[i], low);
           u64 w = weights[bin];
           if (bin == edge && edge != kNone && my_seen++ < edge_n) w = edge_w;
           if (my_run <= in.target && in.target < my_run + w) {
@@ -790,8 +831,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   const bool edged = WIDE && bins && sh.hi_bin >= 0;  // (top-k of more tokens than weigh anything leaves all)
   const int lo = edged ? sh.lo_bin : kNone, hi = edged ? sh.hi_bin : kNone;
   const bool all_rest = by_p && !sh.k_border;  // the total that top-p takes a share of goes on below the list
-  u64 sum = 0, rest = 0, all_above = 0;
-  uint32_t above_n = 0;
+  u64 sum = 0, total = 0, above_w = 0;
   if (!edged) {
 #pragma unroll 2
     for (int j = v0 + lane; j < v1; j += 32) {
@@ -804,31 +844,33 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       }
     }
   } else {
+    const float from_above = least_of_bin<T>(lo - 1, low), from_list = least_of_bin<T>(hi, low);
 #pragma unroll 2
     for (int j = v0 + lane; j < v1; j += 32) {
       float x[N];
       row.load(j, x);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int bin = bin_of(x[i], low);
         const u64 w = weigh(x[i]);
-        const bool above = bin < lo;
-        above_n += above;
-        all_above += above ? w : 0;
-        sum += above && w >= least_w ? w : 0;
-        rest += bin > hi ? w : 0;
-        if (!above && bin <= hi) {
+        const bool above = x[i] >= from_above;
+        total += w;
+        above_w += above ? w : 0;
+        if (by_m) sum += above && w >= least_w ? w : 0;
+        if (!above && x[i] >= from_list) {
           const int at = atomicAdd(&sh.list_n, 1);
           if (at < kList) list[at] = (u64)key_of(x[i]) << 32 | (uint32_t)~(j * N - row.shift + i);
         }
       }
     }
-    if (!all_rest) rest = 0;
+    if (!by_m) sum = above_w;
   }
   u64 edge = 0;  // tokens at or above it (key, then lower indexes) are kept
   if (edged) {
-    const u64 above_w = block_sum<kThreads>(all_above, sh.sc.sum), rest_w = block_sum<kThreads>(rest, sh.sc.sum);
-    const u64 n_above = block_sum<kThreads>(above_n, sh.sc.sum);
+    u64 n_above = 0;  // (these bins have all their tokens)
+#pragma unroll 3
+    for (int i = 0; i < kPerThread; ++i)
+      if (tid * kPerThread + i < lo) n_above += counts[tid * kPerThread + i];
+    block_sums<kThreads>(above_w, total, n_above, sh.sc);
     const int n = sh.list_n;
     if (n > kList) {
       slow_row<T, kThreads>(p, r, key_of(top), t, sh.sc);
@@ -847,8 +889,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     for (int i = i0; i < i1; ++i)
       if (i < n && (u64)i < left_k) mine += weigh(logit_of((uint32_t)(list[i] >> 32)));
     u64 mass = above_w + scan<kThreads>(mine, all_w, sh.sc.sum);
-    const u64 total = above_w + all_w + rest_w;
-    const u64 want = by_p ? share_of(tp, total, true) : ~0ull;
+    // (where all_rest holds, all_w is the list's whole mass)
+    const u64 rest_w = all_rest ? total - above_w - all_w : 0;
+    const u64 want = by_p ? share_of(tp, above_w + all_w + rest_w, true) : ~0ull;
     if (tid == 0) sh.edge = 0, sh.list_over = 0;
     __syncthreads();
     // The last token kept; the first of all always is. A top-p border outside the list is a slow row.
@@ -924,9 +967,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
 
 template <typename T, int kThreads>
 static int launch(const Params& p, int rows, cudaStream_t st) {
-  constexpr int kBinsPadded = kPadded<kThreads>;
-  constexpr int SMEM = (kBinsPadded + 4) * 4 + (kBinsPadded + 2) * 8 + kTable * 8;
-  static_assert(kBinsPadded > kNone && kBinsPadded >= kList, "room for either use");
+  constexpr int kBinsPadded = Bins<T>::template kPadded<kThreads>, kWide = kBinsPadded > kList ? kBinsPadded : kList;
+  constexpr int SMEM = (kBinsPadded + 4) * 4 + (kWide + 2) * 8 + kTable * 8;
+  static_assert(kBinsPadded > Bins<T>::kNone, "room for no bin");
   static_assert(1024 / kThreads * (SMEM + 2048) <= 228 * 1024, "CTAs an SM");
   auto kernel = sample_kernel<T, kThreads>;
   if (allow_shared(reinterpret_cast<const void*>(kernel), SMEM) != cudaSuccess) return CDB_ERR_CUDA;
