@@ -87,27 +87,38 @@ struct Row {
     shift = (int)((reinterpret_cast<uintptr_t>(at) & 15) / sizeof(T));
     vectors = (vocab + shift + N - 1) / N;
   }
-  // Largest and least of a vector.
-  __device__ __forceinline__ void range(int j, float& top, float& least) const {
-    const int i = j * N - shift;
-    if (N == 8 && i >= 0 && i + N <= vocab) {  // two at a time
-      const uint4 w = *reinterpret_cast<const uint4*>(at + i);
+  // The vectors that lie in the row whole are [full0, full1); of one at either end `edge` gives a thread its own, or -1.
+  __device__ __forceinline__ int full0() const { return shift != 0; }
+  __device__ __forceinline__ int full1() const { return (vocab + shift) / N; }
+  __device__ __forceinline__ int edge() const {
+    const int at = threadIdx.x == 0 ? (shift ? 0 : -1) : threadIdx.x == 1 ? full1() : -1;
+    return threadIdx.x == 1 && (at == vectors || at < full0()) ? -1 : at;
+  }
+  __device__ __forceinline__ uint4 whole(int j) const { return *reinterpret_cast<const uint4*>(at + (j * N - shift)); }
+  // Largest, and least, of a whole vector.
+  __device__ __forceinline__ static float largest(const uint4& w) {
+    if constexpr (N == 8) {  // two at a time
       const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(&w);
       const __nv_bfloat162 a = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
-      const __nv_bfloat162 b = __hmin2(__hmin2(v[0], v[1]), __hmin2(v[2], v[3]));
-      top = fmaxf(top, fmaxf(__low2float(a), __high2float(a)));
-      least = fminf(least, fminf(__low2float(b), __high2float(b)));
-      return;
+      return fmaxf(__low2float(a), __high2float(a));
+    } else {
+      return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
     }
-    float x[N];
-    load(j, x);
-#pragma unroll
-    for (int k = 0; k < N; ++k) top = fmaxf(top, x[k]), least = fminf(least, x[k]);
   }
-  __device__ __forceinline__ bool reaches(int j, float from) const {
-    float top = -INFINITY, least = INFINITY;
-    range(j, top, least);
-    return top >= from;
+  __device__ __forceinline__ static float least(const uint4& w) {
+    if constexpr (N == 8) {
+      const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(&w);
+      const __nv_bfloat162 a = __hmin2(__hmin2(v[0], v[1]), __hmin2(v[2], v[3]));
+      return fminf(__low2float(a), __high2float(a));
+    } else {
+      return fminf(fminf(__uint_as_float(w.x), __uint_as_float(w.y)), fminf(__uint_as_float(w.z), __uint_as_float(w.w)));
+    }
+  }
+  // f(token, logit) for every token of a vector.
+  template <typename F>
+  __device__ __forceinline__ void each(int j, F f) const {
+#pragma unroll 1
+    for (int i = max(j * N - shift, 0); i < min(j * N - shift + N, vocab); ++i) f(i, load_one<T>(at, i));
   }
   // Tokens outside the row come as NaN, which weighs nothing.
   __device__ __forceinline__ void load(int j, float (&x)[N]) const {
@@ -491,7 +502,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   // ---- the largest logit, and the least
   float top = -INFINITY, least = INFINITY;  // (maxima and minima leave NaN out)
 #pragma unroll 8
-  for (int j = tid; j < row.vectors; j += kThreads) row.range(j, top, least);
+  for (int j = row.full0() + tid; j < row.full1(); j += kThreads) {
+    const uint4 w = row.whole(j);
+    top = fmaxf(top, Row<T>::largest(w)), least = fminf(least, Row<T>::least(w));
+  }
+  const int my_edge = row.edge();  // (these threads have that vector too)
+  if (my_edge >= 0) row.each(my_edge, [&](int, float x) { top = fmaxf(top, x), least = fminf(least, x); });
   const float my_top = top;
   {
     uint32_t a = key_of(top), b = key_of(least);
@@ -513,12 +529,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   }
   if (greedy) {
     int first = INT32_MAX;
-    for (int j = tid; j < row.vectors && my_top == top; j += kThreads) {
-      float x[N];
-      row.load(j, x);
-#pragma unroll
-      for (int k = N - 1; k >= 0; --k)
-        if (x[k] == top) first = min(first, j * N - row.shift + k);
+    if (my_top == top) {
+      auto find = [&](int i, float x) {
+        if (x == top) first = min(first, i);
+      };
+      for (int j = row.full0() + tid; j < row.full1(); j += kThreads)
+        if (Row<T>::largest(row.whole(j)) == top) row.each(j, find);
+      if (my_edge >= 0) row.each(my_edge, find);
     }
     first = __reduce_min_sync(kAll, first);
     __syncthreads();
@@ -578,17 +595,30 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     __syncthreads();
     const int hi = sh.hi_bin;
     const float from = hi < 0 ? fmaxf(least, cutoff) : least_of_bin<T>(hi, low);
-#pragma unroll 4
-    for (int j = tid; j < row.vectors; j += kThreads) {
-      if (!row.reaches(j, from)) continue;
-      float x[N];
-      row.load(j, x);
+    if (my_top >= from) {
+      for (int j = row.full0() + tid, e = my_edge; j < row.full1() || e >= 0; j += 4 * kThreads) {
+        uint32_t hits = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (x[i] >= from) {
-          const int at = atomicAdd(&sh.list_n, 1);
-          if (at < kList) list[at] = (u64)key_of(x[i]) << 32 | (uint32_t)~(j * N - row.shift + i);
+        for (int i = 0; i < 4; ++i)
+          if (j + i * kThreads < row.full1()) hits |= (uint32_t)(Row<T>::largest(row.whole(j + i * kThreads)) >= from) << i;
+        if (e >= 0) hits |= 16;
+        for (; hits != 0; hits &= hits - 1) {
+          const int at = hits & 15 ? j + (__ffs(hits) - 1) * kThreads : e;
+          float x[N];
+          row.load(at, x);
+          uint32_t in = 0;
+#pragma unroll
+          for (int i = 0; i < N; ++i) in |= (uint32_t)(x[i] >= from) << i;
+          int to = in != 0 ? atomicAdd(&sh.list_n, __popc(in)) : 0;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            if ((in >> i & 1) == 0) continue;
+            if (to < kList) list[to] = (u64)key_of(x[i]) << 32 | (uint32_t)~(at * N - row.shift + i);
+            ++to;
+          }
         }
+        e = -1;
+      }
     }
     if (my_bin != kNone) counts[my_bin] = 0;  // (only that bin's threads, and for whoever comes next)
     __syncthreads();
