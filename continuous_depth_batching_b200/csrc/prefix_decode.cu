@@ -16,15 +16,24 @@
 // comes from in tensor memory, V as it lies in the cache (the product's inner index across its rows). Each team takes a
 // tile through every step; a tile without a partner is taken by both teams, every other step to each. So one team's
 // exponentials run beside the other's products, and a step's keys are read once for 256 rows. One warp issues
-// each team's products, one brings the pages of K and one those of V (TMA, 128-byte swizzle; a warp takes some 80 cycles to
-// issue a copy, so one for both was what bounded a step), five steps ahead.
+// each team's products, one brings the pages of K and one those of V (TMA, 128-byte swizzle; one warp for both was what
+// bounded a step), five steps ahead.
 //
 // Pages of single rows. The pages of all (row, kv head, up to 8 query heads) form one stream that is cut into equal
 // shares for the warps of the other CTAs. A warp brings its pages into a ring of its own (two pages of 8 KB at 128; with
 // 12 warps 192 KB of an SM are on their way) and multiplies them by m16n8k16 products: S^T = K Q^T, O^T = V^T P^T.
 //
-// The weights P are rounded to bf16 for their product with V (2^-8 of each), V's type; l is the sum of the
-// rounded weights, so what is common to them cancels. m only moves when passed by 8, which bf16's range allows.
+// The weights P are rounded to bf16 for their product with V (2^-8 of each), V's type. l is their sum in fp32: single rows
+// sum the rounded weights, so what is common to them cancels; shared steps, where that took 5 % longer, those before.
+// m only moves when passed by 8, which bf16's range allows.
+//
+// What bounds it (16 to 32 heads of 128, B200 at 1.8 GHz). Single rows: memory, 64 x 600 tokens on 16 kv heads 28 us of
+// which 24 are their bytes at 6.6 TB/s, plus the plan and the join. Shared steps of one tile: memory too, 32 KB in 0.6 us. Of two
+// tiles: a warp's chain, 1700 cycles to a step: 220 until S is there, 100 to read it, 225 for the maximum, 1195 for the
+// weights, the other team's on the same unit (1024 of them are 2 x 64 x 8 of the exponential unit). The tensor cores take
+// 1024 (1280: at 64 keys S reads q from shared memory faster than that delivers). Measured against it: a quarter of the
+// weights by a cubic on the other pipe, 4 % less time for another rounding and NaNs that it hides; more of them, none.
+// The plan takes 5 us and the join 5 to 10, most of it waiting for what the launch before wrote.
 #include <cuda.h>
 
 #include "tcgen05.cuh"
@@ -113,6 +122,25 @@ struct Params {
   int32_t* status;
 };
 
+// Two at a time.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -140,10 +168,10 @@ __device__ __forceinline__ int last_at_most(int n, int64_t x, F value) {
   return lo;
 }
 
-// How a call's work is cut, in units of 1/64 us, measured at 16 and 32 heads of 128: a CTA takes 1 us to a step (HBM) and
-// 1.3 where both teams have 128 rows (exponentials), 0.16 us to a page of single rows. Sharing costs another
-// 4 us (more parts, q, tensor memory), so few rows on a short prompt are faster each by itself: 4 rows on 700 tokens, 16
-// heads, take 17 us so and 24 shared.
+// How a call's work is cut, in units of 1/64 us, measured at 16 and 32 heads of 128 as what divides a call best: a CTA
+// takes 1 us to a step (HBM) and 1.3 where both teams have 128 rows (exponentials), 0.16 us to a page of single rows.
+// Sharing costs another 4 us (more parts, q, tensor memory), so few rows on a short prompt are faster each by itself: 4
+// rows on 700 tokens, 16 heads, take 14 us so and 21 shared.
 constexpr int kStepCost = 62, kPairCost = 83, kPageCost = 10, kSharedCost = 256;
 // Of a step of a group of `rows` (row, head)s, `full` to a tile.
 __device__ __forceinline__ int step_cost(int rows, int full) {
@@ -468,6 +496,18 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
       : "memory");
 }
 
+// One lane of a converged warp. (The compiler knows of this one, and not of a compared lane number, that what follows
+// runs on a single lane: products, copies and commits then take their operands straight from uniform registers.)
+__device__ __forceinline__ bool elect() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
 // The CTA's way through its share of the steps, one unit at a time.
 struct Walk {
   Start at;
@@ -522,7 +562,7 @@ __device__ __forceinline__ void shared_steps(const CUtensorMap& map, const Param
   constexpr uint32_t kIdescS = kBf16 | ((uint32_t)(TK >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
   constexpr uint32_t kIdescO = kBf16 | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
   const uint32_t base = smem_u32(smem);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(kAll, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int* abort = &sh.abort;
   Walk w;
 
@@ -535,8 +575,7 @@ __device__ __forceinline__ void shared_steps(const CUtensorMap& map, const Param
     const uint32_t tiles = base + (values ? T::OFF_V : T::OFF_K);
     int t = 0;
     bool ok = true;
-    // lane: page (lane & 3) of the step, 64 columns from 64 * (lane >> 2) on
-    const int page_of = lane & 3, atom = lane >> 2;
+    const int page_of = lane & 3;  // of the step
     for (w.begin(p, start); w.on() && ok; w.next(p)) {
       const int32_t* bt = p.block_table + (int64_t)w.g.slot * p.bt_stride;
       auto fetch = [&](int n) {
@@ -552,14 +591,18 @@ __device__ __forceinline__ void shared_steps(const CUtensorMap& map, const Param
         const int row = have ? id * kBlock + (values ? (int)p.kv_rows : 0) : 2 * (int)p.kv_rows;
         if (t >= R) ok = __all_sync(kAll, wait_for(&free[slot], (t / R + 1) & 1, p.status, abort));  // by step t - R
         if (!ok) break;
-        if (lane == 0) {
+        int rows[kStepPages];
+#pragma unroll
+        for (int i = 0; i < kStepPages; ++i) rows[i] = __shfl_sync(kAll, row, i);
+        if (elect()) {
           if (!values) sh.missing[t % kMissing] = (int)gone;
           mbar_arrive_expect_tx(&full[slot], T::STAGE);
+#pragma unroll
+          for (int i = 0; i < kStepPages * T::ATOMS; ++i)
+            load_box(tiles + slot * T::STAGE + i / kStepPages * (TK * 128) + i % kStepPages * T::BOX, &map,
+                     i / kStepPages * 64, w.kvh, rows[i % kStepPages], smem_u32(&full[slot]));
         }
         __syncwarp();
-        if (atom < T::ATOMS)
-          load_box(tiles + slot * T::STAGE + atom * (TK * 128) + page_of * T::BOX, &map, atom * 64, w.kvh, row,
-                   smem_u32(&full[slot]));
         if (!values && lane < kStepPages && !have && id != INT32_MIN) set_error(p.status, CDB_ERR_INDEX);
         id = next;
         next = after;
@@ -586,8 +629,8 @@ __device__ __forceinline__ void shared_steps(const CUtensorMap& map, const Param
       commit(&tm.odone[buffer & 1]);
       commit(&sh.vfree[step % R]);
     };
-    for (w.begin(p, start); w.on(); w.next(p), ++c) {
-      if (lane == 0 && ok) {
+    if (elect()) {
+      for (w.begin(p, start); w.on() && ok; w.next(p), ++c) {
         ok = wait_for(&sh.qfull, c & 1, p.status, abort);
         const uint32_t q = base + (w.both ? team * T::Q : 0);
         int done = -1;  // the team's last step, whose weights are still to come
@@ -621,9 +664,7 @@ __device__ __forceinline__ void shared_steps(const CUtensorMap& map, const Param
         }
         if (ok && done >= 0) weigh(done, j - 1, add);
       }
-      __syncwarp();
-    }
-    if (lane == 0) {  // on every path: no product may run when the tensor memory is freed
+      // on every path: no product may run when the tensor memory is freed
       commit(&tm.drain);
       mbar_wait(&tm.drain, 0, p.status);
     }
@@ -715,24 +756,30 @@ __device__ __forceinline__ void shared_steps(const CUtensorMap& map, const Param
             m = to;
           }
           const float off = m == -INFINITY ? 0.f : -m;  // (nothing seen yet)
-          float sum = 0.f, more = 0.f;
+          // (pairs take one instruction: 124 us of steps became 118)
+          const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), off2 = make_float2(off, off);
+          float2 sum = make_float2(0.f, 0.f), more = sum;
 #pragma unroll
           for (int b = 0; b < TK / 16; ++b) {
             uint32_t x[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              x[k] = pack_bf16x2(ex2(fmaf(__uint_as_float(s[b * 16 + 2 * k]), p.scale_log2, off)),
-                                 ex2(fmaf(__uint_as_float(s[b * 16 + 2 * k + 1]), p.scale_log2, off)));
-              sum += bf16lo(x[k]);
-              more += bf16hi(x[k]);
+              const float2 y = fma2(make_float2(__uint_as_float(s[b * 16 + 2 * k]), __uint_as_float(s[b * 16 + 2 * k + 1])),
+                                    scale2, off2);
+              const float2 e = make_float2(ex2(y.x), ex2(y.y));
+              x[k] = pack_bf16x2(e.x, e.y);
+              if (k & 1) more = add2(more, e);
+              else sum = add2(sum, e);
             }
             tmem_store8(tmem + (j & 1) * TK + b * 8, x);
           }
-          l += sum + more;
+          sum = add2(sum, more);
+          l += sum.x + sum.y;
           wait_stores();
         }
         fence_before();
-        mbar_arrive(&tm.pfull[j & 1]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tm.pfull[j & 1]);
         some = true;
         ++j;
       }
@@ -1054,7 +1101,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 4; ++i) {
       Shared::Team& tm = sh.team[i >> 1];
       mbar_init(&tm.sfull[i & 1], 2);
-      mbar_init(&tm.pfull[i & 1], TM);
+      mbar_init(&tm.pfull[i & 1], TM / 32);
       mbar_init(&tm.odone[i & 1], 1);
       if (i & 1) mbar_init(&tm.drain, 1);
     }
