@@ -20,7 +20,15 @@
 //      where the border falls into a bin, its neighbourhood's tokens are collected, sorted and summed exactly;
 //   4. the stretch in which the target lies, a few tokens to a thread.
 // Rows that this does not fit (an infinite largest logit, bf16 logits over more than 32 octaves, a border among more
-// fp32 tokens than the list holds) take `slow_row`, which finds its borders by bisection, a bit of the key a pass.
+// fp32 tokens than the list holds) take `slow_row`, which finds its borders by bisection, a bit of the key a pass: 0.3 to
+// 0.7 ms at 49152 tokens (all logits equal; a border in bf16 where some logit is 2^-32 of another).
+//
+// What bounds it: instructions, and for a few rows a chain of passes with a barrier or a scan after each. A weight is some
+// 25 instructions, so 256 rows of 65536 plain take 31 us (5 of HBM; 0.58 instructions a cycle and scheduler); counting
+// into bins 12 cycles a warp of tokens (shared atomics on 32 banks, most of the 18 us of that pass), so 256 fp32 rows of
+// 49152 with top-p take 82 us: 4 the largest, 18 bins, 6 their weights and sums, 19 the weights above and below the border,
+// 8 its list, 6 the token. One row with top-k of 50: 12 us, in steps of 1 to 2. With 32 octaves of bins
+// for fp32, and every token's bin for its sums, those 82 us were 95; one CTA an SM for 256 rows is slower than two of 512 threads.
 #include "cdb_common.cuh"
 
 namespace cdb {
@@ -492,7 +500,10 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   for (int i = tid; i < (kBinsPadded + 4) / 4; i += kThreads) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
   for (int i = tid; i < kTable; i += kThreads) table[i] = g_powers.at[i];
   if (tid == 0) sh.unit = 1. / (double)(1ull << p.scale_bits);
-  if (tid == 0) sh.edge_bin = kNone, sh.edge_count = 0, sh.lo_bin = kBinsPadded, sh.hi_bin = -1, sh.list_n = 0, sh.list_over = 0, sh.k_border = 0;
+  if (tid == 0) {
+    sh.edge_bin = kNone, sh.edge_count = 0, sh.lo_bin = kBinsPadded, sh.hi_bin = -1;
+    sh.list_n = 0, sh.list_over = 0, sh.k_border = 0;
+  }
   pdl_wait();
   const Row<T> row(p, r);
   const float t = p.temperature[r];
@@ -1037,6 +1048,7 @@ extern "C" int cdb_sample_tokens(const void* logits, int logits_fp32, int64_t lo
   p.scale_bits = 62 - bits < 46 ? 62 - bits : 46;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // One CTA an SM has the whole SM while there are no more rows than SMs; two share it where there are more.
-  if (num_rows <= 148) return logits_fp32 ? launch<float, 1024>(p, num_rows, st) : launch<__nv_bfloat16, 1024>(p, num_rows, st);
+  if (num_rows <= 148)
+    return logits_fp32 ? launch<float, 1024>(p, num_rows, st) : launch<__nv_bfloat16, 1024>(p, num_rows, st);
   return logits_fp32 ? launch<float, 512>(p, num_rows, st) : launch<__nv_bfloat16, 512>(p, num_rows, st);
 }

@@ -1,4 +1,5 @@
-// torch.ops.cdb.* of the low-bit decode step and of many continuations of one prompt: argument checks (types and shapes first, then the device,
+// torch.ops.cdb.* of the low-bit decode step and of many continuations of one prompt: argument checks (types and shapes
+// first, then the device,
 // so that a call with CPU tensors is told what else is wrong with it), workspaces and the launch on the current
 // stream, over the C ABI. In C++ because a decode step makes hundreds of these calls and each kernel
 // takes a few microseconds: the same checks cost 17 us of host time a call in Python.

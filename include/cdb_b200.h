@@ -623,6 +623,8 @@ int64_t cdb_prefix_decode_workspace_floats(int num_items, int num_groups, int nu
  *                Group bounds that descend or leave [0, num_items] set CDB_ERR_INDEX, and no blocks are shared.
  *   workspace    cdb_prefix_decode_workspace_floats elements, 16-byte aligned, in any state. Calls that share it
  *                must be ordered. scale > 0.
+ *   num_sms      CTAs that the work is cut for, 2 to 1023. It fixes the order of the sums, and so the result's last bits.
+ * Rows of more than 128 query heads a kv head share nothing.
  * CDB_ERR_UNSUPPORTED above 2^30 - 17 cache rows or 2^30 - 1 (row, head)s. */
 int cdb_prefix_decode_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const void* kv_base,
                                 int num_cache_layers, int64_t kv_rows, int cache_layer, const int32_t* block_table,
@@ -645,7 +647,7 @@ int cdb_prefix_decode_attention(const void* q, int64_t q_stride, void* out, int6
  *   out_ids    int64 [num_rows]; out_logprobs fp32 [num_rows] or NULL: log of the token's share of the kept weights.
  * Logits: NaN counts as -inf and is never drawn; where the largest is +inf, tokens at +inf weigh 1 and
  * others 0. A row without a logit above -inf gives id -1 and log-probability NaN. Weights are whole
- * multiples of 2^-S of the largest, S = min(48, 62 - ceil(log2 vocab)): below half of one a token is never drawn.
+ * multiples of 2^-S of the largest, S = min(46, 62 - ceil(log2 vocab)): below half of one a token is never drawn.
  * vocab <= 2^24. The result depends on nothing but the row. */
 int cdb_sample_tokens(const void* logits, int logits_fp32, int64_t logits_stride, int num_rows, int vocab,
                       const float* uniform, const float* temperature, const int32_t* top_k, const float* top_p,
