@@ -231,3 +231,25 @@ def test_in_a_graph_and_on_another_stream():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(ids, want[i][0]) and torch.equal(logp, want[i][1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shift", [-40.0, -9.0, -0.75, 0.0, 0.75])
+@pytest.mark.parametrize("filters", ["p", "kp", "kpm"])
+def test_borders_below_and_about_zero(dtype, shift, filters):
+    """Borders among negative logits, among ones next to zero (both signs, zeros too), and at the ends of the steps of 2^-7
+    that the upper 16 bits take: a number, and its 32-bit neighbours on either side."""
+
+    g = torch.Generator().manual_seed(int(shift * 4) + 1000)
+    n, v = 10, 9001
+    x = torch.randn(n, v, generator=g) * 1.5 + shift
+    x[:, 5::11] = x[:, 5::11].bfloat16().float()
+    x[:, 6::11] = torch.nextafter(x[:, 5::11][:, : x[:, 6::11].shape[1]], torch.tensor(INF))
+    x[:, 7::11] = torch.nextafter(x[:, 5::11][:, : x[:, 7::11].shape[1]], torch.tensor(-INF))
+    x[::2, ::13] *= 1e-5  # next to zero
+    x[::3, ::17] = torch.tensor([0.0, -0.0]).repeat(v)[: x[::3, ::17].shape[1]]
+    u, t = _mixed(n, g)
+    p = (0.2 + 0.79 * torch.rand(n, generator=g)).tolist()
+    k = torch.randint(600, 8000, (n,), generator=g).tolist() if "k" in filters else None
+    m = [0.001] * n if "m" in filters else None
+    _check(x.to(dtype).to(DEV), u, t, k, p, m)
