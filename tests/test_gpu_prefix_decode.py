@@ -1,8 +1,8 @@
 """Decode attention whose groups share their prompts' blocks, against every row by itself in 64 bits.
 
 Tolerance, with size = sum p |v| / sum p: the output's rounding, 2^-8 of the value; the weights' rounding to bf16 before
-their product with V, at most 2^-8 of each, of which the sum of the rounded weights takes the common part out: 2^-8
-(size + |o|); the fp32 logits (D <= 128 products whose sizes add up to some 10 here, 2^-24 each): 2^-12 size.
+their product with V, at most 2^-8 of each, over the sum of the rounded weights, off by as much: 2^-8 (size + |o|) (over
+the sum of those before, 2^-8 size); the fp32 logits (D <= 128 products whose sizes add up to some 10 here, 2^-24 each): 2^-12 size.
 """
 
 from __future__ import annotations
