@@ -143,21 +143,34 @@ int sm_count(c10::Device dev) {
 void check(int rc, const char* what) { TORCH_CHECK(rc == CDB_OK, what, " failed: ", cdb_status_string(rc), " (status ", rc, ")"); }
 
 // Piece buffer and arrival counters of a decode attention (`op` tells them apart). Eager calls keep one per stream, so
-// that calls on two streams never share one. A captured call takes its own from the graph's memory and
-// zeroes the counters inside the graph, so that two graphs may be replayed at once.
+// that calls on two streams never share one, and hold its lock until all their launches are on the stream: what a call's
+// launches hand on to one another must not be overwritten by those of another host thread's call on that stream. A captured
+// call takes its own from the graph's memory and zeroes the counters inside the graph, so that two graphs may be replayed
+// at once.
 enum Op { kKv8Decode, kPrefixDecode };
-std::pair<Tensor, Tensor> workspace(Op op, c10::Device dev, c10::cuda::CUDAStream stream, int64_t floats,
-                                    int64_t counters) {
+struct Workspace {
+  Tensor floats, counters;
+  std::unique_lock<std::mutex> lock;
+};
+Workspace workspace(Op op, c10::Device dev, c10::cuda::CUDAStream stream, int64_t floats, int64_t counters) {
   const auto f32 = at::TensorOptions().dtype(at::kFloat).device(dev);
   const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
-    return {at::empty({floats}, f32), at::zeros({counters}, i32)};
-  static auto& kept = *new std::map<std::tuple<Op, int, cudaStream_t>, std::pair<Tensor, Tensor>>;
-  std::lock_guard<std::mutex> lock(g_mutex);
-  auto& ws = kept[{op, dev.index(), stream.stream()}];
-  if (!ws.first.defined() || ws.first.numel() < floats || ws.second.numel() < counters)
-    ws = {at::empty({floats}, f32), at::zeros({counters}, i32)};
-  return ws;
+    return {at::empty({floats}, f32), at::zeros({counters}, i32), {}};
+  struct Kept {
+    std::mutex launches;
+    Tensor floats, counters;
+  };
+  static auto& kept = *new std::map<std::tuple<Op, int, cudaStream_t>, Kept>;  // (whose places never move)
+  Kept* ws;
+  {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    ws = &kept[{op, dev.index(), stream.stream()}];
+  }
+  std::unique_lock<std::mutex> lock(ws->launches);
+  if (!ws->floats.defined() || ws->floats.numel() < floats || ws->counters.numel() < counters)
+    ws->floats = at::empty({floats}, f32), ws->counters = at::zeros({counters}, i32);
+  return {ws->floats, ws->counters, std::move(lock)};
 }
 
 // The rotation's tables; returns their positions.
@@ -248,14 +261,14 @@ void kv8_decode_attention(const Tensor& q, const Tensor& out, const Tensor& code
   const auto stream = c10::cuda::getCurrentCUDAStream(dev.index());
   const int ctas = sm_count(dev);
   const Tensor& status = status_word(dev);
-  const auto [ws, counters] = workspace(kKv8Decode, dev, stream, cdb_kv8_decode_workspace_floats(ctas, c.dim),
-                                        cdb_kv8_decode_counters(ctas));
+  const Workspace ws = workspace(kKv8Decode, dev, stream, cdb_kv8_decode_workspace_floats(ctas, c.dim),
+                                 cdb_kv8_decode_counters(ctas));
   check(cdb_kv8_decode_attention(ptr<void>(q), q.stride(0), ptr<void>(out), out.stride(0), ptr<void>(codes),
                                  ptr<float>(scales), c.layers, (int)cache_layer, c.blocks, ptr<int32_t>(block_table),
                                  block_table.stride(0), (int)block_table.size(0), (int)block_table.size(1),
                                  ptr<int32_t>(item_slot), ptr<int32_t>(item_pos), (int)n, (int)num_heads, c.heads,
-                                 c.dim, (float)scale, ctas, ptr<float>(ws), ws.numel(), ptr<int32_t>(counters),
-                                 ptr<int32_t>(status), stream.stream()),
+                                 c.dim, (float)scale, ctas, ptr<float>(ws.floats), ws.floats.numel(),
+                                 ptr<int32_t>(ws.counters), ptr<int32_t>(status), stream.stream()),
         "cdb_kv8_decode_attention");
 }
 
@@ -443,16 +456,16 @@ void prefix_decode_attention(const Tensor& q, const Tensor& out, const Tensor& k
   const auto stream = c10::cuda::getCurrentCUDAStream(dev.index());
   const int sms = sm_count(dev);
   const Tensor& status = status_word(dev);
-  const Tensor ws =
+  const Workspace ws =
       workspace(kPrefixDecode, dev, stream,
-                cdb_prefix_decode_workspace_floats((int)n, (int)groups, (int)num_heads, c.heads, c.dim, sms), 0)
-          .first;
+                cdb_prefix_decode_workspace_floats((int)n, (int)groups, (int)num_heads, c.heads, c.dim, sms), 0);
   check(cdb_prefix_decode_attention(
             ptr<void>(q), q.stride(0), ptr<void>(out), out.stride(0), ptr<void>(kv_pool), c.layers, c.rows,
             (int)cache_layer, ptr<int32_t>(block_table), block_table.stride(0), (int)block_table.size(0),
             (int)block_table.size(1), ptr<int32_t>(item_slot), ptr<int32_t>(item_pos), (int)n,
             ptr<int32_t>(group_start), ptr<int32_t>(prefix_len), (int)groups, (int)num_heads, c.heads, c.dim,
-            (float)scale, sms, ptr<float>(ws), ws.numel(), ptr<int32_t>(status), stream.stream()),
+            (float)scale, sms, ptr<float>(ws.floats), ws.floats.numel(), ptr<int32_t>(status),
+            stream.stream()),
         "cdb_prefix_decode_attention");
 }
 

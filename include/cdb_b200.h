@@ -622,7 +622,8 @@ int64_t cdb_prefix_decode_workspace_floats(int num_items, int num_groups, int nu
  *                does not see whole are not shared. num_groups 0: every row stands alone.
  *                Group bounds that descend or leave [0, num_items] set CDB_ERR_INDEX, and no blocks are shared.
  *   workspace    cdb_prefix_decode_workspace_floats elements, 16-byte aligned, in any state. Calls that share it
- *                must be ordered. scale > 0.
+ *                must be ordered as wholes: a call makes three launches that hand on to one another through it, so
+ *                host threads that share a stream and a workspace must not call at the same time. scale > 0.
  *   num_sms      CTAs that the work is cut for, 2 to 1023. It fixes the order of the sums, and so the result's last bits.
  * Rows of more than 128 query heads a kv head share nothing.
  * CDB_ERR_UNSUPPORTED above 2^30 - 17 cache rows or 2^30 - 1 (row, head)s. */
