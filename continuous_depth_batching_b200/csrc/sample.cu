@@ -24,7 +24,7 @@
 // 0.7 ms at 49152 tokens (all logits equal; a border in bf16 where some logit is 2^-32 of another).
 //
 // What bounds it: instructions, and for a few rows a chain of passes with a barrier or a scan after each. A weight is some
-// 25 instructions, so 256 rows of 65536 plain take 31 us (5 of HBM; 0.58 instructions a cycle and scheduler); counting
+// 30 instructions, so 256 rows of 65536 plain take 35 us (5 of HBM; 0.58 instructions a cycle and scheduler); counting
 // into bins 12 cycles a warp of tokens (shared atomics on 32 banks, most of the 18 us of that pass), so 256 fp32 rows of
 // 49152 with top-p take 82 us: 4 the largest, 18 bins, 6 their weights and sums, 19 the weights above and below the border,
 // 8 its list, 6 the token. One row with top-k of 50: 12 us, in steps of 1 to 2. With 32 octaves of bins
@@ -268,6 +268,9 @@ struct Weigher {
 
 // The same to 2^-30 of each weight from 32-bit operations, for every token of a row. With y = (top - l) log2(e) / t as a
 // sum of two floats: 2^-y = 2^-n 2^-(j / 1024) 2^-r, the second from a table, the third from its series, |r| <= 2^-11.
+// What top - l rounds away belongs to that sum, of bf16 logits too: they lie up to 2^8 octaves apart, and past 2^15 their
+// difference needs more than 24 bits. (Left out for them, 60000 tokens next to 0 under one at 12 were off by 2^-21 each.
+// 256 plain rows of 65536 take 35.3 us with it and 31.1 without; only where a vector holds a logit next to 0, 34.7.)
 constexpr int kTable = 1024;
 struct Powers {
   uint2 at[kTable];
@@ -286,7 +289,6 @@ constexpr Powers powers() {
   return p;
 }
 __device__ const Powers g_powers = powers();
-template <typename T>
 struct FastWeigher {
   float top, c, c_low;  // log2(e) / t in two floats
   int down;             // 63 - S
@@ -295,10 +297,8 @@ struct FastWeigher {
     const float d = top - l;
     const float y = fminf(__fmul_rn(d, c), 63.f);  // (NaN comes as 63 too, and 2^-63 as 0 below)
     float e = fmaf(d, c_low, fmaf(d, c, -y));
-    if constexpr (sizeof(T) == 4) {  // what the subtraction rounded away
-      const float back = d - top;
-      e = fmaf((top - (d - back)) - (l + back), c, e);
-    }
+    const float back = d - top;  // what the subtraction rounded away
+    e = fmaf((top - (d - back)) - (l + back), c, e);
     const float round = y + 12288.f;  // to whole 1 / 1024
     const int step = __float_as_int(round) - __float_as_int(12288.f);
     const float r = (y - (round - 12288.f)) + e;
@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   const float tp = p.top_p ? p.top_p[r] : 1.f, mp = p.min_p ? p.min_p[r] : 0.f;
   const bool by_k = k > 0 && k < p.vocab, by_p = tp < 1.f, by_m = mp > 0.f;
   const u64 least_w = by_m ? share_of(mp, 1ull << p.scale_bits, true) : 0;
-  FastWeigher<T> weigh;
+  FastWeigher weigh;
   {
     constexpr float kLog2e = 1.44269502f, kRest = 1.92596299e-8f;  // their sum is log2(e)
     weigh.top = top;
