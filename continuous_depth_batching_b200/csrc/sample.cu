@@ -6,7 +6,7 @@
 // weights' running sum passes u times their total. What is kept is therefore a border in the order: all logits
 // above one value, and of those equal to it the first few by index.
 //
-// Weights are whole numbers, w 2^S rounded, S = 62 - log2 of the vocabulary's size (46 at most), and sums of them 64-bit
+// Weights are whole numbers, w 2^S rounded down, S = 62 - log2 of the vocabulary's size (46 at most), and sums of them 64-bit
 // whole numbers: exact, the same in any order, and comparable with a border that lies next to them. 32-bit sums
 // would move the borders by 2^-24 of the total, which is the weight of whole tokens in a wide row.
 //
@@ -256,17 +256,17 @@ __device__ __forceinline__ Stretch stretch_of(u64 mine, float share) {
 
 // ---------------------------------------------------------------------------------- weights
 
-// In 64 bits, for a few tokens or bins.
+// In 64 bits, for rows whose largest logit is infinite or whose temperature has no finite inverse in 32.
 struct Weigher {
   double top, inv, one;  // one: 2^S
-  __device__ __forceinline__ double share(float l) const {
+  __device__ __forceinline__ u64 operator()(float l) const {
     const double d = (double)l == top ? 0. : (double)l - top;  // (+inf - +inf)
-    return d >= -1e300 ? exp(d * inv) : 0.;
+    return d >= -1e300 ? (u64)(exp(d * inv) * one) : 0;
   }
-  __device__ __forceinline__ u64 operator()(float l) const { return (u64)__double2ll_rn(share(l) * one); }
 };
 
-// The same to 2^-30 of each weight from 32-bit operations, for every token of a row. With y = (top - l) log2(e) / t as a
+// The same to 2^-30 of each weight from 32-bit operations, for every token of all other rows, whichever way they take: two
+// ways with weights of their own would answer differently as the number of rows chooses between them. With y = (top - l) log2(e) / t as a
 // sum of two floats: 2^-y = 2^-n 2^-(j / 1024) 2^-r, the second from a table, the third from its series, |r| <= 2^-11.
 // What top - l rounds away belongs to that sum, of bf16 logits too: they lie up to 2^8 octaves apart, and past 2^15 their
 // difference needs more than 24 bits. (Left out for them, 60000 tokens next to 0 under one at 12 were off by 2^-21 each.
@@ -289,6 +289,7 @@ constexpr Powers powers() {
   return p;
 }
 __device__ const Powers g_powers = powers();
+
 struct FastWeigher {
   float top, c, c_low;  // log2(e) / t in two floats
   int down;             // 63 - S
@@ -350,20 +351,16 @@ __device__ __forceinline__ void sort(u64* list, int size) {
 
 // ---------------------------------------------------------------------------------- any row, slowly
 
-template <typename T, int kThreads>
-__device__ __noinline__ void slow_row(const Params& p, int r, uint32_t top, float t, Scratch& sc) {
+// `weigh`: by value, since the address of the caller's would keep it out of registers.
+template <typename T, int kThreads, typename W>
+__device__ __noinline__ void slow_row(const Params& p, int r, float top, float t, const W weigh, u64 least_w, Scratch& sc) {
   const int tid = threadIdx.x, v = p.vocab;
   const void* row = static_cast<const T*>(p.logits) + (int64_t)r * p.stride;
-  const bool greedy = !(t > 0.f);
-  Weigher weigh;
-  weigh.top = (double)logit_of(top);
-  weigh.inv = greedy ? 0. : 1. / (double)t;
-  weigh.one = (double)(1ull << p.scale_bits);
   // tokens of keys above `edge` are kept, and the first `ties` at it
-  uint32_t edge = greedy ? top : 0;
-  u64 ties = greedy ? 1 : ~0ull;
+  uint32_t edge = 0;
+  u64 ties = ~0ull;
   const int k = p.top_k ? p.top_k[r] : 0;
-  if (!greedy && k > 0 && k < v) {
+  if (k > 0 && k < v) {
     u64 above = 0;
     for (int bit = 31; bit >= 0; --bit) {  // the largest key that at least k tokens reach
       const uint32_t probe = edge | (1u << bit);
@@ -376,7 +373,7 @@ __device__ __noinline__ void slow_row(const Params& p, int r, uint32_t top, floa
     ties = (u64)k - above;
   }
   const float tp = p.top_p ? p.top_p[r] : 1.f;
-  if (!greedy && tp < 1.f) {
+  if (tp < 1.f) {
     const u64 at_edge = ties == ~0ull ? 0 : weigh(logit_of(edge)) * ties;
     u64 total = 0;
     for (int i = tid; i < v; i += kThreads) {
@@ -406,9 +403,6 @@ __device__ __noinline__ void slow_row(const Params& p, int r, uint32_t top, floa
     if (e != edge || m < ties) ties = m;
     edge = e;
   }
-  const float mp = p.min_p ? p.min_p[r] : 0.f;
-  const bool cut = !greedy && mp > 0.f;
-  const double least = cut ? fmin((double)mp, 1.) : 0.;
   // index order: each thread a stretch of the row
   const int per = (v + kThreads - 1) / kThreads;
   const int lo = min(v, tid * per), hi = min(v, lo + per);
@@ -421,7 +415,9 @@ __device__ __noinline__ void slow_row(const Params& p, int r, uint32_t top, floa
       const uint32_t key = load_key<T>(row, i);
       bool keep = key > edge;
       if (key == edge) keep = seen++ < ties;
-      if (keep && (!cut || key == top || weigh.share(logit_of(key)) >= least)) f(i, greedy ? 1ull : weigh(logit_of(key)));
+      if (!keep) continue;
+      const u64 w = weigh(logit_of(key));
+      if (w >= least_w) f(i, w);
     }
   };
   u64 mine = 0;
@@ -433,8 +429,9 @@ __device__ __noinline__ void slow_row(const Params& p, int r, uint32_t top, floa
     walk([&](int i, u64 w) {
       if (run <= want && want < run + w) {
         p.ids[r] = i;
-        const double l = (double)load_one<T>(row, i), d = l == weigh.top ? 0. : (l - weigh.top) * weigh.inv;
-        if (p.logp) p.logp[r] = greedy ? 0.f : (float)(d - log((double)all / weigh.one));
+        const float l = load_one<T>(row, i);
+        const double d = l == top ? 0. : ((double)l - (double)top) * (1. / (double)t);
+        if (p.logp) p.logp[r] = (float)(d - log((double)all / (double)(1ull << p.scale_bits)));
       }
       run += w;
     });
@@ -564,6 +561,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   const float tp = p.top_p ? p.top_p[r] : 1.f, mp = p.min_p ? p.min_p[r] : 0.f;
   const bool by_k = k > 0 && k < p.vocab, by_p = tp < 1.f, by_m = mp > 0.f;
   const u64 least_w = by_m ? share_of(mp, 1ull << p.scale_bits, true) : 0;
+  if (isinf(top) || isinf(1.44269502f / t)) {
+    const Weigher weigh = {(double)top, 1. / (double)t, (double)(1ull << p.scale_bits)};
+    slow_row<T, kThreads>(p, r, top, t, weigh, least_w, sh.sc);
+    return;
+  }
   FastWeigher weigh;
   {
     constexpr float kLog2e = 1.44269502f, kRest = 1.92596299e-8f;  // their sum is log2(e)
@@ -572,10 +574,6 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     weigh.c_low = isinf(t) ? 0.f : (fmaf(-weigh.c, t, kLog2e) + kRest) / t;
     weigh.down = 63 - p.scale_bits;
     weigh.table = table;
-  }
-  if (isinf(top) || isinf(weigh.c)) {
-    slow_row<T, kThreads>(p, r, key_of(top), t, sh.sc);
-    return;
   }
   // the log-probability of a token among kept weights that add up to `all`
   auto log_share = [&](float l, u64 all) {
@@ -697,7 +695,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       }
     }
     if (__syncthreads_or(strange)) {
-      slow_row<T, kThreads>(p, r, key_of(top), t, sh.sc);
+      slow_row<T, kThreads>(p, r, top, t, weigh, least_w, sh.sc);
       return;
     }
     // Their weights: neighbouring bins, which tend to be filled together, on different threads. Where fp32 has no mean
@@ -914,7 +912,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     block_sums<kThreads>(above_w, total, n_above, sh.sc);
     const int n = sh.list_n;
     if (n > kList) {
-      slow_row<T, kThreads>(p, r, key_of(top), t, sh.sc);
+      slow_row<T, kThreads>(p, r, top, t, weigh, least_w, sh.sc);
       return;
     }
     // sort the list, largest first
@@ -951,7 +949,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     __syncthreads();
     edge = sh.edge;
     if (sh.list_over || edge == 0) {
-      slow_row<T, kThreads>(p, r, key_of(top), t, sh.sc);
+      slow_row<T, kThreads>(p, r, top, t, weigh, least_w, sh.sc);
       return;
     }
   }

@@ -648,7 +648,7 @@ int cdb_prefix_decode_attention(const void* q, int64_t q_stride, void* out, int6
  *   out_ids    int64 [num_rows]; out_logprobs fp32 [num_rows] or NULL: log of the token's share of the kept weights.
  * Logits: NaN counts as -inf and is never drawn; where the largest is +inf, tokens at +inf weigh 1 and
  * others 0. A row without a logit above -inf gives id -1 and log-probability NaN. Weights are whole
- * multiples of 2^-S of the largest, S = min(46, 62 - ceil(log2 vocab)): below half of one a token is never drawn.
+ * multiples of 2^-S of the largest, rounded down, S = min(46, 62 - ceil(log2 vocab)): below one a token is never drawn.
  * vocab <= 2^24. The result depends on nothing but the row. */
 int cdb_sample_tokens(const void* logits, int logits_fp32, int64_t logits_stride, int num_rows, int vocab,
                       const float* uniform, const float* temperature, const int32_t* top_k, const float* top_p,
