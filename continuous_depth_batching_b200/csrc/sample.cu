@@ -20,8 +20,8 @@
 //      where the border falls into a bin, its neighbourhood's tokens are collected, sorted and summed exactly;
 //   4. the stretch in which the target lies, a few tokens to a thread.
 // Rows that this does not fit (an infinite largest logit, bf16 logits over more than 32 octaves, a border among more
-// fp32 tokens than the list holds) take `slow_row`, which finds its borders by bisection, a bit of the key a pass: 0.3 to
-// 0.7 ms at 49152 tokens (all logits equal; a border in bf16 where some logit is 2^-32 of another).
+// fp32 tokens than the list holds) take `slow_row`, which finds its borders by bisection, a bit of the key a pass: 0.25 to
+// 0.6 ms at 49152 tokens (all logits equal; a border in bf16 where some logit is 2^-32 of another).
 //
 // What bounds it: instructions, and for a few rows a chain of passes with a barrier or a scan after each. A weight is some
 // 30 instructions, so 256 rows of 65536 plain take 35 us (5 of HBM; 0.58 instructions a cycle and scheduler); counting
@@ -677,6 +677,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     bool strange = false;
     // fp32: the mean logit of the bins whose tokens weigh e^-6 or more, of which few may make up the total
     const int heavy = WIDE && by_p ? bin_of<T>(top - 6.f * t, low) : -1;
+    const int coarse = max(16 - __clz(p.vocab - 1), 0);  // so that the whole vocabulary's low halves add up to less than 2^32
     if (WIDE && by_p) {
       for (int i = tid; i < kBinsPadded; i += kThreads) weights[i] = 0;
       __syncthreads();
@@ -691,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
         if (!WIDE) strange |= bin == kHalf && x[i] != 0.f;
         if (bin != kNone) atomicAdd(&counts[bin], 1u);
         if (WIDE && bin <= heavy && bin != kNone)
-          atomicAdd(reinterpret_cast<uint32_t*>(&weights[bin]), __float_as_uint(x[i]) & 0xffffu);
+          atomicAdd(reinterpret_cast<uint32_t*>(&weights[bin]), (__float_as_uint(x[i]) & 0xffffu) >> coarse);
       }
     }
     if (__syncthreads_or(strange)) {
@@ -705,7 +706,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       if (n == 0) continue;
       float l = logit_of_bin<T>(b, low);
       if (WIDE && b != kHalf) {
-        const uint32_t in = b <= heavy ? (uint32_t)__fdividef((float)(uint32_t)weights[b], (float)n) : 0x8000u;
+        const uint32_t in =
+            b <= heavy ? (uint32_t)(__fdividef((float)(uint32_t)weights[b], (float)n) * (float)(1 << coarse)) : 0x8000u;
         l = fminf(__uint_as_float(__float_as_uint(l) + in), top);
       }
       weights[b] = weigh(l);
