@@ -394,6 +394,19 @@ std::pair<uintptr_t, uintptr_t> extent(const Tensor& t, int64_t rows, int64_t co
   return {at, at + (uintptr_t)(((rows - 1) * t.stride(0) + cols) * t.element_size())};
 }
 
+// Whether n rows of `cols` columns of two tensors of one type share memory without being the same rows.
+bool partly_overlap(const Tensor& a, const Tensor& b, int64_t n, int64_t cols) {
+  if (n == 0) return false;
+  const bool alike = n == 1 || a.stride(0) == b.stride(0);
+  const auto x = extent(a, n, cols), y = extent(b, n, cols);
+  if (x.second <= y.first || y.second <= x.first || (alike && x.first == y.first)) return false;
+  if (n == 1 || !alike) return true;
+  // columns of one buffer
+  const int64_t pitch = a.stride(0) * (int64_t)a.element_size(), width = cols * (int64_t)a.element_size();
+  const int64_t off = (((int64_t)(y.first - x.first)) % pitch + pitch) % pitch;
+  return off < width || pitch - off < width;
+}
+
 void qk_norm_rope_append(const Tensor& qkv, const OptTensor& q_out, const Tensor& kv_pool, int64_t cache_layer,
                          const Tensor& block_table, const Tensor& item_slot, const Tensor& item_pos,
                          const Tensor& q_weight, const Tensor& k_weight, const OptTensor& rope_cos,
@@ -446,6 +459,8 @@ void prefix_decode_attention(const Tensor& q, const Tensor& out, const Tensor& k
   const int64_t groups = as_int("prefix_len's entries", prefix_len.numel());
   check_rows("q", q, n, num_heads * c.dim);
   check_rows("out", out, n, num_heads * c.dim);
+  TORCH_CHECK_VALUE(!partly_overlap(q, out, n, num_heads * c.dim),
+                    "out may be q's own columns, but may not overlap them otherwise");
   check_ints("item_pos", item_pos, n);
   check_ints("item_slot", item_slot, n);
   check_ints("prefix_len", prefix_len, groups);

@@ -60,7 +60,7 @@ Many continuations of one prompt, over the bf16 paged cache ``kv_pool [layers, 2
 * ``cdb::prefix_decode_attention(q, out, kv_pool, cache_layer, block_table, item_slot, item_pos, group_start,
   prefix_len, num_heads, scale)``: decode attention in which rows ``group_start[g] .. group_start[g + 1] - 1``
   share the blocks of their first ``prefix_len[g]`` tokens, read once for all of them
-  (``cdb_prefix_decode_attention``). Streams and graphs as ``kv8_decode_attention``;
+  (``cdb_prefix_decode_attention``). ``out`` may be ``q``'s own columns. Streams and graphs as ``kv8_decode_attention``;
 * ``cdb::sample_tokens(logits, uniform, temperature, top_k, top_p, min_p, out_ids, out_logprobs)``: the next
   token of every row of bf16 or fp32 logits by temperature, top-k, top-p and min-p (None: off) from one given
   random number a row (``cdb_sample_tokens``).

@@ -614,7 +614,8 @@ int64_t cdb_prefix_decode_workspace_floats(int num_items, int num_groups, int nu
 /* Decode attention: row i attends to positions 0 .. item_pos[i] of slot item_slot[i]; a row with
  * item_pos < 0 is skipped and its out row left as it was. Rows of a group share their first blocks, which
  * are read once for all of them.
- *   q, out       bf16 rows of num_heads * head_dim, q rotated; 16-byte aligned, strides multiples of 8.
+ *   q, out       bf16 rows of num_heads * head_dim, q rotated; 16-byte aligned, strides multiples of 8. out may be q
+ *                itself (a row's output is written when nobody reads its q any more); may not overlap it otherwise.
  *   group_start  [num_groups + 1] ascending: rows group_start[g] .. group_start[g + 1] - 1 are group g.
  *                Rows before the first and behind the last group stand alone.
  *   prefix_len   [num_groups]: the first prefix_len[g] / 16 (rounded down) entries of the rows' block-table
