@@ -667,6 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       }
       return;
     }
+    __syncthreads();  // (every thread has seen how many there are)
     if (tid == 0) sh.hi_bin = -1, sh.list_n = 0;
     __syncthreads();
   }
