@@ -1,7 +1,8 @@
 // Decode attention over the bf16 paged cache for requests that share a prompt.
 //
 // Rows of a group see the same blocks first. For those, Q K^T and P V are matrix products of all the group's
-// rows, so a block is read once for up to 128 of them; behind them every row has pages of its own. Softmax parts (m a
+// rows, so a block is read once for up to 256 of them (row x query head of a kv head); behind them every row has pages of
+// its own. Softmax parts (m a
 // maximum of the logits, l the sum of 2^(x - m), o that of 2^(x - m) v) of any set of keys join by rescaling to
 // one m, so the two kinds of work need not wait for each other: one launch does both side by side, and a
 // last one joins. Three launches in all:
@@ -27,8 +28,8 @@
 // sum the rounded weights, so what is common to them cancels; shared steps, where that took 5 % longer, those before.
 // m only moves when passed by 8, which bf16's range allows.
 //
-// What bounds it (16 to 32 heads of 128, B200 at 1.8 GHz). Single rows: memory, 64 x 600 tokens on 16 kv heads 28 us of
-// which 24 are their bytes at 6.6 TB/s, plus the plan and the join. Shared steps of one tile: memory too, 32 KB in 0.6 us. Of two
+// What bounds it (16 to 32 heads of 128, B200 at 1.8 GHz). Single rows: memory, 256 x 2000 tokens on 8 kv heads 328 us from
+// a graph of which 319 are their bytes at 6.6 TB/s; plan and join beside it where there is less, 64 x 600 tokens 41 us for 24. Shared steps of one tile: memory too, 32 KB in 0.6 us. Of two
 // tiles: a warp's chain, 1700 cycles to a step: 220 until S is there, 100 to read it, 225 for the maximum, 1195 for the
 // weights, the other team's on the same unit (1024 of them are 2 x 64 x 8 of the exponential unit). The tensor cores take
 // 1024 (1280: at 64 keys S reads q from shared memory faster than that delivers). Measured against it: a quarter of the
@@ -169,7 +170,10 @@ __device__ __forceinline__ int last_at_most(int n, int64_t x, F value) {
 }
 
 // How a call's work is cut, in units of 1/64 us, measured at 16 and 32 heads of 128 as what divides a call best: a CTA
-// takes 1 us to a step (HBM) and 1.3 where both teams have 128 rows (exponentials), 0.16 us to a page of single rows.
+// takes 1 us to a step (HBM) and 1.3 where both teams have 128 rows (exponentials), 0.16 us to a page of single rows. Heads
+// of 64 and 96 go by the same numbers, which were not measured for them. What a unit costs a CTA that enters it (q, an empty
+// pipeline, O stored) is not counted, and a group's odd last tile counts as a pair: CTAs of equal cost end 45 to 62 us into a
+// call of 5 groups.
 // Sharing costs another 4 us (more parts, q, tensor memory), so few rows on a short prompt are faster each by itself: 4
 // rows on 700 tokens, 16 heads, take 14 us so and 21 shared.
 constexpr int kStepCost = 62, kPairCost = 83, kPageCost = 10, kSharedCost = 256;

@@ -12,10 +12,11 @@
 // its partner with the partner's w s, and one with the norm. Heads of q come first, then k's, then the values, which
 // are only copied; four heads of a group are in flight at a time.
 //
-// Everything is read and written once: bound by HBM over many rows (5411 rows of 32 + 2 x 8 heads of 128: 28.7 us for 118 MB
-// from a graph, 18 of them at 6.6 TB/s; a row's reads have to come back before its writes go out, and 80 registers leave 24
-// warps an SM to overlap them; 1643 rows of 55 + 2 x 55 heads of 96, interleaved pairs: 9.4 us for 48 MB, 7.3 at that rate), by
-// a chain of three latencies (position, block id and angles, stores) over few (80 rows of 16 + 2 x 16 heads: 2.9 us).
+// Everything is read and written once: bound by HBM over many rows, and by how well their warps fill it. 5411 rows of 32 +
+// 2 x 8 heads of 128 take 29.1 us from a graph for 118 MB, 18 of them at 6.6 TB/s: a warp a row is 1353 CTAs on 888 places
+// (80 registers leave 24 warps an SM), one wave and a half, and a warp's next heads are loaded when the last are stored. 1643
+// rows of 55 + 2 x 55 heads of 96, interleaved pairs: 9.4 us for 48 MB, 7.3 at that rate. Over few rows it is a
+// chain of three latencies (position, block id and angles, stores): 80 rows of 16 + 2 x 16 heads, 3.1 us.
 #include "cdb_common.cuh"
 
 namespace cdb {

@@ -14,21 +14,25 @@
 //   1. its largest and least logit, and every thread's largest;
 //   2. with top-k of up to half the threads: the tokens at or above the k-th largest of the threads' largest, a few more
 //      than k of them, which are sorted; the rest is done on them;
-//   2. with top-p, or more of top-k: how many tokens each of 8192 bins has: the upper 16 bits of the logit's 32, so for
-//      bf16 a bin holds one value, over the 32 octaves below the row's largest magnitude, either sign;
+//   2. with top-p, or more of top-k: how many tokens each of 8192 bins has (fp32: 4096): the upper 16 bits of the logit's 32,
+//      so for bf16 a bin holds one value, over the 32 (16) octaves below the row's largest magnitude, either sign;
 //   3. the kept weights of every warp's stretch of the row. Behind bins bf16 looks a bin's weight up; fp32 computes it, and
 //      where the border falls into a bin, its neighbourhood's tokens are collected, sorted and summed exactly;
 //   4. the stretch in which the target lies, a few tokens to a thread.
 // Rows that this does not fit (an infinite largest logit, bf16 logits over more than 32 octaves, a border among more
 // fp32 tokens than the list holds) take `slow_row`, which finds its borders by bisection, a bit of the key a pass: 0.25 to
-// 0.6 ms at 49152 tokens (all logits equal; a border in bf16 where some logit is 2^-32 of another).
+// 0.6 ms at 49152 tokens (all logits equal; a border in bf16 where some logit is 2^-32 of another). With fp32 and top-p the
+// list holds what lies within 2^-11 of the total about the border, and five deviations of what the bins leave open, so near
+// p = 1 it is a wide row's whole tail: rows of a language model's shape take the slow way from p = 0.998 on at 49152 tokens
+// and temperature 0.7, or 0.995 at 151936 (256 rows: 0.13 ms at p = 0.995 and 1.1 at 0.998; 0.32 at 0.99 and 3.2 to 4.5 above).
 //
 // What bounds it: instructions, and for a few rows a chain of passes with a barrier or a scan after each. A weight is some
 // 30 instructions, so 256 rows of 65536 plain take 35 us (5 of HBM; 0.58 instructions a cycle and scheduler); counting
 // into bins 12 cycles a warp of tokens (shared atomics on 32 banks, most of the 18 us of that pass), so 256 fp32 rows of
-// 49152 with top-p take 82 us: 4 the largest, 18 bins, 6 their weights and sums, 19 the weights above and below the border,
-// 8 its list, 6 the token. One row with top-k of 50: 12 us, in steps of 1 to 2. With 32 octaves of bins
-// for fp32, and every token's bin for its sums, those 82 us were 95; one CTA an SM for 256 rows is slower than two of 512 threads.
+// 49152 with top-p take 81 us. Their median row takes 62: 2 to begin, 10 the largest (memory), 18 bins, 6 their weights and
+// sums, 18 the weights above and below the border, 5 its list, 3 the token; the last rows' lists of thousands take up to 25.
+// One row with top-k of 50: 12 us, in steps of 1 to 2. With 32 octaves of bins
+// for fp32, and every token's bin for its sums, those 81 us were 95; one CTA an SM for 256 rows is slower than two of 512 threads.
 #include "cdb_common.cuh"
 
 namespace cdb {
